@@ -186,6 +186,9 @@ SIGNATURES = {
                                         C.c_int32, C.c_int32, C.c_int32, C.c_double, C.c_int32, C.c_void_p]),
     "eqt_layer_rms_backward": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                                          C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_void_p]),
+    "eqt_embedding_forward": (C.c_int, [C.c_int32] + [C.c_void_p] * 3 + [C.c_int64] * 3 + [C.c_double, C.c_void_p]),
+    "eqt_embedding_grad_scratch": (C.c_int64, [C.c_int32] + [C.c_int64] * 3),
+    "eqt_embedding_grad": (C.c_int, [C.c_int32] + [C.c_void_p] * 3 + [C.c_int64] * 3 + [C.c_double, C.c_void_p, C.c_int64, C.c_void_p]),
     "eqt_last_error": (C.c_char_p, []),
     "eqt_version": (C.c_int, []),
     "eqt_launch_count": (C.c_int64, []),

@@ -643,6 +643,18 @@ int eqt_radius_search(const float* pos, const float* sorted, const int32_t* cell
 int eqt_radius_list_edges(const float* pos, int64_t n, const int64_t* ptr, const int32_t* list, int32_t row, int64_t* src,
                           int64_t* dst, const eqt_edge_features* features, void* stream);
 
+/*
+ * Rows of a table by type: out (n, width) = scale * weight (types, width)[index (n)]; a row of zeros where index is not in
+ * [0, types).  Gradient: gw (types, width) = scale * sum of g over the rows of each type, all of gw written.  Sums in float
+ * (double for EQT_F64), no atomics on values: the same bits at every call.  n and types below 2^31 - 1.
+ * `scratch`: eqt_embedding_grad_scratch bytes, 256-byte aligned (0: none needed).
+ */
+int eqt_embedding_forward(int32_t dtype, const void* weight, const int64_t* index, void* out, int64_t n, int64_t types,
+                          int64_t width, double scale, void* stream);
+int64_t eqt_embedding_grad_scratch(int32_t dtype, int64_t n, int64_t types, int64_t width);
+int eqt_embedding_grad(int32_t dtype, const void* g, const int64_t* index, void* gw, int64_t n, int64_t types, int64_t width,
+                       double scale, void* scratch, int64_t scratch_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
