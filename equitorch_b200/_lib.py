@@ -88,6 +88,13 @@ class UvwRoleStruct(C.Structure):
                 ("stride_k", C.c_int32), ("stride_j", C.c_int32), ("stride_p", C.c_int32)]
 
 
+class AttentionArgs(C.Structure):
+    _fields_ = ([(f, C.c_int32) for f in ("dtype", "heads", "comps", "head_channels", "tile_rows")] + [("scale", C.c_float), ("cap", C.c_float)]
+                + [("n", C.c_int64), ("num_tiles", C.c_int64)] + [(f, C.c_void_p) for f in ("tiles", "q", "k", "v")]
+                + [(f, C.c_int64) for f in ("q_node", "q_comp", "k_node", "k_comp", "v_node", "v_comp")]
+                + [(f, C.c_void_p) for f in ("pos", "slope", "out", "lse", "grad_out", "dq", "dk", "dv", "delta", "geo", "dpos", "dslope")])
+
+
 # name -> (restype, argtypes); every symbol declared in include/eqt_b200.h appears here
 SIGNATURES = {
     "eqt_sparse_product": (C.c_int, [C.POINTER(ProductArgs), C.c_void_p]),
@@ -189,6 +196,8 @@ SIGNATURES = {
     "eqt_embedding_forward": (C.c_int, [C.c_int32] + [C.c_void_p] * 3 + [C.c_int64] * 3 + [C.c_double, C.c_void_p]),
     "eqt_embedding_grad_scratch": (C.c_int64, [C.c_int32] + [C.c_int64] * 3),
     "eqt_embedding_grad": (C.c_int, [C.c_int32] + [C.c_void_p] * 3 + [C.c_int64] * 3 + [C.c_double, C.c_void_p, C.c_int64, C.c_void_p]),
+    "eqt_attention_forward": (C.c_int, [C.POINTER(AttentionArgs), C.c_void_p]),
+    "eqt_attention_backward": (C.c_int, [C.POINTER(AttentionArgs), C.c_void_p]),
     "eqt_last_error": (C.c_char_p, []),
     "eqt_version": (C.c_int, []),
     "eqt_launch_count": (C.c_int64, []),

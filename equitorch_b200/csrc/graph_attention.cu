@@ -1,0 +1,121 @@
+// Attention within packed graphs: checks of the arguments, order of the launches, sums over the heads.
+#include "graph_attention.cuh"
+
+namespace eqt {
+namespace {
+using namespace attention;
+
+// Geometry over the heads: the first `heads` CTAs sum a head's slope gradient in a fixed order, the others the positions' gradients.
+constexpr int GEO_THREADS = 512;
+__global__ void __launch_bounds__(GEO_THREADS) attention_geometry_kernel(const float4* __restrict__ row, const float4* __restrict__ col,
+                                                                         const float* __restrict__ slope, float* __restrict__ dslope,
+                                                                         float* __restrict__ dpos, int64_t n, int heads) {
+  if (blockIdx.x < heads) {
+    __shared__ double part[GEO_THREADS / 32];
+    double sum = 0.0;
+    for (int64_t i = threadIdx.x; i < n; i += GEO_THREADS) sum += row[(int64_t)blockIdx.x * n + i].x;
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int w = 1; w < GEO_THREADS / 32; ++w) sum += part[w];
+      dslope[blockIdx.x] = (float)-sum;
+    }
+    return;
+  }
+  const int64_t i = (int64_t)(blockIdx.x - heads) * GEO_THREADS + threadIdx.x;
+  if (i >= n) return;
+  float x = 0.f, y = 0.f, z = 0.f;
+  for (int h = 0; h < heads; ++h) {
+    const float4 a = row[(int64_t)h * n + i], b = col[(int64_t)h * n + i];
+    const float f = -slope[h];
+    x += f * (a.y - b.y);
+    y += f * (a.z - b.z);
+    z += f * (a.w - b.w);
+  }
+  dpos[3 * i] = x;
+  dpos[3 * i + 1] = y;
+  dpos[3 * i + 2] = z;
+}
+
+int launch_all(Pass pass, const eqt_attention_args* a, const AttentionParams& p, bool geo, cudaStream_t s) {
+  return a->dtype == EQT_F32 ? launch_f32(pass, p, a->num_tiles, a->tile_rows, geo, s)
+                             : launch_bf16(pass, p, a->num_tiles, a->tile_rows, geo, s);
+}
+
+int fill(const eqt_attention_args* a, AttentionParams& p, bool backward) {
+  if (!a) return fail(EQT_ERR_BAD_ARGUMENT, "attention: NULL arguments");
+  if (a->dtype != EQT_F32 && a->dtype != EQT_BF16) return fail(EQT_ERR_UNSUPPORTED, "attention: float32 or bfloat16 features expected");
+  if (a->n < 0 || a->num_tiles < 0 || a->heads < 1 || a->comps < 1 || a->head_channels < 1)
+    return fail(EQT_ERR_BAD_ARGUMENT, "attention: sizes must be positive");
+  if (a->tile_rows != 16 && a->tile_rows != 32 && a->tile_rows != 64) return fail(EQT_ERR_BAD_ARGUMENT, "attention: tiles have 16, 32 or 64 rows");
+  if (a->n > INT32_MAX - 64 || a->num_tiles > INT32_MAX || a->heads > 65535)
+    return fail(EQT_ERR_UNSUPPORTED, "attention: nodes and tiles are numbered in 32 bits, heads in 16");
+  if ((int64_t)a->comps * a->head_channels > 128)
+    return fail(EQT_ERR_UNSUPPORTED, "attention: a head has at most 128 values a node, got %lld", (long long)a->comps * a->head_channels);
+  if (!(a->cap >= 0.f)) return fail(EQT_ERR_BAD_ARGUMENT, "attention: the cap must not be negative");
+  if (a->n && (a->pos != nullptr) != (a->slope != nullptr)) return fail(EQT_ERR_BAD_ARGUMENT, "attention: positions and slopes come together");
+  if (a->num_tiles && (!a->q || !a->k || !a->v || !a->out || !a->tiles || (backward && (!a->grad_out || !a->lse || !a->dq || !a->dk || !a->dv || !a->delta))))
+    return fail(EQT_ERR_BAD_ARGUMENT, "attention: NULL pointer");
+  const bool geo = a->dpos || a->dslope;
+  if (backward && geo && a->n && (!a->pos || !a->dpos || !a->dslope || !a->geo))
+    return fail(EQT_ERR_BAD_ARGUMENT, "attention: the gradients of positions and slopes come together, with positions and scratch");
+  const int64_t channels = (int64_t)a->heads * a->head_channels;
+  const int size = a->dtype == EQT_F32 ? 4 : 2;
+  p = AttentionParams{};
+  p.q = {a->q, a->q_node, a->q_comp};
+  p.k = {a->k, a->k_node, a->k_comp};
+  p.v = {a->v, a->v_node, a->v_comp};
+  p.out = {a->out, a->comps * channels, channels};
+  p.g = {a->grad_out, a->comps * channels, channels};
+  p.out_w = a->out;
+  p.dq = a->dq;
+  p.dk = a->dk;
+  p.dv = a->dv;
+  p.lse = a->lse;
+  p.delta = a->delta;
+  p.geo_row = static_cast<float4*>(a->geo);
+  p.geo_col = p.geo_row ? p.geo_row + a->heads * a->n : nullptr;
+  p.tiles = static_cast<const int4*>(static_cast<const void*>(a->tiles));
+  p.pos = a->pos;
+  p.slope = a->slope;
+  p.n = a->n;
+  p.heads = a->heads;
+  p.comps = a->comps;
+  p.size = a->head_channels;
+  p.scale = a->scale;
+  p.cap = a->cap;
+  uintptr_t bits = (uintptr_t)a->head_channels * size;
+  for (const void* q : {a->q, a->k, a->v, (const void*)a->out, a->grad_out, (const void*)a->dq, (const void*)a->dk, (const void*)a->dv})
+    bits |= reinterpret_cast<uintptr_t>(q);
+  for (int64_t st : {a->q_node, a->q_comp, a->k_node, a->k_comp, a->v_node, a->v_comp}) bits |= (uintptr_t)st * size;
+  p.vec = bits % 16 == 0;
+  return EQT_OK;
+}
+
+}  // namespace
+}  // namespace eqt
+
+using namespace eqt;
+
+extern "C" int eqt_attention_forward(const eqt_attention_args* a, void* stream) {
+  AttentionParams p;
+  if (int rc = fill(a, p, false)) return rc;
+  if (a->num_tiles == 0) return EQT_OK;
+  return launch_all(FORWARD, a, p, false, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int eqt_attention_backward(const eqt_attention_args* a, void* stream) {
+  AttentionParams p;
+  if (int rc = fill(a, p, true)) return rc;
+  const bool geo = a->dslope != nullptr;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (a->num_tiles) {
+    if (int rc = launch_all(ROWS, a, p, geo, s)) return rc;
+    if (int rc = launch_all(COLUMNS, a, p, geo, s)) return rc;
+  }
+  if (!geo) return EQT_OK;
+  attention_geometry_kernel<<<(unsigned)(a->heads + ceil_div(a->n, GEO_THREADS)), GEO_THREADS, 0, s>>>(
+      p.geo_row, p.geo_col, a->slope, a->dslope, a->dpos, a->n, a->heads);
+  return check_launch("attention_geometry");
+}

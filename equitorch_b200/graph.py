@@ -64,3 +64,59 @@ class EdgeGraph:
     @staticmethod
     def from_edge_index(edge_index: Tensor, num_nodes: int) -> "EdgeGraph":
         return EdgeGraph(edge_index[0], edge_index[1], num_nodes)
+
+
+class PackedGraphs:
+    """Which nodes of a batch belong to which graph: graph g has the nodes ``[ptr[g], ptr[g + 1])``, as ``segment_sum`` and
+    ``torch_geometric``'s batches have it.  Computed once per batch, for every layer that works within graphs.
+
+    Nodes before ``ptr[0]`` and from ``ptr[-1]`` on belong to no graph.  Attributes: ``ptr`` (num_graphs + 1, int64), ``num_nodes``,
+    ``num_graphs``, ``covers`` (every node has a graph), ``tile_rows`` and ``tiles`` (num_tiles, 4, int32: first row, first node and
+    one past the last node of its graph, 0), the pieces of at most ``tile_rows`` nodes of one graph that the kernels work on, those of
+    the largest graphs first.  Reads a few numbers back to the host.
+    """
+
+    def __init__(self, ptr: Tensor, num_nodes: int):
+        if ptr.dtype != torch.int64 or ptr.ndim != 1 or ptr.numel() < 1:
+            raise ValueError(f"int64 boundaries of the graphs expected, at least one, got {ptr.dtype} of shape {tuple(ptr.shape)}")
+        if not 0 <= int(num_nodes) < 2 ** 31 - 64:
+            raise ValueError(f"num_nodes must be in [0, 2^31 - 64), got {num_nodes}")
+        self.ptr, self.num_nodes, self.num_graphs = ptr.contiguous().clone(), int(num_nodes), ptr.numel() - 1
+        sizes = self.ptr[1:] - self.ptr[:-1]
+        zero = sizes.new_zeros(1)
+        first, last, least, *tiles = torch.stack([
+            self.ptr[0], self.ptr[-1], torch.cat([zero, sizes]).min(),
+            *(((sizes + r - 1) // r).sum() for r in (16, 32, 64))]).tolist()
+        if least < 0 or first < 0 or last > self.num_nodes:
+            raise ValueError(f"boundaries of the graphs must ascend within [0, {self.num_nodes}]")
+        self.covers = first == 0 and last == self.num_nodes
+        # Rows behind the end of a graph are work for nothing, and a tile of more rows reads the other side fewer times: the largest
+        # tile with at most a quarter more rows than the smaller ones.
+        self.tile_rows = 64 if 64 * tiles[2] <= 1.25 * 32 * tiles[1] else 32 if 32 * tiles[1] <= 1.25 * 16 * tiles[0] else 16
+        count = (sizes + self.tile_rows - 1) // self.tile_rows
+        total = tiles[(16, 32, 64).index(self.tile_rows)]
+        by_size = torch.argsort(sizes, descending=True, stable=True)
+        graph = torch.repeat_interleave(by_size, count[by_size], output_size=total)
+        begin = torch.cumsum(count[by_size], 0) - count[by_size]
+        place = torch.arange(total, device=ptr.device) - torch.repeat_interleave(begin, count[by_size], output_size=total)
+        low = self.ptr[:-1][graph]
+        self.tiles = torch.stack([low + place * self.tile_rows, low, self.ptr[1:][graph], torch.zeros_like(low)], 1).int().contiguous()
+
+    @property
+    def device(self):
+        return self.ptr.device
+
+    def to(self, device) -> "PackedGraphs":
+        out = object.__new__(PackedGraphs)
+        for k, v in self.__dict__.items():
+            setattr(out, k, v.to(device) if isinstance(v, Tensor) else v)
+        return out
+
+    @staticmethod
+    def from_batch(batch: Tensor, num_graphs: int) -> "PackedGraphs":
+        """From the graph of every node, ascending (``batch`` of ``torch_geometric``)."""
+        if batch.dtype != torch.int64 or batch.ndim != 1:
+            raise ValueError(f"int64 graph of every node expected, got {batch.dtype} of shape {tuple(batch.shape)}")
+        if batch.numel() and bool(((batch[1:] < batch[:-1]).any() | (batch[0] < 0) | (batch[-1] >= num_graphs))):
+            raise ValueError(f"the graph of every node must ascend within [0, {num_graphs})")
+        return PackedGraphs(_csr(batch, num_graphs), batch.numel())

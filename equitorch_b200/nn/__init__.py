@@ -4,6 +4,7 @@ from .activations import Gate
 from .cutoffs import CosineCutoff, MollifierCutoff, PolynomialCutoff
 from .radials import BesselBasis
 from .angular import SinCos
+from .attention import GraphAttention
 from .embedding import TypeEmbedding
 from .graph_layers import SO3LinearGraph
 from .linears import IrrepsLinear, IrrepWiseLinear, SO2Linear, SO3Linear
@@ -14,5 +15,5 @@ from .tensor_products import TensorDot, TensorProduct
 from .wigner_d import DenseWignerRotation, SparseWignerRotation, WignerD
 
 __all__ = ["Gate", "MeanSquaredNorm", "Norm", "SquaredNorm", "BatchRMSNorm", "LayerRMSNorm", "SinCos", "IrrepsLinear", "IrrepWiseLinear", "SO2Linear", "SO3Linear", "SO3LinearGraph", "SphericalHarmonics",
-           "TypeEmbedding",
+           "TypeEmbedding", "GraphAttention",
            "TensorDot", "TensorProduct", "DenseWignerRotation", "SparseWignerRotation", "WignerD", "functional"]

@@ -1,6 +1,7 @@
 """Functional API (same names as ``equitorch.nn.functional`` for the tensor-product path)."""
 from .activations import gating
 from .angular import sincos
+from .attention import graph_attention
 from .embedding import type_embedding
 from .linears import (irrep_wise_linear, irreps_linear, so2_linear_uu, so2_linear_uv, so3_linear_uu, so3_linear_uv,
                       tensor_product_1uu, tensor_product_1vu, tensor_product_u1u, tensor_product_u1v,

@@ -655,6 +655,37 @@ int64_t eqt_embedding_grad_scratch(int32_t dtype, int64_t n, int64_t types, int6
 int eqt_embedding_grad(int32_t dtype, const void* g, const int64_t* index, void* gw, int64_t n, int64_t types, int64_t width,
                        double scale, void* scratch, int64_t scratch_bytes, void* stream);
 
+/*
+ * Attention within the graphs of a packed batch.  q, k, v (n, comps, heads * head_channels) with strides in elements between nodes
+ * and components (channels are contiguous); out, grad_out, dq, dk, dv the same shape, contiguous.  A head's comps * head_channels
+ * <= 128 values of a node are one vector.  Node i attends to the nodes j of its graph:
+ *   s = scale <q_i, k_j>;  cap > 0: s = cap tanh(s / cap);  pos (n, 3) and slope (heads) given: s -= slope[h] |pos_i - pos_j|
+ *   out_i = sum_j softmax_j(s) v_j;   lse (heads, n): log2 of the sum of exp(s), written by the forward pass (NULL: not wanted)
+ * tiles (num_tiles, 4): first row, first node and one past the last node of the row's graph, 0; a tile is tile_rows (16, 32, 64)
+ * rows of one graph, cut at the graph's end.  The tiles are to cover each row at most once and to lie in [0, n); rows of no tile are
+ * neither read nor written.  Backward: delta (heads, n) is scratch; dpos (n, 3) and dslope (heads) are both given or both NULL, and
+ * with them geo (2, heads, n, 4) floats of scratch, zero in the rows of no tile, 16-byte aligned.  float32 or bfloat16 features,
+ * all else float32; sums in float32, no atomics.
+ */
+typedef struct eqt_attention_args {
+  int32_t dtype, heads, comps, head_channels, tile_rows;
+  float scale, cap;
+  int64_t n, num_tiles;
+  const int32_t* tiles;
+  const void *q, *k, *v;
+  int64_t q_node, q_comp, k_node, k_comp, v_node, v_comp;
+  const float *pos, *slope;
+  void* out;
+  float* lse;
+  const void* grad_out;
+  void *dq, *dk, *dv;
+  float* delta;
+  void* geo;
+  float *dpos, *dslope;
+} eqt_attention_args;
+int eqt_attention_forward(const eqt_attention_args* args, void* stream);
+int eqt_attention_backward(const eqt_attention_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
