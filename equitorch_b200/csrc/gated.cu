@@ -1,0 +1,231 @@
+// Gated linear layer: the C entry points, and the kernels without tensor cores for float64 and for sizes whose rows do not start on
+// 16-byte boundaries, where the tensor memory accelerator cannot copy tiles.
+//
+// The simple kernel is a tiled product of strided operands, 64 x 64 results a CTA of 256 threads, 4 x 4 a thread, 16 terms at a time;
+// it is bound by the multiply-adds.
+#include <algorithm>
+
+#include "gated.cuh"
+
+namespace eqt {
+namespace gated {
+namespace {
+
+enum Mode { FORWARD, PARTIALS, INPUT_GRAD, WEIGHT_GRAD };
+
+constexpr int TILE = 64, TERMS = 16;
+
+// Results [m][n] = sum_k A[m][k] B[k][n]; two products side by side (FORWARD, PARTIALS) or one.
+template <typename T, int MODE>
+__global__ void __launch_bounds__(256) simple_kernel(const GatedArgs p, int64_t row_tiles) {
+  using A = typename Acc<T>::type;
+  constexpr bool DUAL = MODE == FORWARD || MODE == PARTIALS;
+  __shared__ A sa[TERMS][TILE + 1], sb[DUAL ? 2 : 1][TERMS][TILE + 1];
+  const int tid = threadIdx.x, tm = tid / 16, tn = tid % 16;
+  const T *x = static_cast<const T*>(p.x), *w = static_cast<const T*>(p.w), *d = static_cast<const T*>(p.d);
+  const int64_t nf = p.n * p.f, cf = (int64_t)p.c * p.f;
+  int64_t m0, rows = MODE == WEIGHT_GRAD ? p.c : p.n, k0 = 0, k1;
+  const int n0 = blockIdx.y * TILE, cols = MODE == INPUT_GRAD ? p.c : p.f;
+  int j = 0, split = 0;
+  if (MODE == WEIGHT_GRAD) {
+    j = blockIdx.z & 1;
+    split = blockIdx.z >> 1;
+    m0 = (int64_t)blockIdx.x * TILE;
+    k0 = split * p.split_rows;
+    k1 = min(p.n, k0 + p.split_rows);
+  } else {
+    k1 = MODE == INPUT_GRAD ? 2 * (int64_t)p.f : p.c;
+  }
+  for (int64_t tile = MODE == WEIGHT_GRAD ? 0 : blockIdx.x; tile < row_tiles; tile += MODE == WEIGHT_GRAD ? row_tiles : gridDim.x) {
+    if (MODE != WEIGHT_GRAD) m0 = tile * TILE;
+    A acc[DUAL ? 2 : 1][4][4];
+#pragma unroll
+    for (int q = 0; q < (DUAL ? 2 : 1); ++q)
+#pragma unroll
+      for (int a = 0; a < 4; ++a)
+#pragma unroll
+        for (int b = 0; b < 4; ++b) acc[q][a][b] = A(0);
+    for (int64_t kb = k0; kb < k1; kb += TERMS) {
+      for (int i = tid; i < TILE * TERMS; i += 256) {
+        // neighbouring threads read neighbouring values of each operand
+        const int mk = MODE == WEIGHT_GRAD ? i / TILE : i % TERMS, mm = MODE == WEIGHT_GRAD ? i % TILE : i / TERMS;
+        const int64_t k = kb + mk, m = m0 + mm;
+        A v = A(0);
+        if (k < k1 && m < rows) {
+          if (DUAL) v = static_cast<A>(x[m * p.c + k]);
+          if (MODE == INPUT_GRAD) v = static_cast<A>(k < p.f ? d[m * p.f + k] : d[nf + m * p.f + k - p.f]);
+          if (MODE == WEIGHT_GRAD) v = static_cast<A>(x[k * p.c + m]);
+        }
+        sa[mk][mm] = v;
+        const int nk = MODE == INPUT_GRAD ? i % TERMS : i / TILE, nn = MODE == INPUT_GRAD ? i / TERMS : i % TILE;
+        const int64_t kn = kb + nk, n = n0 + nn;
+        A b0 = A(0), b1 = A(0);
+        if (kn < k1 && n < cols) {
+          if (DUAL) {
+            b0 = static_cast<A>(w[kn * p.f + n]);
+            b1 = static_cast<A>(w[cf + kn * p.f + n]);
+          }
+          if (MODE == INPUT_GRAD) b0 = static_cast<A>(kn < p.f ? w[n * p.f + kn] : w[cf + n * p.f + kn - p.f]);
+          if (MODE == WEIGHT_GRAD) b0 = static_cast<A>(d[j * nf + kn * p.f + n]);
+        }
+        sb[0][nk][nn] = b0;
+        if (DUAL) sb[DUAL ? 1 : 0][nk][nn] = b1;
+      }
+      __syncthreads();
+#pragma unroll 4
+      for (int k = 0; k < TERMS; ++k) {
+        A a[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) a[i] = sa[k][tm * 4 + i];
+#pragma unroll
+        for (int q = 0; q < (DUAL ? 2 : 1); ++q)
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            const A v = sb[q][k][tn + 16 * b];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[q][i][b] += a[i] * v;
+          }
+      }
+      __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const int64_t m = m0 + tm * 4 + i, n = n0 + tn + 16 * b;
+        if (m >= rows || n >= cols) continue;
+        if (MODE == FORWARD) {
+          static_cast<T*>(p.h)[m * p.f + n] = static_cast<T>(activate(acc[0][i][b], p.act).y * acc[DUAL ? 1 : 0][i][b]);
+        } else if (MODE == PARTIALS) {
+          const Value<A> v = activate(acc[0][i][b], p.act);
+          const A g = static_cast<A>(static_cast<const T*>(p.g)[m * p.f + n]);
+          static_cast<T*>(p.d)[m * p.f + n] = static_cast<T>(g * acc[DUAL ? 1 : 0][i][b] * v.dy);
+          static_cast<T*>(p.d)[nf + m * p.f + n] = static_cast<T>(g * v.y);
+        } else if (MODE == INPUT_GRAD) {
+          static_cast<T*>(p.dx)[m * p.c + n] = static_cast<T>(acc[0][i][b]);
+        } else {
+          static_cast<A*>(p.parts)[(split * 2 + j) * cf + m * p.f + n] = acc[0][i][b];
+        }
+      }
+  }
+}
+
+// dW = the sum over the parts of the rows, in their order
+template <typename T>
+__global__ void __launch_bounds__(256) sum_parts_kernel(const typename Acc<T>::type* __restrict__ parts, T* __restrict__ dw, int64_t size, int splits) {
+  using A = typename Acc<T>::type;
+  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < size; i += (int64_t)gridDim.x * blockDim.x) {
+    A sum = A(0);
+#pragma unroll 8
+    for (int s = 0; s < splits; ++s) sum += parts[s * size + i];
+    dw[i] = static_cast<T>(sum);
+  }
+}
+
+template <typename T, int MODE> int run_simple(const GatedArgs& p, cudaStream_t s) {
+  const int64_t tiles = ceil_div(p.n, TILE);
+  dim3 grid((unsigned)std::min<int64_t>(tiles, 1 << 20), (unsigned)ceil_div(MODE == INPUT_GRAD ? p.c : p.f, TILE));
+  if (MODE == WEIGHT_GRAD) grid = dim3((unsigned)ceil_div(p.c, TILE), grid.y, (unsigned)(2 * p.splits));
+  simple_kernel<T, MODE><<<grid, 256, 0, s>>>(p, MODE == WEIGHT_GRAD ? 1 : tiles);
+  return check_launch("gated_simple");
+}
+template <typename T> int backward_simple(const GatedArgs& p, cudaStream_t s) {
+  if (int rc = run_simple<T, PARTIALS>(p, s)) return rc;
+  if (p.dx)
+    if (int rc = run_simple<T, INPUT_GRAD>(p, s)) return rc;
+  return p.dw ? run_simple<T, WEIGHT_GRAD>(p, s) : EQT_OK;
+}
+
+}  // namespace
+
+int simple_forward(int dtype, const GatedArgs& p, cudaStream_t s) {
+  return dtype == EQT_F64 ? run_simple<double, FORWARD>(p, s) : dtype == EQT_F32 ? run_simple<float, FORWARD>(p, s) : run_simple<__nv_bfloat16, FORWARD>(p, s);
+}
+int simple_backward(int dtype, const GatedArgs& p, cudaStream_t s) {
+  return dtype == EQT_F64 ? backward_simple<double>(p, s) : dtype == EQT_F32 ? backward_simple<float>(p, s) : backward_simple<__nv_bfloat16>(p, s);
+}
+int sum_parts(int dtype, const GatedArgs& p, cudaStream_t s) {
+  const int64_t size = 2 * (int64_t)p.c * p.f;
+  const unsigned grid = flat_grid(size, 256, 8);
+  if (dtype == EQT_F64) sum_parts_kernel<double><<<grid, 256, 0, s>>>(static_cast<const double*>(p.parts), static_cast<double*>(p.dw), size, p.splits);
+  else if (dtype == EQT_F32) sum_parts_kernel<float><<<grid, 256, 0, s>>>(static_cast<const float*>(p.parts), static_cast<float*>(p.dw), size, p.splits);
+  else sum_parts_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(static_cast<const float*>(p.parts), static_cast<__nv_bfloat16*>(p.dw), size, p.splits);
+  return check_launch("gated_sum_parts");
+}
+
+namespace {
+
+int size_of(int dtype) { return dtype == EQT_F64 ? 8 : dtype == EQT_F32 ? 4 : 2; }
+
+int check_sizes(int dtype, int64_t n, int64_t c, int64_t f, int act) {
+  if (dtype != EQT_F32 && dtype != EQT_F64 && dtype != EQT_BF16) return fail(EQT_ERR_BAD_ARGUMENT, "gated: unknown dtype %d", dtype);
+  if (act < EQT_ACT_SILU || act > EQT_ACT_SIGMOID) return fail(EQT_ERR_BAD_ARGUMENT, "gated: unknown activation %d", act);
+  if (n < 0 || c < 0 || f < 0) return fail(EQT_ERR_BAD_ARGUMENT, "gated: negative size");
+  if (n > INT32_MAX - 128 || c > 1 << 20 || f > 1 << 20) return fail(EQT_ERR_UNSUPPORTED, "gated: at most 2^31 rows and 2^20 channels");
+  return EQT_OK;
+}
+
+// Whether the tensor memory accelerator can copy tiles of every operand: rows on 16-byte boundaries.
+bool aligned(int dtype, int64_t c, int64_t f, std::initializer_list<const void*> pointers) {
+  uintptr_t bits = (uintptr_t)(c * size_of(dtype)) | (uintptr_t)(f * size_of(dtype));
+  for (const void* p : pointers) bits |= reinterpret_cast<uintptr_t>(p);
+  return dtype != EQT_F64 && bits % 16 == 0;
+}
+
+// Rows are summed in parts so that every SM has a tile of the weights' gradient; a part has 512 rows at least, which the tensor cores
+// take in about the time of one partial result's way to memory and back.
+void split_rows(GatedArgs& p, int64_t n, int64_t c, int64_t f) {
+  const int64_t tiles = 2 * ceil_div(c, 128) * ceil_div(f, 256);
+  int64_t splits = std::max<int64_t>(1, std::min({sm_count() / tiles, ceil_div(n, 512), (int64_t)64}));
+  p.split_rows = ceil_div(ceil_div(n, splits), 64) * 64;
+  p.splits = (int)std::max<int64_t>(1, ceil_div(n, p.split_rows));
+}
+
+size_t up(size_t b) { return (b + 1023) / 1024 * 1024; }
+
+}  // namespace
+}  // namespace gated
+}  // namespace eqt
+
+using namespace eqt;
+using namespace eqt::gated;
+
+extern "C" int eqt_gated_forward(int32_t dtype, const void* x, const void* w, void* h, int64_t n, int64_t c, int64_t f, int32_t act,
+                                 int32_t* status, void* stream) {
+  if (int rc = check_sizes(dtype, n, c, f, act)) return rc;
+  if (n == 0 || f == 0) return EQT_OK;
+  if (!h || (c && (!x || !w)) || !status) return fail(EQT_ERR_BAD_ARGUMENT, "gated: NULL pointer");
+  GatedArgs p{};
+  p.x = x, p.w = w, p.h = h, p.n = n, p.c = (int)c, p.f = (int)f, p.act = act, p.status = status;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return c && aligned(dtype, c, f, {x, w, h}) ? tensor_forward(dtype, p, s) : simple_forward(dtype, p, s);
+}
+
+extern "C" int64_t eqt_gated_backward_scratch(int32_t dtype, int64_t n, int64_t c, int64_t f) {
+  if (check_sizes(dtype, n, c, f, 0) || n == 0 || f == 0 || c == 0) return 0;
+  GatedArgs p{};
+  split_rows(p, n, c, f);
+  return (int64_t)(up((size_t)2 * n * f * size_of(dtype)) + (size_t)p.splits * 2 * c * f * (dtype == EQT_F64 ? 8 : 4));
+}
+
+extern "C" int eqt_gated_backward(int32_t dtype, const void* x, const void* w, const void* g, void* dx, void* dw, void* scratch,
+                                  int64_t scratch_bytes, int64_t n, int64_t c, int64_t f, int32_t act, int32_t* status, void* stream) {
+  if (int rc = check_sizes(dtype, n, c, f, act)) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (n == 0 || f == 0 || c == 0) {
+    if (dx && n && c && cudaMemsetAsync(dx, 0, (size_t)n * c * size_of(dtype), s) != cudaSuccess) return fail(EQT_ERR_CUDA, "cudaMemsetAsync failed");
+    if (dw && f && c && cudaMemsetAsync(dw, 0, (size_t)2 * c * f * size_of(dtype), s) != cudaSuccess) return fail(EQT_ERR_CUDA, "cudaMemsetAsync failed");
+    return EQT_OK;
+  }
+  if (!x || !w || !g || !scratch || !status) return fail(EQT_ERR_BAD_ARGUMENT, "gated backward: NULL pointer");
+  const int64_t need = eqt_gated_backward_scratch(dtype, n, c, f);
+  if (scratch_bytes < need)
+    return fail(EQT_ERR_BAD_ARGUMENT, "gated backward: %lld bytes of scratch given, %lld needed", (long long)scratch_bytes, (long long)need);
+  GatedArgs p{};
+  p.x = x, p.w = w, p.g = g, p.dx = dx, p.dw = dw, p.n = n, p.c = (int)c, p.f = (int)f, p.act = act, p.status = status;
+  split_rows(p, n, c, f);
+  p.d = scratch;
+  p.parts = static_cast<unsigned char*>(scratch) + up((size_t)2 * n * f * size_of(dtype));
+  if (int rc = aligned(dtype, c, f, {x, w, g, dx, dw, scratch}) ? tensor_backward(dtype, p, s) : simple_backward(dtype, p, s)) return rc;
+  return dw ? sum_parts(dtype, p, s) : EQT_OK;
+}

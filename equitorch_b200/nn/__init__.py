@@ -6,6 +6,7 @@ from .radials import BesselBasis
 from .angular import SinCos
 from .attention import GraphAttention
 from .embedding import TypeEmbedding
+from .gated import GatedLinear
 from .graph_layers import SO3LinearGraph
 from .linears import IrrepsLinear, IrrepWiseLinear, SO2Linear, SO3Linear
 from .norm import MeanSquaredNorm, Norm, SquaredNorm
@@ -15,5 +16,5 @@ from .tensor_products import TensorDot, TensorProduct
 from .wigner_d import DenseWignerRotation, SparseWignerRotation, WignerD
 
 __all__ = ["Gate", "MeanSquaredNorm", "Norm", "SquaredNorm", "BatchRMSNorm", "LayerRMSNorm", "SinCos", "IrrepsLinear", "IrrepWiseLinear", "SO2Linear", "SO3Linear", "SO3LinearGraph", "SphericalHarmonics",
-           "TypeEmbedding", "GraphAttention",
+           "TypeEmbedding", "GraphAttention", "GatedLinear",
            "TensorDot", "TensorProduct", "DenseWignerRotation", "SparseWignerRotation", "WignerD", "functional"]

@@ -3,6 +3,7 @@ from .activations import gating
 from .angular import sincos
 from .attention import graph_attention
 from .embedding import type_embedding
+from .gated import gated_linear
 from .linears import (irrep_wise_linear, irreps_linear, so2_linear_uu, so2_linear_uv, so3_linear_uu, so3_linear_uv,
                       tensor_product_1uu, tensor_product_1vu, tensor_product_u1u, tensor_product_u1v,
                       tensor_product_uu1, tensor_product_vu1)
