@@ -65,54 +65,67 @@ __global__ void __launch_bounds__(256) embedding_kernel(const T* __restrict__ we
 // ---- sort by type -------------------------------------------------------------------------------
 // A row that names no type gets the key `types`, which sorts behind all others.
 __device__ __forceinline__ int key_of(const int64_t* index, const int32_t* keys, int64_t i, int64_t types) {
-  if (keys) return keys[i];
+  if (keys) return __ldg(keys + i);
   const int64_t t = __ldg(index + i);
   return (int)((uint64_t)t < (uint64_t)types ? t : types);
 }
 
-// Each warp owns `rows` rows in a row; counts[warp][bin] is how many of them have the digit.
+// Each warp owns `rows` rows in a row; within[warp][bin] is how many rows of the digit the warps of its CTA before it own,
+// counts[CTA][bin] how many the CTA does.
 __global__ void __launch_bounds__(SORT_THREADS) sort_count_kernel(const int64_t* __restrict__ index, const int32_t* __restrict__ keys,
-                                                                  int* __restrict__ counts, int64_t n, int64_t types, int64_t rows,
-                                                                  int shift, int bins) {
+                                                                  int* __restrict__ within, int* __restrict__ counts, int64_t n,
+                                                                  int64_t types, int64_t rows, int shift, int bins) {
   extern __shared__ int tally[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int* mine = tally + warp * bins;
   for (int b = lane; b < bins; b += 32) mine[b] = 0;
   __syncwarp();
   const int64_t w = (int64_t)blockIdx.x * SORT_WARPS + warp, lo = w * rows, hi = min(n, lo + rows);
+#pragma unroll 4
   for (int64_t i = lo + lane; i < hi; i += 32) atomicAdd(&mine[(key_of(index, keys, i, types) >> shift) & (bins - 1)], 1);   // counts: order is free
-  __syncwarp();
-  for (int b = lane; b < bins; b += 32) counts[w * bins + b] = mine[b];
+  __syncthreads();
+  for (int b = threadIdx.x; b < bins; b += SORT_THREADS) {
+    int run = 0;
+#pragma unroll
+    for (int v = 0; v < SORT_WARPS; ++v) {
+      within[((int64_t)blockIdx.x * SORT_WARPS + v) * bins + b] = run;
+      run += tally[v * bins + b];
+    }
+    counts[(int64_t)blockIdx.x * bins + b] = run;
+  }
 }
 
-// counts[warp][bin] becomes the number of rows of the digit that the warps before own; totals[bin] is their sum over all warps.
+// before[CTA][bin] is the number of rows of the digit that the CTAs before own, totals[bin] their number over all CTAs.
 // A lane is a digit, the 32 warps of the CTA share the rows of `counts`.
-__global__ void __launch_bounds__(1024) sort_scan_kernel(int* __restrict__ counts, int* __restrict__ totals, int warps, int bins) {
+__global__ void __launch_bounds__(1024) sort_scan_kernel(const int* __restrict__ counts, int* __restrict__ before, int* __restrict__ totals, int ctas,
+                                                         int bins) {
   __shared__ int part[32][33];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, bin = blockIdx.x * 32 + lane;
-  const int each = (warps + 31) / 32, lo = min(warps, warp * each), hi = min(warps, lo + each);
+  const int each = (ctas + 31) / 32, lo = min(ctas, warp * each), hi = min(ctas, lo + each);
   const bool there = bin < bins;
   int sum = 0;
-  for (int w = lo; w < hi; ++w) sum += there ? counts[(int64_t)w * bins + bin] : 0;
+#pragma unroll 8
+  for (int w = lo; w < hi; ++w) sum += there ? __ldg(counts + (int64_t)w * bins + bin) : 0;
   part[warp][lane] = sum;
   __syncthreads();
-  int before = 0, all = 0;
+  int run = 0, all = 0;
   for (int w = 0; w < 32; ++w) {
-    if (w < warp) before += part[w][lane];
+    if (w < warp) run += part[w][lane];
     all += part[w][lane];
   }
   if (warp == 0 && there) totals[bin] = all;
-  for (int w = lo; w < hi && there; ++w) {
-    int* c = counts + (int64_t)w * bins + bin;
-    const int v = *c;
-    *c = before;
-    before += v;
+#pragma unroll 8
+  for (int w = lo; w < hi; ++w) {
+    const int v = there ? __ldg(counts + (int64_t)w * bins + bin) : 0;
+    if (there) before[(int64_t)w * bins + bin] = run;
+    run += v;
   }
 }
 
 // Rows to their places, in their order within a digit: a warp takes 32 rows at a time, lanes of the same digit rank by lane.
 __global__ void __launch_bounds__(SORT_THREADS) sort_place_kernel(const int64_t* __restrict__ index, const int32_t* __restrict__ keys,
-                                                                  const int32_t* __restrict__ order, const int* __restrict__ counts,
+                                                                  const int32_t* __restrict__ order, const int* __restrict__ within,
+                                                                  const int* __restrict__ before,
                                                                   const int* __restrict__ totals, int32_t* __restrict__ keys_out,
                                                                   int32_t* __restrict__ order_out, int64_t n, int64_t types,
                                                                   int64_t rows, int shift, int bins) {
@@ -136,22 +149,30 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_place_kernel(const int64_t*
   __syncthreads();
   int* mine = place + warp * bins;
   const int64_t w = (int64_t)blockIdx.x * SORT_WARPS + warp, lo = w * rows, hi = min(n, lo + rows);
-  for (int b = lane; b < bins; b += 32) mine[b] = first[b] + counts[w * bins + b];
+  for (int b = lane; b < bins; b += 32) mine[b] = first[b] + before[(int64_t)blockIdx.x * bins + b] + within[w * bins + b];
   __syncwarp();
-  for (int64_t i0 = lo; i0 < hi; i0 += 32) {
-    const int64_t i = i0 + lane;
-    const bool there = i < hi;
-    const int key = there ? key_of(index, keys, i, types) : 0;
-    const int digit = there ? (key >> shift) & (bins - 1) : bins;              // lanes past the end are a digit of their own
-    const unsigned same = __match_any_sync(FULL, digit);
-    const int rank = __popc(same & ((1u << lane) - 1));
-    const int to = there ? mine[digit] + rank : 0;
-    __syncwarp();
-    if (there && rank == 0) mine[digit] += __popc(same);
-    __syncwarp();
-    if (there) {
-      keys_out[to] = key;
-      order_out[to] = order ? order[i] : (int32_t)i;
+  for (int64_t i0 = lo; i0 < hi; i0 += 128) {
+    int key[4], from[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {               // the loads of four steps together
+      const int64_t i = i0 + u * 32 + lane;
+      key[u] = i < hi ? key_of(index, keys, i, types) : 0;
+      from[u] = i < hi && order ? __ldg(order + i) : (int)i;
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const bool there = i0 + u * 32 + lane < hi;
+      const int digit = there ? (key[u] >> shift) & (bins - 1) : bins;         // lanes past the end are a digit of their own
+      const unsigned same = __match_any_sync(FULL, digit);
+      const int rank = __popc(same & ((1u << lane) - 1));
+      const int to = there ? mine[digit] + rank : 0;
+      __syncwarp();
+      if (there && rank == 0) mine[digit] += __popc(same);
+      __syncwarp();
+      if (there) {
+        keys_out[to] = key[u];
+        order_out[to] = from[u];
+      }
     }
   }
 }
@@ -252,7 +273,6 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const int32_t* __
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int teams = 32 / team, mine = lane / team, tl = lane % team;
   const int64_t c = (int64_t)blockIdx.x * JOIN_WARPS + warp, lo = c * piece, hi = min(n, lo + piece);
-  auto crossing = [&](int64_t end, int key) { return end < n && keys[end - 1] == key && keys[end] == key; };
   auto fold = [&](A(&sum)[V]) {                 // sums of the teams of a warp to team 0
     for (int o = 16; o >= team; o >>= 1) {
 #pragma unroll
@@ -263,22 +283,17 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const int32_t* __
   int key = types;
   if (c < pieces) {
     key = keys[hi - 1];
-    if (key < types && crossing(hi, key) && !(lo > 0 && keys[lo - 1] == key)) {
-      last = c + 1;                             // the run ends in the first piece whose end it does not cross
-      for (int step = 0; step < JOIN_ALONE / 32; ++step) {
-        const unsigned through = __ballot_sync(FULL, crossing(min(n, (last + lane + 1) * piece), key));
-        const int more = through == FULL ? 32 : __ffs(~through) - 1;
-        last += more;
-        if (more < 32) break;
-      }
-      if (last - c >= JOIN_ALONE) {             // or is longer than that: look for its end by halves
-        int64_t a = last * piece, b = n;
-        while (a < b) {
-          const int64_t m = (a + b) >> 1;
-          if (keys[m] == key) a = m + 1;
-          else b = m;
-        }
-        last = (a - 1) / piece;
+    if (key < types && hi < n && keys[hi] == key && !(lo > 0 && keys[lo - 1] == key)) {
+      // The run reaches into the pieces whose first row has its type: 32 of them are looked at a step, first the next ones, then by
+      // 32nds of what is left.
+      last = c + 1;                             // reaches in
+      int64_t past = pieces;                    // does not
+      for (int64_t step = 1; past - last > 1; step = (past - last + 31) / 32) {
+        const int64_t at = last + (lane + 1) * step;
+        const unsigned in = __ballot_sync(FULL, at < past && __ldg(keys + at * piece) == key);     // a run of ones from lane 0 on
+        const int reach = __popc(in);
+        if (reach < 32) past = min(past, last + (reach + 1) * step);
+        last += reach * step;
       }
     }
   }
@@ -379,7 +394,7 @@ struct GradPlan {
   int64_t warps, rows;      // of the sort
   int piece;
   int64_t pieces;
-  size_t keys, order, counts, totals, parts, bytes;       // scratch: two buffers each of keys and order
+  size_t keys, order, within, counts, before, totals, parts, bytes;       // scratch: two buffers each of keys and order
 };
 
 int size_of(int dtype) { return dtype == EQT_F64 ? 8 : dtype == EQT_F32 ? 4 : 2; }
@@ -396,14 +411,19 @@ GradPlan grad_plan(int dtype, int64_t n, int64_t types, int64_t width) {
   const int64_t most = (int64_t)sm_count() * 16;
   p.rows = std::max<int64_t>(128, ceil_div(ceil_div(n, most), 32) * 32);
   p.warps = ceil_div(ceil_div(n, p.rows), SORT_WARPS) * SORT_WARPS;
-  const int64_t teams = (int64_t)sm_count() * 80;
-  p.piece = (int)std::max<int64_t>(32, ceil_div(ceil_div(n, teams), UNROLL) * UNROLL);
+  int team = 1;                                           // lanes that have a row: one 16 bytes, at most 32
+  while (team < 32 && team * 16 < width * size_of(dtype)) team *= 2;
+  // Pieces so short that 512 threads an SM have one, but not so short that their borders cost more than their rows.
+  p.piece = (int)std::max<int64_t>(32, ceil_div(ceil_div(n, (int64_t)sm_count() * 512 / team), UNROLL) * UNROLL);
   p.pieces = ceil_div(n, p.piece);
   auto up = [](size_t b) { return (b + 255) / 256 * 256; };
   p.keys = 0;
   p.order = up((size_t)n * 4) * 2;
-  p.counts = p.order + up((size_t)n * 4) * 2;
-  p.totals = p.counts + up((size_t)p.warps * ((size_t)1 << p.digit_bits) * 4);
+  p.within = p.order + up((size_t)n * 4) * 2;
+  const size_t bins = (size_t)4 << p.digit_bits, ctas = (size_t)p.warps / SORT_WARPS;
+  p.counts = p.within + up(p.warps * bins);
+  p.before = p.counts + up(ctas * bins);
+  p.totals = p.before + up(ctas * bins);
   p.parts = p.totals + up((size_t)MAX_BINS * 4);
   p.bytes = p.parts + 2 * up((size_t)p.pieces * width * (dtype == EQT_F64 ? 8 : 4));
   return p;
@@ -433,7 +453,9 @@ int run_grad(int dtype, const void* g, const int64_t* index, void* gw, int64_t n
   const size_t n4 = ((size_t)n * 4 + 255) / 256 * 256;
   int32_t* keys[2] = {reinterpret_cast<int32_t*>(scratch + p.keys), reinterpret_cast<int32_t*>(scratch + p.keys + n4)};
   int32_t* order[2] = {reinterpret_cast<int32_t*>(scratch + p.order), reinterpret_cast<int32_t*>(scratch + p.order + n4)};
+  int* within = reinterpret_cast<int*>(scratch + p.within);
   int* counts = reinterpret_cast<int*>(scratch + p.counts);
+  int* before = reinterpret_cast<int*>(scratch + p.before);
   int* totals = reinterpret_cast<int*>(scratch + p.totals);
   const int bins = 1 << p.digit_bits;
   const unsigned grid = (unsigned)(p.warps / SORT_WARPS);
@@ -443,11 +465,11 @@ int run_grad(int dtype, const void* g, const int64_t* index, void* gw, int64_t n
     const int32_t* k = pass ? keys[at ^ 1] : nullptr;
     const int32_t* o = pass ? order[at ^ 1] : nullptr;
     const int shift = pass * p.digit_bits;
-    sort_count_kernel<<<grid, SORT_THREADS, shared, s>>>(index, k, counts, n, types, p.rows, shift, bins);
+    sort_count_kernel<<<grid, SORT_THREADS, shared, s>>>(index, k, within, counts, n, types, p.rows, shift, bins);
     if (int rc = check_launch("sort_count")) return rc;
-    sort_scan_kernel<<<(unsigned)ceil_div(bins, 32), 1024, 0, s>>>(counts, totals, (int)p.warps, bins);
+    sort_scan_kernel<<<(unsigned)ceil_div(bins, 32), 1024, 0, s>>>(counts, before, totals, (int)grid, bins);
     if (int rc = check_launch("sort_scan")) return rc;
-    sort_place_kernel<<<grid, SORT_THREADS, shared, s>>>(index, k, o, counts, totals, keys[at], order[at], n, types, p.rows, shift, bins);
+    sort_place_kernel<<<grid, SORT_THREADS, shared, s>>>(index, k, o, within, before, totals, keys[at], order[at], n, types, p.rows, shift, bins);
     if (int rc = check_launch("sort_place")) return rc;
   }
   at ^= 1;

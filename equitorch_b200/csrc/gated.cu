@@ -172,13 +172,16 @@ bool aligned(int dtype, int64_t c, int64_t f, std::initializer_list<const void*>
   return dtype != EQT_F64 && bits % 16 == 0;
 }
 
-// Rows are summed in parts so that every SM has a tile of the weights' gradient; a part has 512 rows at least, which the tensor cores
-// take in about the time of one partial result's way to memory and back.
-void split_rows(GatedArgs& p, int64_t n, int64_t c, int64_t f) {
-  const int64_t tiles = 2 * ceil_div(c, 128) * ceil_div(f, 256);
-  int64_t splits = std::max<int64_t>(1, std::min({sm_count() / tiles, ceil_div(n, 512), (int64_t)64}));
-  p.split_rows = ceil_div(ceil_div(n, splits), 64) * 64;
-  p.splits = (int)std::max<int64_t>(1, ceil_div(n, p.split_rows));
+// Rows are summed in parts so that the tiles of the weights' gradient fill the SMs evenly: as many parts as make the longest SM's work
+// shortest, where an item costs its rows and about 256 rows' time for its start, its end and its partial results.
+void split_rows(GatedArgs& p, int dtype, int64_t n, int64_t c, int64_t f) {
+  const int64_t tiles = 2 * ceil_div(c, 128) * ceil_div(f, dtype == EQT_BF16 ? 256 : 128), sms = sm_count();
+  int64_t best = INT64_MAX;
+  for (int64_t s = 1; s <= std::min<int64_t>(sms, ceil_div(n, 128)); ++s) {
+    const int64_t rows = ceil_div(ceil_div(n, s), 64) * 64, cost = ceil_div(tiles * s, sms) * (rows + 256);
+    if (cost < best) best = cost, p.split_rows = rows;
+  }
+  p.splits = (int)ceil_div(n, p.split_rows);
 }
 
 size_t up(size_t b) { return (b + 1023) / 1024 * 1024; }
@@ -198,13 +201,14 @@ extern "C" int eqt_gated_forward(int32_t dtype, const void* x, const void* w, vo
   GatedArgs p{};
   p.x = x, p.w = w, p.h = h, p.n = n, p.c = (int)c, p.f = (int)f, p.act = act, p.status = status;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return c && aligned(dtype, c, f, {x, w, h}) ? tensor_forward(dtype, p, s) : simple_forward(dtype, p, s);
+  if (!c || !aligned(dtype, c, f, {x, w, h})) return simple_forward(dtype, p, s);
+  return dtype == EQT_F32 ? tensor_forward_f32(p, s) : tensor_forward_bf16(p, s);
 }
 
 extern "C" int64_t eqt_gated_backward_scratch(int32_t dtype, int64_t n, int64_t c, int64_t f) {
   if (check_sizes(dtype, n, c, f, 0) || n == 0 || f == 0 || c == 0) return 0;
   GatedArgs p{};
-  split_rows(p, n, c, f);
+  split_rows(p, dtype, n, c, f);
   return (int64_t)(up((size_t)2 * n * f * size_of(dtype)) + (size_t)p.splits * 2 * c * f * (dtype == EQT_F64 ? 8 : 4));
 }
 
@@ -223,9 +227,12 @@ extern "C" int eqt_gated_backward(int32_t dtype, const void* x, const void* w, c
     return fail(EQT_ERR_BAD_ARGUMENT, "gated backward: %lld bytes of scratch given, %lld needed", (long long)scratch_bytes, (long long)need);
   GatedArgs p{};
   p.x = x, p.w = w, p.g = g, p.dx = dx, p.dw = dw, p.n = n, p.c = (int)c, p.f = (int)f, p.act = act, p.status = status;
-  split_rows(p, n, c, f);
+  split_rows(p, dtype, n, c, f);
   p.d = scratch;
   p.parts = static_cast<unsigned char*>(scratch) + up((size_t)2 * n * f * size_of(dtype));
-  if (int rc = aligned(dtype, c, f, {x, w, g, dx, dw, scratch}) ? tensor_backward(dtype, p, s) : simple_backward(dtype, p, s)) return rc;
+  const int rc = !aligned(dtype, c, f, {x, w, g, dx, dw, scratch}) ? simple_backward(dtype, p, s)
+                 : dtype == EQT_F32                                ? tensor_backward_f32(p, s)
+                                                                   : tensor_backward_bf16(p, s);
+  if (rc) return rc;
   return dw ? sum_parts(dtype, p, s) : EQT_OK;
 }

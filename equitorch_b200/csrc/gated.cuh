@@ -28,7 +28,11 @@ template <typename A> __device__ __forceinline__ A exp_neg(A x);
 template <> __device__ __forceinline__ float exp_neg(float x) { return __expf(-x); }
 template <> __device__ __forceinline__ double exp_neg(double x) { return exp(-x); }
 template <typename A> __device__ __forceinline__ A inverse(A x);
-template <> __device__ __forceinline__ float inverse(float x) { return __frcp_rn(x); }
+template <> __device__ __forceinline__ float inverse(float x) {            // one unit in the last place; 0 at infinity
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 template <> __device__ __forceinline__ double inverse(double x) { return 1.0 / x; }
 
 template <typename A> __device__ __forceinline__ Value<A> activate(A a, int act) {
@@ -44,8 +48,10 @@ template <typename A> __device__ __forceinline__ Value<A> activate(A a, int act)
 
 int simple_forward(int dtype, const GatedArgs& p, cudaStream_t s);
 int simple_backward(int dtype, const GatedArgs& p, cudaStream_t s);
-int tensor_forward(int dtype, const GatedArgs& p, cudaStream_t s);
-int tensor_backward(int dtype, const GatedArgs& p, cudaStream_t s);
+int tensor_forward_f32(const GatedArgs& p, cudaStream_t s);         // gated_f32.cu and gated_bf16.cu, which compile side by side
+int tensor_forward_bf16(const GatedArgs& p, cudaStream_t s);
+int tensor_backward_f32(const GatedArgs& p, cudaStream_t s);
+int tensor_backward_bf16(const GatedArgs& p, cudaStream_t s);
 int sum_parts(int dtype, const GatedArgs& p, cudaStream_t s);
 
 }  // namespace gated

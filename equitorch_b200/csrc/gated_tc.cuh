@@ -1,0 +1,619 @@
+// Gated linear layer on the 5th-generation tensor cores: one kernel of warp roles for its four products.
+//
+//   FORWARD      [a | u] = x [W0 | W1]           epilogue h = act(a) u
+//   PARTIALS     the same product                epilogue da, du from g
+//   INPUT_GRAD   dx = [da | du] [W0 | W1]^T      one sum over both halves
+//   WEIGHT_GRAD  dWj = x^T dj                    over parts of the rows, float32 partial results
+//
+// A CTA per SM strides through tiles of 128 rows; a k-block of 128 bytes a row (64 bfloat16, 32 float32) is a stage of the ring.
+// Warp 0 copies tiles (TMA), warp 1 issues the MMAs, the last warps (sixteen, eight for float32) empty the accumulators while the next tile is multiplied;
+// the dual products have both halves of the columns in one MMA, so the activation and the product never leave the SM.
+//
+// bfloat16: the MMA reads tiles as they lie in memory, along k or along the rows (both majors, 128-byte swizzle): 128 x 256 results
+// a tile, four stages of 48 KB.
+// float32: operands are split into TF32 pairs, three MMAs each, as everywhere in this library.  Four warps split a stage between the
+// copy and the MMA, big parts in place; a tile that lies along the rows is turned on the way, 32 x 32 values a warp at a time, so the
+// MMA always finds k along the row.  128 x 128 results a tile, three stages of 64 KB.  The adder of the tensor cores truncates, so the
+// products with small parts have a sum of their own, which leaves one truncation for eight terms in place of three, and a sum is taken
+// in pieces of 128 terms that the epilogue adds with ordinary rounding (128 terms: 4.5e-6 of the norm with one sum, FILL).
+//
+// Every wait is bounded, as in the other tensor-core kernels; on expiry the status flag is raised and the kernel ends.
+#pragma once
+
+#include <algorithm>
+
+#include "gated.cuh"
+
+namespace eqt {
+namespace gated {
+namespace {
+using namespace tc;
+
+enum Mode { FORWARD, PARTIALS, INPUT_GRAD, WEIGHT_GRAD };
+
+constexpr int PIECE = 4;                                 // k-blocks of a float32 piece
+
+template <typename T> struct Form;
+template <> struct Form<__nv_bfloat16> {
+  static constexpr int BK = 64, STAGES = 4, COLS = 256, SPLITTERS = 0, EPI = 16, A_BYTES = 16384, B_AT = 16384, STAGE = 49152;
+};
+template <> struct Form<float> {                         // A big, A small, B big, B small
+  static constexpr int BK = 32, STAGES = 3, COLS = 128, SPLITTERS = 4, EPI = 8, A_BYTES = 16384, B_AT = 32768, STAGE = 65536;
+};
+template <typename T> constexpr int threads() { return 32 * (2 + Form<T>::SPLITTERS + Form<T>::EPI); }
+// Results leave by 32 columns: a warp's patch is 32 rows of them.  PARTIALS has a stage less and two patches a warp, so that the next tile's g is on its way.
+template <typename T, int MODE> constexpr int stages() { return Form<T>::STAGES - (MODE == PARTIALS); }
+template <typename T, int MODE> constexpr size_t shared_bytes() {
+  return 1024 + (size_t)stages<T, MODE>() * Form<T>::STAGE + (MODE == PARTIALS ? 2 : 1) * Form<T>::EPI * 1024 * sizeof(T);
+}
+
+struct alignas(64) Launch {
+  CUtensorMap a[2], b[2];                                // WEIGHT_GRAD: a[0] x, b da and du; INPUT_GRAD: a da and du, b W0 and W1
+  void *out, *out2;
+  const void* g;
+  int64_t rows, out_pitch;                               // rows and columns of the results
+  unsigned items;
+  int64_t part;                                          // WEIGHT_GRAD: results between two partial ones
+  int cols, width;                                       // width: columns a tile (of each half, where there are two)
+  int row_tiles, col_tiles, kblocks;                     // kblocks: of one half for INPUT_GRAD, of all rows for WEIGHT_GRAD
+  int split_blocks;                                      // WEIGHT_GRAD: k-blocks a part
+  int* status;
+};
+
+// What tile a work item is.
+struct Item {
+  int64_t row;
+  int col, half, part, kb0, kb1;
+};
+template <int MODE> __device__ __forceinline__ Item item_of(const Launch& p, unsigned i) {
+  Item t{};
+  t.col = (int)(i % (unsigned)p.col_tiles) * p.width;
+  i /= (unsigned)p.col_tiles;
+  t.row = (int64_t)(MODE == WEIGHT_GRAD ? i % (unsigned)p.row_tiles : i) * TILE_M;
+  t.kb1 = MODE == INPUT_GRAD ? 2 * p.kblocks : p.kblocks;
+  if (MODE == WEIGHT_GRAD) {
+    i /= (unsigned)p.row_tiles;
+    t.half = (int)(i & 1);
+    t.part = (int)(i >> 1);
+    t.kb0 = t.part * p.split_blocks;
+    t.kb1 = min(p.kblocks, t.kb0 + p.split_blocks);
+  }
+  return t;
+}
+
+__device__ __forceinline__ uint32_t idesc_bf16(int n, bool a_rows, bool b_rows) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)a_rows << 15) | ((uint32_t)b_rows << 16) | ((uint32_t)(n >> 3) << 17) |
+         ((uint32_t)(TILE_M >> 4) << 24);
+}
+// Along the rows (MN-major), 128-byte swizzle: 64 values of M or N a line, eight k a group of 1024 bytes, the next 64 values `BK` lines on.
+__device__ __forceinline__ uint64_t desc_rows(uint32_t at) {
+  return (uint64_t)((at & 0x3FFFF) >> 4) | ((uint64_t)((Form<__nv_bfloat16>::BK * 128) >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+__device__ __forceinline__ void mma_bf16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate) : "memory");
+}
+
+// A block of 32 lines of 128 bytes, one warp: float32 to TF32 pairs, the big ones in place, the small ones `small` bytes on.
+__device__ __forceinline__ void split_block(unsigned char* block, int small, bool turn, int lane) {
+  if (!turn) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float4* at = reinterpret_cast<float4*>(block) + i * 32 + lane;
+      float4 hi, lo;
+      split_tf32(*at, hi, lo);
+      *at = hi;
+      *reinterpret_cast<float4*>(reinterpret_cast<unsigned char*>(at) + small) = lo;
+    }
+    return;
+  }
+  // lines are k, values along them rows: lane r collects row r and lays it down in the swizzled order of a row
+  float v[32];
+#pragma unroll
+  for (int k = 0; k < 32; ++k) v[k] = reinterpret_cast<const float*>(block + k * 128)[lane];
+  __syncwarp();
+#pragma unroll
+  for (int c = 0; c < 8; ++c) {
+    float4 hi, lo;
+    split_tf32(make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]), hi, lo);
+    unsigned char* at = block + lane * 128 + ((c ^ (lane & 7)) << 4);
+    *reinterpret_cast<float4*>(at) = hi;
+    *reinterpret_cast<float4*>(at + small) = lo;
+  }
+}
+
+// 32 lines of 32 values (or, as float32 from a bfloat16 kernel, of 16) between global memory and a warp's patch, line r at row r of
+// `base`, pieces of 16 bytes; in the patch the pieces of a line are permuted so that eight lanes' lines, and the lines that eight lanes
+// copy, fall on all banks.
+template <typename T> __device__ __forceinline__ uint4* patch_at(unsigned char* patch, int line, int piece) {
+  if constexpr (sizeof(T) == 4) return reinterpret_cast<uint4*>(patch + line * 128 + ((piece ^ (line & 7)) << 4));
+  return reinterpret_cast<uint4*>(patch + line * 64 + ((piece ^ ((line >> 1) & 3)) << 4));
+}
+template <typename T> __device__ __forceinline__ void patch_out(unsigned char* patch, unsigned char* base, int64_t pitch, int lines, int pieces, int lane) {
+  constexpr int PER = 2 * (int)sizeof(T), STEP = 32 / PER;       // pieces of a line, lines at a time
+  __syncwarp();
+  const int piece = lane % PER;
+#pragma unroll
+  for (int i = 0; i < 32 / STEP; ++i) {
+    const int line = i * STEP + lane / PER;
+    if (line < lines && piece < pieces) *reinterpret_cast<uint4*>(base + line * pitch + piece * 16) = *patch_at<T>(patch, line, piece);
+  }
+  __syncwarp();
+}
+template <typename T>
+__device__ __forceinline__ void patch_in(unsigned char* patch, const unsigned char* base, int64_t pitch, int lines, int pieces, int lane) {
+  constexpr int PER = 2 * (int)sizeof(T), STEP = 32 / PER;
+  const int piece = lane % PER;
+#pragma unroll
+  for (int i = 0; i < 32 / STEP; ++i) {
+    const int line = i * STEP + lane / PER;
+    const bool there = line < lines && piece < pieces;
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                 ::"r"(s32(patch_at<T>(patch, line, piece))), "l"(there ? base + line * pitch + piece * 16 : base), "r"(there ? 16 : 0) : "memory");
+  }
+}
+// Loads of 16 columns of two accumulators, and the wait that the values of the loads before it pass through.
+__device__ __forceinline__ void tmem_issue16(uint32_t at, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+        "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(at) : "memory");
+}
+__device__ __forceinline__ void tmem_arrived(uint32_t (&r)[16], uint32_t (&q)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
+                 "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(q[0]), "+r"(q[1]), "+r"(q[2]), "+r"(q[3]),
+                 "+r"(q[4]), "+r"(q[5]), "+r"(q[6]), "+r"(q[7]), "+r"(q[8]), "+r"(q[9]), "+r"(q[10]), "+r"(q[11]), "+r"(q[12]), "+r"(q[13]),
+                 "+r"(q[14]), "+r"(q[15])
+               :: "memory");
+}
+
+// 16 bytes of values
+template <typename T> __device__ __forceinline__ uint4 to16(const float (&v)[16 / sizeof(T)]) {
+  uint32_t r[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      r[i] = __float_as_uint(v[i]);
+    } else {
+      const __nv_bfloat162 two = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+      r[i] = *reinterpret_cast<const uint32_t*>(&two);
+    }
+  }
+  return make_uint4(r[0], r[1], r[2], r[3]);
+}
+template <typename T> __device__ __forceinline__ void from16(const uint4& u, float (&v)[16 / sizeof(T)]) {
+  const uint32_t r[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      v[i] = __uint_as_float(r[i]);
+    } else {
+      v[2 * i] = __uint_as_float(r[i] << 16);
+      v[2 * i + 1] = __uint_as_float(r[i] & 0xffff0000u);
+    }
+  }
+}
+// A lane's 32 values to its line of the patch.
+template <typename T> __device__ __forceinline__ void line_put(unsigned char* patch, int lane, const float (&v)[32]) {
+  constexpr int GROUP = 16 / (int)sizeof(T);
+#pragma unroll
+  for (int q = 0; q < 32 / GROUP; ++q) {
+    float x[GROUP];
+#pragma unroll
+    for (int i = 0; i < GROUP; ++i) x[i] = v[q * GROUP + i];
+    *patch_at<T>(patch, lane, q) = to16<T>(x);
+  }
+}
+
+template <typename T, int MODE, int ACT>
+__global__ void __launch_bounds__(threads<T>(), 1) gated_tc_kernel(const __grid_constant__ Launch p) {
+  using S = Form<T>;
+  constexpr bool F32 = sizeof(T) == 4, DUAL = MODE == FORWARD || MODE == PARTIALS;
+  constexpr bool A_TURNED = MODE == WEIGHT_GRAD, B_TURNED = MODE != INPUT_GRAD;      // the operand lies along the rows
+  constexpr int LINE = 128 / (int)sizeof(T);                                          // values of a line
+  constexpr int STAGES = stages<T, MODE>();
+  constexpr int ACC_COLS = F32 ? 2 * S::COLS : S::COLS;                               // of tensor memory: float32 has two sums
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ uint64_t full[STAGES], ready[STAGES], empty[STAGES], acc_full[2], acc_empty[2];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_flag;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int n_mma = DUAL ? 2 * p.width : p.width;                                     // columns of an MMA
+  if (tid == 0) {
+    abort_flag = 0;
+    for (int s = 0; s < STAGES; ++s) {
+      bar_init(&full[s], 1);
+      bar_init(&ready[s], F32 ? S::SPLITTERS : 1);
+      bar_init(&empty[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      bar_init(&acc_full[a], 1);
+      bar_init(&acc_empty[a], S::EPI);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s32(&tmem_slot)), "r"(2 * ACC_COLS) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  volatile int* ab = &abort_flag;
+
+  if (warp == 0) {
+    // ---------------- copies ----------------
+    if (lane == 0) {
+      int s = 0;
+      uint32_t ph = 1;
+      bool ok = true;
+      const uint32_t bytes = S::A_BYTES + (uint32_t)n_mma * 128;
+      for (unsigned i = blockIdx.x; i < p.items && ok && !*ab; i += gridDim.x) {
+        const Item t = item_of<MODE>(p, i);
+        for (int kb = t.kb0; kb < t.kb1; ++kb) {
+          if (!bar_wait(&empty[s], ph, ab)) { ok = false; break; }
+          unsigned char* st = base + (size_t)s * S::STAGE;
+          uint64_t* bar = &full[s];
+          bar_expect_tx(bar, bytes);
+          const int h = MODE == INPUT_GRAD ? kb >= p.kblocks : t.half, k = (MODE == INPUT_GRAD && h ? kb - p.kblocks : kb) * S::BK;
+          if (A_TURNED) {
+#pragma unroll
+            for (int c = 0; c < TILE_M / LINE; ++c) tma_load_2d(st + c * S::BK * 128, &p.a[0], (int)t.row + c * LINE, k, bar);
+          } else {
+            tma_load_2d(st, &p.a[MODE == INPUT_GRAD ? h : 0], k, (int)t.row, bar);
+          }
+          unsigned char* sb = st + S::B_AT;
+          if (MODE == INPUT_GRAD) {
+            tma_load_2d(sb, &p.b[h], k, t.col, bar);
+          } else {
+            for (int q = 0; q < (DUAL ? 2 : 1); ++q)
+              for (int c = 0; c < p.width / LINE; ++c, sb += S::BK * 128) tma_load_2d(sb, &p.b[DUAL ? q : t.half], t.col + c * LINE, k, bar);
+          }
+          if (++s == STAGES) s = 0, ph ^= 1;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------- MMAs ----------------
+    if (lane == 0) {
+      int s = 0;
+      uint32_t ph = 0;
+      int piece = 0;
+      bool ok = true;
+      const uint32_t idesc = F32 ? umma_idesc_tf32(n_mma) : idesc_bf16(n_mma, A_TURNED, B_TURNED);
+      for (unsigned i = blockIdx.x; i < p.items && ok && !*ab; i += gridDim.x) {
+        const Item t = item_of<MODE>(p, i);
+        for (int k0 = t.kb0; k0 < t.kb1 && ok; ++piece) {
+          const int k1 = F32 ? min(k0 + PIECE, t.kb1) : t.kb1, a = piece & 1;
+          if (!bar_wait(&acc_empty[a], (uint32_t)(((piece >> 1) & 1) ^ 1), ab)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t d = tmem + (uint32_t)(a * ACC_COLS);
+          for (int kb = k0; kb < k1; ++kb) {
+            if (!bar_wait(F32 ? &ready[s] : &full[s], ph, ab)) { ok = false; break; }
+            tc_fence_after();
+            const uint32_t at = s32(base + (size_t)s * S::STAGE), bt = at + S::B_AT;
+            if (F32) {
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                const uint64_t ah = umma_desc(at + q * 32), al = umma_desc(at + S::A_BYTES + q * 32);
+                const uint64_t bh = umma_desc(bt + q * 32), bl = umma_desc(bt + S::COLS * 128 + q * 32);
+                umma_tf32(d, ah, bh, idesc, kb != k0 || q);
+                umma_tf32(d + S::COLS, al, bh, idesc, kb != k0 || q);
+                umma_tf32(d + S::COLS, ah, bl, idesc, 1);
+              }
+            } else {
+#pragma unroll
+              for (int q = 0; q < 4; ++q)
+                mma_bf16(d, A_TURNED ? desc_rows(at + q * 2048) : umma_desc(at + q * 32), B_TURNED ? desc_rows(bt + q * 2048) : umma_desc(bt + q * 32),
+                         idesc, kb != k0 || q);
+            }
+            umma_commit(&empty[s]);
+            if (++s == STAGES) s = 0, ph ^= 1;
+          }
+          if (ok) umma_commit(&acc_full[a]);
+          k0 = k1;
+        }
+      }
+    }
+  } else if (warp < 2 + S::SPLITTERS) {
+    // ---------------- float32 to TF32 pairs ----------------
+    int s = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    const int w = warp - 2;
+    for (unsigned i = blockIdx.x; i < p.items && ok && !*ab; i += gridDim.x) {
+      const Item t = item_of<MODE>(p, i);
+      for (int kb = t.kb0; kb < t.kb1; ++kb) {
+        if (!bar_wait(&full[s], ph, ab)) { ok = false; break; }
+        unsigned char* st = base + (size_t)s * S::STAGE;
+        split_block(st + w * 4096, S::A_BYTES, A_TURNED, lane);
+        for (int b = w; b < n_mma / 32; b += S::SPLITTERS) split_block(st + S::B_AT + b * 4096, S::COLS * 128, B_TURNED, lane);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) bar_arrive(&ready[s]);
+        if (++s == STAGES) s = 0, ph ^= 1;
+      }
+    }
+  } else {
+    // ---------------- epilogue ----------------
+    // Warps of the same quarter of the lanes share a tile's columns, 32 at a time in turn; of the dual products, 32 of each half.
+    constexpr int SHARES = S::EPI / 4, GROUP = 16 / (int)sizeof(T);
+    const int e = warp - 2 - S::SPLITTERS, quarter = warp & 3, share = e >> 2;
+    unsigned char* patch = base + (size_t)STAGES * S::STAGE + (size_t)e * 1024 * sizeof(T);
+    unsigned char* other = patch + S::EPI * 1024 * sizeof(T);                         // PARTIALS
+    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
+    const int64_t pitch = p.out_pitch * (int)sizeof(T);
+    int piece = 0;
+    bool ok = true;
+    // PARTIALS: g of a tile, asked for a tile before it is used (a share has at most one turn of 32 columns there)
+    auto fetch = [&](unsigned item, unsigned char* where) {
+      const Item x = item_of<MODE>(p, item);
+      const int64_t r = x.row + quarter * 32;
+      const int c = x.col + share * 32, here = (int)max((int64_t)0, min((int64_t)32, p.rows - r));
+      const int valid = share * 32 < p.width ? max(0, min(32, p.cols - c)) : 0;
+      patch_in<T>(where, reinterpret_cast<const unsigned char*>(static_cast<const T*>(p.g) + (here > 0 && valid > 0 ? r * p.out_pitch + c : 0)), pitch,
+                  here, valid / GROUP, lane);
+    };
+    if (MODE == PARTIALS) {
+      if (blockIdx.x < p.items) fetch(blockIdx.x, patch);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    for (unsigned i = blockIdx.x; i < p.items && ok && !*ab; i += gridDim.x) {
+      const Item t = item_of<MODE>(p, i);
+      const int64_t row = t.row + quarter * 32;
+      const int lines = (int)max((int64_t)0, min((int64_t)32, p.rows - row));
+      if (MODE == PARTIALS) {
+        if (i + gridDim.x < p.items) fetch(i + gridDim.x, other);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      }
+      // float32 sums come in pieces and gather in registers: the share's two turns, or its turn of each half
+      float sum[F32 ? 2 : 1][32];
+      uint32_t d = 0;
+      const int pieces = F32 ? (t.kb1 - t.kb0 + PIECE - 1) / PIECE : 1;
+      for (int q = 0; q < pieces; ++q, ++piece) {
+        const int a = piece & 1;
+        if (!bar_wait(&acc_full[a], (uint32_t)((piece >> 1) & 1), ab)) { ok = false; break; }
+        tc_fence_after();
+        d = lanes + (uint32_t)(a * ACC_COLS);
+        if (F32) {
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            const int at = DUAL ? b * p.width + share * 32 : (share + b * SHARES) * 32;
+            if (at >= n_mma) continue;                                                // a narrow tile: the share has no such columns
+#pragma unroll
+            for (int h = 0; h < 32; h += 16) {
+              float v[16];
+              tmem_ld16(d + S::COLS + at + h, v);
+#pragma unroll
+              for (int c = 0; c < 16; ++c) sum[F32 ? b : 0][h + c] = q ? sum[F32 ? b : 0][h + c] + v[c] : v[c];
+              tmem_ld16(d + at + h, v);
+#pragma unroll
+              for (int c = 0; c < 16; ++c) sum[F32 ? b : 0][h + c] += v[c];
+            }
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) bar_arrive(&acc_empty[a]);
+        }
+      }
+      if (!ok) break;
+#pragma unroll
+      for (int turn = 0; turn < 2; ++turn) {
+        const int c0 = (share + turn * SHARES) * 32;
+        if (c0 >= p.width || (DUAL && turn)) break;
+        const int col = t.col + c0, valid = max(0, min(32, p.cols - col));            // columns of this turn in the results
+        const int64_t at = row * p.out_pitch + col;
+        if (!DUAL) {
+          float v[32];
+          if constexpr (F32) {
+#pragma unroll
+            for (int c = 0; c < 32; ++c) v[c] = sum[turn][c];
+          } else {
+            tmem_ld32(d + c0, v);
+          }
+          if (MODE == INPUT_GRAD || F32) {
+            line_put<T>(patch, lane, v);
+            T* out = static_cast<T*>(p.out) + at + (MODE == WEIGHT_GRAD ? (t.part * 2 + t.half) * p.part : 0);
+            patch_out<T>(patch, reinterpret_cast<unsigned char*>(out), pitch, lines, valid / GROUP, lane);
+          } else {                                                                    // partial results are float32: 16 columns at a time
+            float* out = static_cast<float*>(p.out) + at + (t.part * 2 + t.half) * p.part;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                const float x[4] = {v[h * 16 + 4 * c], v[h * 16 + 4 * c + 1], v[h * 16 + 4 * c + 2], v[h * 16 + 4 * c + 3]};
+                *patch_at<T>(patch, lane, c) = to16<float>(x);
+              }
+              patch_out<T>(patch, reinterpret_cast<unsigned char*>(out + h * 16), p.out_pitch * 4, lines, min(16, max(0, valid - h * 16)) / 4, lane);
+            }
+          }
+          continue;
+        }
+        // du waits in registers while da leaves through the patch, in which it takes the place of g
+        uint4 second[F32 ? 1 : 4];
+        if (MODE == PARTIALS) {
+          asm volatile("cp.async.wait_group 1;" ::: "memory");
+          __syncwarp();
+        }
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          uint32_t a[16], u[16];
+          if constexpr (!F32) {
+            tmem_issue16(d + c0 + b * 16, a);
+            tmem_issue16(d + p.width + c0 + b * 16, u);
+            tmem_arrived(a, u);
+          }
+#pragma unroll
+          for (int q = 0; q < 16 / GROUP; ++q) {
+            uint4* at16 = patch_at<T>(patch, lane, b * (16 / GROUP) + q);
+            float x[GROUP], y[GROUP], g[GROUP];
+            if (MODE == PARTIALS) from16<T>(*at16, g);
+#pragma unroll
+            for (int c = 0; c < GROUP; ++c) {
+              const int j = q * GROUP + c;
+              float ai, ui;
+              if constexpr (F32) {
+                ai = sum[0][b * 16 + j];
+                ui = sum[1][b * 16 + j];
+              } else {
+                ai = __uint_as_float(a[j]);
+                ui = __uint_as_float(u[j]);
+              }
+              const Value<float> v = activate(ai, ACT);
+              if (MODE == FORWARD) {
+                x[c] = v.y * ui;
+              } else {
+                x[c] = g[c] * ui * v.dy;
+                y[c] = g[c] * v.y;
+                if (F32) sum[F32 ? 1 : 0][b * 16 + j] = y[c];
+              }
+            }
+            *at16 = to16<T>(x);
+            if (MODE == PARTIALS && !F32) second[F32 ? 0 : b * (16 / GROUP) + q] = to16<T>(y);
+          }
+        }
+        patch_out<T>(patch, reinterpret_cast<unsigned char*>(static_cast<T*>(p.out) + at), pitch, lines, valid / GROUP, lane);
+        if (MODE == PARTIALS) {
+          if constexpr (F32) {
+            line_put<T>(patch, lane, sum[1]);
+          } else {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) *patch_at<T>(patch, lane, c) = second[c];
+          }
+          patch_out<T>(patch, reinterpret_cast<unsigned char*>(static_cast<T*>(p.out2) + at), pitch, lines, valid / GROUP, lane);
+        }
+      }
+      if (!F32) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) bar_arrive(&acc_empty[(piece - 1) & 1]);
+      }
+      if (MODE == PARTIALS) {
+        unsigned char* t0 = patch;
+        patch = other;
+        other = t0;
+      }
+    }
+    if (MODE == PARTIALS) asm volatile("cp.async.wait_all;" ::: "memory");
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * ACC_COLS) : "memory");
+  }
+  if (tid == 0 && abort_flag) {
+    atomicExch(p.status, 2);
+    let_copies_land(full, STAGES);
+  }
+}
+
+// ---- host side ----------------------------------------------------------------------------------
+// A (rows, columns) matrix, columns next to each other, in boxes of `line` columns by `lines` rows.
+template <typename T>
+int map_of(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int line, int lines, bool swizzle) {
+  EncodeTiledFn enc = encode_tiled();
+  if (!enc) return fail(EQT_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
+  int dev = 0;                                           // the encoder needs a current context (see make_map)
+  if (cudaGetDevice(&dev) == cudaSuccess) cudaSetDevice(dev);
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)cols * sizeof(T)};
+  const cuuint32_t box[2] = {(cuuint32_t)line, (cuuint32_t)lines}, ones[2] = {1, 1};
+  const CUresult r = enc(map, sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims,
+                         strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? EQT_OK : fail(EQT_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
+}
+
+// Columns a tile: as few tiles as `most` allows, of one width, a multiple of the columns of a line.  Narrower ones where that leaves
+// SMs idle: a small call is bound by how long one tile takes.
+int width_of(int cols, int most, int line, int64_t others) {
+  int width;
+  for (;; most /= 2) {
+    const int tiles = (int)ceil_div(cols, most);
+    width = (int)ceil_div(ceil_div(cols, tiles), line) * line;
+    if (others * ceil_div(cols, width) * 2 > tc::sm_count() || most / 2 < line) return width;
+  }
+}
+
+template <typename T, int MODE, int ACT = EQT_ACT_SILU> int launch(const GatedArgs& a, cudaStream_t s) {
+  using S = Form<T>;
+  constexpr int LINE = 128 / (int)sizeof(T);
+  constexpr bool DUAL = MODE == FORWARD || MODE == PARTIALS, F32 = sizeof(T) == 4;
+  const size_t size = sizeof(T);
+  const char *w = static_cast<const char*>(a.w), *d = static_cast<const char*>(a.d);
+  const char* w1 = w + (size_t)a.c * a.f * size;
+  const char* d1 = d ? d + (size_t)a.n * a.f * size : nullptr;
+  Launch p{};
+  int rc = EQT_OK;
+  // Operands that lie along the rows come in boxes of one line of values by a k-block; for float32 they are turned on the way and
+  // need no swizzle.
+  if (DUAL) {
+    p.cols = a.f, p.rows = a.n, p.kblocks = (int)ceil_div(a.c, S::BK);
+    p.width = width_of(a.f, S::COLS / 2, LINE, ceil_div(a.n, TILE_M));
+    rc = map_of<T>(&p.a[0], a.x, a.n, a.c, LINE, TILE_M, true);
+    if (!rc) rc = map_of<T>(&p.b[0], w, a.c, a.f, LINE, S::BK, !F32);
+    if (!rc) rc = map_of<T>(&p.b[1], w1, a.c, a.f, LINE, S::BK, !F32);
+    p.out = MODE == FORWARD ? a.h : a.d;
+    p.out2 = const_cast<char*>(d1);
+    p.g = a.g;
+  } else if (MODE == INPUT_GRAD) {
+    p.cols = a.c, p.rows = a.n, p.kblocks = (int)ceil_div(a.f, S::BK);
+    p.width = width_of(a.c, S::COLS, LINE, ceil_div(a.n, TILE_M));
+    rc = map_of<T>(&p.a[0], d, a.n, a.f, LINE, TILE_M, true);
+    if (!rc) rc = map_of<T>(&p.a[1], d1, a.n, a.f, LINE, TILE_M, true);
+    if (!rc) rc = map_of<T>(&p.b[0], w, a.c, a.f, LINE, p.width, true);
+    if (!rc) rc = map_of<T>(&p.b[1], w1, a.c, a.f, LINE, p.width, true);
+    p.out = a.dx;
+  } else {
+    p.cols = a.f, p.rows = a.c, p.kblocks = (int)ceil_div(a.n, S::BK);
+    p.width = width_of(a.f, S::COLS, LINE, 2 * a.splits * ceil_div(a.c, TILE_M));
+    p.split_blocks = (int)(a.split_rows / S::BK);
+    p.part = (int64_t)a.c * a.f;
+    rc = map_of<T>(&p.a[0], a.x, a.n, a.c, LINE, S::BK, !F32);
+    if (!rc) rc = map_of<T>(&p.b[0], d, a.n, a.f, LINE, S::BK, !F32);
+    if (!rc) rc = map_of<T>(&p.b[1], d1, a.n, a.f, LINE, S::BK, !F32);
+    p.out = a.parts;
+  }
+  if (rc) return rc;
+  p.out_pitch = p.cols;
+  p.row_tiles = (int)ceil_div(p.rows, TILE_M);
+  p.col_tiles = (int)ceil_div(p.cols, p.width);
+  const int64_t items = (int64_t)p.row_tiles * p.col_tiles * (MODE == WEIGHT_GRAD ? 2 * a.splits : 1);
+  if (items > INT32_MAX / 2) return fail(EQT_ERR_UNSUPPORTED, "gated: %lld tiles are more than one launch takes", (long long)items);
+  p.items = (unsigned)items;
+  p.status = a.status;
+  if (int r = allow_shared(gated_tc_kernel<T, MODE, ACT>, shared_bytes<T, MODE>())) return r;
+  const unsigned grid = (unsigned)std::min<int64_t>(items, tc::sm_count());
+  gated_tc_kernel<T, MODE, ACT><<<grid, threads<T>(), shared_bytes<T, MODE>(), s>>>(p);
+  return check_launch("gated_tc");
+}
+
+template <typename T, int MODE> int launch_dual(const GatedArgs& a, cudaStream_t s) {
+  switch (a.act) {
+    case EQT_ACT_SILU: return launch<T, MODE, EQT_ACT_SILU>(a, s);
+    case EQT_ACT_GELU: return launch<T, MODE, EQT_ACT_GELU>(a, s);
+    case EQT_ACT_RELU: return launch<T, MODE, EQT_ACT_RELU>(a, s);
+    default: return launch<T, MODE, EQT_ACT_SIGMOID>(a, s);
+  }
+}
+
+template <typename T> int backward(const GatedArgs& a, cudaStream_t s) {
+  if (int rc = launch_dual<T, PARTIALS>(a, s)) return rc;
+  if (a.dx)
+    if (int rc = launch<T, INPUT_GRAD>(a, s)) return rc;
+  return a.dw ? launch<T, WEIGHT_GRAD>(a, s) : EQT_OK;
+}
+
+}  // namespace
+}  // namespace gated
+}  // namespace eqt
