@@ -25,7 +25,11 @@ struct GatedArgs {
 // act(a) and its derivative in the arithmetic type
 template <typename A> struct Value { A y, dy; };
 template <typename A> __device__ __forceinline__ A exp_neg(A x);
-template <> __device__ __forceinline__ float exp_neg(float x) { return __expf(-x); }
+template <> __device__ __forceinline__ float exp_neg(float x) {            // results below 2^-126 are zero, which saves their scaling
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * -1.4426950408889634f));
+  return y;
+}
 template <> __device__ __forceinline__ double exp_neg(double x) { return exp(-x); }
 template <typename A> __device__ __forceinline__ A inverse(A x);
 template <> __device__ __forceinline__ float inverse(float x) {            // one unit in the last place; 0 at infinity

@@ -10,12 +10,15 @@
 // the dual products have both halves of the columns in one MMA, so the activation and the product never leave the SM.
 //
 // bfloat16: the MMA reads tiles as they lie in memory, along k or along the rows (both majors, 128-byte swizzle): 128 x 256 results
-// a tile, four stages of 48 KB.
+// a tile, four stages of 48 KB.  What bounds that is L2: a k-block of 48 KB per 512 cycles of MMA and SM is 12 to 14 TB/s over all
+// SMs, and no more arrived.  So where there is work for all of them, two CTAs of a cluster share a tile of 256 x 256: each copies its
+// 128 rows of A and half of B, 32 KB a k-block, the first one's MMAs read both SMs' shared memory, and each SM has the results of its
+// rows (100k x 256 -> 1024: gradient of x 101 -> 93 us, of the weights 90 -> 83; 8192 x 1024 -> 4096: 115 -> 103).
 // float32: operands are split into TF32 pairs, three MMAs each, as everywhere in this library.  Four warps split a stage between the
 // copy and the MMA, big parts in place; a tile that lies along the rows is turned on the way, 32 x 32 values a warp at a time, so the
 // MMA always finds k along the row.  128 x 128 results a tile, three stages of 64 KB.  The adder of the tensor cores truncates, so the
 // products with small parts have a sum of their own, which leaves one truncation for eight terms in place of three, and a sum is taken
-// in pieces of 128 terms that the epilogue adds with ordinary rounding (128 terms: 4.5e-6 of the norm with one sum, FILL).
+// in pieces of 128 terms that the epilogue adds with ordinary rounding (128 terms: 4.5e-6 of the norm with one sum, 7e-7 so).
 //
 // Every wait is bounded, as in the other tensor-core kernels; on expiry the status flag is raised and the kernel ends.
 #pragma once
@@ -33,18 +36,30 @@ enum Mode { FORWARD, PARTIALS, INPUT_GRAD, WEIGHT_GRAD };
 
 constexpr int PIECE = 4;                                 // k-blocks of a float32 piece
 
+// HELD: the k-blocks of B stay in shared memory for all tiles of a column, only A comes by (100k x 256 -> 1024 forward: 123 -> 106 us).
+enum Shape { ALONE, PAIR, HELD };
 template <typename T> struct Form;
 template <> struct Form<__nv_bfloat16> {
-  static constexpr int BK = 64, STAGES = 4, COLS = 256, SPLITTERS = 0, EPI = 16, A_BYTES = 16384, B_AT = 16384, STAGE = 49152;
+  static constexpr int BK = 64, COLS = 256, SPLITTERS = 0, EPI = 16, A_BYTES = 16384, HELD_BLOCKS = 4;
+  static constexpr int A_STAGE = A_BYTES, B_STAGE = 32768;
 };
-template <> struct Form<float> {                         // A big, A small, B big, B small
-  static constexpr int BK = 32, STAGES = 3, COLS = 128, SPLITTERS = 4, EPI = 8, A_BYTES = 16384, B_AT = 32768, STAGE = 65536;
+template <> struct Form<float> {                         // big and small parts
+  static constexpr int BK = 32, COLS = 128, SPLITTERS = 4, EPI = 8, A_BYTES = 16384, HELD_BLOCKS = 2;
+  static constexpr int A_STAGE = 2 * A_BYTES, B_STAGE = 32768;
 };
 template <typename T> constexpr int threads() { return 32 * (2 + Form<T>::SPLITTERS + Form<T>::EPI); }
-// Results leave by 32 columns: a warp's patch is 32 rows of them.  PARTIALS has a stage less and two patches a warp, so that the next tile's g is on its way.
-template <typename T, int MODE> constexpr int stages() { return Form<T>::STAGES - (MODE == PARTIALS); }
-template <typename T, int MODE> constexpr size_t shared_bytes() {
-  return 1024 + (size_t)stages<T, MODE>() * Form<T>::STAGE + (MODE == PARTIALS ? 2 : 1) * Form<T>::EPI * 1024 * sizeof(T);
+// Results leave by 32 columns: a warp's patch is 32 rows of them; PARTIALS has two, so that the next tile's g is on its way.  What is
+// left of the shared memory are stages: of both operands, of half of B (PAIR), of A alone (HELD).
+template <typename T, int MODE> constexpr int patch_bytes() { return (MODE == PARTIALS ? 2 : 1) * Form<T>::EPI * 1024 * (int)sizeof(T); }
+template <typename T, int SHAPE> constexpr int held_bytes() { return SHAPE == HELD ? Form<T>::HELD_BLOCKS * Form<T>::B_STAGE : 0; }
+template <typename T, int SHAPE> constexpr int stage_bytes() {
+  return Form<T>::A_STAGE + (SHAPE == HELD ? 0 : SHAPE == PAIR ? Form<T>::B_STAGE / 2 : Form<T>::B_STAGE);
+}
+template <typename T, int MODE, int SHAPE> constexpr int stages() {
+  return (231424 - 1024 - patch_bytes<T, MODE>() - held_bytes<T, SHAPE>()) / stage_bytes<T, SHAPE>();
+}
+template <typename T, int MODE, int SHAPE> constexpr size_t shared_bytes() {
+  return 1024 + patch_bytes<T, MODE>() + held_bytes<T, SHAPE>() + (size_t)stages<T, MODE, SHAPE>() * stage_bytes<T, SHAPE>();
 }
 
 struct alignas(64) Launch {
@@ -65,11 +80,12 @@ struct Item {
   int64_t row;
   int col, half, part, kb0, kb1;
 };
-template <int MODE> __device__ __forceinline__ Item item_of(const Launch& p, unsigned i) {
+template <int MODE, int SHAPE> __device__ __forceinline__ Item item_of(const Launch& p, unsigned i) {
+  constexpr int CTAS = SHAPE == PAIR ? 2 : 1;
   Item t{};
   t.col = (int)(i % (unsigned)p.col_tiles) * p.width;
   i /= (unsigned)p.col_tiles;
-  t.row = (int64_t)(MODE == WEIGHT_GRAD ? i % (unsigned)p.row_tiles : i) * TILE_M;
+  t.row = (int64_t)(MODE == WEIGHT_GRAD ? i % (unsigned)p.row_tiles : i) * (CTAS * TILE_M);
   t.kb1 = MODE == INPUT_GRAD ? 2 * p.kblocks : p.kblocks;
   if (MODE == WEIGHT_GRAD) {
     i /= (unsigned)p.row_tiles;
@@ -81,20 +97,25 @@ template <int MODE> __device__ __forceinline__ Item item_of(const Launch& p, uns
   return t;
 }
 
-__device__ __forceinline__ uint32_t idesc_bf16(int n, bool a_rows, bool b_rows) {
+__device__ __forceinline__ uint32_t idesc_bf16(int m, int n, bool a_rows, bool b_rows) {
   return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)a_rows << 15) | ((uint32_t)b_rows << 16) | ((uint32_t)(n >> 3) << 17) |
-         ((uint32_t)(TILE_M >> 4) << 24);
+         ((uint32_t)(m >> 4) << 24);
 }
-// Along the rows (MN-major), 128-byte swizzle: 64 values of M or N a line, eight k a group of 1024 bytes, the next 64 values `BK` lines on.
-__device__ __forceinline__ uint64_t desc_rows(uint32_t at) {
-  return (uint64_t)((at & 0x3FFFF) >> 4) | ((uint64_t)((Form<__nv_bfloat16>::BK * 128) >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
-         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-}
-__device__ __forceinline__ void mma_bf16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate) : "memory");
+// Along the rows (MN-major), 128-byte swizzle: 64 values of M or N a line, eight k a group of 1024 bytes, the next 64 values `BK` lines
+// on.  The low word of the descriptor; the high word is that of tiles along k, UMMA_DESC_HI.
+__device__ __forceinline__ uint32_t lo_rows(uint32_t at) { return ((at & 0x3FFFF) >> 4) | (uint32_t)((Form<__nv_bfloat16>::BK * 128) >> 4) << 16; }
+// One thread issues all MMAs, and what it does between two of them counts: low words stepped by immediates, as for TF32.
+template <bool TWO, bool ACCUMULATE> __device__ __forceinline__ void mma_bf16(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
+  if constexpr (TWO)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tmov.b64 a, {%1, %4};\n\tmov.b64 b, {%2, %4};\n\tsetp.ne.b32 p, %5, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %3, p;\n\t}"
+        ::"r"(d), "r"(a), "r"(b), "r"(idesc), "n"(UMMA_DESC_HI), "n"(ACCUMULATE ? 1 : 0) : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tmov.b64 a, {%1, %4};\n\tmov.b64 b, {%2, %4};\n\tsetp.ne.b32 p, %5, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}"
+        ::"r"(d), "r"(a), "r"(b), "r"(idesc), "n"(UMMA_DESC_HI), "n"(ACCUMULATE ? 1 : 0) : "memory");
 }
 
 // A block of 32 lines of 128 bytes, one warp: float32 to TF32 pairs, the big ones in place, the small ones `small` bytes on.
@@ -211,20 +232,77 @@ template <typename T> __device__ __forceinline__ void line_put(unsigned char* pa
   }
 }
 
-template <typename T, int MODE, int ACT>
+// ---- pairs of CTAs ------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Arrival at the barrier of the same place in the first CTA of the pair.
+__device__ __forceinline__ void bar_arrive_first(uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .b32 at;\n\tmapa.shared::cluster.u32 at, %0, 0;\n\tmbarrier.arrive.release.cluster.shared::cluster.b64 _, [at];\n\t}"
+      ::"r"(s32(bar)) : "memory");
+}
+__device__ __forceinline__ bool bar_try_cluster(uint64_t* b, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok) : "r"(s32(b)), "r"(parity) : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool bar_wait_cluster(uint64_t* b, uint32_t parity, volatile int* abort_flag) {
+  for (int i = 0; i < TC_WAIT_SPINS; ++i) {
+    if (bar_try_cluster(b, parity)) return true;
+    if ((i & 63) == 63) {
+      if (*abort_flag) return false;
+      __nanosleep(128);
+    }
+  }
+  *abort_flag = 1;
+  return false;
+}
+// A copy to this CTA's shared memory whose bytes count at the first CTA's barrier: bit 24 of a shared address is the place in the pair.
+template <bool TWO> __device__ __forceinline__ void copy_2d(void* dst, const CUtensorMap* map, int c0, int c1, uint64_t* bar) {
+  if constexpr (!TWO) {
+    tma_load_2d(dst, map, c0, c1, bar);
+  } else {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+        ::"r"(s32(dst)), "l"(map), "r"(s32(bar) & 0xFEFFFFFFu), "r"(c0), "r"(c1) : "memory");
+  }
+}
+template <bool TWO> __device__ __forceinline__ void commit(uint64_t* bar) {
+  if constexpr (!TWO) {
+    umma_commit(bar);
+  } else {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                 ::"r"(s32(bar)), "h"((uint16_t)3) : "memory");
+  }
+}
+
+template <typename T, int MODE, int ACT, int SHAPE>
 __global__ void __launch_bounds__(threads<T>(), 1) gated_tc_kernel(const __grid_constant__ Launch p) {
   using S = Form<T>;
-  constexpr bool F32 = sizeof(T) == 4, DUAL = MODE == FORWARD || MODE == PARTIALS;
+  constexpr bool F32 = sizeof(T) == 4, TWO = SHAPE == PAIR, DUAL = MODE == FORWARD || MODE == PARTIALS;
   constexpr bool A_TURNED = MODE == WEIGHT_GRAD, B_TURNED = MODE != INPUT_GRAD;      // the operand lies along the rows
   constexpr int LINE = 128 / (int)sizeof(T);                                          // values of a line
-  constexpr int STAGES = stages<T, MODE>();
+  constexpr int STAGES = stages<T, MODE, SHAPE>(), STAGE = stage_bytes<T, SHAPE>();
+  static_assert(STAGES >= 2 && (SHAPE != HELD || DUAL), "two stages at least; B stays for the dual products");
   constexpr int ACC_COLS = F32 ? 2 * S::COLS : S::COLS;                               // of tensor memory: float32 has two sums
+  constexpr int CTAS = TWO ? 2 : 1;
   extern __shared__ unsigned char smem_raw[];
-  __shared__ uint64_t full[STAGES], ready[STAGES], empty[STAGES], acc_full[2], acc_empty[2];
+  __shared__ uint64_t full[STAGES], ready[STAGES], empty[STAGES], acc_full[2], acc_empty[2], held_full, held_ready;
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rank = TWO ? (int)cluster_rank() : 0;
+  const unsigned first_item = blockIdx.x / CTAS, item_step = gridDim.x / CTAS;        // HELD: a multiple of the columns, so a CTA has one
   unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  unsigned char *held = base, *ring = base + held_bytes<T, SHAPE>();
   const int n_mma = DUAL ? 2 * p.width : p.width;                                     // columns of an MMA
   if (tid == 0) {
     abort_flag = 0;
@@ -235,16 +313,24 @@ __global__ void __launch_bounds__(threads<T>(), 1) gated_tc_kernel(const __grid_
     }
     for (int a = 0; a < 2; ++a) {
       bar_init(&acc_full[a], 1);
-      bar_init(&acc_empty[a], S::EPI);
+      bar_init(&acc_empty[a], CTAS * S::EPI);
     }
+    bar_init(&held_full, 1);
+    bar_init(&held_ready, F32 ? S::SPLITTERS : 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s32(&tmem_slot)), "r"(2 * ACC_COLS) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    if constexpr (TWO) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s32(&tmem_slot)), "r"(2 * ACC_COLS) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s32(&tmem_slot)), "r"(2 * ACC_COLS) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
   }
   tc_fence_before();
   __syncthreads();
+  if (TWO) cluster_sync();                              // barriers and tensor memory of both are there
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
   volatile int* ab = &abort_flag;
@@ -255,27 +341,40 @@ __global__ void __launch_bounds__(threads<T>(), 1) gated_tc_kernel(const __grid_
       int s = 0;
       uint32_t ph = 1;
       bool ok = true;
-      const uint32_t bytes = S::A_BYTES + (uint32_t)n_mma * 128;
-      for (unsigned i = blockIdx.x; i < p.items && ok && !*ab; i += gridDim.x) {
-        const Item t = item_of<MODE>(p, i);
+      const uint32_t bytes = CTAS * S::A_BYTES + (SHAPE == HELD ? 0 : (uint32_t)n_mma * 128);
+      if (SHAPE == HELD && first_item < p.items) {
+        const int col = item_of<MODE, SHAPE>(p, first_item).col;
+        bar_expect_tx(&held_full, (uint32_t)(p.kblocks * n_mma) * 128);
+        for (int kb = 0; kb < p.kblocks; ++kb)
+          for (int q = 0; q < 2; ++q)
+            for (int c = 0; c < p.width / LINE; ++c)
+              tma_load_2d(held + kb * S::B_STAGE + (q * (p.width / LINE) + c) * S::BK * 128, &p.b[q], col + c * LINE, kb * S::BK, &held_full);
+      }
+      for (unsigned i = first_item; i < p.items && ok && !*ab; i += item_step) {
+        const Item t = item_of<MODE, SHAPE>(p, i);
+        const int row = (int)t.row + rank * TILE_M;
+        // Columns of B that this CTA copies: all, or its half; of the dual products' pair, one weight's.
+        const int b_cols = TWO && !DUAL ? p.width / 2 : p.width, col = t.col + (TWO && !DUAL ? rank * b_cols : 0);
         for (int kb = t.kb0; kb < t.kb1; ++kb) {
           if (!bar_wait(&empty[s], ph, ab)) { ok = false; break; }
-          unsigned char* st = base + (size_t)s * S::STAGE;
+          unsigned char* st = ring + (size_t)s * STAGE;
           uint64_t* bar = &full[s];
-          bar_expect_tx(bar, bytes);
+          if (rank == 0) bar_expect_tx(bar, bytes);
           const int h = MODE == INPUT_GRAD ? kb >= p.kblocks : t.half, k = (MODE == INPUT_GRAD && h ? kb - p.kblocks : kb) * S::BK;
           if (A_TURNED) {
 #pragma unroll
-            for (int c = 0; c < TILE_M / LINE; ++c) tma_load_2d(st + c * S::BK * 128, &p.a[0], (int)t.row + c * LINE, k, bar);
+            for (int c = 0; c < TILE_M / LINE; ++c) copy_2d<TWO>(st + c * S::BK * 128, &p.a[0], row + c * LINE, k, bar);
           } else {
-            tma_load_2d(st, &p.a[MODE == INPUT_GRAD ? h : 0], k, (int)t.row, bar);
+            copy_2d<TWO>(st, &p.a[MODE == INPUT_GRAD ? h : 0], k, row, bar);
           }
-          unsigned char* sb = st + S::B_AT;
-          if (MODE == INPUT_GRAD) {
-            tma_load_2d(sb, &p.b[h], k, t.col, bar);
+          unsigned char* sb = st + S::A_STAGE;
+          if (SHAPE == HELD) {
+          } else if (MODE == INPUT_GRAD) {
+            copy_2d<TWO>(sb, &p.b[h], k, col, bar);
           } else {
-            for (int q = 0; q < (DUAL ? 2 : 1); ++q)
-              for (int c = 0; c < p.width / LINE; ++c, sb += S::BK * 128) tma_load_2d(sb, &p.b[DUAL ? q : t.half], t.col + c * LINE, k, bar);
+            const int q0 = DUAL ? rank : t.half, q1 = DUAL && !TWO ? 2 : q0 + 1;
+            for (int q = q0; q < q1; ++q)
+              for (int c = 0; c < b_cols / LINE; ++c, sb += S::BK * 128) copy_2d<TWO>(sb, &p.b[q], col + c * LINE, k, bar);
           }
           if (++s == STAGES) s = 0, ph ^= 1;
         }
@@ -283,42 +382,56 @@ __global__ void __launch_bounds__(threads<T>(), 1) gated_tc_kernel(const __grid_
     }
   } else if (warp == 1) {
     // ---------------- MMAs ----------------
-    if (lane == 0) {
+    if (lane == 0 && rank == 0) {
       int s = 0;
       uint32_t ph = 0;
       int piece = 0;
       bool ok = true;
-      const uint32_t idesc = F32 ? umma_idesc_tf32(n_mma) : idesc_bf16(n_mma, A_TURNED, B_TURNED);
-      for (unsigned i = blockIdx.x; i < p.items && ok && !*ab; i += gridDim.x) {
-        const Item t = item_of<MODE>(p, i);
+      const uint32_t idesc = F32 ? umma_idesc_tf32(n_mma) : idesc_bf16(CTAS * TILE_M, n_mma, A_TURNED, B_TURNED);
+      if (SHAPE == HELD) {
+        ok = bar_wait(F32 ? &held_ready : &held_full, 0, ab);
+        tc_fence_after();
+      }
+      for (unsigned i = first_item; i < p.items && ok && !*ab; i += item_step) {
+        const Item t = item_of<MODE, SHAPE>(p, i);
         for (int k0 = t.kb0; k0 < t.kb1 && ok; ++piece) {
           const int k1 = F32 ? min(k0 + PIECE, t.kb1) : t.kb1, a = piece & 1;
-          if (!bar_wait(&acc_empty[a], (uint32_t)(((piece >> 1) & 1) ^ 1), ab)) { ok = false; break; }
+          const uint32_t parity = (uint32_t)(((piece >> 1) & 1) ^ 1);
+          if (!(TWO ? bar_wait_cluster(&acc_empty[a], parity, ab) : bar_wait(&acc_empty[a], parity, ab))) { ok = false; break; }
           tc_fence_after();
           const uint32_t d = tmem + (uint32_t)(a * ACC_COLS);
           for (int kb = k0; kb < k1; ++kb) {
-            if (!bar_wait(F32 ? &ready[s] : &full[s], ph, ab)) { ok = false; break; }
+            if (!(TWO ? bar_wait_cluster(&full[s], ph, ab) : bar_wait(F32 ? &ready[s] : &full[s], ph, ab))) { ok = false; break; }
             tc_fence_after();
-            const uint32_t at = s32(base + (size_t)s * S::STAGE), bt = at + S::B_AT;
-            if (F32) {
+            const uint32_t at = s32(ring + (size_t)s * STAGE), bt = SHAPE == HELD ? s32(held + kb * S::B_STAGE) : at + S::A_STAGE;
+            if constexpr (F32) {
+              const uint32_t ah = umma_lo(at), al = ah + S::A_BYTES / 16, bh = umma_lo(bt), bl = bh + S::COLS * 8;
+              if (kb == k0) {
+                umma_tf32_lo<false>(d, ah, bh, idesc);
+                umma_tf32_lo<false>(d + S::COLS, al, bh, idesc);
+              } else {
+                umma_tf32_lo<true>(d, ah, bh, idesc);
+                umma_tf32_lo<true>(d + S::COLS, al, bh, idesc);
+              }
+              umma_tf32_lo<true>(d + S::COLS, ah, bl, idesc);
 #pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                const uint64_t ah = umma_desc(at + q * 32), al = umma_desc(at + S::A_BYTES + q * 32);
-                const uint64_t bh = umma_desc(bt + q * 32), bl = umma_desc(bt + S::COLS * 128 + q * 32);
-                umma_tf32(d, ah, bh, idesc, kb != k0 || q);
-                umma_tf32(d + S::COLS, al, bh, idesc, kb != k0 || q);
-                umma_tf32(d + S::COLS, ah, bl, idesc, 1);
+              for (int q = 1; q < 4; ++q) {
+                umma_tf32_lo<true>(d, ah + q * 2, bh + q * 2, idesc);
+                umma_tf32_lo<true>(d + S::COLS, al + q * 2, bh + q * 2, idesc);
+                umma_tf32_lo<true>(d + S::COLS, ah + q * 2, bl + q * 2, idesc);
               }
             } else {
+              constexpr int A_STEP = A_TURNED ? 128 : 2, B_STEP = B_TURNED ? 128 : 2;                // 16 of k, in 16 bytes
+              const uint32_t a_lo = A_TURNED ? lo_rows(at) : umma_lo(at), b_lo = B_TURNED ? lo_rows(bt) : umma_lo(bt);
+              if (kb == k0) mma_bf16<TWO, false>(d, a_lo, b_lo, idesc);
+              else mma_bf16<TWO, true>(d, a_lo, b_lo, idesc);
 #pragma unroll
-              for (int q = 0; q < 4; ++q)
-                mma_bf16(d, A_TURNED ? desc_rows(at + q * 2048) : umma_desc(at + q * 32), B_TURNED ? desc_rows(bt + q * 2048) : umma_desc(bt + q * 32),
-                         idesc, kb != k0 || q);
+              for (int q = 1; q < 4; ++q) mma_bf16<TWO, true>(d, a_lo + q * A_STEP, b_lo + q * B_STEP, idesc);
             }
-            umma_commit(&empty[s]);
+            commit<TWO>(&empty[s]);
             if (++s == STAGES) s = 0, ph ^= 1;
           }
-          if (ok) umma_commit(&acc_full[a]);
+          if (ok) commit<TWO>(&acc_full[a]);
           k0 = k1;
         }
       }
@@ -329,13 +442,21 @@ __global__ void __launch_bounds__(threads<T>(), 1) gated_tc_kernel(const __grid_
     uint32_t ph = 0;
     bool ok = true;
     const int w = warp - 2;
-    for (unsigned i = blockIdx.x; i < p.items && ok && !*ab; i += gridDim.x) {
-      const Item t = item_of<MODE>(p, i);
+    if (SHAPE == HELD && first_item < p.items) {
+      ok = bar_wait(&held_full, 0, ab);
+      for (int b = w; b < p.kblocks * (n_mma / 32) && ok; b += S::SPLITTERS)
+        split_block(held + b / (n_mma / 32) * S::B_STAGE + b % (n_mma / 32) * 4096, S::COLS * 128, B_TURNED, lane);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) bar_arrive(&held_ready);
+    }
+    for (unsigned i = first_item; i < p.items && ok && !*ab; i += item_step) {
+      const Item t = item_of<MODE, SHAPE>(p, i);
       for (int kb = t.kb0; kb < t.kb1; ++kb) {
         if (!bar_wait(&full[s], ph, ab)) { ok = false; break; }
-        unsigned char* st = base + (size_t)s * S::STAGE;
+        unsigned char* st = ring + (size_t)s * STAGE;
         split_block(st + w * 4096, S::A_BYTES, A_TURNED, lane);
-        for (int b = w; b < n_mma / 32; b += S::SPLITTERS) split_block(st + S::B_AT + b * 4096, S::COLS * 128, B_TURNED, lane);
+        for (int b = w; b < n_mma / 32 && SHAPE != HELD; b += S::SPLITTERS) split_block(st + S::A_STAGE + b * 4096, S::COLS * 128, B_TURNED, lane);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) bar_arrive(&ready[s]);
@@ -345,35 +466,31 @@ __global__ void __launch_bounds__(threads<T>(), 1) gated_tc_kernel(const __grid_
   } else {
     // ---------------- epilogue ----------------
     // Warps of the same quarter of the lanes share a tile's columns, 32 at a time in turn; of the dual products, 32 of each half.
-    constexpr int SHARES = S::EPI / 4, GROUP = 16 / (int)sizeof(T);
+    constexpr int SHARES = S::EPI / 4, GROUP = 16 / (int)sizeof(T), TURNS = S::COLS / (DUAL ? 64 : 32) / SHARES;
     const int e = warp - 2 - S::SPLITTERS, quarter = warp & 3, share = e >> 2;
-    unsigned char* patch = base + (size_t)STAGES * S::STAGE + (size_t)e * 1024 * sizeof(T);
+    unsigned char* patch = ring + (size_t)STAGES * STAGE + (size_t)e * 1024 * sizeof(T);
     unsigned char* other = patch + S::EPI * 1024 * sizeof(T);                         // PARTIALS
     const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
     const int64_t pitch = p.out_pitch * (int)sizeof(T);
     int piece = 0;
     bool ok = true;
-    // PARTIALS: g of a tile, asked for a tile before it is used (a share has at most one turn of 32 columns there)
-    auto fetch = [&](unsigned item, unsigned char* where) {
-      const Item x = item_of<MODE>(p, item);
-      const int64_t r = x.row + quarter * 32;
-      const int c = x.col + share * 32, here = (int)max((int64_t)0, min((int64_t)32, p.rows - r));
-      const int valid = share * 32 < p.width ? max(0, min(32, p.cols - c)) : 0;
-      patch_in<T>(where, reinterpret_cast<const unsigned char*>(static_cast<const T*>(p.g) + (here > 0 && valid > 0 ? r * p.out_pitch + c : 0)), pitch,
-                  here, valid / GROUP, lane);
-    };
-    if (MODE == PARTIALS) {
-      if (blockIdx.x < p.items) fetch(blockIdx.x, patch);
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    }
-    for (unsigned i = blockIdx.x; i < p.items && ok && !*ab; i += gridDim.x) {
-      const Item t = item_of<MODE>(p, i);
-      const int64_t row = t.row + quarter * 32;
-      const int lines = (int)max((int64_t)0, min((int64_t)32, p.rows - row));
-      if (MODE == PARTIALS) {
-        if (i + gridDim.x < p.items) fetch(i + gridDim.x, other);
-        asm volatile("cp.async.commit_group;" ::: "memory");
+    // PARTIALS: g of a turn, asked for a turn before it is used
+    auto fetch = [&](unsigned item, int turn, unsigned char* where) {
+      if (item < p.items) {
+        const Item x = item_of<MODE, SHAPE>(p, item);
+        const int64_t r = x.row + rank * TILE_M + quarter * 32;
+        const int c0 = (share + turn * SHARES) * 32, c = x.col + c0, here = (int)max((int64_t)0, min((int64_t)32, p.rows - r));
+        const int valid = c0 < p.width ? max(0, min(32, p.cols - c)) : 0;
+        patch_in<T>(where, reinterpret_cast<const unsigned char*>(static_cast<const T*>(p.g) + (here > 0 && valid > 0 ? r * p.out_pitch + c : 0)), pitch,
+                    here, valid / GROUP, lane);
       }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    if (MODE == PARTIALS) fetch(first_item, 0, patch);
+    for (unsigned i = first_item; i < p.items && ok && !*ab; i += item_step) {
+      const Item t = item_of<MODE, SHAPE>(p, i);
+      const int64_t row = t.row + rank * TILE_M + quarter * 32;
+      const int lines = (int)max((int64_t)0, min((int64_t)32, p.rows - row));
       // float32 sums come in pieces and gather in registers: the share's two turns, or its turn of each half
       float sum[F32 ? 2 : 1][32];
       uint32_t d = 0;
@@ -406,16 +523,20 @@ __global__ void __launch_bounds__(threads<T>(), 1) gated_tc_kernel(const __grid_
       }
       if (!ok) break;
 #pragma unroll
-      for (int turn = 0; turn < 2; ++turn) {
+      for (int turn = 0; turn < TURNS; ++turn) {
         const int c0 = (share + turn * SHARES) * 32;
-        if (c0 >= p.width || (DUAL && turn)) break;
+        if (c0 >= p.width) break;
+        if (MODE == PARTIALS) {
+          if (turn + 1 < TURNS && c0 + SHARES * 32 < p.width) fetch(i, turn + 1, other);
+          else fetch(i + item_step, 0, other);
+        }
         const int col = t.col + c0, valid = max(0, min(32, p.cols - col));            // columns of this turn in the results
         const int64_t at = row * p.out_pitch + col;
         if (!DUAL) {
           float v[32];
           if constexpr (F32) {
 #pragma unroll
-            for (int c = 0; c < 32; ++c) v[c] = sum[turn][c];
+            for (int c = 0; c < 32; ++c) v[c] = sum[F32 ? turn : 0][c];
           } else {
             tmem_ld32(d + c0, v);
           }
@@ -457,23 +578,31 @@ __global__ void __launch_bounds__(threads<T>(), 1) gated_tc_kernel(const __grid_
             float x[GROUP], y[GROUP], g[GROUP];
             if (MODE == PARTIALS) from16<T>(*at16, g);
 #pragma unroll
-            for (int c = 0; c < GROUP; ++c) {
+            for (int c = 0; c < GROUP; c += 2) {
               const int j = q * GROUP + c;
-              float ai, ui;
-              if constexpr (F32) {
-                ai = sum[0][b * 16 + j];
-                ui = sum[1][b * 16 + j];
-              } else {
-                ai = __uint_as_float(a[j]);
-                ui = __uint_as_float(u[j]);
+              float ai[2], ui[2];
+              Value<float> v[2];
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                if constexpr (F32) {
+                  ai[h] = sum[0][b * 16 + j + h];
+                  ui[h] = sum[1][b * 16 + j + h];
+                } else {
+                  ai[h] = __uint_as_float(a[j + h]);
+                  ui[h] = __uint_as_float(u[j + h]);
+                }
               }
-              const Value<float> v = activate(ai, ACT);
-              if (MODE == FORWARD) {
-                x[c] = v.y * ui;
-              } else {
-                x[c] = g[c] * ui * v.dy;
-                y[c] = g[c] * v.y;
-                if (F32) sum[F32 ? 1 : 0][b * 16 + j] = y[c];
+              v[0] = activate(ai[0], ACT);
+              v[1] = activate(ai[1], ACT);
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                if (MODE == FORWARD) {
+                  x[c + h] = v[h].y * ui[h];
+                } else {
+                  x[c + h] = g[c + h] * ui[h] * v[h].dy;
+                  y[c + h] = g[c + h] * v[h].y;
+                  if (F32) sum[F32 ? 1 : 0][b * 16 + j + h] = y[c + h];
+                }
               }
             }
             *at16 = to16<T>(x);
@@ -489,17 +618,18 @@ __global__ void __launch_bounds__(threads<T>(), 1) gated_tc_kernel(const __grid_
             for (int c = 0; c < 4; ++c) *patch_at<T>(patch, lane, c) = second[c];
           }
           patch_out<T>(patch, reinterpret_cast<unsigned char*>(static_cast<T*>(p.out2) + at), pitch, lines, valid / GROUP, lane);
+          unsigned char* t0 = patch;
+          patch = other;
+          other = t0;
         }
       }
       if (!F32) {
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) bar_arrive(&acc_empty[(piece - 1) & 1]);
-      }
-      if (MODE == PARTIALS) {
-        unsigned char* t0 = patch;
-        patch = other;
-        other = t0;
+        if (lane == 0) {
+          if (TWO && rank) bar_arrive_first(&acc_empty[(piece - 1) & 1]);
+          else bar_arrive(&acc_empty[(piece - 1) & 1]);
+        }
       }
     }
     if (MODE == PARTIALS) asm volatile("cp.async.wait_all;" ::: "memory");
@@ -507,14 +637,19 @@ __global__ void __launch_bounds__(threads<T>(), 1) gated_tc_kernel(const __grid_
 
   tc_fence_before();
   __syncthreads();
-  if (warp == 1) {
-    __syncwarp();
-    tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * ACC_COLS) : "memory");
-  }
   if (tid == 0 && abort_flag) {
     atomicExch(p.status, 2);
     let_copies_land(full, STAGES);
+  }
+  __syncthreads();
+  if (TWO) cluster_sync();                              // nothing of the other CTA reaches this one's memory any more
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    if constexpr (TWO)
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * ACC_COLS) : "memory");
+    else
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * ACC_COLS) : "memory");
   }
 }
 
@@ -536,17 +671,19 @@ int map_of(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int l
 
 // Columns a tile: as few tiles as `most` allows, of one width, a multiple of the columns of a line.  Narrower ones where that leaves
 // SMs idle: a small call is bound by how long one tile takes.
-int width_of(int cols, int most, int line, int64_t others) {
+int width_of(int cols, int most, int line, bool narrow, int64_t others) {
   int width;
   for (;; most /= 2) {
     const int tiles = (int)ceil_div(cols, most);
     width = (int)ceil_div(ceil_div(cols, tiles), line) * line;
-    if (others * ceil_div(cols, width) * 2 > tc::sm_count() || most / 2 < line) return width;
+    if (!narrow || others * ceil_div(cols, width) * 2 > tc::sm_count() || most / 2 < line) return width;
   }
 }
 
-template <typename T, int MODE, int ACT = EQT_ACT_SILU> int launch(const GatedArgs& a, cudaStream_t s) {
+template <typename T, int MODE, int SHAPE, int ACT> int launch_form(const GatedArgs& a, cudaStream_t s) {
   using S = Form<T>;
+  constexpr bool TWO = SHAPE == PAIR;
+  constexpr int ROWS = TWO ? 2 * TILE_M : TILE_M;       // of a tile
   constexpr int LINE = 128 / (int)sizeof(T);
   constexpr bool DUAL = MODE == FORWARD || MODE == PARTIALS, F32 = sizeof(T) == 4;
   const size_t size = sizeof(T);
@@ -559,7 +696,7 @@ template <typename T, int MODE, int ACT = EQT_ACT_SILU> int launch(const GatedAr
   // need no swizzle.
   if (DUAL) {
     p.cols = a.f, p.rows = a.n, p.kblocks = (int)ceil_div(a.c, S::BK);
-    p.width = width_of(a.f, S::COLS / 2, LINE, ceil_div(a.n, TILE_M));
+    p.width = width_of(a.f, S::COLS / 2, LINE, !TWO, ceil_div(a.n, ROWS));
     rc = map_of<T>(&p.a[0], a.x, a.n, a.c, LINE, TILE_M, true);
     if (!rc) rc = map_of<T>(&p.b[0], w, a.c, a.f, LINE, S::BK, !F32);
     if (!rc) rc = map_of<T>(&p.b[1], w1, a.c, a.f, LINE, S::BK, !F32);
@@ -568,15 +705,15 @@ template <typename T, int MODE, int ACT = EQT_ACT_SILU> int launch(const GatedAr
     p.g = a.g;
   } else if (MODE == INPUT_GRAD) {
     p.cols = a.c, p.rows = a.n, p.kblocks = (int)ceil_div(a.f, S::BK);
-    p.width = width_of(a.c, S::COLS, LINE, ceil_div(a.n, TILE_M));
+    p.width = width_of(a.c, S::COLS, LINE, !TWO, ceil_div(a.n, ROWS));
     rc = map_of<T>(&p.a[0], d, a.n, a.f, LINE, TILE_M, true);
     if (!rc) rc = map_of<T>(&p.a[1], d1, a.n, a.f, LINE, TILE_M, true);
-    if (!rc) rc = map_of<T>(&p.b[0], w, a.c, a.f, LINE, p.width, true);
-    if (!rc) rc = map_of<T>(&p.b[1], w1, a.c, a.f, LINE, p.width, true);
+    if (!rc) rc = map_of<T>(&p.b[0], w, a.c, a.f, LINE, TWO ? p.width / 2 : p.width, true);
+    if (!rc) rc = map_of<T>(&p.b[1], w1, a.c, a.f, LINE, TWO ? p.width / 2 : p.width, true);
     p.out = a.dx;
   } else {
     p.cols = a.f, p.rows = a.c, p.kblocks = (int)ceil_div(a.n, S::BK);
-    p.width = width_of(a.f, S::COLS, LINE, 2 * a.splits * ceil_div(a.c, TILE_M));
+    p.width = width_of(a.f, S::COLS, TWO ? 2 * LINE : LINE, !TWO, 2 * a.splits * ceil_div(a.c, ROWS));    // a pair halves it
     p.split_blocks = (int)(a.split_rows / S::BK);
     p.part = (int64_t)a.c * a.f;
     rc = map_of<T>(&p.a[0], a.x, a.n, a.c, LINE, S::BK, !F32);
@@ -586,16 +723,49 @@ template <typename T, int MODE, int ACT = EQT_ACT_SILU> int launch(const GatedAr
   }
   if (rc) return rc;
   p.out_pitch = p.cols;
-  p.row_tiles = (int)ceil_div(p.rows, TILE_M);
+  p.row_tiles = (int)ceil_div(p.rows, ROWS);
   p.col_tiles = (int)ceil_div(p.cols, p.width);
   const int64_t items = (int64_t)p.row_tiles * p.col_tiles * (MODE == WEIGHT_GRAD ? 2 * a.splits : 1);
   if (items > INT32_MAX / 2) return fail(EQT_ERR_UNSUPPORTED, "gated: %lld tiles are more than one launch takes", (long long)items);
   p.items = (unsigned)items;
   p.status = a.status;
-  if (int r = allow_shared(gated_tc_kernel<T, MODE, ACT>, shared_bytes<T, MODE>())) return r;
-  const unsigned grid = (unsigned)std::min<int64_t>(items, tc::sm_count());
-  gated_tc_kernel<T, MODE, ACT><<<grid, threads<T>(), shared_bytes<T, MODE>(), s>>>(p);
+  const size_t shared = shared_bytes<T, MODE, SHAPE>();
+  auto kernel = gated_tc_kernel<T, MODE, ACT, SHAPE>;
+  if (int r = allow_shared(kernel, shared)) return r;
+  constexpr int CTAS = TWO ? 2 : 1;
+  cudaLaunchConfig_t config{};
+  int64_t at_once = std::min<int64_t>(items, tc::sm_count() / CTAS);
+  if (SHAPE == HELD) at_once = std::min<int64_t>(items, tc::sm_count() / p.col_tiles * p.col_tiles);
+  config.gridDim = dim3((unsigned)(at_once * CTAS));
+  config.blockDim = dim3(threads<T>());
+  config.dynamicSmemBytes = shared;
+  config.stream = s;
+  cudaLaunchAttribute cluster{};
+  cluster.id = cudaLaunchAttributeClusterDimension;
+  cluster.val.clusterDim.x = CTAS;
+  cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+  config.attrs = &cluster;
+  config.numAttrs = TWO ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&config, kernel, p);
+  if (e != cudaSuccess) return fail(EQT_ERR_CUDA, "gated_tc: %s", cudaGetErrorString(e));
   return check_launch("gated_tc");
+}
+
+// HELD where B's k-blocks fit and the columns' tiles divide the SMs with little left over; pairs of CTAs from the size on that gives most
+// SMs a tile of 256 rows, below it tiles of 128 rows fill more of them.
+template <typename T, int MODE, int ACT = EQT_ACT_SILU> int launch(const GatedArgs& a, cudaStream_t s) {
+  constexpr bool DUAL = MODE == FORWARD || MODE == PARTIALS;
+  if constexpr (MODE == FORWARD) {
+    const int64_t columns = ceil_div(a.f, Form<T>::COLS / 2), sms = tc::sm_count();
+    if (a.c <= Form<T>::BK * Form<T>::HELD_BLOCKS && sms / columns * columns * 10 >= sms * 9 && ceil_div(a.n, TILE_M) * columns >= 2 * sms)
+      return launch_form<T, MODE, HELD, ACT>(a, s);
+  }
+  if constexpr (sizeof(T) == 2) {
+    const int64_t rows = MODE == WEIGHT_GRAD ? a.c : a.n, cols = MODE == INPUT_GRAD ? a.c : a.f;
+    const int64_t tiles = ceil_div(rows, 256) * ceil_div(cols, DUAL ? 128 : 256) * (MODE == WEIGHT_GRAD ? 2 * a.splits : 1);
+    if (rows > TILE_M && tiles * 5 >= tc::sm_count() * 2 && (!DUAL || a.c >= 512)) return launch_form<T, MODE, PAIR, ACT>(a, s);
+  }
+  return launch_form<T, MODE, ALONE, ACT>(a, s);
 }
 
 template <typename T, int MODE> int launch_dual(const GatedArgs& a, cudaStream_t s) {
