@@ -66,9 +66,8 @@ int fill(const eqt_attention_args* a, AttentionParams& p, bool backward) {
   p.q = {a->q, a->q_node, a->q_comp};
   p.k = {a->k, a->k_node, a->k_comp};
   p.v = {a->v, a->v_node, a->v_comp};
-  p.out = {a->out, a->comps * channels, channels};
   p.g = {a->grad_out, a->comps * channels, channels};
-  p.out_w = a->out;
+  p.out = a->out;
   p.dq = a->dq;
   p.dk = a->dk;
   p.dv = a->dv;

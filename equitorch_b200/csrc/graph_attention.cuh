@@ -36,8 +36,8 @@ struct Operand {
 };
 
 struct AttentionParams {
-  Operand q, k, v, out, g;
-  void *out_w, *dq, *dk, *dv;
+  Operand q, k, v, g;
+  void *out, *dq, *dk, *dv;
   float *lse, *delta;        // [head][node]; lse in units of log2
   float4 *geo_row, *geo_col; // [head][node]: (sum dS r, sum dS u) by rows; (0, sum dS u) by columns
   const int4* tiles;         // first row, first and one past the last node of its graph
@@ -99,13 +99,18 @@ __device__ __forceinline__ void score_mma(float (&acc)[NT][4], const __nv_bfloat
     }
   }
 }
+// The tensor cores' adder truncates, so the products with small parts have a sum of their own: one truncation for eight terms.
 template <int DP, int NT>
 __device__ __forceinline__ void score_mma(float (&acc)[NT][4], const float* a, const float* b, int lane) {
   constexpr int LD = Row<float, DP>::LD;
   const int g = lane >> 2, t = lane & 3;
   const float *ap = a + g * LD + t, *bp = b + g * LD + t;
+  float fine[NT][4];
 #pragma unroll
-  for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+  for (int n = 0; n < NT; ++n) {
+    acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+    fine[n][0] = fine[n][1] = fine[n][2] = fine[n][3] = 0.f;
+  }
 #pragma unroll 4
   for (int ks = 0; ks < DP / 8; ++ks) {
     float hi[4], lo[4];
@@ -118,11 +123,15 @@ __device__ __forceinline__ void score_mma(float (&acc)[NT][4], const float* a, c
       float h0, l0, h1, l1;
       tc::split_tf32(bp[n * 8 * LD + ks * 8], h0, l0);
       tc::split_tf32(bp[n * 8 * LD + ks * 8 + 4], h1, l1);
-      mma_tf32(acc[n], lo, h0, h1);
-      mma_tf32(acc[n], hi, l0, l1);
       mma_tf32(acc[n], hi, h0, h1);
+      mma_tf32(fine[n], lo, h0, h1);
+      mma_tf32(fine[n], hi, l0, l1);
     }
   }
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[n][i] += fine[n][i];
 }
 
 // o[16 rows][DP] += p[16][8 NT] X[8 NT][DP], p in the layout that score_mma leaves
@@ -160,23 +169,26 @@ __device__ __forceinline__ void out_mma(float (&o)[DP / 8][4], const float (&p)[
     tc::split_tf32(p[j][3], hi[j][3], lo[j][3]);
   }
 #pragma unroll
-  for (int d = 0; d < DP / 8; d += 4) {
-    float s[4][4];
+  for (int d = 0; d < DP / 8; d += 2) {
+    float s[2][4], h[2][NT][2];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) s[e][0] = s[e][1] = s[e][2] = s[e][3] = 0.f;
+    for (int e = 0; e < 2; ++e) s[e][0] = s[e][1] = s[e][2] = s[e][3] = 0.f;
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float h0, l0, h1, l1;
-        tc::split_tf32(xp[j * 8 * LD + (d + e) * 8], h0, l0);
-        tc::split_tf32(xp[j * 8 * LD + LD + (d + e) * 8], h1, l1);
-        mma_tf32(s[e], lo[j], h0, h1);
+      for (int e = 0; e < 2; ++e) {
+        float l0, l1;
+        tc::split_tf32(xp[j * 8 * LD + (d + e) * 8], h[e][j][0], l0);
+        tc::split_tf32(xp[j * 8 * LD + LD + (d + e) * 8], h[e][j][1], l1);
+        mma_tf32(s[e], lo[j], h[e][j][0], h[e][j][1]);
         mma_tf32(s[e], hi[j], l0, l1);
-        mma_tf32(s[e], hi[j], h0, h1);
       }
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
+    for (int j = 0; j < NT; ++j)                         // large products last: truncations before them are of small sums
+#pragma unroll
+      for (int e = 0; e < 2; ++e) mma_tf32(s[e], hi[j], h[e][j][0], h[e][j][1]);
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
 #pragma unroll
       for (int i = 0; i < 4; ++i) o[d + e][i] += s[e][i];
   }
@@ -193,13 +205,89 @@ __device__ __forceinline__ float rsqrt_fast(float x) {
   asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// tanh to some 1e-7 absolute, which is what a score needs: (e - 1) / (e + 1), e = exp(2 x), kept finite.
-// float32 scores take the function of the library, which keeps small values to the last bit.
-template <typename T> __device__ __forceinline__ float tanh_of(float x) {
-  const float e = exp2_fast(fminf(x * (2.f * LOG2E), 64.f));
-  return __fdividef(e - 1.f, e + 1.f);
+// Two float32 values an instruction: what the warps issue is the bound beside the special functions, and packed arithmetic is half of it.
+using pair = unsigned long long;
+__device__ __forceinline__ pair both(float x, float y) {
+  pair r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
 }
-template <> __device__ __forceinline__ float tanh_of<float>(float x) { return tanhf(x); }
+__device__ __forceinline__ void parts(pair v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ pair add2(pair a, pair b) {
+  pair r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ pair mul2(pair a, pair b) {
+  pair r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ pair fma2(pair a, pair b, pair c) {
+  pair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// From products to scores without the distance, in units of log2: unit z, or unit tanh(z to_cap).  tanh is up to a half an odd polynomial
+// (fitted for the least relative error, 7.4e-8 in float32 arithmetic), above it 1 - 2 / (e^2x + 1).  Scores mostly stay below half the
+// cap, and a warp whose tile does so needs no special function for them.
+__device__ __forceinline__ float tanh_any(float x) {
+  const float y = fabsf(x), w = x * x, large = copysignf(1.f - __fdividef(2.f, exp2_fast(fminf(y * (2.f * LOG2E), 64.f)) + 1.f), x);
+  const float small = fmaf(x, w * fmaf(w, fmaf(w, fmaf(w, 0.01724148727953434f, -0.05304549261927605f), 0.13325878977775574f), -0.333331435918808f), x);
+  return y <= 0.5f ? small : x == x ? large : x;
+}
+template <int NT> __device__ __forceinline__ void cap_tile(float (&z)[NT][4], float unit, float to_cap) {
+  if (to_cap == 0.f) {
+    const pair u = both(unit, unit);
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) parts(mul2(both(z[n][2 * r], z[n][2 * r + 1]), u), z[n][2 * r], z[n][2 * r + 1]);
+    return;
+  }
+  float most = 0.f;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) most = fmaxf(fmaxf(most, fmaxf(fabsf(z[n][0]), fabsf(z[n][1]))), fmaxf(fabsf(z[n][2]), fabsf(z[n][3])));
+  if (__all_sync(0xffffffffu, most * to_cap <= 0.5f)) {  // the maximum drops NaNs; they stay NaN either way
+    const float f = to_cap * to_cap;                     // the polynomial's argument is (z to_cap)^2
+    const float c0 = -0.333331435918808f * f, c1 = 0.13325878977775574f * f * f, c2 = -0.05304549261927605f * f * f * f, c3 = 0.01724148727953434f * f * f * f * f;
+    const pair k0 = both(c0, c0), k1 = both(c1, c1), k2 = both(c2, c2), k3 = both(c3, c3), u = both(unit * to_cap, unit * to_cap);
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const pair x = both(z[n][2 * r], z[n][2 * r + 1]), w = mul2(x, x), y = mul2(x, u);
+        parts(fma2(y, mul2(w, fma2(w, fma2(w, fma2(w, k3, k2), k1), k0)), y), z[n][2 * r], z[n][2 * r + 1]);
+      }
+  } else {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) z[n][i] = unit * tanh_any(z[n][i] * to_cap);
+  }
+}
+
+// The way from a row to two columns, one over the distances and the distances.  One over is finite where two nodes coincide, so that
+// the distance comes out as zero, and the way over it too.
+struct Way { pair x, y, z, inverse, length; };
+__device__ __forceinline__ Way way_to(const float* columns, int stride, pair mx, pair my, pair mz) {      // m: minus the row's position
+  Way w;
+  w.x = add2(*reinterpret_cast<const pair*>(columns), mx);
+  w.y = add2(*reinterpret_cast<const pair*>(columns + stride), my);
+  w.z = add2(*reinterpret_cast<const pair*>(columns + 2 * stride), mz);
+  const pair square = fma2(w.z, w.z, fma2(w.y, w.y, mul2(w.x, w.x)));
+  float a, b;
+  parts(square, a, b);
+  w.inverse = both(rsqrt_fast(fmaxf(a, 1e-30f)), rsqrt_fast(fmaxf(b, 1e-30f)));
+  w.length = mul2(square, w.inverse);
+  return w;
+}
+
+__device__ __forceinline__ float quad_sum(float v) {
+  v += __shfl_xor_sync(0xffffffffu, v, 1);
+  return v + __shfl_xor_sync(0xffffffffu, v, 2);
+}
 
 // ---- tiles in shared memory ---------------------------------------------------------------------
 __device__ __forceinline__ void copy16(void* dst, const void* src, bool there) {
@@ -282,22 +370,53 @@ __device__ __forceinline__ void store_rows(T* buf, void* out, const float (&o)[D
   }
 }
 
-// Positions of the rows [first, first + ROWS_TILE), by all threads of the CTA.
-template <int ROWS_TILE>
-__device__ __forceinline__ void load_positions(float4* dst, const float* pos, int first, int end) {
-  for (int i = threadIdx.x; i < ROWS_TILE * 3; i += THREADS) {
-    const int r = i / 3, x = i - r * 3;
-    const bool there = first + r < end;
-    copy4(reinterpret_cast<float*>(dst + r) + x, pos + (int64_t)(there ? first + r : 0) * 3 + x, there);
+// Sum over a head's values of g and the result, for rows g and g + 8 of a warp: four lanes a row.
+template <typename T, int DP>
+__device__ __forceinline__ void row_delta(const T* grads, int first, int end, int head, const AttentionParams& p, int lane, float (&delta)[2]) {
+  constexpr int LD = Row<T, DP>::LD;
+  const int g = lane >> 2, t = lane & 3, d = p.comps * p.size, channels = p.heads * p.size;
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    float sum = 0.f;
+    if (first + g + 8 * r < end) {
+      const T* o = static_cast<const T*>(p.out) + (int64_t)(first + g + 8 * r) * p.comps * channels + (int64_t)head * p.size;
+      const T* a = grads + (g + 8 * r) * LD;
+      constexpr int V = 16 / (int)sizeof(T);
+      for (int j0 = t * V; j0 < d; j0 += 4 * V) {        // the same order of sums with any alignment
+        if (p.vec) {
+          const int m = j0 / p.size;
+          const uint4 raw = *reinterpret_cast<const uint4*>(o + (int64_t)m * channels + j0 - m * p.size);
+          const T* v = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+          for (int i = 0; i < V; ++i) sum += static_cast<float>(a[j0 + i]) * static_cast<float>(v[i]);
+        } else {
+          for (int j = j0; j < min(d, j0 + V); ++j) {
+            const int m = j / p.size;
+            sum += static_cast<float>(a[j]) * static_cast<float>(o[(int64_t)m * channels + j - m * p.size]);
+          }
+        }
+      }
+    }
+    delta[r] = quad_sum(sum);
   }
 }
 
-__device__ __forceinline__ float3 position(const float* pos, int row, int end) {
-  return row < end ? make_float3(pos[(int64_t)row * 3], pos[(int64_t)row * 3 + 1], pos[(int64_t)row * 3 + 2]) : make_float3(0.f, 0.f, 0.f);
+// Positions of the rows [first, first + ROWS_TILE), all x, all y, all z, by all threads of the CTA.
+template <int ROWS_TILE>
+__device__ __forceinline__ void load_positions(float* dst, const float* pos, int first, int end) {
+  for (int i = threadIdx.x; i < ROWS_TILE * 3; i += THREADS) {
+    const int r = i / 3, x = i - r * 3;
+    const bool there = first + r < end;
+    copy4(dst + x * ROWS_TILE + r, pos + (int64_t)(there ? first + r : 0) * 3 + x, there);
+  }
 }
-__device__ __forceinline__ float quad_sum(float v) {
-  v += __shfl_xor_sync(0xffffffffu, v, 1);
-  return v + __shfl_xor_sync(0xffffffffu, v, 2);
+
+// Minus the position of a row, each coordinate twice.
+struct Here { pair x, y, z; };
+__device__ __forceinline__ Here minus_position(const float* pos, int row, int end) {
+  float x = 0.f, y = 0.f, z = 0.f;
+  if (row < end) x = -pos[(int64_t)row * 3], y = -pos[(int64_t)row * 3 + 1], z = -pos[(int64_t)row * 3 + 2];
+  return {both(x, x), both(y, y), both(z, z)};
 }
 __device__ __forceinline__ float quad_max(float v) {
   v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
@@ -314,7 +433,7 @@ template <typename T, int DP, int WR, int KT> struct Shape {
 };
 
 template <typename T, int DP, int WR, int KT>
-__global__ void __launch_bounds__(THREADS) attention_forward_kernel(const __grid_constant__ AttentionParams p) {
+__global__ void __launch_bounds__(THREADS, DP <= 64 ? 4 : 3) attention_forward_kernel(const __grid_constant__ AttentionParams p) {
   using S = Shape<T, DP, WR, KT>;
   constexpr int LD = S::LD, NT = KT / 8;
   extern __shared__ __align__(16) unsigned char smem[];
@@ -325,7 +444,7 @@ __global__ void __launch_bounds__(THREADS) attention_forward_kernel(const __grid
   const int first = tile.x, lo = tile.y, hi = tile.z;
   T* base = reinterpret_cast<T*>(smem) + slot * S::head_elements(1);
   T *rows = base, *stage = base + S::TILE * LD;
-  float4* spos = reinterpret_cast<float4*>(smem + S::bytes(1, 0));       // two tiles of positions
+  float* spos = reinterpret_cast<float*>(smem + S::bytes(1, 0));         // two tiles of positions
   const bool here = head < p.heads;
   const int end = here ? hi : 0;                                         // a place without a head copies nothing
   if (p.comps * p.size < DP) {                                           // the columns behind the head's values stay zero
@@ -336,7 +455,7 @@ __global__ void __launch_bounds__(THREADS) attention_forward_kernel(const __grid
   auto fetch = [&](int key, int s) {
     load_rows<T, DP, S::TH, KT>(stage + s * S::STAGE, p.k, piece, key, end, head, p, ht);
     load_rows<T, DP, S::TH, KT>(stage + s * S::STAGE + KT * LD, p.v, piece, key, end, head, p, ht);
-    if (p.pos) load_positions<KT>(spos + s * KT, p.pos, key, hi);
+    if (p.pos) load_positions<KT>(spos + s * 3 * KT, p.pos, key, hi);
     copies_commit();
   };
   load_rows<T, DP, S::TH, S::TILE>(rows, p.q, piece, first, end, head, p, ht);
@@ -348,13 +467,14 @@ __global__ void __launch_bounds__(THREADS) attention_forward_kernel(const __grid
   float o[DP / 8][4], top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
 #pragma unroll
   for (int n = 0; n < DP / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
-  const float scale2 = p.scale * LOG2E, cap2 = p.cap * LOG2E, to_cap = p.cap > 0.f ? p.scale / p.cap : 0.f;
-  float slope2 = 0.f;
-  float3 p0, p1;
+  const float to_cap = p.cap > 0.f ? p.scale / p.cap : 0.f, unit = (p.cap > 0.f ? p.cap : p.scale) * LOG2E;   // of a score: the tanh, or the product
+  pair slope2 = 0;                                                       // minus the slope, twice, in units of log2
+  Here at[2];
   if (p.pos) {
-    slope2 = here ? p.slope[head] * LOG2E : 0.f;
-    p0 = position(p.pos, row + g, hi);
-    p1 = position(p.pos, row + g + 8, hi);
+    const float f = here ? -p.slope[head] * LOG2E : 0.f;
+    slope2 = both(f, f);
+    at[0] = minus_position(p.pos, row + g, hi);
+    at[1] = minus_position(p.pos, row + g + 8, hi);
   }
   int s = 0;
   for (int key = lo; key < hi; key += KT, s ^= 1) {
@@ -369,27 +489,14 @@ __global__ void __launch_bounds__(THREADS) attention_forward_kernel(const __grid
       const T *ks = stage + s * S::STAGE, *vs = ks + KT * LD;
       float z[NT][4];
       score_mma<DP, NT>(z, mine, ks, lane);
-      if (p.cap > 0.f) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) z[n][i] = cap2 * tanh_of<T>(z[n][i] * to_cap);
-      } else {
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) z[n][i] *= scale2;
-      }
+      cap_tile<NT>(z, unit, to_cap);
       if (p.pos) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const float4 pk = spos[s * KT + n * 8 + 2 * t + i];
-            const float x0 = p0.x - pk.x, y0 = p0.y - pk.y, z0 = p0.z - pk.z, x1 = p1.x - pk.x, y1 = p1.y - pk.y, z1 = p1.z - pk.z;
-            const float d0 = x0 * x0 + y0 * y0 + z0 * z0, d1 = x1 * x1 + y1 * y1 + z1 * z1;
-            z[n][i] -= slope2 * (d0 > 0.f ? d0 * rsqrt_fast(d0) : 0.f);
-            z[n][2 + i] -= slope2 * (d1 > 0.f ? d1 * rsqrt_fast(d1) : 0.f);
+          for (int r = 0; r < 2; ++r) {
+            const Way w = way_to(spos + s * 3 * KT + n * 8 + 2 * t, KT, at[r].x, at[r].y, at[r].z);
+            parts(fma2(w.length, slope2, both(z[n][2 * r], z[n][2 * r + 1])), z[n][2 * r], z[n][2 * r + 1]);
           }
       }
       if (key + KT > hi) {
@@ -399,27 +506,42 @@ __global__ void __launch_bounds__(THREADS) attention_forward_kernel(const __grid
           for (int i = 0; i < 2; ++i)
             if (key + n * 8 + 2 * t + i >= hi) z[n][i] = z[n][2 + i] = -INFINITY;
       }
+      float most[2], keep[2];
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        float m = -INFINITY;
+        float m = top[r];
 #pragma unroll
         for (int n = 0; n < NT; ++n) m = fmaxf(m, fmaxf(z[n][2 * r], z[n][2 * r + 1]));
-        m = fmaxf(quad_max(m), top[r]);
-        const float from = m == -INFINITY ? 0.f : m, keep = exp2_fast(top[r] - from);
-        top[r] = m;
-        float add = 0.f;
+        most[r] = quad_max(m);
+      }
+      if (__any_sync(0xffffffffu, most[0] > top[0] || most[1] > top[1])) {             // the running sums have a new unit
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          keep[r] = exp2_fast(top[r] - (most[r] == -INFINITY ? 0.f : most[r]));
+          sum[r] *= keep[r];
+          top[r] = most[r];
+        }
+#pragma unroll
+        for (int n = 0; n < DP / 8; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[n][i] *= keep[i >> 1];
+      }
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const float from = top[r] == -INFINITY ? 0.f : -top[r];
+        const pair shift = both(from, from);
+        pair add = 0;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          z[n][2 * r] = exp2_fast(z[n][2 * r] - from);
-          z[n][2 * r + 1] = exp2_fast(z[n][2 * r + 1] - from);
-          add += z[n][2 * r] + z[n][2 * r + 1];
+          float x, y;
+          parts(add2(both(z[n][2 * r], z[n][2 * r + 1]), shift), x, y);
+          z[n][2 * r] = exp2_fast(x);
+          z[n][2 * r + 1] = exp2_fast(y);
+          add = add2(add, both(z[n][2 * r], z[n][2 * r + 1]));
         }
-        sum[r] = sum[r] * keep + add;
-#pragma unroll
-        for (int n = 0; n < DP / 8; ++n) {
-          o[n][2 * r] *= keep;
-          o[n][2 * r + 1] *= keep;
-        }
+        float x, y;
+        parts(add, x, y);
+        sum[r] += x + y;
       }
       out_mma<DP, NT>(o, z, vs, lane);
     }
@@ -433,17 +555,17 @@ __global__ void __launch_bounds__(THREADS) attention_forward_kernel(const __grid
     if (row + g < hi) to[0] = top[0] + log2f(sum[0]);
     if (row + g + 8 < hi) to[8] = top[1] + log2f(sum[1]);
   }
-  store_rows<T, DP>(const_cast<T*>(mine), p.out_w, o, 1.f / sum[0], 1.f / sum[1], row, hi, head, p, lane);
+  const float f0 = 1.f / sum[0], f1 = 1.f / sum[1];
+  store_rows<T, DP>(const_cast<T*>(mine), p.out, o, f0, f1, row, hi, head, p, lane);
 }
 
 // Backward by rows: dq, delta, and with positions the rows' sums of dS r and dS u.
-// These sums are float32 results also where the features are bfloat16, so they do not go by the delta of the rounded output: with
-// w = r or u, sum_j dS w = sum_j P dP w - (sum_j P dP) (sum_j P w), and the columns' pass is given sum_j P dP.
+// These sums are float32 results also where the features are bfloat16, so there they do not go by the delta of the rounded weights and
+// result: with w = r or u, sum_j dS w = sum_j P dP w - (sum_j P dP) (sum_j P w), and the columns' pass is given sum_j P dP.
 template <typename T, int DP, int WR, int KT, bool GEO>
 __global__ void __launch_bounds__(THREADS) attention_rows_kernel(const __grid_constant__ AttentionParams p) {
   using S = Shape<T, DP, WR, KT>;
   constexpr int LD = S::LD, NT = KT / 8;
-  static_assert(2 * KT >= S::TILE, "the output's rows fit a stage");
   extern __shared__ __align__(16) unsigned char smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int slot = warp / WR, ht = tid - slot * S::TH;
@@ -452,7 +574,7 @@ __global__ void __launch_bounds__(THREADS) attention_rows_kernel(const __grid_co
   const int first = tile.x, lo = tile.y, hi = tile.z;
   T* base = reinterpret_cast<T*>(smem) + slot * S::head_elements(2);
   T *rows = base, *grads = base + S::TILE * LD, *stage = base + 2 * S::TILE * LD;
-  float4* spos = reinterpret_cast<float4*>(smem + S::bytes(2, 0));
+  float* spos = reinterpret_cast<float*>(smem + S::bytes(2, 0));
   const bool here = head < p.heads;
   const int end = here ? hi : 0;
   if (p.comps * p.size < DP) {
@@ -463,30 +585,21 @@ __global__ void __launch_bounds__(THREADS) attention_rows_kernel(const __grid_co
   auto fetch = [&](int key, int s) {
     load_rows<T, DP, S::TH, KT>(stage + s * S::STAGE, p.k, piece, key, end, head, p, ht);
     load_rows<T, DP, S::TH, KT>(stage + s * S::STAGE + KT * LD, p.v, piece, key, end, head, p, ht);
-    if (p.pos) load_positions<KT>(spos + s * KT, p.pos, key, hi);
+    if (p.pos) load_positions<KT>(spos + s * 3 * KT, p.pos, key, hi);
     copies_commit();
   };
   load_rows<T, DP, S::TH, S::TILE>(rows, p.q, piece, first, end, head, p, ht);
   load_rows<T, DP, S::TH, S::TILE>(grads, p.g, piece, first, end, head, p, ht);
-  load_rows<T, DP, S::TH, S::TILE>(stage + S::STAGE, p.out, piece, first, end, head, p, ht);   // the output, where the second tile will be
+  copies_commit();
   fetch(lo, 0);
-  copies_wait<0>();
+  copies_wait<1>();
   __syncthreads();
 
   const int row = first + (warp % WR) * 16;
   const bool work = here && row < hi;
   const T *mq = rows + (warp % WR) * 16 * LD, *mg = grads + (warp % WR) * 16 * LD;
   float delta[2] = {0.f, 0.f}, lse[2] = {INFINITY, INFINITY};
-  {
-    const T *a = mg + g * LD, *b = stage + S::STAGE + ((warp % WR) * 16 + g) * LD;
-    for (int c = t; c < DP; c += 4) {
-      delta[0] += static_cast<float>(a[c]) * static_cast<float>(b[c]);
-      delta[1] += static_cast<float>(a[8 * LD + c]) * static_cast<float>(b[8 * LD + c]);
-    }
-    delta[0] = quad_sum(delta[0]);
-    delta[1] = quad_sum(delta[1]);
-  }
-  __syncthreads();                                                       // the output has been read
+  if (work) row_delta<T, DP>(mg, row, hi, head, p, lane, delta);
   const bool is[2] = {work && row + g < hi, work && row + g + 8 < hi};
   const int64_t at = (int64_t)head * p.n + row + g;
   if (is[0]) lse[0] = p.lse[at];
@@ -494,18 +607,22 @@ __global__ void __launch_bounds__(THREADS) attention_rows_kernel(const __grid_co
   float dq[DP / 8][4];
 #pragma unroll
   for (int n = 0; n < DP / 8; ++n) dq[n][0] = dq[n][1] = dq[n][2] = dq[n][3] = 0.f;
-  float all[2] = {0.f, 0.f}, pw[2][4], pdw[2][4];                          // sum P dP, sum P w, sum P dP w; w = (r, u)
+  pair geo[2][4], flat[2][4], all[2] = {0, 0};                             // sum dS w, or of P dP w; sum P w; sum P dP; two columns' each
 #pragma unroll
   for (int r = 0; r < 2; ++r)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) pw[r][i] = pdw[r][i] = 0.f;
-  const float scale2 = p.scale * LOG2E, cap2 = p.cap * LOG2E, to_cap = p.cap > 0.f ? p.scale / p.cap : 0.f;
-  float slope2 = 0.f;
-  float3 pr[2];
+    for (int i = 0; i < 4; ++i) geo[r][i] = flat[r][i] = 0;
+  constexpr bool APART = sizeof(T) == 2;
+  const float to_cap = p.cap > 0.f ? p.scale / p.cap : 0.f, unit = (p.cap > 0.f ? p.cap : p.scale) * LOG2E;   // of a score: the tanh, or the product
+  const float bend = p.cap > 0.f ? -p.scale / (unit * unit) : 0.f;         // scale (1 - tanh^2), from unit tanh
+  const pair scale2 = both(p.scale, p.scale), bend2 = both(bend, bend);
+  pair slope2 = 0;
+  Here place[2];
   if (p.pos) {
-    slope2 = here ? p.slope[head] * LOG2E : 0.f;
-    pr[0] = position(p.pos, row + g, hi);
-    pr[1] = position(p.pos, row + g + 8, hi);
+    const float f = here ? -p.slope[head] * LOG2E : 0.f;
+    slope2 = both(f, f);
+    place[0] = minus_position(p.pos, row + g, hi);
+    place[1] = minus_position(p.pos, row + g + 8, hi);
   }
   int s = 0;
   for (int key = lo; key < hi; key += KT, s ^= 1) {
@@ -521,46 +638,41 @@ __global__ void __launch_bounds__(THREADS) attention_rows_kernel(const __grid_co
       float z[NT][4], dp[NT][4];
       score_mma<DP, NT>(z, mq, ks, lane);
       score_mma<DP, NT>(dp, mg, vs, lane);
+      cap_tile<NT>(z, unit, to_cap);
+      const bool last = key + KT > hi;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const float4 pk = p.pos ? spos[s * KT + n * 8 + 2 * t + i] : make_float4(0.f, 0.f, 0.f, 0.f);
-          const bool there = key + n * 8 + 2 * t + i < hi;
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            float& zz = z[n][2 * r + i];
-            float slant = p.scale, score;
-            if (p.cap > 0.f) {
-              const float th = tanh_of<T>(zz * to_cap);
-              score = cap2 * th;
-              slant = p.scale * (1.f - th * th);
-            } else {
-              score = zz * scale2;
-            }
-            float dx, dy, dz, inv = 0.f, dist = 0.f;
-            if (p.pos) {
-              dx = pr[r].x - pk.x, dy = pr[r].y - pk.y, dz = pr[r].z - pk.z;
-              const float d2 = dx * dx + dy * dy + dz * dz;
-              inv = d2 > 0.f ? rsqrt_fast(d2) : 0.f;
-              dist = d2 * inv;
-              score -= slope2 * dist;
-            }
-            const float w = there ? exp2_fast(score - lse[r]) : 0.f, d = dp[n][2 * r + i];
-            if (GEO) {
-              const float wd = w * d, wi = w * inv, wdi = wd * inv;
-              all[r] += wd;
-              pw[r][0] += w * dist;
-              pw[r][1] += wi * dx;
-              pw[r][2] += wi * dy;
-              pw[r][3] += wi * dz;
-              pdw[r][0] += wd * dist;
-              pdw[r][1] += wdi * dx;
-              pdw[r][2] += wdi * dy;
-              pdw[r][3] += wdi * dz;
-            }
-            zz = w * (d - delta[r]) * slant;
+        for (int r = 0; r < 2; ++r) {
+          const pair score0 = both(z[n][2 * r], z[n][2 * r + 1]), d = both(dp[n][2 * r], dp[n][2 * r + 1]);
+          pair score = score0;
+          Way v;
+          if (p.pos) {
+            v = way_to(spos + s * 3 * KT + n * 8 + 2 * t, KT, place[r].x, place[r].y, place[r].z);
+            score = fma2(v.length, slope2, score);
           }
+          float x, y;
+          parts(add2(score, both(-lse[r], -lse[r])), x, y);
+          if (last) {
+            if (key + n * 8 + 2 * t >= hi) x = -INFINITY;
+            if (key + n * 8 + 2 * t + 1 >= hi) y = -INFINITY;
+          }
+          const pair w = both(exp2_fast(x), exp2_fast(y)), e = mul2(w, add2(d, both(-delta[r], -delta[r])));
+          if (GEO) {
+            const pair f = APART ? mul2(w, d) : e, fi = mul2(f, v.inverse), wi = mul2(w, v.inverse);
+            if (APART) {
+              all[r] = add2(all[r], f);
+              flat[r][0] = fma2(w, v.length, flat[r][0]);
+              flat[r][1] = fma2(wi, v.x, flat[r][1]);
+              flat[r][2] = fma2(wi, v.y, flat[r][2]);
+              flat[r][3] = fma2(wi, v.z, flat[r][3]);
+            }
+            geo[r][0] = fma2(f, v.length, geo[r][0]);
+            geo[r][1] = fma2(fi, v.x, geo[r][1]);
+            geo[r][2] = fma2(fi, v.y, geo[r][2]);
+            geo[r][3] = fma2(fi, v.z, geo[r][3]);
+          }
+          parts(mul2(e, fma2(mul2(score0, score0), bend2, scale2)), z[n][2 * r], z[n][2 * r + 1]);
         }
       out_mma<DP, NT>(dq, z, ks, lane);
     }
@@ -570,10 +682,22 @@ __global__ void __launch_bounds__(THREADS) attention_rows_kernel(const __grid_co
   if (GEO) {
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      delta[r] = quad_sum(all[r]);
+      float x, y, sums[4];
+      if (APART) {
+        parts(all[r], x, y);
+        delta[r] = quad_sum(x + y);
+      }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) pdw[r][i] = quad_sum(pdw[r][i]) - delta[r] * quad_sum(pw[r][i]);
-      if (is[r] && t == 0) p.geo_row[at + 8 * r] = make_float4(pdw[r][0], pdw[r][1], pdw[r][2], pdw[r][3]);
+      for (int i = 0; i < 4; ++i) {
+        parts(geo[r][i], x, y);
+        sums[i] = quad_sum(x + y);
+        if (APART) {
+          parts(flat[r][i], x, y);
+          sums[i] -= delta[r] * quad_sum(x + y);
+        }
+      }
+      const float4 v = make_float4(sums[0], -sums[1], -sums[2], -sums[3]);   // u points from the column to the row
+      if (is[r] && t == 0) p.geo_row[at + 8 * r] = v;
     }
   }
   if (t == 0) {
@@ -597,8 +721,8 @@ __global__ void __launch_bounds__(THREADS) attention_columns_kernel(const __grid
   const int first = tile.x, lo = tile.y, hi = tile.z;
   T* base = reinterpret_cast<T*>(smem) + slot * S::head_elements(2);
   T *keys = base, *values = base + S::TILE * LD, *stage = base + 2 * S::TILE * LD;
-  float4* spos = reinterpret_cast<float4*>(smem + S::bytes(2, 0));
-  float* stats = reinterpret_cast<float*>(spos + 2 * KT) + slot * 4 * KT;           // [tile][lse, delta][KT]
+  float* spos = reinterpret_cast<float*>(smem + S::bytes(2, 0));
+  float* stats = spos + 6 * KT + slot * 4 * KT;           // [tile][lse, delta][KT]
   const bool here = head < p.heads;
   const int end = here ? hi : 0;
   if (p.comps * p.size < DP) {
@@ -615,7 +739,7 @@ __global__ void __launch_bounds__(THREADS) attention_columns_kernel(const __grid
       copy4(stats + (2 * s) * KT + i, p.lse + at, there);
       copy4(stats + (2 * s + 1) * KT + i, p.delta + at, there);
     }
-    if (p.pos) load_positions<KT>(spos + s * KT, p.pos, query, hi);
+    if (p.pos) load_positions<KT>(spos + s * 3 * KT, p.pos, query, hi);
     copies_commit();
   };
   load_rows<T, DP, S::TH, S::TILE>(keys, p.k, piece, first, end, head, p, ht);
@@ -625,19 +749,23 @@ __global__ void __launch_bounds__(THREADS) attention_columns_kernel(const __grid
   const int row = first + (warp % WR) * 16;
   const bool work = here && row < hi;
   const T *mk = keys + (warp % WR) * 16 * LD, *mv = values + (warp % WR) * 16 * LD;
-  float dk[DP / 8][4], dv[DP / 8][4], geo[2][3] = {{0.f, 0.f, 0.f}, {0.f, 0.f, 0.f}};
+  float dk[DP / 8][4], dv[DP / 8][4];
+  pair geo[2][3] = {{0, 0, 0}, {0, 0, 0}};
 #pragma unroll
   for (int n = 0; n < DP / 8; ++n) {
     dk[n][0] = dk[n][1] = dk[n][2] = dk[n][3] = 0.f;
     dv[n][0] = dv[n][1] = dv[n][2] = dv[n][3] = 0.f;
   }
-  const float scale2 = p.scale * LOG2E, cap2 = p.cap * LOG2E, to_cap = p.cap > 0.f ? p.scale / p.cap : 0.f;
-  float slope2 = 0.f;
-  float3 pr[2];
+  const float to_cap = p.cap > 0.f ? p.scale / p.cap : 0.f, unit = (p.cap > 0.f ? p.cap : p.scale) * LOG2E;
+  const float bend = p.cap > 0.f ? -p.scale / (unit * unit) : 0.f;
+  const pair scale2 = both(p.scale, p.scale), bend2 = both(bend, bend), minus = both(-1.f, -1.f);
+  pair slope2 = 0;
+  Here place[2];
   if (p.pos) {
-    slope2 = here ? p.slope[head] * LOG2E : 0.f;
-    pr[0] = position(p.pos, row + g, hi);
-    pr[1] = position(p.pos, row + g + 8, hi);
+    const float f = here ? -p.slope[head] * LOG2E : 0.f;
+    slope2 = both(f, f);
+    place[0] = minus_position(p.pos, row + g, hi);
+    place[1] = minus_position(p.pos, row + g + 8, hi);
   }
   int s = 0;
   for (int query = lo; query < hi; query += KT, s ^= 1) {
@@ -654,43 +782,41 @@ __global__ void __launch_bounds__(THREADS) attention_columns_kernel(const __grid
       float z[NT][4], dp[NT][4];
       score_mma<DP, NT>(z, mk, qs, lane);
       score_mma<DP, NT>(dp, mv, gs, lane);
+      cap_tile<NT>(z, unit, to_cap);
+      const bool last = query + KT > hi;
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int n = 0; n < NT; ++n) {
+        const int c = n * 8 + 2 * t;
+        const pair lse = *reinterpret_cast<const pair*>(ls + c), delta = *reinterpret_cast<const pair*>(ds + c);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int c = n * 8 + 2 * t + i;
-          const float4 pk = p.pos ? spos[s * KT + c] : make_float4(0.f, 0.f, 0.f, 0.f);
-          const bool there = query + c < hi;
-          const float lse = ls[c], delta = ds[c];
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            float &zz = z[n][2 * r + i], &dd = dp[n][2 * r + i];
-            float slant = p.scale, score;
-            if (p.cap > 0.f) {
-              const float th = tanh_of<T>(zz * to_cap);
-              score = cap2 * th;
-              slant = p.scale * (1.f - th * th);
-            } else {
-              score = zz * scale2;
-            }
-            float dx, dy, dz, inv = 0.f;
-            if (p.pos) {                                                 // from the key to the query
-              dx = pk.x - pr[r].x, dy = pk.y - pr[r].y, dz = pk.z - pr[r].z;
-              const float d2 = dx * dx + dy * dy + dz * dz;
-              inv = d2 > 0.f ? rsqrt_fast(d2) : 0.f;
-              score -= slope2 * (d2 * inv);
-            }
-            const float w = there ? exp2_fast(score - lse) : 0.f, e = w * (dd - delta);
-            if (GEO) {
-              const float ei = e * inv;
-              geo[r][0] += ei * dx;
-              geo[r][1] += ei * dy;
-              geo[r][2] += ei * dz;
-            }
-            zz = w;
-            dd = e * slant;
+        for (int r = 0; r < 2; ++r) {
+          const pair score0 = both(z[n][2 * r], z[n][2 * r + 1]), d = both(dp[n][2 * r], dp[n][2 * r + 1]);
+          pair score = score0;
+          Way v;
+          if (p.pos) {                                                   // from the key to the query
+            v = way_to(spos + s * 3 * KT + c, KT, place[r].x, place[r].y, place[r].z);
+            score = fma2(v.length, slope2, score);
           }
+          float x, y;
+          parts(fma2(lse, minus, score), x, y);
+          if (last) {
+            if (query + c >= hi) x = -INFINITY;
+            if (query + c + 1 >= hi) y = -INFINITY;
+          }
+          x = exp2_fast(x);
+          y = exp2_fast(y);
+          const pair e = mul2(both(x, y), fma2(delta, minus, d));
+          if (GEO) {
+            const pair ei = mul2(e, v.inverse);
+            geo[r][0] = fma2(ei, v.x, geo[r][0]);
+            geo[r][1] = fma2(ei, v.y, geo[r][1]);
+            geo[r][2] = fma2(ei, v.z, geo[r][2]);
+          }
+          z[n][2 * r] = x;
+          z[n][2 * r + 1] = y;
+          parts(mul2(e, fma2(mul2(score0, score0), bend2, scale2)), dp[n][2 * r], dp[n][2 * r + 1]);
         }
+      }
       out_mma<DP, NT>(dv, z, gs, lane);
       out_mma<DP, NT>(dk, dp, qs, lane);
     }
@@ -700,7 +826,13 @@ __global__ void __launch_bounds__(THREADS) attention_columns_kernel(const __grid
   if (GEO) {
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      const float4 v = make_float4(0.f, quad_sum(geo[r][0]), quad_sum(geo[r][1]), quad_sum(geo[r][2]));
+      float x, y, sums[3];
+#pragma unroll
+      for (int i = 0; i < 3; ++i) {
+        parts(geo[r][i], x, y);
+        sums[i] = quad_sum(x + y);
+      }
+      const float4 v = make_float4(0.f, sums[0], sums[1], sums[2]);
       if (t == 0 && row + g + 8 * r < hi) p.geo_col[(int64_t)head * p.n + row + g + 8 * r] = v;
     }
   }
@@ -711,30 +843,32 @@ __global__ void __launch_bounds__(THREADS) attention_columns_kernel(const __grid
 // ---- host side ----------------------------------------------------------------------------------
 enum Pass { FORWARD, ROWS, COLUMNS };
 
-template <typename T, int DP, int WR, int KT>
+// KF and KB: keys, or queries, of a tile in the forward and in the backward pass
+template <typename T, int DP, int WR, int KF, int KB>
 int launch(Pass pass, const AttentionParams& p, int64_t tiles, bool geo, cudaStream_t s) {
-  using S = Shape<T, DP, WR, KT>;
-  const dim3 grid((unsigned)tiles, (unsigned)ceil_div(p.heads, S::HEADS));
+  using F = Shape<T, DP, WR, KF>;
+  using B = Shape<T, DP, WR, KB>;
+  const dim3 grid((unsigned)tiles, (unsigned)ceil_div(p.heads, F::HEADS));
   auto run = [&](auto kernel, size_t bytes, const char* what) {
     if (int rc = allow_shared(kernel, bytes)) return rc;
     kernel<<<grid, THREADS, bytes, s>>>(p);
     return check_launch(what);
   };
-  constexpr int POS = 2 * KT * 16, STATS = S::HEADS * 4 * KT * 4;
-  if (pass == FORWARD) return run(attention_forward_kernel<T, DP, WR, KT>, S::bytes(1, POS), "attention_forward");
+  constexpr int POSITIONS = 2 * 12 * KB, STATS = B::HEADS * 16 * KB;     // two tiles each
+  if (pass == FORWARD) return run(attention_forward_kernel<T, DP, WR, KF>, F::bytes(1, 2 * 12 * KF), "attention_forward");
   if (pass == ROWS)
-    return geo ? run(attention_rows_kernel<T, DP, WR, KT, true>, S::bytes(2, POS), "attention_rows")
-               : run(attention_rows_kernel<T, DP, WR, KT, false>, S::bytes(2, POS), "attention_rows");
-  return geo ? run(attention_columns_kernel<T, DP, WR, KT, true>, S::bytes(2, POS + STATS), "attention_columns")
-             : run(attention_columns_kernel<T, DP, WR, KT, false>, S::bytes(2, POS + STATS), "attention_columns");
+    return geo ? run(attention_rows_kernel<T, DP, WR, KB, true>, B::bytes(2, POSITIONS), "attention_rows")
+               : run(attention_rows_kernel<T, DP, WR, KB, false>, B::bytes(2, POSITIONS), "attention_rows");
+  return geo ? run(attention_columns_kernel<T, DP, WR, KB, true>, B::bytes(2, POSITIONS + STATS), "attention_columns")
+             : run(attention_columns_kernel<T, DP, WR, KB, false>, B::bytes(2, POSITIONS + STATS), "attention_columns");
 }
 
 template <typename T, int DP>
 int launch_rows(Pass pass, const AttentionParams& p, int64_t tiles, int tile_rows, bool geo, cudaStream_t s) {
-  constexpr int KT = sizeof(T) == 2 && DP <= 64 ? 64 : 32;       // wide heads need the registers; float32 needs twice the registers and shared memory a value
-  if (tile_rows == 64) return launch<T, DP, 4, KT>(pass, p, tiles, geo, s);
-  if (tile_rows == 32) return launch<T, DP, 2, 32>(pass, p, tiles, geo, s);
-  return launch<T, DP, 1, 16>(pass, p, tiles, geo, s);
+  constexpr int KF = sizeof(T) == 2 && DP <= 64 ? 64 : 32;               // wide heads, float32 and the backward pass need the registers
+  if (tile_rows == 64) return launch<T, DP, 4, KF, 32>(pass, p, tiles, geo, s);
+  if (tile_rows == 32) return launch<T, DP, 2, 32, 32>(pass, p, tiles, geo, s);
+  return launch<T, DP, 1, 16, 16>(pass, p, tiles, geo, s);
 }
 
 template <typename T>
