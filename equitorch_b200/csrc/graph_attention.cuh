@@ -271,11 +271,15 @@ template <int NT> __device__ __forceinline__ void cap_tile(float (&z)[NT][4], fl
 // The way from a row to two columns, one over the distances and the distances.  One over is finite where two nodes coincide, so that
 // the distance comes out as zero, and the way over it too.
 struct Way { pair x, y, z, inverse, length; };
-__device__ __forceinline__ Way way_to(const float* columns, int stride, pair mx, pair my, pair mz) {      // m: minus the row's position
+struct Place { pair x, y, z; };                          // of two columns, or twice that of a row
+__device__ __forceinline__ Place columns_at(const float* columns, int stride) {
+  return {*reinterpret_cast<const pair*>(columns), *reinterpret_cast<const pair*>(columns + stride), *reinterpret_cast<const pair*>(columns + 2 * stride)};
+}
+__device__ __forceinline__ Way way_to(const Place& columns, const Place& minus_row) {
   Way w;
-  w.x = add2(*reinterpret_cast<const pair*>(columns), mx);
-  w.y = add2(*reinterpret_cast<const pair*>(columns + stride), my);
-  w.z = add2(*reinterpret_cast<const pair*>(columns + 2 * stride), mz);
+  w.x = add2(columns.x, minus_row.x);
+  w.y = add2(columns.y, minus_row.y);
+  w.z = add2(columns.z, minus_row.z);
   const pair square = fma2(w.z, w.z, fma2(w.y, w.y, mul2(w.x, w.x)));
   float a, b;
   parts(square, a, b);
@@ -356,12 +360,11 @@ __device__ __forceinline__ void store_rows(T* buf, void* out, const float (&o)[D
   const int d = p.comps * p.size, channels = p.heads * p.size;
   T* to = static_cast<T*>(out) + (int64_t)head * p.size;
   if (p.vec) {
-    const int pieces = d / V;
-    for (int i = lane; i < 16 * pieces; i += 32) {
-      const int r = i / pieces, j = (i - r * pieces) * V, m = j / p.size, c = j - m * p.size;
-      if (first + r < end)
-        *reinterpret_cast<uint4*>(to + ((int64_t)(first + r) * p.comps + m) * channels + c) = *reinterpret_cast<const uint4*>(buf + r * LD + j);
-    }
+    const Piece<T, DP, 32> piece(lane, p.comps, p.size);
+    if (!piece.there) return;
+    to += (int64_t)piece.comp * channels + piece.channel;
+    for (int r = piece.row; r < 16 && first + r < end; r += Piece<T, DP, 32>::ROWS)
+      *reinterpret_cast<uint4*>(to + (int64_t)(first + r) * p.comps * channels) = *reinterpret_cast<const uint4*>(buf + r * LD + piece.at);
     return;
   }
   for (int i = lane; i < 16 * d; i += 32) {
@@ -405,15 +408,14 @@ __device__ __forceinline__ void row_delta(const T* grads, int first, int end, in
 template <int ROWS_TILE>
 __device__ __forceinline__ void load_positions(float* dst, const float* pos, int first, int end) {
   for (int i = threadIdx.x; i < ROWS_TILE * 3; i += THREADS) {
-    const int r = i / 3, x = i - r * 3;
+    const int x = i / ROWS_TILE, r = i % ROWS_TILE;
     const bool there = first + r < end;
-    copy4(dst + x * ROWS_TILE + r, pos + (int64_t)(there ? first + r : 0) * 3 + x, there);
+    copy4(dst + i, pos + (int64_t)(there ? first + r : 0) * 3 + x, there);
   }
 }
 
 // Minus the position of a row, each coordinate twice.
-struct Here { pair x, y, z; };
-__device__ __forceinline__ Here minus_position(const float* pos, int row, int end) {
+__device__ __forceinline__ Place minus_position(const float* pos, int row, int end) {
   float x = 0.f, y = 0.f, z = 0.f;
   if (row < end) x = -pos[(int64_t)row * 3], y = -pos[(int64_t)row * 3 + 1], z = -pos[(int64_t)row * 3 + 2];
   return {both(x, x), both(y, y), both(z, z)};
@@ -433,7 +435,7 @@ template <typename T, int DP, int WR, int KT> struct Shape {
 };
 
 template <typename T, int DP, int WR, int KT>
-__global__ void __launch_bounds__(THREADS, DP <= 64 ? 4 : 3) attention_forward_kernel(const __grid_constant__ AttentionParams p) {
+__global__ void __launch_bounds__(THREADS, DP <= 32 ? 6 : DP <= 64 ? 4 : 3) attention_forward_kernel(const __grid_constant__ AttentionParams p) {
   using S = Shape<T, DP, WR, KT>;
   constexpr int LD = S::LD, NT = KT / 8;
   extern __shared__ __align__(16) unsigned char smem[];
@@ -469,7 +471,7 @@ __global__ void __launch_bounds__(THREADS, DP <= 64 ? 4 : 3) attention_forward_k
   for (int n = 0; n < DP / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
   const float to_cap = p.cap > 0.f ? p.scale / p.cap : 0.f, unit = (p.cap > 0.f ? p.cap : p.scale) * LOG2E;   // of a score: the tanh, or the product
   pair slope2 = 0;                                                       // minus the slope, twice, in units of log2
-  Here at[2];
+  Place at[2];
   if (p.pos) {
     const float f = here ? -p.slope[head] * LOG2E : 0.f;
     slope2 = both(f, f);
@@ -492,12 +494,12 @@ __global__ void __launch_bounds__(THREADS, DP <= 64 ? 4 : 3) attention_forward_k
       cap_tile<NT>(z, unit, to_cap);
       if (p.pos) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int n = 0; n < NT; ++n) {
+          const Place columns = columns_at(spos + s * 3 * KT + n * 8 + 2 * t, KT);
 #pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            const Way w = way_to(spos + s * 3 * KT + n * 8 + 2 * t, KT, at[r].x, at[r].y, at[r].z);
-            parts(fma2(w.length, slope2, both(z[n][2 * r], z[n][2 * r + 1])), z[n][2 * r], z[n][2 * r + 1]);
-          }
+          for (int r = 0; r < 2; ++r)
+            parts(fma2(way_to(columns, at[r]).length, slope2, both(z[n][2 * r], z[n][2 * r + 1])), z[n][2 * r], z[n][2 * r + 1]);
+        }
       }
       if (key + KT > hi) {
 #pragma unroll
@@ -563,7 +565,7 @@ __global__ void __launch_bounds__(THREADS, DP <= 64 ? 4 : 3) attention_forward_k
 // These sums are float32 results also where the features are bfloat16, so there they do not go by the delta of the rounded weights and
 // result: with w = r or u, sum_j dS w = sum_j P dP w - (sum_j P dP) (sum_j P w), and the columns' pass is given sum_j P dP.
 template <typename T, int DP, int WR, int KT, bool GEO>
-__global__ void __launch_bounds__(THREADS) attention_rows_kernel(const __grid_constant__ AttentionParams p) {
+__global__ void __launch_bounds__(THREADS, DP <= 32 ? 4 : DP <= 96 ? 3 : 2) attention_rows_kernel(const __grid_constant__ AttentionParams p) {
   using S = Shape<T, DP, WR, KT>;
   constexpr int LD = S::LD, NT = KT / 8;
   extern __shared__ __align__(16) unsigned char smem[];
@@ -617,7 +619,7 @@ __global__ void __launch_bounds__(THREADS) attention_rows_kernel(const __grid_co
   const float bend = p.cap > 0.f ? -p.scale / (unit * unit) : 0.f;         // scale (1 - tanh^2), from unit tanh
   const pair scale2 = both(p.scale, p.scale), bend2 = both(bend, bend);
   pair slope2 = 0;
-  Here place[2];
+  Place place[2];
   if (p.pos) {
     const float f = here ? -p.slope[head] * LOG2E : 0.f;
     slope2 = both(f, f);
@@ -641,14 +643,16 @@ __global__ void __launch_bounds__(THREADS) attention_rows_kernel(const __grid_co
       cap_tile<NT>(z, unit, to_cap);
       const bool last = key + KT > hi;
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int n = 0; n < NT; ++n) {
+        Place columns;
+        if (p.pos) columns = columns_at(spos + s * 3 * KT + n * 8 + 2 * t, KT);
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           const pair score0 = both(z[n][2 * r], z[n][2 * r + 1]), d = both(dp[n][2 * r], dp[n][2 * r + 1]);
           pair score = score0;
           Way v;
           if (p.pos) {
-            v = way_to(spos + s * 3 * KT + n * 8 + 2 * t, KT, place[r].x, place[r].y, place[r].z);
+            v = way_to(columns, place[r]);
             score = fma2(v.length, slope2, score);
           }
           float x, y;
@@ -674,6 +678,7 @@ __global__ void __launch_bounds__(THREADS) attention_rows_kernel(const __grid_co
           }
           parts(mul2(e, fma2(mul2(score0, score0), bend2, scale2)), z[n][2 * r], z[n][2 * r + 1]);
         }
+      }
       out_mma<DP, NT>(dq, z, ks, lane);
     }
     __syncthreads();
@@ -710,7 +715,7 @@ __global__ void __launch_bounds__(THREADS) attention_rows_kernel(const __grid_co
 // Backward by columns: dk, dv, and with positions the columns' sums of dS u.  The CTA's rows are keys; queries and the output's
 // gradients come by in tiles, and the products are the transposed ones.
 template <typename T, int DP, int WR, int KT, bool GEO>
-__global__ void __launch_bounds__(THREADS) attention_columns_kernel(const __grid_constant__ AttentionParams p) {
+__global__ void __launch_bounds__(THREADS, DP <= 32 ? 4 : DP <= 64 ? 3 : 2) attention_columns_kernel(const __grid_constant__ AttentionParams p) {
   using S = Shape<T, DP, WR, KT>;
   constexpr int LD = S::LD, NT = KT / 8;
   extern __shared__ __align__(16) unsigned char smem[];
@@ -760,7 +765,7 @@ __global__ void __launch_bounds__(THREADS) attention_columns_kernel(const __grid
   const float bend = p.cap > 0.f ? -p.scale / (unit * unit) : 0.f;
   const pair scale2 = both(p.scale, p.scale), bend2 = both(bend, bend), minus = both(-1.f, -1.f);
   pair slope2 = 0;
-  Here place[2];
+  Place place[2];
   if (p.pos) {
     const float f = here ? -p.slope[head] * LOG2E : 0.f;
     slope2 = both(f, f);
@@ -788,13 +793,15 @@ __global__ void __launch_bounds__(THREADS) attention_columns_kernel(const __grid
       for (int n = 0; n < NT; ++n) {
         const int c = n * 8 + 2 * t;
         const pair lse = *reinterpret_cast<const pair*>(ls + c), delta = *reinterpret_cast<const pair*>(ds + c);
+        Place columns;
+        if (p.pos) columns = columns_at(spos + s * 3 * KT + c, KT);
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           const pair score0 = both(z[n][2 * r], z[n][2 * r + 1]), d = both(dp[n][2 * r], dp[n][2 * r + 1]);
           pair score = score0;
           Way v;
           if (p.pos) {                                                   // from the key to the query
-            v = way_to(spos + s * 3 * KT + c, KT, place[r].x, place[r].y, place[r].z);
+            v = way_to(columns, place[r]);
             score = fma2(v.length, slope2, score);
           }
           float x, y;
@@ -876,6 +883,7 @@ int launch_width(Pass pass, const AttentionParams& p, int64_t tiles, int tile_ro
   const int d = p.comps * p.size;
   if (d <= 32) return launch_rows<T, 32>(pass, p, tiles, tile_rows, geo, s);
   if (d <= 64) return launch_rows<T, 64>(pass, p, tiles, tile_rows, geo, s);
+  if (d <= 80) return launch_rows<T, 80>(pass, p, tiles, tile_rows, geo, s);       // nine components of eight channels
   if (d <= 96) return launch_rows<T, 96>(pass, p, tiles, tile_rows, geo, s);
   return launch_rows<T, 128>(pass, p, tiles, tile_rows, geo, s);
 }
