@@ -64,15 +64,16 @@ __global__ void __launch_bounds__(256) embedding_kernel(const T* __restrict__ we
 
 // ---- sort by type -------------------------------------------------------------------------------
 // A row that names no type gets the key `types`, which sorts behind all others.
-__device__ __forceinline__ int key_of(const int64_t* index, const int32_t* keys, int64_t i, int64_t types) {
-  if (keys) return __ldg(keys + i);
+// Key and row travel as one value of eight bytes: places are scattered, so a store costs a sector whatever its size.
+__device__ __forceinline__ int2 entry_of(const int64_t* index, const int2* sorted, int64_t i, int64_t types) {
+  if (sorted) return __ldg(sorted + i);
   const int64_t t = __ldg(index + i);
-  return (int)((uint64_t)t < (uint64_t)types ? t : types);
+  return make_int2((int)((uint64_t)t < (uint64_t)types ? t : types), (int)i);
 }
 
 // Each warp owns `rows` rows in a row; within[warp][bin] is how many rows of the digit the warps of its CTA before it own,
 // counts[CTA][bin] how many the CTA does.
-__global__ void __launch_bounds__(SORT_THREADS) sort_count_kernel(const int64_t* __restrict__ index, const int32_t* __restrict__ keys,
+__global__ void __launch_bounds__(SORT_THREADS) sort_count_kernel(const int64_t* __restrict__ index, const int2* __restrict__ sorted,
                                                                   int* __restrict__ within, int* __restrict__ counts, int64_t n,
                                                                   int64_t types, int64_t rows, int shift, int bins) {
   extern __shared__ int tally[];
@@ -82,7 +83,7 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_count_kernel(const int64_t*
   __syncwarp();
   const int64_t w = (int64_t)blockIdx.x * SORT_WARPS + warp, lo = w * rows, hi = min(n, lo + rows);
 #pragma unroll 4
-  for (int64_t i = lo + lane; i < hi; i += 32) atomicAdd(&mine[(key_of(index, keys, i, types) >> shift) & (bins - 1)], 1);   // counts: order is free
+  for (int64_t i = lo + lane; i < hi; i += 32) atomicAdd(&mine[(entry_of(index, sorted, i, types).x >> shift) & (bins - 1)], 1);   // counts: order is free
   __syncthreads();
   for (int b = threadIdx.x; b < bins; b += SORT_THREADS) {
     int run = 0;
@@ -123,12 +124,10 @@ __global__ void __launch_bounds__(1024) sort_scan_kernel(const int* __restrict__
 }
 
 // Rows to their places, in their order within a digit: a warp takes 32 rows at a time, lanes of the same digit rank by lane.
-__global__ void __launch_bounds__(SORT_THREADS) sort_place_kernel(const int64_t* __restrict__ index, const int32_t* __restrict__ keys,
-                                                                  const int32_t* __restrict__ order, const int* __restrict__ within,
-                                                                  const int* __restrict__ before,
-                                                                  const int* __restrict__ totals, int32_t* __restrict__ keys_out,
-                                                                  int32_t* __restrict__ order_out, int64_t n, int64_t types,
-                                                                  int64_t rows, int shift, int bins) {
+__global__ void __launch_bounds__(SORT_THREADS) sort_place_kernel(const int64_t* __restrict__ index, const int2* __restrict__ sorted,
+                                                                  const int* __restrict__ within, const int* __restrict__ before,
+                                                                  const int* __restrict__ totals, int2* __restrict__ out, int64_t n,
+                                                                  int64_t types, int64_t rows, int shift, int bins) {
   extern __shared__ int place[];                // [warp][bin]
   __shared__ int first[MAX_BINS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -152,27 +151,23 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_place_kernel(const int64_t*
   for (int b = lane; b < bins; b += 32) mine[b] = first[b] + before[(int64_t)blockIdx.x * bins + b] + within[w * bins + b];
   __syncwarp();
   for (int64_t i0 = lo; i0 < hi; i0 += 128) {
-    int key[4], from[4];
+    int2 entry[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {               // the loads of four steps together
       const int64_t i = i0 + u * 32 + lane;
-      key[u] = i < hi ? key_of(index, keys, i, types) : 0;
-      from[u] = i < hi && order ? __ldg(order + i) : (int)i;
+      entry[u] = i < hi ? entry_of(index, sorted, i, types) : make_int2(0, 0);
     }
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const bool there = i0 + u * 32 + lane < hi;
-      const int digit = there ? (key[u] >> shift) & (bins - 1) : bins;         // lanes past the end are a digit of their own
+      const int digit = there ? (entry[u].x >> shift) & (bins - 1) : bins;     // lanes past the end are a digit of their own
       const unsigned same = __match_any_sync(FULL, digit);
       const int rank = __popc(same & ((1u << lane) - 1));
       const int to = there ? mine[digit] + rank : 0;
       __syncwarp();
       if (there && rank == 0) mine[digit] += __popc(same);
       __syncwarp();
-      if (there) {
-        keys_out[to] = key[u];
-        order_out[to] = from[u];
-      }
+      if (there) out[to] = entry[u];
     }
   }
 }
@@ -194,8 +189,7 @@ __device__ __forceinline__ void put_part(A* p, const A (&sum)[V]) {
 // A team of `team` lanes (a power of two) adds up the sorted rows [c * piece, (c + 1) * piece), V columns a lane.  A type whose rows
 // all lie in the piece is written at once; what began in a piece before goes to head[c], what goes on in the next to tail[c].
 template <typename T, int V>
-__global__ void __launch_bounds__(TEAM_THREADS) piece_sum_kernel(const T* __restrict__ g, const int32_t* __restrict__ keys,
-                                                                 const int32_t* __restrict__ order, T* __restrict__ gw,
+__global__ void __launch_bounds__(TEAM_THREADS) piece_sum_kernel(const T* __restrict__ g, const int2* __restrict__ sorted, T* __restrict__ gw,
                                                                  typename Acc<T>::type* __restrict__ head,
                                                                  typename Acc<T>::type* __restrict__ tail, int64_t n, int types,
                                                                  int64_t pitch, int cols, int team, int piece, int64_t pieces,
@@ -209,8 +203,8 @@ __global__ void __launch_bounds__(TEAM_THREADS) piece_sum_kernel(const T* __rest
   A sum[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) sum[i] = A(0);
-  int now = keys[lo];
-  bool open = lo > 0 && keys[lo - 1] == now;                                   // the run began in a piece before
+  int now = sorted[lo].x;
+  bool open = lo > 0 && sorted[lo - 1].x == now;                                   // the run began in a piece before
   auto close = [&](int key, bool goes_on) {
     if (key < types) {
       if (open) put_part(head + c * pitch + (int64_t)col * V, sum);
@@ -222,19 +216,19 @@ __global__ void __launch_bounds__(TEAM_THREADS) piece_sum_kernel(const T* __rest
     open = false;
   };
   for (int64_t i = lo; i < hi; i += UNROLL) {
-    int key[UNROLL];
+    int2 entry[UNROLL];
     Packed<T, V> row[UNROLL];
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u) key[u] = i + u < hi ? __ldg(keys + i + u) : types;
+    for (int u = 0; u < UNROLL; ++u) entry[u] = i + u < hi ? __ldg(sorted + i + u) : make_int2(types, 0);
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u)
-      if (key[u] < types) row[u] = *reinterpret_cast<const Packed<T, V>*>(gc + (int64_t)__ldg(order + i + u) * pitch);
+      if (entry[u].x < types) row[u] = *reinterpret_cast<const Packed<T, V>*>(gc + (int64_t)entry[u].y * pitch);
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
       if (i + u >= hi) break;
-      if (key[u] != now) {
+      if (entry[u].x != now) {
         close(now, false);
-        now = key[u];
+        now = entry[u].x;
       }
       if (now < types) {
 #pragma unroll
@@ -242,7 +236,7 @@ __global__ void __launch_bounds__(TEAM_THREADS) piece_sum_kernel(const T* __rest
       }
     }
   }
-  close(now, hi < n && keys[hi] == now);
+  close(now, hi < n && sorted[hi].x == now);
 }
 
 // Adds up parts tail[c], head[c + 1 .. last] of a run, V columns a lane: team `mine` of `teams` takes every teams-th part in order.
@@ -262,7 +256,7 @@ __device__ __forceinline__ void add_parts(const A* __restrict__ head, const A* _
 // where they are many.  Teams of lanes take the parts in turn and are added up in a fixed order.
 constexpr int JOIN_WARPS = 8, JOIN_ALONE = 64;
 template <typename T, int V>
-__global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const int32_t* __restrict__ keys, T* __restrict__ gw,
+__global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const int2* __restrict__ sorted, T* __restrict__ gw,
                                                                const typename Acc<T>::type* __restrict__ head,
                                                                const typename Acc<T>::type* __restrict__ tail, int64_t n, int types,
                                                                int64_t pitch, int cols, int team, int piece, int64_t pieces,
@@ -282,15 +276,15 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const int32_t* __
   int64_t last = -1;
   int key = types;
   if (c < pieces) {
-    key = keys[hi - 1];
-    if (key < types && hi < n && keys[hi] == key && !(lo > 0 && keys[lo - 1] == key)) {
+    key = sorted[hi - 1].x;
+    if (key < types && hi < n && sorted[hi].x == key && !(lo > 0 && sorted[lo - 1].x == key)) {
       // The run reaches into the pieces whose first row has its type: 32 of them are looked at a step, first the next ones, then by
       // 32nds of what is left.
       last = c + 1;                             // reaches in
       int64_t past = pieces;                    // does not
       for (int64_t step = 1; past - last > 1; step = (past - last + 31) / 32) {
         const int64_t at = last + (lane + 1) * step;
-        const unsigned in = __ballot_sync(FULL, at < past && __ldg(keys + at * piece) == key);     // a run of ones from lane 0 on
+        const unsigned in = __ballot_sync(FULL, at < past && __ldg(&sorted[at * piece].x) == key);     // a run of ones from lane 0 on
         const int reach = __popc(in);
         if (reach < 32) past = min(past, last + (reach + 1) * step);
         last += reach * step;
@@ -315,7 +309,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const int32_t* __
     const int64_t end = long_last[w];
     if (end < 0) continue;
     const int64_t first = (int64_t)blockIdx.x * JOIN_WARPS + w;
-    const int64_t type = keys[min(n, (first + 1) * piece) - 1];
+    const int64_t type = sorted[min(n, (first + 1) * piece) - 1].x;
     for (int col0 = 0; col0 < cols; col0 += team) {
       const int col = col0 + tl;
       A sum[V];
@@ -394,7 +388,7 @@ struct GradPlan {
   int64_t warps, rows;      // of the sort
   int piece;
   int64_t pieces;
-  size_t keys, order, within, counts, before, totals, parts, bytes;       // scratch: two buffers each of keys and order
+  size_t sorted, within, counts, before, totals, parts, bytes;       // scratch: two buffers of sorted rows
 };
 
 int size_of(int dtype) { return dtype == EQT_F64 ? 8 : dtype == EQT_F32 ? 4 : 2; }
@@ -413,13 +407,13 @@ GradPlan grad_plan(int dtype, int64_t n, int64_t types, int64_t width) {
   p.warps = ceil_div(ceil_div(n, p.rows), SORT_WARPS) * SORT_WARPS;
   int team = 1;                                           // lanes that have a row: one 16 bytes, at most 32
   while (team < 32 && team * 16 < width * size_of(dtype)) team *= 2;
-  // Pieces so short that 512 threads an SM have one, but not so short that their borders cost more than their rows.
-  p.piece = (int)std::max<int64_t>(32, ceil_div(ceil_div(n, (int64_t)sm_count() * 512 / team), UNROLL) * UNROLL);
+  // Pieces so short that 256 threads an SM have one, but not so short that their borders cost more than their rows (2.0M rows of 64
+  // bytes, 14161 types, sums and joins: 100 us with 256 threads, 107 with 512, 104 with 1024, 121 with 2048).
+  p.piece = (int)std::max<int64_t>(32, ceil_div(ceil_div(n, (int64_t)sm_count() * 256 / team), UNROLL) * UNROLL);
   p.pieces = ceil_div(n, p.piece);
   auto up = [](size_t b) { return (b + 255) / 256 * 256; };
-  p.keys = 0;
-  p.order = up((size_t)n * 4) * 2;
-  p.within = p.order + up((size_t)n * 4) * 2;
+  p.sorted = 0;
+  p.within = up((size_t)n * 8) * 2;
   const size_t bins = (size_t)4 << p.digit_bits, ctas = (size_t)p.warps / SORT_WARPS;
   p.counts = p.within + up(p.warps * bins);
   p.before = p.counts + up(ctas * bins);
@@ -450,9 +444,7 @@ int run_grad(int dtype, const void* g, const int64_t* index, void* gw, int64_t n
     return check_launch("type_sum");
   }
   if (cudaMemsetAsync(gw, 0, (size_t)types * width * sizeof(T), s) != cudaSuccess) return fail(EQT_ERR_CUDA, "cudaMemsetAsync failed");
-  const size_t n4 = ((size_t)n * 4 + 255) / 256 * 256;
-  int32_t* keys[2] = {reinterpret_cast<int32_t*>(scratch + p.keys), reinterpret_cast<int32_t*>(scratch + p.keys + n4)};
-  int32_t* order[2] = {reinterpret_cast<int32_t*>(scratch + p.order), reinterpret_cast<int32_t*>(scratch + p.order + n4)};
+  int2* sorted[2] = {reinterpret_cast<int2*>(scratch + p.sorted), reinterpret_cast<int2*>(scratch + p.sorted + ((size_t)n * 8 + 255) / 256 * 256)};
   int* within = reinterpret_cast<int*>(scratch + p.within);
   int* counts = reinterpret_cast<int*>(scratch + p.counts);
   int* before = reinterpret_cast<int*>(scratch + p.before);
@@ -462,14 +454,13 @@ int run_grad(int dtype, const void* g, const int64_t* index, void* gw, int64_t n
   const size_t shared = (size_t)SORT_WARPS * bins * 4;     // at most 8 KB
   int at = 0;
   for (int pass = 0; pass < p.passes; ++pass, at ^= 1) {
-    const int32_t* k = pass ? keys[at ^ 1] : nullptr;
-    const int32_t* o = pass ? order[at ^ 1] : nullptr;
+    const int2* from = pass ? sorted[at ^ 1] : nullptr;
     const int shift = pass * p.digit_bits;
-    sort_count_kernel<<<grid, SORT_THREADS, shared, s>>>(index, k, within, counts, n, types, p.rows, shift, bins);
+    sort_count_kernel<<<grid, SORT_THREADS, shared, s>>>(index, from, within, counts, n, types, p.rows, shift, bins);
     if (int rc = check_launch("sort_count")) return rc;
     sort_scan_kernel<<<(unsigned)ceil_div(bins, 32), 1024, 0, s>>>(counts, before, totals, (int)grid, bins);
     if (int rc = check_launch("sort_scan")) return rc;
-    sort_place_kernel<<<grid, SORT_THREADS, shared, s>>>(index, k, o, within, before, totals, keys[at], order[at], n, types, p.rows, shift, bins);
+    sort_place_kernel<<<grid, SORT_THREADS, shared, s>>>(index, from, within, before, totals, sorted[at], n, types, p.rows, shift, bins);
     if (int rc = check_launch("sort_place")) return rc;
   }
   at ^= 1;
@@ -478,11 +469,11 @@ int run_grad(int dtype, const void* g, const int64_t* index, void* gw, int64_t n
   A* head = reinterpret_cast<A*>(scratch + p.parts);
   A* tail = reinterpret_cast<A*>(scratch + p.parts + ((size_t)p.pieces * width * sizeof(A) + 255) / 256 * 256);
   const dim3 sums((unsigned)ceil_div(p.pieces * team, TEAM_THREADS), (unsigned)ceil_div(cols, team));
-  piece_sum_kernel<T, V><<<sums, TEAM_THREADS, 0, s>>>(static_cast<const T*>(g), keys[at], order[at], static_cast<T*>(gw), head, tail, n,
+  piece_sum_kernel<T, V><<<sums, TEAM_THREADS, 0, s>>>(static_cast<const T*>(g), sorted[at], static_cast<T*>(gw), head, tail, n,
                                                         (int)types, width, cols, team, p.piece, p.pieces, scale);
   if (int rc = check_launch("piece_sum")) return rc;
   join_kernel<T, V><<<(unsigned)ceil_div(p.pieces, JOIN_WARPS), JOIN_WARPS * 32, 0, s>>>(
-      keys[at], static_cast<T*>(gw), head, tail, n, (int)types, width, cols, team, p.piece, p.pieces, scale);
+      sorted[at], static_cast<T*>(gw), head, tail, n, (int)types, width, cols, team, p.piece, p.pieces, scale);
   return check_launch("join");
 }
 

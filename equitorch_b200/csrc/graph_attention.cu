@@ -38,6 +38,76 @@ __global__ void __launch_bounds__(GEO_THREADS) attention_geometry_kernel(const f
   dpos[3 * i + 2] = z;
 }
 
+// ---- tiles of a packed batch --------------------------------------------------------------------
+constexpr int PACK_THREADS = 1024, CLASSES = 64;
+// Graphs of about one size: two classes an octave, the largest first.
+__device__ __forceinline__ int size_class(int64_t size) {
+  const int octave = 63 - __clzll(size);
+  return CLASSES - 1 - min(CLASSES - 1, 2 * octave + (octave ? (int)(size >> (octave - 1)) & 1 : 0));
+}
+
+// stats: first boundary, last boundary, least size, and how many tiles of 16, 32 and 64 rows there are.
+__global__ void __launch_bounds__(PACK_THREADS) pack_stats_kernel(const int64_t* __restrict__ ptr, int64_t graphs, int64_t* __restrict__ stats) {
+  __shared__ long long least, tiles[3];
+  if (threadIdx.x == 0) least = INT64_MAX, tiles[0] = tiles[1] = tiles[2] = 0;
+  __syncthreads();
+  long long low = INT64_MAX, sum[3] = {0, 0, 0};
+  for (int64_t g = threadIdx.x; g < graphs; g += PACK_THREADS) {
+    const int64_t size = ptr[g + 1] - ptr[g];
+    low = min(low, (long long)size);
+    for (int i = 0; i < 3; ++i) sum[i] += size > 0 ? (size + (16 << i) - 1) >> (4 + i) : 0;
+  }
+  atomicMin(&least, low);
+  for (int i = 0; i < 3; ++i) atomicAdd(reinterpret_cast<unsigned long long*>(&tiles[i]), (unsigned long long)sum[i]);
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    stats[0] = ptr[0];
+    stats[1] = ptr[graphs];
+    stats[2] = graphs ? least : 0;
+    for (int i = 0; i < 3; ++i) stats[3 + i] = tiles[i];
+  }
+}
+
+// The tiles, those of the larger classes first; within a class a graph's place is any, which changes no result.
+__global__ void __launch_bounds__(PACK_THREADS) pack_tiles_kernel(const int64_t* __restrict__ ptr, int64_t graphs, int4* __restrict__ tiles,
+                                                                  int64_t num_tiles, int rows) {
+  __shared__ unsigned long long place[CLASSES];
+  const int lane = threadIdx.x & 31;
+  auto tiles_of = [&](int64_t size) { return size > 0 ? (size + rows - 1) / rows : 0; };
+  if (threadIdx.x < CLASSES) place[threadIdx.x] = 0;
+  __syncthreads();
+  for (int64_t g = threadIdx.x; g < graphs; g += PACK_THREADS) {
+    const int64_t size = ptr[g + 1] - ptr[g];
+    if (size > 0) atomicAdd(&place[size_class(size)], (unsigned long long)tiles_of(size));
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    unsigned long long run = 0;
+    for (int c = 0; c < CLASSES; ++c) {
+      const unsigned long long here = place[c];
+      place[c] = run;
+      run += here;
+    }
+  }
+  __syncthreads();
+  for (int64_t g0 = threadIdx.x - lane; g0 < graphs; g0 += PACK_THREADS) {
+    const int64_t g = g0 + lane;
+    const int64_t lo = g < graphs ? ptr[g] : 0, hi = g < graphs ? ptr[g + 1] : 0, count = tiles_of(hi - lo);
+    const int64_t at = count ? (int64_t)atomicAdd(&place[size_class(hi - lo)], (unsigned long long)count) : 0;
+    constexpr int ALONE = 4;                             // tiles that a lane writes by itself; the warp writes those of larger graphs
+    for (int64_t t = 0; t < count && count <= ALONE; ++t)
+      if (at + t < num_tiles) tiles[at + t] = make_int4((int)(lo + t * rows), (int)lo, (int)hi, 0);
+    unsigned many = __ballot_sync(0xffffffffu, count > ALONE);
+    while (many) {
+      const int who = __ffs(many) - 1;
+      many &= many - 1;
+      const int64_t l = __shfl_sync(0xffffffffu, lo, who), h = __shfl_sync(0xffffffffu, hi, who), a = __shfl_sync(0xffffffffu, at, who);
+      for (int64_t t = lane; l + t * rows < h; t += 32)
+        if (a + t < num_tiles) tiles[a + t] = make_int4((int)(l + t * rows), (int)l, (int)h, 0);
+    }
+  }
+}
+
 int launch_all(Pass pass, const eqt_attention_args* a, const AttentionParams& p, bool geo, cudaStream_t s) {
   return a->dtype == EQT_F32 ? launch_f32(pass, p, a->num_tiles, a->tile_rows, geo, s)
                              : launch_bf16(pass, p, a->num_tiles, a->tile_rows, geo, s);
@@ -117,4 +187,18 @@ extern "C" int eqt_attention_backward(const eqt_attention_args* a, void* stream)
   attention_geometry_kernel<<<(unsigned)(a->heads + ceil_div(a->n, GEO_THREADS)), GEO_THREADS, 0, s>>>(
       p.geo_row, p.geo_col, a->slope, a->dslope, a->dpos, a->n, a->heads);
   return check_launch("attention_geometry");
+}
+
+extern "C" int eqt_pack_graphs_stats(const int64_t* ptr, int64_t graphs, int64_t* stats, void* stream) {
+  if (!ptr || !stats || graphs < 0) return fail(EQT_ERR_BAD_ARGUMENT, "pack_graphs: NULL pointer or negative size");
+  pack_stats_kernel<<<1, PACK_THREADS, 0, static_cast<cudaStream_t>(stream)>>>(ptr, graphs, stats);
+  return check_launch("pack_stats");
+}
+
+extern "C" int eqt_pack_graphs_tiles(const int64_t* ptr, int64_t graphs, int32_t* tiles, int64_t num_tiles, int32_t rows, void* stream) {
+  if (num_tiles == 0 || graphs == 0) return EQT_OK;
+  if (!ptr || !tiles || graphs < 0 || num_tiles < 0) return fail(EQT_ERR_BAD_ARGUMENT, "pack_graphs: NULL pointer or negative size");
+  if (rows != 16 && rows != 32 && rows != 64) return fail(EQT_ERR_BAD_ARGUMENT, "pack_graphs: tiles have 16, 32 or 64 rows");
+  pack_tiles_kernel<<<1, PACK_THREADS, 0, static_cast<cudaStream_t>(stream)>>>(ptr, graphs, reinterpret_cast<int4*>(tiles), num_tiles, rows);
+  return check_launch("pack_tiles");
 }

@@ -685,6 +685,13 @@ typedef struct eqt_attention_args {
 } eqt_attention_args;
 int eqt_attention_forward(const eqt_attention_args* args, void* stream);
 int eqt_attention_backward(const eqt_attention_args* args, void* stream);
+/*
+ * The tiles of a packed batch: graph g has the nodes [ptr[g], ptr[g + 1]).  stats (6): ptr[0], ptr[graphs], the least size, and how many
+ * tiles of 16, 32 and 64 rows the graphs have; the caller checks them (a tile outside the nodes must not reach the attention) and gives
+ * room for as many tiles as its choice of rows has.  Larger graphs' tiles come first, by classes of size.
+ */
+int eqt_pack_graphs_stats(const int64_t* ptr, int64_t graphs, int64_t* stats, void* stream);
+int eqt_pack_graphs_tiles(const int64_t* ptr, int64_t graphs, int32_t* tiles, int64_t num_tiles, int32_t rows, void* stream);
 
 /*
  * Gated linear layer: h (n, f) = act(x W0) * (x W1) for x (n, c) and w (2, c, f), contiguous.  Backward, from g = dL/dh: dx (n, c)

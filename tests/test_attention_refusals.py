@@ -83,3 +83,5 @@ def test_library_checks_its_arguments(wrong):
     assert lib.eqt_attention_backward(ctypes.byref(_lib.AttentionArgs(**good)), None) == 1
     given = dict(grad_out=16, lse=16, dq=16, dk=16, dv=16, delta=16)
     assert lib.eqt_attention_backward(ctypes.byref(_lib.AttentionArgs(**good, **given, dpos=16, dslope=16)), None) == 1
+    assert lib.eqt_pack_graphs_stats(None, 1, 16, None) == 1 and lib.eqt_pack_graphs_tiles(16, 1, 16, 1, 48, None) == 1
+    assert lib.eqt_pack_graphs_tiles(16, 1, None, 1, 16, None) == 1 and lib.eqt_pack_graphs_tiles(None, 0, None, 0, 16, None) == 0

@@ -246,6 +246,25 @@ def test_no_nodes_and_no_graphs():
         assert all(not t.any() for t in got)
 
 
+@pytest.mark.parametrize("sizes,first,behind", [([1], 0, 0), ([0, 0], 0, 0), ([], 0, 3), ([30] * 70, 0, 0), ([16, 3, 0, 5], 2, 3),
+                                                ([100, 64, 1, 200, 5001, 3], 0, 9), (list(range(1500)), 1, 0)])
+def test_pieces_on_the_gpu_are_those_of_the_host(sizes, first, behind):
+    ptr = torch.tensor([first] + sizes).cumsum(0)
+    n = int(ptr[-1]) + behind
+    here, there = PackedGraphs(ptr, n), PackedGraphs(ptr.to(DEV), n)
+    assert (here.tile_rows, here.covers) == (there.tile_rows, there.covers)
+    assert sorted(here.tiles.tolist()) == sorted(there.tiles.tolist())
+    lengths = [hi - lo for _, lo, hi, _ in there.tiles.tolist()]
+    assert all(2 * a >= b for a, b in zip(lengths, lengths[1:]))               # by classes of size, the largest first
+    assert torch.equal(here.to(DEV).tiles, here.tiles.to(DEV))
+
+
+def test_bad_boundaries_on_the_gpu():
+    for ptr, n in ([0, 5, 3], 5), ([-1, 5], 5), ([0, 6], 5), ([0, 2 ** 40], 5):
+        with pytest.raises(ValueError, match="ascend"):
+            PackedGraphs(torch.tensor(ptr, device=DEV), n)
+
+
 def test_module_and_batch_vector():
     batch = torch.tensor([0] * 7 + [2] * 30, device=DEV)
     graphs = PackedGraphs.from_batch(batch, 4)
