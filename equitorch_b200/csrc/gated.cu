@@ -1,7 +1,9 @@
-// Gated linear layer: the C entry points, and the kernels without tensor cores for float64 and for sizes whose rows do not start on
-// 16-byte boundaries, where the tensor memory accelerator cannot copy tiles.
+// Gated linear layer: the C entry points, and the kernels for float64, which have no tensor cores.
 //
-// The simple kernel is a tiled product of strided operands, 64 x 64 results a CTA of 256 threads, 4 x 4 a thread, 16 terms at a time;
+// The tensor memory accelerator copies tiles of operands whose rows start on 16-byte boundaries, so x and W of other widths are first
+// copied to scratch with wider rows; da, du and the partial results have such rows anyway, and results are stored as they are to lie.
+//
+// The float64 kernel is a tiled product of strided operands, 64 x 64 results a CTA of 256 threads, 4 x 4 a thread, 16 terms at a time;
 // it is bound by the multiply-adds.
 #include <algorithm>
 
@@ -16,9 +18,10 @@ enum Mode { FORWARD, PARTIALS, INPUT_GRAD, WEIGHT_GRAD };
 constexpr int TILE = 64, TERMS = 16;
 
 // Results [m][n] = sum_k A[m][k] B[k][n]; two products side by side (FORWARD, PARTIALS) or one.
-template <typename T, int MODE>
-__global__ void __launch_bounds__(256) simple_kernel(const GatedArgs p, int64_t row_tiles) {
-  using A = typename Acc<T>::type;
+template <int MODE>
+__global__ void __launch_bounds__(256) double_kernel(const GatedArgs p, int64_t row_tiles) {
+  using T = double;
+  using A = double;
   constexpr bool DUAL = MODE == FORWARD || MODE == PARTIALS;
   __shared__ A sa[TERMS][TILE + 1], sb[DUAL ? 2 : 1][TERMS][TILE + 1];
   const int tid = threadIdx.x, tm = tid / 16, tn = tid % 16;
@@ -112,48 +115,55 @@ __global__ void __launch_bounds__(256) simple_kernel(const GatedArgs p, int64_t 
 
 // dW = the sum over the parts of the rows, in their order
 template <typename T>
-__global__ void __launch_bounds__(256) sum_parts_kernel(const typename Acc<T>::type* __restrict__ parts, T* __restrict__ dw, int64_t size, int splits) {
+__global__ void __launch_bounds__(256) sum_parts_kernel(const typename Acc<T>::type* __restrict__ parts, T* __restrict__ dw, int rows, int f, int pitch,
+                                                        int splits) {
   using A = typename Acc<T>::type;
+  const int64_t size = (int64_t)rows * f, part = (int64_t)rows * pitch;
   for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < size; i += (int64_t)gridDim.x * blockDim.x) {
+    const int row = (int)(i / f);
+    const A* from = parts + (int64_t)row * pitch + (i - (int64_t)row * f);
     A sum = A(0);
 #pragma unroll 8
-    for (int s = 0; s < splits; ++s) sum += parts[s * size + i];
+    for (int s = 0; s < splits; ++s) sum += from[s * part];
     dw[i] = static_cast<T>(sum);
   }
 }
-
-template <typename T, int MODE> int run_simple(const GatedArgs& p, cudaStream_t s) {
-  const int64_t tiles = ceil_div(p.n, TILE);
-  dim3 grid((unsigned)std::min<int64_t>(tiles, 1 << 20), (unsigned)ceil_div(MODE == INPUT_GRAD ? p.c : p.f, TILE));
-  if (MODE == WEIGHT_GRAD) grid = dim3((unsigned)ceil_div(p.c, TILE), grid.y, (unsigned)(2 * p.splits));
-  simple_kernel<T, MODE><<<grid, 256, 0, s>>>(p, MODE == WEIGHT_GRAD ? 1 : tiles);
-  return check_launch("gated_simple");
-}
-template <typename T> int backward_simple(const GatedArgs& p, cudaStream_t s) {
-  if (int rc = run_simple<T, PARTIALS>(p, s)) return rc;
-  if (p.dx)
-    if (int rc = run_simple<T, INPUT_GRAD>(p, s)) return rc;
-  return p.dw ? run_simple<T, WEIGHT_GRAD>(p, s) : EQT_OK;
-}
-
-}  // namespace
-
-int simple_forward(int dtype, const GatedArgs& p, cudaStream_t s) {
-  return dtype == EQT_F64 ? run_simple<double, FORWARD>(p, s) : dtype == EQT_F32 ? run_simple<float, FORWARD>(p, s) : run_simple<__nv_bfloat16, FORWARD>(p, s);
-}
-int simple_backward(int dtype, const GatedArgs& p, cudaStream_t s) {
-  return dtype == EQT_F64 ? backward_simple<double>(p, s) : dtype == EQT_F32 ? backward_simple<float>(p, s) : backward_simple<__nv_bfloat16>(p, s);
-}
-int sum_parts(int dtype, const GatedArgs& p, cudaStream_t s) {
-  const int64_t size = 2 * (int64_t)p.c * p.f;
-  const unsigned grid = flat_grid(size, 256, 8);
-  if (dtype == EQT_F64) sum_parts_kernel<double><<<grid, 256, 0, s>>>(static_cast<const double*>(p.parts), static_cast<double*>(p.dw), size, p.splits);
-  else if (dtype == EQT_F32) sum_parts_kernel<float><<<grid, 256, 0, s>>>(static_cast<const float*>(p.parts), static_cast<float*>(p.dw), size, p.splits);
-  else sum_parts_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(static_cast<const float*>(p.parts), static_cast<__nv_bfloat16*>(p.dw), size, p.splits);
+template <typename T> int sum_parts(const GatedArgs& p, cudaStream_t s) {
+  sum_parts_kernel<T><<<flat_grid(2 * (int64_t)p.c * p.f, 256, 8), 256, 0, s>>>(static_cast<const typename Acc<T>::type*>(p.parts), static_cast<T*>(p.dw),
+                                                                                 2 * p.c, p.f, p.d_pitch, p.splits);
   return check_launch("gated_sum_parts");
 }
 
-namespace {
+// rows of `cols` values to rows of `pitch`; what lies between is not read
+template <typename T>
+__global__ void __launch_bounds__(256) widen_kernel(const T* __restrict__ from, T* __restrict__ to, int64_t rows, int cols, int pitch) {
+  const int64_t size = rows * cols;
+#pragma unroll 4
+  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < size; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t row = size <= UINT32_MAX ? (unsigned)i / (unsigned)cols : i / cols;
+    to[row * pitch + (i - row * cols)] = from[i];
+  }
+}
+int widen(int dtype, const void* from, void* to, int64_t rows, int cols, int pitch, cudaStream_t s) {
+  const unsigned grid = flat_grid(ceil_div(rows * cols, 4), 256);
+  if (dtype == EQT_F32) widen_kernel<<<grid, 256, 0, s>>>(static_cast<const float*>(from), static_cast<float*>(to), rows, cols, pitch);
+  else widen_kernel<<<grid, 256, 0, s>>>(static_cast<const uint16_t*>(from), static_cast<uint16_t*>(to), rows, cols, pitch);
+  return check_launch("gated_widen");
+}
+
+template <int MODE> int run_double(const GatedArgs& p, cudaStream_t s) {
+  const int64_t tiles = ceil_div(p.n, TILE);
+  dim3 grid((unsigned)std::min<int64_t>(tiles, 1 << 20), (unsigned)ceil_div(MODE == INPUT_GRAD ? p.c : p.f, TILE));
+  if (MODE == WEIGHT_GRAD) grid = dim3((unsigned)ceil_div(p.c, TILE), grid.y, (unsigned)(2 * p.splits));
+  double_kernel<MODE><<<grid, 256, 0, s>>>(p, MODE == WEIGHT_GRAD ? 1 : tiles);
+  return check_launch("gated_double");
+}
+int backward_double(const GatedArgs& p, cudaStream_t s) {
+  if (int rc = run_double<PARTIALS>(p, s)) return rc;
+  if (p.dx)
+    if (int rc = run_double<INPUT_GRAD>(p, s)) return rc;
+  return p.dw ? run_double<WEIGHT_GRAD>(p, s) : EQT_OK;
+}
 
 int size_of(int dtype) { return dtype == EQT_F64 ? 8 : dtype == EQT_F32 ? 4 : 2; }
 
@@ -163,13 +173,6 @@ int check_sizes(int dtype, int64_t n, int64_t c, int64_t f, int act) {
   if (n < 0 || c < 0 || f < 0) return fail(EQT_ERR_BAD_ARGUMENT, "gated: negative size");
   if (n > INT32_MAX - 128 || c > 1 << 20 || f > 1 << 20) return fail(EQT_ERR_UNSUPPORTED, "gated: at most 2^31 rows and 2^20 channels");
   return EQT_OK;
-}
-
-// Whether the tensor memory accelerator can copy tiles of every operand: rows on 16-byte boundaries.
-bool aligned(int dtype, int64_t c, int64_t f, std::initializer_list<const void*> pointers) {
-  uintptr_t bits = (uintptr_t)(c * size_of(dtype)) | (uintptr_t)(f * size_of(dtype));
-  for (const void* p : pointers) bits |= reinterpret_cast<uintptr_t>(p);
-  return dtype != EQT_F64 && bits % 16 == 0;
 }
 
 // Rows are summed in parts so that the tiles of the weights' gradient fill the SMs evenly: as many parts as make the longest SM's work
@@ -186,6 +189,46 @@ void split_rows(GatedArgs& p, int dtype, int64_t n, int64_t c, int64_t f) {
 
 size_t up(size_t b) { return (b + 1023) / 1024 * 1024; }
 
+// Scratch: x and W with wider rows where theirs do not start on 16-byte boundaries, and for the backward pass da, du and the parts.
+struct Scratch { size_t x, w, d, parts, bytes; };
+Scratch lay_out(GatedArgs& p, int dtype, int64_t n, int64_t c, int64_t f, bool backward) {
+  const size_t size = size_of(dtype);
+  const int group = dtype == EQT_F64 ? 1 : (int)(16 / size);
+  auto wide = [&](int64_t v) { return (int)(ceil_div(v, group) * group); };
+  p.x_pitch = wide(c);
+  p.w_pitch = p.d_pitch = wide(f);
+  Scratch s{};
+  s.w = p.x_pitch == c ? 0 : up((size_t)n * p.x_pitch * size);
+  s.d = s.w + (p.w_pitch == f ? 0 : up((size_t)2 * c * p.w_pitch * size));
+  s.parts = s.bytes = s.d;
+  if (backward) {
+    split_rows(p, dtype, n, c, f);
+    s.parts = s.d + up((size_t)2 * n * p.d_pitch * size);
+    s.bytes = s.parts + (size_t)p.splits * 2 * c * p.d_pitch * (dtype == EQT_F64 ? 8 : 4);
+  }
+  return s;
+}
+
+// Puts x and W of the right pitch into p.
+int widen_operands(GatedArgs& p, int dtype, const Scratch& at, void* scratch, cudaStream_t s) {
+  unsigned char* base = static_cast<unsigned char*>(scratch);
+  if (p.x_pitch != p.c) {
+    if (int rc = widen(dtype, p.x, base + at.x, p.n, p.c, p.x_pitch, s)) return rc;
+    p.x = base + at.x;
+  }
+  if (p.w_pitch != p.f) {
+    if (int rc = widen(dtype, p.w, base + at.w, 2 * (int64_t)p.c, p.f, p.w_pitch, s)) return rc;
+    p.w = base + at.w;
+  }
+  return EQT_OK;
+}
+
+int check_pointers(int dtype, std::initializer_list<const void*> pointers) {
+  uintptr_t bits = 0;
+  for (const void* p : pointers) bits |= reinterpret_cast<uintptr_t>(p);
+  return dtype == EQT_F64 || bits % 16 == 0 ? EQT_OK : fail(EQT_ERR_BAD_ARGUMENT, "gated: operands must start on 16-byte boundaries");
+}
+
 }  // namespace
 }  // namespace gated
 }  // namespace eqt
@@ -193,23 +236,29 @@ size_t up(size_t b) { return (b + 1023) / 1024 * 1024; }
 using namespace eqt;
 using namespace eqt::gated;
 
-extern "C" int eqt_gated_forward(int32_t dtype, const void* x, const void* w, void* h, int64_t n, int64_t c, int64_t f, int32_t act,
-                                 int32_t* status, void* stream) {
-  if (int rc = check_sizes(dtype, n, c, f, act)) return rc;
-  if (n == 0 || f == 0) return EQT_OK;
-  if (!h || (c && (!x || !w)) || !status) return fail(EQT_ERR_BAD_ARGUMENT, "gated: NULL pointer");
-  GatedArgs p{};
-  p.x = x, p.w = w, p.h = h, p.n = n, p.c = (int)c, p.f = (int)f, p.act = act, p.status = status;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (!c || !aligned(dtype, c, f, {x, w, h})) return simple_forward(dtype, p, s);
-  return dtype == EQT_F32 ? tensor_forward_f32(p, s) : tensor_forward_bf16(p, s);
-}
-
-extern "C" int64_t eqt_gated_backward_scratch(int32_t dtype, int64_t n, int64_t c, int64_t f) {
+extern "C" int64_t eqt_gated_scratch(int32_t dtype, int64_t n, int64_t c, int64_t f, int32_t backward) {
   if (check_sizes(dtype, n, c, f, 0) || n == 0 || f == 0 || c == 0) return 0;
   GatedArgs p{};
-  split_rows(p, dtype, n, c, f);
-  return (int64_t)(up((size_t)2 * n * f * size_of(dtype)) + (size_t)p.splits * 2 * c * f * (dtype == EQT_F64 ? 8 : 4));
+  return (int64_t)lay_out(p, dtype, n, c, f, backward != 0).bytes;
+}
+
+extern "C" int eqt_gated_forward(int32_t dtype, const void* x, const void* w, void* h, void* scratch, int64_t scratch_bytes, int64_t n, int64_t c,
+                                 int64_t f, int32_t act, int32_t* status, void* stream) {
+  if (int rc = check_sizes(dtype, n, c, f, act)) return rc;
+  if (n == 0 || f == 0) return EQT_OK;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (!h) return fail(EQT_ERR_BAD_ARGUMENT, "gated: NULL pointer");
+  if (c == 0) return cudaMemsetAsync(h, 0, (size_t)n * f * size_of(dtype), s) == cudaSuccess ? EQT_OK : fail(EQT_ERR_CUDA, "cudaMemsetAsync failed");
+  GatedArgs p{};
+  const Scratch at = lay_out(p, dtype, n, c, f, false);
+  if (!x || !w || !status || (at.bytes && !scratch)) return fail(EQT_ERR_BAD_ARGUMENT, "gated: NULL pointer");
+  if (scratch_bytes < (int64_t)at.bytes)
+    return fail(EQT_ERR_BAD_ARGUMENT, "gated: %lld bytes of scratch given, %lld needed", (long long)scratch_bytes, (long long)at.bytes);
+  if (int rc = check_pointers(dtype, {x, w, h, scratch})) return rc;
+  p.x = x, p.w = w, p.h = h, p.n = n, p.c = (int)c, p.f = (int)f, p.act = act, p.status = status;
+  if (dtype == EQT_F64) return run_double<FORWARD>(p, s);
+  if (int rc = widen_operands(p, dtype, at, scratch, s)) return rc;
+  return dtype == EQT_F32 ? tensor_forward_f32(p, s) : tensor_forward_bf16(p, s);
 }
 
 extern "C" int eqt_gated_backward(int32_t dtype, const void* x, const void* w, const void* g, void* dx, void* dw, void* scratch,
@@ -222,17 +271,20 @@ extern "C" int eqt_gated_backward(int32_t dtype, const void* x, const void* w, c
     return EQT_OK;
   }
   if (!x || !w || !g || !scratch || !status) return fail(EQT_ERR_BAD_ARGUMENT, "gated backward: NULL pointer");
-  const int64_t need = eqt_gated_backward_scratch(dtype, n, c, f);
-  if (scratch_bytes < need)
-    return fail(EQT_ERR_BAD_ARGUMENT, "gated backward: %lld bytes of scratch given, %lld needed", (long long)scratch_bytes, (long long)need);
   GatedArgs p{};
+  const Scratch at = lay_out(p, dtype, n, c, f, true);
+  if (scratch_bytes < (int64_t)at.bytes)
+    return fail(EQT_ERR_BAD_ARGUMENT, "gated backward: %lld bytes of scratch given, %lld needed", (long long)scratch_bytes, (long long)at.bytes);
+  if (int rc = check_pointers(dtype, {x, w, g, dx, dw, scratch})) return rc;
   p.x = x, p.w = w, p.g = g, p.dx = dx, p.dw = dw, p.n = n, p.c = (int)c, p.f = (int)f, p.act = act, p.status = status;
-  split_rows(p, dtype, n, c, f);
-  p.d = scratch;
-  p.parts = static_cast<unsigned char*>(scratch) + up((size_t)2 * n * f * size_of(dtype));
-  const int rc = !aligned(dtype, c, f, {x, w, g, dx, dw, scratch}) ? simple_backward(dtype, p, s)
-                 : dtype == EQT_F32                                ? tensor_backward_f32(p, s)
-                                                                   : tensor_backward_bf16(p, s);
-  if (rc) return rc;
-  return dw ? sum_parts(dtype, p, s) : EQT_OK;
+  p.d = static_cast<unsigned char*>(scratch) + at.d;
+  p.parts = static_cast<unsigned char*>(scratch) + at.parts;
+  if (dtype == EQT_F64) {
+    if (int rc = backward_double(p, s)) return rc;
+    return dw ? sum_parts<double>(p, s) : EQT_OK;
+  }
+  if (int rc = widen_operands(p, dtype, at, scratch, s)) return rc;
+  if (int rc = dtype == EQT_F32 ? tensor_backward_f32(p, s) : tensor_backward_bf16(p, s)) return rc;
+  if (!dw) return EQT_OK;
+  return dtype == EQT_F32 ? sum_parts<float>(p, s) : sum_parts<__nv_bfloat16>(p, s);
 }

@@ -17,6 +17,7 @@ struct GatedArgs {
   void* parts;               // (splits, 2, C, F) of the arithmetic type: sums over parts of the rows
   int64_t n;
   int c, f, act;
+  int x_pitch, w_pitch, d_pitch;    // values between two rows of x, of W, of da, du and the parts
   int splits;
   int64_t split_rows;
   int* status;
@@ -50,13 +51,10 @@ template <typename A> __device__ __forceinline__ Value<A> activate(A a, int act)
   return {a * s, s * (A(1) + a * (A(1) - s))};
 }
 
-int simple_forward(int dtype, const GatedArgs& p, cudaStream_t s);
-int simple_backward(int dtype, const GatedArgs& p, cudaStream_t s);
 int tensor_forward_f32(const GatedArgs& p, cudaStream_t s);         // gated_f32.cu and gated_bf16.cu, which compile side by side
 int tensor_forward_bf16(const GatedArgs& p, cudaStream_t s);
 int tensor_backward_f32(const GatedArgs& p, cudaStream_t s);
 int tensor_backward_bf16(const GatedArgs& p, cudaStream_t s);
-int sum_parts(int dtype, const GatedArgs& p, cudaStream_t s);
 
 }  // namespace gated
 }  // namespace eqt

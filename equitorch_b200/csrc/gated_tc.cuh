@@ -66,12 +66,13 @@ struct alignas(64) Launch {
   CUtensorMap a[2], b[2];                                // WEIGHT_GRAD: a[0] x, b da and du; INPUT_GRAD: a da and du, b W0 and W1
   void *out, *out2;
   const void* g;
-  int64_t rows, out_pitch;                               // rows and columns of the results
+  int64_t rows, out_pitch, g_pitch;                      // rows of the results, values between two of theirs and of g's
   unsigned items;
   int64_t part;                                          // WEIGHT_GRAD: results between two partial ones
   int cols, width;                                       // width: columns a tile (of each half, where there are two)
   int row_tiles, col_tiles, kblocks;                     // kblocks: of one half for INPUT_GRAD, of all rows for WEIGHT_GRAD
   int split_blocks;                                      // WEIGHT_GRAD: k-blocks a part
+  int whole;                                             // rows of the results and of g start on 16-byte boundaries
   int* status;
 };
 
@@ -163,6 +164,23 @@ template <typename T> __device__ __forceinline__ void patch_out(unsigned char* p
     if (line < lines && piece < pieces) *reinterpret_cast<uint4*>(base + line * pitch + piece * 16) = *patch_at<T>(patch, line, piece);
   }
   __syncwarp();
+}
+// The same for rows that start anywhere: a lane is a column.
+template <typename T> __device__ __forceinline__ T* patch_value(unsigned char* patch, int line, int column) {
+  constexpr int GROUP = 16 / (int)sizeof(T);
+  return reinterpret_cast<T*>(patch_at<T>(patch, line, column / GROUP)) + column % GROUP;
+}
+template <typename T> __device__ __forceinline__ void patch_out_any(unsigned char* patch, T* base, int64_t pitch, int lines, int columns, int lane) {
+  __syncwarp();
+#pragma unroll 4
+  for (int line = 0; line < lines; ++line)
+    if (lane < columns) base[line * pitch + lane] = *patch_value<T>(patch, line, lane);
+  __syncwarp();
+}
+template <typename T> __device__ __forceinline__ void patch_in_any(unsigned char* patch, const T* base, int64_t pitch, int lines, int columns, int lane) {
+#pragma unroll 8
+  for (int line = 0; line < 32; ++line)
+    *patch_value<T>(patch, line, lane) = line < lines && lane < columns ? base[line * pitch + lane] : static_cast<T>(0.f);
 }
 template <typename T>
 __device__ __forceinline__ void patch_in(unsigned char* patch, const unsigned char* base, int64_t pitch, int lines, int pieces, int lane) {
@@ -481,8 +499,9 @@ __global__ void __launch_bounds__(threads<T>(), 1) gated_tc_kernel(const __grid_
         const int64_t r = x.row + rank * TILE_M + quarter * 32;
         const int c0 = (share + turn * SHARES) * 32, c = x.col + c0, here = (int)max((int64_t)0, min((int64_t)32, p.rows - r));
         const int valid = c0 < p.width ? max(0, min(32, p.cols - c)) : 0;
-        patch_in<T>(where, reinterpret_cast<const unsigned char*>(static_cast<const T*>(p.g) + (here > 0 && valid > 0 ? r * p.out_pitch + c : 0)), pitch,
-                    here, valid / GROUP, lane);
+        const T* from = static_cast<const T*>(p.g) + (here > 0 && valid > 0 ? r * p.g_pitch + c : 0);
+        if (p.whole) patch_in<T>(where, reinterpret_cast<const unsigned char*>(from), p.g_pitch * (int)sizeof(T), here, valid / GROUP, lane);
+        else patch_in_any<T>(where, from, p.g_pitch, here, valid, lane);
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
@@ -543,7 +562,8 @@ __global__ void __launch_bounds__(threads<T>(), 1) gated_tc_kernel(const __grid_
           if (MODE == INPUT_GRAD || F32) {
             line_put<T>(patch, lane, v);
             T* out = static_cast<T*>(p.out) + at + (MODE == WEIGHT_GRAD ? (t.part * 2 + t.half) * p.part : 0);
-            patch_out<T>(patch, reinterpret_cast<unsigned char*>(out), pitch, lines, valid / GROUP, lane);
+            if (MODE == WEIGHT_GRAD || p.whole) patch_out<T>(patch, reinterpret_cast<unsigned char*>(out), pitch, lines, (valid + GROUP - 1) / GROUP, lane);
+            else patch_out_any<T>(patch, out, p.out_pitch, lines, valid, lane);
           } else {                                                                    // partial results are float32: 16 columns at a time
             float* out = static_cast<float*>(p.out) + at + (t.part * 2 + t.half) * p.part;
 #pragma unroll
@@ -553,7 +573,7 @@ __global__ void __launch_bounds__(threads<T>(), 1) gated_tc_kernel(const __grid_
                 const float x[4] = {v[h * 16 + 4 * c], v[h * 16 + 4 * c + 1], v[h * 16 + 4 * c + 2], v[h * 16 + 4 * c + 3]};
                 *patch_at<T>(patch, lane, c) = to16<float>(x);
               }
-              patch_out<T>(patch, reinterpret_cast<unsigned char*>(out + h * 16), p.out_pitch * 4, lines, min(16, max(0, valid - h * 16)) / 4, lane);
+              patch_out<T>(patch, reinterpret_cast<unsigned char*>(out + h * 16), p.out_pitch * 4, lines, (min(16, max(0, valid - h * 16)) + 3) / 4, lane);
             }
           }
           continue;
@@ -609,7 +629,9 @@ __global__ void __launch_bounds__(threads<T>(), 1) gated_tc_kernel(const __grid_
             if (MODE == PARTIALS && !F32) second[F32 ? 0 : b * (16 / GROUP) + q] = to16<T>(y);
           }
         }
-        patch_out<T>(patch, reinterpret_cast<unsigned char*>(static_cast<T*>(p.out) + at), pitch, lines, valid / GROUP, lane);
+        // da and du have rows of their own, wide enough for the last piece; h lies as it has to
+        if (MODE == PARTIALS || p.whole) patch_out<T>(patch, reinterpret_cast<unsigned char*>(static_cast<T*>(p.out) + at), pitch, lines, (valid + GROUP - 1) / GROUP, lane);
+        else patch_out_any<T>(patch, static_cast<T*>(p.out) + at, p.out_pitch, lines, valid, lane);
         if (MODE == PARTIALS) {
           if constexpr (F32) {
             line_put<T>(patch, lane, sum[1]);
@@ -617,7 +639,7 @@ __global__ void __launch_bounds__(threads<T>(), 1) gated_tc_kernel(const __grid_
 #pragma unroll
             for (int c = 0; c < 4; ++c) *patch_at<T>(patch, lane, c) = second[c];
           }
-          patch_out<T>(patch, reinterpret_cast<unsigned char*>(static_cast<T*>(p.out2) + at), pitch, lines, valid / GROUP, lane);
+          patch_out<T>(patch, reinterpret_cast<unsigned char*>(static_cast<T*>(p.out2) + at), pitch, lines, (valid + GROUP - 1) / GROUP, lane);
           unsigned char* t0 = patch;
           patch = other;
           other = t0;
@@ -654,14 +676,14 @@ __global__ void __launch_bounds__(threads<T>(), 1) gated_tc_kernel(const __grid_
 }
 
 // ---- host side ----------------------------------------------------------------------------------
-// A (rows, columns) matrix, columns next to each other, in boxes of `line` columns by `lines` rows.
+// A (rows, columns) matrix, columns next to each other, rows `pitch` values apart, in boxes of `line` columns by `lines` rows.
 template <typename T>
-int map_of(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int line, int lines, bool swizzle) {
+int map_of(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t pitch, int line, int lines, bool swizzle) {
   EncodeTiledFn enc = encode_tiled();
   if (!enc) return fail(EQT_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
   int dev = 0;                                           // the encoder needs a current context (see make_map)
   if (cudaGetDevice(&dev) == cudaSuccess) cudaSetDevice(dev);
-  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)cols * sizeof(T)};
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)pitch * sizeof(T)};
   const cuuint32_t box[2] = {(cuuint32_t)line, (cuuint32_t)lines}, ones[2] = {1, 1};
   const CUresult r = enc(map, sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims,
                          strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
@@ -688,8 +710,8 @@ template <typename T, int MODE, int SHAPE, int ACT> int launch_form(const GatedA
   constexpr bool DUAL = MODE == FORWARD || MODE == PARTIALS, F32 = sizeof(T) == 4;
   const size_t size = sizeof(T);
   const char *w = static_cast<const char*>(a.w), *d = static_cast<const char*>(a.d);
-  const char* w1 = w + (size_t)a.c * a.f * size;
-  const char* d1 = d ? d + (size_t)a.n * a.f * size : nullptr;
+  const char* w1 = w + (size_t)a.c * a.w_pitch * size;
+  const char* d1 = d ? d + (size_t)a.n * a.d_pitch * size : nullptr;
   Launch p{};
   int rc = EQT_OK;
   // Operands that lie along the rows come in boxes of one line of values by a k-block; for float32 they are turned on the way and
@@ -697,32 +719,34 @@ template <typename T, int MODE, int SHAPE, int ACT> int launch_form(const GatedA
   if (DUAL) {
     p.cols = a.f, p.rows = a.n, p.kblocks = (int)ceil_div(a.c, S::BK);
     p.width = width_of(a.f, S::COLS / 2, LINE, !TWO, ceil_div(a.n, ROWS));
-    rc = map_of<T>(&p.a[0], a.x, a.n, a.c, LINE, TILE_M, true);
-    if (!rc) rc = map_of<T>(&p.b[0], w, a.c, a.f, LINE, S::BK, !F32);
-    if (!rc) rc = map_of<T>(&p.b[1], w1, a.c, a.f, LINE, S::BK, !F32);
+    rc = map_of<T>(&p.a[0], a.x, a.n, a.c, a.x_pitch, LINE, TILE_M, true);
+    if (!rc) rc = map_of<T>(&p.b[0], w, a.c, a.f, a.w_pitch, LINE, S::BK, !F32);
+    if (!rc) rc = map_of<T>(&p.b[1], w1, a.c, a.f, a.w_pitch, LINE, S::BK, !F32);
     p.out = MODE == FORWARD ? a.h : a.d;
     p.out2 = const_cast<char*>(d1);
     p.g = a.g;
   } else if (MODE == INPUT_GRAD) {
     p.cols = a.c, p.rows = a.n, p.kblocks = (int)ceil_div(a.f, S::BK);
     p.width = width_of(a.c, S::COLS, LINE, !TWO, ceil_div(a.n, ROWS));
-    rc = map_of<T>(&p.a[0], d, a.n, a.f, LINE, TILE_M, true);
-    if (!rc) rc = map_of<T>(&p.a[1], d1, a.n, a.f, LINE, TILE_M, true);
-    if (!rc) rc = map_of<T>(&p.b[0], w, a.c, a.f, LINE, TWO ? p.width / 2 : p.width, true);
-    if (!rc) rc = map_of<T>(&p.b[1], w1, a.c, a.f, LINE, TWO ? p.width / 2 : p.width, true);
+    rc = map_of<T>(&p.a[0], d, a.n, a.f, a.d_pitch, LINE, TILE_M, true);
+    if (!rc) rc = map_of<T>(&p.a[1], d1, a.n, a.f, a.d_pitch, LINE, TILE_M, true);
+    if (!rc) rc = map_of<T>(&p.b[0], w, a.c, a.f, a.w_pitch, LINE, TWO ? p.width / 2 : p.width, true);
+    if (!rc) rc = map_of<T>(&p.b[1], w1, a.c, a.f, a.w_pitch, LINE, TWO ? p.width / 2 : p.width, true);
     p.out = a.dx;
   } else {
     p.cols = a.f, p.rows = a.c, p.kblocks = (int)ceil_div(a.n, S::BK);
     p.width = width_of(a.f, S::COLS, TWO ? 2 * LINE : LINE, !TWO, 2 * a.splits * ceil_div(a.c, ROWS));    // a pair halves it
     p.split_blocks = (int)(a.split_rows / S::BK);
-    p.part = (int64_t)a.c * a.f;
-    rc = map_of<T>(&p.a[0], a.x, a.n, a.c, LINE, S::BK, !F32);
-    if (!rc) rc = map_of<T>(&p.b[0], d, a.n, a.f, LINE, S::BK, !F32);
-    if (!rc) rc = map_of<T>(&p.b[1], d1, a.n, a.f, LINE, S::BK, !F32);
+    p.part = (int64_t)a.c * a.d_pitch;
+    rc = map_of<T>(&p.a[0], a.x, a.n, a.c, a.x_pitch, LINE, S::BK, !F32);
+    if (!rc) rc = map_of<T>(&p.b[0], d, a.n, a.f, a.d_pitch, LINE, S::BK, !F32);
+    if (!rc) rc = map_of<T>(&p.b[1], d1, a.n, a.f, a.d_pitch, LINE, S::BK, !F32);
     p.out = a.parts;
   }
   if (rc) return rc;
-  p.out_pitch = p.cols;
+  p.out_pitch = MODE == PARTIALS || MODE == WEIGHT_GRAD ? a.d_pitch : p.cols;
+  p.g_pitch = a.f;
+  p.whole = p.cols * sizeof(T) % 16 == 0;
   p.row_tiles = (int)ceil_div(p.rows, ROWS);
   p.col_tiles = (int)ceil_div(p.cols, p.width);
   const int64_t items = (int64_t)p.row_tiles * p.col_tiles * (MODE == WEIGHT_GRAD ? 2 * a.splits : 1);

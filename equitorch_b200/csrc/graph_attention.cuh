@@ -345,7 +345,7 @@ __device__ __forceinline__ void load_rows(T* dst, const Operand& x, const Piece<
 template <typename T, int DP>
 __device__ __forceinline__ void store_rows(T* buf, void* out, const float (&o)[DP / 8][4], float f0, float f1, int first, int end, int head,
                                            const AttentionParams& p, int lane) {
-  constexpr int LD = Row<T, DP>::LD, V = 16 / (int)sizeof(T);
+  constexpr int LD = Row<T, DP>::LD;
   const int g = lane >> 2, t = lane & 3;
   __syncwarp();
 #pragma unroll
@@ -872,8 +872,10 @@ int launch(Pass pass, const AttentionParams& p, int64_t tiles, bool geo, cudaStr
 
 template <typename T, int DP>
 int launch_rows(Pass pass, const AttentionParams& p, int64_t tiles, int tile_rows, bool geo, cudaStream_t s) {
-  constexpr int KF = sizeof(T) == 2 && DP <= 64 ? 64 : 32;               // wide heads, float32 and the backward pass need the registers
-  if (tile_rows == 64) return launch<T, DP, 4, KF, 32>(pass, p, tiles, geo, s);
+  // Wide heads, float32 and the backward pass need the registers; float32's backward pass also the shared memory (48 graphs of 40 to
+  // 250 nodes, heads of 72 values: by rows 184 us with 32, 170 with 16, by columns the same).
+  constexpr int KF = sizeof(T) == 2 && DP <= 64 ? 64 : 32, KB = sizeof(T) == 2 ? 32 : 16;
+  if (tile_rows == 64) return launch<T, DP, 4, KF, KB>(pass, p, tiles, geo, s);
   if (tile_rows == 32) return launch<T, DP, 2, 32, 32>(pass, p, tiles, geo, s);
   return launch<T, DP, 1, 16, 16>(pass, p, tiles, geo, s);
 }

@@ -37,10 +37,12 @@ def gated_forward(x: Tensor, weight: Tensor, activation: str) -> Tensor:
     c, f = weight.shape[1:]
     h = torch.empty(*x.shape[:-1], f, dtype=x.dtype, device=dev)
     n = h.numel() // f if f else 0
+    code, lib = _lib.DTYPE_CODE[x.dtype], _lib.lib()
     with _lib.on_device(dev):
-        _lib.check(_lib.lib().eqt_gated_forward(_lib.DTYPE_CODE[x.dtype], x.data_ptr(), weight.data_ptr(), h.data_ptr(), n, c, f,
-                                                ACTIVATIONS[activation], status_flag(dev).data_ptr(), _lib.stream_ptr(dev)),
-                   "eqt_gated_forward")
+        size = lib.eqt_gated_scratch(code, n, c, f, 0)
+        scratch = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+        _lib.check(lib.eqt_gated_forward(code, x.data_ptr(), weight.data_ptr(), h.data_ptr(), _lib.ptr(scratch), size, n, c, f,
+                                         ACTIVATIONS[activation], status_flag(dev).data_ptr(), _lib.stream_ptr(dev)), "eqt_gated_forward")
     return h
 
 
@@ -54,7 +56,7 @@ def gated_backward(grad: Tensor, x: Tensor, weight: Tensor, activation: str, wan
     dw = torch.empty_like(weight) if want_weight else None
     code, lib = _lib.DTYPE_CODE[x.dtype], _lib.lib()
     with _lib.on_device(dev):
-        size = lib.eqt_gated_backward_scratch(code, n, c, f)
+        size = lib.eqt_gated_scratch(code, n, c, f, 1)
         scratch = torch.empty(size, dtype=torch.uint8, device=dev)
         _lib.check(lib.eqt_gated_backward(code, x.data_ptr(), weight.data_ptr(), grad.data_ptr(), _lib.ptr(dx), _lib.ptr(dw),
                                           scratch.data_ptr(), size, n, c, f, ACTIVATIONS[activation], status_flag(dev).data_ptr(),

@@ -696,14 +696,15 @@ int eqt_pack_graphs_tiles(const int64_t* ptr, int64_t graphs, int32_t* tiles, in
 /*
  * Gated linear layer: h (n, f) = act(x W0) * (x W1) for x (n, c) and w (2, c, f), contiguous.  Backward, from g = dL/dh: dx (n, c)
  * and dw (2, c, f), either may be NULL; both products are formed again, nothing of the forward pass is kept.  All in one dtype, sums
- * in float (double for EQT_F64); da and du are rounded to the dtype between the kernels.  float32 and bfloat16 with rows and pointers on
- * 16-byte boundaries run on the tensor cores (float32 as three TF32 products), everything else on the ordinary units.  `scratch`:
- * eqt_gated_backward_scratch bytes, 16-byte aligned.  `status` (int32 on the device) is raised where a bounded wait gave up.
+ * in float (double for EQT_F64); da and du are rounded to the dtype between the kernels.  float32 (as three TF32 products) and bfloat16
+ * run on the tensor cores and their pointers lie on 16-byte boundaries; rows whose length is no multiple of 16 bytes are copied to wider
+ * ones first.  `scratch`: eqt_gated_scratch bytes, 16-byte aligned (0: none needed).  `status` (int32 on the device) is raised where a
+ * bounded wait gave up.
  */
 enum eqt_activation { EQT_ACT_SILU = 0, EQT_ACT_GELU = 1, EQT_ACT_RELU = 2, EQT_ACT_SIGMOID = 3 };
-int eqt_gated_forward(int32_t dtype, const void* x, const void* w, void* h, int64_t n, int64_t c, int64_t f, int32_t act,
-                      int32_t* status, void* stream);
-int64_t eqt_gated_backward_scratch(int32_t dtype, int64_t n, int64_t c, int64_t f);
+int64_t eqt_gated_scratch(int32_t dtype, int64_t n, int64_t c, int64_t f, int32_t backward);
+int eqt_gated_forward(int32_t dtype, const void* x, const void* w, void* h, void* scratch, int64_t scratch_bytes, int64_t n, int64_t c,
+                      int64_t f, int32_t act, int32_t* status, void* stream);
 int eqt_gated_backward(int32_t dtype, const void* x, const void* w, const void* g, void* dx, void* dw, void* scratch,
                        int64_t scratch_bytes, int64_t n, int64_t c, int64_t f, int32_t act, int32_t* status, void* stream);
 

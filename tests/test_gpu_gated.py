@@ -73,7 +73,7 @@ def test_tensor_cores(rows, c, f, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float64])
-@pytest.mark.parametrize("rows,c,f", [(1, 1, 1), (65, 17, 33), (700, 31, 90), (3001, 7, 65)])
+@pytest.mark.parametrize("rows,c,f", [(1, 1, 1), (65, 17, 33), (700, 31, 90), (3001, 7, 65), (20011, 100, 301), (300, 515, 70)])
 def test_odd_sizes(rows, c, f, dtype):
     _check(*_inputs(rows, c, f, dtype), "silu")
 
