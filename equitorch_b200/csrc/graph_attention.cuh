@@ -318,26 +318,39 @@ template <typename T, int DP, int TH> struct Piece {
   }
 };
 
-// Rows [first, first + ROWS_TILE) of one head to shared memory, zeros from `end` on.
+// Where a thread's pieces of an operand's rows begin, moved on from tile to tile by additions.
+template <typename T, int DP, int TH> struct Source {
+  const T* at;
+  int64_t step;              // between the rows that the thread copies
+  __device__ __forceinline__ Source(const Operand& x, const Piece<T, DP, TH>& piece, int first, int head, const AttentionParams& p)
+      : at(static_cast<const T*>(x.p) + (int64_t)(first + piece.row) * x.node + piece.comp * x.comp + (int64_t)head * p.size + piece.channel),
+        step(x.node * Piece<T, DP, TH>::ROWS) {}
+};
+
+// The next ROWS_TILE rows of one head to shared memory, zeros from the `left`-th on; `first` is the row of the first.
 template <typename T, int DP, int TH, int ROWS_TILE>
-__device__ __forceinline__ void load_rows(T* dst, const Operand& x, const Piece<T, DP, TH>& piece, int first, int end, int head,
+__device__ __forceinline__ void load_rows(T* dst, Source<T, DP, TH>& source, const Operand& x, const Piece<T, DP, TH>& piece, int first, int left, int head,
                                           const AttentionParams& p, int tid) {
-  constexpr int LD = Row<T, DP>::LD;
+  constexpr int LD = Row<T, DP>::LD, ROWS = Piece<T, DP, TH>::ROWS;
   if (p.vec) {
-    if (!piece.there) return;
-    const T* src = static_cast<const T*>(x.p) + piece.comp * x.comp + (int64_t)head * p.size + piece.channel;
+    if (piece.there) {
+      T* to = dst + piece.row * LD + piece.at;
+      const T* from = source.at;
 #pragma unroll
-    for (int r = piece.row; r < ROWS_TILE; r += Piece<T, DP, TH>::ROWS) {
-      const bool there = first + r < end;
-      copy16(dst + r * LD + piece.at, src + (int64_t)(there ? first + r : 0) * x.node, there);
+      for (int r = 0; r < ROWS_TILE; r += ROWS, from += source.step) {
+        if (ROWS_TILE % ROWS && r + piece.row >= ROWS_TILE) break;
+        const bool there = r + piece.row < left;
+        copy16(to + r * LD, there ? from : static_cast<const T*>(x.p), there);
+      }
     }
+    source.at += x.node * ROWS_TILE;
     return;
   }
   const int d = p.comps * p.size;
   for (int i = tid; i < ROWS_TILE * d; i += TH) {
     const int r = i / d, j = i - r * d, m = j / p.size, c = j - m * p.size;
-    dst[r * LD + j] = first + r < end ? static_cast<const T*>(x.p)[(int64_t)(first + r) * x.node + m * x.comp + (int64_t)head * p.size + c]
-                                      : static_cast<T>(0.f);
+    dst[r * LD + j] = r < left ? static_cast<const T*>(x.p)[(int64_t)(first + r) * x.node + m * x.comp + (int64_t)head * p.size + c]
+                               : static_cast<T>(0.f);
   }
 }
 
@@ -454,13 +467,18 @@ __global__ void __launch_bounds__(THREADS, DP <= 32 ? 6 : DP <= 64 ? 4 : 3) atte
     __syncthreads();
   }
   const Piece<T, DP, S::TH> piece(ht, p.comps, p.size);
+  Source<T, DP, S::TH> from_k(p.k, piece, lo, head, p), from_v(p.v, piece, lo, head, p);
   auto fetch = [&](int key, int s) {
-    load_rows<T, DP, S::TH, KT>(stage + s * S::STAGE, p.k, piece, key, end, head, p, ht);
-    load_rows<T, DP, S::TH, KT>(stage + s * S::STAGE + KT * LD, p.v, piece, key, end, head, p, ht);
+    load_rows<T, DP, S::TH, KT>(stage + s * S::STAGE, from_k, p.k, piece, key, end - key, head, p, ht);
+    load_rows<T, DP, S::TH, KT>(stage + s * S::STAGE + KT * LD, from_v, p.v, piece, key, end - key, head, p, ht);
     if (p.pos) load_positions<KT>(spos + s * 3 * KT, p.pos, key, hi);
     copies_commit();
   };
-  load_rows<T, DP, S::TH, S::TILE>(rows, p.q, piece, first, end, head, p, ht);
+  auto load_tile = [&](T* dst, const Operand& x) {       // the CTA's own rows
+    Source<T, DP, S::TH> from(x, piece, first, head, p);
+    load_rows<T, DP, S::TH, S::TILE>(dst, from, x, piece, first, end - first, head, p, ht);
+  };
+  load_tile(rows, p.q);
   fetch(lo, 0);
 
   const int row = first + (warp % WR) * 16;                              // of the warp
@@ -584,14 +602,19 @@ __global__ void __launch_bounds__(THREADS, DP <= 32 ? 4 : DP <= 96 ? 3 : 2) atte
     __syncthreads();
   }
   const Piece<T, DP, S::TH> piece(ht, p.comps, p.size);
+  Source<T, DP, S::TH> from_k(p.k, piece, lo, head, p), from_v(p.v, piece, lo, head, p);
   auto fetch = [&](int key, int s) {
-    load_rows<T, DP, S::TH, KT>(stage + s * S::STAGE, p.k, piece, key, end, head, p, ht);
-    load_rows<T, DP, S::TH, KT>(stage + s * S::STAGE + KT * LD, p.v, piece, key, end, head, p, ht);
+    load_rows<T, DP, S::TH, KT>(stage + s * S::STAGE, from_k, p.k, piece, key, end - key, head, p, ht);
+    load_rows<T, DP, S::TH, KT>(stage + s * S::STAGE + KT * LD, from_v, p.v, piece, key, end - key, head, p, ht);
     if (p.pos) load_positions<KT>(spos + s * 3 * KT, p.pos, key, hi);
     copies_commit();
   };
-  load_rows<T, DP, S::TH, S::TILE>(rows, p.q, piece, first, end, head, p, ht);
-  load_rows<T, DP, S::TH, S::TILE>(grads, p.g, piece, first, end, head, p, ht);
+  auto load_tile = [&](T* dst, const Operand& x) {       // the CTA's own rows
+    Source<T, DP, S::TH> from(x, piece, first, head, p);
+    load_rows<T, DP, S::TH, S::TILE>(dst, from, x, piece, first, end - first, head, p, ht);
+  };
+  load_tile(rows, p.q);
+  load_tile(grads, p.g);
   copies_commit();
   fetch(lo, 0);
   copies_wait<1>();
@@ -735,9 +758,10 @@ __global__ void __launch_bounds__(THREADS, DP <= 32 ? 4 : DP <= 64 ? 3 : 2) atte
     __syncthreads();
   }
   const Piece<T, DP, S::TH> piece(ht, p.comps, p.size);
+  Source<T, DP, S::TH> from_q(p.q, piece, lo, head, p), from_g(p.g, piece, lo, head, p);
   auto fetch = [&](int query, int s) {
-    load_rows<T, DP, S::TH, KT>(stage + s * S::STAGE, p.q, piece, query, end, head, p, ht);
-    load_rows<T, DP, S::TH, KT>(stage + s * S::STAGE + KT * LD, p.g, piece, query, end, head, p, ht);
+    load_rows<T, DP, S::TH, KT>(stage + s * S::STAGE, from_q, p.q, piece, query, end - query, head, p, ht);
+    load_rows<T, DP, S::TH, KT>(stage + s * S::STAGE + KT * LD, from_g, p.g, piece, query, end - query, head, p, ht);
     for (int i = ht; i < KT; i += S::TH) {
       const bool there = query + i < end;
       const int64_t at = there ? (int64_t)head * p.n + query + i : 0;
@@ -747,8 +771,12 @@ __global__ void __launch_bounds__(THREADS, DP <= 32 ? 4 : DP <= 64 ? 3 : 2) atte
     if (p.pos) load_positions<KT>(spos + s * 3 * KT, p.pos, query, hi);
     copies_commit();
   };
-  load_rows<T, DP, S::TH, S::TILE>(keys, p.k, piece, first, end, head, p, ht);
-  load_rows<T, DP, S::TH, S::TILE>(values, p.v, piece, first, end, head, p, ht);
+  auto load_tile = [&](T* dst, const Operand& x) {       // the CTA's own rows
+    Source<T, DP, S::TH> from(x, piece, first, head, p);
+    load_rows<T, DP, S::TH, S::TILE>(dst, from, x, piece, first, end - first, head, p, ht);
+  };
+  load_tile(keys, p.k);
+  load_tile(values, p.v);
   fetch(lo, 0);
 
   const int row = first + (warp % WR) * 16;
