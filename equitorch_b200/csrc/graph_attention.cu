@@ -6,13 +6,14 @@ namespace {
 using namespace attention;
 
 // Geometry over the heads: the first `heads` CTAs sum a head's slope gradient in a fixed order, the others the positions' gradients.
-constexpr int GEO_THREADS = 512;
+constexpr int GEO_THREADS = 1024;
 __global__ void __launch_bounds__(GEO_THREADS) attention_geometry_kernel(const float4* __restrict__ row, const float4* __restrict__ col,
                                                                          const float* __restrict__ slope, float* __restrict__ dslope,
                                                                          float* __restrict__ dpos, int64_t n, int heads) {
   if (blockIdx.x < heads) {
     __shared__ double part[GEO_THREADS / 32];
     double sum = 0.0;
+#pragma unroll 8
     for (int64_t i = threadIdx.x; i < n; i += GEO_THREADS) sum += row[(int64_t)blockIdx.x * n + i].x;
     for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = sum;

@@ -454,8 +454,9 @@ __global__ void __launch_bounds__(THREADS, DP <= 32 ? 6 : DP <= 64 ? 4 : 3) atte
   extern __shared__ __align__(16) unsigned char smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int slot = warp / WR, ht = tid - slot * S::TH;                   // the head's place in the CTA, the thread's place in the head
-  const int head = blockIdx.y * S::HEADS + slot;
-  const int4 tile = p.tiles[blockIdx.x];
+  const unsigned groups = (p.heads + S::HEADS - 1) / S::HEADS;           // all heads of a tile first: the largest graphs' tiles come first
+  const int head = (int)(blockIdx.x % groups) * S::HEADS + slot;
+  const int4 tile = p.tiles[blockIdx.x / groups];
   const int first = tile.x, lo = tile.y, hi = tile.z;
   T* base = reinterpret_cast<T*>(smem) + slot * S::head_elements(1);
   T *rows = base, *stage = base + S::TILE * LD;
@@ -589,8 +590,9 @@ __global__ void __launch_bounds__(THREADS, DP <= 32 ? 4 : DP <= 96 ? 3 : 2) atte
   extern __shared__ __align__(16) unsigned char smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int slot = warp / WR, ht = tid - slot * S::TH;
-  const int head = blockIdx.y * S::HEADS + slot;
-  const int4 tile = p.tiles[blockIdx.x];
+  const unsigned groups = (p.heads + S::HEADS - 1) / S::HEADS;           // all heads of a tile first: the largest graphs' tiles come first
+  const int head = (int)(blockIdx.x % groups) * S::HEADS + slot;
+  const int4 tile = p.tiles[blockIdx.x / groups];
   const int first = tile.x, lo = tile.y, hi = tile.z;
   T* base = reinterpret_cast<T*>(smem) + slot * S::head_elements(2);
   T *rows = base, *grads = base + S::TILE * LD, *stage = base + 2 * S::TILE * LD;
@@ -744,8 +746,9 @@ __global__ void __launch_bounds__(THREADS, DP <= 32 ? 4 : DP <= 64 ? 3 : 2) atte
   extern __shared__ __align__(16) unsigned char smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int slot = warp / WR, ht = tid - slot * S::TH;
-  const int head = blockIdx.y * S::HEADS + slot;
-  const int4 tile = p.tiles[blockIdx.x];
+  const unsigned groups = (p.heads + S::HEADS - 1) / S::HEADS;           // all heads of a tile first: the largest graphs' tiles come first
+  const int head = (int)(blockIdx.x % groups) * S::HEADS + slot;
+  const int4 tile = p.tiles[blockIdx.x / groups];
   const int first = tile.x, lo = tile.y, hi = tile.z;
   T* base = reinterpret_cast<T*>(smem) + slot * S::head_elements(2);
   T *keys = base, *values = base + S::TILE * LD, *stage = base + 2 * S::TILE * LD;
@@ -883,7 +886,9 @@ template <typename T, int DP, int WR, int KF, int KB>
 int launch(Pass pass, const AttentionParams& p, int64_t tiles, bool geo, cudaStream_t s) {
   using F = Shape<T, DP, WR, KF>;
   using B = Shape<T, DP, WR, KB>;
-  const dim3 grid((unsigned)tiles, (unsigned)ceil_div(p.heads, F::HEADS));
+  const int64_t ctas = tiles * ceil_div(p.heads, F::HEADS);
+  if (ctas > INT32_MAX) return fail(EQT_ERR_UNSUPPORTED, "attention: %lld tiles and heads are more than one launch takes", (long long)ctas);
+  const unsigned grid = (unsigned)ctas;
   auto run = [&](auto kernel, size_t bytes, const char* what) {
     if (int rc = allow_shared(kernel, bytes)) return rc;
     kernel<<<grid, THREADS, bytes, s>>>(p);

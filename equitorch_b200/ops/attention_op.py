@@ -84,13 +84,14 @@ def attention_backward(grad: Tensor, q: Tensor, k: Tensor, v: Tensor, graphs: Pa
     pos, slope = (None, None) if pos is None else (pos.contiguous(), slope.contiguous())
     dq, dk, dv = _new(q, graphs), _new(q, graphs), _new(q, graphs)
     args = _args(q, k, v, graphs, heads, scale, cap, pos, slope, out, lse)
-    delta = torch.empty_like(lse)
-    args.grad_out, args.dq, args.dk, args.dv, args.delta = grad.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), delta.data_ptr()
-    dslope = dpos = geo = None
+    args.grad_out, args.dq, args.dk, args.dv = grad.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
+    dslope = dpos = None
+    rows = lse.numel()                                   # of scratch: eight numbers of geometry and one of the softmax's gradient each
+    scratch = (torch.empty if graphs.covers else torch.zeros)(rows * (9 if want_geometry else 1), dtype=torch.float32, device=dev)
+    args.delta = scratch.data_ptr() + 4 * (scratch.numel() - rows)
     if want_geometry:
         dslope, dpos = torch.empty_like(slope), torch.empty_like(pos)
-        geo = (torch.empty if graphs.covers else torch.zeros)(2, heads, q.shape[0], 4, dtype=torch.float32, device=dev)
-        args.geo, args.dpos, args.dslope = geo.data_ptr(), dpos.data_ptr(), dslope.data_ptr()
+        args.geo, args.dpos, args.dslope = scratch.data_ptr(), dpos.data_ptr(), dslope.data_ptr()
     with _lib.on_device(dev):
         _lib.check(_lib.lib().eqt_attention_backward(C.byref(args), _lib.stream_ptr(dev)), "eqt_attention_backward")
     return dq, dk, dv, dslope, dpos
