@@ -31,6 +31,17 @@ template <typename K> inline int allow_shared(K kernel, size_t most) {
   return e == cudaSuccess ? EQT_OK : fail(EQT_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
 }
 
+// The same where every launch of the kernel asks for as much: once for each device, whose bit in `done` says so.
+template <typename K> inline int allow_shared_once(K kernel, size_t most, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return allow_shared(kernel, most);
+  const uint64_t bit = uint64_t(1) << dev;
+  if (done.load(std::memory_order_relaxed) & bit) return EQT_OK;
+  const int rc = allow_shared(kernel, most);
+  if (rc == EQT_OK) done.fetch_or(bit, std::memory_order_relaxed);
+  return rc;
+}
+
 // ---- storage <-> arithmetic types --------------------------------------------------------
 template <typename T> struct Acc { using type = float; };
 template <> struct Acc<double> { using type = double; };

@@ -480,8 +480,8 @@ int run_grad(int dtype, const void* g, const int64_t* index, void* gw, int64_t n
 int check_sizes(int dtype, int64_t n, int64_t types, int64_t width) {
   if (dtype != EQT_F32 && dtype != EQT_F64 && dtype != EQT_BF16) return fail(EQT_ERR_BAD_ARGUMENT, "embedding: unknown dtype %d", dtype);
   if (n < 0 || types < 0 || width < 0) return fail(EQT_ERR_BAD_ARGUMENT, "embedding: negative size");
-  if (n > INT32_MAX - 1 || types > INT32_MAX - 1 || width > INT32_MAX / 16)
-    return fail(EQT_ERR_UNSUPPORTED, "embedding: rows and types are numbered in 32 bits, a row has at most 2^27 values");
+  if (n > INT32_MAX - 1 || types > INT32_MAX - 1 || width > 1 << 20)
+    return fail(EQT_ERR_UNSUPPORTED, "embedding: rows and types are numbered in 32 bits, a row has at most 2^20 values");
   return EQT_OK;
 }
 

@@ -681,8 +681,6 @@ template <typename T>
 int map_of(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t pitch, int line, int lines, bool swizzle) {
   EncodeTiledFn enc = encode_tiled();
   if (!enc) return fail(EQT_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
-  int dev = 0;                                           // the encoder needs a current context (see make_map)
-  if (cudaGetDevice(&dev) == cudaSuccess) cudaSetDevice(dev);
   const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)pitch * sizeof(T)};
   const cuuint32_t box[2] = {(cuuint32_t)line, (cuuint32_t)lines}, ones[2] = {1, 1};
   const CUresult r = enc(map, sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims,
@@ -713,7 +711,8 @@ template <typename T, int MODE, int SHAPE, int ACT> int launch_form(const GatedA
   const char* w1 = w + (size_t)a.c * a.w_pitch * size;
   const char* d1 = d ? d + (size_t)a.n * a.d_pitch * size : nullptr;
   Launch p{};
-  int rc = EQT_OK;
+  int rc = EQT_OK, dev = 0;
+  if (cudaGetDevice(&dev) == cudaSuccess) cudaSetDevice(dev);          // the encoder of the maps needs a current context (see make_map)
   // Operands that lie along the rows come in boxes of one line of values by a k-block; for float32 they are turned on the way and
   // need no swizzle.
   if (DUAL) {
@@ -755,7 +754,8 @@ template <typename T, int MODE, int SHAPE, int ACT> int launch_form(const GatedA
   p.status = a.status;
   const size_t shared = shared_bytes<T, MODE, SHAPE>();
   auto kernel = gated_tc_kernel<T, MODE, ACT, SHAPE>;
-  if (int r = allow_shared(kernel, shared)) return r;
+  static std::atomic<uint64_t> allowed{0};               // this kernel's
+  if (int r = allow_shared_once(kernel, shared, allowed)) return r;
   constexpr int CTAS = TWO ? 2 : 1;
   cudaLaunchConfig_t config{};
   int64_t at_once = std::min<int64_t>(items, tc::sm_count() / CTAS);

@@ -124,7 +124,8 @@ int fill(const eqt_attention_args* a, AttentionParams& p, bool backward) {
     return fail(EQT_ERR_UNSUPPORTED, "attention: nodes and tiles are numbered in 32 bits, heads in 16");
   if ((int64_t)a->comps * a->head_channels > 128)
     return fail(EQT_ERR_UNSUPPORTED, "attention: a head has at most 128 values a node, got %lld", (long long)a->comps * a->head_channels);
-  if (!(a->cap >= 0.f)) return fail(EQT_ERR_BAD_ARGUMENT, "attention: the cap must not be negative");
+  if (a->cap != 0.f && !(a->cap >= 1e-12f && a->cap <= 1e12f)) return fail(EQT_ERR_BAD_ARGUMENT, "attention: the cap must be 0 or from 1e-12 to 1e12");
+  if (!(fabsf(a->scale) <= 1e12f)) return fail(EQT_ERR_BAD_ARGUMENT, "attention: the scale must be at most 1e12");
   if (a->n && (a->pos != nullptr) != (a->slope != nullptr)) return fail(EQT_ERR_BAD_ARGUMENT, "attention: positions and slopes come together");
   if (a->num_tiles && (!a->q || !a->k || !a->v || !a->out || !a->tiles || (backward && (!a->grad_out || !a->lse || !a->dq || !a->dk || !a->dv || !a->delta))))
     return fail(EQT_ERR_BAD_ARGUMENT, "attention: NULL pointer");

@@ -237,8 +237,8 @@ __device__ __forceinline__ float tanh_any(float x) {
   const float small = fmaf(x, w * fmaf(w, fmaf(w, fmaf(w, 0.01724148727953434f, -0.05304549261927605f), 0.13325878977775574f), -0.333331435918808f), x);
   return y <= 0.5f ? small : x == x ? large : x;
 }
-template <int NT> __device__ __forceinline__ void cap_tile(float (&z)[NT][4], float unit, float to_cap) {
-  if (to_cap == 0.f) {
+template <int NT> __device__ __forceinline__ void cap_tile(float (&z)[NT][4], float unit, float to_cap, bool capped) {
+  if (!capped) {
     const pair u = both(unit, unit);
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -249,7 +249,8 @@ template <int NT> __device__ __forceinline__ void cap_tile(float (&z)[NT][4], fl
   float most = 0.f;
 #pragma unroll
   for (int n = 0; n < NT; ++n) most = fmaxf(fmaxf(most, fmaxf(fabsf(z[n][0]), fabsf(z[n][1]))), fmaxf(fabsf(z[n][2]), fabsf(z[n][3])));
-  if (__all_sync(0xffffffffu, most * to_cap <= 0.5f)) {  // the maximum drops NaNs; they stay NaN either way
+  // The maximum drops NaNs; they stay NaN either way.  Above 1e4 the polynomial's coefficients would leave the range of float32.
+  if (fabsf(to_cap) <= 1e4f && __all_sync(0xffffffffu, most * fabsf(to_cap) <= 0.5f)) {
     const float f = to_cap * to_cap;                     // the polynomial's argument is (z to_cap)^2
     const float c0 = -0.333331435918808f * f, c1 = 0.13325878977775574f * f * f, c2 = -0.05304549261927605f * f * f * f, c3 = 0.01724148727953434f * f * f * f * f;
     const pair k0 = both(c0, c0), k1 = both(c1, c1), k2 = both(c2, c2), k3 = both(c3, c3), u = both(unit * to_cap, unit * to_cap);
@@ -510,7 +511,7 @@ __global__ void __launch_bounds__(THREADS, DP <= 32 ? 6 : DP <= 64 ? 4 : 3) atte
       const T *ks = stage + s * S::STAGE, *vs = ks + KT * LD;
       float z[NT][4];
       score_mma<DP, NT>(z, mine, ks, lane);
-      cap_tile<NT>(z, unit, to_cap);
+      cap_tile<NT>(z, unit, to_cap, p.cap > 0.f);
       if (p.pos) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -665,7 +666,7 @@ __global__ void __launch_bounds__(THREADS, DP <= 32 ? 4 : DP <= 96 ? 3 : 2) atte
       float z[NT][4], dp[NT][4];
       score_mma<DP, NT>(z, mq, ks, lane);
       score_mma<DP, NT>(dp, mg, vs, lane);
-      cap_tile<NT>(z, unit, to_cap);
+      cap_tile<NT>(z, unit, to_cap, p.cap > 0.f);
       const bool last = key + KT > hi;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
@@ -701,7 +702,7 @@ __global__ void __launch_bounds__(THREADS, DP <= 32 ? 4 : DP <= 96 ? 3 : 2) atte
             geo[r][2] = fma2(fi, v.y, geo[r][2]);
             geo[r][3] = fma2(fi, v.z, geo[r][3]);
           }
-          parts(mul2(e, fma2(mul2(score0, score0), bend2, scale2)), z[n][2 * r], z[n][2 * r + 1]);
+          parts(mul2(e, fma2(mul2(score0, bend2), score0, scale2)), z[n][2 * r], z[n][2 * r + 1]);
         }
       }
       out_mma<DP, NT>(dq, z, ks, lane);
@@ -818,7 +819,7 @@ __global__ void __launch_bounds__(THREADS, DP <= 32 ? 4 : DP <= 64 ? 3 : 2) atte
       float z[NT][4], dp[NT][4];
       score_mma<DP, NT>(z, mk, qs, lane);
       score_mma<DP, NT>(dp, mv, gs, lane);
-      cap_tile<NT>(z, unit, to_cap);
+      cap_tile<NT>(z, unit, to_cap, p.cap > 0.f);
       const bool last = query + KT > hi;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
@@ -852,7 +853,7 @@ __global__ void __launch_bounds__(THREADS, DP <= 32 ? 4 : DP <= 64 ? 3 : 2) atte
           }
           z[n][2 * r] = x;
           z[n][2 * r + 1] = y;
-          parts(mul2(e, fma2(mul2(score0, score0), bend2, scale2)), dp[n][2 * r], dp[n][2 * r + 1]);
+          parts(fma2(mul2(mul2(score0, bend2), score0), e, mul2(e, scale2)), dp[n][2 * r], dp[n][2 * r + 1]);
         }
       }
       out_mma<DP, NT>(dv, z, gs, lane);
@@ -889,18 +890,19 @@ int launch(Pass pass, const AttentionParams& p, int64_t tiles, bool geo, cudaStr
   const int64_t ctas = tiles * ceil_div(p.heads, F::HEADS);
   if (ctas > INT32_MAX) return fail(EQT_ERR_UNSUPPORTED, "attention: %lld tiles and heads are more than one launch takes", (long long)ctas);
   const unsigned grid = (unsigned)ctas;
-  auto run = [&](auto kernel, size_t bytes, const char* what) {
-    if (int rc = allow_shared(kernel, bytes)) return rc;
+  static std::atomic<uint64_t> allowed[5];                               // of the five kernels below
+  auto run = [&](auto kernel, size_t bytes, const char* what, int which) {
+    if (int rc = allow_shared_once(kernel, bytes, allowed[which])) return rc;
     kernel<<<grid, THREADS, bytes, s>>>(p);
     return check_launch(what);
   };
   constexpr int POSITIONS = 2 * 12 * KB, STATS = B::HEADS * 16 * KB;     // two tiles each
-  if (pass == FORWARD) return run(attention_forward_kernel<T, DP, WR, KF>, F::bytes(1, 2 * 12 * KF), "attention_forward");
+  if (pass == FORWARD) return run(attention_forward_kernel<T, DP, WR, KF>, F::bytes(1, 2 * 12 * KF), "attention_forward", 0);
   if (pass == ROWS)
-    return geo ? run(attention_rows_kernel<T, DP, WR, KB, true>, B::bytes(2, POSITIONS), "attention_rows")
-               : run(attention_rows_kernel<T, DP, WR, KB, false>, B::bytes(2, POSITIONS), "attention_rows");
-  return geo ? run(attention_columns_kernel<T, DP, WR, KB, true>, B::bytes(2, POSITIONS + STATS), "attention_columns")
-             : run(attention_columns_kernel<T, DP, WR, KB, false>, B::bytes(2, POSITIONS + STATS), "attention_columns");
+    return geo ? run(attention_rows_kernel<T, DP, WR, KB, true>, B::bytes(2, POSITIONS), "attention_rows", 1)
+               : run(attention_rows_kernel<T, DP, WR, KB, false>, B::bytes(2, POSITIONS), "attention_rows", 2);
+  return geo ? run(attention_columns_kernel<T, DP, WR, KB, true>, B::bytes(2, POSITIONS + STATS), "attention_columns", 3)
+             : run(attention_columns_kernel<T, DP, WR, KB, false>, B::bytes(2, POSITIONS + STATS), "attention_columns", 4);
 }
 
 template <typename T, int DP>

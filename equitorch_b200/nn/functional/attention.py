@@ -42,13 +42,13 @@ def graph_attention(q: Tensor, k: Tensor, v: Tensor, graphs: PackedGraphs, num_h
     components of its channels, so with features of one sequence of irreps in the basis of this package the scores do not change
     under rotations and the result turns as the features do.
 
-    ``scale``: one over the root of a head's values where not given.  ``cap``: the products, not the distances, are capped; without
-    it they are taken as they are.  ``pos`` (N, 3) and ``slope`` (num_heads,), float32, come together; without them there is no
+    ``scale``: one over the root of a head's values where not given.  ``cap`` (1e-12 to 1e12): the products, not the distances, are capped;
+    without it they are taken as they are.  ``pos`` (N, 3) and ``slope`` (num_heads,), float32, come together; without them there is no
     distance term.  Nodes of no graph get zeros, and graphs do not touch each other, whatever values they hold.
 
     Differentiable once in ``q``, ``k``, ``v``, ``pos`` and ``slope`` (the gradient of a distance is zero where two nodes coincide);
     sums in float32, one order of sums, no atomics."""
-    _ops.check(q, k, v, graphs, num_heads, cap, pos, slope)
+    _ops.check(q, k, v, graphs, num_heads, scale, cap, pos, slope)
     if scale is None:
         scale = (q.shape[1] * q.shape[2] // num_heads) ** -0.5
     return _GraphAttention.apply(q, k, v, pos, slope, graphs, num_heads, float(scale), None if cap is None else float(cap))

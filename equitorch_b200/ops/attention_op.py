@@ -14,8 +14,8 @@ from ..graph import PackedGraphs
 MAX_HEAD = 128
 
 
-def check(q: Tensor, k: Tensor, v: Tensor, graphs: PackedGraphs, heads: int, cap: Optional[float], pos: Optional[Tensor],
-          slope: Optional[Tensor]) -> None:
+def check(q: Tensor, k: Tensor, v: Tensor, graphs: PackedGraphs, heads: int, scale: Optional[float], cap: Optional[float],
+          pos: Optional[Tensor], slope: Optional[Tensor]) -> None:
     if not isinstance(graphs, PackedGraphs):
         raise TypeError(f"PackedGraphs expected, got {type(graphs).__name__}")
     if q.ndim != 3:
@@ -30,8 +30,10 @@ def check(q: Tensor, k: Tensor, v: Tensor, graphs: PackedGraphs, heads: int, cap
         raise ValueError(f"{heads} heads cannot share features of shape {tuple(q.shape)}")
     if q.shape[1] * q.shape[2] // heads > MAX_HEAD:
         raise ValueError(f"a head has at most {MAX_HEAD} values a node: {q.shape[1]} components of {q.shape[2] // heads} channels are more")
-    if cap is not None and not 0 < cap < float("inf"):
-        raise ValueError(f"the cap must be positive and finite, got {cap}")
+    if cap is not None and not 1e-12 <= cap <= 1e12:
+        raise ValueError(f"the cap must be from 1e-12 to 1e12, got {cap}")
+    if scale is not None and not abs(scale) <= 1e12:
+        raise ValueError(f"the scale must be at most 1e12, got {scale}")
     if (pos is None) != (slope is None):
         raise ValueError("positions and slopes come together")
     if pos is not None:

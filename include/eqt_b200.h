@@ -646,7 +646,7 @@ int eqt_radius_list_edges(const float* pos, int64_t n, const int64_t* ptr, const
 /*
  * Rows of a table by type: out (n, width) = scale * weight (types, width)[index (n)]; a row of zeros where index is not in
  * [0, types).  Gradient: gw (types, width) = scale * sum of g over the rows of each type, all of gw written.  Sums in float
- * (double for EQT_F64), no atomics on values: the same bits at every call.  n and types below 2^31 - 1.
+ * (double for EQT_F64), no atomics on values: the same bits at every call.  n and types below 2^31 - 1, width <= 2^20.
  * `scratch`: eqt_embedding_grad_scratch bytes, 256-byte aligned (0: none needed).
  */
 int eqt_embedding_forward(int32_t dtype, const void* weight, const int64_t* index, void* out, int64_t n, int64_t types,
@@ -659,7 +659,7 @@ int eqt_embedding_grad(int32_t dtype, const void* g, const int64_t* index, void*
  * Attention within the graphs of a packed batch.  q, k, v (n, comps, heads * head_channels) with strides in elements between nodes
  * and components (channels are contiguous); out, grad_out, dq, dk, dv the same shape, contiguous.  A head's comps * head_channels
  * <= 128 values of a node are one vector.  Node i attends to the nodes j of its graph:
- *   s = scale <q_i, k_j>;  cap > 0: s = cap tanh(s / cap);  pos (n, 3) and slope (heads) given: s -= slope[h] |pos_i - pos_j|
+ *   s = scale <q_i, k_j>, |scale| <= 1e12;  cap in [1e-12, 1e12] (0: none): s = cap tanh(s / cap);  pos (n, 3) and slope (heads) given: s -= slope[h] |pos_i - pos_j|
  *   out_i = sum_j softmax_j(s) v_j;   lse (heads, n): log2 of the sum of exp(s), written by the forward pass (NULL: not wanted)
  * tiles (num_tiles, 4): first row, first node and one past the last node of the row's graph, 0; a tile is tile_rows (16, 32, 64)
  * rows of one graph, cut at the graph's end.  The tiles are to cover each row at most once and to lie in [0, n); rows of no tile are

@@ -54,7 +54,8 @@ def test_refusals():
     with pytest.raises(TypeError, match="PackedGraphs"):
         call(graphs=torch.tensor([0, 6]))
     for bad in (dict(q=x[:, 0]), dict(k=x[:5]), dict(v=torch.zeros(6, 1, 8)), dict(heads=3), dict(heads=0), dict(cap=0.0), dict(cap=-1.0),
-                dict(cap=float("nan")), dict(cap=float("inf")), dict(pos=pos), dict(slope=slope), dict(pos=pos[:5], slope=slope),
+                dict(cap=float("nan")), dict(cap=float("inf")), dict(cap=1e-13), dict(scale=float("nan")),
+                dict(scale=-1e13), dict(pos=pos), dict(slope=slope), dict(pos=pos[:5], slope=slope),
                 dict(pos=pos, slope=torch.zeros(3))):
         with pytest.raises(ValueError):
             call(**bad)
@@ -73,7 +74,7 @@ def test_refusals():
         enn.GraphAttention(2, distance_bias=False)(x, x, x, graphs, pos)
 
 
-@pytest.mark.parametrize("wrong", [dict(dtype=1), dict(heads=0), dict(tile_rows=48), dict(cap=-1.0), dict(cap=float("nan")), dict(q=None),
+@pytest.mark.parametrize("wrong", [dict(dtype=1), dict(heads=0), dict(tile_rows=48), dict(cap=-1.0), dict(cap=float("nan")), dict(cap=1e20), dict(scale=float("inf")), dict(q=None),
                                    dict(tiles=None), dict(pos=16), dict(head_channels=129), dict(n=2 ** 31), dict(n=-1)])
 def test_library_checks_its_arguments(wrong):
     good = dict(dtype=0, heads=2, comps=1, head_channels=8, tile_rows=16, scale=1.0, cap=0.0, n=4, num_tiles=1, tiles=16, q=16, k=16, v=16, out=16)

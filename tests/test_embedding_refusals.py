@@ -24,5 +24,6 @@ def test_library_checks_its_arguments():
     assert lib.eqt_embedding_forward(0, 16, 16, 16, -1, 1, 4, 1.0, None) == 1
     assert lib.eqt_embedding_forward(0, 16, None, 16, 1, 1, 4, 1.0, None) == 1
     assert lib.eqt_embedding_forward(0, 16, 16, 16, 2 ** 31, 1, 4, 1.0, None) == 2
+    assert lib.eqt_embedding_forward(0, 16, 16, 16, 1, 1, 2 ** 20 + 1, 1.0, None) == 2
     assert lib.eqt_embedding_grad(0, None, 16, 16, 1, 1, 4, 1.0, None, 0, None) == 1
     assert lib.eqt_embedding_grad(0, 16, 16, 16, 1, 2 ** 31, 4, 1.0, None, 0, None) == 2

@@ -154,6 +154,39 @@ def test_large_scores_and_coinciding_nodes(dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("scale,cap", [(-0.3, 4.0), (-0.3, None), (0.0, 4.0), (0.0, None), (0.2, 1e-6), (0.2, 1e-12), (0.2, 1e12), (-3.0, 0.5)])
+def test_scales_and_caps(dtype, scale, cap):
+    leaves, cot, graphs = _inputs([20, 70], 1, 2, 32, dtype, True)
+    with torch.no_grad():
+        leaves[0][3] = 0                                  # products that are zero to the last bit
+    got = _run(leaves, cot, graphs, 2, scale, cap)
+    want, tol = _reference(leaves, cot, graphs, 2, abs(scale), cap) if scale >= 0 else _reference(
+        [-leaves[0], *leaves[1:]], cot, graphs, 2, -scale, cap)
+    if scale < 0:
+        want[1] = -want[1]
+    assert all(((x.double() - y).abs() <= e + 1e-30).all() for x, y, e in zip(got, want, tol))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_products_far_below_the_others(dtype):
+    """Nodes that the others do not see, by products of -1e25: no weight, and no gradient that is not a number."""
+    leaves, cot, graphs = _inputs([40], 1, 1, 32, dtype, False)
+    with torch.no_grad():
+        leaves[0][:, :, 0] = 1e12
+        leaves[1][:, :, 0] = 0
+        leaves[1][5:9, :, 0] = -1e13
+    got = _run(leaves, cot, graphs, 1, 1.0, None)
+    assert all(torch.isfinite(t).all() for t in got)
+    seen = torch.ones(40, dtype=torch.bool, device=DEV)
+    seen[5:9] = False
+    rest = [t.detach()[seen].requires_grad_(True) for t in leaves]
+    few = _run([leaves[0].detach()[seen].requires_grad_(True), *rest[1:]], cot[seen], PackedGraphs(torch.tensor([0, 36], device=DEV), 36), 1, 1.0, None)
+    u = 2.0 ** -7 if dtype == torch.bfloat16 else 2.0 ** -18
+    assert (got[0][seen].double() - few[0].double()).norm() <= u * few[0].double().norm()
+    assert not got[2][5:9].any() and not got[3][5:9].any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_strides(dtype):
     """q, k, v as slices of one tensor, a gradient that is not contiguous, and tensors off the 16-byte boundary."""
     g = torch.Generator().manual_seed(3)
