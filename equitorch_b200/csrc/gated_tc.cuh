@@ -14,7 +14,7 @@
 // SMs, and no more arrived.  So where there is work for all of them, two CTAs of a cluster share a tile of 256 x 256: each copies its
 // 128 rows of A and half of B, 32 KB a k-block, the first one's MMAs read both SMs' shared memory, and each SM has the results of its
 // rows (100k x 256 -> 1024: gradient of x 101 -> 93 us, of the weights 90 -> 83; 8192 x 1024 -> 4096: 115 -> 103).
-// float32: operands are split into TF32 pairs, three MMAs each, as everywhere in this library.  Four warps split a stage between the
+// float32: operands are split into TF32 pairs, three MMAs each, as everywhere in this library.  Eight warps split a stage between the
 // copy and the MMA, big parts in place; a tile that lies along the rows is turned on the way, 32 x 32 values a warp at a time, so the
 // MMA always finds k along the row.  128 x 128 results a tile, three stages of 64 KB.  The adder of the tensor cores truncates, so the
 // products with small parts have a sum of their own, which leaves one truncation for eight terms in place of three, and a sum is taken
@@ -40,14 +40,14 @@ constexpr int PIECE = 4;                                 // k-blocks of a float3
 enum Shape { ALONE, PAIR, HELD };
 template <typename T> struct Form;
 template <> struct Form<__nv_bfloat16> {
-  static constexpr int BK = 64, COLS = 256, SPLITTERS = 0, EPI = 16, A_BYTES = 16384, HELD_BLOCKS = 4;
+  static constexpr int BK = 64, COLS = 256, FIRST = 2, SPLITTERS = 0, EPI = 16, A_BYTES = 16384, HELD_BLOCKS = 4;
   static constexpr int A_STAGE = A_BYTES, B_STAGE = 32768;
 };
 template <> struct Form<float> {                         // big and small parts
-  static constexpr int BK = 32, COLS = 128, SPLITTERS = 4, EPI = 8, A_BYTES = 16384, HELD_BLOCKS = 2;
+  static constexpr int BK = 32, COLS = 128, FIRST = 4, SPLITTERS = 8, EPI = 8, A_BYTES = 16384, HELD_BLOCKS = 2;
   static constexpr int A_STAGE = 2 * A_BYTES, B_STAGE = 32768;
 };
-template <typename T> constexpr int threads() { return 32 * (2 + Form<T>::SPLITTERS + Form<T>::EPI); }
+template <typename T> constexpr int threads() { return 32 * (Form<T>::FIRST + Form<T>::SPLITTERS + Form<T>::EPI); }
 // Results leave by 32 columns: a warp's patch is 32 rows of them; PARTIALS has two, so that the next tile's g is on its way.  What is
 // left of the shared memory are stages: of both operands, of half of B (PAIR), of A alone (HELD).
 template <typename T, int MODE> constexpr int patch_bytes() { return (MODE == PARTIALS ? 2 : 1) * Form<T>::EPI * 1024 * (int)sizeof(T); }
@@ -353,6 +353,10 @@ __global__ void __launch_bounds__(threads<T>(), 1) gated_tc_kernel(const __grid_
   const uint32_t tmem = tmem_slot;
   volatile int* ab = &abort_flag;
 
+  // float32: 640 threads of 96 registers, of which those that copy and issue and those that split leave some to the epilogue (all three
+  // shares are of whole groups of four warps: 40 + 2 * 64 + 2 * 152 = 472 <= 5 * 96).
+  if (warp < S::FIRST) {
+  if constexpr (F32) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
   if (warp == 0) {
     // ---------------- copies ----------------
     if (lane == 0) {
@@ -454,12 +458,14 @@ __global__ void __launch_bounds__(threads<T>(), 1) gated_tc_kernel(const __grid_
         }
       }
     }
-  } else if (warp < 2 + S::SPLITTERS) {
+  }
+  } else if (warp < S::FIRST + S::SPLITTERS) {
+    if constexpr (F32) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     // ---------------- float32 to TF32 pairs ----------------
     int s = 0;
     uint32_t ph = 0;
     bool ok = true;
-    const int w = warp - 2;
+    const int w = warp - S::FIRST;
     if (SHAPE == HELD && first_item < p.items) {
       ok = bar_wait(&held_full, 0, ab);
       for (int b = w; b < p.kblocks * (n_mma / 32) && ok; b += S::SPLITTERS)
@@ -473,8 +479,9 @@ __global__ void __launch_bounds__(threads<T>(), 1) gated_tc_kernel(const __grid_
       for (int kb = t.kb0; kb < t.kb1; ++kb) {
         if (!bar_wait(&full[s], ph, ab)) { ok = false; break; }
         unsigned char* st = ring + (size_t)s * STAGE;
-        split_block(st + w * 4096, S::A_BYTES, A_TURNED, lane);
-        for (int b = w; b < n_mma / 32 && SHAPE != HELD; b += S::SPLITTERS) split_block(st + S::A_STAGE + b * 4096, S::COLS * 128, B_TURNED, lane);
+        // four blocks of A, up to four of B: one a warp
+        if (w < 4) split_block(st + w * 4096, S::A_BYTES, A_TURNED, lane);
+        else if (SHAPE != HELD && w - 4 < n_mma / 32) split_block(st + S::A_STAGE + (w - 4) * 4096, S::COLS * 128, B_TURNED, lane);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) bar_arrive(&ready[s]);
@@ -483,9 +490,10 @@ __global__ void __launch_bounds__(threads<T>(), 1) gated_tc_kernel(const __grid_
     }
   } else {
     // ---------------- epilogue ----------------
+    if constexpr (F32) asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
     // Warps of the same quarter of the lanes share a tile's columns, 32 at a time in turn; of the dual products, 32 of each half.
     constexpr int SHARES = S::EPI / 4, GROUP = 16 / (int)sizeof(T), TURNS = S::COLS / (DUAL ? 64 : 32) / SHARES;
-    const int e = warp - 2 - S::SPLITTERS, quarter = warp & 3, share = e >> 2;
+    const int e = warp - S::FIRST - S::SPLITTERS, quarter = warp & 3, share = e >> 2;
     unsigned char* patch = ring + (size_t)STAGES * STAGE + (size_t)e * 1024 * sizeof(T);
     unsigned char* other = patch + S::EPI * 1024 * sizeof(T);                         // PARTIALS
     const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
