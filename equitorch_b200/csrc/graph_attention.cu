@@ -27,6 +27,7 @@ __global__ void __launch_bounds__(GEO_THREADS) attention_geometry_kernel(const f
   const int64_t i = (int64_t)(blockIdx.x - heads) * GEO_THREADS + threadIdx.x;
   if (i >= n) return;
   float x = 0.f, y = 0.f, z = 0.f;
+#pragma unroll 4
   for (int h = 0; h < heads; ++h) {
     const float4 a = row[(int64_t)h * n + i], b = col[(int64_t)h * n + i];
     const float f = -slope[h];

@@ -16,10 +16,14 @@
 // result is written by one CTA and sums have one order; no atomics.
 //
 // Matrix instructions are the warp-wide mma.sync.  Measured on this GPU they run at 552 TFLOP/s in bf16 and the special function unit
-// at 4.6e12 results/s.  A score costs one root (distance), two results for the cap and one exponential, so a head of 64 values takes
-// 256 flops of the tensor cores for up to four results: 0.46 ps against 0.87 ps.  What bounds the calls is the special functions and
-// the arithmetic around them, and tiles of 16 rows fit graphs of tens of nodes, where tiles of 128 rows would be three quarters empty.
-// float32 operands are split into TF32 pairs, three products each.
+// at 4.6e12 results/s.  A score costs one root (distance) and one exponential, the cap two results more unless its polynomial does, so
+// a head of 64 values takes 256 flops of the tensor cores, 0.46 ps, for two to four results, 0.43 to 0.87 ps, and some twenty
+// instructions of arithmetic: matrix instructions at any rate would leave the larger part.  And tiles of 16 rows fit graphs of tens of
+// nodes, where tiles of 128 rows would be three quarters empty.  float32 operands are split into TF32 pairs, three products each.
+//
+// One graph of 5001 nodes, 8 heads of 64 bfloat16 values, distance and cap: forward 357 us (143 TFLOP/s), by rows 620, by columns 690;
+// 16 graphs of up to 2000 nodes, 8 heads of 32, forward with distance: 175 us, the special functions half busy.  What bounds them is
+// the latency of dependent instructions at the three to six warps a scheduler that the registers leave.
 #pragma once
 
 #include "tc_common.cuh"
@@ -448,8 +452,10 @@ template <typename T, int DP, int WR, int KT> struct Shape {
   static constexpr size_t bytes(int residents, int extra) { return HEADS * head_elements(residents) * sizeof(T) + (size_t)extra; }
 };
 
+// CTAs an SM, here and below: as measured, against one more or fewer (forward, heads of 32: ragged graphs 167 us with 5, 175 with 6, 190 with
+// 7, molecules 81, 76 and 74; backward, molecules: by rows 141 with 4, 158 with 3, 164 with 5).
 template <typename T, int DP, int WR, int KT>
-__global__ void __launch_bounds__(THREADS, DP <= 32 ? 6 : DP <= 64 ? 4 : 3) attention_forward_kernel(const __grid_constant__ AttentionParams p) {
+__global__ void __launch_bounds__(THREADS, DP <= 32 ? (WR == 4 ? 5 : sizeof(T) == 2 ? 7 : 6) : DP <= 64 ? 4 : 3) attention_forward_kernel(const __grid_constant__ AttentionParams p) {
   using S = Shape<T, DP, WR, KT>;
   constexpr int LD = S::LD, NT = KT / 8;
   extern __shared__ __align__(16) unsigned char smem[];
