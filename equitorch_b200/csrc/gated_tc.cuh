@@ -6,8 +6,8 @@
 //   WEIGHT_GRAD  dWj = x^T dj                    over parts of the rows, float32 partial results
 //
 // A CTA per SM strides through tiles of 128 rows; a k-block of 128 bytes a row (64 bfloat16, 32 float32) is a stage of the ring.
-// Warp 0 copies tiles (TMA), warp 1 issues the MMAs, the last warps (sixteen, eight for float32) empty the accumulators while the next tile is multiplied;
-// the dual products have both halves of the columns in one MMA, so the activation and the product never leave the SM.
+// Warp 0 copies tiles (TMA), warp 1 issues the MMAs, the last warps (sixteen, eight for float32) empty the accumulators while the next
+// tile is multiplied; the dual products have both halves of the columns in one MMA, so the activation and the product never leave the SM.
 //
 // bfloat16: the MMA reads tiles as they lie in memory, along k or along the rows (both majors, 128-byte swizzle): 128 x 256 results
 // a tile, four stages of 48 KB.  What bounds that is L2: a k-block of 48 KB per 512 cycles of MMA and SM is 12 to 14 TB/s over all
@@ -356,109 +356,109 @@ __global__ void __launch_bounds__(threads<T>(), 1) gated_tc_kernel(const __grid_
   // float32: 640 threads of 96 registers, of which those that copy and issue and those that split leave some to the epilogue (all three
   // shares are of whole groups of four warps: 40 + 2 * 64 + 2 * 152 = 472 <= 5 * 96).
   if (warp < S::FIRST) {
-  if constexpr (F32) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-  if (warp == 0) {
-    // ---------------- copies ----------------
-    if (lane == 0) {
-      int s = 0;
-      uint32_t ph = 1;
-      bool ok = true;
-      const uint32_t bytes = CTAS * S::A_BYTES + (SHAPE == HELD ? 0 : (uint32_t)n_mma * 128);
-      if (SHAPE == HELD && first_item < p.items) {
-        const int col = item_of<MODE, SHAPE>(p, first_item).col;
-        bar_expect_tx(&held_full, (uint32_t)(p.kblocks * n_mma) * 128);
-        for (int kb = 0; kb < p.kblocks; ++kb)
-          for (int q = 0; q < 2; ++q)
-            for (int c = 0; c < p.width / LINE; ++c)
-              tma_load_2d(held + kb * S::B_STAGE + (q * (p.width / LINE) + c) * S::BK * 128, &p.b[q], col + c * LINE, kb * S::BK, &held_full);
-      }
-      for (unsigned i = first_item; i < p.items && ok && !*ab; i += item_step) {
-        const Item t = item_of<MODE, SHAPE>(p, i);
-        const int row = (int)t.row + rank * TILE_M;
-        // Columns of B that this CTA copies: all, or its half; of the dual products' pair, one weight's.
-        const int b_cols = TWO && !DUAL ? p.width / 2 : p.width, col = t.col + (TWO && !DUAL ? rank * b_cols : 0);
-        for (int kb = t.kb0; kb < t.kb1; ++kb) {
-          if (!bar_wait(&empty[s], ph, ab)) { ok = false; break; }
-          unsigned char* st = ring + (size_t)s * STAGE;
-          uint64_t* bar = &full[s];
-          if (rank == 0) bar_expect_tx(bar, bytes);
-          const int h = MODE == INPUT_GRAD ? kb >= p.kblocks : t.half, k = (MODE == INPUT_GRAD && h ? kb - p.kblocks : kb) * S::BK;
-          if (A_TURNED) {
-#pragma unroll
-            for (int c = 0; c < TILE_M / LINE; ++c) copy_2d<TWO>(st + c * S::BK * 128, &p.a[0], row + c * LINE, k, bar);
-          } else {
-            copy_2d<TWO>(st, &p.a[MODE == INPUT_GRAD ? h : 0], k, row, bar);
-          }
-          unsigned char* sb = st + S::A_STAGE;
-          if (SHAPE == HELD) {
-          } else if (MODE == INPUT_GRAD) {
-            copy_2d<TWO>(sb, &p.b[h], k, col, bar);
-          } else {
-            const int q0 = DUAL ? rank : t.half, q1 = DUAL && !TWO ? 2 : q0 + 1;
-            for (int q = q0; q < q1; ++q)
-              for (int c = 0; c < b_cols / LINE; ++c, sb += S::BK * 128) copy_2d<TWO>(sb, &p.b[q], col + c * LINE, k, bar);
-          }
-          if (++s == STAGES) s = 0, ph ^= 1;
+    if constexpr (F32) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (warp == 0) {
+      // ---------------- copies ----------------
+      if (lane == 0) {
+        int s = 0;
+        uint32_t ph = 1;
+        bool ok = true;
+        const uint32_t bytes = CTAS * S::A_BYTES + (SHAPE == HELD ? 0 : (uint32_t)n_mma * 128);
+        if (SHAPE == HELD && first_item < p.items) {
+          const int col = item_of<MODE, SHAPE>(p, first_item).col;
+          bar_expect_tx(&held_full, (uint32_t)(p.kblocks * n_mma) * 128);
+          for (int kb = 0; kb < p.kblocks; ++kb)
+            for (int q = 0; q < 2; ++q)
+              for (int c = 0; c < p.width / LINE; ++c)
+                tma_load_2d(held + kb * S::B_STAGE + (q * (p.width / LINE) + c) * S::BK * 128, &p.b[q], col + c * LINE, kb * S::BK, &held_full);
         }
-      }
-    }
-  } else if (warp == 1) {
-    // ---------------- MMAs ----------------
-    if (lane == 0 && rank == 0) {
-      int s = 0;
-      uint32_t ph = 0;
-      int piece = 0;
-      bool ok = true;
-      const uint32_t idesc = F32 ? umma_idesc_tf32(n_mma) : idesc_bf16(CTAS * TILE_M, n_mma, A_TURNED, B_TURNED);
-      if (SHAPE == HELD) {
-        ok = bar_wait(F32 ? &held_ready : &held_full, 0, ab);
-        tc_fence_after();
-      }
-      for (unsigned i = first_item; i < p.items && ok && !*ab; i += item_step) {
-        const Item t = item_of<MODE, SHAPE>(p, i);
-        for (int k0 = t.kb0; k0 < t.kb1 && ok; ++piece) {
-          const int k1 = F32 ? min(k0 + PIECE, t.kb1) : t.kb1, a = piece & 1;
-          const uint32_t parity = (uint32_t)(((piece >> 1) & 1) ^ 1);
-          if (!(TWO ? bar_wait_cluster(&acc_empty[a], parity, ab) : bar_wait(&acc_empty[a], parity, ab))) { ok = false; break; }
-          tc_fence_after();
-          const uint32_t d = tmem + (uint32_t)(a * ACC_COLS);
-          for (int kb = k0; kb < k1; ++kb) {
-            if (!(TWO ? bar_wait_cluster(&full[s], ph, ab) : bar_wait(F32 ? &ready[s] : &full[s], ph, ab))) { ok = false; break; }
-            tc_fence_after();
-            const uint32_t at = s32(ring + (size_t)s * STAGE), bt = SHAPE == HELD ? s32(held + kb * S::B_STAGE) : at + S::A_STAGE;
-            if constexpr (F32) {
-              const uint32_t ah = umma_lo(at), al = ah + S::A_BYTES / 16, bh = umma_lo(bt), bl = bh + S::COLS * 8;
-              if (kb == k0) {
-                umma_tf32_lo<false>(d, ah, bh, idesc);
-                umma_tf32_lo<false>(d + S::COLS, al, bh, idesc);
-              } else {
-                umma_tf32_lo<true>(d, ah, bh, idesc);
-                umma_tf32_lo<true>(d + S::COLS, al, bh, idesc);
-              }
-              umma_tf32_lo<true>(d + S::COLS, ah, bl, idesc);
+        for (unsigned i = first_item; i < p.items && ok && !*ab; i += item_step) {
+          const Item t = item_of<MODE, SHAPE>(p, i);
+          const int row = (int)t.row + rank * TILE_M;
+          // Columns of B that this CTA copies: all, or its half; of the dual products' pair, one weight's.
+          const int b_cols = TWO && !DUAL ? p.width / 2 : p.width, col = t.col + (TWO && !DUAL ? rank * b_cols : 0);
+          for (int kb = t.kb0; kb < t.kb1; ++kb) {
+            if (!bar_wait(&empty[s], ph, ab)) { ok = false; break; }
+            unsigned char* st = ring + (size_t)s * STAGE;
+            uint64_t* bar = &full[s];
+            if (rank == 0) bar_expect_tx(bar, bytes);
+            const int h = MODE == INPUT_GRAD ? kb >= p.kblocks : t.half, k = (MODE == INPUT_GRAD && h ? kb - p.kblocks : kb) * S::BK;
+            if (A_TURNED) {
 #pragma unroll
-              for (int q = 1; q < 4; ++q) {
-                umma_tf32_lo<true>(d, ah + q * 2, bh + q * 2, idesc);
-                umma_tf32_lo<true>(d + S::COLS, al + q * 2, bh + q * 2, idesc);
-                umma_tf32_lo<true>(d + S::COLS, ah + q * 2, bl + q * 2, idesc);
-              }
+              for (int c = 0; c < TILE_M / LINE; ++c) copy_2d<TWO>(st + c * S::BK * 128, &p.a[0], row + c * LINE, k, bar);
             } else {
-              constexpr int A_STEP = A_TURNED ? 128 : 2, B_STEP = B_TURNED ? 128 : 2;                // 16 of k, in 16 bytes
-              const uint32_t a_lo = A_TURNED ? lo_rows(at) : umma_lo(at), b_lo = B_TURNED ? lo_rows(bt) : umma_lo(bt);
-              if (kb == k0) mma_bf16<TWO, false>(d, a_lo, b_lo, idesc);
-              else mma_bf16<TWO, true>(d, a_lo, b_lo, idesc);
-#pragma unroll
-              for (int q = 1; q < 4; ++q) mma_bf16<TWO, true>(d, a_lo + q * A_STEP, b_lo + q * B_STEP, idesc);
+              copy_2d<TWO>(st, &p.a[MODE == INPUT_GRAD ? h : 0], k, row, bar);
             }
-            commit<TWO>(&empty[s]);
+            unsigned char* sb = st + S::A_STAGE;
+            if (SHAPE == HELD) {
+            } else if (MODE == INPUT_GRAD) {
+              copy_2d<TWO>(sb, &p.b[h], k, col, bar);
+            } else {
+              const int q0 = DUAL ? rank : t.half, q1 = DUAL && !TWO ? 2 : q0 + 1;
+              for (int q = q0; q < q1; ++q)
+                for (int c = 0; c < b_cols / LINE; ++c, sb += S::BK * 128) copy_2d<TWO>(sb, &p.b[q], col + c * LINE, k, bar);
+            }
             if (++s == STAGES) s = 0, ph ^= 1;
           }
-          if (ok) commit<TWO>(&acc_full[a]);
-          k0 = k1;
+        }
+      }
+    } else if (warp == 1) {
+      // ---------------- MMAs ----------------
+      if (lane == 0 && rank == 0) {
+        int s = 0;
+        uint32_t ph = 0;
+        int piece = 0;
+        bool ok = true;
+        const uint32_t idesc = F32 ? umma_idesc_tf32(n_mma) : idesc_bf16(CTAS * TILE_M, n_mma, A_TURNED, B_TURNED);
+        if (SHAPE == HELD) {
+          ok = bar_wait(F32 ? &held_ready : &held_full, 0, ab);
+          tc_fence_after();
+        }
+        for (unsigned i = first_item; i < p.items && ok && !*ab; i += item_step) {
+          const Item t = item_of<MODE, SHAPE>(p, i);
+          for (int k0 = t.kb0; k0 < t.kb1 && ok; ++piece) {
+            const int k1 = F32 ? min(k0 + PIECE, t.kb1) : t.kb1, a = piece & 1;
+            const uint32_t parity = (uint32_t)(((piece >> 1) & 1) ^ 1);
+            if (!(TWO ? bar_wait_cluster(&acc_empty[a], parity, ab) : bar_wait(&acc_empty[a], parity, ab))) { ok = false; break; }
+            tc_fence_after();
+            const uint32_t d = tmem + (uint32_t)(a * ACC_COLS);
+            for (int kb = k0; kb < k1; ++kb) {
+              if (!(TWO ? bar_wait_cluster(&full[s], ph, ab) : bar_wait(F32 ? &ready[s] : &full[s], ph, ab))) { ok = false; break; }
+              tc_fence_after();
+              const uint32_t at = s32(ring + (size_t)s * STAGE), bt = SHAPE == HELD ? s32(held + kb * S::B_STAGE) : at + S::A_STAGE;
+              if constexpr (F32) {
+                const uint32_t ah = umma_lo(at), al = ah + S::A_BYTES / 16, bh = umma_lo(bt), bl = bh + S::COLS * 8;
+                if (kb == k0) {
+                  umma_tf32_lo<false>(d, ah, bh, idesc);
+                  umma_tf32_lo<false>(d + S::COLS, al, bh, idesc);
+                } else {
+                  umma_tf32_lo<true>(d, ah, bh, idesc);
+                  umma_tf32_lo<true>(d + S::COLS, al, bh, idesc);
+                }
+                umma_tf32_lo<true>(d + S::COLS, ah, bl, idesc);
+#pragma unroll
+                for (int q = 1; q < 4; ++q) {
+                  umma_tf32_lo<true>(d, ah + q * 2, bh + q * 2, idesc);
+                  umma_tf32_lo<true>(d + S::COLS, al + q * 2, bh + q * 2, idesc);
+                  umma_tf32_lo<true>(d + S::COLS, ah + q * 2, bl + q * 2, idesc);
+                }
+              } else {
+                constexpr int A_STEP = A_TURNED ? 128 : 2, B_STEP = B_TURNED ? 128 : 2;                // 16 of k, in 16 bytes
+                const uint32_t a_lo = A_TURNED ? lo_rows(at) : umma_lo(at), b_lo = B_TURNED ? lo_rows(bt) : umma_lo(bt);
+                if (kb == k0) mma_bf16<TWO, false>(d, a_lo, b_lo, idesc);
+                else mma_bf16<TWO, true>(d, a_lo, b_lo, idesc);
+#pragma unroll
+                for (int q = 1; q < 4; ++q) mma_bf16<TWO, true>(d, a_lo + q * A_STEP, b_lo + q * B_STEP, idesc);
+              }
+              commit<TWO>(&empty[s]);
+              if (++s == STAGES) s = 0, ph ^= 1;
+            }
+            if (ok) commit<TWO>(&acc_full[a]);
+            k0 = k1;
+          }
         }
       }
     }
-  }
   } else if (warp < S::FIRST + S::SPLITTERS) {
     if constexpr (F32) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     // ---------------- float32 to TF32 pairs ----------------
@@ -670,6 +670,7 @@ __global__ void __launch_bounds__(threads<T>(), 1) gated_tc_kernel(const __grid_
   if (tid == 0 && abort_flag) {
     atomicExch(p.status, 2);
     let_copies_land(full, STAGES);
+    if (SHAPE == HELD) let_copies_land(&held_full, 1);
   }
   __syncthreads();
   if (TWO) cluster_sync();                              // nothing of the other CTA reaches this one's memory any more
@@ -783,8 +784,10 @@ template <typename T, int MODE, int SHAPE, int ACT> int launch_form(const GatedA
   return check_launch("gated_tc");
 }
 
-// HELD where B's k-blocks fit and the columns' tiles divide the SMs with little left over; pairs of CTAs from the size on that gives most
-// SMs a tile of 256 rows, below it tiles of 128 rows fill more of them.
+// HELD for the forward pass where B's k-blocks fit and the columns' tiles divide the SMs with little left over (123 -> 106 us at 100k x
+// 256 -> 1024; the partial results 149 -> 167 us, since their patches leave A two stages).  Pairs of CTAs from the size on that gives most
+// SMs a tile of 256 rows, below it tiles of 128 rows fill more of them; not for the dual products of short sums, whose tiles change hands
+// too often (the same call in pairs: forward 132, partial results 171 us).
 template <typename T, int MODE, int ACT = EQT_ACT_SILU> int launch(const GatedArgs& a, cudaStream_t s) {
   constexpr bool DUAL = MODE == FORWARD || MODE == PARTIALS;
   if constexpr (MODE == FORWARD) {
