@@ -120,8 +120,12 @@ __global__ void __launch_bounds__(256) sum_parts_kernel(const typename Acc<T>::t
   using A = typename Acc<T>::type;
   const int64_t size = (int64_t)rows * f, part = (int64_t)rows * pitch;
   for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < size; i += (int64_t)gridDim.x * blockDim.x) {
-    const int row = (int)(i / f);
-    const A* from = parts + (int64_t)row * pitch + (i - (int64_t)row * f);
+    int64_t at = i;
+    if (pitch != f) {
+      const int64_t row = size <= UINT32_MAX ? (unsigned)i / (unsigned)f : i / f;
+      at = row * pitch + (i - row * f);
+    }
+    const A* from = parts + at;
     A sum = A(0);
 #pragma unroll 8
     for (int s = 0; s < splits; ++s) sum += from[s * part];
