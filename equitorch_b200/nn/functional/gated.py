@@ -29,7 +29,8 @@ def gated_linear(input: Tensor, weight: Tensor, activation: str = "silu") -> Ten
     function), ``relu`` or ``sigmoid``; of equivariant features it may act on invariant components only.
 
     float32, float64 or bfloat16, sums in float32 (float64 for float64).  Differentiable once; the backward pass forms both
-    projections again, keeps only ``x`` and the weight, and takes scratch of twice the result's size.  float32 and bfloat16 run on the tensor cores; where channels or hidden
-    are no multiples of 16 bytes (4 or 8 values) the operands are first copied to wider rows."""
+    projections again, keeps only ``x`` and the weight, and takes scratch of twice the result's size.  float32 and bfloat16 run on
+    the tensor cores; where channels or hidden are no multiples of 16 bytes (4 or 8 values) the operands are first copied to wider
+    rows."""
     _ops.check(input, weight, activation)
     return _GatedLinear.apply(input, weight, activation)
