@@ -82,8 +82,9 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 // load, and the four by eight places of a TF32 fragment (and of one transposed), fall on different banks.
 template <typename T, int DP> struct Row { static constexpr int LD = DP + 16 / (int)sizeof(T); };
 
-// acc[16 rows][8 NT] = A[16][DP] B[8 NT][DP]^T
-template <int DP, int NT>
+// acc[16 rows][8 NT] = A[16][DP] B[8 NT][DP]^T.  The pass by columns has the operands the other way round (TURNED) and takes the products in
+// the same order: a score has the same bits in all passes, so its weight belongs to the saved statistics however large it is.
+template <int DP, int NT, bool TURNED = false>
 __device__ __forceinline__ void score_mma(float (&acc)[NT][4], const __nv_bfloat16* a, const __nv_bfloat16* b, int lane) {
   constexpr int LD = Row<__nv_bfloat16, DP>::LD;
   const __nv_bfloat16* ap = a + (lane & 15) * LD + (lane >> 4) * 8;
@@ -104,7 +105,7 @@ __device__ __forceinline__ void score_mma(float (&acc)[NT][4], const __nv_bfloat
   }
 }
 // The tensor cores' adder truncates, so the products with small parts have a sum of their own: one truncation for eight terms.
-template <int DP, int NT>
+template <int DP, int NT, bool TURNED = false>
 __device__ __forceinline__ void score_mma(float (&acc)[NT][4], const float* a, const float* b, int lane) {
   constexpr int LD = Row<float, DP>::LD;
   const int g = lane >> 2, t = lane & 3;
@@ -128,8 +129,9 @@ __device__ __forceinline__ void score_mma(float (&acc)[NT][4], const float* a, c
       tc::split_tf32(bp[n * 8 * LD + ks * 8], h0, l0);
       tc::split_tf32(bp[n * 8 * LD + ks * 8 + 4], h1, l1);
       mma_tf32(acc[n], hi, h0, h1);
+      if (TURNED) mma_tf32(fine[n], hi, l0, l1);
       mma_tf32(fine[n], lo, h0, h1);
-      mma_tf32(fine[n], hi, l0, l1);
+      if (!TURNED) mma_tf32(fine[n], hi, l0, l1);
     }
   }
 #pragma unroll
@@ -233,16 +235,19 @@ __device__ __forceinline__ pair fma2(pair a, pair b, pair c) {
   return r;
 }
 
-// From products to scores without the distance, in units of log2: unit z, or unit tanh(z to_cap).  tanh is up to a half an odd polynomial
-// (fitted for the least relative error, 7.4e-8 in float32 arithmetic), above it 1 - 2 / (e^2x + 1).  Scores mostly stay below half the
-// cap, and a warp whose tile does so needs no special function for them.
-__device__ __forceinline__ float tanh_any(float x) {
+// From products to scores without the distance, in units of log2: unit z, or unit tanh(x) with x = z to_cap.  tanh is up to a half an odd
+// polynomial (fitted for the least relative error, 7.4e-8 in float32 arithmetic), above it 1 - 2 / (e^2x + 1).  Scores mostly stay below
+// half the cap, and a warp whose tile does so needs no special function for them.  The polynomial's argument is x itself: to_cap may be
+// anything from 0 to 1e24, and powers of it, as factors of the coefficients, leave the range of float32.  Both branches take the same steps
+// for an x below a half, so that a score has the same bits whatever tile it is in, in the forward and in both backward passes.
+constexpr float TANH3 = -0.333331435918808f, TANH5 = 0.13325878977775574f, TANH7 = -0.05304549261927605f, TANH9 = 0.01724148727953434f;
+__device__ __forceinline__ float capped(float x, float unit) {
   const float y = fabsf(x), w = x * x, large = copysignf(1.f - __fdividef(2.f, exp2_fast(fminf(y * (2.f * LOG2E), 64.f)) + 1.f), x);
-  const float small = fmaf(x, w * fmaf(w, fmaf(w, fmaf(w, 0.01724148727953434f, -0.05304549261927605f), 0.13325878977775574f), -0.333331435918808f), x);
-  return y <= 0.5f ? small : x == x ? large : x;
+  const float z = x * unit, more = w * fmaf(w, fmaf(w, fmaf(w, TANH9, TANH7), TANH5), TANH3);
+  return y <= 0.5f ? fmaf(z, more, z) : x == x ? unit * large : x;
 }
-template <int NT> __device__ __forceinline__ void cap_tile(float (&z)[NT][4], float unit, float to_cap, bool capped) {
-  if (!capped) {
+template <int NT> __device__ __forceinline__ void cap_tile(float (&z)[NT][4], float unit, float to_cap, bool has_cap) {
+  if (!has_cap) {
     const pair u = both(unit, unit);
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -250,14 +255,16 @@ template <int NT> __device__ __forceinline__ void cap_tile(float (&z)[NT][4], fl
       for (int r = 0; r < 2; ++r) parts(mul2(both(z[n][2 * r], z[n][2 * r + 1]), u), z[n][2 * r], z[n][2 * r + 1]);
     return;
   }
+  const pair to = both(to_cap, to_cap);
   float most = 0.f;
 #pragma unroll
-  for (int n = 0; n < NT; ++n) most = fmaxf(fmaxf(most, fmaxf(fabsf(z[n][0]), fabsf(z[n][1]))), fmaxf(fabsf(z[n][2]), fabsf(z[n][3])));
-  // The maximum drops NaNs; they stay NaN either way.  Above 1e4 the polynomial's coefficients would leave the range of float32.
-  if (fabsf(to_cap) <= 1e4f && __all_sync(0xffffffffu, most * fabsf(to_cap) <= 0.5f)) {
-    const float f = to_cap * to_cap;                     // the polynomial's argument is (z to_cap)^2
-    const float c0 = -0.333331435918808f * f, c1 = 0.13325878977775574f * f * f, c2 = -0.05304549261927605f * f * f * f, c3 = 0.01724148727953434f * f * f * f * f;
-    const pair k0 = both(c0, c0), k1 = both(c1, c1), k2 = both(c2, c2), k3 = both(c3, c3), u = both(unit * to_cap, unit * to_cap);
+  for (int n = 0; n < NT; ++n) {
+#pragma unroll
+    for (int r = 0; r < 2; ++r) parts(mul2(both(z[n][2 * r], z[n][2 * r + 1]), to), z[n][2 * r], z[n][2 * r + 1]);
+    most = fmaxf(fmaxf(most, fmaxf(fabsf(z[n][0]), fabsf(z[n][1]))), fmaxf(fabsf(z[n][2]), fabsf(z[n][3])));
+  }
+  if (__all_sync(0xffffffffu, most <= 0.5f)) {           // the maximum drops NaNs; they stay NaN either way
+    const pair k0 = both(TANH3, TANH3), k1 = both(TANH5, TANH5), k2 = both(TANH7, TANH7), k3 = both(TANH9, TANH9), u = both(unit, unit);
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -269,7 +276,7 @@ template <int NT> __device__ __forceinline__ void cap_tile(float (&z)[NT][4], fl
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) z[n][i] = unit * tanh_any(z[n][i] * to_cap);
+      for (int i = 0; i < 4; ++i) z[n][i] = capped(z[n][i], unit);
   }
 }
 
@@ -648,8 +655,8 @@ __global__ void __launch_bounds__(THREADS, DP <= 32 ? 4 : DP <= 96 ? 3 : 2) atte
     for (int i = 0; i < 4; ++i) geo[r][i] = flat[r][i] = 0;
   constexpr bool APART = sizeof(T) == 2;
   const float to_cap = p.cap > 0.f ? p.scale / p.cap : 0.f, unit = (p.cap > 0.f ? p.cap : p.scale) * LOG2E;   // of a score: the tanh, or the product
-  const float bend = p.cap > 0.f ? -p.scale / (unit * unit) : 0.f;         // scale (1 - tanh^2), from unit tanh
-  const pair scale2 = both(p.scale, p.scale), bend2 = both(bend, bend);
+  const float bend = p.cap > 0.f ? -1.f / (unit * unit) : 0.f;             // 1 - tanh^2, from unit tanh; the scale follows at the end
+  const pair one2 = both(1.f, 1.f), bend2 = both(bend, bend);
   pair slope2 = 0;
   Place place[2];
   if (p.pos) {
@@ -708,7 +715,7 @@ __global__ void __launch_bounds__(THREADS, DP <= 32 ? 4 : DP <= 96 ? 3 : 2) atte
             geo[r][2] = fma2(fi, v.y, geo[r][2]);
             geo[r][3] = fma2(fi, v.z, geo[r][3]);
           }
-          parts(mul2(e, fma2(mul2(score0, bend2), score0, scale2)), z[n][2 * r], z[n][2 * r + 1]);
+          parts(mul2(e, fma2(mul2(score0, bend2), score0, one2)), z[n][2 * r], z[n][2 * r + 1]);
         }
       }
       out_mma<DP, NT>(dq, z, ks, lane);
@@ -741,7 +748,7 @@ __global__ void __launch_bounds__(THREADS, DP <= 32 ? 4 : DP <= 96 ? 3 : 2) atte
     if (is[0]) p.delta[at] = delta[0];
     if (is[1]) p.delta[at + 8] = delta[1];
   }
-  store_rows<T, DP>(const_cast<T*>(mq), p.dq, dq, 1.f, 1.f, row, hi, head, p, lane);
+  store_rows<T, DP>(const_cast<T*>(mq), p.dq, dq, p.scale, p.scale, row, hi, head, p, lane);
 }
 
 // Backward by columns: dk, dv, and with positions the columns' sums of dS u.  The CTA's rows are keys; queries and the output's
@@ -800,8 +807,8 @@ __global__ void __launch_bounds__(THREADS, DP <= 32 ? 4 : DP <= 64 ? 3 : 2) atte
     dv[n][0] = dv[n][1] = dv[n][2] = dv[n][3] = 0.f;
   }
   const float to_cap = p.cap > 0.f ? p.scale / p.cap : 0.f, unit = (p.cap > 0.f ? p.cap : p.scale) * LOG2E;
-  const float bend = p.cap > 0.f ? -p.scale / (unit * unit) : 0.f;
-  const pair scale2 = both(p.scale, p.scale), bend2 = both(bend, bend), minus = both(-1.f, -1.f);
+  const float bend = p.cap > 0.f ? -1.f / (unit * unit) : 0.f;
+  const pair one2 = both(1.f, 1.f), bend2 = both(bend, bend), minus = both(-1.f, -1.f);
   pair slope2 = 0;
   Place place[2];
   if (p.pos) {
@@ -823,8 +830,8 @@ __global__ void __launch_bounds__(THREADS, DP <= 32 ? 4 : DP <= 64 ? 3 : 2) atte
       const T *qs = stage + s * S::STAGE, *gs = qs + KT * LD;
       const float *ls = stats + 2 * s * KT, *ds = ls + KT;
       float z[NT][4], dp[NT][4];
-      score_mma<DP, NT>(z, mk, qs, lane);
-      score_mma<DP, NT>(dp, mv, gs, lane);
+      score_mma<DP, NT, true>(z, mk, qs, lane);
+      score_mma<DP, NT, true>(dp, mv, gs, lane);
       cap_tile<NT>(z, unit, to_cap, p.cap > 0.f);
       const bool last = query + KT > hi;
 #pragma unroll
@@ -859,7 +866,7 @@ __global__ void __launch_bounds__(THREADS, DP <= 32 ? 4 : DP <= 64 ? 3 : 2) atte
           }
           z[n][2 * r] = x;
           z[n][2 * r + 1] = y;
-          parts(fma2(mul2(mul2(score0, bend2), score0), e, mul2(e, scale2)), dp[n][2 * r], dp[n][2 * r + 1]);
+          parts(mul2(e, fma2(mul2(score0, bend2), score0, one2)), dp[n][2 * r], dp[n][2 * r + 1]);
         }
       }
       out_mma<DP, NT>(dv, z, gs, lane);
@@ -881,7 +888,7 @@ __global__ void __launch_bounds__(THREADS, DP <= 32 ? 4 : DP <= 64 ? 3 : 2) atte
       if (t == 0 && row + g + 8 * r < hi) p.geo_col[(int64_t)head * p.n + row + g + 8 * r] = v;
     }
   }
-  store_rows<T, DP>(const_cast<T*>(mk), p.dk, dk, 1.f, 1.f, row, hi, head, p, lane);
+  store_rows<T, DP>(const_cast<T*>(mk), p.dk, dk, p.scale, p.scale, row, hi, head, p, lane);
   store_rows<T, DP>(const_cast<T*>(mv), p.dv, dv, 1.f, 1.f, row, hi, head, p, lane);
 }
 
