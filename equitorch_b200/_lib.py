@@ -92,7 +92,7 @@ class AttentionArgs(C.Structure):
     _fields_ = ([(f, C.c_int32) for f in ("dtype", "heads", "comps", "head_channels", "tile_rows")] + [("scale", C.c_float), ("cap", C.c_float)]
                 + [("n", C.c_int64), ("num_tiles", C.c_int64)] + [(f, C.c_void_p) for f in ("tiles", "q", "k", "v")]
                 + [(f, C.c_int64) for f in ("q_node", "q_comp", "k_node", "k_comp", "v_node", "v_comp")]
-                + [(f, C.c_void_p) for f in ("pos", "slope", "out", "lse", "grad_out", "dq", "dk", "dv", "delta", "geo", "dpos", "dslope")])
+                + [(f, C.c_void_p) for f in ("pos", "slope", "out", "stats", "grad_out", "dq", "dk", "dv", "delta", "geo", "dpos", "dslope")])
 
 
 # name -> (restype, argtypes); every symbol declared in include/eqt_b200.h appears here

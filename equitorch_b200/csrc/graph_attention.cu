@@ -128,7 +128,7 @@ int fill(const eqt_attention_args* a, AttentionParams& p, bool backward) {
   if (a->cap != 0.f && !(a->cap >= 1e-12f && a->cap <= 1e12f)) return fail(EQT_ERR_BAD_ARGUMENT, "attention: the cap must be 0 or from 1e-12 to 1e12");
   if (!(fabsf(a->scale) <= 1e12f)) return fail(EQT_ERR_BAD_ARGUMENT, "attention: the scale must be at most 1e12");
   if (a->n && (a->pos != nullptr) != (a->slope != nullptr)) return fail(EQT_ERR_BAD_ARGUMENT, "attention: positions and slopes come together");
-  if (a->num_tiles && (!a->q || !a->k || !a->v || !a->out || !a->tiles || (backward && (!a->grad_out || !a->lse || !a->dq || !a->dk || !a->dv || !a->delta))))
+  if (a->num_tiles && (!a->q || !a->k || !a->v || !a->out || !a->tiles || (backward && (!a->grad_out || !a->stats || !a->dq || !a->dk || !a->dv || !a->delta))))
     return fail(EQT_ERR_BAD_ARGUMENT, "attention: NULL pointer");
   const bool geo = a->dpos || a->dslope;
   if (backward && geo && a->n && (!a->pos || !a->dpos || !a->dslope || !a->geo))
@@ -144,7 +144,8 @@ int fill(const eqt_attention_args* a, AttentionParams& p, bool backward) {
   p.dq = a->dq;
   p.dk = a->dk;
   p.dv = a->dv;
-  p.lse = a->lse;
+  p.top = a->stats;
+  p.inverse = a->stats ? a->stats + a->heads * a->n : nullptr;
   p.delta = a->delta;
   p.geo_row = static_cast<float4*>(a->geo);
   p.geo_col = p.geo_row ? p.geo_row + a->heads * a->n : nullptr;

@@ -42,7 +42,8 @@ struct Operand {
 struct AttentionParams {
   Operand q, k, v, g;
   void *out, *dq, *dk, *dv;
-  float *lse, *delta;        // [head][node]; lse in units of log2
+  float *top, *inverse;      // [head][node]: the row's greatest score in units of log2, one over its sum of weights from there
+  float* delta;              // [head][node]
   float4 *geo_row, *geo_col; // [head][node]: (sum dS r, sum dS u) by rows; (0, sum dS u) by columns
   const int4* tiles;         // first row, first and one past the last node of its graph
   const float *pos, *slope;
@@ -585,16 +586,17 @@ __global__ void __launch_bounds__(THREADS, DP <= 32 ? (WR == 4 ? 5 : sizeof(T) =
   if (!work) return;
   sum[0] = quad_sum(sum[0]);
   sum[1] = quad_sum(sum[1]);
-  if (p.lse && t == 0) {
-    float* to = p.lse + (int64_t)head * p.n + row + g;
-    if (row + g < hi) to[0] = top[0] + log2f(sum[0]);
-    if (row + g + 8 < hi) to[8] = top[1] + log2f(sum[1]);
-  }
   const float f0 = 1.f / sum[0], f1 = 1.f / sum[1];
+  if (p.top && t == 0) {                                                 // apart: their sum would lose the logarithm beside a large score
+    const int64_t to = (int64_t)head * p.n + row + g;
+    if (row + g < hi) p.top[to] = top[0], p.inverse[to] = f0;
+    if (row + g + 8 < hi) p.top[to + 8] = top[1], p.inverse[to + 8] = f1;
+  }
   store_rows<T, DP>(const_cast<T*>(mine), p.out, o, f0, f1, row, hi, head, p, lane);
 }
 
-// Backward by rows: dq, delta, and with positions the rows' sums of dS r and dS u.
+// Backward by rows: dq, delta, and with positions the rows' sums of dS r and dS u.  Weights are taken from the row's greatest score, and
+// one over their sum follows at the end.
 // These sums are float32 results also where the features are bfloat16, so there they do not go by the delta of the rounded weights and
 // result: with w = r or u, sum_j dS w = sum_j P dP w - (sum_j P dP) (sum_j P w), and the columns' pass is given sum_j P dP.
 template <typename T, int DP, int WR, int KT, bool GEO>
@@ -639,12 +641,12 @@ __global__ void __launch_bounds__(THREADS, DP <= 32 ? 4 : DP <= 96 ? 3 : 2) atte
   const int row = first + (warp % WR) * 16;
   const bool work = here && row < hi;
   const T *mq = rows + (warp % WR) * 16 * LD, *mg = grads + (warp % WR) * 16 * LD;
-  float delta[2] = {0.f, 0.f}, lse[2] = {INFINITY, INFINITY};
+  float delta[2] = {0.f, 0.f}, top[2] = {INFINITY, INFINITY}, inverse[2] = {0.f, 0.f};
   if (work) row_delta<T, DP>(mg, row, hi, head, p, lane, delta);
   const bool is[2] = {work && row + g < hi, work && row + g + 8 < hi};
   const int64_t at = (int64_t)head * p.n + row + g;
-  if (is[0]) lse[0] = p.lse[at];
-  if (is[1]) lse[1] = p.lse[at + 8];
+  if (is[0]) top[0] = p.top[at], inverse[0] = p.inverse[at];
+  if (is[1]) top[1] = p.top[at + 8], inverse[1] = p.inverse[at + 8];
   float dq[DP / 8][4];
 #pragma unroll
   for (int n = 0; n < DP / 8; ++n) dq[n][0] = dq[n][1] = dq[n][2] = dq[n][3] = 0.f;
@@ -695,7 +697,7 @@ __global__ void __launch_bounds__(THREADS, DP <= 32 ? 4 : DP <= 96 ? 3 : 2) atte
             score = fma2(v.length, slope2, score);
           }
           float x, y;
-          parts(add2(score, both(-lse[r], -lse[r])), x, y);
+          parts(add2(score, both(-top[r], -top[r])), x, y);
           if (last) {
             if (key + n * 8 + 2 * t >= hi) x = -INFINITY;
             if (key + n * 8 + 2 * t + 1 >= hi) y = -INFINITY;
@@ -729,7 +731,7 @@ __global__ void __launch_bounds__(THREADS, DP <= 32 ? 4 : DP <= 96 ? 3 : 2) atte
       float x, y, sums[4];
       if (APART) {
         parts(all[r], x, y);
-        delta[r] = quad_sum(x + y);
+        delta[r] = quad_sum(x + y) * inverse[r];
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -739,6 +741,7 @@ __global__ void __launch_bounds__(THREADS, DP <= 32 ? 4 : DP <= 96 ? 3 : 2) atte
           parts(flat[r][i], x, y);
           sums[i] -= delta[r] * quad_sum(x + y);
         }
+        sums[i] *= inverse[r];
       }
       const float4 v = make_float4(sums[0], -sums[1], -sums[2], -sums[3]);   // u points from the column to the row
       if (is[r] && t == 0) p.geo_row[at + 8 * r] = v;
@@ -748,7 +751,7 @@ __global__ void __launch_bounds__(THREADS, DP <= 32 ? 4 : DP <= 96 ? 3 : 2) atte
     if (is[0]) p.delta[at] = delta[0];
     if (is[1]) p.delta[at + 8] = delta[1];
   }
-  store_rows<T, DP>(const_cast<T*>(mq), p.dq, dq, p.scale, p.scale, row, hi, head, p, lane);
+  store_rows<T, DP>(const_cast<T*>(mq), p.dq, dq, p.scale * inverse[0], p.scale * inverse[1], row, hi, head, p, lane);
 }
 
 // Backward by columns: dk, dv, and with positions the columns' sums of dS u.  The CTA's rows are keys; queries and the output's
@@ -767,7 +770,7 @@ __global__ void __launch_bounds__(THREADS, DP <= 32 ? 4 : DP <= 64 ? 3 : 2) atte
   T* base = reinterpret_cast<T*>(smem) + slot * S::head_elements(2);
   T *keys = base, *values = base + S::TILE * LD, *stage = base + 2 * S::TILE * LD;
   float* spos = reinterpret_cast<float*>(smem + S::bytes(2, 0));
-  float* stats = spos + 6 * KT + slot * 4 * KT;           // [tile][lse, delta][KT]
+  float* stats = spos + 6 * KT + slot * 6 * KT;           // [tile][top, inverse, delta][KT]
   const bool here = head < p.heads;
   const int end = here ? hi : 0;
   if (p.comps * p.size < DP) {
@@ -782,8 +785,9 @@ __global__ void __launch_bounds__(THREADS, DP <= 32 ? 4 : DP <= 64 ? 3 : 2) atte
     for (int i = ht; i < KT; i += S::TH) {
       const bool there = query + i < end;
       const int64_t at = there ? (int64_t)head * p.n + query + i : 0;
-      copy4(stats + (2 * s) * KT + i, p.lse + at, there);
-      copy4(stats + (2 * s + 1) * KT + i, p.delta + at, there);
+      copy4(stats + (3 * s) * KT + i, p.top + at, there);
+      copy4(stats + (3 * s + 1) * KT + i, p.inverse + at, there);
+      copy4(stats + (3 * s + 2) * KT + i, p.delta + at, there);
     }
     if (p.pos) load_positions<KT>(spos + s * 3 * KT, p.pos, query, hi);
     copies_commit();
@@ -828,7 +832,7 @@ __global__ void __launch_bounds__(THREADS, DP <= 32 ? 4 : DP <= 64 ? 3 : 2) atte
     __syncthreads();
     if (work) {
       const T *qs = stage + s * S::STAGE, *gs = qs + KT * LD;
-      const float *ls = stats + 2 * s * KT, *ds = ls + KT;
+      const float* st = stats + 3 * s * KT;
       float z[NT][4], dp[NT][4];
       score_mma<DP, NT, true>(z, mk, qs, lane);
       score_mma<DP, NT, true>(dp, mv, gs, lane);
@@ -837,7 +841,8 @@ __global__ void __launch_bounds__(THREADS, DP <= 32 ? 4 : DP <= 64 ? 3 : 2) atte
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         const int c = n * 8 + 2 * t;
-        const pair lse = *reinterpret_cast<const pair*>(ls + c), delta = *reinterpret_cast<const pair*>(ds + c);
+        const pair top = *reinterpret_cast<const pair*>(st + c), inverse = *reinterpret_cast<const pair*>(st + KT + c),
+                   delta = *reinterpret_cast<const pair*>(st + 2 * KT + c);
         Place columns;
         if (p.pos) columns = columns_at(spos + s * 3 * KT + c, KT);
 #pragma unroll
@@ -850,22 +855,19 @@ __global__ void __launch_bounds__(THREADS, DP <= 32 ? 4 : DP <= 64 ? 3 : 2) atte
             score = fma2(v.length, slope2, score);
           }
           float x, y;
-          parts(fma2(lse, minus, score), x, y);
+          parts(fma2(top, minus, score), x, y);
           if (last) {
             if (query + c >= hi) x = -INFINITY;
             if (query + c + 1 >= hi) y = -INFINITY;
           }
-          x = exp2_fast(x);
-          y = exp2_fast(y);
-          const pair e = mul2(both(x, y), fma2(delta, minus, d));
+          const pair w = mul2(both(exp2_fast(x), exp2_fast(y)), inverse), e = mul2(w, fma2(delta, minus, d));
           if (GEO) {
             const pair ei = mul2(e, v.inverse);
             geo[r][0] = fma2(ei, v.x, geo[r][0]);
             geo[r][1] = fma2(ei, v.y, geo[r][1]);
             geo[r][2] = fma2(ei, v.z, geo[r][2]);
           }
-          z[n][2 * r] = x;
-          z[n][2 * r + 1] = y;
+          parts(w, z[n][2 * r], z[n][2 * r + 1]);
           parts(mul2(e, fma2(mul2(score0, bend2), score0, one2)), dp[n][2 * r], dp[n][2 * r + 1]);
         }
       }
@@ -909,7 +911,7 @@ int launch(Pass pass, const AttentionParams& p, int64_t tiles, bool geo, cudaStr
     kernel<<<grid, THREADS, bytes, s>>>(p);
     return check_launch(what);
   };
-  constexpr int POSITIONS = 2 * 12 * KB, STATS = B::HEADS * 16 * KB;     // two tiles each
+  constexpr int POSITIONS = 2 * 12 * KB, STATS = B::HEADS * 24 * KB;     // two tiles each
   if (pass == FORWARD) return run(attention_forward_kernel<T, DP, WR, KF>, F::bytes(1, 2 * 12 * KF), "attention_forward", 0);
   if (pass == ROWS)
     return geo ? run(attention_rows_kernel<T, DP, WR, KB, true>, B::bytes(2, POSITIONS), "attention_rows", 1)

@@ -15,17 +15,17 @@ from ...ops import attention_op as _ops
 class _GraphAttention(Function):
     @staticmethod
     def forward(ctx, q, k, v, pos, slope, graphs, heads, scale, cap):
-        out, lse = _ops.attention_forward(q, k, v, graphs, heads, scale, cap, pos, slope, any(ctx.needs_input_grad))
-        ctx.save_for_backward(q, k, v, pos, slope, out, lse)
+        out, stats = _ops.attention_forward(q, k, v, graphs, heads, scale, cap, pos, slope, any(ctx.needs_input_grad))
+        ctx.save_for_backward(q, k, v, pos, slope, out, stats)
         ctx.graphs, ctx.heads, ctx.scale, ctx.cap = graphs, heads, scale, cap
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        q, k, v, pos, slope, out, lse = ctx.saved_tensors
+        q, k, v, pos, slope, out, stats = ctx.saved_tensors
         need = ctx.needs_input_grad
-        dq, dk, dv, dslope, dpos = _ops.attention_backward(grad, q, k, v, ctx.graphs, ctx.heads, ctx.scale, ctx.cap, pos, slope, out, lse,
+        dq, dk, dv, dslope, dpos = _ops.attention_backward(grad, q, k, v, ctx.graphs, ctx.heads, ctx.scale, ctx.cap, pos, slope, out, stats,
                                                            need[3] or need[4])
         return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, dpos if need[3] else None,
                 dslope if need[4] else None, None, None, None, None)

@@ -49,14 +49,14 @@ def _rows(x: Tensor) -> Tensor:
     return x if x.stride(2) == 1 or x.shape[2] == 1 else x.contiguous()
 
 
-def _args(q, k, v, graphs, heads, scale, cap, pos, slope, out, lse) -> _lib.AttentionArgs:
+def _args(q, k, v, graphs, heads, scale, cap, pos, slope, out, stats) -> _lib.AttentionArgs:
     n, comps, channels = q.shape
     return _lib.AttentionArgs(
         dtype=_lib.DTYPE_CODE[q.dtype], heads=heads, comps=comps, head_channels=channels // heads, tile_rows=graphs.tile_rows,
         scale=scale, cap=cap or 0.0, n=n, num_tiles=graphs.tiles.shape[0], tiles=graphs.tiles.data_ptr(),
         q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), q_node=q.stride(0), q_comp=q.stride(1), k_node=k.stride(0),
         k_comp=k.stride(1), v_node=v.stride(0), v_comp=v.stride(1), pos=_lib.ptr(pos), slope=_lib.ptr(slope),
-        out=out.data_ptr(), lse=_lib.ptr(lse))
+        out=out.data_ptr(), stats=_lib.ptr(stats))
 
 
 def _new(like: Tensor, graphs: PackedGraphs) -> Tensor:
@@ -65,30 +65,30 @@ def _new(like: Tensor, graphs: PackedGraphs) -> Tensor:
 
 
 def attention_forward(q: Tensor, k: Tensor, v: Tensor, graphs: PackedGraphs, heads: int, scale: float, cap: Optional[float],
-                      pos: Optional[Tensor], slope: Optional[Tensor], want_lse: bool) -> Tuple[Tensor, Optional[Tensor]]:
+                      pos: Optional[Tensor], slope: Optional[Tensor], want_stats: bool) -> Tuple[Tensor, Optional[Tensor]]:
     dev = q.device
     q, k, v = _rows(q), _rows(k), _rows(v)
     pos, slope = (None, None) if pos is None else (pos.contiguous(), slope.contiguous())
     out = _new(q, graphs)
-    lse = torch.empty(heads, q.shape[0], dtype=torch.float32, device=dev) if want_lse else None
-    args = _args(q, k, v, graphs, heads, scale, cap, pos, slope, out, lse)
+    stats = torch.empty(2, heads, q.shape[0], dtype=torch.float32, device=dev) if want_stats else None
+    args = _args(q, k, v, graphs, heads, scale, cap, pos, slope, out, stats)
     with _lib.on_device(dev):
         _lib.check(_lib.lib().eqt_attention_forward(C.byref(args), _lib.stream_ptr(dev)), "eqt_attention_forward")
-    return out, lse
+    return out, stats
 
 
 def attention_backward(grad: Tensor, q: Tensor, k: Tensor, v: Tensor, graphs: PackedGraphs, heads: int, scale: float,
-                       cap: Optional[float], pos: Optional[Tensor], slope: Optional[Tensor], out: Tensor, lse: Tensor,
+                       cap: Optional[float], pos: Optional[Tensor], slope: Optional[Tensor], out: Tensor, stats: Tensor,
                        want_geometry: bool):
     """Gradients of q, k, v and, where wanted, of the slopes and positions (else ``None``)."""
     dev = q.device
     q, k, v, grad = _rows(q), _rows(k), _rows(v), grad.contiguous()
     pos, slope = (None, None) if pos is None else (pos.contiguous(), slope.contiguous())
     dq, dk, dv = _new(q, graphs), _new(q, graphs), _new(q, graphs)
-    args = _args(q, k, v, graphs, heads, scale, cap, pos, slope, out, lse)
+    args = _args(q, k, v, graphs, heads, scale, cap, pos, slope, out, stats)
     args.grad_out, args.dq, args.dk, args.dv = grad.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
     dslope = dpos = None
-    rows = lse.numel()                                   # of scratch: eight numbers of geometry and one of the softmax's gradient each
+    rows = heads * q.shape[0]                             # of scratch: eight numbers of geometry and one of the softmax's gradient each
     scratch = (torch.empty if graphs.covers else torch.zeros)(rows * (9 if want_geometry else 1), dtype=torch.float32, device=dev)
     args.delta = scratch.data_ptr() + 4 * (scratch.numel() - rows)
     if want_geometry:

@@ -660,7 +660,8 @@ int eqt_embedding_grad(int32_t dtype, const void* g, const int64_t* index, void*
  * and components (channels are contiguous); out, grad_out, dq, dk, dv the same shape, contiguous.  A head's comps * head_channels
  * <= 128 values of a node are one vector.  Node i attends to the nodes j of its graph:
  *   s = scale <q_i, k_j>, |scale| <= 1e12;  cap in [1e-12, 1e12] (0: none): s = cap tanh(s / cap);  pos (n, 3) and slope (heads) given: s -= slope[h] |pos_i - pos_j|
- *   out_i = sum_j softmax_j(s) v_j;   lse (heads, n): log2 of the sum of exp(s), written by the forward pass (NULL: not wanted)
+ *   out_i = sum_j softmax_j(s) v_j;   stats (2, heads, n), written by the forward pass (NULL: not wanted): the greatest s of the row
+ * times log2(e), and one over the sum of exp(s) relative to it
  * tiles (num_tiles, 4): first row, first node and one past the last node of the row's graph, 0; a tile is tile_rows (16, 32, 64)
  * rows of one graph, cut at the graph's end.  The tiles are to cover each row at most once and to lie in [0, n); rows of no tile are
  * neither read nor written.  Backward: delta (heads, n) is scratch; dpos (n, 3) and dslope (heads) are both given or both NULL, and
@@ -676,7 +677,7 @@ typedef struct eqt_attention_args {
   int64_t q_node, q_comp, k_node, k_comp, v_node, v_comp;
   const float *pos, *slope;
   void* out;
-  float* lse;
+  float* stats;
   const void* grad_out;
   void *dq, *dk, *dv;
   float* delta;
