@@ -599,7 +599,7 @@ __global__ void __launch_bounds__(THREADS, DP <= 32 ? (WR == 4 ? 5 : sizeof(T) =
 // one over their sum follows at the end.
 // These sums are float32 results also where the features are bfloat16, so there they do not go by the delta of the rounded weights and
 // result: with w = r or u, sum_j dS w = sum_j P dP w - (sum_j P dP) (sum_j P w), and the columns' pass is given sum_j P dP.
-template <typename T, int DP, int WR, int KT, bool GEO>
+template <typename T, int DP, int WR, int KT, bool GEO, bool CAP>
 __global__ void __launch_bounds__(THREADS, DP <= 32 ? 4 : DP <= 96 ? 3 : 2) attention_rows_kernel(const __grid_constant__ AttentionParams p) {
   using S = Shape<T, DP, WR, KT>;
   constexpr int LD = S::LD, NT = KT / 8;
@@ -656,8 +656,8 @@ __global__ void __launch_bounds__(THREADS, DP <= 32 ? 4 : DP <= 96 ? 3 : 2) atte
 #pragma unroll
     for (int i = 0; i < 4; ++i) geo[r][i] = flat[r][i] = 0;
   constexpr bool APART = sizeof(T) == 2;
-  const float to_cap = p.cap > 0.f ? p.scale / p.cap : 0.f, unit = (p.cap > 0.f ? p.cap : p.scale) * LOG2E;   // of a score: the tanh, or the product
-  const float bend = p.cap > 0.f ? -1.f / (unit * unit) : 0.f;             // 1 - tanh^2, from unit tanh; the scale follows at the end
+  const float to_cap = CAP ? p.scale / p.cap : 0.f, unit = (CAP ? p.cap : p.scale) * LOG2E;   // of a score: the tanh, or the product
+  const float bend = -1.f / (unit * unit);                                 // 1 - tanh^2, from unit tanh; the scale follows at the end
   const pair one2 = both(1.f, 1.f), bend2 = both(bend, bend);
   pair slope2 = 0;
   Place place[2];
@@ -681,7 +681,7 @@ __global__ void __launch_bounds__(THREADS, DP <= 32 ? 4 : DP <= 96 ? 3 : 2) atte
       float z[NT][4], dp[NT][4];
       score_mma<DP, NT>(z, mq, ks, lane);
       score_mma<DP, NT>(dp, mg, vs, lane);
-      cap_tile<NT>(z, unit, to_cap, p.cap > 0.f);
+      cap_tile<NT>(z, unit, to_cap, CAP);
       const bool last = key + KT > hi;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
@@ -717,7 +717,9 @@ __global__ void __launch_bounds__(THREADS, DP <= 32 ? 4 : DP <= 96 ? 3 : 2) atte
             geo[r][2] = fma2(fi, v.y, geo[r][2]);
             geo[r][3] = fma2(fi, v.z, geo[r][3]);
           }
-          parts(mul2(e, fma2(mul2(score0, bend2), score0, one2)), z[n][2 * r], z[n][2 * r + 1]);
+          pair dz = e;                                                   // without a cap a score may be minus infinity, its weight zero
+          if (CAP) dz = mul2(e, fma2(mul2(score0, bend2), score0, one2));
+          parts(dz, z[n][2 * r], z[n][2 * r + 1]);
         }
       }
       out_mma<DP, NT>(dq, z, ks, lane);
@@ -756,7 +758,7 @@ __global__ void __launch_bounds__(THREADS, DP <= 32 ? 4 : DP <= 96 ? 3 : 2) atte
 
 // Backward by columns: dk, dv, and with positions the columns' sums of dS u.  The CTA's rows are keys; queries and the output's
 // gradients come by in tiles, and the products are the transposed ones.
-template <typename T, int DP, int WR, int KT, bool GEO>
+template <typename T, int DP, int WR, int KT, bool GEO, bool CAP>
 __global__ void __launch_bounds__(THREADS, DP <= 32 ? 4 : DP <= 64 ? 3 : 2) attention_columns_kernel(const __grid_constant__ AttentionParams p) {
   using S = Shape<T, DP, WR, KT>;
   constexpr int LD = S::LD, NT = KT / 8;
@@ -810,8 +812,8 @@ __global__ void __launch_bounds__(THREADS, DP <= 32 ? 4 : DP <= 64 ? 3 : 2) atte
     dk[n][0] = dk[n][1] = dk[n][2] = dk[n][3] = 0.f;
     dv[n][0] = dv[n][1] = dv[n][2] = dv[n][3] = 0.f;
   }
-  const float to_cap = p.cap > 0.f ? p.scale / p.cap : 0.f, unit = (p.cap > 0.f ? p.cap : p.scale) * LOG2E;
-  const float bend = p.cap > 0.f ? -1.f / (unit * unit) : 0.f;
+  const float to_cap = CAP ? p.scale / p.cap : 0.f, unit = (CAP ? p.cap : p.scale) * LOG2E;
+  const float bend = -1.f / (unit * unit);
   const pair one2 = both(1.f, 1.f), bend2 = both(bend, bend), minus = both(-1.f, -1.f);
   pair slope2 = 0;
   Place place[2];
@@ -836,7 +838,7 @@ __global__ void __launch_bounds__(THREADS, DP <= 32 ? 4 : DP <= 64 ? 3 : 2) atte
       float z[NT][4], dp[NT][4];
       score_mma<DP, NT, true>(z, mk, qs, lane);
       score_mma<DP, NT, true>(dp, mv, gs, lane);
-      cap_tile<NT>(z, unit, to_cap, p.cap > 0.f);
+      cap_tile<NT>(z, unit, to_cap, CAP);
       const bool last = query + KT > hi;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
@@ -868,7 +870,9 @@ __global__ void __launch_bounds__(THREADS, DP <= 32 ? 4 : DP <= 64 ? 3 : 2) atte
             geo[r][2] = fma2(ei, v.z, geo[r][2]);
           }
           parts(w, z[n][2 * r], z[n][2 * r + 1]);
-          parts(mul2(e, fma2(mul2(score0, bend2), score0, one2)), dp[n][2 * r], dp[n][2 * r + 1]);
+          pair dz = e;
+          if (CAP) dz = mul2(e, fma2(mul2(score0, bend2), score0, one2));
+          parts(dz, dp[n][2 * r], dp[n][2 * r + 1]);
         }
       }
       out_mma<DP, NT>(dv, z, gs, lane);
@@ -905,7 +909,7 @@ int launch(Pass pass, const AttentionParams& p, int64_t tiles, bool geo, cudaStr
   const int64_t ctas = tiles * ceil_div(p.heads, F::HEADS);
   if (ctas > INT32_MAX) return fail(EQT_ERR_UNSUPPORTED, "attention: %lld tiles and heads are more than one launch takes", (long long)ctas);
   const unsigned grid = (unsigned)ctas;
-  static std::atomic<uint64_t> allowed[5];                               // of the five kernels below
+  static std::atomic<uint64_t> allowed[9];                               // of the kernels below
   auto run = [&](auto kernel, size_t bytes, const char* what, int which) {
     if (int rc = allow_shared_once(kernel, bytes, allowed[which])) return rc;
     kernel<<<grid, THREADS, bytes, s>>>(p);
@@ -913,11 +917,20 @@ int launch(Pass pass, const AttentionParams& p, int64_t tiles, bool geo, cudaStr
   };
   constexpr int POSITIONS = 2 * 12 * KB, STATS = B::HEADS * 24 * KB;     // two tiles each
   if (pass == FORWARD) return run(attention_forward_kernel<T, DP, WR, KF>, F::bytes(1, 2 * 12 * KF), "attention_forward", 0);
-  if (pass == ROWS)
-    return geo ? run(attention_rows_kernel<T, DP, WR, KB, true>, B::bytes(2, POSITIONS), "attention_rows", 1)
-               : run(attention_rows_kernel<T, DP, WR, KB, false>, B::bytes(2, POSITIONS), "attention_rows", 2);
-  return geo ? run(attention_columns_kernel<T, DP, WR, KB, true>, B::bytes(2, POSITIONS + STATS), "attention_columns", 3)
-             : run(attention_columns_kernel<T, DP, WR, KB, false>, B::bytes(2, POSITIONS + STATS), "attention_columns", 4);
+  const bool cap = p.cap > 0.f;
+  const int which = 2 * geo + cap;
+  if (pass == ROWS) {
+    constexpr size_t bytes = B::bytes(2, POSITIONS);
+    if (geo) return cap ? run(attention_rows_kernel<T, DP, WR, KB, true, true>, bytes, "attention_rows", 1 + which)
+                        : run(attention_rows_kernel<T, DP, WR, KB, true, false>, bytes, "attention_rows", 1 + which);
+    return cap ? run(attention_rows_kernel<T, DP, WR, KB, false, true>, bytes, "attention_rows", 1 + which)
+               : run(attention_rows_kernel<T, DP, WR, KB, false, false>, bytes, "attention_rows", 1 + which);
+  }
+  constexpr size_t bytes = B::bytes(2, POSITIONS + STATS);
+  if (geo) return cap ? run(attention_columns_kernel<T, DP, WR, KB, true, true>, bytes, "attention_columns", 5 + which)
+                      : run(attention_columns_kernel<T, DP, WR, KB, true, false>, bytes, "attention_columns", 5 + which);
+  return cap ? run(attention_columns_kernel<T, DP, WR, KB, false, true>, bytes, "attention_columns", 5 + which)
+             : run(attention_columns_kernel<T, DP, WR, KB, false, false>, bytes, "attention_columns", 5 + which);
 }
 
 template <typename T, int DP>

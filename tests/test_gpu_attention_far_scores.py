@@ -48,3 +48,40 @@ def test_equal_greatest_scores(dtype, n, alike, size, capped, bias):
         over = (x.double()[:, 0] - want).abs() / tol.clamp(min=1e-300)
         assert over.max() <= 1, f"{name}: {float(over.max()):.3g} times its bound"
     assert not bias or not (got[4].any() or got[5].any())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n", [15, 40, 200])
+@pytest.mark.parametrize("bias", [False, True])
+def test_products_of_minus_infinity(dtype, n, bias):
+    """Keys whose products leave the range of the type: nobody sees them, and every gradient is what it is without them."""
+    g = torch.Generator().manual_seed(2)
+    q, k, v, cot = (torch.randn(n, 1, 32, generator=g) for _ in range(4))
+    q[:, 0, 0], k[:, 0, 0] = 100.0, 0.0
+    q[[0, n - 1], 0, 0] = 0.0                                                               # these two see them
+    k[5:9, 0, 0] = -5e36                                                                    # -5e38 is past float32's -3.4e38
+    leaves = [t.to(dtype).to(DEV).requires_grad_(True) for t in (q, k, v)]
+    if bias:
+        leaves += [torch.rand(n, 3, generator=g).to(DEV).requires_grad_(True), torch.ones(1, device=DEV).requires_grad_(True)]
+    cot = cot.to(dtype).to(DEV)
+
+    def run(leaves, cot):
+        n = cot.shape[0]
+        out = F.graph_attention(*leaves[:3], PackedGraphs(torch.tensor([0, n], device=DEV), n), 1, 0.5, None, *leaves[3:])
+        return [out.detach(), *torch.autograd.grad(out, leaves, cot)]
+    got = run(leaves, cot)
+    assert all(torch.isfinite(t).all() for t in got)
+    cot[0] = cot[n - 1] = 0                                                                 # and now nobody's result has anything of them
+    got = run(leaves, cot)
+    assert not got[2][5:9].any() and not got[3][5:9].any()
+    seen = torch.ones(n, dtype=torch.bool, device=DEV)
+    seen[5:9] = False
+    # the same terms in tiles that begin elsewhere: roundings of sums and results, and for bfloat16 of the weights; rows 5 to 8 themselves
+    # attend to the others, so gradients of k and v are compared where those rows have no cotangent
+    cot[5:9] = 0
+    got, few = run(leaves, cot), run([t.detach()[seen].requires_grad_(True) for t in leaves[:4]] + leaves[4:], cot[seen])
+    u = 2.0 ** -6 if dtype == torch.bfloat16 else 2.0 ** -18
+    got[0][[0, n - 1]], few[0][[0, -1]] = 0, 0                                              # these two see them
+    for a, b in zip(got[:5], few[:5]):                                                      # of features and positions, row by row
+        a = a[seen]
+        assert (a.double() - b.double()).norm() <= u * b.double().norm()
