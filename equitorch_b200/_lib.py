@@ -90,7 +90,7 @@ class UvwRoleStruct(C.Structure):
 
 class AttentionArgs(C.Structure):
     _fields_ = ([(f, C.c_int32) for f in ("dtype", "heads", "comps", "head_channels", "tile_rows")] + [("scale", C.c_float), ("cap", C.c_float)]
-                + [("n", C.c_int64), ("num_tiles", C.c_int64)] + [(f, C.c_void_p) for f in ("tiles", "q", "k", "v")]
+                + [(f, C.c_int64) for f in ("n", "longest", "num_tiles")] + [(f, C.c_void_p) for f in ("tiles", "q", "k", "v")]
                 + [(f, C.c_int64) for f in ("q_node", "q_comp", "k_node", "k_comp", "v_node", "v_comp")]
                 + [(f, C.c_void_p) for f in ("pos", "slope", "out", "stats", "grad_out", "dq", "dk", "dv", "delta", "geo", "dpos", "dslope")])
 

@@ -48,25 +48,28 @@ __device__ __forceinline__ int size_class(int64_t size) {
   return CLASSES - 1 - min(CLASSES - 1, 2 * octave + (octave ? (int)(size >> (octave - 1)) & 1 : 0));
 }
 
-// stats: first boundary, last boundary, least size, and how many tiles of 16, 32 and 64 rows there are.
+// stats: first boundary, last boundary, least and greatest size, and how many tiles of 16, 32 and 64 rows there are.
 __global__ void __launch_bounds__(PACK_THREADS) pack_stats_kernel(const int64_t* __restrict__ ptr, int64_t graphs, int64_t* __restrict__ stats) {
-  __shared__ long long least, tiles[3];
-  if (threadIdx.x == 0) least = INT64_MAX, tiles[0] = tiles[1] = tiles[2] = 0;
+  __shared__ long long least, greatest, tiles[3];
+  if (threadIdx.x == 0) least = INT64_MAX, greatest = 0, tiles[0] = tiles[1] = tiles[2] = 0;
   __syncthreads();
-  long long low = INT64_MAX, sum[3] = {0, 0, 0};
+  long long low = INT64_MAX, high = 0, sum[3] = {0, 0, 0};
   for (int64_t g = threadIdx.x; g < graphs; g += PACK_THREADS) {
     const int64_t size = ptr[g + 1] - ptr[g];
     low = min(low, (long long)size);
+    high = max(high, (long long)size);
     for (int i = 0; i < 3; ++i) sum[i] += size > 0 ? (size + (16 << i) - 1) >> (4 + i) : 0;
   }
   atomicMin(&least, low);
+  atomicMax(&greatest, high);
   for (int i = 0; i < 3; ++i) atomicAdd(reinterpret_cast<unsigned long long*>(&tiles[i]), (unsigned long long)sum[i]);
   __syncthreads();
   if (threadIdx.x == 0) {
     stats[0] = ptr[0];
     stats[1] = ptr[graphs];
     stats[2] = graphs ? least : 0;
-    for (int i = 0; i < 3; ++i) stats[3 + i] = tiles[i];
+    stats[3] = greatest;
+    for (int i = 0; i < 3; ++i) stats[4 + i] = tiles[i];
   }
 }
 
@@ -118,7 +121,7 @@ int launch_all(Pass pass, const eqt_attention_args* a, const AttentionParams& p,
 int fill(const eqt_attention_args* a, AttentionParams& p, bool backward) {
   if (!a) return fail(EQT_ERR_BAD_ARGUMENT, "attention: NULL arguments");
   if (a->dtype != EQT_F32 && a->dtype != EQT_BF16) return fail(EQT_ERR_UNSUPPORTED, "attention: float32 or bfloat16 features expected");
-  if (a->n < 0 || a->num_tiles < 0 || a->heads < 1 || a->comps < 1 || a->head_channels < 1)
+  if (a->n < 0 || a->longest < 0 || a->num_tiles < 0 || a->heads < 1 || a->comps < 1 || a->head_channels < 1)
     return fail(EQT_ERR_BAD_ARGUMENT, "attention: sizes must be positive");
   if (a->tile_rows != 16 && a->tile_rows != 32 && a->tile_rows != 64) return fail(EQT_ERR_BAD_ARGUMENT, "attention: tiles have 16, 32 or 64 rows");
   if (a->n > INT32_MAX - 64 || a->num_tiles > INT32_MAX || a->heads > 65535)
@@ -156,6 +159,10 @@ int fill(const eqt_attention_args* a, AttentionParams& p, bool backward) {
   p.heads = a->heads;
   p.comps = a->comps;
   p.size = a->head_channels;
+  const int64_t longest = a->longest ? a->longest : a->n;
+  p.folds = a->dtype == EQT_BF16 && longest > FOLD;
+  if (p.folds && a->num_tiles && a->tile_rows != 64)
+    return fail(EQT_ERR_UNSUPPORTED, "attention: bfloat16 with graphs of more than %d nodes needs tiles of 64 rows, got %d", FOLD, a->tile_rows);
   p.scale = a->scale;
   p.cap = a->cap;
   uintptr_t bits = (uintptr_t)a->head_channels * size;

@@ -50,6 +50,7 @@ struct AttentionParams {
   int64_t n;
   int heads, comps, size;    // size: channels a head
   float scale, cap;          // cap 0: none
+  int folds;                 // bfloat16: a graph of more than FOLD nodes
   int vec;                   // 16-byte pieces of every operand lie on 16-byte boundaries
 };
 
@@ -199,6 +200,35 @@ __device__ __forceinline__ void out_mma(float (&o)[DP / 8][4], const float (&p)[
 #pragma unroll
       for (int i = 0; i < 4; ++i) o[d + e][i] += s[e][i];
   }
+}
+
+// The bfloat16 products add up in the matrix instructions, whose adder truncates: a sum of one sign loses 1.2e-7 of itself at every step of
+// 16 terms (outputs of 400,000 nodes: 3e-3, as much as their rounding).  So every FOLD terms a sum joins, with ordinary rounding, another
+// one that waits in local memory; 4096 terms lose 3e-5.  Only the kernels for graphs that are longer do so (FOLDS), which take tiles of 64 rows:
+// the code costs the others 3 % in registers.  float32 sums join after every tile anyway.
+constexpr int FOLD = 4096;
+template <int DP, int MORE = 0> struct Far {             // a thread's sums, and MORE numbers beside them
+  float values[DP / 2 + MORE];
+  __device__ __forceinline__ float* at() {
+    float* p = values;
+    asm volatile("" : "+l"(p));                          // values stay in memory: their address is known to no one
+    return p;
+  }
+};
+template <int DP> __device__ __forceinline__ void fold(float* far, float (&o)[DP / 8][4], bool first, float keep0 = 1.f, float keep1 = 1.f) {
+#pragma unroll
+  for (int n = 0; n < DP / 8; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      far[4 * n + i] = first ? o[n][i] : fmaf(far[4 * n + i], i < 2 ? keep0 : keep1, o[n][i]);
+      o[n][i] = 0.f;
+    }
+}
+template <int DP> __device__ __forceinline__ void unfold(const float* far, float (&o)[DP / 8][4], float keep0 = 1.f, float keep1 = 1.f) {
+#pragma unroll
+  for (int n = 0; n < DP / 8; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[n][i] = fmaf(far[4 * n + i], i < 2 ? keep0 : keep1, o[n][i]);
 }
 
 // ---- special functions --------------------------------------------------------------------------
@@ -462,7 +492,7 @@ template <typename T, int DP, int WR, int KT> struct Shape {
 
 // CTAs an SM, here and below: as measured, against one more or fewer (forward, heads of 32: ragged graphs 167 us with 5, 175 with 6, 190 with
 // 7, molecules 81, 76 and 74; backward, molecules: by rows 141 with 4, 158 with 3, 164 with 5).
-template <typename T, int DP, int WR, int KT>
+template <typename T, int DP, int WR, int KT, bool FOLDS>
 __global__ void __launch_bounds__(THREADS, DP <= 32 ? (WR == 4 ? 5 : sizeof(T) == 2 ? 7 : 6) : DP <= 64 ? 4 : 3) attention_forward_kernel(const __grid_constant__ AttentionParams p) {
   using S = Shape<T, DP, WR, KT>;
   constexpr int LD = S::LD, NT = KT / 8;
@@ -512,78 +542,93 @@ __global__ void __launch_bounds__(THREADS, DP <= 32 ? (WR == 4 ? 5 : sizeof(T) =
     at[0] = minus_position(p.pos, row + g, hi);
     at[1] = minus_position(p.pos, row + g + 8, hi);
   }
-  int s = 0;
-  for (int key = lo; key < hi; key += KT, s ^= 1) {
-    if (key + KT < hi) {
-      fetch(key + KT, s ^ 1);
-      copies_wait<1>();
-    } else {
-      copies_wait<0>();
-    }
-    __syncthreads();
-    if (work) {
-      const T *ks = stage + s * S::STAGE, *vs = ks + KT * LD;
-      float z[NT][4];
-      score_mma<DP, NT>(z, mine, ks, lane);
-      cap_tile<NT>(z, unit, to_cap, p.cap > 0.f);
-      if (p.pos) {
+  Far<DP, 2> waiting;                                                    // and the greatest scores that it goes by
+  auto keep_far = [&](const float* far, int r) { return exp2_fast(far[DP / 2 + r] - (top[r] == -INFINITY ? 0.f : top[r])); };
+  int s = 0, key = lo;
+  do {
+    const int stop = FOLDS && hi - key > FOLD ? key + FOLD : hi;
+    for (; key < stop; key += KT, s ^= 1) {
+      if (key + KT < hi) {
+        fetch(key + KT, s ^ 1);
+        copies_wait<1>();
+      } else {
+        copies_wait<0>();
+      }
+      __syncthreads();
+      if (work) {
+        const T *ks = stage + s * S::STAGE, *vs = ks + KT * LD;
+        float z[NT][4];
+        score_mma<DP, NT>(z, mine, ks, lane);
+        cap_tile<NT>(z, unit, to_cap, p.cap > 0.f);
+        if (p.pos) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const Place columns = columns_at(spos + s * 3 * KT + n * 8 + 2 * t, KT);
+          for (int n = 0; n < NT; ++n) {
+            const Place columns = columns_at(spos + s * 3 * KT + n * 8 + 2 * t, KT);
 #pragma unroll
-          for (int r = 0; r < 2; ++r)
-            parts(fma2(way_to(columns, at[r]).length, slope2, both(z[n][2 * r], z[n][2 * r + 1])), z[n][2 * r], z[n][2 * r + 1]);
+            for (int r = 0; r < 2; ++r)
+              parts(fma2(way_to(columns, at[r]).length, slope2, both(z[n][2 * r], z[n][2 * r + 1])), z[n][2 * r], z[n][2 * r + 1]);
+          }
         }
-      }
-      if (key + KT > hi) {
+        if (key + KT > hi) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+          for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
-            if (key + n * 8 + 2 * t + i >= hi) z[n][i] = z[n][2 + i] = -INFINITY;
-      }
-      float most[2], keep[2];
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        float m = top[r];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) m = fmaxf(m, fmaxf(z[n][2 * r], z[n][2 * r + 1]));
-        most[r] = quad_max(m);
-      }
-      if (__any_sync(0xffffffffu, most[0] > top[0] || most[1] > top[1])) {             // the running sums have a new unit
+            for (int i = 0; i < 2; ++i)
+              if (key + n * 8 + 2 * t + i >= hi) z[n][i] = z[n][2 + i] = -INFINITY;
+        }
+        float most[2], keep[2];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          keep[r] = exp2_fast(top[r] - (most[r] == -INFINITY ? 0.f : most[r]));
-          sum[r] *= keep[r];
-          top[r] = most[r];
+          float m = top[r];
+#pragma unroll
+          for (int n = 0; n < NT; ++n) m = fmaxf(m, fmaxf(z[n][2 * r], z[n][2 * r + 1]));
+          most[r] = quad_max(m);
+        }
+        if (__any_sync(0xffffffffu, most[0] > top[0] || most[1] > top[1])) {             // the running sums have a new unit
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            keep[r] = exp2_fast(top[r] - (most[r] == -INFINITY ? 0.f : most[r]));
+            sum[r] *= keep[r];
+            top[r] = most[r];
+          }
+#pragma unroll
+          for (int n = 0; n < DP / 8; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[n][i] *= keep[i >> 1];
         }
 #pragma unroll
-        for (int n = 0; n < DP / 8; ++n)
+        for (int r = 0; r < 2; ++r) {
+          const float from = top[r] == -INFINITY ? 0.f : -top[r];
+          const pair shift = both(from, from);
+          pair add = 0;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) o[n][i] *= keep[i >> 1];
-      }
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const float from = top[r] == -INFINITY ? 0.f : -top[r];
-        const pair shift = both(from, from);
-        pair add = 0;
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
+          for (int n = 0; n < NT; ++n) {
+            float x, y;
+            parts(add2(both(z[n][2 * r], z[n][2 * r + 1]), shift), x, y);
+            z[n][2 * r] = exp2_fast(x);
+            z[n][2 * r + 1] = exp2_fast(y);
+            add = add2(add, both(z[n][2 * r], z[n][2 * r + 1]));
+          }
           float x, y;
-          parts(add2(both(z[n][2 * r], z[n][2 * r + 1]), shift), x, y);
-          z[n][2 * r] = exp2_fast(x);
-          z[n][2 * r + 1] = exp2_fast(y);
-          add = add2(add, both(z[n][2 * r], z[n][2 * r + 1]));
+          parts(add, x, y);
+          sum[r] += x + y;
         }
-        float x, y;
-        parts(add, x, y);
-        sum[r] += x + y;
+        out_mma<DP, NT>(o, z, vs, lane);
       }
-      out_mma<DP, NT>(o, z, vs, lane);
+      __syncthreads();
     }
-    __syncthreads();
-  }
+    if (FOLDS && key < hi && work) {
+      float* far = waiting.at();
+      const bool first_time = key - lo == FOLD;
+      fold<DP>(far, o, first_time, first_time ? 1.f : keep_far(far, 0), first_time ? 1.f : keep_far(far, 1));
+      far[DP / 2] = top[0], far[DP / 2 + 1] = top[1];
+    }
+  } while (FOLDS && key < hi);
   if (!work) return;
+  if (FOLDS && hi - lo > FOLD) {
+    const float* far = waiting.at();
+    unfold<DP>(far, o, keep_far(far, 0), keep_far(far, 1));
+  }
   sum[0] = quad_sum(sum[0]);
   sum[1] = quad_sum(sum[1]);
   const float f0 = 1.f / sum[0], f1 = 1.f / sum[1];
@@ -599,7 +644,7 @@ __global__ void __launch_bounds__(THREADS, DP <= 32 ? (WR == 4 ? 5 : sizeof(T) =
 // one over their sum follows at the end.
 // These sums are float32 results also where the features are bfloat16, so there they do not go by the delta of the rounded weights and
 // result: with w = r or u, sum_j dS w = sum_j P dP w - (sum_j P dP) (sum_j P w), and the columns' pass is given sum_j P dP.
-template <typename T, int DP, int WR, int KT, bool GEO, bool CAP>
+template <typename T, int DP, int WR, int KT, bool FOLDS, bool GEO, bool CAP>
 __global__ void __launch_bounds__(THREADS, DP <= 32 ? 4 : DP <= 96 ? 3 : 2) attention_rows_kernel(const __grid_constant__ AttentionParams p) {
   using S = Shape<T, DP, WR, KT>;
   constexpr int LD = S::LD, NT = KT / 8;
@@ -667,66 +712,72 @@ __global__ void __launch_bounds__(THREADS, DP <= 32 ? 4 : DP <= 96 ? 3 : 2) atte
     place[0] = minus_position(p.pos, row + g, hi);
     place[1] = minus_position(p.pos, row + g + 8, hi);
   }
-  int s = 0;
-  for (int key = lo; key < hi; key += KT, s ^= 1) {
-    if (key + KT < hi) {
-      fetch(key + KT, s ^ 1);
-      copies_wait<1>();
-    } else {
-      copies_wait<0>();
-    }
-    __syncthreads();
-    if (work) {
-      const T *ks = stage + s * S::STAGE, *vs = ks + KT * LD;
-      float z[NT][4], dp[NT][4];
-      score_mma<DP, NT>(z, mq, ks, lane);
-      score_mma<DP, NT>(dp, mg, vs, lane);
-      cap_tile<NT>(z, unit, to_cap, CAP);
-      const bool last = key + KT > hi;
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        Place columns;
-        if (p.pos) columns = columns_at(spos + s * 3 * KT + n * 8 + 2 * t, KT);
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const pair score0 = both(z[n][2 * r], z[n][2 * r + 1]), d = both(dp[n][2 * r], dp[n][2 * r + 1]);
-          pair score = score0;
-          Way v;
-          if (p.pos) {
-            v = way_to(columns, place[r]);
-            score = fma2(v.length, slope2, score);
-          }
-          float x, y;
-          parts(add2(score, both(-top[r], -top[r])), x, y);
-          if (last) {
-            if (key + n * 8 + 2 * t >= hi) x = -INFINITY;
-            if (key + n * 8 + 2 * t + 1 >= hi) y = -INFINITY;
-          }
-          const pair w = both(exp2_fast(x), exp2_fast(y)), e = mul2(w, add2(d, both(-delta[r], -delta[r])));
-          if (GEO) {
-            const pair f = APART ? mul2(w, d) : e, fi = mul2(f, v.inverse), wi = mul2(w, v.inverse);
-            if (APART) {
-              all[r] = add2(all[r], f);
-              flat[r][0] = fma2(w, v.length, flat[r][0]);
-              flat[r][1] = fma2(wi, v.x, flat[r][1]);
-              flat[r][2] = fma2(wi, v.y, flat[r][2]);
-              flat[r][3] = fma2(wi, v.z, flat[r][3]);
-            }
-            geo[r][0] = fma2(f, v.length, geo[r][0]);
-            geo[r][1] = fma2(fi, v.x, geo[r][1]);
-            geo[r][2] = fma2(fi, v.y, geo[r][2]);
-            geo[r][3] = fma2(fi, v.z, geo[r][3]);
-          }
-          pair dz = e;                                                   // without a cap a score may be minus infinity, its weight zero
-          if (CAP) dz = mul2(e, fma2(mul2(score0, bend2), score0, one2));
-          parts(dz, z[n][2 * r], z[n][2 * r + 1]);
-        }
+  Far<DP> waiting;
+  int s = 0, key = lo;
+  do {
+    const int stop = FOLDS && hi - key > FOLD ? key + FOLD : hi;
+    for (; key < stop; key += KT, s ^= 1) {
+      if (key + KT < hi) {
+        fetch(key + KT, s ^ 1);
+        copies_wait<1>();
+      } else {
+        copies_wait<0>();
       }
-      out_mma<DP, NT>(dq, z, ks, lane);
+      __syncthreads();
+      if (work) {
+        const T *ks = stage + s * S::STAGE, *vs = ks + KT * LD;
+        float z[NT][4], dp[NT][4];
+        score_mma<DP, NT>(z, mq, ks, lane);
+        score_mma<DP, NT>(dp, mg, vs, lane);
+        cap_tile<NT>(z, unit, to_cap, CAP);
+        const bool last = key + KT > hi;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          Place columns;
+          if (p.pos) columns = columns_at(spos + s * 3 * KT + n * 8 + 2 * t, KT);
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const pair score0 = both(z[n][2 * r], z[n][2 * r + 1]), d = both(dp[n][2 * r], dp[n][2 * r + 1]);
+            pair score = score0;
+            Way v;
+            if (p.pos) {
+              v = way_to(columns, place[r]);
+              score = fma2(v.length, slope2, score);
+            }
+            float x, y;
+            parts(add2(score, both(-top[r], -top[r])), x, y);
+            if (last) {
+              if (key + n * 8 + 2 * t >= hi) x = -INFINITY;
+              if (key + n * 8 + 2 * t + 1 >= hi) y = -INFINITY;
+            }
+            const pair w = both(exp2_fast(x), exp2_fast(y)), e = mul2(w, add2(d, both(-delta[r], -delta[r])));
+            if (GEO) {
+              const pair f = APART ? mul2(w, d) : e, fi = mul2(f, v.inverse), wi = mul2(w, v.inverse);
+              if (APART) {
+                all[r] = add2(all[r], f);
+                flat[r][0] = fma2(w, v.length, flat[r][0]);
+                flat[r][1] = fma2(wi, v.x, flat[r][1]);
+                flat[r][2] = fma2(wi, v.y, flat[r][2]);
+                flat[r][3] = fma2(wi, v.z, flat[r][3]);
+              }
+              geo[r][0] = fma2(f, v.length, geo[r][0]);
+              geo[r][1] = fma2(fi, v.x, geo[r][1]);
+              geo[r][2] = fma2(fi, v.y, geo[r][2]);
+              geo[r][3] = fma2(fi, v.z, geo[r][3]);
+            }
+            pair dz = e;                                                   // without a cap a score may be minus infinity, its weight zero
+            if (CAP) dz = mul2(e, fma2(mul2(score0, bend2), score0, one2));
+            parts(dz, z[n][2 * r], z[n][2 * r + 1]);
+          }
+        }
+        out_mma<DP, NT>(dq, z, ks, lane);
+      }
+      __syncthreads();
     }
-    __syncthreads();
-  }
+    if (FOLDS && key < hi && work) fold<DP>(waiting.at(), dq, key - lo == FOLD);
+  } while (FOLDS && key < hi);
   if (!work) return;
+  if (FOLDS && hi - lo > FOLD) unfold<DP>(waiting.at(), dq);
   if (GEO) {
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
@@ -758,7 +809,7 @@ __global__ void __launch_bounds__(THREADS, DP <= 32 ? 4 : DP <= 96 ? 3 : 2) atte
 
 // Backward by columns: dk, dv, and with positions the columns' sums of dS u.  The CTA's rows are keys; queries and the output's
 // gradients come by in tiles, and the products are the transposed ones.
-template <typename T, int DP, int WR, int KT, bool GEO, bool CAP>
+template <typename T, int DP, int WR, int KT, bool FOLDS, bool GEO, bool CAP>
 __global__ void __launch_bounds__(THREADS, DP <= 32 ? 4 : DP <= 64 ? 3 : 2) attention_columns_kernel(const __grid_constant__ AttentionParams p) {
   using S = Shape<T, DP, WR, KT>;
   constexpr int LD = S::LD, NT = KT / 8;
@@ -823,64 +874,76 @@ __global__ void __launch_bounds__(THREADS, DP <= 32 ? 4 : DP <= 64 ? 3 : 2) atte
     place[0] = minus_position(p.pos, row + g, hi);
     place[1] = minus_position(p.pos, row + g + 8, hi);
   }
-  int s = 0;
-  for (int query = lo; query < hi; query += KT, s ^= 1) {
-    if (query + KT < hi) {
-      fetch(query + KT, s ^ 1);
-      copies_wait<1>();
-    } else {
-      copies_wait<0>();
-    }
-    __syncthreads();
-    if (work) {
-      const T *qs = stage + s * S::STAGE, *gs = qs + KT * LD;
-      const float* st = stats + 3 * s * KT;
-      float z[NT][4], dp[NT][4];
-      score_mma<DP, NT, true>(z, mk, qs, lane);
-      score_mma<DP, NT, true>(dp, mv, gs, lane);
-      cap_tile<NT>(z, unit, to_cap, CAP);
-      const bool last = query + KT > hi;
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const int c = n * 8 + 2 * t;
-        const pair top = *reinterpret_cast<const pair*>(st + c), inverse = *reinterpret_cast<const pair*>(st + KT + c),
-                   delta = *reinterpret_cast<const pair*>(st + 2 * KT + c);
-        Place columns;
-        if (p.pos) columns = columns_at(spos + s * 3 * KT + c, KT);
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const pair score0 = both(z[n][2 * r], z[n][2 * r + 1]), d = both(dp[n][2 * r], dp[n][2 * r + 1]);
-          pair score = score0;
-          Way v;
-          if (p.pos) {                                                   // from the key to the query
-            v = way_to(columns, place[r]);
-            score = fma2(v.length, slope2, score);
-          }
-          float x, y;
-          parts(fma2(top, minus, score), x, y);
-          if (last) {
-            if (query + c >= hi) x = -INFINITY;
-            if (query + c + 1 >= hi) y = -INFINITY;
-          }
-          const pair w = mul2(both(exp2_fast(x), exp2_fast(y)), inverse), e = mul2(w, fma2(delta, minus, d));
-          if (GEO) {
-            const pair ei = mul2(e, v.inverse);
-            geo[r][0] = fma2(ei, v.x, geo[r][0]);
-            geo[r][1] = fma2(ei, v.y, geo[r][1]);
-            geo[r][2] = fma2(ei, v.z, geo[r][2]);
-          }
-          parts(w, z[n][2 * r], z[n][2 * r + 1]);
-          pair dz = e;
-          if (CAP) dz = mul2(e, fma2(mul2(score0, bend2), score0, one2));
-          parts(dz, dp[n][2 * r], dp[n][2 * r + 1]);
-        }
+  Far<DP> waiting_k, waiting_v;
+  int s = 0, query = lo;
+  do {
+    const int stop = FOLDS && hi - query > FOLD ? query + FOLD : hi;
+    for (; query < stop; query += KT, s ^= 1) {
+      if (query + KT < hi) {
+        fetch(query + KT, s ^ 1);
+        copies_wait<1>();
+      } else {
+        copies_wait<0>();
       }
-      out_mma<DP, NT>(dv, z, gs, lane);
-      out_mma<DP, NT>(dk, dp, qs, lane);
+      __syncthreads();
+      if (work) {
+        const T *qs = stage + s * S::STAGE, *gs = qs + KT * LD;
+        const float* st = stats + 3 * s * KT;
+        float z[NT][4], dp[NT][4];
+        score_mma<DP, NT, true>(z, mk, qs, lane);
+        score_mma<DP, NT, true>(dp, mv, gs, lane);
+        cap_tile<NT>(z, unit, to_cap, CAP);
+        const bool last = query + KT > hi;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const int c = n * 8 + 2 * t;
+          const pair top = *reinterpret_cast<const pair*>(st + c), inverse = *reinterpret_cast<const pair*>(st + KT + c),
+                     delta = *reinterpret_cast<const pair*>(st + 2 * KT + c);
+          Place columns;
+          if (p.pos) columns = columns_at(spos + s * 3 * KT + c, KT);
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const pair score0 = both(z[n][2 * r], z[n][2 * r + 1]), d = both(dp[n][2 * r], dp[n][2 * r + 1]);
+            pair score = score0;
+            Way v;
+            if (p.pos) {                                                   // from the key to the query
+              v = way_to(columns, place[r]);
+              score = fma2(v.length, slope2, score);
+            }
+            float x, y;
+            parts(fma2(top, minus, score), x, y);
+            if (last) {
+              if (query + c >= hi) x = -INFINITY;
+              if (query + c + 1 >= hi) y = -INFINITY;
+            }
+            const pair w = mul2(both(exp2_fast(x), exp2_fast(y)), inverse), e = mul2(w, fma2(delta, minus, d));
+            if (GEO) {
+              const pair ei = mul2(e, v.inverse);
+              geo[r][0] = fma2(ei, v.x, geo[r][0]);
+              geo[r][1] = fma2(ei, v.y, geo[r][1]);
+              geo[r][2] = fma2(ei, v.z, geo[r][2]);
+            }
+            parts(w, z[n][2 * r], z[n][2 * r + 1]);
+            pair dz = e;
+            if (CAP) dz = mul2(e, fma2(mul2(score0, bend2), score0, one2));
+            parts(dz, dp[n][2 * r], dp[n][2 * r + 1]);
+          }
+        }
+        out_mma<DP, NT>(dv, z, gs, lane);
+        out_mma<DP, NT>(dk, dp, qs, lane);
+      }
+      __syncthreads();
     }
-    __syncthreads();
-  }
+    if (FOLDS && query < hi && work) {
+      fold<DP>(waiting_k.at(), dk, query - lo == FOLD);
+      fold<DP>(waiting_v.at(), dv, query - lo == FOLD);
+    }
+  } while (FOLDS && query < hi);
   if (!work) return;
+  if (FOLDS && hi - lo > FOLD) {
+    unfold<DP>(waiting_k.at(), dk);
+    unfold<DP>(waiting_v.at(), dv);
+  }
   if (GEO) {
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
@@ -902,7 +965,7 @@ __global__ void __launch_bounds__(THREADS, DP <= 32 ? 4 : DP <= 64 ? 3 : 2) atte
 enum Pass { FORWARD, ROWS, COLUMNS };
 
 // KF and KB: keys, or queries, of a tile in the forward and in the backward pass
-template <typename T, int DP, int WR, int KF, int KB>
+template <typename T, int DP, int WR, int KF, int KB, bool FOLDS = false>
 int launch(Pass pass, const AttentionParams& p, int64_t tiles, bool geo, cudaStream_t s) {
   using F = Shape<T, DP, WR, KF>;
   using B = Shape<T, DP, WR, KB>;
@@ -916,21 +979,21 @@ int launch(Pass pass, const AttentionParams& p, int64_t tiles, bool geo, cudaStr
     return check_launch(what);
   };
   constexpr int POSITIONS = 2 * 12 * KB, STATS = B::HEADS * 24 * KB;     // two tiles each
-  if (pass == FORWARD) return run(attention_forward_kernel<T, DP, WR, KF>, F::bytes(1, 2 * 12 * KF), "attention_forward", 0);
+  if (pass == FORWARD) return run(attention_forward_kernel<T, DP, WR, KF, FOLDS>, F::bytes(1, 2 * 12 * KF), "attention_forward", 0);
   const bool cap = p.cap > 0.f;
   const int which = 2 * geo + cap;
   if (pass == ROWS) {
     constexpr size_t bytes = B::bytes(2, POSITIONS);
-    if (geo) return cap ? run(attention_rows_kernel<T, DP, WR, KB, true, true>, bytes, "attention_rows", 1 + which)
-                        : run(attention_rows_kernel<T, DP, WR, KB, true, false>, bytes, "attention_rows", 1 + which);
-    return cap ? run(attention_rows_kernel<T, DP, WR, KB, false, true>, bytes, "attention_rows", 1 + which)
-               : run(attention_rows_kernel<T, DP, WR, KB, false, false>, bytes, "attention_rows", 1 + which);
+    if (geo) return cap ? run(attention_rows_kernel<T, DP, WR, KB, FOLDS, true, true>, bytes, "attention_rows", 1 + which)
+                        : run(attention_rows_kernel<T, DP, WR, KB, FOLDS, true, false>, bytes, "attention_rows", 1 + which);
+    return cap ? run(attention_rows_kernel<T, DP, WR, KB, FOLDS, false, true>, bytes, "attention_rows", 1 + which)
+               : run(attention_rows_kernel<T, DP, WR, KB, FOLDS, false, false>, bytes, "attention_rows", 1 + which);
   }
   constexpr size_t bytes = B::bytes(2, POSITIONS + STATS);
-  if (geo) return cap ? run(attention_columns_kernel<T, DP, WR, KB, true, true>, bytes, "attention_columns", 5 + which)
-                      : run(attention_columns_kernel<T, DP, WR, KB, true, false>, bytes, "attention_columns", 5 + which);
-  return cap ? run(attention_columns_kernel<T, DP, WR, KB, false, true>, bytes, "attention_columns", 5 + which)
-             : run(attention_columns_kernel<T, DP, WR, KB, false, false>, bytes, "attention_columns", 5 + which);
+  if (geo) return cap ? run(attention_columns_kernel<T, DP, WR, KB, FOLDS, true, true>, bytes, "attention_columns", 5 + which)
+                      : run(attention_columns_kernel<T, DP, WR, KB, FOLDS, true, false>, bytes, "attention_columns", 5 + which);
+  return cap ? run(attention_columns_kernel<T, DP, WR, KB, FOLDS, false, true>, bytes, "attention_columns", 5 + which)
+             : run(attention_columns_kernel<T, DP, WR, KB, FOLDS, false, false>, bytes, "attention_columns", 5 + which);
 }
 
 template <typename T, int DP>
@@ -938,6 +1001,9 @@ int launch_rows(Pass pass, const AttentionParams& p, int64_t tiles, int tile_row
   // Wide heads, float32 and the backward pass need the registers; float32's backward pass also the shared memory (48 graphs of 40 to
   // 250 nodes, heads of 72 values: by rows 184 us with 32, 170 with 16, by columns the same).
   constexpr int KF = sizeof(T) == 2 && DP <= 64 ? 64 : 32, KB = sizeof(T) == 2 ? 32 : 16;
+  if constexpr (sizeof(T) == 2) {
+    if (p.folds) return launch<T, DP, 4, KF, KB, true>(pass, p, tiles, geo, s);
+  }
   if (tile_rows == 64) return launch<T, DP, 4, KF, KB>(pass, p, tiles, geo, s);
   if (tile_rows == 32) return launch<T, DP, 2, 32, 32>(pass, p, tiles, geo, s);
   return launch<T, DP, 1, 16, 16>(pass, p, tiles, geo, s);

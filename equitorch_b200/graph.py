@@ -73,7 +73,7 @@ class PackedGraphs:
     ``torch_geometric``'s batches have it.  Computed once per batch, for every layer that works within graphs.
 
     Nodes before ``ptr[0]`` and from ``ptr[-1]`` on belong to no graph.  Attributes: ``ptr`` (num_graphs + 1, int64), ``num_nodes``,
-    ``num_graphs``, ``covers`` (every node has a graph), ``tile_rows`` and ``tiles`` (num_tiles, 4, int32: first row, first node and
+    ``num_graphs``, ``longest`` (nodes of the largest graph), ``covers`` (every node has a graph), ``tile_rows`` and ``tiles`` (num_tiles, 4, int32: first row, first node and
     one past the last node of its graph, 0), the pieces of at most ``tile_rows`` nodes of one graph that the kernels work on, those of
     the largest graphs first.  Reads a few numbers back to the host.  Boundaries may lie on the host too (``to`` moves the result).
     """
@@ -85,20 +85,21 @@ class PackedGraphs:
             raise ValueError(f"num_nodes must be in [0, 2^31 - 64), got {num_nodes}")
         self.ptr, self.num_nodes, self.num_graphs = ptr.contiguous().clone(), int(num_nodes), ptr.numel() - 1
         on_gpu = self.ptr.is_cuda
-        first, last, least, *tiles = (self._stats_gpu() if on_gpu else self._stats()).tolist()
+        first, last, least, self.longest, *tiles = (self._stats_gpu() if on_gpu else self._stats()).tolist()
         if least < 0 or first < 0 or last > self.num_nodes:
             raise ValueError(f"boundaries of the graphs must ascend within [0, {self.num_nodes}]")
         self.covers = first == 0 and last == self.num_nodes
         # Rows behind the end of a graph are work for nothing, and a tile of more rows reads the other side fewer times: the largest
         # tile with at most an eighth (a quarter, for the largest) more rows than the smaller ones.  Forward and backward pass of
         # attention with tiles of 16, 32 and 64 rows: 2000 graphs of 5 to 60 nodes (1.2 and 1.5 times the rows) 347, 384 and 454 us,
-        # 48 graphs of 40 to 250 (1.05 and 1.16 times) 752, 655 and 497.
-        self.tile_rows = 64 if 64 * tiles[2] <= 1.25 * 32 * tiles[1] else 32 if 32 * tiles[1] <= 1.125 * 16 * tiles[0] else 16
+        # 48 graphs of 40 to 250 (1.05 and 1.16 times) 752, 655 and 497.  A graph of more than 4096 nodes, which is most of a batch's work,
+        # takes the largest in any company: the kernels whose sums reach that far have no other.
+        self.tile_rows = 64 if self.longest > 4096 or 64 * tiles[2] <= 1.25 * 32 * tiles[1] else 32 if 32 * tiles[1] <= 1.125 * 16 * tiles[0] else 16
         total = tiles[(16, 32, 64).index(self.tile_rows)]
         self.tiles = self._tiles_gpu(total) if on_gpu else self._tiles(total)
 
     def _stats_gpu(self) -> Tensor:
-        stats = torch.empty(6, dtype=torch.int64, device=self.device)
+        stats = torch.empty(7, dtype=torch.int64, device=self.device)
         with _lib.on_device(self.device):
             _lib.check(_lib.lib().eqt_pack_graphs_stats(self.ptr.data_ptr(), self.num_graphs, stats.data_ptr(), _lib.stream_ptr(self.device)),
                        "eqt_pack_graphs_stats")
@@ -114,8 +115,8 @@ class PackedGraphs:
     def _stats(self) -> Tensor:
         """For boundaries that a data loader holds on the host."""
         sizes = self.ptr[1:] - self.ptr[:-1]
-        least = sizes.min() if self.num_graphs else sizes.new_zeros(())
-        return torch.stack([self.ptr[0], self.ptr[-1], least, *(((sizes.clamp(min=0) + r - 1) // r).sum() for r in (16, 32, 64))])
+        least, greatest = (sizes.min(), sizes.max()) if self.num_graphs else (sizes.new_zeros(()),) * 2
+        return torch.stack([self.ptr[0], self.ptr[-1], least, greatest, *(((sizes.clamp(min=0) + r - 1) // r).sum() for r in (16, 32, 64))])
 
     def _tiles(self, total: int) -> Tensor:
         sizes = self.ptr[1:] - self.ptr[:-1]

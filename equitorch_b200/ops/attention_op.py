@@ -53,7 +53,7 @@ def _args(q, k, v, graphs, heads, scale, cap, pos, slope, out, stats) -> _lib.At
     n, comps, channels = q.shape
     return _lib.AttentionArgs(
         dtype=_lib.DTYPE_CODE[q.dtype], heads=heads, comps=comps, head_channels=channels // heads, tile_rows=graphs.tile_rows,
-        scale=scale, cap=cap or 0.0, n=n, num_tiles=graphs.tiles.shape[0], tiles=graphs.tiles.data_ptr(),
+        scale=scale, cap=cap or 0.0, n=n, longest=graphs.longest, num_tiles=graphs.tiles.shape[0], tiles=graphs.tiles.data_ptr(),
         q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), q_node=q.stride(0), q_comp=q.stride(1), k_node=k.stride(0),
         k_comp=k.stride(1), v_node=v.stride(0), v_comp=v.stride(1), pos=_lib.ptr(pos), slope=_lib.ptr(slope),
         out=out.data_ptr(), stats=_lib.ptr(stats))

@@ -663,7 +663,8 @@ int eqt_embedding_grad(int32_t dtype, const void* g, const int64_t* index, void*
  *   out_i = sum_j softmax_j(s) v_j;   stats (2, heads, n), written by the forward pass (NULL: not wanted): the greatest s of the row
  * times log2(e), and one over the sum of exp(s) relative to it
  * tiles (num_tiles, 4): first row, first node and one past the last node of the row's graph, 0; a tile is tile_rows (16, 32, 64)
- * rows of one graph, cut at the graph's end.  The tiles are to cover each row at most once and to lie in [0, n); rows of no tile are
+ * rows of one graph, cut at the graph's end; bfloat16 with a graph of more than 4096 nodes takes tiles of 64 rows.  longest: nodes of the
+ * largest graph (0: not known, n of them).  The tiles are to cover each row at most once and to lie in [0, n); rows of no tile are
  * neither read nor written.  Backward: delta (heads, n) is scratch; dpos (n, 3) and dslope (heads) are both given or both NULL, and
  * with them geo (2, heads, n, 4) floats of scratch, zero in the rows of no tile, 16-byte aligned.  float32 or bfloat16 features,
  * all else float32; sums in float32, no atomics.
@@ -671,7 +672,7 @@ int eqt_embedding_grad(int32_t dtype, const void* g, const int64_t* index, void*
 typedef struct eqt_attention_args {
   int32_t dtype, heads, comps, head_channels, tile_rows;
   float scale, cap;
-  int64_t n, num_tiles;
+  int64_t n, longest, num_tiles;
   const int32_t* tiles;
   const void *q, *k, *v;
   int64_t q_node, q_comp, k_node, k_comp, v_node, v_comp;
@@ -687,8 +688,8 @@ typedef struct eqt_attention_args {
 int eqt_attention_forward(const eqt_attention_args* args, void* stream);
 int eqt_attention_backward(const eqt_attention_args* args, void* stream);
 /*
- * The tiles of a packed batch: graph g has the nodes [ptr[g], ptr[g + 1]).  stats (6): ptr[0], ptr[graphs], the least size, and how many
- * tiles of 16, 32 and 64 rows the graphs have; the caller checks them (a tile outside the nodes must not reach the attention) and gives
+ * The tiles of a packed batch: graph g has the nodes [ptr[g], ptr[g + 1]).  stats (7): ptr[0], ptr[graphs], the least and the greatest
+ * size, and how many tiles of 16, 32 and 64 rows the graphs have; the caller checks them (a tile outside the nodes must not reach the attention) and gives
  * room for as many tiles as its choice of rows has.  Larger graphs' tiles come first, by classes of size.
  */
 int eqt_pack_graphs_stats(const int64_t* ptr, int64_t graphs, int64_t* stats, void* stream);
