@@ -204,9 +204,9 @@ __device__ __forceinline__ void out_mma(float (&o)[DP / 8][4], const float (&p)[
 
 // The bfloat16 products add up in the matrix instructions, whose adder truncates: a sum of one sign loses 1.2e-7 of itself at every step of
 // 16 terms (outputs of 400,000 nodes: 3e-3, as much as their rounding).  So every FOLD terms a sum joins, with ordinary rounding, another
-// one that waits in local memory; 4096 terms lose 3e-5.  Only the kernels for graphs that are longer do so (FOLDS), which take tiles of 64 rows:
+// one that waits in local memory; 8192 terms lose 6e-5.  Only the kernels for graphs that are longer do so (FOLDS), which take tiles of 64 rows:
 // the code costs the others 3 % in registers.  float32 sums join after every tile anyway.
-constexpr int FOLD = 4096;
+constexpr int FOLD = 8192;
 template <int DP, int MORE = 0> struct Far {             // a thread's sums, and MORE numbers beside them
   float values[DP / 2 + MORE];
   __device__ __forceinline__ float* at() {

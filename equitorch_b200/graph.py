@@ -73,8 +73,8 @@ class PackedGraphs:
     ``torch_geometric``'s batches have it.  Computed once per batch, for every layer that works within graphs.
 
     Nodes before ``ptr[0]`` and from ``ptr[-1]`` on belong to no graph.  Attributes: ``ptr`` (num_graphs + 1, int64), ``num_nodes``,
-    ``num_graphs``, ``longest`` (nodes of the largest graph), ``covers`` (every node has a graph), ``tile_rows`` and ``tiles`` (num_tiles, 4, int32: first row, first node and
-    one past the last node of its graph, 0), the pieces of at most ``tile_rows`` nodes of one graph that the kernels work on, those of
+    ``num_graphs``, ``longest`` (nodes of the largest graph), ``covers`` (every node has a graph), ``tile_rows`` and ``tiles``
+    (num_tiles, 4, int32: first row, first node and one past the last node of its graph, 0), the pieces of at most ``tile_rows`` nodes of one graph that the kernels work on, those of
     the largest graphs first.  Reads a few numbers back to the host.  Boundaries may lie on the host too (``to`` moves the result).
     """
 
@@ -92,9 +92,9 @@ class PackedGraphs:
         # Rows behind the end of a graph are work for nothing, and a tile of more rows reads the other side fewer times: the largest
         # tile with at most an eighth (a quarter, for the largest) more rows than the smaller ones.  Forward and backward pass of
         # attention with tiles of 16, 32 and 64 rows: 2000 graphs of 5 to 60 nodes (1.2 and 1.5 times the rows) 347, 384 and 454 us,
-        # 48 graphs of 40 to 250 (1.05 and 1.16 times) 752, 655 and 497.  A graph of more than 4096 nodes, which is most of a batch's work,
+        # 48 graphs of 40 to 250 (1.05 and 1.16 times) 752, 655 and 497.  A graph of more than 8192 nodes, which is most of a batch's work,
         # takes the largest in any company: the kernels whose sums reach that far have no other.
-        self.tile_rows = 64 if self.longest > 4096 or 64 * tiles[2] <= 1.25 * 32 * tiles[1] else 32 if 32 * tiles[1] <= 1.125 * 16 * tiles[0] else 16
+        self.tile_rows = 64 if self.longest > 8192 or 64 * tiles[2] <= 1.25 * 32 * tiles[1] else 32 if 32 * tiles[1] <= 1.125 * 16 * tiles[0] else 16
         total = tiles[(16, 32, 64).index(self.tile_rows)]
         self.tiles = self._tiles_gpu(total) if on_gpu else self._tiles(total)
 

@@ -663,7 +663,7 @@ int eqt_embedding_grad(int32_t dtype, const void* g, const int64_t* index, void*
  *   out_i = sum_j softmax_j(s) v_j;   stats (2, heads, n), written by the forward pass (NULL: not wanted): the greatest s of the row
  * times log2(e), and one over the sum of exp(s) relative to it
  * tiles (num_tiles, 4): first row, first node and one past the last node of the row's graph, 0; a tile is tile_rows (16, 32, 64)
- * rows of one graph, cut at the graph's end; bfloat16 with a graph of more than 4096 nodes takes tiles of 64 rows.  longest: nodes of the
+ * rows of one graph, cut at the graph's end; bfloat16 with a graph of more than 8192 nodes takes tiles of 64 rows.  longest: nodes of the
  * largest graph (0: not known, n of them).  The tiles are to cover each row at most once and to lie in [0, n); rows of no tile are
  * neither read nor written.  Backward: delta (heads, n) is scratch; dpos (n, 3) and dslope (heads) are both given or both NULL, and
  * with them geo (2, heads, n, 4) floats of scratch, zero in the rows of no tile, 16-byte aligned.  float32 or bfloat16 features,

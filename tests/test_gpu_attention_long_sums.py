@@ -52,7 +52,7 @@ def test_sums_of_one_sign(bias):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("size,sizes", [(16, [5, 4096, 4097, 0, 4160, 33]), (64, [8193, 7]), (128, [4100])])
+@pytest.mark.parametrize("size,sizes", [(16, [5, 8192, 8193, 0, 8260, 33]), (64, [16385, 7]), (128, [8200])])
 @pytest.mark.parametrize("bias,cap", [(True, 10.0), (False, None)])
 def test_around_the_border_against_float64(dtype, size, sizes, bias, cap):
     """Sums that join another sum never, once and twice, beside small graphs."""
@@ -63,7 +63,7 @@ def test_around_the_border_against_float64(dtype, size, sizes, bias, cap):
 
 def test_scores_that_grow_along_the_keys():
     """The greatest score moves on after every join, so the waiting sums change their unit each time."""
-    n = 13_000
+    n = 17_000
     g = torch.Generator().manual_seed(4)
     q, k, v, cot = (torch.randn(n, 1, 32, generator=g) for _ in range(4))
     q[:, 0, 0] = torch.linspace(-1, 1, n)[torch.randperm(n, generator=g)]
