@@ -34,10 +34,13 @@ using namespace tc;
 
 enum Mode { FORWARD, PARTIALS, INPUT_GRAD, WEIGHT_GRAD };
 
-constexpr int PIECE = 4;                                 // k-blocks of a float32 piece
+// k-blocks of a piece: float32 sums are always taken in pieces; bfloat16 ones (SHAPE LONG) where more than LONGEST terms would be one sum,
+// which loses up to 1.8e-7 of itself every 16 terms: 3.6e-4 for 32768, a tenth of its rounding, 1.2e-2 for the 2^20 channels allowed.
+constexpr int PIECE = 4, LONG_PIECE = 128;
+constexpr int64_t LONGEST = 32768;
 
 // HELD: the k-blocks of B stay in shared memory for all tiles of a column, only A comes by (100k x 256 -> 1024 forward: 123 -> 106 us).
-enum Shape { ALONE, PAIR, HELD };
+enum Shape { ALONE, PAIR, HELD, LONG };
 template <typename T> struct Form;
 template <> struct Form<__nv_bfloat16> {
   static constexpr int BK = 64, COLS = 256, FIRST = 2, SPLITTERS = 0, EPI = 16, A_BYTES = 16384, HELD_BLOCKS = 4;
@@ -305,13 +308,14 @@ template <bool TWO> __device__ __forceinline__ void commit(uint64_t* bar) {
 template <typename T, int MODE, int ACT, int SHAPE>
 __global__ void __launch_bounds__(threads<T>(), 1) gated_tc_kernel(const __grid_constant__ Launch p) {
   using S = Form<T>;
-  constexpr bool F32 = sizeof(T) == 4, TWO = SHAPE == PAIR, DUAL = MODE == FORWARD || MODE == PARTIALS;
+  constexpr bool F32 = sizeof(T) == 4, TWO = SHAPE == PAIR, PIECES = F32 || SHAPE == LONG, DUAL = MODE == FORWARD || MODE == PARTIALS;
   constexpr bool A_TURNED = MODE == WEIGHT_GRAD, B_TURNED = MODE != INPUT_GRAD;      // the operand lies along the rows
   constexpr int LINE = 128 / (int)sizeof(T);                                          // values of a line
   constexpr int STAGES = stages<T, MODE, SHAPE>(), STAGE = stage_bytes<T, SHAPE>();
   static_assert(STAGES >= 2 && (SHAPE != HELD || DUAL), "two stages at least; B stays for the dual products");
+  static_assert(SHAPE != LONG || (!F32 && MODE != WEIGHT_GRAD), "rows are summed in parts, float32 in pieces anyway");
   constexpr int ACC_COLS = F32 ? 2 * S::COLS : S::COLS;                               // of tensor memory: float32 has two sums
-  constexpr int CTAS = TWO ? 2 : 1;
+  constexpr int CTAS = TWO ? 2 : 1, BLOCKS = F32 ? PIECE : LONG_PIECE;
   extern __shared__ unsigned char smem_raw[];
   __shared__ uint64_t full[STAGES], ready[STAGES], empty[STAGES], acc_full[2], acc_empty[2], held_full, held_ready;
   __shared__ uint32_t tmem_slot;
@@ -417,7 +421,7 @@ __global__ void __launch_bounds__(threads<T>(), 1) gated_tc_kernel(const __grid_
         for (unsigned i = first_item; i < p.items && ok && !*ab; i += item_step) {
           const Item t = item_of<MODE, SHAPE>(p, i);
           for (int k0 = t.kb0; k0 < t.kb1 && ok; ++piece) {
-            const int k1 = F32 ? min(k0 + PIECE, t.kb1) : t.kb1, a = piece & 1;
+            const int k1 = PIECES ? min(k0 + BLOCKS, t.kb1) : t.kb1, a = piece & 1;
             const uint32_t parity = (uint32_t)(((piece >> 1) & 1) ^ 1);
             if (!(TWO ? bar_wait_cluster(&acc_empty[a], parity, ab) : bar_wait(&acc_empty[a], parity, ab))) { ok = false; break; }
             tc_fence_after();
@@ -518,16 +522,16 @@ __global__ void __launch_bounds__(threads<T>(), 1) gated_tc_kernel(const __grid_
       const Item t = item_of<MODE, SHAPE>(p, i);
       const int64_t row = t.row + rank * TILE_M + quarter * 32;
       const int lines = (int)max((int64_t)0, min((int64_t)32, p.rows - row));
-      // float32 sums come in pieces and gather in registers: the share's two turns, or its turn of each half
-      float sum[F32 ? 2 : 1][32];
+      // sums that come in pieces gather in registers: the share's two turns, or its turn of each half
+      float sum[PIECES ? 2 : 1][32];
       uint32_t d = 0;
-      const int pieces = F32 ? (t.kb1 - t.kb0 + PIECE - 1) / PIECE : 1;
+      const int pieces = PIECES ? (t.kb1 - t.kb0 + BLOCKS - 1) / BLOCKS : 1;
       for (int q = 0; q < pieces; ++q, ++piece) {
         const int a = piece & 1;
         if (!bar_wait(&acc_full[a], (uint32_t)((piece >> 1) & 1), ab)) { ok = false; break; }
         tc_fence_after();
         d = lanes + (uint32_t)(a * ACC_COLS);
-        if (F32) {
+        if constexpr (PIECES) {
 #pragma unroll
           for (int b = 0; b < 2; ++b) {
             const int at = DUAL ? b * p.width + share * 32 : (share + b * SHARES) * 32;
@@ -535,12 +539,14 @@ __global__ void __launch_bounds__(threads<T>(), 1) gated_tc_kernel(const __grid_
 #pragma unroll
             for (int h = 0; h < 32; h += 16) {
               float v[16];
-              tmem_ld16(d + S::COLS + at + h, v);
+              tmem_ld16(d + (F32 ? S::COLS : 0) + at + h, v);
 #pragma unroll
-              for (int c = 0; c < 16; ++c) sum[F32 ? b : 0][h + c] = q ? sum[F32 ? b : 0][h + c] + v[c] : v[c];
-              tmem_ld16(d + at + h, v);
+              for (int c = 0; c < 16; ++c) sum[b][h + c] = q ? sum[b][h + c] + v[c] : v[c];
+              if constexpr (F32) {
+                tmem_ld16(d + at + h, v);
 #pragma unroll
-              for (int c = 0; c < 16; ++c) sum[F32 ? b : 0][h + c] += v[c];
+                for (int c = 0; c < 16; ++c) sum[b][h + c] += v[c];
+              }
             }
           }
           tc_fence_before();
@@ -561,9 +567,9 @@ __global__ void __launch_bounds__(threads<T>(), 1) gated_tc_kernel(const __grid_
         const int64_t at = row * p.out_pitch + col;
         if (!DUAL) {
           float v[32];
-          if constexpr (F32) {
+          if constexpr (PIECES) {
 #pragma unroll
-            for (int c = 0; c < 32; ++c) v[c] = sum[F32 ? turn : 0][c];
+            for (int c = 0; c < 32; ++c) v[c] = sum[turn][c];
           } else {
             tmem_ld32(d + c0, v);
           }
@@ -595,7 +601,7 @@ __global__ void __launch_bounds__(threads<T>(), 1) gated_tc_kernel(const __grid_
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
           uint32_t a[16], u[16];
-          if constexpr (!F32) {
+          if constexpr (!PIECES) {
             tmem_issue16(d + c0 + b * 16, a);
             tmem_issue16(d + p.width + c0 + b * 16, u);
             tmem_arrived(a, u);
@@ -612,7 +618,7 @@ __global__ void __launch_bounds__(threads<T>(), 1) gated_tc_kernel(const __grid_
               Value<float> v[2];
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
-                if constexpr (F32) {
+                if constexpr (PIECES) {
                   ai[h] = sum[0][b * 16 + j + h];
                   ui[h] = sum[1][b * 16 + j + h];
                 } else {
@@ -653,7 +659,7 @@ __global__ void __launch_bounds__(threads<T>(), 1) gated_tc_kernel(const __grid_
           other = t0;
         }
       }
-      if (!F32) {
+      if (!PIECES) {
         tc_fence_before();
         __syncwarp();
         if (lane == 0) {
@@ -794,6 +800,9 @@ template <typename T, int MODE, int ACT = EQT_ACT_SILU> int launch(const GatedAr
     const int64_t columns = ceil_div(a.f, Form<T>::COLS / 2), sms = tc::sm_count();
     if (a.c <= Form<T>::BK * Form<T>::HELD_BLOCKS && sms / columns * columns * 10 >= sms * 9 && ceil_div(a.n, TILE_M) * columns >= 2 * sms)
       return launch_form<T, MODE, HELD, ACT>(a, s);
+  }
+  if constexpr (sizeof(T) == 2 && MODE != WEIGHT_GRAD) {
+    if ((DUAL ? (int64_t)a.c : 2 * (int64_t)a.f) > LONGEST) return launch_form<T, MODE, LONG, ACT>(a, s);
   }
   if constexpr (sizeof(T) == 2) {
     const int64_t rows = MODE == WEIGHT_GRAD ? a.c : a.n, cols = MODE == INPUT_GRAD ? a.c : a.f;
