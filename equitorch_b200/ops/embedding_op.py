@@ -40,9 +40,9 @@ def embedding_grad(index: Tensor, grad: Tensor, types: int, scale: float) -> Ten
     index, grad = index.contiguous(), grad.contiguous()
     n, width, code = index.numel(), math.prod(row), _lib.DTYPE_CODE[grad.dtype]
     gw = torch.empty(types, *row, dtype=grad.dtype, device=dev)
-    size = _lib.lib().eqt_embedding_grad_scratch(code, n, types, width)
-    scratch = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
-    with _lib.on_device(dev):
+    with _lib.on_device(dev):                                # the size goes by the SMs of the current device
+        size = _lib.lib().eqt_embedding_grad_scratch(code, n, types, width)
+        scratch = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
         _lib.check(_lib.lib().eqt_embedding_grad(code, grad.data_ptr(), index.data_ptr(), gw.data_ptr(), n, types, width, scale,
                                                  _lib.ptr(scratch), size, _lib.stream_ptr(dev)), "eqt_embedding_grad")
     return gw

@@ -647,7 +647,7 @@ int eqt_radius_list_edges(const float* pos, int64_t n, const int64_t* ptr, const
  * Rows of a table by type: out (n, width) = scale * weight (types, width)[index (n)]; a row of zeros where index is not in
  * [0, types).  Gradient: gw (types, width) = scale * sum of g over the rows of each type, all of gw written.  Sums in float
  * (double for EQT_F64), no atomics on values: the same bits at every call.  n and types below 2^31 - 1, width <= 2^20.
- * `scratch`: eqt_embedding_grad_scratch bytes, 256-byte aligned (0: none needed).
+ * `scratch`: eqt_embedding_grad_scratch bytes, 256-byte aligned (0: none needed), as many as it says with the same device current.
  */
 int eqt_embedding_forward(int32_t dtype, const void* weight, const int64_t* index, void* out, int64_t n, int64_t types,
                           int64_t width, double scale, void* stream);
@@ -700,7 +700,7 @@ int eqt_pack_graphs_tiles(const int64_t* ptr, int64_t graphs, int32_t* tiles, in
  * and dw (2, c, f), either may be NULL; both products are formed again, nothing of the forward pass is kept.  All in one dtype, sums
  * in float (double for EQT_F64); da and du are rounded to the dtype between the kernels.  float32 (as three TF32 products) and bfloat16
  * run on the tensor cores and their pointers lie on 16-byte boundaries; rows whose length is no multiple of 16 bytes are copied to wider
- * ones first.  `scratch`: eqt_gated_scratch bytes, 16-byte aligned (0: none needed).  `status` (int32 on the device) is raised where a
+ * ones first.  `scratch`: eqt_gated_scratch bytes, 16-byte aligned (0: none needed), as many as it says with the same device current.  `status` (int32 on the device) is raised where a
  * bounded wait gave up.
  */
 enum eqt_activation { EQT_ACT_SILU = 0, EQT_ACT_GELU = 1, EQT_ACT_RELU = 2, EQT_ACT_SIGMOID = 3 };
