@@ -201,6 +201,7 @@ SIGNATURES = {
     "eqt_pack_graphs_stats": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p]),
     "eqt_pack_graphs_tiles": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_int32, C.c_void_p]),
     "eqt_gated_scratch": (C.c_int64, [C.c_int32] + [C.c_int64] * 3 + [C.c_int32]),
+    "eqt_gated_form": (C.c_int32, [C.c_int32] + [C.c_int64] * 3 + [C.c_int32]),
     "eqt_gated_forward": (C.c_int, [C.c_int32] + [C.c_void_p] * 4 + [C.c_int64] * 4 + [C.c_int32, C.c_void_p, C.c_void_p]),
     "eqt_gated_backward": (C.c_int, [C.c_int32] + [C.c_void_p] * 6 + [C.c_int64] * 4 + [C.c_int32, C.c_void_p, C.c_void_p]),
     "eqt_last_error": (C.c_char_p, []),

@@ -250,6 +250,14 @@ extern "C" int64_t eqt_gated_scratch(int32_t dtype, int64_t n, int64_t c, int64_
   return (int64_t)lay_out(p, dtype, n, c, f, backward != 0).bytes;
 }
 
+extern "C" int32_t eqt_gated_form(int32_t dtype, int64_t n, int64_t c, int64_t f, int32_t product) {
+  if (check_sizes(dtype, n, c, f, 0) || dtype == EQT_F64 || n == 0 || f == 0 || c == 0 || product < FORWARD || product > WEIGHT_GRAD) return -1;
+  GatedArgs p{};
+  lay_out(p, dtype, n, c, f, true);
+  p.n = n, p.c = (int)c, p.f = (int)f;
+  return dtype == EQT_F32 ? tensor_form_f32(p, product) : tensor_form_bf16(p, product);
+}
+
 extern "C" int eqt_gated_forward(int32_t dtype, const void* x, const void* w, void* h, void* scratch, int64_t scratch_bytes, int64_t n, int64_t c,
                                  int64_t f, int32_t act, int32_t* status, void* stream) {
   if (int rc = check_sizes(dtype, n, c, f, act)) return rc;

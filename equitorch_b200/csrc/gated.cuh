@@ -55,6 +55,8 @@ int tensor_forward_f32(const GatedArgs& p, cudaStream_t s);         // gated_f32
 int tensor_forward_bf16(const GatedArgs& p, cudaStream_t s);
 int tensor_backward_f32(const GatedArgs& p, cudaStream_t s);
 int tensor_backward_bf16(const GatedArgs& p, cudaStream_t s);
+int tensor_form_f32(const GatedArgs& p, int product);                // eqt_gated_form
+int tensor_form_bf16(const GatedArgs& p, int product);
 
 }  // namespace gated
 }  // namespace eqt

@@ -36,6 +36,8 @@ enum Mode { FORWARD, PARTIALS, INPUT_GRAD, WEIGHT_GRAD };
 
 // k-blocks of a piece: float32 sums are always taken in pieces; bfloat16 ones (SHAPE LONG) where more than LONGEST terms would be one sum,
 // which loses up to 1.8e-7 of itself every 16 terms: 3.6e-4 for 32768, a tenth of its rounding, 1.2e-2 for the 2^20 channels allowed.
+// The pieces cost the registers of a tile and pairs of CTAs: 2048 x 32776 -> 2048 forward 571 us, 32768 channels in pairs 407; gradient of x at
+// 8192 x 1024, hidden 16392 657 us, 16384 in pairs 437.
 constexpr int PIECE = 4, LONG_PIECE = 128;
 constexpr int64_t LONGEST = 32768;
 
@@ -794,20 +796,34 @@ template <typename T, int MODE, int SHAPE, int ACT> int launch_form(const GatedA
 // 256 -> 1024; the partial results 149 -> 167 us, since their patches leave A two stages).  Pairs of CTAs from the size on that gives most
 // SMs a tile of 256 rows, below it tiles of 128 rows fill more of them; not for the dual products of short sums, whose tiles change hands
 // too often (the same call in pairs: forward 132, partial results 171 us).
-template <typename T, int MODE, int ACT = EQT_ACT_SILU> int launch(const GatedArgs& a, cudaStream_t s) {
+template <typename T, int MODE> Shape shape_of(const GatedArgs& a) {
   constexpr bool DUAL = MODE == FORWARD || MODE == PARTIALS;
-  if constexpr (MODE == FORWARD) {
-    const int64_t columns = ceil_div(a.f, Form<T>::COLS / 2), sms = tc::sm_count();
-    if (a.c <= Form<T>::BK * Form<T>::HELD_BLOCKS && sms / columns * columns * 10 >= sms * 9 && ceil_div(a.n, TILE_M) * columns >= 2 * sms)
-      return launch_form<T, MODE, HELD, ACT>(a, s);
+  const int64_t sms = tc::sm_count();
+  if (MODE == FORWARD) {
+    const int64_t columns = ceil_div(a.f, Form<T>::COLS / 2);
+    if (a.c <= Form<T>::BK * Form<T>::HELD_BLOCKS && sms / columns * columns * 10 >= sms * 9 && ceil_div(a.n, TILE_M) * columns >= 2 * sms) return HELD;
   }
-  if constexpr (sizeof(T) == 2 && MODE != WEIGHT_GRAD) {
-    if ((DUAL ? (int64_t)a.c : 2 * (int64_t)a.f) > LONGEST) return launch_form<T, MODE, LONG, ACT>(a, s);
+  if (sizeof(T) == 4) return ALONE;
+  if (MODE != WEIGHT_GRAD && (DUAL ? (int64_t)a.c : 2 * (int64_t)a.f) > LONGEST) return LONG;
+  const int64_t rows = MODE == WEIGHT_GRAD ? a.c : a.n, cols = MODE == INPUT_GRAD ? a.c : a.f;
+  const int64_t tiles = ceil_div(rows, 256) * ceil_div(cols, DUAL ? 128 : 256) * (MODE == WEIGHT_GRAD ? 2 * a.splits : 1);
+  return rows > TILE_M && tiles * 5 >= sms * 2 && (!DUAL || a.c >= 512) ? PAIR : ALONE;
+}
+template <typename T> Shape shape_of(const GatedArgs& a, int product) {
+  return product == FORWARD ? shape_of<T, FORWARD>(a) : product == PARTIALS ? shape_of<T, PARTIALS>(a)
+         : product == INPUT_GRAD ? shape_of<T, INPUT_GRAD>(a) : shape_of<T, WEIGHT_GRAD>(a);
+}
+
+template <typename T, int MODE, int ACT = EQT_ACT_SILU> int launch(const GatedArgs& a, cudaStream_t s) {
+  const Shape shape = shape_of<T, MODE>(a);
+  if constexpr (MODE == FORWARD) {
+    if (shape == HELD) return launch_form<T, MODE, HELD, ACT>(a, s);
   }
   if constexpr (sizeof(T) == 2) {
-    const int64_t rows = MODE == WEIGHT_GRAD ? a.c : a.n, cols = MODE == INPUT_GRAD ? a.c : a.f;
-    const int64_t tiles = ceil_div(rows, 256) * ceil_div(cols, DUAL ? 128 : 256) * (MODE == WEIGHT_GRAD ? 2 * a.splits : 1);
-    if (rows > TILE_M && tiles * 5 >= tc::sm_count() * 2 && (!DUAL || a.c >= 512)) return launch_form<T, MODE, PAIR, ACT>(a, s);
+    if (shape == PAIR) return launch_form<T, MODE, PAIR, ACT>(a, s);
+    if constexpr (MODE != WEIGHT_GRAD) {
+      if (shape == LONG) return launch_form<T, MODE, LONG, ACT>(a, s);
+    }
   }
   return launch_form<T, MODE, ALONE, ACT>(a, s);
 }

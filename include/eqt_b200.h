@@ -705,6 +705,9 @@ int eqt_pack_graphs_tiles(const int64_t* ptr, int64_t graphs, int32_t* tiles, in
  */
 enum eqt_activation { EQT_ACT_SILU = 0, EQT_ACT_GELU = 1, EQT_ACT_RELU = 2, EQT_ACT_SIGMOID = 3 };
 int64_t eqt_gated_scratch(int32_t dtype, int64_t n, int64_t c, int64_t f, int32_t backward);
+/* Which form of the tensor-core kernel a call of these sizes runs on the current device: 0 tiles of 128 rows, 1 pairs of CTAs, 2 weights held
+ * in shared memory, 3 sums in pieces; -1 where none does.  product: 0 forward, 1 da and du, 2 dx, 3 dw. */
+int32_t eqt_gated_form(int32_t dtype, int64_t n, int64_t c, int64_t f, int32_t product);
 int eqt_gated_forward(int32_t dtype, const void* x, const void* w, void* h, void* scratch, int64_t scratch_bytes, int64_t n, int64_t c,
                       int64_t f, int32_t act, int32_t* status, void* stream);
 int eqt_gated_backward(int32_t dtype, const void* x, const void* w, const void* g, void* dx, void* dw, void* scratch,
