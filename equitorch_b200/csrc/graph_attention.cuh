@@ -142,29 +142,40 @@ __device__ __forceinline__ void score_mma(float (&acc)[NT][4], const float* a, c
     for (int i = 0; i < 4; ++i) acc[n][i] += fine[n][i];
 }
 
-// o[16 rows][DP] += p[16][8 NT] X[8 NT][DP], p in the layout that score_mma leaves
-template <int DP, int NT>
+// o[16 rows][DP] += p[16][8 NT] X[8 NT][DP], p in the layout that score_mma leaves.  Weights and score gradients are rounded to bfloat16
+// here, as the operands are; their sums stay in float32.  FINE: what the rounding left goes in too.
+template <int DP, int NT, bool FINE = false>
 __device__ __forceinline__ void out_mma(float (&o)[DP / 8][4], const float (&p)[NT][4], const __nv_bfloat16* x, int lane) {
   constexpr int LD = Row<__nv_bfloat16, DP>::LD;
   const __nv_bfloat16* xp = x + (lane & 15) * LD + (lane >> 4) * 8;
 #pragma unroll
   for (int j = 0; j < NT / 2; ++j) {
-    // weights and score gradients are rounded to bfloat16 here, as the operands are; their sums stay in float32
     const uint32_t a[4] = {pack_bf16(p[2 * j][0], p[2 * j][1]), pack_bf16(p[2 * j][2], p[2 * j][3]),
                            pack_bf16(p[2 * j + 1][0], p[2 * j + 1][1]), pack_bf16(p[2 * j + 1][2], p[2 * j + 1][3])};
+    uint32_t rest[4];
+    if (FINE) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        rest[i] = pack_bf16(p[2 * j + (i >> 1)][2 * (i & 1)] - __uint_as_float(a[i] << 16),
+                            p[2 * j + (i >> 1)][2 * (i & 1) + 1] - __uint_as_float(a[i] & 0xffff0000u));
+    }
 #pragma unroll
     for (int d = 0; d < DP / 16; ++d) {
       uint32_t rb[4];
       ldmatrix4_trans(rb, xp + j * 16 * LD + d * 16);
       mma_bf16(o[2 * d], a, rb[0], rb[1]);
       mma_bf16(o[2 * d + 1], a, rb[2], rb[3]);
+      if (FINE) {
+        mma_bf16(o[2 * d], rest, rb[0], rb[1]);
+        mma_bf16(o[2 * d + 1], rest, rb[2], rb[3]);
+      }
     }
   }
 }
 // The k-th place of a TF32 fragment may be any row of X as long as both operands agree: place t is row 2 t and place t + 4 row 2 t + 1,
 // which is where score_mma left the weights.  The tensor cores' adder truncates, so a tile's sum starts at zero and joins the running
 // one with ordinary rounding.
-template <int DP, int NT>
+template <int DP, int NT, bool FINE = false>
 __device__ __forceinline__ void out_mma(float (&o)[DP / 8][4], const float (&p)[NT][4], const float* x, int lane) {
   constexpr int LD = Row<float, DP>::LD;
   const float* xp = x + (lane & 3) * 2 * LD + (lane >> 2);
@@ -642,8 +653,10 @@ __global__ void __launch_bounds__(THREADS, DP <= 32 ? (WR == 4 ? 5 : sizeof(T) =
 
 // Backward by rows: dq, delta, and with positions the rows' sums of dS r and dS u.  Weights are taken from the row's greatest score, and
 // one over their sum follows at the end.
-// These sums are float32 results also where the features are bfloat16, so there they do not go by the delta of the rounded weights and
-// result: with w = r or u, sum_j dS w = sum_j P dP w - (sum_j P dP) (sum_j P w), and the columns' pass is given sum_j P dP.
+// bfloat16: dq goes by the delta of rounded weights and outputs, which are at hand; the columns' pass is given sum_j P dP, which is known at the
+// end, and so do the sums for slopes and positions, float32 results, go: with w = r or u, sum_j dS w = sum_j P dP w - (sum_j P dP) (sum_j P w).
+// As dq has that error already, its score gradients go into the product in two parts (one graph of 5001 nodes, 2-norm of the error: 2.75e-3
+// with one part, 2.08e-3 with two, which cost 610 -> 666 us; a rounding of the result alone is 1.7e-3).
 template <typename T, int DP, int WR, int KT, bool FOLDS, bool GEO, bool CAP>
 __global__ void __launch_bounds__(THREADS, DP <= 32 ? 4 : DP <= 96 ? 3 : 2) attention_rows_kernel(const __grid_constant__ AttentionParams p) {
   using S = Shape<T, DP, WR, KT>;
@@ -751,10 +764,10 @@ __global__ void __launch_bounds__(THREADS, DP <= 32 ? 4 : DP <= 96 ? 3 : 2) atte
               if (key + n * 8 + 2 * t + 1 >= hi) y = -INFINITY;
             }
             const pair w = both(exp2_fast(x), exp2_fast(y)), e = mul2(w, add2(d, both(-delta[r], -delta[r])));
+            if (APART) all[r] = fma2(w, d, all[r]);
             if (GEO) {
               const pair f = APART ? mul2(w, d) : e, fi = mul2(f, v.inverse), wi = mul2(w, v.inverse);
               if (APART) {
-                all[r] = add2(all[r], f);
                 flat[r][0] = fma2(w, v.length, flat[r][0]);
                 flat[r][1] = fma2(wi, v.x, flat[r][1]);
                 flat[r][2] = fma2(wi, v.y, flat[r][2]);
@@ -770,7 +783,7 @@ __global__ void __launch_bounds__(THREADS, DP <= 32 ? 4 : DP <= 96 ? 3 : 2) atte
             parts(dz, z[n][2 * r], z[n][2 * r + 1]);
           }
         }
-        out_mma<DP, NT>(dq, z, ks, lane);
+        out_mma<DP, NT, true>(dq, z, ks, lane);
       }
       __syncthreads();
     }
@@ -778,14 +791,18 @@ __global__ void __launch_bounds__(THREADS, DP <= 32 ? 4 : DP <= 96 ? 3 : 2) atte
   } while (FOLDS && key < hi);
   if (!work) return;
   if (FOLDS && hi - lo > FOLD) unfold<DP>(waiting.at(), dq);
+  if (APART) {
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      float x, y;
+      parts(all[r], x, y);
+      delta[r] = quad_sum(x + y) * inverse[r];
+    }
+  }
   if (GEO) {
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       float x, y, sums[4];
-      if (APART) {
-        parts(all[r], x, y);
-        delta[r] = quad_sum(x + y) * inverse[r];
-      }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         parts(geo[r][i], x, y);
