@@ -4,7 +4,8 @@
 //   gradient:  gw[t, :]  = scale * sum over n with index[n] = t of g[n, :]
 //
 // Both are bound by memory: one read of g (or one write of out) and of the indices.  The gradient uses no atomics on values, so two
-// calls give the same bits.  Few rows: a CTA per type looks through all indices.  Otherwise the rows are sorted by type (a counting
+// calls give the same bits.  Rows of whole 16 bytes on 16-byte boundaries go by pieces of 16 bytes, others by single values (2.0M bfloat16 rows,
+// 14161 types, both directions: 32 values 240 us, 31 values 386, 33 values 507).  Few rows: a CTA per type looks through all indices.  Otherwise the rows are sorted by type (a counting
 // sort of one digit of up to eight bits a pass, least digit first, in the order of the rows within a type), teams of lanes add up
 // equal pieces of the sorted rows whatever types they hold, and sums that cross the border of a piece are joined afterwards in the
 // order of the pieces.

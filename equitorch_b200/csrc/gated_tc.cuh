@@ -795,7 +795,14 @@ template <typename T, int MODE, int SHAPE, int ACT> int launch_form(const GatedA
 // HELD for the forward pass where B's k-blocks fit and the columns' tiles divide the SMs with little left over (123 -> 106 us at 100k x
 // 256 -> 1024; the partial results 149 -> 167 us, since their patches leave A two stages).  Pairs of CTAs from the size on that gives most
 // SMs a tile of 256 rows, below it tiles of 128 rows fill more of them; not for the dual products of short sums, whose tiles change hands
-// too often (the same call in pairs: forward 132, partial results 171 us).
+// too often (the same call in pairs: forward 132, partial results 171 us).  Both sides at the borders, tiles of 128 rows | pairs | held, us:
+//   forward, 100k rows x 384 -> 1024 161 | 147, x 448 -> 2048 367 | 319; 50k x 512 -> 1024 116 | 104; 2048 x 512 -> 1024 10.2 | 11.2
+//   forward, 20k x 256 -> 512 18.9 | 21.8 | 17.7, 5000 x 256 -> 512 10.4 | 11.8 | 10.5; float32 50k x 64 -> 200 37.6 | - | 35.6, 20k x 64 -> 64 11.4 | - | 11.3
+//   partial results, 100k x 384 -> 1024 194 | 203, x 448 -> 2048 435 | 424; 50k x 512 -> 1024 131 | 132, 640 -> 2048 289 | 249
+//   gradient of x, 100k x 256 -> 1024 106 | 96; 8192 x 512 -> 1024 20.9 | 20.9; 4096 x 512 -> 1024 17.5 | 19.3; 20k x 256 -> 512 18.5 | 19.4
+//   of the weights, 100k x 256 -> 1024 100 | 84, x 384 -> 1024 144 | 177 (a quarter of the pairs' rows are empty), 50k x 512 -> 2048 191 | 166; 5000
+//   x 256 -> 512 10.2 | 11.4
+// So the rule is off by up to a fifth where channels are no multiple of 256 (weights), and forward sums of 257 to 511 channels would gain a tenth.
 template <typename T, int MODE> Shape shape_of(const GatedArgs& a) {
   constexpr bool DUAL = MODE == FORWARD || MODE == PARTIALS;
   const int64_t sms = tc::sm_count();

@@ -18,12 +18,16 @@
 // Matrix instructions are the warp-wide mma.sync.  Measured on this GPU they run at 552 TFLOP/s in bf16 and the special function unit
 // at 4.6e12 results/s.  A score costs one root (distance) and one exponential, the cap two results more unless its polynomial does, so
 // a head of 64 values takes 256 flops of the tensor cores, 0.46 ps, for two to four results, 0.43 to 0.87 ps, and some twenty
-// instructions of arithmetic: matrix instructions at any rate would leave the larger part.  And tiles of 16 rows fit graphs of tens of
-// nodes, where tiles of 128 rows would be three quarters empty.  float32 operands are split into TF32 pairs, three products each.
+// instructions of arithmetic.  Tiles of 16 rows fit graphs of tens of nodes, where tiles of 128 rows would be three quarters empty.  float32
+// operands are split into TF32 pairs, three products each.
 //
-// One graph of 5001 nodes, 8 heads of 64 bfloat16 values, distance and cap: forward 357 us (143 TFLOP/s), by rows 620, by columns 690;
-// 16 graphs of up to 2000 nodes, 8 heads of 32, forward with distance: 175 us, the special functions half busy.  What bounds them is
-// the latency of dependent instructions at the three to six warps a scheduler that the registers leave.
+// One graph of 5001 nodes, 8 heads of 64 bfloat16 values, distance and cap: forward 355 us (144 TFLOP/s), by rows 667, by columns 652;
+// 16 graphs of up to 2000 nodes, 8 heads of 32, forward with distance: 173 us, the special functions half busy.  No pipe is full: what
+// bounds them is the latency of dependent instructions at the two to seven warps a scheduler that the registers leave.  For graphs of some hundred
+// nodes and more, tcgen05 with accumulators in tensor memory would take them out of the registers; that has not been built or measured.
+//
+// Operands whose 16-byte pieces do not lie on 16-byte boundaries (12 bfloat16 channels a head, say) are read value by value, without
+// asynchronous copies: 2000 molecules, 8 heads of 12 channels 1268 us a forward and backward pass, of 16 channels 387.
 #pragma once
 
 #include "tc_common.cuh"
@@ -289,7 +293,7 @@ __device__ __forceinline__ float capped(float x, float unit) {
   return y <= 0.5f ? fmaf(z, more, z) : x == x ? unit * large : x;
 }
 template <int NT> __device__ __forceinline__ void cap_tile(float (&z)[NT][4], float unit, float to_cap, bool has_cap) {
-  if (!has_cap) {
+  if (!has_cap) {                                        // the product is rounded before the greatest score is taken off, as in every pass
     const pair u = both(unit, unit);
 #pragma unroll
     for (int n = 0; n < NT; ++n)

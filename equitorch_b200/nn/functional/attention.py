@@ -37,7 +37,8 @@ def graph_attention(q: Tensor, k: Tensor, v: Tensor, graphs: PackedGraphs, num_h
 
     .. math:: out_i = \sum_j softmax_j(s_{ij}) v_j, \quad s_{ij} = cap \tanh(scale \langle q_i, k_j \rangle / cap) - slope_h |p_i - p_j|
 
-    ``q``, ``k``, ``v`` are ``(N, components, channels)``, float32 or bfloat16, of any strides; the channels are split over
+    ``q``, ``k``, ``v`` are ``(N, components, channels)``, float32 or bfloat16, of any strides (three times as fast where each component's
+    channels of a head are whole 16 bytes on 16-byte boundaries); the channels are split over
     ``num_heads`` heads of at most 128 values (components times channels a head) a node.  A head's inner product runs over all
     components of its channels, so with features of one sequence of irreps in the basis of this package the scores do not change
     under rotations and the result turns as the features do.
@@ -46,8 +47,9 @@ def graph_attention(q: Tensor, k: Tensor, v: Tensor, graphs: PackedGraphs, num_h
     without it they are taken as they are.  ``pos`` (N, 3) and ``slope`` (num_heads,), float32, come together; without them there is no
     distance term.  Nodes of no graph get zeros, and graphs do not touch each other, whatever values they hold.
 
-    Differentiable once in ``q``, ``k``, ``v``, ``pos`` and ``slope`` (the gradient of a distance is zero where two nodes coincide);
-    sums in float32, one order of sums, no atomics."""
+    Differentiable once in ``q``, ``k``, ``v``, ``pos`` and ``slope``: forces from ``pos`` at inference, but no training on forces through it.
+    The gradient of a distance is zero where two nodes coincide; nodes closer than 1e-15 count as closer than they are.  Sums in float32, one
+    order of sums, no atomics; of bfloat16 features, weights and their gradients are rounded to bfloat16 for the products."""
     _ops.check(q, k, v, graphs, num_heads, scale, cap, pos, slope)
     if scale is None:
         scale = (q.shape[1] * q.shape[2] // num_heads) ** -0.5

@@ -28,7 +28,7 @@ def gated_linear(input: Tensor, weight: Tensor, activation: str = "silu") -> Ten
     the first half of a gated feed-forward block, in one kernel.  ``activation`` is ``silu``, ``gelu`` (the one with the error
     function), ``relu`` or ``sigmoid``; of equivariant features it may act on invariant components only.
 
-    float32, float64 or bfloat16, sums in float32 (float64 for float64).  Differentiable once; the backward pass forms both
+    float32, float64 or bfloat16, sums in float32 (float64 for float64).  Differentiable once (no training on forces through it); the backward pass forms both
     projections again, keeps only ``x`` and the weight, and takes scratch of twice the result's size.  float32 and bfloat16 run on
     the tensor cores; where channels or hidden are no multiples of 16 bytes (4 or 8 values) the operands are first copied to wider
     rows."""
