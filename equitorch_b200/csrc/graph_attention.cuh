@@ -293,7 +293,9 @@ __device__ __forceinline__ float capped(float x, float unit) {
   return y <= 0.5f ? fmaf(z, more, z) : x == x ? unit * large : x;
 }
 template <int NT> __device__ __forceinline__ void cap_tile(float (&z)[NT][4], float unit, float to_cap, bool has_cap) {
-  if (!has_cap) {                                        // the product is rounded before the greatest score is taken off, as in every pass
+  // The assembler joins a packed product with a packed addition that is its only use, rounding modifiers or not (measured).  These products have
+  // another use in every pass (the row's maximum, the distance), so scores are rounded before the greatest is taken off, all alike.
+  if (!has_cap) {
     const pair u = both(unit, unit);
 #pragma unroll
     for (int n = 0; n < NT; ++n)
