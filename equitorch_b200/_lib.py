@@ -95,6 +95,31 @@ class AttentionArgs(C.Structure):
                 + [(f, C.c_void_p) for f in ("pos", "slope", "out", "stats", "grad_out", "dq", "dk", "dv", "delta", "geo", "dpos", "dslope")])
 
 
+class RotaryArgs(C.Structure):
+    _fields_ = ([(f, C.c_int32) for f in ("dtype", "comps", "heads", "kv_heads", "size", "half", "interleaved", "backward")] + [("magnitude", C.c_float)]
+                + [(f, C.c_int64) for f in ("n", "q_node", "q_comp", "k_node", "k_comp")]
+                + [(f, C.c_void_p) for f in ("q", "k", "q_out", "k_out", "positions", "frequencies")])
+
+
+class WindowStepArgs(C.Structure):
+    _fields_ = ([(f, C.c_int32) for f in ("dtype", "comps", "heads", "kv_heads", "head_channels")] + [("scale", C.c_float)]
+                + [(f, C.c_int64) for f in ("chains", "capacity", "before", "sinks", "q_chain", "q_comp", "k_chain", "k_node", "k_comp", "v_chain",
+                                            "v_node", "v_comp", "scratch_floats")]
+                + [(f, C.c_void_p) for f in ("q", "k", "v", "out", "lengths", "scratch")])
+
+
+class WindowAttentionArgs(C.Structure):
+    _fields_ = ([(f, C.c_int32) for f in ("dtype", "comps", "heads", "kv_heads", "head_channels", "tile_rows")] + [("scale", C.c_float)]
+                + [(f, C.c_int64) for f in ("n", "num_graphs", "longest", "num_tiles", "before", "after", "sinks", "q_node", "q_comp", "k_node", "k_comp",
+                                            "v_node", "v_comp", "scratch_bytes")]
+                + [(f, C.c_void_p) for f in ("ptr", "tiles", "q", "k", "v", "grad", "out", "dq", "dk", "dv", "stats", "scratch", "status")])
+
+
+class TypeLossArgs(C.Structure):
+    _fields_ = ([(f, C.c_int32) for f in ("dtype", "reduction")] + [(f, C.c_int64) for f in ("n", "c", "t", "scratch_bytes")]
+                + [(f, C.c_void_p) for f in ("x", "w", "target", "losses", "lse", "result", "count", "grad", "dx", "dw", "scratch", "status")])
+
+
 # name -> (restype, argtypes); every symbol declared in include/eqt_b200.h appears here
 SIGNATURES = {
     "eqt_sparse_product": (C.c_int, [C.POINTER(ProductArgs), C.c_void_p]),
@@ -204,6 +229,20 @@ SIGNATURES = {
     "eqt_gated_form": (C.c_int32, [C.c_int32] + [C.c_int64] * 3 + [C.c_int32]),
     "eqt_gated_forward": (C.c_int, [C.c_int32] + [C.c_void_p] * 4 + [C.c_int64] * 4 + [C.c_int32, C.c_void_p, C.c_void_p]),
     "eqt_gated_backward": (C.c_int, [C.c_int32] + [C.c_void_p] * 6 + [C.c_int64] * 4 + [C.c_int32, C.c_void_p, C.c_void_p]),
+    "eqt_add_rms_norm_forward": (C.c_int, [C.c_int32] + [C.c_void_p] * 6 + [C.c_int64] * 3 + [C.c_double, C.c_void_p]),
+    "eqt_add_rms_norm_e4m3": (C.c_int, [C.c_int32] + [C.c_void_p] * 6 + [C.c_int64] * 4 + [C.c_double, C.c_void_p]),
+    "eqt_add_rms_norm_scratch": (C.c_int64, [C.c_int32] + [C.c_int64] * 3),
+    "eqt_add_rms_norm_backward": (C.c_int, [C.c_int32] + [C.c_void_p] * 8 + [C.c_int64] * 4 + [C.c_void_p]),
+    "eqt_rotary": (C.c_int, [C.POINTER(RotaryArgs), C.c_void_p]),
+    "eqt_window_step_scratch": (C.c_int64, [C.POINTER(WindowStepArgs)]),
+    "eqt_window_step": (C.c_int, [C.POINTER(WindowStepArgs), C.c_void_p]),
+    "eqt_window_attention_scratch": (C.c_int64, [C.POINTER(WindowAttentionArgs), C.c_int32]),
+    "eqt_window_attention_form": (C.c_int32, [C.POINTER(WindowAttentionArgs)]),
+    "eqt_window_attention_forward": (C.c_int, [C.POINTER(WindowAttentionArgs), C.c_void_p]),
+    "eqt_window_attention_backward": (C.c_int, [C.POINTER(WindowAttentionArgs), C.c_void_p]),
+    "eqt_type_loss_scratch": (C.c_int64, [C.POINTER(TypeLossArgs), C.c_int32]),
+    "eqt_type_loss_forward": (C.c_int, [C.POINTER(TypeLossArgs), C.c_void_p]),
+    "eqt_type_loss_backward": (C.c_int, [C.POINTER(TypeLossArgs), C.c_void_p]),
     "eqt_last_error": (C.c_char_p, []),
     "eqt_version": (C.c_int, []),
     "eqt_launch_count": (C.c_int64, []),

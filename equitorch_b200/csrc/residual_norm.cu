@@ -1,0 +1,562 @@
+// Root-mean-square norm of a node's values with the residual's addition before it, forward, backward, and with the result in 8 bits.
+//
+// A row is a node's D = d C values (components times channels), so that the norm of equivariant features is invariant:
+//
+//     h = x + res      r = (mean h^2 + eps)^-1/2      y = h r w[channel]
+//     backward, from g = dL/dy and gh = dL/dh (the stream goes on):  gw = g w,  u = h r
+//         dx = dres = gh + r (gw - u mean(gw u))        dw[channel] = sum over nodes and components of g u
+//     8 bits: of every group of values, t = h w, m = max |t|:   value = e4m3(448 t / m), scale = m r / 448
+//
+// All of it is bound by HBM: 16 bytes a bfloat16 value and its residual forward and backward.  A row stays in the registers of 32, 128 or 512
+// threads, as few as hold it with four pieces of 16 bytes each: one reads x and the residual, adds, reduces by shuffles and writes.  A CTA
+// strides over the rows, so the weight is read once and the backward pass has the weight's gradient in registers, summed over the CTA's rows; the
+// CTAs' sums are added in their order by a second kernel (no atomics).  Rows that are no whole pieces of 16 bytes, or longer than 2048
+// pieces, are read twice by loops.
+// 100,003 nodes of 4 x 256 bfloat16 values: see the launches' times at launch_forward and launch_backward.
+#include <cuda_fp8.h>
+
+#include <algorithm>
+
+#include "common.cuh"
+
+namespace eqt {
+namespace residual_norm {
+namespace {
+
+constexpr int PIECES = 4;                                // of 16 bytes a thread
+constexpr float E4M3_MAX = 448.f;
+
+struct NormArgs {
+  const void *x, *res, *w, *g, *gh;
+  void *y, *total, *dx, *dw;
+  uint8_t* values;
+  float *scales, *rstd, *parts;
+  int64_t n;
+  int length, channels, group;                           // values of a row; of a group of 8-bit values
+  float eps;
+};
+
+template <typename T> constexpr int VALUES = 16 / (int)sizeof(T);
+
+template <typename T> __device__ __forceinline__ void unpack(const uint4& u, float (&v)[VALUES<T>]) {
+  const uint32_t r[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      v[i] = __uint_as_float(r[i]);
+    } else {
+      v[2 * i] = __uint_as_float(r[i] << 16);
+      v[2 * i + 1] = __uint_as_float(r[i] & 0xffff0000u);
+    }
+  }
+}
+template <typename T> __device__ __forceinline__ uint4 pack(const float (&v)[VALUES<T>]) {
+  uint32_t r[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      r[i] = __float_as_uint(v[i]);
+    } else {
+      const __nv_bfloat162 two = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+      r[i] = *reinterpret_cast<const uint32_t*>(&two);
+    }
+  }
+  return make_uint4(r[0], r[1], r[2], r[3]);
+}
+
+template <typename V> __device__ __forceinline__ V larger(V a, V b) { return a > b ? a : b; }
+struct Sum {
+  template <typename V> __device__ __forceinline__ V operator()(V a, V b) const { return a + b; }
+};
+struct Max {                                             // drops NaNs
+  template <typename V> __device__ __forceinline__ V operator()(V a, V b) const { return b > a || a != a ? b : a; }
+};
+// Over `lanes` neighbouring threads of a warp, a power of two.
+template <typename V, typename F> __device__ __forceinline__ V across_lanes(V v, int lanes, F f) {
+  for (int o = lanes >> 1; o > 0; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+// Over the THREADS of a row, all of which call it; `buffer` holds a value a warp and is not the one of the call before.
+template <int THREADS, typename V, typename F> __device__ __forceinline__ V across_row(V v, V* buffer, F f) {
+  v = across_lanes(v, 32, f);
+  if constexpr (THREADS > 32) {
+    if ((threadIdx.x & 31) == 0) buffer[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = buffer[0];
+#pragma unroll
+    for (int i = 1; i < THREADS / 32; ++i) v = f(v, buffer[i]);
+  }
+  return v;
+}
+
+// One over the root, as rounded once.
+__device__ __forceinline__ float inverse_root(float sum, int length, float eps) { return __frsqrt_rn(sum / (float)length + eps); }
+
+// ---- 8 bits -------------------------------------------------------------------------------------
+// The result is the nearest of 8 bits to 448 t / m, ties to even, as if computed without rounding before.  In float32, with at most six
+// roundings, the quotient is within 2^-21 of itself; where that leaves two answers (two or three values in 100,000, more where t and m have
+// few bits and ties are real) it is formed in float64 and brought to float32 rounding to odd, which keeps on which side of a border it is.
+__device__ __forceinline__ uint8_t to_e4m3(float v) { return (uint8_t)__nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3); }
+__device__ __forceinline__ uint16_t to_e4m3(float v, float w) { return (uint16_t)__nv_cvt_float2_to_fp8x2(make_float2(v, w), __NV_SATFINITE, __NV_E4M3); }
+__device__ __noinline__ uint8_t to_e4m3_exact(double t, double m) {
+  const double q = t * (double)E4M3_MAX / m;
+  float f = __double2float_rz(q);
+  if ((double)f != q) f = __uint_as_float(__float_as_uint(f) | 1u);
+  return to_e4m3(f);
+}
+constexpr float NEAR = 4.76837158203125e-7f;             // 2^-21
+constexpr float TINY = 1e-30f;                           // below it 448 / m may be infinite
+__device__ __forceinline__ double exact_value(float x, float res, float w) { return ((double)x + (double)res) * (double)w; }
+
+// ---- rows in registers --------------------------------------------------------------------------
+// OUT: 0 values of the type, 1 8 bits with a scale a row, 2 with a scale every p.group values (whole pieces, a power of two of at most 32)
+template <typename T, int ROW_THREADS, int OUT, bool RES>
+__global__ void __launch_bounds__(ROW_THREADS < 128 ? 128 : ROW_THREADS) forward_kernel(const NormArgs p) {
+  constexpr int V = VALUES<T>, ROWS = ROW_THREADS < 128 ? 128 / ROW_THREADS : 1;
+  __shared__ float buffer[2][ROW_THREADS / 32], most_of[2][ROW_THREADS / 32];
+  __shared__ double exact_of[2][ROW_THREADS / 32];
+  const int at = threadIdx.x % ROW_THREADS, pieces = p.length / V;
+  uint4 w[PIECES];
+#pragma unroll
+  for (int i = 0; i < PIECES; ++i) {
+    const int k = at + i * ROW_THREADS;
+    w[i] = make_uint4(0, 0, 0, 0);
+    if (p.w && k < pieces) w[i] = reinterpret_cast<const uint4*>(p.w)[k % (p.channels / V)];
+  }
+  int turn = 0;
+  for (int64_t row0 = (int64_t)blockIdx.x * ROWS; row0 < p.n; row0 += (int64_t)gridDim.x * ROWS, turn ^= 1) {
+    const int64_t row = row0 + threadIdx.x / ROW_THREADS;
+    const bool there = row < p.n;
+    const int64_t first = row * pieces;
+    uint4 x[PIECES], r[PIECES];
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      const int k = at + i * ROW_THREADS;
+      const bool on = there && k < pieces;
+      x[i] = on ? __ldg(reinterpret_cast<const uint4*>(p.x) + first + k) : make_uint4(0, 0, 0, 0);
+      if (RES) r[i] = on ? __ldg(reinterpret_cast<const uint4*>(p.res) + first + k) : make_uint4(0, 0, 0, 0);
+    }
+    float h[PIECES][V], sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      unpack<T>(x[i], h[i]);
+      if (RES) {
+        float b[V];
+        unpack<T>(r[i], b);
+#pragma unroll
+        for (int j = 0; j < V; ++j) h[i][j] += b[j];
+      }
+#pragma unroll
+      for (int j = 0; j < V; ++j) sum = fmaf(h[i][j], h[i][j], sum);
+    }
+    const float inverse = inverse_root(across_row<ROW_THREADS>(sum, buffer[turn], Sum()), p.length, p.eps);
+    if (p.rstd && at == 0 && there) p.rstd[row] = inverse;
+    if (RES && p.total) {
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) {
+        const int k = at + i * ROW_THREADS;
+        if (there && k < pieces) reinterpret_cast<uint4*>(p.total)[first + k] = pack<T>(h[i]);
+      }
+    }
+    if constexpr (OUT == 0) {
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) {
+        const int k = at + i * ROW_THREADS;
+        float y[V], c[V];
+        unpack<T>(w[i], c);
+#pragma unroll
+        for (int j = 0; j < V; ++j) y[j] = p.w ? h[i][j] * inverse * c[j] : h[i][j] * inverse;
+        if (there && k < pieces) reinterpret_cast<uint4*>(p.y)[first + k] = pack<T>(y);
+      }
+    } else {
+      // the greatest |t| of a group: found in float32, and of the values within its error, in float64
+      const int lanes = OUT == 2 ? p.group / V : 32;
+      float most[PIECES];
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) {
+        float c[V];
+        unpack<T>(w[i], c);
+        most[i] = 0.f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) most[i] = Max()(most[i], fabsf(p.w ? h[i][j] * c[j] : h[i][j]));
+        if (OUT == 2) most[i] = across_lanes(most[i], lanes, Max());
+        else if (i) most[0] = Max()(most[0], most[i]);
+      }
+      if (OUT == 1) most[0] = across_row<ROW_THREADS>(most[0], most_of[turn], Max());
+      double exact[PIECES];
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) {
+        float c[V], a[V], b[V];
+        unpack<T>(w[i], c);
+        unpack<T>(x[i], a);
+        if (RES) unpack<T>(r[i], b);
+        const float m = OUT == 1 ? most[0] : most[i];
+        exact[i] = 0.0;
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if (fabsf(p.w ? h[i][j] * c[j] : h[i][j]) >= m * (1.f - NEAR))
+            exact[i] = Max()(exact[i], fabs(exact_value(a[j], RES ? b[j] : 0.f, p.w ? c[j] : 1.f)));
+        if (OUT == 2) exact[i] = across_lanes(exact[i], lanes, Max());
+        else if (i) exact[0] = Max()(exact[0], exact[i]);
+      }
+      if (OUT == 1) exact[0] = across_row<ROW_THREADS>(exact[0], exact_of[turn], Max());
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) {
+        const int k = at + i * ROW_THREADS;
+        if (!there || k >= pieces) continue;
+        const float m = OUT == 1 ? most[0] : most[i], to = m > 0.f ? __fdiv_rn(E4M3_MAX, m) : 0.f;
+        const double em = OUT == 1 ? exact[0] : exact[i];
+        float c[V], a[V], b[V];
+        unpack<T>(w[i], c);
+        uint16_t held[V / 2];
+#pragma unroll
+        for (int j = 0; j < V; j += 2) {
+          const float q0 = (p.w ? h[i][j] * c[j] : h[i][j]) * to, q1 = (p.w ? h[i][j + 1] * c[j + 1] : h[i][j + 1]) * to;
+          const uint16_t low = to_e4m3(q0 * (1.f - NEAR), q1 * (1.f - NEAR)), high = to_e4m3(q0 * (1.f + NEAR), q1 * (1.f + NEAR));
+          held[j / 2] = low;
+          if (low != high || (m < TINY && m > 0.f)) {
+            unpack<T>(x[i], a);
+            if (RES) unpack<T>(r[i], b);
+            held[j / 2] = (uint16_t)(to_e4m3_exact(exact_value(a[j], RES ? b[j] : 0.f, p.w ? c[j] : 1.f), em) |
+                                     to_e4m3_exact(exact_value(a[j + 1], RES ? b[j + 1] : 0.f, p.w ? c[j + 1] : 1.f), em) << 8);
+          }
+        }
+        uint8_t* to_values = p.values + (first + k) * V;
+        if constexpr (V == 8) *reinterpret_cast<uint2*>(to_values) = make_uint2(held[0] | (uint32_t)held[1] << 16, held[2] | (uint32_t)held[3] << 16);
+        else *reinterpret_cast<uint32_t*>(to_values) = held[0] | (uint32_t)held[1] << 16;
+        const float scale = (float)(em * (double)inverse / (double)E4M3_MAX);
+        if (OUT == 2 && k % lanes == 0) p.scales[(first + k) / lanes] = scale;
+        if (OUT == 1 && k == 0) p.scales[row] = scale;
+      }
+    }
+  }
+}
+
+// parts [CTA][values of a row]: the CTA's sums of g u
+template <typename T, int ROW_THREADS>
+__global__ void __launch_bounds__(ROW_THREADS < 128 ? 128 : ROW_THREADS) backward_kernel(const NormArgs p) {
+  constexpr int V = VALUES<T>, ROWS = ROW_THREADS < 128 ? 128 / ROW_THREADS : 1;
+  __shared__ float buffer[2][ROW_THREADS / 32];
+  __shared__ float sums[ROWS > 1 ? PIECES * 32 * V : 1];
+  const int at = threadIdx.x % ROW_THREADS, pieces = p.length / V;
+  uint4 w[PIECES];
+  float dw[PIECES][V];
+#pragma unroll
+  for (int i = 0; i < PIECES; ++i) {
+    const int k = at + i * ROW_THREADS;
+    w[i] = make_uint4(0, 0, 0, 0);
+    if (p.w && k < pieces) w[i] = reinterpret_cast<const uint4*>(p.w)[k % (p.channels / V)];
+#pragma unroll
+    for (int j = 0; j < V; ++j) dw[i][j] = 0.f;
+  }
+  int turn = 0;
+  for (int64_t row0 = (int64_t)blockIdx.x * ROWS; row0 < p.n; row0 += (int64_t)gridDim.x * ROWS, turn ^= 1) {
+    const int64_t row = row0 + threadIdx.x / ROW_THREADS;
+    const bool there = row < p.n;
+    const int64_t first = row * pieces;
+    uint4 g[PIECES], t[PIECES], s[PIECES];
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      const int k = at + i * ROW_THREADS;
+      const bool on = there && k < pieces;
+      g[i] = on ? __ldg(reinterpret_cast<const uint4*>(p.g) + first + k) : make_uint4(0, 0, 0, 0);
+      t[i] = on ? __ldg(reinterpret_cast<const uint4*>(p.total) + first + k) : make_uint4(0, 0, 0, 0);
+      s[i] = p.gh && on ? __ldg(reinterpret_cast<const uint4*>(p.gh) + first + k) : make_uint4(0, 0, 0, 0);
+    }
+    const float inverse = there ? __ldg(p.rstd + row) : 0.f;
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      float a[V], c[V], h[V];
+      unpack<T>(g[i], a);
+      unpack<T>(w[i], c);
+      unpack<T>(t[i], h);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float u = h[j] * inverse;
+        dw[i][j] = fmaf(a[j], u, dw[i][j]);
+        sum = fmaf(p.w ? a[j] * c[j] : a[j], u, sum);
+      }
+    }
+    const float mean = across_row<ROW_THREADS>(sum, buffer[turn], Sum()) / (float)p.length;
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      const int k = at + i * ROW_THREADS;
+      float a[V], c[V], h[V], e[V], out[V];
+      unpack<T>(g[i], a);
+      unpack<T>(w[i], c);
+      unpack<T>(t[i], h);
+      unpack<T>(s[i], e);
+#pragma unroll
+      for (int j = 0; j < V; ++j) out[j] = fmaf(inverse, fmaf(-(h[j] * inverse), mean, p.w ? a[j] * c[j] : a[j]), e[j]);
+      if (there && k < pieces) reinterpret_cast<uint4*>(p.dx)[first + k] = pack<T>(out);
+    }
+  }
+  if (!p.parts) return;
+  float* part = p.parts + (int64_t)blockIdx.x * p.length;
+  if constexpr (ROWS > 1) {                              // the CTA's rows in their order
+    for (int q = 0; q < ROWS; ++q) {
+      if ((int)threadIdx.x / ROW_THREADS == q) {
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i)
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            float& sum = sums[(i * 32 + at) * V + j];
+            sum = q ? sum + dw[i][j] : dw[i][j];
+          }
+      }
+      __syncthreads();
+    }
+    for (int k = threadIdx.x; k < p.length; k += blockDim.x) part[k] = sums[k];
+  } else {
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      const int k = at + i * ROW_THREADS;
+      if (k >= pieces) continue;
+#pragma unroll
+      for (int j = 0; j < V; ++j) part[k * V + j] = dw[i][j];
+    }
+  }
+}
+
+// ---- rows of any length and alignment -----------------------------------------------------------
+constexpr int LONG_THREADS = 256;
+template <typename T, bool EIGHT> __global__ void __launch_bounds__(LONG_THREADS) forward_long_kernel(const NormArgs p) {
+  __shared__ float buffer[2][LONG_THREADS / 32], most_of[2][LONG_THREADS / 32];
+  __shared__ double exact_of[2][LONG_THREADS / 32];
+  const T *x = static_cast<const T*>(p.x), *res = static_cast<const T*>(p.res), *w = static_cast<const T*>(p.w);
+  int turn = 0;
+  for (int64_t row = blockIdx.x; row < p.n; row += gridDim.x, turn ^= 1) {
+    const int64_t first = row * p.length;
+    auto value = [&](int k) { return ld(x + first + k) + (res ? ld(res + first + k) : 0.f); };
+    auto weight = [&](int k) { return w ? ld(w + k % p.channels) : 1.f; };
+    auto exact_at = [&](int k) { return fabs(exact_value(ld(x + first + k), res ? ld(res + first + k) : 0.f, weight(k))); };
+    float sum = 0.f;
+    for (int k = threadIdx.x; k < p.length; k += LONG_THREADS) {
+      const float h = value(k);
+      sum = fmaf(h, h, sum);
+    }
+    const float inverse = inverse_root(across_row<LONG_THREADS>(sum, buffer[turn], Sum()), p.length, p.eps);
+    if (p.rstd && threadIdx.x == 0) p.rstd[row] = inverse;
+    if constexpr (!EIGHT) {
+      for (int k = threadIdx.x; k < p.length; k += LONG_THREADS) {
+        const float h = value(k);
+        st(static_cast<T*>(p.y) + first + k, w ? h * inverse * weight(k) : h * inverse);
+        if (res && p.total) st(static_cast<T*>(p.total) + first + k, h);
+      }
+    } else {
+      const bool whole = p.group == p.length;
+      const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+      float most = 0.f;
+      double exact = 0.0;
+      if (whole) {                                       // one group: by all threads
+        for (int k = threadIdx.x; k < p.length; k += LONG_THREADS) most = Max()(most, fabsf(value(k) * weight(k)));
+        most = across_row<LONG_THREADS>(most, most_of[turn], Max());
+        for (int k = threadIdx.x; k < p.length; k += LONG_THREADS)
+          if (fabsf(value(k) * weight(k)) >= most * (1.f - NEAR)) exact = Max()(exact, exact_at(k));
+        exact = across_row<LONG_THREADS>(exact, exact_of[turn], Max());
+      }
+      for (int start = whole ? 0 : warp * p.group; start < p.length; start += whole ? p.length : LONG_THREADS / 32 * p.group) {
+        const int from = whole ? (int)threadIdx.x : start + lane, step = whole ? LONG_THREADS : 32, end = start + p.group;
+        if (!whole) {
+          most = 0.f;
+          exact = 0.0;
+          for (int k = from; k < end; k += step) most = Max()(most, fabsf(value(k) * weight(k)));
+          most = across_lanes(most, 32, Max());
+          for (int k = from; k < end; k += step)
+            if (fabsf(value(k) * weight(k)) >= most * (1.f - NEAR)) exact = Max()(exact, exact_at(k));
+          exact = across_lanes(exact, 32, Max());
+        }
+        const float to = most > 0.f ? __fdiv_rn(E4M3_MAX, most) : 0.f;
+        for (int k = from; k < end; k += step) {
+          const float h = value(k), q = h * weight(k) * to;
+          uint8_t held = to_e4m3(q * (1.f - NEAR));
+          if (held != to_e4m3(q * (1.f + NEAR)) || (most < TINY && most > 0.f))
+            held = to_e4m3_exact(exact_value(ld(x + first + k), res ? ld(res + first + k) : 0.f, weight(k)), exact);
+          p.values[first + k] = held;
+          if (res && p.total) st(static_cast<T*>(p.total) + first + k, h);
+        }
+        if (whole ? threadIdx.x == 0 : lane == 0) p.scales[row * (p.length / p.group) + start / p.group] = (float)(exact * (double)inverse / (double)E4M3_MAX);
+      }
+    }
+  }
+}
+
+template <typename T> __global__ void __launch_bounds__(LONG_THREADS) backward_long_kernel(const NormArgs p) {
+  __shared__ float buffer[2][LONG_THREADS / 32];
+  const T *g = static_cast<const T*>(p.g), *gh = static_cast<const T*>(p.gh), *total = static_cast<const T*>(p.total), *w = static_cast<const T*>(p.w);
+  int turn = 0;
+  for (int64_t row = blockIdx.x; row < p.n; row += gridDim.x, turn ^= 1) {
+    const int64_t first = row * p.length;
+    const float inverse = p.rstd[row];
+    auto weighted = [&](int k) { return w ? ld(g + first + k) * ld(w + k % p.channels) : ld(g + first + k); };
+    float sum = 0.f;
+    for (int k = threadIdx.x; k < p.length; k += LONG_THREADS) sum = fmaf(weighted(k), ld(total + first + k) * inverse, sum);
+    const float mean = across_row<LONG_THREADS>(sum, buffer[turn], Sum()) / (float)p.length;
+    for (int k = threadIdx.x; k < p.length; k += LONG_THREADS)
+      st(static_cast<T*>(p.dx) + first + k, fmaf(inverse, fmaf(-(ld(total + first + k) * inverse), mean, weighted(k)), gh ? ld(gh + first + k) : 0.f));
+  }
+}
+// The weight's gradient of such rows: a thread has a place of the row, a CTA a part of the rows.
+template <typename T> __global__ void __launch_bounds__(LONG_THREADS) weight_long_kernel(const NormArgs p, int64_t part_rows) {
+  const T *g = static_cast<const T*>(p.g), *total = static_cast<const T*>(p.total);
+  const int k = blockIdx.y * LONG_THREADS + threadIdx.x;
+  if (k >= p.length) return;
+  const int64_t end = min(p.n, (int64_t)(blockIdx.x + 1) * part_rows);
+  float sum = 0.f;
+#pragma unroll 4
+  for (int64_t row = blockIdx.x * part_rows; row < end; ++row) sum = fmaf(ld(g + row * p.length + k), ld(total + row * p.length + k) * __ldg(p.rstd + row), sum);
+  p.parts[(int64_t)blockIdx.x * p.length + k] = sum;
+}
+
+// dw[c] = the parts' sums over the components: a CTA has 32 channels, eight warps take parts in turn
+template <typename T> __global__ void __launch_bounds__(256) weight_sum_kernel(const NormArgs p, int parts) {
+  __shared__ float sums[8][32];
+  const int c = blockIdx.x * 32 + (threadIdx.x & 31), warp = threadIdx.x >> 5, comps = p.length / p.channels;
+  float sum = 0.f;
+  if (c < p.channels)
+    for (int m = 0; m < comps; ++m) {
+      const float* from = p.parts + m * p.channels + c;
+#pragma unroll 8
+      for (int q = warp; q < parts; q += 8) sum += from[(int64_t)q * p.length];
+    }
+  sums[warp][threadIdx.x & 31] = sum;
+  __syncthreads();
+  if (warp || c >= p.channels) return;
+#pragma unroll
+  for (int i = 1; i < 8; ++i) sum += sums[i][threadIdx.x];
+  st(static_cast<T*>(p.dw) + c, sum);
+}
+
+// ---- host side ----------------------------------------------------------------------------------
+int size_of(int dtype) { return dtype == EQT_F32 ? 4 : 2; }
+
+// Threads of a row held in registers; 0 where it is read by loops.
+int row_threads(int dtype, int64_t length, int64_t channels, uintptr_t bits) {
+  const int v = 16 / size_of(dtype);
+  if (bits % 16 || length % v || channels % v) return 0;
+  const int64_t pieces = length / v;
+  return pieces <= 32 * PIECES ? 32 : pieces <= 128 * PIECES ? 128 : pieces <= 512 * PIECES ? 512 : 0;
+}
+// CTAs of the backward pass, whose sums of the weight's gradient are added afterwards: two waves of what fits an SM.
+unsigned part_ctas(int threads, int64_t n) {
+  const int64_t rows = threads == 32 ? 4 : 1;
+  return (unsigned)std::min<int64_t>(ceil_div(n, rows), (int64_t)sm_count() * (threads == 512 ? 2 : 6));
+}
+// Parts of the rows where they are read by loops.
+int64_t long_parts(int64_t n) { return std::min<int64_t>(ceil_div(n, 16), 128); }
+
+int check(int dtype, int64_t n, int64_t comps, int64_t channels) {
+  if (dtype != EQT_F32 && dtype != EQT_BF16) return fail(EQT_ERR_BAD_ARGUMENT, "add_rms_norm: unknown dtype %d", dtype);
+  if (n < 0 || comps < 0 || channels < 0) return fail(EQT_ERR_BAD_ARGUMENT, "add_rms_norm: negative size");
+  if (n > INT32_MAX || comps > 1 << 24 || channels > 1 << 24 || comps * channels > 1 << 24)
+    return fail(EQT_ERR_UNSUPPORTED, "add_rms_norm: at most 2^31 nodes of 2^24 values");
+  return EQT_OK;
+}
+
+template <typename T, int THREADS, int OUT> int launch_rows(const NormArgs& p, cudaStream_t s) {
+  constexpr int ROWS = THREADS < 128 ? 128 / THREADS : 1;
+  const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(p.n, ROWS), (int64_t)sm_count() * (THREADS == 512 ? 4 : 16));
+  if (p.res) forward_kernel<T, THREADS, OUT, true><<<grid, THREADS < 128 ? 128 : THREADS, 0, s>>>(p);
+  else forward_kernel<T, THREADS, OUT, false><<<grid, THREADS < 128 ? 128 : THREADS, 0, s>>>(p);
+  return check_launch("add_rms_norm");
+}
+template <typename T, int OUT> int launch_forward(const NormArgs& p, int threads, cudaStream_t s) {
+  switch (threads) {
+    case 32: return launch_rows<T, 32, OUT>(p, s);
+    case 128: return launch_rows<T, 128, OUT>(p, s);
+    case 512: return launch_rows<T, 512, OUT>(p, s);
+  }
+  forward_long_kernel<T, OUT != 0><<<(unsigned)std::min<int64_t>(p.n, (int64_t)sm_count() * 8), LONG_THREADS, 0, s>>>(p);
+  return check_launch("add_rms_norm");
+}
+template <typename T> int launch_backward(const NormArgs& p, int threads, cudaStream_t s) {
+  int parts;
+  if (threads) {
+    parts = (int)part_ctas(threads, p.n);
+    if (threads == 32) backward_kernel<T, 32><<<parts, 128, 0, s>>>(p);
+    else if (threads == 128) backward_kernel<T, 128><<<parts, 128, 0, s>>>(p);
+    else backward_kernel<T, 512><<<parts, 512, 0, s>>>(p);
+    if (int rc = check_launch("add_rms_norm_backward")) return rc;
+  } else {
+    backward_long_kernel<T><<<(unsigned)std::min<int64_t>(p.n, (int64_t)sm_count() * 8), LONG_THREADS, 0, s>>>(p);
+    if (int rc = check_launch("add_rms_norm_backward")) return rc;
+    if (!p.parts) return EQT_OK;
+    parts = (int)long_parts(p.n);
+    weight_long_kernel<T><<<dim3((unsigned)parts, (unsigned)ceil_div(p.length, LONG_THREADS)), LONG_THREADS, 0, s>>>(p, ceil_div(p.n, parts));
+    if (int rc = check_launch("add_rms_norm_weight")) return rc;
+  }
+  if (!p.parts) return EQT_OK;
+  weight_sum_kernel<T><<<(unsigned)ceil_div(p.channels, 32), 256, 0, s>>>(p, parts);
+  return check_launch("add_rms_norm_weight_sum");
+}
+
+uintptr_t bits_of(std::initializer_list<const void*> pointers) {
+  uintptr_t bits = 0;
+  for (const void* p : pointers) bits |= reinterpret_cast<uintptr_t>(p);
+  return bits;
+}
+
+}  // namespace
+}  // namespace residual_norm
+}  // namespace eqt
+
+using namespace eqt;
+using namespace eqt::residual_norm;
+
+extern "C" int eqt_add_rms_norm_forward(int32_t dtype, const void* x, const void* residual, const void* weight, void* out, void* total, float* rstd,
+                                        int64_t n, int64_t comps, int64_t channels, double eps, void* stream) {
+  if (int rc = check(dtype, n, comps, channels)) return rc;
+  if (n == 0 || comps * channels == 0) return EQT_OK;
+  if (!x || !out) return fail(EQT_ERR_BAD_ARGUMENT, "add_rms_norm: NULL pointer");
+  NormArgs p{};
+  p.x = x, p.res = residual, p.w = weight, p.y = out, p.total = total, p.rstd = rstd, p.n = n, p.eps = (float)eps;
+  p.length = (int)(comps * channels), p.channels = (int)channels;
+  const int threads = row_threads(dtype, p.length, channels, bits_of({x, residual, weight, out, total}));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return dtype == EQT_F32 ? launch_forward<float, 0>(p, threads, s) : launch_forward<__nv_bfloat16, 0>(p, threads, s);
+}
+
+extern "C" int eqt_add_rms_norm_e4m3(int32_t dtype, const void* x, const void* residual, const void* weight, void* values, float* scales, void* total,
+                                     int64_t n, int64_t comps, int64_t channels, int64_t group, double eps, void* stream) {
+  if (int rc = check(dtype, n, comps, channels)) return rc;
+  if (n == 0 || comps * channels == 0) return EQT_OK;
+  if (!x || !values || !scales) return fail(EQT_ERR_BAD_ARGUMENT, "add_rms_norm: NULL pointer");
+  if (group < 1 || (comps * channels) % group) return fail(EQT_ERR_BAD_ARGUMENT, "add_rms_norm: rows of %lld values are no groups of %lld", (long long)(comps * channels), (long long)group);
+  NormArgs p{};
+  p.x = x, p.res = residual, p.w = weight, p.values = static_cast<uint8_t*>(values), p.scales = scales, p.total = total, p.n = n, p.eps = (float)eps;
+  p.length = (int)(comps * channels), p.channels = (int)channels, p.group = (int)group;
+  int threads = row_threads(dtype, p.length, channels, bits_of({x, residual, weight, values, total}));
+  const int64_t lanes = group * size_of(dtype) / 16;
+  const bool whole = group == p.length, pieces = group * size_of(dtype) % 16 == 0 && lanes <= 32 && (lanes & (lanes - 1)) == 0;
+  if (!whole && !pieces) threads = 0;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (dtype == EQT_F32) return whole ? launch_forward<float, 1>(p, threads, s) : launch_forward<float, 2>(p, threads, s);
+  return whole ? launch_forward<__nv_bfloat16, 1>(p, threads, s) : launch_forward<__nv_bfloat16, 2>(p, threads, s);
+}
+
+extern "C" int64_t eqt_add_rms_norm_scratch(int32_t dtype, int64_t n, int64_t comps, int64_t channels) {
+  if (check(dtype, n, comps, channels)) return 0;
+  const int threads = row_threads(dtype, comps * channels, channels, 0);
+  return std::max<int64_t>(threads ? part_ctas(threads, n) : 0, long_parts(n)) * comps * channels;
+}
+
+extern "C" int eqt_add_rms_norm_backward(int32_t dtype, const void* grad, const void* grad_total, const void* total, const void* weight, const float* rstd,
+                                         void* dx, void* dweight, float* scratch, int64_t scratch_floats, int64_t n, int64_t comps, int64_t channels,
+                                         void* stream) {
+  if (int rc = check(dtype, n, comps, channels)) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (n == 0 || comps * channels == 0) {
+    if (dweight && channels && cudaMemsetAsync(dweight, 0, (size_t)channels * size_of(dtype), s) != cudaSuccess) return fail(EQT_ERR_CUDA, "cudaMemsetAsync failed");
+    return EQT_OK;
+  }
+  if (!grad || !total || !rstd || !dx || (dweight && !scratch)) return fail(EQT_ERR_BAD_ARGUMENT, "add_rms_norm backward: NULL pointer");
+  if (dweight && scratch_floats < eqt_add_rms_norm_scratch(dtype, n, comps, channels))
+    return fail(EQT_ERR_BAD_ARGUMENT, "add_rms_norm backward: %lld values of scratch given, %lld needed", (long long)scratch_floats,
+                (long long)eqt_add_rms_norm_scratch(dtype, n, comps, channels));
+  NormArgs p{};
+  p.g = grad, p.gh = grad_total, p.total = const_cast<void*>(total), p.w = weight, p.rstd = const_cast<float*>(rstd), p.dx = dx, p.dw = dweight;
+  p.parts = dweight ? scratch : nullptr, p.n = n, p.length = (int)(comps * channels), p.channels = (int)channels;
+  const int threads = row_threads(dtype, p.length, channels, bits_of({grad, grad_total, total, weight, dx}));
+  return dtype == EQT_F32 ? launch_backward<float>(p, threads, s) : launch_backward<__nv_bfloat16>(p, threads, s);
+}

@@ -713,6 +713,95 @@ int eqt_gated_forward(int32_t dtype, const void* x, const void* w, void* h, void
 int eqt_gated_backward(int32_t dtype, const void* x, const void* w, const void* g, void* dx, void* dw, void* scratch,
                        int64_t scratch_bytes, int64_t n, int64_t c, int64_t f, int32_t act, int32_t* status, void* stream);
 
+/* Root-mean-square norm of a node's values (comps components of `channels` channels) after the residual's addition:  h = x + residual,
+ * out = h (mean h^2 + eps)^-1/2 weight[channel].  residual, weight, total (h, written where a residual is given) and rstd (n floats, the
+ * inverse roots, for the backward pass) may be NULL.  All (n, comps, channels), contiguous, float32 or bfloat16; weight (channels).
+ * The e4m3 form has 8-bit values and a float scale for every `group` values (a divisor of comps * channels); value = the nearest to 448 t / max |t| of
+ * t = h weight, ties to even, not a rounded quotient's.
+ * Backward: dx (also the residual's gradient) from grad and grad_total (dL/dh; may be NULL), and dweight (may be NULL); no atomics.
+ * scratch: eqt_add_rms_norm_scratch floats, needed for dweight. */
+int eqt_add_rms_norm_forward(int32_t dtype, const void* x, const void* residual, const void* weight, void* out, void* total, float* rstd, int64_t n,
+                             int64_t comps, int64_t channels, double eps, void* stream);
+int eqt_add_rms_norm_e4m3(int32_t dtype, const void* x, const void* residual, const void* weight, void* values, float* scales, void* total, int64_t n,
+                          int64_t comps, int64_t channels, int64_t group, double eps, void* stream);
+int64_t eqt_add_rms_norm_scratch(int32_t dtype, int64_t n, int64_t comps, int64_t channels);
+int eqt_add_rms_norm_backward(int32_t dtype, const void* grad, const void* grad_total, const void* total, const void* weight, const float* rstd, void* dx,
+                              void* dweight, float* scratch, int64_t scratch_floats, int64_t n, int64_t comps, int64_t channels, void* stream);
+
+/* Rotary positions of q and, where given, k: (n, comps, heads * size), channels next to each other, any strides (in values) of nodes and
+ * components; results contiguous.  The first 2 * half channels of a head turn by positions[node] * frequencies[pair] (backward: by minus that)
+ * and are multiplied by `magnitude`; pairs are (j, j + half) or, interleaved, (2 j, 2 j + 1). */
+typedef struct {
+  int32_t dtype, comps, heads, kv_heads, size, half, interleaved, backward;
+  float magnitude;
+  int64_t n, q_node, q_comp, k_node, k_comp;
+  const void *q, *k;
+  void *q_out, *k_out;
+  const int64_t* positions;
+  const double* frequencies;
+} eqt_rotary_args;
+int eqt_rotary(const eqt_rotary_args* args, void* stream);
+
+/* Attention of one new node of every chain over a cache: q (chains, comps, heads * head_channels), k and v (chains, capacity, comps,
+ * kv_heads * head_channels), strides in values.  lengths[chain] nodes of the cache count, the last of them the new one: it sees the nodes from
+ * lengths - 1 - before on and the first `sinks`.  out (chains, comps, heads * head_channels), contiguous; zeros for a chain of length zero.
+ * Lengths are read on the device; one above the capacity counts as the capacity.  scratch: eqt_window_step_scratch floats. */
+typedef struct {
+  int32_t dtype, comps, heads, kv_heads, head_channels;
+  float scale;
+  int64_t chains, capacity, before, sinks, q_chain, q_comp, k_chain, k_node, k_comp, v_chain, v_node, v_comp, scratch_floats;
+  const void *q, *k, *v;
+  void* out;
+  const int64_t* lengths;
+  float* scratch;
+} eqt_window_step_args;
+int64_t eqt_window_step_scratch(const eqt_window_step_args* args);
+int eqt_window_step(const eqt_window_step_args* args, void* stream);
+
+/* Attention within windows of packed chains.  The nodes of chain g are [ptr[g], ptr[g + 1]); node i sees the nodes j of its chain with j <= i + after
+ * and, of those, the ones from i - before on and the chain's first `sinks`.  q, out and dq (n, comps, heads * head_channels), k, v, dk and dv (n,
+ * comps, kv_heads * head_channels); inputs with channels next to each other and any strides (in values), the others contiguous; float32 or
+ * bfloat16; at most 128 values (comps * head_channels) a head.  Head h has the keys of head h / (heads / kv_heads).
+ *   s_ij = scale <q_i, k_j>,   out_i = sum_j softmax_j(s_ij) v_j;   rows of nodes that belong to no chain are zero, their gradients too
+ * stats (2, heads, n): a row's greatest score in units of log2 and one over its sum of weights from there, needed for the backward pass.  tiles: as for eqt_attention_forward.  scratch:
+ * eqt_window_attention_scratch bytes, 16-byte aligned; status as for eqt_gated_forward.  Backward: grad contiguous; all three gradients are written; no atomics. */
+typedef struct {
+  int32_t dtype, comps, heads, kv_heads, head_channels, tile_rows;
+  float scale;
+  int64_t n, num_graphs, longest, num_tiles, before, after, sinks, q_node, q_comp, k_node, k_comp, v_node, v_comp, scratch_bytes;
+  const int64_t* ptr;
+  const int32_t* tiles;
+  const void *q, *k, *v, *grad;
+  void *out, *dq, *dk, *dv;
+  float* stats;
+  void* scratch;
+  int32_t* status;
+} eqt_window_attention_args;
+int64_t eqt_window_attention_scratch(const eqt_window_attention_args* args, int32_t backward);
+/* 1 where a call runs tiles of 128 nodes on the 5th-generation tensor cores, 0 where it runs the tiles of one chain. */
+int32_t eqt_window_attention_form(const eqt_window_attention_args* args);
+int eqt_window_attention_forward(const eqt_window_attention_args* args, void* stream);
+int eqt_window_attention_backward(const eqt_window_attention_args* args, void* stream);
+
+/* Cross entropy over the types of a table: logits z = x w^T of x (n, c) and w (t, c), never kept;  losses[i] = log sum_t exp z_it - z_i,target.
+ * Rows of a negative target do not count: their loss is zero and they have no gradient.  A target from t on gives NaN.  reduction: 0 none,
+ * 1 sum, 2 mean over the rows that count (zero if none does), to result[0]; count[0]: how many count.  lse (n): the rows' log sums, for the backward pass.
+ * Backward: grad (n floats for reduction 0, else 1) and what the forward pass left; dx (n, c), dw (t, c), either may be NULL.  float32 (as six
+ * bfloat16 products of three parts each) or bfloat16, all contiguous; sums in float32, no atomics.  scratch: eqt_type_loss_scratch bytes, 16-byte aligned. */
+typedef struct {
+  int32_t dtype, reduction;
+  int64_t n, c, t, scratch_bytes;
+  const void *x, *w;
+  const int64_t* target;
+  float *losses, *lse, *result, *count;
+  const float* grad;
+  void *dx, *dw, *scratch;
+  int32_t* status;
+} eqt_type_loss_args;
+int64_t eqt_type_loss_scratch(const eqt_type_loss_args* args, int32_t backward);
+int eqt_type_loss_forward(const eqt_type_loss_args* args, void* stream);
+int eqt_type_loss_backward(const eqt_type_loss_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
