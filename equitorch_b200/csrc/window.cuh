@@ -1,0 +1,119 @@
+// Attention within windows of packed chains: what its kernels share.
+//
+// Node i of a chain [lo, hi) sees the nodes j of it with  j <= i + after  and  (j >= i - before  or  j < lo + sinks):
+//
+//     s_ij = scale <q_i, k_j>      P_ij = exp(s_ij) / sum_j exp(s_ij)      out_i = sum_j P_ij v_j
+//     dP_ij = <g_i, v_j>           delta_i = <g_i, out_i>                  dS_ij = P_ij (dP_ij - delta_i)
+//     dv_j = sum_i P_ij g_i        dq_i = scale sum_j dS_ij k_j            dk_j = scale sum_i dS_ij q_i
+//
+// over the heads that share k and v, for dk and dv.
+//
+// A tile's products run over nodes that some of its rows do not see, with weights of zero, and zero times infinity or a NaN is a NaN.  So a row whose
+// result is not finite is done again, one visible node at a time (`again_*`): a NaN that is not seen does not reach it, and one that is seen does.
+#pragma once
+
+#include "graph_attention.cuh"
+
+namespace eqt {
+namespace window {
+using attention::AttentionParams;
+using attention::Operand;
+using attention::exp2_fast;
+using attention::LOG2E;
+
+struct WindowParams {
+  AttentionParams q, kv;     // of the heads of queries; of the heads of keys (dk and dv)
+  int before, after, sinks, group;
+};
+
+__device__ __forceinline__ bool sees(const WindowParams& p, int i, int j, int lo) { return j <= i + p.after && (j >= i - p.before || j < lo + p.sinks); }
+
+// A lane's values (every 32nd) of a head's row; and of an operand with contiguous rows of `heads` heads.
+template <typename T> __device__ __forceinline__ void lane_row(float (&v)[4], const Operand& x, int node, int head, const AttentionParams& p, int lane) {
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const int e = lane + 32 * c, comp = e / p.size;
+    v[c] = comp < p.comps ? static_cast<float>(static_cast<const T*>(x.p)[node * x.node + comp * x.comp + (int64_t)head * p.size + e - comp * p.size]) : 0.f;
+  }
+}
+template <typename T> __device__ __forceinline__ void lane_put(void* out, const float (&v)[4], float f, int node, int head, const AttentionParams& p, int lane) {
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const int e = lane + 32 * c, comp = e / p.size;
+    if (comp < p.comps) st(static_cast<T*>(out) + (((int64_t)node * p.comps + comp) * p.heads + head) * p.size + e - comp * p.size, v[c] * f);
+  }
+}
+__device__ __forceinline__ float lanes_dot(const float (&a)[4], const float (&b)[4]) {
+  float s = a[0] * b[0] + a[1] * b[1] + a[2] * b[2] + a[3] * b[3];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  return s;
+}
+
+// One row, by a warp.
+template <typename T> __device__ __noinline__ void again_forward(const WindowParams& p, int i, int head, int lo, int hi, int lane) {
+  const int kv = head / p.group;
+  float q[4], k[4], v[4], o[4] = {0.f, 0.f, 0.f, 0.f}, top = -INFINITY, sum = 0.f;
+  lane_row<T>(q, p.q.q, i, head, p.q, lane);
+  const int end = (int)min((int64_t)hi, (int64_t)i + p.after + 1);
+  for (int j = lo; j < end; ++j) {
+    if (j >= lo + p.sinks && j < i - p.before) j = i - p.before;
+    lane_row<T>(k, p.q.k, j, kv, p.q, lane);
+    lane_row<T>(v, p.q.v, j, kv, p.q, lane);
+    const float s = lanes_dot(q, k) * (p.q.scale * LOG2E), now = fmaxf(top, s), base = now == -INFINITY ? 0.f : now;
+    const float keep = exp2_fast(top - base), w = exp2_fast(s - base);
+    sum = sum * keep + w;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) o[c] = w == 0.f ? o[c] * keep : fmaf(w, v[c], o[c] * keep);      // a score of minus infinity is no part of the sum
+    top = now;
+  }
+  lane_put<T>(p.q.out, o, 1.f / sum, i, head, p.q, lane);
+}
+template <typename T> __device__ __noinline__ void again_rows(const WindowParams& p, int i, int head, int lo, int hi, int lane) {
+  const int kv = head / p.group;
+  const int64_t at = (int64_t)head * p.q.n + i;
+  const float top = p.q.top[at], inverse = p.q.inverse[at], delta = p.q.delta[at];
+  float q[4], k[4], v[4], g[4], dq[4] = {0.f, 0.f, 0.f, 0.f};
+  lane_row<T>(q, p.q.q, i, head, p.q, lane);
+  lane_row<T>(g, p.q.g, i, head, p.q, lane);
+  const int end = (int)min((int64_t)hi, (int64_t)i + p.after + 1);
+  for (int j = lo; j < end; ++j) {
+    if (j >= lo + p.sinks && j < i - p.before) j = i - p.before;
+    lane_row<T>(k, p.q.k, j, kv, p.q, lane);
+    lane_row<T>(v, p.q.v, j, kv, p.q, lane);
+    const float w = exp2_fast(lanes_dot(q, k) * (p.q.scale * LOG2E) - top) * inverse, ds = w * (lanes_dot(g, v) - delta);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) dq[c] = fmaf(ds, k[c], dq[c]);
+  }
+  lane_put<T>(p.q.dq, dq, p.q.scale, i, head, p.q, lane);
+}
+template <typename T> __device__ __noinline__ void again_columns(const WindowParams& p, int j, int kv, int lo, int hi, int lane) {
+  float q[4], k[4], v[4], g[4], dk[4] = {0.f, 0.f, 0.f, 0.f}, dv[4] = {0.f, 0.f, 0.f, 0.f};
+  lane_row<T>(k, p.q.k, j, kv, p.q, lane);
+  lane_row<T>(v, p.q.v, j, kv, p.q, lane);
+  const int start = (int)max((int64_t)lo, (int64_t)j - p.after), end = j < lo + p.sinks ? hi : (int)min((int64_t)hi, (int64_t)j + p.before + 1);
+  for (int head = kv * p.group; head < (kv + 1) * p.group; ++head)
+    for (int i = start; i < end; ++i) {
+      const int64_t at = (int64_t)head * p.q.n + i;
+      lane_row<T>(q, p.q.q, i, head, p.q, lane);
+      lane_row<T>(g, p.q.g, i, head, p.q, lane);
+      const float w = exp2_fast(lanes_dot(q, k) * (p.q.scale * LOG2E) - p.q.top[at]) * p.q.inverse[at], ds = w * (lanes_dot(g, v) - p.q.delta[at]);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        dv[c] = fmaf(w, g[c], dv[c]);
+        dk[c] = fmaf(ds, q[c], dk[c]);
+      }
+    }
+  lane_put<T>(p.kv.dk, dk, p.q.scale, j, kv, p.kv, lane);
+  lane_put<T>(p.kv.dv, dv, 1.f, j, kv, p.kv, lane);
+}
+
+__device__ __forceinline__ bool is_finite(float x) { return fabsf(x) < INFINITY; }
+
+int tiles_forward_f32(const WindowParams& p, int tile_rows, int64_t num_tiles, cudaStream_t s);   // window_f32.cu and window_bf16.cu
+int tiles_forward_bf16(const WindowParams& p, int tile_rows, int64_t num_tiles, cudaStream_t s);
+int tiles_backward_f32(const WindowParams& p, int tile_rows, int64_t num_tiles, cudaStream_t s);
+int tiles_backward_bf16(const WindowParams& p, int tile_rows, int64_t num_tiles, cudaStream_t s);
+
+}  // namespace window
+}  // namespace eqt

@@ -1,6 +1,83 @@
-#include "common.cuh"
+// Attention within windows of packed chains: the C entry points.
+#include <algorithm>
+
+#include "window.cuh"
+
+namespace eqt {
+namespace window {
+namespace {
+
+size_t up(size_t b) { return (b + 1023) / 1024 * 1024; }
+
+int check(const eqt_window_attention_args* a) {
+  if (!a) return fail(EQT_ERR_BAD_ARGUMENT, "window_attention: NULL pointer");
+  if (a->dtype != EQT_F32 && a->dtype != EQT_BF16) return fail(EQT_ERR_BAD_ARGUMENT, "window_attention: unknown dtype %d", a->dtype);
+  if (a->n < 0 || a->num_graphs < 0 || a->num_tiles < 0 || a->before < 0 || a->after < 0 || a->sinks < 0 || a->heads < 1 || a->kv_heads < 1 || a->comps < 1 ||
+      a->head_channels < 1 || a->heads % a->kv_heads || (a->tile_rows != 16 && a->tile_rows != 32 && a->tile_rows != 64))
+    return fail(EQT_ERR_BAD_ARGUMENT, "window_attention: sizes");
+  if (a->n >= 1 << 30 || (int64_t)a->comps * a->head_channels > 128 || a->heads > 65535)
+    return fail(EQT_ERR_UNSUPPORTED, "window_attention: fewer than 2^30 nodes, 128 values a head and 65535 heads");
+  return EQT_OK;
+}
+
+// What all kernels take.  Windows reach no further than the longest chain, so a place and a reach, both below 2^30, add up in 32 bits.
+WindowParams params(const eqt_window_attention_args& a, float* delta) {
+  WindowParams p{};
+  const int64_t reach = std::min<int64_t>(std::max<int64_t>(a.longest, 1), a.n);
+  p.before = (int)std::min(a.before, reach), p.after = (int)std::min(a.after, reach), p.sinks = (int)std::min(a.sinks, reach);
+  p.group = a.heads / a.kv_heads;
+  AttentionParams& q = p.q;
+  const int64_t width = (int64_t)a.heads * a.head_channels;
+  q.q = {a.q, a.q_node, a.q_comp}, q.k = {a.k, a.k_node, a.k_comp}, q.v = {a.v, a.v_node, a.v_comp}, q.g = {a.grad, a.comps * width, width};
+  q.out = a.out, q.dq = a.dq, q.dk = a.dk, q.dv = a.dv, q.top = a.stats, q.inverse = a.stats ? a.stats + a.heads * a.n : nullptr, q.delta = delta;
+  q.tiles = reinterpret_cast<const int4*>(a.tiles), q.n = a.n, q.heads = a.heads, q.comps = a.comps, q.size = a.head_channels, q.scale = a.scale;
+  const int v = a.dtype == EQT_F32 ? 4 : 8;
+  const int64_t strides = a.q_node | a.q_comp | a.k_node | a.k_comp | a.v_node | a.v_comp;
+  uintptr_t bits = 0;
+  for (const void* x : {a.q, a.k, a.v, a.grad, (const void*)a.out, (const void*)a.dq, (const void*)a.dk, (const void*)a.dv}) bits |= reinterpret_cast<uintptr_t>(x);
+  q.vec = bits % 16 == 0 && strides % v == 0 && a.head_channels % v == 0;
+  p.kv = q;
+  p.kv.heads = a.kv_heads;
+  return p;
+}
+
+int64_t delta_bytes(const eqt_window_attention_args& a) { return (int64_t)up((size_t)a.heads * a.n * 4); }
+
+}  // namespace
+}  // namespace window
+}  // namespace eqt
+
 using namespace eqt;
-extern "C" int64_t eqt_window_attention_scratch(const eqt_window_attention_args*, int32_t) { return 0; }
-extern "C" int32_t eqt_window_attention_form(const eqt_window_attention_args*) { return 0; }
-extern "C" int eqt_window_attention_forward(const eqt_window_attention_args*, void*) { return fail(EQT_ERR_UNSUPPORTED, "window attention: no kernel yet"); }
-extern "C" int eqt_window_attention_backward(const eqt_window_attention_args*, void*) { return fail(EQT_ERR_UNSUPPORTED, "window attention: no kernel yet"); }
+using namespace eqt::window;
+
+extern "C" int64_t eqt_window_attention_scratch(const eqt_window_attention_args* a, int32_t backward) {
+  if (check(a)) return 0;
+  return backward ? delta_bytes(*a) : 0;
+}
+
+extern "C" int32_t eqt_window_attention_form(const eqt_window_attention_args* a) {
+  if (check(a)) return -1;
+  return 0;
+}
+
+extern "C" int eqt_window_attention_forward(const eqt_window_attention_args* args, void* stream) {
+  if (int rc = check(args)) return rc;
+  const eqt_window_attention_args& a = *args;
+  if (a.n == 0 || a.num_tiles == 0) return EQT_OK;
+  if (!a.q || !a.k || !a.v || !a.out || !a.tiles) return fail(EQT_ERR_BAD_ARGUMENT, "window_attention: NULL pointer");
+  const WindowParams p = params(a, nullptr);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return a.dtype == EQT_F32 ? tiles_forward_f32(p, a.tile_rows, a.num_tiles, s) : tiles_forward_bf16(p, a.tile_rows, a.num_tiles, s);
+}
+
+extern "C" int eqt_window_attention_backward(const eqt_window_attention_args* args, void* stream) {
+  if (int rc = check(args)) return rc;
+  const eqt_window_attention_args& a = *args;
+  if (a.n == 0 || a.num_tiles == 0) return EQT_OK;
+  if (!a.q || !a.k || !a.v || !a.grad || !a.out || !a.stats || !a.dq || !a.dk || !a.dv || !a.tiles) return fail(EQT_ERR_BAD_ARGUMENT, "window_attention backward: NULL pointer");
+  if (!a.scratch || a.scratch_bytes < delta_bytes(a))
+    return fail(EQT_ERR_BAD_ARGUMENT, "window_attention backward: %lld bytes of scratch given, %lld needed", (long long)a.scratch_bytes, (long long)delta_bytes(a));
+  const WindowParams p = params(a, static_cast<float*>(a.scratch));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return a.dtype == EQT_F32 ? tiles_backward_f32(p, a.tile_rows, a.num_tiles, s) : tiles_backward_bf16(p, a.tile_rows, a.num_tiles, s);
+}

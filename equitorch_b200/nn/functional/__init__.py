@@ -18,6 +18,6 @@ from .sphericals import spherical_harmonics
 from .tensor_products import tensor_dot_uu, tensor_dot_uv, tensor_product_uuu, tensor_product_uvw
 from .type_loss import type_cross_entropy
 from .wigner_d import dense_wigner_rotation, sparse_wigner_rotation, wigner_d_matrix
-from .window import window_attention_step
+from .window import window_attention, window_attention_step
 
 __all__ = [n for n in dir() if not n.startswith("_")]
