@@ -87,7 +87,7 @@ template <typename T> __device__ __noinline__ void again_rows(const WindowParams
   }
   lane_put<T>(p.q.dq, dq, p.q.scale, i, head, p.q, lane);
 }
-template <typename T> __device__ __noinline__ void again_columns(const WindowParams& p, int j, int kv, int lo, int hi, int lane) {
+template <typename T> __device__ __noinline__ void again_columns(const WindowParams& p, int j, int kv, int lo, int hi, int lane, bool put_dv = true, bool put_dk = true) {
   float q[4], k[4], v[4], g[4], dk[4] = {0.f, 0.f, 0.f, 0.f}, dv[4] = {0.f, 0.f, 0.f, 0.f};
   lane_row<T>(k, p.q.k, j, kv, p.q, lane);
   lane_row<T>(v, p.q.v, j, kv, p.q, lane);
@@ -104,8 +104,8 @@ template <typename T> __device__ __noinline__ void again_columns(const WindowPar
         dk[c] = fmaf(ds, q[c], dk[c]);
       }
     }
-  lane_put<T>(p.kv.dk, dk, p.q.scale, j, kv, p.kv, lane);
-  lane_put<T>(p.kv.dv, dv, 1.f, j, kv, p.kv, lane);
+  if (put_dk) lane_put<T>(p.kv.dk, dk, p.q.scale, j, kv, p.kv, lane);
+  if (put_dv) lane_put<T>(p.kv.dv, dv, 1.f, j, kv, p.kv, lane);
 }
 
 __device__ __forceinline__ bool is_finite(float x) { return fabsf(x) < INFINITY; }

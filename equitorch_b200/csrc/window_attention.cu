@@ -1,7 +1,7 @@
 // Attention within windows of packed chains: the C entry points.
 #include <algorithm>
 
-#include "window.cuh"
+#include "window_tc.cuh"
 
 namespace eqt {
 namespace window {
@@ -41,7 +41,32 @@ WindowParams params(const eqt_window_attention_args& a, float* delta) {
   return p;
 }
 
-int64_t delta_bytes(const eqt_window_attention_args& a) { return (int64_t)up((size_t)a.heads * a.n * 4); }
+// Tiles of 128 nodes on the tensor cores: bfloat16 whose pieces lie on 16-byte boundaries, and a positive scale, by which the greatest product is the greatest
+// score.
+bool on_tensor_cores(const eqt_window_attention_args& a) {
+  if (a.dtype != EQT_BF16 || !(a.scale > 0.f)) return false;
+  const int64_t strides = a.q_node | a.q_comp | a.k_node | a.k_comp | a.v_node | a.v_comp;
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) | reinterpret_cast<uintptr_t>(a.out) |
+                         reinterpret_cast<uintptr_t>(a.grad) | reinterpret_cast<uintptr_t>(a.dq) | reinterpret_cast<uintptr_t>(a.dk) | reinterpret_cast<uintptr_t>(a.dv);
+  return bits % 16 == 0 && strides % 8 == 0 && a.head_channels % 8 == 0;
+}
+
+// Scratch: the nodes' chains, and for the backward pass the deltas.
+int64_t spans_bytes(const eqt_window_attention_args& a) { return a.dtype == EQT_BF16 ? (int64_t)up((size_t)a.n * sizeof(int2)) : 0; }
+int64_t scratch_bytes(const eqt_window_attention_args& a, bool backward) { return spans_bytes(a) + (backward ? (int64_t)up((size_t)a.heads * a.n * 4) : 0); }
+int check_scratch(const eqt_window_attention_args& a, bool backward) {
+  const int64_t need = scratch_bytes(a, backward);
+  if (need && (!a.scratch || a.scratch_bytes < need))
+    return fail(EQT_ERR_BAD_ARGUMENT, "window_attention: %lld bytes of scratch given, %lld needed", (long long)a.scratch_bytes, (long long)need);
+  return reinterpret_cast<uintptr_t>(a.scratch) % 16 ? fail(EQT_ERR_BAD_ARGUMENT, "window_attention: scratch must start on a 16-byte boundary") : EQT_OK;
+}
+int tensor_params(TcParams& t, const eqt_window_attention_args& a, const WindowParams& p, cudaStream_t s) {
+  if (!a.ptr || !a.status) return fail(EQT_ERR_BAD_ARGUMENT, "window_attention: NULL pointer");
+  t.w = p;
+  t.spans = static_cast<const int2*>(a.scratch);
+  t.status = a.status;
+  return spans(a.ptr, a.num_graphs, static_cast<int2*>(a.scratch), a.n, s);
+}
 
 }  // namespace
 }  // namespace window
@@ -52,12 +77,12 @@ using namespace eqt::window;
 
 extern "C" int64_t eqt_window_attention_scratch(const eqt_window_attention_args* a, int32_t backward) {
   if (check(a)) return 0;
-  return backward ? delta_bytes(*a) : 0;
+  return scratch_bytes(*a, backward != 0);
 }
 
 extern "C" int32_t eqt_window_attention_form(const eqt_window_attention_args* a) {
   if (check(a)) return -1;
-  return 0;
+  return on_tensor_cores(*a);
 }
 
 extern "C" int eqt_window_attention_forward(const eqt_window_attention_args* args, void* stream) {
@@ -65,8 +90,14 @@ extern "C" int eqt_window_attention_forward(const eqt_window_attention_args* arg
   const eqt_window_attention_args& a = *args;
   if (a.n == 0 || a.num_tiles == 0) return EQT_OK;
   if (!a.q || !a.k || !a.v || !a.out || !a.tiles) return fail(EQT_ERR_BAD_ARGUMENT, "window_attention: NULL pointer");
+  if (int rc = check_scratch(a, false)) return rc;
   const WindowParams p = params(a, nullptr);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (on_tensor_cores(a)) {
+    TcParams t;
+    if (int rc = tensor_params(t, a, p, s)) return rc;
+    return tc_forward(t, s);
+  }
   return a.dtype == EQT_F32 ? tiles_forward_f32(p, a.tile_rows, a.num_tiles, s) : tiles_forward_bf16(p, a.tile_rows, a.num_tiles, s);
 }
 
@@ -75,9 +106,13 @@ extern "C" int eqt_window_attention_backward(const eqt_window_attention_args* ar
   const eqt_window_attention_args& a = *args;
   if (a.n == 0 || a.num_tiles == 0) return EQT_OK;
   if (!a.q || !a.k || !a.v || !a.grad || !a.out || !a.stats || !a.dq || !a.dk || !a.dv || !a.tiles) return fail(EQT_ERR_BAD_ARGUMENT, "window_attention backward: NULL pointer");
-  if (!a.scratch || a.scratch_bytes < delta_bytes(a))
-    return fail(EQT_ERR_BAD_ARGUMENT, "window_attention backward: %lld bytes of scratch given, %lld needed", (long long)a.scratch_bytes, (long long)delta_bytes(a));
-  const WindowParams p = params(a, static_cast<float*>(a.scratch));
+  if (int rc = check_scratch(a, true)) return rc;
+  const WindowParams p = params(a, reinterpret_cast<float*>(static_cast<unsigned char*>(a.scratch) + spans_bytes(a)));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (on_tensor_cores(a)) {
+    TcParams t;
+    if (int rc = tensor_params(t, a, p, s)) return rc;
+    return tc_backward(t, s);
+  }
   return a.dtype == EQT_F32 ? tiles_backward_f32(p, a.tile_rows, a.num_tiles, s) : tiles_backward_bf16(p, a.tile_rows, a.num_tiles, s);
 }

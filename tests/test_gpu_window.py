@@ -5,11 +5,19 @@ import torch
 from equitorch_b200.graph import PackedGraphs
 from equitorch_b200.nn import functional as F
 
+from equitorch_b200.ops.fused_tp_op import check_status
+
 from .window_reference import reference, seen
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
 TYPES = [torch.float32, torch.bfloat16]
+
+
+@pytest.fixture(autouse=True)
+def no_wait_gave_up():
+    yield
+    check_status()
 
 
 def make(sizes, comps, heads, kv_heads, size, dtype, seed=0, extra=0, spread=1.0):
@@ -92,6 +100,16 @@ def test_nodes_of_no_chain(dtype):
     compare(got, want, bound)
     for t in got:
         assert not t[:5].any() and not t[85:].any()
+
+
+@pytest.mark.parametrize("size", [64, 128])
+def test_many_tiles_at_once(size):
+    """Far more tiles than SMs, again and again, so that waits of every length occur: the same bits each time."""
+    sizes = [50 + 450 * i // 119 for i in range(120)]
+    qkv, g, graphs = make(sizes, 1, 8, 2, size, torch.bfloat16)
+    first = run(qkv, g, graphs, 8, 64, 64, 4, kv_heads=2)
+    for _ in range(30):
+        assert all(torch.equal(a, b) for a, b in zip(first, run(qkv, g, graphs, 8, 64, 64, 4, kv_heads=2)))
 
 
 def test_no_nodes():
