@@ -8,7 +8,7 @@
 //     8 bits: of every group of values, t = h w, m = max |t|:   value = e4m3(448 t / m), scale = m r / 448
 //
 // All of it is bound by HBM: 16 bytes a bfloat16 value and its residual forward and backward.  A row stays in the registers of 32, 128 or 512
-// threads, as few as hold it with four pieces of 16 bytes each: one reads x and the residual, adds, reduces by shuffles and writes.  A CTA
+// threads, one, two or four pieces of 16 bytes each: one reads x and the residual, adds, reduces by shuffles and writes.  A CTA
 // strides over the rows, so the weight is read once and the backward pass has the weight's gradient in registers, summed over the CTA's rows; the
 // CTAs' sums are added in their order by a second kernel (no atomics).  Rows that are no whole pieces of 16 bytes, or longer than 2048
 // pieces, are read twice by loops.
@@ -16,6 +16,7 @@
 #include <cuda_fp8.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -23,7 +24,6 @@ namespace eqt {
 namespace residual_norm {
 namespace {
 
-constexpr int PIECES = 4;                                // of 16 bytes a thread
 constexpr float E4M3_MAX = 448.f;
 
 struct NormArgs {
@@ -106,11 +106,13 @@ __device__ __noinline__ uint8_t to_e4m3_exact(double t, double m) {
 }
 constexpr float NEAR = 4.76837158203125e-7f;             // 2^-21
 constexpr float TINY = 1e-30f;                           // below it 448 / m may be infinite
+// m r / 448, whose last steps must not round to a number below the normal ones before the others have brought it up.
+__device__ __forceinline__ float scale_of(float most, float inverse) { return (float)((double)most * (double)inverse * (1.0 / (double)E4M3_MAX)); }
 __device__ __forceinline__ double exact_value(float x, float res, float w) { return ((double)x + (double)res) * (double)w; }
 
 // ---- rows in registers --------------------------------------------------------------------------
 // OUT: 0 values of the type, 1 8 bits with a scale a row, 2 with a scale every p.group values (whole pieces, a power of two of at most 32)
-template <typename T, int ROW_THREADS, int OUT, bool RES>
+template <typename T, int ROW_THREADS, int PIECES, int OUT, bool RES>
 __global__ void __launch_bounds__(ROW_THREADS < 128 ? 128 : ROW_THREADS) forward_kernel(const NormArgs p) {
   constexpr int V = VALUES<T>, ROWS = ROW_THREADS < 128 ? 128 / ROW_THREADS : 1;
   __shared__ float buffer[2][ROW_THREADS / 32], most_of[2][ROW_THREADS / 32];
@@ -169,62 +171,74 @@ __global__ void __launch_bounds__(ROW_THREADS < 128 ? 128 : ROW_THREADS) forward
         if (there && k < pieces) reinterpret_cast<uint4*>(p.y)[first + k] = pack<T>(y);
       }
     } else {
-      // the greatest |t| of a group: found in float32, and of the values within its error, in float64
       const int lanes = OUT == 2 ? p.group / V : 32;
-      float most[PIECES];
+      float most[PIECES], all = 0.f;
 #pragma unroll
       for (int i = 0; i < PIECES; ++i) {
         float c[V];
         unpack<T>(w[i], c);
         most[i] = 0.f;
 #pragma unroll
-        for (int j = 0; j < V; ++j) most[i] = Max()(most[i], fabsf(p.w ? h[i][j] * c[j] : h[i][j]));
+        for (int j = 0; j < V; ++j) {
+          if (p.w) h[i][j] *= c[j];
+          most[i] = Max()(most[i], fabsf(h[i][j]));
+        }
         if (OUT == 2) most[i] = across_lanes(most[i], lanes, Max());
-        else if (i) most[0] = Max()(most[0], most[i]);
+        else all = Max()(all, most[i]);
       }
-      if (OUT == 1) most[0] = across_row<ROW_THREADS>(most[0], most_of[turn], Max());
-      double exact[PIECES];
+      if (OUT == 1) all = across_row<ROW_THREADS>(all, most_of[turn], Max());
+      // both ends of what the quotient may be: one answer, or the long way round
+      uint16_t held[PIECES][V / 2];
+      bool unsure = false;
 #pragma unroll
       for (int i = 0; i < PIECES; ++i) {
-        float c[V], a[V], b[V];
-        unpack<T>(w[i], c);
-        unpack<T>(x[i], a);
-        if (RES) unpack<T>(r[i], b);
-        const float m = OUT == 1 ? most[0] : most[i];
-        exact[i] = 0.0;
+        if (OUT == 1) most[i] = all;
+        const float to = most[i] > 0.f ? __fdiv_rn(E4M3_MAX, most[i]) : 0.f, less = to * (1.f - NEAR), more = to * (1.f + NEAR);
+        unsure = unsure || (most[i] < TINY && most[i] > 0.f);
 #pragma unroll
-        for (int j = 0; j < V; ++j)
-          if (fabsf(p.w ? h[i][j] * c[j] : h[i][j]) >= m * (1.f - NEAR))
-            exact[i] = Max()(exact[i], fabs(exact_value(a[j], RES ? b[j] : 0.f, p.w ? c[j] : 1.f)));
-        if (OUT == 2) exact[i] = across_lanes(exact[i], lanes, Max());
-        else if (i) exact[0] = Max()(exact[0], exact[i]);
+        for (int j = 0; j < V; j += 2) {
+          held[i][j / 2] = to_e4m3(h[i][j] * less, h[i][j + 1] * less);
+          unsure = unsure || held[i][j / 2] != to_e4m3(h[i][j] * more, h[i][j + 1] * more);
+        }
       }
-      if (OUT == 1) exact[0] = across_row<ROW_THREADS>(exact[0], exact_of[turn], Max());
+      if (OUT == 1 ? __syncthreads_or(unsure) : __any_sync(0xffffffffu, unsure)) {
+        double exact[PIECES], whole = 0.0;
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+          float c[V], a[V], b[V];
+          unpack<T>(w[i], c);
+          unpack<T>(x[i], a);
+          if (RES) unpack<T>(r[i], b);
+          exact[i] = 0.0;
+#pragma unroll
+          for (int j = 0; j < V; ++j) exact[i] = Max()(exact[i], fabs(exact_value(a[j], RES ? b[j] : 0.f, p.w ? c[j] : 1.f)));
+          if (OUT == 2) exact[i] = across_lanes(exact[i], lanes, Max());
+          else whole = Max()(whole, exact[i]);
+        }
+        if (OUT == 1) whole = across_row<ROW_THREADS>(whole, exact_of[turn], Max());
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+          const double m = OUT == 1 ? whole : exact[i];
+          const float to = most[i] > 0.f ? __fdiv_rn(E4M3_MAX, most[i]) : 0.f, more = to * (1.f + NEAR);
+          float c[V], a[V], b[V];
+          unpack<T>(w[i], c);
+          unpack<T>(x[i], a);
+          if (RES) unpack<T>(r[i], b);
+#pragma unroll
+          for (int j = 0; j < V; j += 2)
+            if (held[i][j / 2] != to_e4m3(h[i][j] * more, h[i][j + 1] * more) || (most[i] < TINY && most[i] > 0.f))
+              held[i][j / 2] = (uint16_t)(to_e4m3_exact(exact_value(a[j], RES ? b[j] : 0.f, p.w ? c[j] : 1.f), m) |
+                                          to_e4m3_exact(exact_value(a[j + 1], RES ? b[j + 1] : 0.f, p.w ? c[j + 1] : 1.f), m) << 8);
+        }
+      }
 #pragma unroll
       for (int i = 0; i < PIECES; ++i) {
         const int k = at + i * ROW_THREADS;
         if (!there || k >= pieces) continue;
-        const float m = OUT == 1 ? most[0] : most[i], to = m > 0.f ? __fdiv_rn(E4M3_MAX, m) : 0.f;
-        const double em = OUT == 1 ? exact[0] : exact[i];
-        float c[V], a[V], b[V];
-        unpack<T>(w[i], c);
-        uint16_t held[V / 2];
-#pragma unroll
-        for (int j = 0; j < V; j += 2) {
-          const float q0 = (p.w ? h[i][j] * c[j] : h[i][j]) * to, q1 = (p.w ? h[i][j + 1] * c[j + 1] : h[i][j + 1]) * to;
-          const uint16_t low = to_e4m3(q0 * (1.f - NEAR), q1 * (1.f - NEAR)), high = to_e4m3(q0 * (1.f + NEAR), q1 * (1.f + NEAR));
-          held[j / 2] = low;
-          if (low != high || (m < TINY && m > 0.f)) {
-            unpack<T>(x[i], a);
-            if (RES) unpack<T>(r[i], b);
-            held[j / 2] = (uint16_t)(to_e4m3_exact(exact_value(a[j], RES ? b[j] : 0.f, p.w ? c[j] : 1.f), em) |
-                                     to_e4m3_exact(exact_value(a[j + 1], RES ? b[j + 1] : 0.f, p.w ? c[j + 1] : 1.f), em) << 8);
-          }
-        }
         uint8_t* to_values = p.values + (first + k) * V;
-        if constexpr (V == 8) *reinterpret_cast<uint2*>(to_values) = make_uint2(held[0] | (uint32_t)held[1] << 16, held[2] | (uint32_t)held[3] << 16);
-        else *reinterpret_cast<uint32_t*>(to_values) = held[0] | (uint32_t)held[1] << 16;
-        const float scale = (float)(em * (double)inverse / (double)E4M3_MAX);
+        if constexpr (V == 8) *reinterpret_cast<uint2*>(to_values) = make_uint2(held[i][0] | (uint32_t)held[i][1] << 16, held[i][2] | (uint32_t)held[i][3] << 16);
+        else *reinterpret_cast<uint32_t*>(to_values) = held[i][0] | (uint32_t)held[i][1] << 16;
+        const float scale = scale_of(most[i], inverse);
         if (OUT == 2 && k % lanes == 0) p.scales[(first + k) / lanes] = scale;
         if (OUT == 1 && k == 0) p.scales[row] = scale;
       }
@@ -233,7 +247,7 @@ __global__ void __launch_bounds__(ROW_THREADS < 128 ? 128 : ROW_THREADS) forward
 }
 
 // parts [CTA][values of a row]: the CTA's sums of g u
-template <typename T, int ROW_THREADS>
+template <typename T, int ROW_THREADS, int PIECES>
 __global__ void __launch_bounds__(ROW_THREADS < 128 ? 128 : ROW_THREADS) backward_kernel(const NormArgs p) {
   constexpr int V = VALUES<T>, ROWS = ROW_THREADS < 128 ? 128 / ROW_THREADS : 1;
   __shared__ float buffer[2][ROW_THREADS / 32];
@@ -376,7 +390,7 @@ template <typename T, bool EIGHT> __global__ void __launch_bounds__(LONG_THREADS
           p.values[first + k] = held;
           if (res && p.total) st(static_cast<T*>(p.total) + first + k, h);
         }
-        if (whole ? threadIdx.x == 0 : lane == 0) p.scales[row * (p.length / p.group) + start / p.group] = (float)(exact * (double)inverse / (double)E4M3_MAX);
+        if (whole ? threadIdx.x == 0 : lane == 0) p.scales[row * (p.length / p.group) + start / p.group] = scale_of(most, inverse);
       }
     }
   }
@@ -409,34 +423,52 @@ template <typename T> __global__ void __launch_bounds__(LONG_THREADS) weight_lon
   p.parts[(int64_t)blockIdx.x * p.length + k] = sum;
 }
 
-// dw[c] = the parts' sums over the components: a CTA has 32 channels, eight warps take parts in turn
-template <typename T> __global__ void __launch_bounds__(256) weight_sum_kernel(const NormArgs p, int parts) {
-  __shared__ float sums[8][32];
-  const int c = blockIdx.x * 32 + (threadIdx.x & 31), warp = threadIdx.x >> 5, comps = p.length / p.channels;
+// dw[c] = the parts' sums over the components: a CTA has eight channels, 64 slices of the parts each
+constexpr int SLICES = 64;
+template <typename T> __global__ void __launch_bounds__(8 * SLICES) weight_sum_kernel(const NormArgs p, int parts) {
+  __shared__ float sums[SLICES / 4][8];
+  const int c = blockIdx.x * 8 + (threadIdx.x & 7), comps = p.length / p.channels;
   float sum = 0.f;
   if (c < p.channels)
     for (int m = 0; m < comps; ++m) {
       const float* from = p.parts + m * p.channels + c;
 #pragma unroll 8
-      for (int q = warp; q < parts; q += 8) sum += from[(int64_t)q * p.length];
+      for (int q = threadIdx.x >> 3; q < parts; q += SLICES) sum += from[(int64_t)q * p.length];
     }
-  sums[warp][threadIdx.x & 31] = sum;
+  sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+  sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+  if ((threadIdx.x & 31) < 8) sums[threadIdx.x >> 5][threadIdx.x & 7] = sum;
   __syncthreads();
-  if (warp || c >= p.channels) return;
+  if (threadIdx.x >= 8 || c >= p.channels) return;
+  sum = 0.f;
 #pragma unroll
-  for (int i = 1; i < 8; ++i) sum += sums[i][threadIdx.x];
+  for (int i = 0; i < SLICES / 4; ++i) sum += sums[i][threadIdx.x];
   st(static_cast<T*>(p.dw) + c, sum);
 }
 
 // ---- host side ----------------------------------------------------------------------------------
 int size_of(int dtype) { return dtype == EQT_F32 ? 4 : 2; }
 
-// Threads of a row held in registers; 0 where it is read by loops.
-int row_threads(int dtype, int64_t length, int64_t channels, uintptr_t bits) {
+// Threads of a row held in registers, and pieces of 16 bytes a thread; 0 threads where it is read by loops.
+struct Rows { int threads, pieces; };
+Rows rows_of(int dtype, int64_t length, int64_t channels, uintptr_t bits) {
   const int v = 16 / size_of(dtype);
-  if (bits % 16 || length % v || channels % v) return 0;
+  if (bits % 16 || length % v || channels % v) return {0, 0};
   const int64_t pieces = length / v;
-  return pieces <= 32 * PIECES ? 32 : pieces <= 128 * PIECES ? 128 : pieces <= 512 * PIECES ? 512 : 0;
+  if (pieces <= 128) return {32, pieces <= 32 ? 1 : pieces <= 64 ? 2 : 4};
+  if (pieces <= 512) return {128, pieces <= 256 ? 2 : 4};
+  return pieces <= 2048 ? Rows{512, pieces <= 1024 ? 2 : 4} : Rows{0, 0};
+}
+// A call of `f` with the threads and pieces as constants.
+template <int N> using Constant = std::integral_constant<int, N>;
+template <typename F> void with_rows(Rows r, F f) {
+  if (r.threads == 32 && r.pieces == 1) f(Constant<32>(), Constant<1>());
+  else if (r.threads == 32 && r.pieces == 2) f(Constant<32>(), Constant<2>());
+  else if (r.threads == 32) f(Constant<32>(), Constant<4>());
+  else if (r.threads == 128 && r.pieces == 2) f(Constant<128>(), Constant<2>());
+  else if (r.threads == 128) f(Constant<128>(), Constant<4>());
+  else if (r.pieces == 2) f(Constant<512>(), Constant<2>());
+  else f(Constant<512>(), Constant<4>());
 }
 // CTAs of the backward pass, whose sums of the weight's gradient are added afterwards: two waves of what fits an SM.
 unsigned part_ctas(int threads, int64_t n) {
@@ -454,29 +486,27 @@ int check(int dtype, int64_t n, int64_t comps, int64_t channels) {
   return EQT_OK;
 }
 
-template <typename T, int THREADS, int OUT> int launch_rows(const NormArgs& p, cudaStream_t s) {
-  constexpr int ROWS = THREADS < 128 ? 128 / THREADS : 1;
-  const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(p.n, ROWS), (int64_t)sm_count() * (THREADS == 512 ? 4 : 16));
-  if (p.res) forward_kernel<T, THREADS, OUT, true><<<grid, THREADS < 128 ? 128 : THREADS, 0, s>>>(p);
-  else forward_kernel<T, THREADS, OUT, false><<<grid, THREADS < 128 ? 128 : THREADS, 0, s>>>(p);
-  return check_launch("add_rms_norm");
-}
-template <typename T, int OUT> int launch_forward(const NormArgs& p, int threads, cudaStream_t s) {
-  switch (threads) {
-    case 32: return launch_rows<T, 32, OUT>(p, s);
-    case 128: return launch_rows<T, 128, OUT>(p, s);
-    case 512: return launch_rows<T, 512, OUT>(p, s);
+template <typename T, int OUT> int launch_forward(const NormArgs& p, Rows r, cudaStream_t s) {
+  if (r.threads) {
+    const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(p.n, r.threads == 32 ? 4 : 1), (int64_t)sm_count() * (r.threads == 512 ? 4 : 16));
+    with_rows(r, [&](auto threads, auto pieces) {
+      constexpr int N = decltype(threads)::value, K = decltype(pieces)::value;
+      if (p.res) forward_kernel<T, N, K, OUT, true><<<grid, N < 128 ? 128 : N, 0, s>>>(p);
+      else forward_kernel<T, N, K, OUT, false><<<grid, N < 128 ? 128 : N, 0, s>>>(p);
+    });
+  } else {
+    forward_long_kernel<T, OUT != 0><<<(unsigned)std::min<int64_t>(p.n, (int64_t)sm_count() * 8), LONG_THREADS, 0, s>>>(p);
   }
-  forward_long_kernel<T, OUT != 0><<<(unsigned)std::min<int64_t>(p.n, (int64_t)sm_count() * 8), LONG_THREADS, 0, s>>>(p);
   return check_launch("add_rms_norm");
 }
-template <typename T> int launch_backward(const NormArgs& p, int threads, cudaStream_t s) {
+template <typename T> int launch_backward(const NormArgs& p, Rows r, cudaStream_t s) {
   int parts;
-  if (threads) {
-    parts = (int)part_ctas(threads, p.n);
-    if (threads == 32) backward_kernel<T, 32><<<parts, 128, 0, s>>>(p);
-    else if (threads == 128) backward_kernel<T, 128><<<parts, 128, 0, s>>>(p);
-    else backward_kernel<T, 512><<<parts, 512, 0, s>>>(p);
+  if (r.threads) {
+    parts = (int)part_ctas(r.threads, p.n);
+    with_rows(r, [&](auto threads, auto pieces) {
+      constexpr int N = decltype(threads)::value, K = decltype(pieces)::value;
+      backward_kernel<T, N, K><<<parts, N < 128 ? 128 : N, 0, s>>>(p);
+    });
     if (int rc = check_launch("add_rms_norm_backward")) return rc;
   } else {
     backward_long_kernel<T><<<(unsigned)std::min<int64_t>(p.n, (int64_t)sm_count() * 8), LONG_THREADS, 0, s>>>(p);
@@ -487,7 +517,7 @@ template <typename T> int launch_backward(const NormArgs& p, int threads, cudaSt
     if (int rc = check_launch("add_rms_norm_weight")) return rc;
   }
   if (!p.parts) return EQT_OK;
-  weight_sum_kernel<T><<<(unsigned)ceil_div(p.channels, 32), 256, 0, s>>>(p, parts);
+  weight_sum_kernel<T><<<(unsigned)ceil_div(p.channels, 8), 8 * SLICES, 0, s>>>(p, parts);
   return check_launch("add_rms_norm_weight_sum");
 }
 
@@ -512,9 +542,9 @@ extern "C" int eqt_add_rms_norm_forward(int32_t dtype, const void* x, const void
   NormArgs p{};
   p.x = x, p.res = residual, p.w = weight, p.y = out, p.total = total, p.rstd = rstd, p.n = n, p.eps = (float)eps;
   p.length = (int)(comps * channels), p.channels = (int)channels;
-  const int threads = row_threads(dtype, p.length, channels, bits_of({x, residual, weight, out, total}));
+  const Rows rows = rows_of(dtype, p.length, channels, bits_of({x, residual, weight, out, total}));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return dtype == EQT_F32 ? launch_forward<float, 0>(p, threads, s) : launch_forward<__nv_bfloat16, 0>(p, threads, s);
+  return dtype == EQT_F32 ? launch_forward<float, 0>(p, rows, s) : launch_forward<__nv_bfloat16, 0>(p, rows, s);
 }
 
 extern "C" int eqt_add_rms_norm_e4m3(int32_t dtype, const void* x, const void* residual, const void* weight, void* values, float* scales, void* total,
@@ -526,19 +556,19 @@ extern "C" int eqt_add_rms_norm_e4m3(int32_t dtype, const void* x, const void* r
   NormArgs p{};
   p.x = x, p.res = residual, p.w = weight, p.values = static_cast<uint8_t*>(values), p.scales = scales, p.total = total, p.n = n, p.eps = (float)eps;
   p.length = (int)(comps * channels), p.channels = (int)channels, p.group = (int)group;
-  int threads = row_threads(dtype, p.length, channels, bits_of({x, residual, weight, values, total}));
+  Rows rows = rows_of(dtype, p.length, channels, bits_of({x, residual, weight, values, total}));
   const int64_t lanes = group * size_of(dtype) / 16;
   const bool whole = group == p.length, pieces = group * size_of(dtype) % 16 == 0 && lanes <= 32 && (lanes & (lanes - 1)) == 0;
-  if (!whole && !pieces) threads = 0;
+  if (!whole && !pieces) rows = {0, 0};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (dtype == EQT_F32) return whole ? launch_forward<float, 1>(p, threads, s) : launch_forward<float, 2>(p, threads, s);
-  return whole ? launch_forward<__nv_bfloat16, 1>(p, threads, s) : launch_forward<__nv_bfloat16, 2>(p, threads, s);
+  if (dtype == EQT_F32) return whole ? launch_forward<float, 1>(p, rows, s) : launch_forward<float, 2>(p, rows, s);
+  return whole ? launch_forward<__nv_bfloat16, 1>(p, rows, s) : launch_forward<__nv_bfloat16, 2>(p, rows, s);
 }
 
 extern "C" int64_t eqt_add_rms_norm_scratch(int32_t dtype, int64_t n, int64_t comps, int64_t channels) {
   if (check(dtype, n, comps, channels)) return 0;
-  const int threads = row_threads(dtype, comps * channels, channels, 0);
-  return std::max<int64_t>(threads ? part_ctas(threads, n) : 0, long_parts(n)) * comps * channels;
+  const Rows rows = rows_of(dtype, comps * channels, channels, 0);
+  return std::max<int64_t>(rows.threads ? part_ctas(rows.threads, n) : 0, long_parts(n)) * comps * channels;
 }
 
 extern "C" int eqt_add_rms_norm_backward(int32_t dtype, const void* grad, const void* grad_total, const void* total, const void* weight, const float* rstd,
@@ -557,6 +587,6 @@ extern "C" int eqt_add_rms_norm_backward(int32_t dtype, const void* grad, const 
   NormArgs p{};
   p.g = grad, p.gh = grad_total, p.total = const_cast<void*>(total), p.w = weight, p.rstd = const_cast<float*>(rstd), p.dx = dx, p.dw = dweight;
   p.parts = dweight ? scratch : nullptr, p.n = n, p.length = (int)(comps * channels), p.channels = (int)channels;
-  const int threads = row_threads(dtype, p.length, channels, bits_of({grad, grad_total, total, weight, dx}));
-  return dtype == EQT_F32 ? launch_backward<float>(p, threads, s) : launch_backward<__nv_bfloat16>(p, threads, s);
+  const Rows rows = rows_of(dtype, p.length, channels, bits_of({grad, grad_total, total, weight, dx}));
+  return dtype == EQT_F32 ? launch_backward<float>(p, rows, s) : launch_backward<__nv_bfloat16>(p, rows, s);
 }

@@ -5,10 +5,10 @@
 // of the first 2 `half` channels of a head, pairs (j, j + half) or (2 j, 2 j + 1); the other channels are passed on.  All components of a
 // node's features turn alike, so that rotations of space and these commute.  The gradient is the same with -t.
 //
-// Bound by HBM: every value is read and written once.  A CTA takes 32 nodes at a time: their angles go to shared memory as (cos, sin), each
-// computed once for all heads and components of q and k, in float64 up to what is left of whole turns (the product of a position of a
-// million and a frequency has no place in float32: half an ulp of it is 0.03 of a radian).  Then a thread takes the same piece of a head for
-// node after node: two times 16 bytes of both halves, or 16 bytes of neighbouring pairs; single values where these do not lie on 16-byte boundaries.
+// Bound by HBM: every value is read and written once.  A CTA's angles go to shared memory as (cos, sin), each computed once for all heads and
+// components of q and k, in float64 up to what is left of whole turns (the product of a position of a million and a frequency has no
+// place in float32: half an ulp of it is 0.03 of a radian).  A thread has the same piece of a head of four nodes in registers, on their way while the angles
+// are made: two times 16 bytes of both halves, or 16 bytes of neighbouring pairs; single values where these do not lie on 16-byte boundaries.
 #include <algorithm>
 
 #include "common.cuh"
@@ -17,7 +17,7 @@ namespace eqt {
 namespace rotary {
 namespace {
 
-constexpr int NODES = 32, THREADS = 256;
+constexpr int THREADS = 128, AT_ONCE = 4;                // AT_ONCE: nodes whose pieces a thread has in registers
 
 struct Rows {                                            // q or k
   const void* in;
@@ -35,114 +35,151 @@ struct RotaryArgs {
   double turns;                                          // one over a whole turn, negative for the gradient
 };
 
-template <typename T> __device__ __forceinline__ float get(const T* p) { return static_cast<float>(*p); }
-
-// V values of a head at `from`: pairs of places (first, second) and the angles' places
-template <typename T, int V, bool INTERLEAVED>
-__device__ __forceinline__ void turn_piece(const T* from, T* to, const float2* angles, int unit, int half, float magnitude) {
+// A piece as it lies in memory: 16 bytes, or one value, of each of the two places that turn together (interleaved: of the one place).
+template <typename T, int V> struct Raw { using type = uint4; };
+template <typename T> struct Raw<T, 1> { using type = T; };
+template <typename T, int V> __device__ __forceinline__ void open(const typename Raw<T, V>::type& raw, float (&v)[V]) {
   if constexpr (V == 1) {
-    const int pairs = half;
-    if (unit < pairs) {
-      const int i = INTERLEAVED ? 2 * unit : unit, j = INTERLEAVED ? 2 * unit + 1 : unit + half;
-      const float a = get(from + i) * magnitude, b = get(from + j) * magnitude;
-      const float2 t = angles[unit];
-      st(to + i, a * t.x - b * t.y);
-      st(to + j, a * t.y + b * t.x);
-    } else {
-      to[half + unit] = from[half + unit];
-    }
+    v[0] = static_cast<float>(raw);
   } else {
-    constexpr int W = 4;                                 // words of 16 bytes
-    auto words = [](const T* p, float (&v)[V]) {
-      const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
-      const uint32_t r[W] = {u.x, u.y, u.z, u.w};
+    const uint32_t r[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
-      for (int i = 0; i < W; ++i) {
-        if constexpr (V == 4) v[i] = __uint_as_float(r[i]);
-        else v[2 * i] = __uint_as_float(r[i] << 16), v[2 * i + 1] = __uint_as_float(r[i] & 0xffff0000u);
-      }
-    };
-    auto put = [](T* p, const float (&v)[V]) {
-      uint32_t r[W];
-#pragma unroll
-      for (int i = 0; i < W; ++i) {
-        if constexpr (V == 4) r[i] = __float_as_uint(v[i]);
-        else {
-          const __nv_bfloat162 two = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-          r[i] = *reinterpret_cast<const uint32_t*>(&two);
-        }
-      }
-      *reinterpret_cast<uint4*>(p) = make_uint4(r[0], r[1], r[2], r[3]);
-    };
-    const int turned = INTERLEAVED ? 2 * half / V : half / V;
-    if (unit >= turned) {
-      const int at = (INTERLEAVED ? unit : unit + turned) * V;
-      *reinterpret_cast<uint4*>(to + at) = __ldg(reinterpret_cast<const uint4*>(from + at));
-      return;
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (V == 4) v[i] = __uint_as_float(r[i]);
+      else v[2 * i] = __uint_as_float(r[i] << 16), v[2 * i + 1] = __uint_as_float(r[i] & 0xffff0000u);
     }
-    float a[V];
-    words(from + unit * V, a);
-    if constexpr (INTERLEAVED) {
+  }
+}
+template <typename T, int V> __device__ __forceinline__ void put(T* to, const float (&v)[V]) {
+  if constexpr (V == 1) {
+    st(to, v[0]);
+  } else {
+    uint32_t r[4];
 #pragma unroll
-      for (int i = 0; i < V; i += 2) {
-        const float2 t = angles[(unit * V + i) / 2];
-        const float x = a[i] * magnitude, y = a[i + 1] * magnitude;
-        a[i] = x * t.x - y * t.y;
-        a[i + 1] = x * t.y + y * t.x;
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (V == 4) r[i] = __float_as_uint(v[i]);
+      else {
+        const __nv_bfloat162 two = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+        r[i] = *reinterpret_cast<const uint32_t*>(&two);
       }
-    } else {
-      float b[V];
-      words(from + half + unit * V, b);
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float2 t = angles[unit * V + i];
-        const float x = a[i] * magnitude, y = b[i] * magnitude;
-        a[i] = x * t.x - y * t.y;
-        b[i] = x * t.y + y * t.x;
-      }
-      put(to + half + unit * V, b);
     }
-    put(to + unit * V, a);
+    *reinterpret_cast<uint4*>(to) = make_uint4(r[0], r[1], r[2], r[3]);
   }
 }
 
-template <typename T, int V, bool INTERLEAVED> __global__ void __launch_bounds__(THREADS) rotary_kernel(const RotaryArgs p) {
+// The same roundings wherever it is called, so that results do not go by alignment.
+__device__ __forceinline__ void turn(float a, float b, float2 t, float& x, float& y) {
+  x = fmaf(a, t.x, -__fmul_rn(b, t.y));
+  y = fmaf(a, t.y, __fmul_rn(b, t.x));
+}
+
+// Where a thread's piece of a head is.
+template <typename T, int V, bool INTERLEAVED> struct Place {
+  const T* from;
+  T* to;
+  int64_t in_step, out_step;                             // between nodes
+  int first, second, pair;                               // channels of the two places (of the one: `second` < 0), their first pair; none turns: `pair` < 0
+  __device__ __forceinline__ Place(const RotaryArgs& p, int piece, int a_side, int64_t node) {
+    const bool other = piece >= a_side;
+    const Rows& rows = p.side[other];
+    if (other) piece -= a_side;
+    const int unit = piece % p.units, head = piece / p.units % rows.heads, comp = piece / p.units / rows.heads;
+    in_step = rows.node;
+    out_step = rows.out_node;
+    from = static_cast<const T*>(rows.in) + node * in_step + comp * rows.comp + (int64_t)head * p.size;
+    to = static_cast<T*>(rows.out) + node * out_step + comp * rows.out_comp + (int64_t)head * p.size;
+    if constexpr (V == 1) {                              // a pair, or one channel behind the pairs
+      const bool turns = unit < p.half;
+      pair = turns ? unit : -1;
+      first = !turns ? p.half + unit : INTERLEAVED ? 2 * unit : unit;
+      second = !turns ? -1 : INTERLEAVED ? 2 * unit + 1 : unit + p.half;
+    } else if constexpr (INTERLEAVED) {
+      first = unit * V;
+      second = -1;
+      pair = first < 2 * p.half ? first / 2 : -1;
+    } else {
+      const bool turns = unit * V < p.half;
+      pair = turns ? unit * V : -1;
+      first = turns ? unit * V : unit * V + p.half;
+      second = turns ? unit * V + p.half : -1;
+    }
+  }
+};
+
+template <typename T, int V, bool INTERLEAVED> __global__ void __launch_bounds__(THREADS) rotary_kernel(const RotaryArgs p, int together) {
+  using R = typename Raw<T, V>::type;
+  using Q = Place<T, V, INTERLEAVED>;
   extern __shared__ float2 angles[];                     // [node][pair]
   const int a_side = p.comps * p.side[0].heads * p.units, per_node = a_side + (p.sides > 1 ? p.comps * p.side[1].heads * p.units : 0);
-  const int together = max(1, THREADS / per_node);       // nodes that the CTA's threads take at a time
-  for (int64_t first = (int64_t)blockIdx.x * NODES; first < p.n; first += (int64_t)gridDim.x * NODES) {
-    const int here = (int)min((int64_t)NODES, p.n - first);
-    __syncthreads();
-    for (int i = threadIdx.x; i < here * p.half; i += THREADS) {
-      const int node = i / p.half, pair = i - node * p.half;
-      double t = (double)p.positions[first + node] * (p.frequencies[pair] * p.turns);
-      t -= rint(t);
-      float s, c;
-      sincospif(2.f * (float)t, &s, &c);
-      angles[i] = make_float2(c, s);
-    }
-    __syncthreads();
-    for (int at = threadIdx.x; at < together * per_node; at += THREADS) {
-      const int sub = at / per_node;
-      int piece = at - sub * per_node;
-      const bool second = piece >= a_side;
-      const Rows& rows = p.side[second];
-      if (second) piece -= a_side;
-      const int unit = piece % p.units, head = piece / p.units % rows.heads, comp = piece / p.units / rows.heads;
-      const T* from = static_cast<const T*>(rows.in) + (first + sub) * rows.node + comp * rows.comp + (int64_t)head * p.size;
-      T* to = static_cast<T*>(rows.out) + (first + sub) * rows.out_node + comp * rows.out_comp + (int64_t)head * p.size;
-#pragma unroll 4
-      for (int node = sub; node < here; node += together, from += together * rows.node, to += together * rows.out_node)
-        turn_piece<T, V, INTERLEAVED>(from, to, angles + node * p.half, unit, p.half, p.magnitude);
+  const int nodes = together * AT_ONCE, pieces = together * per_node;
+  for (int64_t first = (int64_t)blockIdx.x * nodes; first < p.n; first += (int64_t)gridDim.x * nodes) {
+    const int here = (int)min((int64_t)nodes, p.n - first);
+    bool ready = false;                                  // the angles
+    // all threads take as many rounds: the first one's pieces are on their way while the angles are made
+    for (int at0 = 0; at0 < pieces; at0 += THREADS) {
+      const int at = at0 + threadIdx.x, sub = at / per_node;
+      const bool mine = at < pieces;
+      const Q place(p, mine ? at - sub * per_node : 0, a_side, first + (mine ? sub : 0));
+      R a[AT_ONCE], b[AT_ONCE];
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; ++i)
+        if (mine && sub + i * together < here) {
+          const T* from = place.from + (int64_t)i * together * place.in_step;
+          a[i] = *reinterpret_cast<const R*>(from + place.first);
+          if (place.second >= 0) b[i] = *reinterpret_cast<const R*>(from + place.second);
+        }
+      if (!ready) {
+        __syncthreads();
+        for (int i = threadIdx.x; i < here * p.half; i += THREADS) {
+          const int node = i / p.half, pair = i - node * p.half;
+          double t = (double)p.positions[first + node] * (p.frequencies[pair] * p.turns);
+          t -= rint(t);
+          float s, c;
+          sincospif(2.f * (float)t, &s, &c);
+          angles[i] = make_float2(c * p.magnitude, s * p.magnitude);
+        }
+        __syncthreads();
+        ready = true;
+      }
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; ++i)
+        if (mine && sub + i * together < here) {
+          T* to = place.to + (int64_t)i * together * place.out_step;
+          if (place.pair < 0) {
+            *reinterpret_cast<R*>(to + place.first) = a[i];
+            continue;
+          }
+          const float2* t = angles + (sub + i * together) * p.half + place.pair;
+          float x[V], y[V];
+          open<T, V>(a[i], x);
+          if constexpr (INTERLEAVED && V > 1) {
+#pragma unroll
+            for (int j = 0; j < V; j += 2) {
+              const float u = x[j], v = x[j + 1];
+              turn(u, v, t[j / 2], x[j], x[j + 1]);
+            }
+          } else {
+            open<T, V>(b[i], y);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+              const float u = x[j], v = y[j];
+              turn(u, v, t[j], x[j], y[j]);
+            }
+            put<T, V>(to + place.second, y);
+          }
+          put<T, V>(to + place.first, x);
+        }
     }
   }
 }
 
 template <typename T, int V> int launch(const RotaryArgs& p, bool interleaved, cudaStream_t s) {
-  const size_t shared = (size_t)NODES * p.half * sizeof(float2);
-  const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(p.n, NODES), (int64_t)sm_count() * 16);
-  if (interleaved) rotary_kernel<T, V, true><<<grid, THREADS, shared, s>>>(p);
-  else rotary_kernel<T, V, false><<<grid, THREADS, shared, s>>>(p);
+  int64_t heads = p.side[0].heads + (p.sides > 1 ? p.side[1].heads : 0);
+  const int together = (int)std::max<int64_t>(1, std::min<int64_t>(THREADS / (p.comps * heads * p.units), 8192 / (std::max(1, p.half) * AT_ONCE * sizeof(float2))));
+  const size_t shared = (size_t)together * AT_ONCE * p.half * sizeof(float2);
+  const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(p.n, together * AT_ONCE), (int64_t)sm_count() * 64);
+  if (interleaved) rotary_kernel<T, V, true><<<grid, THREADS, shared, s>>>(p, together);
+  else rotary_kernel<T, V, false><<<grid, THREADS, shared, s>>>(p, together);
   return check_launch("rotary");
 }
 template <typename T> int run(RotaryArgs& p, bool interleaved, cudaStream_t s) {

@@ -14,12 +14,12 @@
 // G of a piece is at most PIECE_BYTES, so scratch does not grow with the table; a piece has a whole number of waves of WEIGHT's tiles.  Sums that
 // would leave SMs idle are cut into parts, float32 partial results that one kernel adds in their order.  Floor: 8 n t c flops for both passes.
 //
-// A CTA per SM; warp 0 copies tiles (TMA), warp 1 issues the MMAs, the others (sixteen, eight for float32) are the epilogue.  A k-block is 64
+// A CTA per SM; warp 0 copies tiles (TMA), warp 1 issues the MMAs, the other eight are the epilogue.  A k-block is 64
 // values of k; operands lie along k or along the rows, as they are in memory.  bfloat16: tiles of 128 x 256, four stages of 48 KB, two sums of 256 columns in tensor memory.
 // float32: operands are split once into three bfloat16 parts (24 bits), six products of which leave 2^-26 of a term; a stage has all parts of
 // both operands, 96 KB for 128 x 128 results, and products with small parts have a sum of their own, so that the truncation of the tensor cores' adder counts once every
-// 16 terms.  A sum is taken out of the tensor cores every `fold` k-blocks: 8 for float32 (512 terms lose at most 4e-6), 256 for bfloat16 (16384 terms, 2e-4, a
-// tenth of the rounding of a result).
+// 16 terms.  A float32 sum is taken out of the tensor cores every `fold` k-blocks (512 terms lose at most 4e-6); bfloat16 sums are of at most MOST_TERMS, which
+// lose 2e-4, a tenth of the rounding of a result: longer ones are cut into parts.
 //
 // Rows whose target is negative may hold anything: their G is set, not multiplied, to zero, and the backward pass reads x from a copy in which they are zero.
 #include <algorithm>
@@ -32,18 +32,18 @@ namespace {
 using namespace tc;
 
 enum Mode { LOGITS, SCORES, INPUT, WEIGHT };
-constexpr int BK = 64, SHARE = 64;                       // k of a block; columns of a thread of the epilogue
+constexpr int BK = 64, EPI = 8;                          // k of a block; warps of the epilogue
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr int64_t PIECE_BYTES = int64_t(256) << 20;
+constexpr int64_t PIECE_BYTES = int64_t(256) << 20, MOST_TERMS = 16384;
 
 template <int PARTS> constexpr int cols() { return PARTS == 1 ? 256 : 128; }             // of a tile
-template <int PARTS> constexpr int epilogue_warps() { return PARTS == 1 ? 16 : 8; }
-template <int PARTS> constexpr int threads() { return 32 * (2 + epilogue_warps<PARTS>()); }
+template <int PARTS> constexpr int share() { return cols<PARTS>() / 2; }                 // of a tile's columns, that a thread of the epilogue has
+constexpr int THREADS = 32 * (2 + EPI);
 template <int PARTS> constexpr int a_bytes() { return PARTS * TILE_M * BK * 2; }
 template <int PARTS> constexpr int stage_bytes() { return a_bytes<PARTS>() + PARTS * cols<PARTS>() * BK * 2; }
 constexpr int PATCH = 2048;                              // a warp's: 32 rows of 64 bytes
-template <int PARTS> constexpr int stages() { return (232448 - 1024 - epilogue_warps<PARTS>() * PATCH - 1024) / stage_bytes<PARTS>(); }
-template <int PARTS> constexpr size_t shared_bytes() { return 1024 + (size_t)stages<PARTS>() * stage_bytes<PARTS>() + epilogue_warps<PARTS>() * PATCH; }
+template <int PARTS> constexpr int stages() { return (232448 - 1024 - EPI * PATCH - 1024) / stage_bytes<PARTS>(); }
+template <int PARTS> constexpr size_t shared_bytes() { return 1024 + (size_t)stages<PARTS>() * stage_bytes<PARTS>() + EPI * PATCH; }
 
 struct alignas(64) Launch {
   CUtensorMap a, b;
@@ -63,6 +63,8 @@ struct alignas(64) Launch {
   int reduction;
   int* status;
 };
+
+__host__ __device__ inline int shares_of(int width, int share) { return width > share ? 2 : 1; }
 
 struct Item {
   int64_t row;
@@ -125,9 +127,9 @@ template <typename T> __device__ __forceinline__ void store_block(unsigned char*
   }
 }
 
-template <int PARTS, int MODE> __global__ void __launch_bounds__(threads<PARTS>(), 1) loss_kernel(const __grid_constant__ Launch p) {
+template <int PARTS, int MODE> __global__ void __launch_bounds__(THREADS, 1) loss_kernel(const __grid_constant__ Launch p) {
   constexpr bool F32 = PARTS == 3, A_TURNED = MODE == WEIGHT, B_TURNED = MODE == INPUT || MODE == WEIGHT;
-  constexpr int STAGES = stages<PARTS>(), STAGE = stage_bytes<PARTS>(), COLS = cols<PARTS>(), EPI = epilogue_warps<PARTS>();
+  constexpr int STAGES = stages<PARTS>(), STAGE = stage_bytes<PARTS>(), COLS = cols<PARTS>();
   static_assert(STAGES >= 2, "two stages at least");
   extern __shared__ unsigned char smem_raw[];
   __shared__ uint64_t full[STAGES], empty[STAGES], acc_full[2], acc_empty[2];
@@ -237,11 +239,12 @@ template <int PARTS, int MODE> __global__ void __launch_bounds__(threads<PARTS>(
     }
   } else {
     // ---------------- epilogue ----------------
-    // Warps of the same quarter of the lanes have 64 columns of a tile each.
-    const int e = warp - 2, quarter = warp & 3, share = e >> 2;
+    // Warps of the same quarter of the lanes have half of a tile's columns each, 32 at a time.
+    constexpr int SHARE = share<PARTS>();
+    const int e = warp - 2, quarter = warp & 3, half = e >> 2;
     unsigned char* patch = ring + (size_t)STAGES * STAGE + (size_t)e * PATCH;
-    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(share * SHARE);
-    const bool mine = share * SHARE < p.width;           // a narrow tile: the share has no columns
+    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * SHARE);
+    const int mine = max(0, min(SHARE, p.width - half * SHARE));                         // columns of a narrow tile may be none
     int piece = 0;
     bool ok = true;
     for (unsigned i = blockIdx.x; i < p.items && ok && !*ab; i += gridDim.x) {
@@ -257,98 +260,125 @@ template <int PARTS, int MODE> __global__ void __launch_bounds__(threads<PARTS>(
         part = p.reduction == 0 ? p.grad[row] : p.reduction == 1 ? p.grad[0] : p.grad[0] / p.count[0];
         if (target >= p.types) part = NAN;
       }
+      // 32 columns from `col` on, of which `valid` exist
+      auto block = [&](float* v, int col, int valid) {
+        if constexpr (MODE == LOGITS) {
+          if (valid < 32) {
+#pragma unroll
+            for (int c = 0; c < 32; ++c) v[c] = c < valid ? v[c] : -INFINITY;
+          }
+          const int64_t at = target - col;
+          if (at >= 0 && at < min(valid, 32)) {
+            float z = 0.f;
+#pragma unroll
+            for (int c = 0; c < 32; ++c) z = c == (int)at ? v[c] : z;
+            p.target_logit[row] = z;
+          }
+          float most[4] = {top, -INFINITY, -INFINITY, -INFINITY}, add[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < 32; ++c) most[c & 3] = fmaxf(most[c & 3], v[c]);
+          const float now = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])), base = now == -INFINITY ? 0.f : now * LOG2E;
+#pragma unroll
+          for (int c = 0; c < 32; ++c) add[c & 3] += exp2_fast(fmaf(v[c], LOG2E, -base));
+          sum = sum * exp2_fast(fmaf(top, LOG2E, -base)) + ((add[0] + add[1]) + (add[2] + add[3]));
+          top = now;
+        } else if constexpr (MODE == SCORES) {
+          const float base = lse * LOG2E;
+#pragma unroll
+          for (int c = 0; c < 32; ++c) v[c] = part * (F32 ? exp2_fast((v[c] - lse) * LOG2E) : exp2_fast(fmaf(v[c], LOG2E, -base)));
+          if (__any_sync(0xffffffffu, target < 0)) {     // set, whatever the product
+#pragma unroll
+            for (int c = 0; c < 32; ++c) v[c] = target < 0 ? 0.f : v[c];
+          }
+          const int64_t at = target - p.a_first - col;
+          if (at >= 0 && at < min(valid, 32)) {
+#pragma unroll
+            for (int c = 0; c < 32; ++c) v[c] = c == (int)at ? v[c] - part : v[c];
+          }
+          __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.out) + row0 * p.out_pitch + col;
+#pragma unroll
+          for (int q = 0; q < PARTS; ++q) {
+            store_block<__nv_bfloat16>(patch, v, out + q * p.out_part, p.out_pitch, lines, valid, true, lane);
+            if constexpr (F32) {
+#pragma unroll
+              for (int c = 0; c < 32; ++c) v[c] -= __bfloat162float(__float2bfloat16_rn(v[c]));
+            }
+          }
+        } else {
+          if (MODE == INPUT && p.typed && target < 0) {
+#pragma unroll
+            for (int c = 0; c < 32; ++c) v[c] = 0.f;
+          }
+          if (F32 || !p.typed) {
+            float* out = static_cast<float*>(p.out) + (p.typed ? 0 : (p.slot + t.part) * p.out_part) + row0 * p.out_pitch + col;
+            store_block<float>(patch, v, out, p.out_pitch, lines, valid, p.whole, lane);
+            store_block<float>(patch, v + 16, out + 16, p.out_pitch, lines, valid - 16, p.whole, lane);
+          } else {
+            store_block<__nv_bfloat16>(patch, v, static_cast<__nv_bfloat16*>(p.out) + row0 * p.out_pitch + col, p.out_pitch, lines, valid, p.whole, lane);
+          }
+        }
+      };
       for (int tile = t.tile0; tile < t.tile1 && ok; ++tile) {
-        float v[SHARE];
-        for (int k0 = t.kb0; k0 < t.kb1; k0 += p.fold, ++piece) {
-          const int a = piece & 1;
-          if (!bar_wait(&acc_full[a], (uint32_t)((piece >> 1) & 1), ab)) { ok = false; break; }
-          tc_fence_after();
-          if (mine) {
+        const int col = tile * p.width + half * SHARE, valid = min(p.columns, (tile + 1) * p.width) - col;
+        auto release = [&](int a) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) bar_arrive(&acc_empty[a]);
+        };
+        if constexpr (F32) {                             // pieces of the sum, of two sums each, gather in registers
+          float v[SHARE];
+          for (int k0 = t.kb0; k0 < t.kb1; k0 += p.fold, ++piece) {
+            const int a = piece & 1;
+            if (!bar_wait(&acc_full[a], (uint32_t)((piece >> 1) & 1), ab)) { ok = false; break; }
+            tc_fence_after();
+            if (mine) {
 #pragma unroll
-            for (int h = 0; h < SHARE; h += 32) {
-              uint32_t r[32];
-              tmem_issue32(lanes + (uint32_t)(a * 256 + h), r);
-              tmem_arrived32(r);
+              for (int h = 0; h < SHARE; h += 32) {
+                uint32_t r[32];
+                tmem_issue32(lanes + (uint32_t)(a * 256 + h), r);
+                tmem_arrived32(r);
 #pragma unroll
-              for (int c = 0; c < 32; ++c) v[h + c] = k0 > t.kb0 ? v[h + c] + __uint_as_float(r[c]) : __uint_as_float(r[c]);
-              if constexpr (F32) {
+                for (int c = 0; c < 32; ++c) v[h + c] = k0 > t.kb0 ? v[h + c] + __uint_as_float(r[c]) : __uint_as_float(r[c]);
                 tmem_issue32(lanes + (uint32_t)(a * 256 + COLS + h), r);
                 tmem_arrived32(r);
 #pragma unroll
                 for (int c = 0; c < 32; ++c) v[h + c] += __uint_as_float(r[c]);
               }
             }
+            release(a);
           }
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) bar_arrive(&acc_empty[a]);
-        }
-        if (!ok) break;
-        if (!mine) continue;
-        const int col = tile * p.width + share * SHARE, valid = min(SHARE, min(p.columns, (tile + 1) * p.width) - col);
-        if constexpr (MODE == LOGITS) {
-          if (valid < SHARE) {
+          if (!ok) break;
+          if (mine) {
 #pragma unroll
-            for (int c = 0; c < SHARE; ++c) v[c] = c < valid ? v[c] : -INFINITY;
+            for (int h = 0; h < SHARE; h += 32) block(v + h, col + h, valid - h);
           }
-          const int64_t at = target - col;
-          if (at >= 0 && at < valid) {
-            float z = 0.f;
-#pragma unroll
-            for (int c = 0; c < SHARE; ++c) z = c == (int)at ? v[c] : z;
-            p.target_logit[row] = z;
-          }
-          float most[4] = {top, -INFINITY, -INFINITY, -INFINITY}, add[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int c = 0; c < SHARE; ++c) most[c & 3] = fmaxf(most[c & 3], v[c]);
-          const float now = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])), base = now == -INFINITY ? 0.f : now * LOG2E;
-#pragma unroll
-          for (int c = 0; c < SHARE; ++c) add[c & 3] += exp2_fast(fmaf(v[c], LOG2E, -base));
-          sum = sum * exp2_fast(fmaf(top, LOG2E, -base)) + ((add[0] + add[1]) + (add[2] + add[3]));
-          top = now;
-        } else if constexpr (MODE == SCORES) {
-          const int64_t at = target - p.a_first - col;
-          const bool counts = target >= 0;
-          const float base = lse * LOG2E;
-#pragma unroll
-          for (int c = 0; c < SHARE; ++c) {
-            float w = F32 ? exp2_fast((v[c] - lse) * LOG2E) : exp2_fast(fmaf(v[c], LOG2E, -base));
-            v[c] = counts ? part * w : 0.f;
-          }
-          if (at >= 0 && at < valid) {
-#pragma unroll
-            for (int c = 0; c < SHARE; ++c) v[c] = c == (int)at ? v[c] - part : v[c];
-          }
-          __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.out) + row0 * p.out_pitch + col;
-#pragma unroll
-          for (int q = 0; q < PARTS; ++q) {
+        } else {                                         // one sum; the next columns are on their way while these are worked on
+          const int a = piece & 1;
+          if (!bar_wait(&acc_full[a], (uint32_t)((piece >> 1) & 1), ab)) { ok = false; break; }
+          ++piece;
+          tc_fence_after();
+          uint32_t r[2][32];
+          if (mine) {
+            tmem_issue32(lanes + (uint32_t)(a * 256), r[0]);
 #pragma unroll
             for (int h = 0; h < SHARE; h += 32) {
-              store_block<__nv_bfloat16>(patch, v + h, out + q * p.out_part + h, p.out_pitch, lines, valid - h, true, lane);
-              if constexpr (F32) {
+              if (h >= mine) break;
+              uint32_t(&now)[32] = r[(h / 32) & 1];
+              tmem_arrived32(now);
+              if (h + 32 < mine) tmem_issue32(lanes + (uint32_t)(a * 256 + h + 32), r[(h / 32 + 1) & 1]);
+              else release(a);
+              float v[32];
 #pragma unroll
-                for (int c = 0; c < 32; ++c) v[h + c] -= __bfloat162float(__float2bfloat16_rn(v[h + c]));
-              }
+              for (int c = 0; c < 32; ++c) v[c] = __uint_as_float(now[c]);
+              block(v, col + h, valid - h);
             }
-          }
-        } else {
-          if (MODE == INPUT && p.typed && target < 0) {
-#pragma unroll
-            for (int c = 0; c < SHARE; ++c) v[c] = 0.f;
-          }
-          if (F32 || !p.typed) {
-            float* out = static_cast<float*>(p.out) + (p.typed ? 0 : (p.slot + t.part) * p.out_part) + row0 * p.out_pitch + col;
-#pragma unroll
-            for (int h = 0; h < SHARE; h += 16) store_block<float>(patch, v + h, out + h, p.out_pitch, lines, valid - h, p.whole, lane);
           } else {
-            __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.out) + row0 * p.out_pitch + col;
-#pragma unroll
-            for (int h = 0; h < SHARE; h += 32) store_block<__nv_bfloat16>(patch, v + h, out + h, p.out_pitch, lines, valid - h, p.whole, lane);
+            release(a);
           }
         }
       }
       if (MODE == LOGITS && ok && there && mine)
-        static_cast<float2*>(p.out)[(int64_t)(t.tile0 / p.run * (p.width / SHARE) + share) * p.rows + row] = make_float2(top, sum);
+        static_cast<float2*>(p.out)[(int64_t)(t.tile0 / p.run * shares_of(p.width, SHARE) + half) * p.rows + row] = make_float2(top, sum);
     }
   }
 
@@ -367,23 +397,44 @@ template <int PARTS, int MODE> __global__ void __launch_bounds__(threads<PARTS>(
 }
 
 // ---- before and after ---------------------------------------------------------------------------
-// A matrix (rows, cols) to rows of `pitch` bfloat16 values, in three parts of float32 ones; rows whose target is negative as zeros.
-template <typename T> __global__ void __launch_bounds__(256) prepare_kernel(const T* __restrict__ from, __nv_bfloat16* __restrict__ to, int64_t rows, int cols,
-                                                                            int pitch, const int64_t* __restrict__ target) {
-  const int64_t part = rows * pitch;
-  const int pieces = pitch / 8;
-  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < rows * pieces; i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t row = i / pieces;
+// Matrices (rows, cols) to rows of `pitch` bfloat16 values, in three parts of float32 ones; rows whose target is negative as zeros.  Two at once.
+struct Prepare {
+  const void* from;
+  __nv_bfloat16* to;
+  int64_t rows;
+  const int64_t* target;
+};
+template <typename T> __global__ void __launch_bounds__(256) prepare_kernel(const Prepare first, const Prepare second, int cols, int pitch) {
+  const Prepare& p = blockIdx.y ? second : first;
+  const int64_t part = p.rows * pitch;
+  const unsigned pieces = pitch / 8;
+  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < p.rows * pieces; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t row = i <= UINT32_MAX ? (unsigned)i / pieces : i / pieces;
     const int col = (int)(i - row * pieces) * 8;
-    const bool none = target && target[row] < 0;
+    const bool none = p.target && p.target[row] < 0;
+    const T* from = static_cast<const T*>(p.from) + row * cols + col;
     float v[8], w[8], u[8];
+    if (cols % 8 == 0) {
+      if constexpr (sizeof(T) == 4) {
+        const float4 a = reinterpret_cast<const float4*>(from)[0], b = reinterpret_cast<const float4*>(from)[1];
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+      } else {
+        const uint4 a = *reinterpret_cast<const uint4*>(from);
+        const uint32_t r[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[2 * j] = __uint_as_float(r[j] << 16), v[2 * j + 1] = __uint_as_float(r[j] & 0xffff0000u);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = col + j < cols ? ld(from + j) : 0.f;
+    }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      v[j] = !none && col + j < cols ? ld(from + row * cols + col + j) : 0.f;
+      if (none) v[j] = 0.f;
       if constexpr (sizeof(T) == 4) split3(v[j], v[j], w[j], u[j]);
     }
     auto put = [&](const float (&x)[8], int q) {
-      *reinterpret_cast<uint4*>(to + q * part + row * pitch + col) = make_uint4(two_bf16(x[0], x[1]), two_bf16(x[2], x[3]), two_bf16(x[4], x[5]), two_bf16(x[6], x[7]));
+      *reinterpret_cast<uint4*>(p.to + q * part + row * pitch + col) = make_uint4(two_bf16(x[0], x[1]), two_bf16(x[2], x[3]), two_bf16(x[4], x[5]), two_bf16(x[6], x[7]));
     };
     put(v, 0);
     if constexpr (sizeof(T) == 4) {
@@ -439,17 +490,38 @@ __global__ void __launch_bounds__(1024) reduce_kernel(const float* __restrict__ 
   if (result) result[0] = (float)(mean ? sum / (double)(c ? c : 1) : sum);
 }
 
-// Partial results [slots][rows][pitch] added in their order; rows of a negative target are zeros.
+// Partial results [slots][rows][pitch] added in their order, eight columns a thread; rows of a negative target are zeros.
 template <typename T> __global__ void __launch_bounds__(256) sum_kernel(const float* __restrict__ parts, T* __restrict__ out, int64_t rows, int cols, int pitch, int slots,
                                                                         const int64_t* __restrict__ target) {
   const int64_t part = rows * pitch;
-  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < rows * cols; i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t row = i / cols;
-    const float* from = parts + row * pitch + (i - row * cols);
-    float sum = 0.f;
-#pragma unroll 8
-    for (int s = 0; s < slots; ++s) sum += from[s * part];
-    st(out + i, target && target[row] < 0 ? 0.f : sum);
+  const unsigned pieces = pitch / 8;
+  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < rows * pieces; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t row = i <= UINT32_MAX ? (unsigned)i / pieces : i / pieces;
+    const int col = (int)(i - row * pieces) * 8;
+    const float4* from = reinterpret_cast<const float4*>(parts + row * pitch + col);
+    float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int s = 0; s < slots; ++s) {
+      const float4 a = from[s * (part / 4)], b = from[s * (part / 4) + 1];
+      sum[0] += a.x, sum[1] += a.y, sum[2] += a.z, sum[3] += a.w, sum[4] += b.x, sum[5] += b.y, sum[6] += b.z, sum[7] += b.w;
+    }
+    if (target && target[row] < 0) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sum[j] = 0.f;
+    }
+    T* to = out + row * cols + col;
+    if (cols % 8 == 0) {
+      if constexpr (sizeof(T) == 4) {
+        reinterpret_cast<float4*>(to)[0] = make_float4(sum[0], sum[1], sum[2], sum[3]);
+        reinterpret_cast<float4*>(to)[1] = make_float4(sum[4], sum[5], sum[6], sum[7]);
+      } else {
+        *reinterpret_cast<uint4*>(to) = make_uint4(two_bf16(sum[0], sum[1]), two_bf16(sum[2], sum[3]), two_bf16(sum[4], sum[5]), two_bf16(sum[6], sum[7]));
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (col + j < cols) st(to + j, sum[j]);
+    }
   }
 }
 
@@ -469,10 +541,10 @@ int width_of(int64_t columns, int most) {
   const int64_t tiles = ceil_div(columns, most);
   return (int)up_to(ceil_div(columns, tiles), 64);
 }
-// Parts of a sum of `blocks` k-blocks for `tiles` results: as many as fill the SMs, of at least eight blocks.
+// Parts of a sum of `blocks` k-blocks for `tiles` results: as many as fill the SMs, of at least eight blocks, and at most MOST_TERMS.
 void cut(int64_t blocks, int64_t tiles, int& parts, int& part_blocks) {
   const int64_t wanted = std::max<int64_t>(1, sm_count() / std::max<int64_t>(1, tiles));
-  part_blocks = (int)std::max<int64_t>(std::min<int64_t>(blocks, 8), ceil_div(blocks, wanted));
+  part_blocks = (int)std::min<int64_t>(MOST_TERMS / BK, std::max<int64_t>(std::min<int64_t>(blocks, 8), ceil_div(blocks, wanted)));
   parts = (int)ceil_div(blocks, part_blocks);
 }
 Plan plan_of(const eqt_type_loss_args& a, bool backward) {
@@ -492,7 +564,7 @@ Plan plan_of(const eqt_type_loss_args& a, bool backward) {
     p.run = (int)std::min<int64_t>(32, std::max<int64_t>(1, row_tiles * col_tiles / (sms * 8)));
     p.runs = (int)ceil_div(col_tiles, p.run);
     p.states = at;
-    p.logit = p.states + up((size_t)p.runs * (p.width_t / SHARE) * a.n * sizeof(float2));
+    p.logit = p.states + up((size_t)p.runs * shares_of(p.width_t, p.cols / 2) * a.n * sizeof(float2));
     p.bytes = p.logit + up((size_t)a.n * 4);
     return p;
   }
@@ -516,7 +588,7 @@ int check(const eqt_type_loss_args* a) {
   if (a->dtype != EQT_F32 && a->dtype != EQT_BF16) return fail(EQT_ERR_BAD_ARGUMENT, "type_loss: unknown dtype %d", a->dtype);
   if (a->reduction < 0 || a->reduction > 2) return fail(EQT_ERR_BAD_ARGUMENT, "type_loss: unknown reduction %d", a->reduction);
   if (a->n < 0 || a->c < 1 || a->t < 1) return fail(EQT_ERR_BAD_ARGUMENT, "type_loss: sizes");
-  if (a->n > INT32_MAX - 256 || a->t > INT32_MAX - 256 || a->c > 1 << 20) return fail(EQT_ERR_UNSUPPORTED, "type_loss: at most 2^31 rows and types and 2^20 channels");
+  if (a->n > INT32_MAX - 256 || a->t > INT32_MAX - 256 || a->c > MOST_TERMS) return fail(EQT_ERR_UNSUPPORTED, "type_loss: at most 2^31 rows and types and 16384 channels");
   if (ceil_div(a->n, TILE_M) * ceil_div(a->t, 64) > INT32_MAX / 2) return fail(EQT_ERR_UNSUPPORTED, "type_loss: rows times types are more than one launch takes");
   return EQT_OK;
 }
@@ -525,19 +597,13 @@ template <int PARTS, int MODE> int launch(const Launch& p, cudaStream_t s) {
   auto kernel = loss_kernel<PARTS, MODE>;
   static std::atomic<uint64_t> allowed{0};
   if (int rc = allow_shared_once(kernel, shared_bytes<PARTS>(), allowed)) return rc;
-  kernel<<<std::min<unsigned>(p.items, (unsigned)sm_count()), threads<PARTS>(), shared_bytes<PARTS>(), s>>>(p);
+  kernel<<<std::min<unsigned>(p.items, (unsigned)sm_count()), THREADS, shared_bytes<PARTS>(), s>>>(p);
   return check_launch("type_loss");
 }
 template <int MODE> int launch(int parts, const Launch& p, cudaStream_t s) { return parts == 1 ? launch<1, MODE>(p, s) : launch<3, MODE>(p, s); }
 
-int prepare(const eqt_type_loss_args& a, const Plan& p, const void* from, void* to, int64_t rows, const int64_t* target, cudaStream_t s) {
-  const unsigned grid = flat_grid(rows * (p.pitch / 8), 256);
-  if (a.dtype == EQT_F32) prepare_kernel<<<grid, 256, 0, s>>>(static_cast<const float*>(from), static_cast<__nv_bfloat16*>(to), rows, (int)a.c, p.pitch, target);
-  else prepare_kernel<<<grid, 256, 0, s>>>(static_cast<const __nv_bfloat16*>(from), static_cast<__nv_bfloat16*>(to), rows, (int)a.c, p.pitch, target);
-  return check_launch("type_loss_prepare");
-}
 int sum_parts(int dtype, const float* parts, void* out, int64_t rows, int cols, int pitch, int slots, const int64_t* target, cudaStream_t s) {
-  const unsigned grid = flat_grid(rows * cols, 256);
+  const unsigned grid = flat_grid(rows * (pitch / 8), 256);
   if (dtype == EQT_F32) sum_kernel<<<grid, 256, 0, s>>>(parts, static_cast<float*>(out), rows, cols, pitch, slots, target);
   else sum_kernel<<<grid, 256, 0, s>>>(parts, static_cast<__nv_bfloat16*>(out), rows, cols, pitch, slots, target);
   return check_launch("type_loss_sum");
@@ -547,15 +613,21 @@ int sum_parts(int dtype, const float* parts, void* out, int64_t rows, int cols, 
 int operands(const eqt_type_loss_args& a, const Plan& p, bool backward, const void*& x, const void*& w, cudaStream_t s) {
   unsigned char* base = static_cast<unsigned char*>(a.scratch);
   x = a.x, w = a.w;
+  Prepare jobs[2];
+  int count = 0;
   if (p.w) {
-    if (int rc = prepare(a, p, a.x, base + p.x, a.n, backward ? a.target : nullptr, s)) return rc;
+    jobs[count++] = {a.x, reinterpret_cast<__nv_bfloat16*>(base + p.x), a.n, backward ? a.target : nullptr};
     x = base + p.x;
   }
   if (p.parts > 1 || p.pitch != a.c) {
-    if (int rc = prepare(a, p, a.w, base + p.w, a.t, nullptr, s)) return rc;
+    jobs[count++] = {a.w, reinterpret_cast<__nv_bfloat16*>(base + p.w), a.t, nullptr};
     w = base + p.w;
   }
-  return EQT_OK;
+  if (!count) return EQT_OK;
+  const dim3 grid(flat_grid(std::max(jobs[0].rows, jobs[count - 1].rows) * (p.pitch / 8), 256), (unsigned)count);
+  if (a.dtype == EQT_F32) prepare_kernel<float><<<grid, 256, 0, s>>>(jobs[0], jobs[count - 1], (int)a.c, p.pitch);
+  else prepare_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(jobs[0], jobs[count - 1], (int)a.c, p.pitch);
+  return check_launch("type_loss_prepare");
 }
 
 int check_pointers(const eqt_type_loss_args& a, size_t need) {
@@ -567,7 +639,7 @@ int check_pointers(const eqt_type_loss_args& a, size_t need) {
   return EQT_OK;
 }
 
-constexpr int fold_of(int parts) { return parts == 3 ? 8 : 256; }
+constexpr int fold_of(int parts) { return parts == 3 ? 8 : (int)(MOST_TERMS / BK); }
 
 }  // namespace
 }  // namespace type_loss
@@ -600,7 +672,7 @@ extern "C" int eqt_type_loss_forward(const eqt_type_loss_args* args, void* strea
     l.run = p.run, l.kblocks = (int)ceil_div(a.c, BK), l.fold = fold_of(p.parts), l.items = (unsigned)(l.row_tiles * p.runs);
     l.out = base + p.states, l.target = a.target, l.types = a.t, l.target_logit = reinterpret_cast<float*>(base + p.logit), l.status = a.status;
     if (int rc = launch<LOGITS>(p.parts, l, s)) return rc;
-    rows_kernel<<<(unsigned)ceil_div(a.n, 32), 256, 0, s>>>(reinterpret_cast<const float2*>(base + p.states), p.runs * (p.width_t / SHARE), l.target_logit, a.target, a.n,
+    rows_kernel<<<(unsigned)ceil_div(a.n, 32), 256, 0, s>>>(reinterpret_cast<const float2*>(base + p.states), p.runs * shares_of(p.width_t, p.cols / 2), l.target_logit, a.target, a.n,
                                                             a.t, a.lse, a.losses);
     if (int rc = check_launch("type_loss_rows")) return rc;
   }

@@ -9,14 +9,14 @@
 // itself crosses threads on the way.  Teams, and then parts, are joined by their maxima at the end, in one order.
 #include <algorithm>
 
-#include "common.cuh"
+#include "graph_attention.cuh"
 
 namespace eqt {
 namespace window_step {
 namespace {
 
-constexpr int THREADS = 128, MOST_VALUES = 128;
-constexpr float LOG2E = 1.4426950408889634f;
+constexpr int THREADS = 128, MOST_VALUES = 128, AHEAD = 6;
+using attention::LOG2E;
 
 struct StepArgs {
   const void *q, *k, *v;
@@ -29,18 +29,17 @@ struct StepArgs {
   float scale;                                           // times log2 e
 };
 
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
+using attention::add2;
+using attention::both;
+using attention::exp2_fast;
+using attention::fma2;
+using attention::mul2;
+using attention::pair;
+using attention::parts;
 
 // V values from memory: 16 bytes, or one
-template <typename T, int V> __device__ __forceinline__ void load(const T* p, float (&v)[V]) {
-  if constexpr (V == 1) {
-    v[0] = static_cast<float>(*p);
-  } else {
-    const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
+template <int V> __device__ __forceinline__ void unpack(const uint4& u, float (&v)[V]) {
+  if constexpr (V > 1) {
     const uint32_t r[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -48,6 +47,10 @@ template <typename T, int V> __device__ __forceinline__ void load(const T* p, fl
       else v[2 * i] = __uint_as_float(r[i] << 16), v[2 * i + 1] = __uint_as_float(r[i] & 0xffff0000u);
     }
   }
+}
+template <typename T, int V> __device__ __forceinline__ void load(const T* p, float (&v)[V]) {
+  if constexpr (V == 1) v[0] = static_cast<float>(*p);
+  else unpack<V>(__ldg(reinterpret_cast<const uint4*>(p)), v);
 }
 
 // What a softmax over some keys leaves.  Without a key the maximum is minus infinity and the sums are zero.
@@ -65,7 +68,8 @@ template <int N> __device__ __forceinline__ void join(State<N>& a, float top, fl
 // TEAM threads a key, PIECES pieces of V values each; H heads at a time
 template <typename T, int V, int TEAM, int PIECES, int H> __global__ void __launch_bounds__(THREADS) step_kernel(const StepArgs p) {
   constexpr int N = V * PIECES, TEAMS = THREADS / TEAM;
-  __shared__ float tops[TEAMS][H], sums[TEAMS][H], values[TEAMS / (32 / TEAM)][H][TEAM * N];
+  __shared__ float tops[THREADS / 32][H], sums[THREADS / 32][H], values[THREADS / 32][H][TEAM * N];
+  __shared__ uint4 ring[V > 1 ? AHEAD : 1][2][V > 1 ? THREADS : 1];
   const int lane = threadIdx.x % TEAM, team = threadIdx.x / TEAM, warp = threadIdx.x >> 5;
   const int part = blockIdx.x, blocks = (p.group + H - 1) / H, kv = blockIdx.y / blocks, head0 = kv * p.group + blockIdx.y % blocks * H;
   const int here = min(H, (kv + 1) * p.group - head0);
@@ -93,39 +97,65 @@ template <typename T, int V, int TEAM, int PIECES, int H> __global__ void __laun
       for (int j = 0; j < V; ++j) q[h][i * V + j] = t[j] * p.scale;
     }
   }
-  State<N> state[H];
+  pair q2[H][N / 2], o2[H][N / 2];
+  float tops_[H], sums_[H];
 #pragma unroll
   for (int h = 0; h < H; ++h) {
-    state[h].top = -INFINITY;
-    state[h].sum = 0.f;
+    tops_[h] = -INFINITY;
+    sums_[h] = 0.f;
 #pragma unroll
-    for (int j = 0; j < N; ++j) state[h].o[j] = 0.f;
+    for (int c = 0; c < N / 2; ++c) {
+      q2[h][c] = both(q[h][2 * c], q[h][2 * c + 1]);
+      o2[h][c] = 0;
+    }
+  }
+  auto key_of = [&](int64_t i) { return i < sinks ? i : low + i - sinks; };
+  // Pieces of 16 bytes are on their way AHEAD rounds before they are used, each thread's to a place of its own, so that no thread waits for another.
+  auto ask = [&](int64_t round, int place) {
+    if constexpr (V > 1) {
+      if (round + team < end && on[0]) {
+        const int64_t j = key_of(round + team);
+        attention::copy16(&ring[place][0][threadIdx.x], static_cast<const T*>(p.k) + k_at[0] + j * p.k_node, true);
+        attention::copy16(&ring[place][1][threadIdx.x], static_cast<const T*>(p.v) + v_at[0] + j * p.v_node, true);
+      }
+      attention::copies_commit();
+    }
+  };
+  if constexpr (V > 1) {
+    if (!on[0])
+      for (int i = 0; i < AHEAD; ++i) ring[i][0][threadIdx.x] = ring[i][1][threadIdx.x] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < AHEAD - 1; ++i) ask(first + i * TEAMS, i);
   }
   // all threads of a warp take as many rounds, so that the shuffles find them; teams without a key add nothing
-#pragma unroll 2
+  int place = 0;
   for (int64_t round = first; round < end; round += TEAMS) {
     const int64_t i = round + team;
     const bool there = i < end;
-    const int64_t j = there ? (i < sinks ? i : low + i - sinks) : 0;
     float k[N], v[N];
+    if constexpr (V > 1) {
+      ask(round + (AHEAD - 1) * TEAMS, place == 0 ? AHEAD - 1 : place - 1);
+      attention::copies_wait<AHEAD - 1>();
+      unpack<V>(ring[place][0][threadIdx.x], k);
+      unpack<V>(ring[place][1][threadIdx.x], v);
+      if (++place == AHEAD) place = 0;
+    } else {
+      const int64_t j = there ? key_of(i) : 0;
 #pragma unroll
-    for (int m = 0; m < PIECES; ++m) {
-      float t[V], u[V];
-#pragma unroll
-      for (int c = 0; c < V; ++c) t[c] = u[c] = 0.f;
-      if (there && on[m]) {
-        load<T, V>(static_cast<const T*>(p.k) + k_at[m] + j * p.k_node, t);
-        load<T, V>(static_cast<const T*>(p.v) + v_at[m] + j * p.v_node, u);
+      for (int m = 0; m < PIECES; ++m) {
+        k[m] = there && on[m] ? static_cast<float>(static_cast<const T*>(p.k)[k_at[m] + j * p.k_node]) : 0.f;
+        v[m] = there && on[m] ? static_cast<float>(static_cast<const T*>(p.v)[v_at[m] + j * p.v_node]) : 0.f;
       }
-#pragma unroll
-      for (int c = 0; c < V; ++c) k[m * V + c] = t[c], v[m * V + c] = u[c];
     }
     float score[H];
 #pragma unroll
     for (int h = 0; h < H; ++h) {
-      score[h] = 0.f;
+      pair sum = mul2(q2[h][0], both(k[0], k[1]));
 #pragma unroll
-      for (int c = 0; c < N; ++c) score[h] = fmaf(q[h][c], k[c], score[h]);
+      for (int c = 1; c < N / 2; ++c) sum = fma2(q2[h][c], both(k[2 * c], k[2 * c + 1]), sum);
+      float x, y;
+      parts(sum, x, y);
+      score[h] = x + y;
     }
 #pragma unroll
     for (int o = TEAM / 2; o > 0; o >>= 1)
@@ -134,20 +164,32 @@ template <typename T, int V, int TEAM, int PIECES, int H> __global__ void __laun
     if (there) {
 #pragma unroll
       for (int h = 0; h < H; ++h) {
-        State<N>& s = state[h];
-        if (score[h] > s.top || score[h] != score[h]) {  // a new maximum (or not a number, which stays)
-          const float keep = exp2_fast(s.top - score[h]);
-          s.sum *= keep;
+        if (score[h] > tops_[h] || score[h] != score[h]) {                // a new maximum (or not a number, which stays)
+          const float keep = exp2_fast(tops_[h] - score[h]);
+          sums_[h] *= keep;
+          const pair keeps = both(keep, keep);
 #pragma unroll
-          for (int c = 0; c < N; ++c) s.o[c] *= keep;
-          s.top = score[h];
+          for (int c = 0; c < N / 2; ++c) o2[h][c] = mul2(o2[h][c], keeps);
+          tops_[h] = score[h];
         }
-        const float w = score[h] == -INFINITY ? 0.f : exp2_fast(score[h] - s.top);
-        s.sum += w;
+        const float w = score[h] == -INFINITY ? 0.f : exp2_fast(score[h] - tops_[h]);
+        const pair weights = both(w, w);
+        sums_[h] += w;
+        if (w != 0.f) {                                  // of a weight of zero, nothing, whatever the value
 #pragma unroll
-        for (int c = 0; c < N; ++c) s.o[c] = fmaf(w, v[c], s.o[c]);
+          for (int c = 0; c < N / 2; ++c) o2[h][c] = fma2(weights, both(v[2 * c], v[2 * c + 1]), o2[h][c]);
+        }
       }
     }
+  }
+  if constexpr (V > 1) attention::copies_wait<0>();
+  State<N> state[H];
+#pragma unroll
+  for (int h = 0; h < H; ++h) {
+    state[h].top = tops_[h];
+    state[h].sum = sums_[h];
+#pragma unroll
+    for (int c = 0; c < N / 2; ++c) parts(o2[h][c], state[h].o[2 * c], state[h].o[2 * c + 1]);
   }
   // teams of a warp by shuffles, then warps through shared memory
 #pragma unroll
@@ -228,10 +270,10 @@ template <typename T> __global__ void __launch_bounds__(THREADS) step_join_kerne
 }
 
 constexpr int64_t LEAST_KEYS = 64;                       // of a part: joining costs as much as some keys
-// Parts of the visible keys: as many as give every SM four CTAs.
+// Parts of the visible keys: so many that SMs with shorter chains take more of them.
 void cut(StepArgs& p, int64_t chains, int kv_heads) {
   const int64_t visible = std::max<int64_t>(1, std::min<int64_t>(p.capacity, p.before + 1 + p.sinks));
-  const int64_t others = std::max<int64_t>(1, chains * kv_heads), wanted = ceil_div((int64_t)sm_count() * 8, others);
+  const int64_t others = std::max<int64_t>(1, chains * kv_heads), wanted = ceil_div((int64_t)sm_count() * 16, others);
   const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(wanted, ceil_div(visible, LEAST_KEYS)), 1024));
   p.part_keys = ceil_div(ceil_div(visible, parts), 16) * 16;
   p.num_parts = (int)ceil_div(visible, p.part_keys);

@@ -44,7 +44,9 @@ def add_rms_norm(x: Tensor, residual: Optional[Tensor] = None, weight: Optional[
 
     Differentiable once, in ``x``, ``residual`` and ``weight``; the weight's gradient uses no atomics and is the same bits at every call."""
     _ops.check(x, residual, weight, eps)
-    return _AddRMSNorm.apply(x, residual, weight, float(eps))
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, residual, weight)):
+        return _AddRMSNorm.apply(x, residual, weight, float(eps))
+    return _ops.norm_forward(x, residual, weight, float(eps), False)[:2]
 
 
 def add_rms_norm_e4m3(x: Tensor, residual: Optional[Tensor] = None, weight: Optional[Tensor] = None, eps: float = 1e-6, group: Optional[int] = None

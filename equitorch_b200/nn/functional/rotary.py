@@ -18,13 +18,13 @@ class _Rotary(Function):
     def forward(ctx, q, k, positions, frequencies, heads, kv_heads, interleaved, magnitude, backward):
         ctx.save_for_backward(positions, frequencies)
         ctx.args = heads, kv_heads, interleaved, magnitude
-        ctx.turned_back, ctx.shapes = backward, (q.shape, None if k is None else k.shape)
+        ctx.turned_back = backward
         return _ops.rotary(q, k, positions, frequencies, heads, kv_heads, interleaved, magnitude, backward)
 
     @staticmethod
     def backward(ctx, dq, dk):
         positions, frequencies = ctx.saved_tensors
-        dq, dk = _Rotary.apply(dq, dk if ctx.shapes[1] is not None else None, positions, frequencies, *ctx.args, not ctx.turned_back)
+        dq, dk = _Rotary.apply(dq, dk if ctx.needs_input_grad[1] else None, positions, frequencies, *ctx.args, not ctx.turned_back)
         return (dq if ctx.needs_input_grad[0] else None, dk if ctx.needs_input_grad[1] else None, *[None] * 7)
 
 
@@ -71,5 +71,7 @@ def rotary(q: Tensor, k: Optional[Tensor], positions: Tensor, frequencies: Tenso
     Differentiable any number of times in ``q`` and ``k``."""
     kv_heads = num_heads if kv_heads is None else kv_heads
     _ops.check(q, k, positions, frequencies, num_heads, kv_heads)
-    out = _Rotary.apply(q, k, positions, frequencies, num_heads, kv_heads, bool(interleaved), float(magnitude), False)
+    args = q, k, positions, frequencies, num_heads, kv_heads, bool(interleaved), float(magnitude), False
+    wanted = torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))
+    out = _Rotary.apply(*args) if wanted else _ops.rotary(*args)
     return out[0] if k is None else out

@@ -50,7 +50,10 @@ def window_attention(q: Tensor, k: Tensor, v: Tensor, graphs: PackedGraphs, num_
     _ops.check(q, k, v, graphs, num_heads, kv_heads, (before, after, sinks), scale)
     if scale is None:
         scale = (q.shape[1] * q.shape[2] // num_heads) ** -0.5
-    return _WindowAttention.apply(q, k, v, graphs, num_heads, kv_heads, (before, after, sinks), float(scale))
+    args = q, k, v, graphs, num_heads, kv_heads, (before, after, sinks), float(scale)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _WindowAttention.apply(*args)
+    return _ops.window_forward(*args, False)[0]
 
 
 def window_attention_step(q: Tensor, keys: Tensor, values: Tensor, lengths: Tensor, num_heads: int, before: int, sinks: int = 0,
