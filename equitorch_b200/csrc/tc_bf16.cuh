@@ -15,18 +15,19 @@ __host__ __device__ inline uint32_t idesc_bf16(int m, int n, bool a_rows = false
 __device__ __forceinline__ uint32_t umma_lo_rows(uint32_t at, uint32_t group_bytes) { return ((at & 0x3FFFF) >> 4) | ((group_bytes >> 4) << 16); }
 constexpr uint32_t K_STEP = 2, ROWS_STEP = 128;          // 16 of k in units of 16 bytes, along k and along the rows
 
-__device__ __forceinline__ void umma_bf16(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+// One thread issues all MMAs, and what it does between two of them counts: low words stepped by immediates, as for TF32.
+template <bool ACCUMULATE> __device__ __forceinline__ void umma_bf16(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tmov.b64 a, {%1, %4};\n\tmov.b64 b, {%2, %4};\n\tsetp.ne.b32 p, %5, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}"
-      ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(idesc), "n"(UMMA_DESC_HI), "r"(accumulate) : "memory");
+      ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(idesc), "n"(UMMA_DESC_HI), "n"(ACCUMULATE ? 1 : 0) : "memory");
 }
 // A in tensor memory: a lane is a row, two values of k a column
-__device__ __forceinline__ void umma_bf16_ta(uint32_t d, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+template <bool ACCUMULATE> __device__ __forceinline__ void umma_bf16_ta(uint32_t d, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tmov.b64 b, {%2, %4};\n\tsetp.ne.b32 p, %5, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}"
-      ::"r"(d), "r"(a_tmem), "r"(b_lo), "r"(idesc), "n"(UMMA_DESC_HI), "r"(accumulate) : "memory");
+      ::"r"(d), "r"(a_tmem), "r"(b_lo), "r"(idesc), "n"(UMMA_DESC_HI), "n"(ACCUMULATE ? 1 : 0) : "memory");
 }
 
 // Loads of 32 columns, and the wait that the values of the loads before it pass through.

@@ -23,6 +23,7 @@
 //
 // Rows whose target is negative may hold anything: their G is set, not multiplied, to zero, and the backward pass reads x from a copy in which they are zero.
 #include <algorithm>
+#include <type_traits>
 
 #include "tc_bf16.cuh"
 
@@ -216,19 +217,22 @@ template <int PARTS, int MODE> __global__ void __launch_bounds__(THREADS, 1) los
               const uint32_t at = s32(ring + (size_t)s * STAGE), bt = at + a_bytes<PARTS>();
               const uint32_t a_lo = A_TURNED ? umma_lo_rows(at, 8192) : umma_lo(at), b_lo = B_TURNED ? umma_lo_rows(bt, 8192) : umma_lo(bt);
               constexpr uint32_t A_PART = TILE_M * BK * 2 / 16, B_PART = COLS * BK * 2 / 16;
-              const uint32_t more = kb > k0;
-#pragma unroll
-              for (int q = 0; q < 4; ++q) {
+              auto parts_of = [&](int q, auto first) {
+                constexpr bool MORE = !decltype(first)::value;
                 const uint32_t an = a_lo + q * A_STEP, bn = b_lo + q * B_STEP;
-                umma_bf16(d, an, bn, idesc, more | (q > 0));
+                umma_bf16<MORE>(d, an, bn, idesc);
                 if constexpr (F32) {
-                  umma_bf16(d + COLS, an, bn + 2 * B_PART, idesc, more | (q > 0));
-                  umma_bf16(d + COLS, an + 2 * A_PART, bn, idesc, 1);
-                  umma_bf16(d + COLS, an + A_PART, bn + B_PART, idesc, 1);
-                  umma_bf16(d + COLS, an, bn + B_PART, idesc, 1);
-                  umma_bf16(d + COLS, an + A_PART, bn, idesc, 1);
+                  umma_bf16<MORE>(d + COLS, an, bn + 2 * B_PART, idesc);
+                  umma_bf16<true>(d + COLS, an + 2 * A_PART, bn, idesc);
+                  umma_bf16<true>(d + COLS, an + A_PART, bn + B_PART, idesc);
+                  umma_bf16<true>(d + COLS, an, bn + B_PART, idesc);
+                  umma_bf16<true>(d + COLS, an + A_PART, bn, idesc);
                 }
-              }
+              };
+              if (kb == k0) parts_of(0, std::true_type());
+              else parts_of(0, std::false_type());
+#pragma unroll
+              for (int q = 1; q < 4; ++q) parts_of(q, std::false_type());
               umma_commit(&empty[s]);
               if (++s == STAGES) s = 0, ph ^= 1;
             }

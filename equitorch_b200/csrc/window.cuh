@@ -24,7 +24,36 @@ using attention::LOG2E;
 struct WindowParams {
   AttentionParams q, kv;     // of the heads of queries; of the heads of keys (dk and dv)
   int before, after, sinks, group;
+  // Gradients of the first nodes of chains from queries behind their windows, made apart (SPLIT) because a chain may have any number of those: sums of dS q and of P g
+  // by blocks of FAR_BLOCK nodes of the batch, [pair of a block and a chain][head of keys][16 first nodes][dk, dv][node][value], then joined in the chain's first place.
+  const int64_t* ptr;
+  int64_t chains;
+  float* far;
+  int split;
 };
+constexpr int FAR_BLOCK = 512, FAR_ROWS = 16, MOST_SPLIT_SINKS = 64;
+__host__ __device__ inline int far_groups(const WindowParams& p) { return (p.sinks + FAR_ROWS - 1) / FAR_ROWS; }
+// A block b and a chain g that has nodes in it are pair b + g, which no other two are: going on, either the block or the chain moves by one.
+__device__ __forceinline__ int64_t far_place(const WindowParams& p, int64_t pair, int kv, int group) {
+  return ((pair * p.kv.heads + kv) * far_groups(p) + group) * (2 * FAR_ROWS * (int64_t)(p.q.comps * p.q.size));
+}
+// The last chain g with `of(g)` at most `x`, `of` ascending; -1 if there is none.
+template <typename F> __device__ __forceinline__ int64_t last_chain(int64_t chains, int64_t x, F of) {
+  int64_t lo = -1, hi = chains - 1;
+  while (lo < hi) {
+    const int64_t mid = lo + (hi - lo + 1) / 2;
+    if (of(mid) <= x) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+// What queries behind its window give a first node j of the chain [lo, hi): dk, with dv FAR_ROWS rows on; none: NULL.
+__device__ __forceinline__ const float* far_of(const WindowParams& p, int j, int kv, int lo, int hi) {
+  if (!p.split || j >= lo + p.sinks || j + p.before + 1 >= hi) return nullptr;
+  const int64_t g = last_chain(p.chains, j, [&](int64_t c) { return p.ptr[c]; });
+  const int group = (j - lo) / FAR_ROWS, first = lo + group * FAR_ROWS;
+  return p.far + far_place(p, (first + p.before + 1) / FAR_BLOCK + g, kv, group) + (int64_t)(j - first) * (p.q.comps * p.q.size);
+}
 
 __device__ __forceinline__ bool sees(const WindowParams& p, int i, int j, int lo) { return j <= i + p.after && (j >= i - p.before || j < lo + p.sinks); }
 
@@ -110,7 +139,8 @@ template <typename T> __device__ __noinline__ void again_columns(const WindowPar
 
 __device__ __forceinline__ bool is_finite(float x) { return fabsf(x) < INFINITY; }
 
-int tiles_forward_f32(const WindowParams& p, int tile_rows, int64_t num_tiles, cudaStream_t s);   // window_f32.cu and window_bf16.cu
+int far_bf16(const WindowParams& p, cudaStream_t s);                                                             // window_f32.cu and window_bf16.cu
+int tiles_forward_f32(const WindowParams& p, int tile_rows, int64_t num_tiles, cudaStream_t s);
 int tiles_forward_bf16(const WindowParams& p, int tile_rows, int64_t num_tiles, cudaStream_t s);
 int tiles_backward_f32(const WindowParams& p, int tile_rows, int64_t num_tiles, cudaStream_t s);
 int tiles_backward_bf16(const WindowParams& p, int tile_rows, int64_t num_tiles, cudaStream_t s);

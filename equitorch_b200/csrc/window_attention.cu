@@ -21,7 +21,7 @@ int check(const eqt_window_attention_args* a) {
 }
 
 // What all kernels take.  Windows reach no further than the longest chain, so a place and a reach, both below 2^30, add up in 32 bits.
-WindowParams params(const eqt_window_attention_args& a, float* delta) {
+WindowParams params(const eqt_window_attention_args& a) {
   WindowParams p{};
   const int64_t reach = std::min<int64_t>(std::max<int64_t>(a.longest, 1), a.n);
   p.before = (int)std::min(a.before, reach), p.after = (int)std::min(a.after, reach), p.sinks = (int)std::min(a.sinks, reach);
@@ -29,7 +29,7 @@ WindowParams params(const eqt_window_attention_args& a, float* delta) {
   AttentionParams& q = p.q;
   const int64_t width = (int64_t)a.heads * a.head_channels;
   q.q = {a.q, a.q_node, a.q_comp}, q.k = {a.k, a.k_node, a.k_comp}, q.v = {a.v, a.v_node, a.v_comp}, q.g = {a.grad, a.comps * width, width};
-  q.out = a.out, q.dq = a.dq, q.dk = a.dk, q.dv = a.dv, q.top = a.stats, q.inverse = a.stats ? a.stats + a.heads * a.n : nullptr, q.delta = delta;
+  q.out = a.out, q.dq = a.dq, q.dk = a.dk, q.dv = a.dv, q.top = a.stats, q.inverse = a.stats ? a.stats + a.heads * a.n : nullptr, q.delta = nullptr;
   q.tiles = reinterpret_cast<const int4*>(a.tiles), q.n = a.n, q.heads = a.heads, q.comps = a.comps, q.size = a.head_channels, q.scale = a.scale;
   const int v = a.dtype == EQT_F32 ? 4 : 8;
   const int64_t strides = a.q_node | a.q_comp | a.k_node | a.k_comp | a.v_node | a.v_comp;
@@ -38,6 +38,11 @@ WindowParams params(const eqt_window_attention_args& a, float* delta) {
   q.vec = bits % 16 == 0 && strides % v == 0 && a.head_channels % v == 0;
   p.kv = q;
   p.kv.heads = a.kv_heads;
+  // A tile of keys that holds a chain's first nodes would walk to the chain's end, alone, while the others are done: one chain of 32,781 nodes, 8 heads of 128
+  // values, window of 1024, backward by columns 876 us, with these queries apart 390 in all.  Two launches more, so not for what is walked in a few steps; and not for so
+  // many first nodes that tiles are full of them.
+  p.ptr = a.ptr, p.chains = a.num_graphs;
+  p.split = p.sinks > 0 && p.sinks <= MOST_SPLIT_SINKS && a.longest - p.before > 2 * FAR_BLOCK;
   return p;
 }
 
@@ -51,9 +56,15 @@ bool on_tensor_cores(const eqt_window_attention_args& a) {
   return bits % 16 == 0 && strides % 8 == 0 && a.head_channels % 8 == 0;
 }
 
-// Scratch: the nodes' chains, and for the backward pass the deltas.
+// Scratch: the nodes' chains, and for the backward pass the deltas and what far queries give first nodes.
 int64_t spans_bytes(const eqt_window_attention_args& a) { return a.dtype == EQT_BF16 ? (int64_t)up((size_t)a.n * sizeof(int2)) : 0; }
-int64_t scratch_bytes(const eqt_window_attention_args& a, bool backward) { return spans_bytes(a) + (backward ? (int64_t)up((size_t)a.heads * a.n * 4) : 0); }
+int64_t delta_bytes(const eqt_window_attention_args& a) { return (int64_t)up((size_t)a.heads * a.n * 4); }
+int64_t scratch_bytes(const eqt_window_attention_args& a, bool backward) {
+  if (!backward) return spans_bytes(a);
+  const WindowParams p = params(a);
+  const int64_t pairs = ceil_div(a.n, FAR_BLOCK) + a.num_graphs;
+  return spans_bytes(a) + delta_bytes(a) + (p.split ? pairs * a.kv_heads * far_groups(p) * 2 * FAR_ROWS * a.comps * a.head_channels * 4 : 0);
+}
 int check_scratch(const eqt_window_attention_args& a, bool backward) {
   const int64_t need = scratch_bytes(a, backward);
   if (need && (!a.scratch || a.scratch_bytes < need))
@@ -91,7 +102,7 @@ extern "C" int eqt_window_attention_forward(const eqt_window_attention_args* arg
   if (a.n == 0 || a.num_tiles == 0) return EQT_OK;
   if (!a.q || !a.k || !a.v || !a.out || !a.tiles) return fail(EQT_ERR_BAD_ARGUMENT, "window_attention: NULL pointer");
   if (int rc = check_scratch(a, false)) return rc;
-  const WindowParams p = params(a, nullptr);
+  const WindowParams p = params(a);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (on_tensor_cores(a)) {
     TcParams t;
@@ -107,7 +118,11 @@ extern "C" int eqt_window_attention_backward(const eqt_window_attention_args* ar
   if (a.n == 0 || a.num_tiles == 0) return EQT_OK;
   if (!a.q || !a.k || !a.v || !a.grad || !a.out || !a.stats || !a.dq || !a.dk || !a.dv || !a.tiles) return fail(EQT_ERR_BAD_ARGUMENT, "window_attention backward: NULL pointer");
   if (int rc = check_scratch(a, true)) return rc;
-  const WindowParams p = params(a, reinterpret_cast<float*>(static_cast<unsigned char*>(a.scratch) + spans_bytes(a)));
+  WindowParams p = params(a);
+  if (p.split && !a.ptr) return fail(EQT_ERR_BAD_ARGUMENT, "window_attention backward: NULL pointer");
+  unsigned char* base = static_cast<unsigned char*>(a.scratch) + spans_bytes(a);
+  p.q.delta = p.kv.delta = reinterpret_cast<float*>(base);
+  p.far = reinterpret_cast<float*>(base + delta_bytes(a));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (on_tensor_cores(a)) {
     TcParams t;

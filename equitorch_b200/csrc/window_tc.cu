@@ -15,7 +15,7 @@
 // dS goes into dq's product in two parts, as within whole graphs: dq has the error of delta, which goes by the rounded result, already.
 //
 // Two CTAs an SM hide each other's chain of copy, product, softmax and product; COLUMNS of more than 64 values, whose two sums take half of the
-// tensor memory, has one CTA of two groups of softmax warps that take turns.  Warps 0 to 3 (7): softmax; then one that issues the MMAs and three that copy (16 bytes a
+// tensor memory, has one CTA of two groups of softmax warps that take turns.  Warps 0 to 3 (7): softmax; then two that issue MMAs and two that copy (16 bytes a
 // thread to the places of the 128-byte swizzle, so that heads of any whole pieces and components of any stride fit one layout).
 //
 // Bound by the special functions at 64 values a head (a score is 4 x 64 flops, 0.16 ps of the tensor cores, and one exponential, 0.22 ps) and by the
@@ -29,20 +29,17 @@ namespace eqt {
 namespace window {
 namespace {
 using namespace tc;
-using attention::copy16;
 using attention::copy4;
-using attention::copies_commit;
-using attention::copies_wait;
 using T = __nv_bfloat16;
 
 enum Mode { FORWARD, ROWS, COLUMNS };
-constexpr int KEYS = 64, LOADERS = 96;                   // of the other side at a time; threads that copy
+constexpr int KEYS = 64, LOADERS = 64;                   // of the other side at a time; threads that copy
 constexpr float FAR = 8.f;                               // of log2, that a score may be above the unit
 
 template <int DP, int MODE> struct Form {
   static constexpr int GROUPS = MODE == COLUMNS && DP == 128 ? 2 : 1;               // of softmax warps, each with a buffer of scores
   static constexpr int BUFFERS = MODE == FORWARD ? 2 : GROUPS;
-  static constexpr int SOFT = 4 * GROUPS, THREADS = 32 * (SOFT + 4), CTAS = GROUPS == 2 ? 1 : 2;
+  static constexpr int SOFT = 4 * GROUPS, THREADS = 32 * (SOFT + 2) + LOADERS, CTAS = GROUPS == 2 ? 1 : 2;
   static constexpr int OWN = MODE == FORWARD ? 1 : 2;                                // operands of the tile's rows
   static constexpr int OWN_BYTES = TILE_M * DP * 2, SLOT_BYTES = KEYS * DP * 2;
   static constexpr int SLOTS = MODE == FORWARD ? (DP == 128 ? 4 : 8) : MODE == ROWS ? (DP == 128 ? 3 : 6) : 8;
@@ -50,23 +47,57 @@ template <int DP, int MODE> struct Form {
   static constexpr int BUFFER = MODE == FORWARD ? KEYS : 2 * KEYS;                   // columns of tensor memory: S, or S and dP
   static constexpr int SUM_AT = BUFFERS * BUFFER, COLS = GROUPS == 2 ? 512 : 256;
   static constexpr size_t bytes() { return (size_t)OWN * OWN_BYTES + (size_t)SLOTS * SLOT_BYTES + NUMBERS + 512; }
+  static_assert(LOADERS == KEYS, "a number of a query each");
   static_assert(SUM_AT + (MODE == COLUMNS ? 2 : 1) * DP <= COLS, "tensor memory");
 };
 
-// Rows [first, first + ROWS) of one head, 128-byte swizzle, 64 values a line and ROWS lines a group; zeros from the `left`-th row on and behind the head's values.
-template <int DP, int ROWS_> __device__ __forceinline__ void load_operand(unsigned char* dst, const Operand& x, int first, int left, int head, const AttentionParams& p, int thread) {
-  constexpr int PIECES = DP / 8, STEP = LOADERS / PIECES;
-  const int col = thread % PIECES, at = col * 8, values = p.comps * p.size;
-  if (at >= (values + 15) / 16 * 16) return;
-  const bool on = at < values;
-  const int comp = on ? at / p.size : 0;
-  const T* from = static_cast<const T*>(x.p) + comp * x.comp + (int64_t)head * p.size + (on ? at - comp * p.size : 0);
-  unsigned char* to = dst + (col >> 3) * (ROWS_ * 128);
-#pragma unroll 4
-  for (int r = thread / PIECES; r < ROWS_; r += STEP) {
-    const bool there = on && r < left;
-    copy16(to + r * 128 + (((col & 7) ^ (r & 7)) << 4), there ? from + (int64_t)(first + r) * x.node : static_cast<const T*>(x.p), there);
+// What a thread copies of an operand's rows: in each group of 64 values the same 16 bytes of every eighth row, so that where they come from and go
+// (128-byte swizzle, a line of 128 bytes a row) moves on by additions.  Zeros behind the head's values, up to whole sixteens.
+template <int DP> struct Copier {
+  static constexpr int GROUPS = DP / 64;
+  const T* from[GROUPS];
+  int64_t node;
+  int row, size;
+  uint32_t to;
+  bool on[GROUPS], there[GROUPS];                        // has values; has a place
+  __device__ __forceinline__ Copier(const Operand& x, const AttentionParams& p, int thread) : node(x.node), row(thread >> 3), size(p.size) {
+    const int col = thread & 7, values = p.comps * p.size;
+    to = (uint32_t)(row * 128 + ((col ^ row) << 4));
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) {
+      const int at = (col + 8 * g) * 8;
+      on[g] = at < values;
+      there[g] = at < (values + 15) / 16 * 16;
+      const int comp = on[g] ? at / p.size : 0;
+      from[g] = static_cast<const T*>(x.p) + comp * x.comp + (on[g] ? at - comp * p.size : 0) + row * node;
+    }
   }
+  // rows [first, first + ROWS) of a head, zeros from the `left`-th on
+  template <int ROWS_> __device__ __forceinline__ void rows(unsigned char* dst, int first, int left, int head) const {
+    const int64_t move = first * node + (int64_t)head * size, step = 8 * node;
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) {
+      if (!there[g]) continue;
+      const T* f = from[g] + move;
+      const uint32_t d = s32(dst) + to + g * (ROWS_ * 128);
+      if (left >= ROWS_ && on[g]) {
+#pragma unroll
+        for (int r = 0; r < ROWS_ / 8; ++r, f += step)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d + r * 1024), "l"(f) : "memory");
+      } else {
+#pragma unroll
+        for (int r = 0; r < ROWS_ / 8; ++r, f += step) {
+          const bool in = on[g] && 8 * r + row < left;
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d + r * 1024), "l"(in ? f : from[g]), "r"(in ? 16 : 0) : "memory");
+        }
+      }
+    }
+  }
+};
+
+// The barrier has an arrival of this thread when its copies so far have landed.
+__device__ __forceinline__ void land_at(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(s32(bar)) : "memory");
 }
 
 // The bits of [lo, hi) within 64
@@ -93,7 +124,7 @@ template <int MODE> __device__ __forceinline__ Stretch stretch_of(const TcParams
   s.to1 = last + 1;
   if (MODE == COLUMNS) {
     if (a.y > a.x) s.from1 = max(a.x, first - w.after);
-    if (b.y > b.x) s.to1 = max(b.x, first) < b.x + w.sinks ? b.y : min(b.y, last + w.before + 1);
+    if (b.y > b.x) s.to1 = !w.split && max(b.x, first) < b.x + w.sinks ? b.y : min(b.y, last + w.before + 1);
   } else {
     if (a.y > a.x) {
       s.from1 = max(a.x, first - w.before);
@@ -115,8 +146,8 @@ __device__ __forceinline__ void tmem_put16(uint32_t at, const uint32_t* r) {
 }
 __device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// A lane's row of results, `f` times, to (n, components, heads, channels); whether all of it was finite.
-template <int DP> __device__ __forceinline__ bool put_row(uint32_t sum, float f, bool on, void* out, int row, int head, const AttentionParams& p) {
+// A lane's row of results, with `more` where given, `f` times, to (n, components, heads, channels); whether all of it was finite.
+template <int DP> __device__ __forceinline__ bool put_row(uint32_t sum, float f, bool on, void* out, int row, int head, const AttentionParams& p, const float* more = nullptr) {
   bool finite = true;
   const int values = p.comps * p.size;
   T* to = static_cast<T*>(out) + ((int64_t)row * p.comps * p.heads + head) * p.size;
@@ -133,7 +164,7 @@ template <int DP> __device__ __forceinline__ bool put_row(uint32_t sum, float f,
       float v[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        v[j] = __uint_as_float(r[c + j]);
+        v[j] = __uint_as_float(r[c + j]) + (more ? more[at + j] : 0.f);
         finite = finite && is_finite(v[j]);
         v[j] *= f;
       }
@@ -153,10 +184,10 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
   unsigned char *own = smem, *ring = own + F::OWN * F::OWN_BYTES;
   float* numbers = reinterpret_cast<float*>(ring + SLOTS * F::SLOT_BYTES);
   uint64_t* bars = reinterpret_cast<uint64_t*>(ring + SLOTS * F::SLOT_BYTES + F::NUMBERS);
-  uint64_t *full = bars, *empty = full + SLOTS, *own_full = empty + SLOTS, *scores = own_full + 1, *weights = scores + BUFFERS, *done = weights + BUFFERS, *added = done + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(added + 1);
+  uint64_t *full = bars, *empty = full + SLOTS, *own_full = empty + SLOTS, *scores = own_full + 1, *weights = scores + BUFFERS, *freed = weights + BUFFERS, *done = freed + BUFFERS;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
   int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
-  static_assert((2 * SLOTS + 3 + 2 * BUFFERS) * 8 + 8 <= 512, "barriers");
+  static_assert((2 * SLOTS + 2 + 3 * BUFFERS) * 8 + 8 <= 512, "barriers");
 
   const WindowParams& w = p.w;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -170,16 +201,16 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
   if (tid == 0) {
     *abort_flag = (s32(smem) & 1023) != 0;                // the swizzle goes by addresses
     for (int s = 0; s < SLOTS; ++s) {
-      bar_init(&full[s], LOADERS / 32);
+      bar_init(&full[s], LOADERS);
       bar_init(&empty[s], 1);
     }
-    bar_init(own_full, LOADERS / 32);
+    bar_init(own_full, LOADERS);
     for (int b = 0; b < BUFFERS; ++b) {
       bar_init(&scores[b], 1);
       bar_init(&weights[b], 4);
+      bar_init(&freed[b], 1);
     }
     bar_init(done, 1);                                   // all products
-    bar_init(added, 1);                                  // FORWARD: the product of a step; a wait by parity may be one phase behind, no more
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == F::SOFT) {
@@ -192,151 +223,115 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
   const uint32_t tmem = *tmem_slot;
   volatile int* ab = abort_flag;
 
-  if (warp > F::SOFT) {
+  if (warp > F::SOFT + 1) {
     // ---------------- copies ----------------
-    // Items in the order of their use: FORWARD k, v; ROWS v, k; COLUMNS q with its numbers, g.  An item is handed over, once it has landed, after the next
-    // ones have been asked for; before a wait for a place, all that are under way are.
-    const int thread = tid - 32 * (F::SOFT + 1);
-    constexpr int LAG = SLOTS > 4 ? 2 : 1;
+    // Items in the order of their use: FORWARD k, v; ROWS v, k; COLUMNS q with its numbers, g.  A thread's copies arrive at the item's barrier when they
+    // have landed; the thread that issues the MMAs, which sees them all there, puts the fence between them and the tensor cores.
+    const int thread = tid - 32 * (F::SOFT + 2);
     const int left = last + 1 - first;
-    if (MODE == FORWARD) {
-      load_operand<DP, TILE_M>(own, w.q.q, first, left, head, w.q, thread);
-    } else if (MODE == ROWS) {
-      load_operand<DP, TILE_M>(own, w.q.q, first, left, head, w.q, thread);
-      load_operand<DP, TILE_M>(own + F::OWN_BYTES, w.q.g, first, left, head, w.q, thread);
-    } else {
-      load_operand<DP, TILE_M>(own, w.q.k, first, left, kv, w.q, thread);
-      load_operand<DP, TILE_M>(own + F::OWN_BYTES, w.q.v, first, left, kv, w.q, thread);
-    }
-    copies_commit();
-    int handed = -1;                                     // the tile's own rows are item -1
-    auto hand_over = [&](int upto) {
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      for (; handed < upto; ++handed)
-        if (lane == 0) bar_arrive(handed < 0 ? own_full : &full[handed % SLOTS]);
-    };
+    const Copier<DP> even(MODE == FORWARD ? w.q.k : MODE == ROWS ? w.q.v : w.q.q, w.q, thread);
+    const Copier<DP> odd(MODE == FORWARD ? w.q.v : MODE == ROWS ? w.q.k : w.q.g, w.q, thread);
+    Copier<DP>(MODE == COLUMNS ? w.q.k : w.q.q, w.q, thread).template rows<TILE_M>(own, first, left, head);
+    if (MODE != FORWARD) Copier<DP>(MODE == COLUMNS ? w.q.v : w.q.g, w.q, thread).template rows<TILE_M>(own + F::OWN_BYTES, first, left, head);
+    land_at(own_full);
     bool ok = true;
     for (int item = 0; item < 2 * steps && ok; ++item) {
       const int slot = item % SLOTS, step = item >> 1;
       if (item >= SLOTS) {
-        const uint32_t parity = (uint32_t)((item / SLOTS - 1) & 1);
-        bool free = bar_try(&empty[slot], parity);
-        if (!__all_sync(0xffffffffu, free)) {
-          copies_wait<0>();
-          hand_over(item);
-          ok = __all_sync(0xffffffffu, bar_wait(&empty[slot], parity, ab));
-          if (!ok) break;
-        }
+        ok = __all_sync(0xffffffffu, bar_wait(&empty[slot], (uint32_t)((item / SLOTS - 1) & 1), ab));
+        if (!ok) break;
       }
       int end;
       const int at = walk.at(MODE == COLUMNS ? step % walk.steps : step, end);
       unsigned char* to = ring + slot * F::SLOT_BYTES;
-      if (MODE == COLUMNS) {
-        const int h = kv * w.group + step / walk.steps;
-        load_operand<DP, KEYS>(to, item & 1 ? w.q.g : w.q.q, at, end - at, h, w.q, thread);
-        if (!(item & 1))
-          for (int c = thread; c < 3 * KEYS; c += LOADERS) {
-            const int r = c % KEYS;
-            const float* from = c < KEYS ? w.q.top : c < 2 * KEYS ? w.q.inverse : w.q.delta;
-            const bool there = at + r < end;
-            copy4(numbers + slot / 2 * 3 * KEYS + c, from + (there ? (int64_t)h * w.q.n + at + r : 0), there);
-          }
-      } else {
-        load_operand<DP, KEYS>(to, (item & 1) == (MODE == FORWARD) ? w.q.v : w.q.k, at, end - at, kv, w.q, thread);
+      const int h = MODE == COLUMNS ? kv * w.group + step / walk.steps : kv;
+      (item & 1 ? odd : even).template rows<KEYS>(to, at, end - at, h);
+      if (MODE == COLUMNS && !(item & 1)) {
+        const bool there = at + thread < end;
+        const int64_t from = there ? (int64_t)h * w.q.n + at + thread : 0;
+        float* num = numbers + slot / 2 * 3 * KEYS + thread;
+        copy4(num, w.q.top + from, there);
+        copy4(num + KEYS, w.q.inverse + from, there);
+        copy4(num + 2 * KEYS, w.q.delta + from, there);
       }
-      copies_commit();
-      if (item >= LAG) {
-        copies_wait<LAG>();
-        hand_over(item - LAG + 1);
-      }
+      land_at(&full[slot]);
     }
-    copies_wait<0>();
-    hand_over(2 * steps);
-  } else if (warp == F::SOFT) {
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  } else if (warp >= F::SOFT) {
     // ---------------- MMAs ----------------
+    // One thread makes scores, another adds weighted rows up: each MMA costs its thread some sixty cycles whatever its size, and a step has up to 24.
     if (lane == 0) {
       const uint32_t to_scores = idesc_bf16(TILE_M, KEYS), to_sums = idesc_bf16(TILE_M, wide, false, true);
-      const uint32_t own_at = s32(own), ring_at = s32(ring);
+      const uint32_t own_at = s32(own), ring_at = s32(ring), sum = tmem + F::SUM_AT;
       const int ksteps = wide / 16;
       auto slot_at = [&](int item) { return ring_at + (uint32_t)(item % SLOTS) * F::SLOT_BYTES; };
       auto arrived = [&](int item) { return bar_wait(&full[item % SLOTS], (uint32_t)((item / SLOTS) & 1), ab); };
+      auto fence = [] { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); };
+      // scores of a step are free when the products that read them BUFFERS steps before are done
+      auto free_again = [&](int j) { return j < BUFFERS || bar_wait(&freed[j % BUFFERS], (uint32_t)((j / BUFFERS - 1) & 1), ab); };
+      auto weighted = [&](int j) { return bar_wait(&weights[j % BUFFERS], (uint32_t)((j / BUFFERS) & 1), ab); };
       // d (128 rows x 64) = rows of the tile times rows of the slot
       auto score = [&](uint32_t d, uint32_t a, uint32_t b) {
         const uint32_t a_lo = umma_lo(a), b_lo = umma_lo(b);
-        for (int k = 0; k < ksteps; ++k)
-          umma_bf16(d, a_lo + (k >> 2) * (TILE_M * 128 / 16) + (k & 3) * K_STEP, b_lo + (k >> 2) * (KEYS * 128 / 16) + (k & 3) * K_STEP, to_scores, k > 0);
+        umma_bf16<false>(d, a_lo, b_lo, to_scores);
+#pragma unroll
+        for (int k = 1; k < DP / 16; ++k)
+          if (k < ksteps) umma_bf16<true>(d, a_lo + (k >> 2) * (TILE_M * 128 / 16) + (k & 3) * K_STEP, b_lo + (k >> 2) * (KEYS * 128 / 16) + (k & 3) * K_STEP, to_scores);
       };
       // d (128 rows x values) += weights in tensor memory times the slot
       auto add = [&](uint32_t d, uint32_t a, uint32_t b, bool more) {
         const uint32_t b_lo = umma_lo_rows(b, KEYS * 128);
+        if (more) umma_bf16_ta<true>(d, a, b_lo, to_sums);
+        else umma_bf16_ta<false>(d, a, b_lo, to_sums);
 #pragma unroll
-        for (int k = 0; k < KEYS / 16; ++k) umma_bf16_ta(d, a + k * 8, b_lo + k * ROWS_STEP, to_sums, more || k > 0);
+        for (int k = 1; k < KEYS / 16; ++k) umma_bf16_ta<true>(d, a + k * 8, b_lo + k * ROWS_STEP, to_sums);
       };
-      bool ok = bar_wait(own_full, 0, ab);
-      const uint32_t sum = tmem + F::SUM_AT;
-      if (MODE == FORWARD) {
-        auto issue = [&](int j) {
-          ok = ok && arrived(2 * j);
-          if (!ok) return;
-          tc_fence_after();
-          score(tmem + (j & 1) * F::BUFFER, own_at, slot_at(2 * j));
-          umma_commit(&scores[j & 1]);
-          umma_commit(&empty[2 * j % SLOTS]);
-        };
-        if (steps) issue(0);
+      bool ok = true;
+      if (warp == F::SOFT) {
+        ok = bar_wait(own_full, 0, ab);
         for (int j = 0; j < steps && ok; ++j) {
-          if (j + 1 < steps) issue(j + 1);
-          ok = ok && bar_wait(&weights[j & 1], (uint32_t)((j >> 1) & 1), ab) && arrived(2 * j + 1);
-          if (!ok) break;
-          tc_fence_after();
-          add(sum, tmem + (j & 1) * F::BUFFER, slot_at(2 * j + 1), j > 0);
-          umma_commit(&empty[(2 * j + 1) % SLOTS]);
-          umma_commit(added);
-        }
-        if (ok) umma_commit(done);
-      } else if (MODE == ROWS) {
-        for (int j = 0; j < steps && ok; ++j) {
-          ok = arrived(2 * j);
-          if (!ok) break;
-          tc_fence_after();
-          score(tmem + KEYS, own_at + F::OWN_BYTES, slot_at(2 * j));
-          umma_commit(&empty[2 * j % SLOTS]);
-          ok = arrived(2 * j + 1);
-          if (!ok) break;
-          tc_fence_after();
-          score(tmem, own_at, slot_at(2 * j + 1));
-          umma_commit(&scores[0]);
-          ok = bar_wait(&weights[0], (uint32_t)(j & 1), ab);
-          if (!ok) break;
-          tc_fence_after();
-          add(sum, tmem, slot_at(2 * j + 1), j > 0);
-          add(sum, tmem + 32, slot_at(2 * j + 1), true);
-          umma_commit(&empty[(2 * j + 1) % SLOTS]);
-        }
-        if (ok) umma_commit(done);
-      } else {
-        auto issue = [&](int j) {
-          ok = ok && arrived(2 * j) && arrived(2 * j + 1);
-          if (!ok) return;
-          tc_fence_after();
           const uint32_t d = tmem + (j % BUFFERS) * F::BUFFER;
-          score(d, own_at, slot_at(2 * j));
-          score(d + KEYS, own_at + F::OWN_BYTES, slot_at(2 * j + 1));
+          if (MODE == ROWS) {
+            // dP's place is free when the softmax has read it, that of S when dS has been used
+            ok = arrived(2 * j) && (j == 0 || weighted(j - 1));
+            if (!ok) break;
+            fence();
+            tc_fence_after();
+            score(d + KEYS, own_at + F::OWN_BYTES, slot_at(2 * j));
+            umma_commit(&empty[2 * j % SLOTS]);
+            ok = arrived(2 * j + 1) && free_again(j);
+            if (!ok) break;
+            fence();
+            tc_fence_after();
+            score(d, own_at, slot_at(2 * j + 1));
+          } else {
+            ok = arrived(2 * j) && (MODE == FORWARD || arrived(2 * j + 1)) && free_again(j);
+            if (!ok) break;
+            fence();
+            tc_fence_after();
+            score(d, own_at, slot_at(2 * j));
+            if (MODE == FORWARD) umma_commit(&empty[2 * j % SLOTS]);
+            else score(d + KEYS, own_at + F::OWN_BYTES, slot_at(2 * j + 1));
+          }
           umma_commit(&scores[j % BUFFERS]);
-        };
-        if (steps) issue(0);
+        }
+      } else {
         for (int j = 0; j < steps && ok; ++j) {
-          if (BUFFERS == 2 && j + 1 < steps) issue(j + 1);
-          ok = ok && bar_wait(&weights[j % BUFFERS], (uint32_t)((j / BUFFERS) & 1), ab);
+          const uint32_t d = tmem + (j % BUFFERS) * F::BUFFER;
+          ok = arrived(2 * j + 1) && (MODE != COLUMNS || arrived(2 * j));
+          if (!ok) break;
+          fence();
+          ok = weighted(j);
           if (!ok) break;
           tc_fence_after();
-          const uint32_t d = tmem + (j % BUFFERS) * F::BUFFER;
           add(sum, d, slot_at(2 * j + 1), j > 0);
-          add(sum + DP, d + KEYS, slot_at(2 * j), j > 0);
-          umma_commit(&empty[2 * j % SLOTS]);
+          if (MODE == ROWS) add(sum, d + 32, slot_at(2 * j + 1), true);
+          if (MODE == COLUMNS) {
+            add(sum + DP, d + KEYS, slot_at(2 * j), j > 0);
+            umma_commit(&empty[2 * j % SLOTS]);
+          }
           umma_commit(&empty[(2 * j + 1) % SLOTS]);
-          if (BUFFERS == 1 && j + 1 < steps) issue(j + 1);
+          umma_commit(&freed[j % BUFFERS]);
         }
         if (ok) umma_commit(done);
       }
@@ -351,7 +346,7 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
     const float unit = w.q.scale * LOG2E;
     // what the row sees: [lo, hi), and the first nodes [span.x, far)
     const int lo = !on ? 0 : max(span.x, row - (MODE == COLUMNS ? w.after : w.before));
-    const int hi = !on ? 0 : MODE == COLUMNS ? (row < span.x + w.sinks ? span.y : min(span.y, row + w.before + 1)) : min(span.y, row + w.after + 1);
+    const int hi = !on ? 0 : MODE == COLUMNS ? (!w.split && row < span.x + w.sinks ? span.y : min(span.y, row + w.before + 1)) : min(span.y, row + w.after + 1);
     const int far = on && MODE != COLUMNS ? min(lo, span.x + w.sinks) : 0;
     bool ok = true;
     auto seen = [&](int at, int end) {
@@ -393,7 +388,7 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
           total *= keep;
           if (higher) base = now;
           if (j > 0) {
-            ok = bar_wait(added, (uint32_t)((j - 1) & 1), ab);
+            ok = bar_wait(&freed[(j - 1) & 1], (uint32_t)(((j - 1) >> 1) & 1), ab);
             if (!__all_sync(0xffffffffu, ok)) break;
             tc_fence_after();
 #pragma unroll
@@ -561,8 +556,9 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
       if (ok && steps) {                                  // of two groups, one stores each sum
         tc_fence_after();
         bool finite = true;
-        if (group == 0) finite = put_row<DP>(sum_at, 1.f, on, w.kv.dv, row, kv, w.kv);
-        if (group == GROUPS - 1) finite = put_row<DP>(sum_at + DP, w.q.scale, on, w.kv.dk, row, kv, w.kv) && finite;
+        const float* more = on ? far_of(w, row, kv, span.x, span.y) : nullptr;
+        if (group == 0) finite = put_row<DP>(sum_at, 1.f, on, w.kv.dv, row, kv, w.kv, more ? more + FAR_ROWS * values : nullptr);
+        if (group == GROUPS - 1) finite = put_row<DP>(sum_at + DP, w.q.scale, on, w.kv.dk, row, kv, w.kv, more) && finite;
         __syncwarp();
         for (unsigned bad = __ballot_sync(0xffffffffu, on && !finite); bad; bad &= bad - 1) {
           const int r = __ffs(bad) - 1;
@@ -622,5 +618,7 @@ int eqt::window::tc_forward(const TcParams& p, cudaStream_t s) {
 int eqt::window::tc_backward(const TcParams& p, cudaStream_t s) {
   const bool narrow = p.w.q.comps * p.w.q.size <= 64;
   if (int rc = narrow ? launch<64, ROWS>(p, s) : launch<128, ROWS>(p, s)) return rc;
+  if (p.w.split)
+    if (int rc = far_bf16(p.w, s)) return rc;
   return narrow ? launch<64, COLUMNS>(p, s) : launch<128, COLUMNS>(p, s);
 }

@@ -40,7 +40,7 @@ __device__ __forceinline__ Walk queries_of(const WindowParams& p, int first, int
   Walk w;
   w.from0 = w.to0 = lo;
   w.from1 = max(lo, first - p.after);
-  w.to1 = first < lo + p.sinks ? hi : min(hi, last + p.before);
+  w.to1 = first < lo + p.sinks && !p.split ? hi : min(hi, last + p.before);
   return w;
 }
 
@@ -309,7 +309,8 @@ __global__ void __launch_bounds__(THREADS, DP <= 64 ? 3 : 2) window_columns_kern
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int c = n * 8 + 2 * t + (i & 1), q = query + c;
-          const bool on = q < end && sees(p, q, row + g + 8 * (i >> 1), lo);
+          const int j = row + g + 8 * (i >> 1);
+          const bool on = q < end && sees(p, q, j, lo) && (!p.split || q <= j + p.before);
           z[n][i] = on ? exp2_fast(z[n][i] * unit - num[c]) * num[KT + c] : 0.f;
           dp[n][i] = on ? z[n][i] * (dp[n][i] - num[2 * KT + c]) : 0.f;
         }
@@ -319,13 +320,153 @@ __global__ void __launch_bounds__(THREADS, DP <= 64 ? 3 : 2) window_columns_kern
     __syncthreads();
   }
   if (!work) return;
+  if (p.split && row < lo + p.sinks) {
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int j = row + g + 8 * r, values = p.q.comps * p.q.size;
+      const float* far = j < hi ? far_of(p, j, kv, lo, hi) : nullptr;
+      if (!far) continue;
+#pragma unroll
+      for (int n = 0; n < DP / 8; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int c = n * 8 + 2 * t + i;
+          if (c >= values) continue;
+          dk[n][2 * r + i] += far[c];
+          dv[n][2 * r + i] += far[FAR_ROWS * values + c];
+        }
+    }
+  }
   const bool ok0 = finite_rows(dk, 0) && finite_rows(dv, 0), ok1 = finite_rows(dk, 1) && finite_rows(dv, 1);
   store_rows<T, DP>(const_cast<T*>(mk), p.kv.dk, dk, p.q.scale, p.q.scale, row, hi, kv, p.kv, lane);
   store_rows<T, DP>(const_cast<T*>(mv), p.kv.dv, dv, 1.f, 1.f, row, hi, kv, p.kv, lane);
   each_bad_row(!ok0, !ok1, row, hi, [&](int j) { again_columns<T>(p, j, kv, lo, hi, lane); });
 }
 
+// 16 first nodes of a chain and the queries behind their windows in one block of the batch: a CTA, whose warps take the steps of all heads in turn and
+// add their sums up in order.
+template <typename T, int DP, int KT> __global__ void __launch_bounds__(THREADS) window_far_kernel(const __grid_constant__ WindowParams p) {
+  using S = attention::Shape<T, DP, 1, KT>;
+  constexpr int LD = S::LD, NT = KT / 8;
+  extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ int64_t chain;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3, kv = blockIdx.y, values = p.q.comps * p.q.size;
+  if (tid == 0) chain = last_chain(p.chains, blockIdx.x, [&](int64_t c) { return p.ptr[c] / FAR_BLOCK + c; });
+  if (values < DP)
+    for (size_t i = tid; i < S::bytes(2, 0) / 16; i += THREADS) reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
+  __syncthreads();
+  if (chain < 0) return;
+  const int lo = (int)p.ptr[chain], hi = (int)p.ptr[chain + 1];
+  const int64_t block = blockIdx.x - chain;
+  const int first = lo + (int)blockIdx.z * FAR_ROWS, last = min(min(lo + p.sinks, hi), first + FAR_ROWS);
+  if (hi <= lo || block > (hi - 1) / FAR_BLOCK || first >= last) return;
+  const int from = max((int)(block * FAR_BLOCK), first + p.before + 1), to = (int)min((block + 1) * FAR_BLOCK, (int64_t)hi);
+  if (from >= to) return;
+  T *keys = reinterpret_cast<T*>(smem) + warp * S::head_elements(2), *vals = keys + 16 * LD, *stage = vals + 16 * LD;
+  float* numbers = reinterpret_cast<float*>(smem + S::bytes(2, 0)) + warp * 6 * KT;
+  const int blocks = (to - from + KT - 1) / KT, steps = blocks * p.group;
+  auto fetch = [&](int step, int s) {
+    const int head = kv * p.group + step / blocks, i = from + step % blocks * KT;
+    load_tile<T, DP, 32, KT>(stage + s * S::STAGE, p.q.q, i, to - i, head, p.q, lane);
+    load_tile<T, DP, 32, KT>(stage + s * S::STAGE + KT * LD, p.q.g, i, to - i, head, p.q, lane);
+    for (int c = lane; c < 3 * KT; c += 32) {
+      const int r = c % KT;
+      const float* x = c < KT ? p.q.top : c < 2 * KT ? p.q.inverse : p.q.delta;
+      const bool there = i + r < to;
+      copy4(numbers + s * 3 * KT + c, x + (there ? (int64_t)head * p.q.n + i + r : 0), there);
+    }
+    copies_commit();
+  };
+  load_tile<T, DP, 32, 16>(keys, p.q.k, first, last - first, kv, p.q, lane);
+  load_tile<T, DP, 32, 16>(vals, p.q.v, first, last - first, kv, p.q, lane);
+  if (warp < steps) fetch(warp, 0);
+  const float unit = p.q.scale * LOG2E;
+  float dk[DP / 8][4], dv[DP / 8][4];
+#pragma unroll
+  for (int n = 0; n < DP / 8; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) dk[n][i] = dv[n][i] = 0.f;
+  for (int step = warp, s = 0; step < steps; step += WARPS, s ^= 1) {
+    if (step + WARPS < steps) {
+      fetch(step + WARPS, s ^ 1);
+      copies_wait<1>();
+    } else {
+      copies_wait<0>();
+    }
+    __syncwarp();
+    const int query = from + step % blocks * KT;
+    const T *qs = stage + s * S::STAGE, *gs = qs + KT * LD;
+    const float* num = numbers + s * 3 * KT;
+    float z[NT][4], dp[NT][4];
+    score_mma<DP, NT, true>(z, keys, qs, lane);
+    score_mma<DP, NT, true>(dp, vals, gs, lane);
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int c = n * 8 + 2 * t + (i & 1), j = first + g + 8 * (i >> 1);
+        const bool on = query + c < to && j < last && query + c > j + p.before;
+        z[n][i] = on ? exp2_fast(z[n][i] * unit - num[c]) * num[KT + c] : 0.f;
+        dp[n][i] = on ? z[n][i] * (dp[n][i] - num[2 * KT + c]) : 0.f;
+      }
+    out_mma<DP, NT>(dv, z, gs, lane);
+    out_mma<DP, NT>(dk, dp, qs, lane);
+    __syncwarp();
+  }
+  copies_wait<0>();
+  float* sums = reinterpret_cast<float*>(smem);          // [dk, dv][node][value], where the tiles were
+  for (int w = 0; w < WARPS; ++w) {
+    __syncthreads();
+    if (warp != w) continue;
+#pragma unroll
+    for (int n = 0; n < DP / 8; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int at = (g + 8 * (i >> 1)) * DP + n * 8 + 2 * t + (i & 1);
+        sums[at] = w ? sums[at] + dk[n][i] : dk[n][i];
+        sums[FAR_ROWS * DP + at] = w ? sums[FAR_ROWS * DP + at] + dv[n][i] : dv[n][i];
+      }
+  }
+  __syncthreads();
+  float* out = p.far + far_place(p, blockIdx.x, kv, blockIdx.z);
+  for (int i = tid; i < 2 * FAR_ROWS * values; i += THREADS) out[i] = sums[i / values * DP + i % values];
+}
+// The blocks of a chain, in their order, into its first one: a thread has one number.
+__global__ void __launch_bounds__(256) window_far_join_kernel(const __grid_constant__ WindowParams p, int groups) {
+  const int64_t chain = blockIdx.x;
+  const int group = blockIdx.z % groups, at = blockIdx.z / groups * 256 + threadIdx.x;
+  const int lo = (int)p.ptr[chain], hi = (int)p.ptr[chain + 1], first = lo + group * FAR_ROWS;
+  if (hi <= lo || first >= lo + p.sinks || first + p.before + 1 >= hi || at >= 2 * FAR_ROWS * p.q.comps * p.q.size) return;
+  const int64_t begin = (first + p.before + 1) / FAR_BLOCK, end = (hi - 1) / FAR_BLOCK;
+  const int64_t step = far_place(p, 1, 0, 0);
+  float* to = p.far + far_place(p, begin + chain, blockIdx.y, group) + at;
+  float sum = 0.f;
+#pragma unroll 16
+  for (int64_t b = 0; b <= end - begin; ++b) sum += to[b * step];
+  *to = sum;
+}
+
 // ---- host side ----------------------------------------------------------------------------------
+template <typename T, int DP> int launch_far(const WindowParams& p, cudaStream_t s) {
+  constexpr int KT = DP > 64 ? 16 : 32;
+  using S = attention::Shape<T, DP, 1, KT>;
+  const int64_t pairs = ceil_div(p.q.n, FAR_BLOCK) + p.chains;
+  if (pairs > INT32_MAX || p.kv.heads > 65535) return fail(EQT_ERR_UNSUPPORTED, "window_attention: %lld chains are more than one launch takes", (long long)p.chains);
+  const size_t shared = S::bytes(2, WARPS * 6 * KT * 4);
+  auto kernel = window_far_kernel<T, DP, KT>;
+  static std::atomic<uint64_t> allowed{0};
+  if (int rc = allow_shared_once(kernel, shared, allowed)) return rc;
+  kernel<<<dim3((unsigned)pairs, (unsigned)p.kv.heads, (unsigned)far_groups(p)), THREADS, shared, s>>>(p);
+  if (int rc = check_launch("window_far")) return rc;
+  const int groups = far_groups(p), chunks = (int)ceil_div(2 * FAR_ROWS * p.q.comps * p.q.size, 256);
+  window_far_join_kernel<<<dim3((unsigned)p.chains, (unsigned)p.kv.heads, (unsigned)(groups * chunks)), 256, 0, s>>>(p, groups);
+  return check_launch("window_far_join");
+}
+template <typename T> int far(const WindowParams& p, cudaStream_t s) {
+  const int values = p.q.comps * p.q.size;
+  return values <= 16 ? launch_far<T, 16>(p, s) : values <= 32 ? launch_far<T, 32>(p, s) : values <= 64 ? launch_far<T, 64>(p, s) : launch_far<T, 128>(p, s);
+}
+
 enum Pass { FORWARD, ROWS, COLUMNS };
 template <typename T, int DP, int WR, int KT, int PASS> int launch(const WindowParams& p, int64_t num_tiles, cudaStream_t s) {
   using S = attention::Shape<T, DP, WR, KT>;
@@ -358,6 +499,8 @@ template <typename T, int PASS> int by_values(const WindowParams& p, int tile_ro
 
 template <typename T> int tiles_backward(const WindowParams& p, int tile_rows, int64_t num_tiles, cudaStream_t s) {
   if (int rc = by_values<T, ROWS>(p, tile_rows, num_tiles, s)) return rc;
+  if (p.split)
+    if (int rc = far<T>(p, s)) return rc;
   return by_values<T, COLUMNS>(p, tile_rows, num_tiles, s);
 }
 

@@ -102,6 +102,19 @@ def test_nodes_of_no_chain(dtype):
         assert not t[:5].any() and not t[85:].any()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(1, 2, 1, 64), (1, 1, 1, 128), (3, 2, 2, 7), (1, 4, 2, 16)])
+@pytest.mark.parametrize("sinks", [1, 4, 20, 64, 65, 700])
+def test_first_nodes_of_long_chains(sinks, shape, dtype):
+    """Queries far behind the window of a chain's first nodes: blocks of the batch that hold several chains, one, and a part of one."""
+    comps, heads, kv_heads, size = shape
+    sizes, window = (3, 1500, 0, 40, 90, 2050, 700), (30, 2, sinks)
+    qkv, g, _ = make(sizes, comps, heads, kv_heads, size, dtype, extra=9)
+    graphs = PackedGraphs(torch.tensor([9] + list(sizes), device=DEV).cumsum(0), sum(sizes) + 9)
+    want, bound = reference(*qkv, g, seen(sizes, sum(sizes) + 9, *window, first=9), heads, kv_heads, None)
+    compare(run(qkv, g, graphs, heads, *window, kv_heads=kv_heads), want, bound)
+
+
 @pytest.mark.parametrize("size", [64, 128])
 def test_many_tiles_at_once(size):
     """Far more tiles than SMs, again and again, so that waits of every length occur: the same bits each time."""
