@@ -76,6 +76,7 @@ int tensor_params(TcParams& t, const eqt_window_attention_args& a, const WindowP
   t.w = p;
   t.spans = static_cast<const int2*>(a.scratch);
   t.status = a.status;
+  t.pack = p.group % 8 == 0 ? 8 : p.group % 4 == 0 ? 4 : p.group % 2 == 0 ? 2 : 1;
   return spans(a.ptr, a.num_graphs, static_cast<int2*>(a.scratch), a.n, s);
 }
 

@@ -42,7 +42,7 @@ template <int DP, int MODE> struct Form {
   static constexpr int SOFT = 4 * GROUPS, THREADS = 32 * (SOFT + 2) + LOADERS, CTAS = GROUPS == 2 ? 1 : 2;
   static constexpr int OWN = MODE == FORWARD ? 1 : 2;                                // operands of the tile's rows
   static constexpr int OWN_BYTES = TILE_M * DP * 2, SLOT_BYTES = KEYS * DP * 2;
-  static constexpr int SLOTS = MODE == FORWARD ? (DP == 128 ? 4 : 8) : MODE == ROWS ? (DP == 128 ? 3 : 6) : 8;
+  static constexpr int SLOTS = MODE == FORWARD && DP == 128 ? 4 : MODE == ROWS && DP == 128 ? 3 : 8;
   static constexpr int NUMBERS = MODE == COLUMNS ? SLOTS / 2 * 3 * KEYS * 4 : 0;     // bytes: a query's greatest score, inverse sum, delta
   static constexpr int BUFFER = MODE == FORWARD ? KEYS : 2 * KEYS;                   // columns of tensor memory: S, or S and dP
   static constexpr int SUM_AT = BUFFERS * BUFFER, COLS = GROUPS == 2 ? 512 : 256;
@@ -72,26 +72,50 @@ template <int DP> struct Copier {
       from[g] = static_cast<const T*>(x.p) + comp * x.comp + (on[g] ? at - comp * p.size : 0) + row * node;
     }
   }
-  // rows [first, first + ROWS) of a head, zeros from the `left`-th on
-  template <int ROWS_> __device__ __forceinline__ void rows(unsigned char* dst, int first, int left, int head) const {
+  // KEYS rows of a head from `first` on, zeros from the `left`-th on
+  __device__ __forceinline__ void next(unsigned char* dst, int first, int left, int head) const {
     const int64_t move = first * node + (int64_t)head * size, step = 8 * node;
+    const T* f[GROUPS];
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) f[g] = from[g] + move;
+    uint32_t d = s32(dst) + to;
+#pragma unroll 2
+    for (int r = row; r < KEYS; r += 8, d += 1024) {
+#pragma unroll
+      for (int g = 0; g < GROUPS; ++g, f[g - 1] += step)
+        if (there[g]) copy(d + g * (KEYS * 128), f[g], g, on[g] && r < left);
+    }
+  }
+  // the same of a stretch that begins with `ns` rows from `from0` on and goes on at `from1`, from its `at`-th row on
+  __device__ __forceinline__ void mixed(unsigned char* dst, int at, int ns, int from0, int from1, int left, int head) const {
 #pragma unroll
     for (int g = 0; g < GROUPS; ++g) {
       if (!there[g]) continue;
-      const T* f = from[g] + move;
-      const uint32_t d = s32(dst) + to + g * (ROWS_ * 128);
-      if (left >= ROWS_ && on[g]) {
-#pragma unroll
-        for (int r = 0; r < ROWS_ / 8; ++r, f += step)
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d + r * 1024), "l"(f) : "memory");
-      } else {
-#pragma unroll
-        for (int r = 0; r < ROWS_ / 8; ++r, f += step) {
-          const bool in = on[g] && 8 * r + row < left;
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d + r * 1024), "l"(in ? f : from[g]), "r"(in ? 16 : 0) : "memory");
-        }
+      const uint32_t d = s32(dst) + to + g * (KEYS * 128);
+#pragma unroll 1
+      for (int r = 0; r < KEYS; r += 8) {
+        const int v = at + r + row, first = (v < ns ? from0 + v : from1 + v - ns) - row;
+        copy(d + r * 128, from[g] + first * node + (int64_t)head * size, g, on[g] && r + row < left);
       }
     }
+  }
+  // the tile's own: `high` rows of one head after the other
+  __device__ __forceinline__ void own(unsigned char* dst, int first, int left, int head, int high) const {
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) {
+      if (!there[g]) continue;
+      const uint32_t d = s32(dst) + to + g * (TILE_M * 128);
+      const T* f = from[g] + first * node + (int64_t)head * size;
+      int q = 0;
+#pragma unroll 2
+      for (int r = 0; r < TILE_M; r += 8) {
+        copy(d + r * 128, f + q * node, g, on[g] && q + row < left);
+        if ((q += 8) == high) q = 0, f += size;
+      }
+    }
+  }
+  __device__ __forceinline__ void copy(uint32_t d, const T* f, int g, bool in) const {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(in ? f : from[g]), "r"(in ? 16 : 0) : "memory");
   }
 };
 
@@ -107,20 +131,16 @@ __device__ __forceinline__ uint64_t bits_of(int lo, int hi) {
   return hi > lo ? (~uint64_t(0) >> (64 - (hi - lo))) << lo : 0;
 }
 
-// What a tile walks over.
+// What a tile walks over: `ns` first nodes of the chain that its first row is in, from `from0` on, then [from1, to1), as one sequence.
 struct Stretch {
-  int from0, to0, steps0, from1, to1, steps;
-  __device__ __forceinline__ int at(int step, int& end) const {
-    const bool second = step >= steps0;
-    end = second ? to1 : to0;
-    return second ? from1 + (step - steps0) * KEYS : from0 + step * KEYS;
-  }
+  int from0, ns, from1, to1, total, steps;
 };
 template <int MODE> __device__ __forceinline__ Stretch stretch_of(const TcParams& p, int first, int last) {       // rows first to last
   const WindowParams& w = p.w;
   const int2 a = p.spans[first], b = p.spans[last];
   Stretch s;
-  s.from0 = s.to0 = s.from1 = first;
+  s.from0 = s.from1 = first;
+  s.ns = 0;
   s.to1 = last + 1;
   if (MODE == COLUMNS) {
     if (a.y > a.x) s.from1 = max(a.x, first - w.after);
@@ -129,12 +149,12 @@ template <int MODE> __device__ __forceinline__ Stretch stretch_of(const TcParams
     if (a.y > a.x) {
       s.from1 = max(a.x, first - w.before);
       s.from0 = a.x;
-      s.to0 = min(s.from1, a.x + w.sinks);
+      s.ns = min(s.from1, a.x + w.sinks) - a.x;
     }
     if (b.y > b.x) s.to1 = min(b.y, last + w.after + 1);
   }
-  s.steps0 = max(0, (s.to0 - s.from0 + KEYS - 1) / KEYS);
-  s.steps = s.steps0 + max(0, (s.to1 - s.from1 + KEYS - 1) / KEYS);
+  s.total = s.ns + s.to1 - s.from1;
+  s.steps = (s.total + KEYS - 1) / KEYS;
   return s;
 }
 
@@ -184,16 +204,17 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
   unsigned char *own = smem, *ring = own + F::OWN * F::OWN_BYTES;
   float* numbers = reinterpret_cast<float*>(ring + SLOTS * F::SLOT_BYTES);
   uint64_t* bars = reinterpret_cast<uint64_t*>(ring + SLOTS * F::SLOT_BYTES + F::NUMBERS);
-  uint64_t *full = bars, *empty = full + SLOTS, *own_full = empty + SLOTS, *scores = own_full + 1, *weights = scores + BUFFERS, *freed = weights + BUFFERS, *done = freed + BUFFERS;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  uint64_t *full = bars, *empty = full + SLOTS, *own_full = empty + SLOTS, *scores = own_full + 1, *weights = scores + BUFFERS, *freed = weights + BUFFERS, *done = freed + BUFFERS, *gathered = done + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gathered + 1);
   int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
-  static_assert((2 * SLOTS + 2 + 3 * BUFFERS) * 8 + 8 <= 512, "barriers");
+  static_assert((2 * SLOTS + 3 + 3 * BUFFERS) * 8 + 8 <= 512, "barriers");
 
   const WindowParams& w = p.w;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int heads = MODE == COLUMNS ? w.kv.heads : w.q.heads;
-  const int head = (int)(blockIdx.x % (unsigned)heads), kv = MODE == COLUMNS ? head : head / w.group;
-  const int first = (int)(blockIdx.x / (unsigned)heads) * TILE_M, last = min((int)w.q.n, first + TILE_M) - 1;
+  // A tile is `pack` heads that share their keys by `high` nodes: with fewer nodes, the walk over what any of them sees is shorter.
+  const int pack = MODE == COLUMNS ? 1 : p.pack, high = TILE_M / pack, heads = (MODE == COLUMNS ? w.kv.heads : w.q.heads) / pack;
+  const int head = (int)(blockIdx.x % (unsigned)heads) * pack, kv = MODE == COLUMNS ? head : head / w.group;
+  const int first = (int)(blockIdx.x / (unsigned)heads) * high, last = min((int)w.q.n, first + high) - 1;
   const Stretch walk = stretch_of<MODE>(p, first, last);
   const int steps = walk.steps * (MODE == COLUMNS ? w.group : 1);
   const int values = w.q.comps * w.q.size, wide = (values + 15) / 16 * 16;
@@ -201,16 +222,17 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
   if (tid == 0) {
     *abort_flag = (s32(smem) & 1023) != 0;                // the swizzle goes by addresses
     for (int s = 0; s < SLOTS; ++s) {
-      bar_init(&full[s], LOADERS);
+      bar_init(&full[s], !p.tma ? LOADERS : MODE == COLUMNS && !(s & 1) ? LOADERS + 1 : 1);
       bar_init(&empty[s], 1);
     }
-    bar_init(own_full, LOADERS);
+    bar_init(own_full, p.tma ? 1 : LOADERS);
     for (int b = 0; b < BUFFERS; ++b) {
       bar_init(&scores[b], 1);
       bar_init(&weights[b], 4);
       bar_init(&freed[b], 1);
     }
     bar_init(done, 1);                                   // all products
+    bar_init(gathered, LOADERS);                         // a mixed item where others are copied by TMA
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == F::SOFT) {
@@ -223,43 +245,65 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
   const uint32_t tmem = *tmem_slot;
   volatile int* ab = abort_flag;
 
-  if (warp > F::SOFT + 1) {
+  if (warp >= F::SOFT + 2) {
     // ---------------- copies ----------------
-    // Items in the order of their use: FORWARD k, v; ROWS v, k; COLUMNS q with its numbers, g.  A thread's copies arrive at the item's barrier when they
-    // have landed; the thread that issues the MMAs, which sees them all there, puts the fence between them and the tensor cores.
+    // Items in the order of their use: FORWARD k, v; ROWS v, k; COLUMNS q with its numbers, g.  Heads of 64 or 128 values in one component are
+    // copied by one thread (TMA); a stretch's first nodes, and all of other heads, by the threads: their copies arrive at the item's barrier when they have landed, and
+    // the thread that issues the MMAs, which sees them all there, puts the fence between them and the tensor cores.  Copying by hand takes the warps
+    // issue slots that the softmax wants (one chain of 32,781 nodes, 8 heads of 128 values, by hand and by TMA: HAND | TMA us).
     const int thread = tid - 32 * (F::SOFT + 2);
     const int left = last + 1 - first;
     const Copier<DP> even(MODE == FORWARD ? w.q.k : MODE == ROWS ? w.q.v : w.q.q, w.q, thread);
     const Copier<DP> odd(MODE == FORWARD ? w.q.v : MODE == ROWS ? w.q.k : w.q.g, w.q, thread);
-    Copier<DP>(MODE == COLUMNS ? w.q.k : w.q.q, w.q, thread).template rows<TILE_M>(own, first, left, head);
-    if (MODE != FORWARD) Copier<DP>(MODE == COLUMNS ? w.q.v : w.q.g, w.q, thread).template rows<TILE_M>(own + F::OWN_BYTES, first, left, head);
-    land_at(own_full);
-    bool ok = true;
-    for (int item = 0; item < 2 * steps && ok; ++item) {
-      const int slot = item % SLOTS, step = item >> 1;
-      if (item >= SLOTS) {
-        ok = __all_sync(0xffffffffu, bar_wait(&empty[slot], (uint32_t)((item / SLOTS - 1) & 1), ab));
-        if (!ok) break;
+    if (!p.tma) {
+      Copier<DP>(MODE == COLUMNS ? w.q.k : w.q.q, w.q, thread).own(own, first, left, head, high);
+      if (MODE != FORWARD) Copier<DP>(MODE == COLUMNS ? w.q.v : w.q.g, w.q, thread).own(own + F::OWN_BYTES, first, left, head, high);
+      land_at(own_full);
+    } else if (thread == 0) {
+      bar_expect_tx(own_full, F::OWN * F::OWN_BYTES);
+      for (int x = 0; x < F::OWN; ++x)
+        for (int h = 0; h < pack; ++h)
+          for (int g = 0; g < DP / 64; ++g)
+            tma_load_3d(own + x * F::OWN_BYTES + g * (TILE_M * 128) + h * high * 128, &p.own[x], (head + h) * DP + g * 64, first, 0, own_full);
+    }
+    int at = 0, h = MODE == COLUMNS ? kv * w.group : kv;
+    for (int item = 0; item < 2 * steps; ++item) {
+      const int slot = item % SLOTS;
+      const bool mixed = MODE != COLUMNS && at < walk.ns, numbered = MODE == COLUMNS && !(item & 1);
+      if (!p.tma || mixed || numbered || thread == 0) {  // the others have nothing to do with tiles that are copied whole
+        if (item >= SLOTS && !bar_wait(&empty[slot], (uint32_t)((item / SLOTS - 1) & 1), ab)) break;
+        unsigned char* to = ring + slot * F::SLOT_BYTES;
+        const Copier<DP>& x = item & 1 ? odd : even;
+        if (mixed) {
+          x.mixed(to, at, walk.ns, walk.from0, walk.from1, walk.total - at, h);
+          if (p.tma) {                                   // one arrival for all, none of whom is an item ahead
+            land_at(gathered);
+            if (!bar_wait(gathered, (uint32_t)(item & 1), ab)) break;
+            if (thread == 0) bar_arrive(&full[slot]);
+          }
+        } else if (!p.tma) {
+          x.next(to, walk.from1 + at - walk.ns, walk.total - at, h);
+        } else if (thread == 0) {
+          bar_expect_tx(&full[slot], F::SLOT_BYTES);
+          for (int g = 0; g < DP / 64; ++g) tma_load_3d(to + g * (KEYS * 128), &p.ring[item & 1], h * DP + g * 64, walk.from1 + at - walk.ns, 0, &full[slot]);
+        }
+        if (numbered) {
+          const int i = walk.from1 + at + thread;
+          const bool there = i < walk.to1;
+          const int64_t from = there ? (int64_t)h * w.q.n + i : 0;
+          float* num = numbers + slot / 2 * 3 * KEYS + thread;
+          copy4(num, w.q.top + from, there);
+          copy4(num + KEYS, w.q.inverse + from, there);
+          copy4(num + 2 * KEYS, w.q.delta + from, there);
+        }
+        if (!p.tma || numbered) land_at(&full[slot]);
       }
-      int end;
-      const int at = walk.at(MODE == COLUMNS ? step % walk.steps : step, end);
-      unsigned char* to = ring + slot * F::SLOT_BYTES;
-      const int h = MODE == COLUMNS ? kv * w.group + step / walk.steps : kv;
-      (item & 1 ? odd : even).template rows<KEYS>(to, at, end - at, h);
-      if (MODE == COLUMNS && !(item & 1)) {
-        const bool there = at + thread < end;
-        const int64_t from = there ? (int64_t)h * w.q.n + at + thread : 0;
-        float* num = numbers + slot / 2 * 3 * KEYS + thread;
-        copy4(num, w.q.top + from, there);
-        copy4(num + KEYS, w.q.inverse + from, there);
-        copy4(num + 2 * KEYS, w.q.delta + from, there);
-      }
-      land_at(&full[slot]);
+      if ((item & 1) && (at += KEYS) >= walk.total) at = 0, ++h;         // COLUMNS: the next head
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
   } else if (warp >= F::SOFT) {
     // ---------------- MMAs ----------------
-    // One thread makes scores, another adds weighted rows up: each MMA costs its thread some sixty cycles whatever its size, and a step has up to 24.
+    // One thread makes S and dP, another adds weighted rows up: each MMA costs its thread some ninety cycles whatever its size, and a step has up to 24.
     if (lane == 0) {
       const uint32_t to_scores = idesc_bf16(TILE_M, KEYS), to_sums = idesc_bf16(TILE_M, wide, false, true);
       const uint32_t own_at = s32(own), ring_at = s32(ring), sum = tmem + F::SUM_AT;
@@ -287,33 +331,31 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
         for (int k = 1; k < KEYS / 16; ++k) umma_bf16_ta<true>(d, a + k * 8, b_lo + k * ROWS_STEP, to_sums);
       };
       bool ok = true;
+      constexpr int S_ITEM = MODE == ROWS ? 1 : 0;
+      auto make_s = [&](int j) {
+        ok = ok && arrived(2 * j + S_ITEM) && free_again(j);
+        if (!ok) return;
+        fence();
+        tc_fence_after();
+        score(tmem + (j % BUFFERS) * F::BUFFER, own_at, slot_at(2 * j + S_ITEM));
+        if (MODE == FORWARD) umma_commit(&empty[2 * j % SLOTS]);
+      };
+      // By rows, the place of dP is free when the softmax has read it.
+      auto make_dp = [&](int j) {
+        ok = ok && arrived(2 * j + 1 - S_ITEM) && (MODE == COLUMNS || j < BUFFERS || weighted(j - BUFFERS));
+        if (!ok) return;
+        fence();
+        tc_fence_after();
+        score(tmem + (j % BUFFERS) * F::BUFFER + KEYS, own_at + F::OWN_BYTES, slot_at(2 * j + 1 - S_ITEM));
+        if (MODE == ROWS) umma_commit(&empty[2 * j % SLOTS]);
+      };
       if (warp == F::SOFT) {
         ok = bar_wait(own_full, 0, ab);
         for (int j = 0; j < steps && ok; ++j) {
-          const uint32_t d = tmem + (j % BUFFERS) * F::BUFFER;
-          if (MODE == ROWS) {
-            // dP's place is free when the softmax has read it, that of S when dS has been used
-            ok = arrived(2 * j) && (j == 0 || weighted(j - 1));
-            if (!ok) break;
-            fence();
-            tc_fence_after();
-            score(d + KEYS, own_at + F::OWN_BYTES, slot_at(2 * j));
-            umma_commit(&empty[2 * j % SLOTS]);
-            ok = arrived(2 * j + 1) && free_again(j);
-            if (!ok) break;
-            fence();
-            tc_fence_after();
-            score(d, own_at, slot_at(2 * j + 1));
-          } else {
-            ok = arrived(2 * j) && (MODE == FORWARD || arrived(2 * j + 1)) && free_again(j);
-            if (!ok) break;
-            fence();
-            tc_fence_after();
-            score(d, own_at, slot_at(2 * j));
-            if (MODE == FORWARD) umma_commit(&empty[2 * j % SLOTS]);
-            else score(d + KEYS, own_at + F::OWN_BYTES, slot_at(2 * j + 1));
-          }
-          umma_commit(&scores[j % BUFFERS]);
+          if (MODE == ROWS) make_dp(j);
+          make_s(j);
+          if (MODE == COLUMNS) make_dp(j);
+          if (ok) umma_commit(&scores[j % BUFFERS]);
         }
       } else {
         for (int j = 0; j < steps && ok; ++j) {
@@ -338,7 +380,7 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
     }
   } else {
     // ---------------- softmax ----------------
-    const int quarter = warp & 3, row = first + quarter * 32 + lane;
+    const int quarter = warp & 3, group = warp >> 2, place = quarter * 32 + lane, row = first + place % high, mine = head + place / high;       // its head
     const bool there = row <= last;
     const int2 span = there ? p.spans[row] : make_int2(0, 0);
     const bool on = span.y > span.x;
@@ -349,9 +391,14 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
     const int hi = !on ? 0 : MODE == COLUMNS ? (!w.split && row < span.x + w.sinks ? span.y : min(span.y, row + w.before + 1)) : min(span.y, row + w.after + 1);
     const int far = on && MODE != COLUMNS ? min(lo, span.x + w.sinks) : 0;
     bool ok = true;
-    auto seen = [&](int at, int end) {
-      uint64_t bits = bits_of(lo - at, min(hi, end) - at);
-      if (MODE != COLUMNS) bits |= bits_of(span.x - at, min(far, end) - at);
+    // as bits of the 64 from the stretch's `at`-th on; first nodes are before `from1`, or in the stretch behind it, or both
+    auto seen = [&](int at) {
+      const int shift = walk.from1 - walk.ns + at;
+      uint64_t bits = bits_of(lo - shift, hi - shift);
+      if (MODE != COLUMNS) {
+        bits |= bits_of(max(span.x, walk.from1) - shift, far - shift);
+        if (at < walk.ns && span.x < walk.from1) bits |= bits_of(span.x - walk.from0 - at, min(far - walk.from0, walk.ns) - at);
+      }
       return bits;
     };
     if (MODE == FORWARD) {
@@ -365,9 +412,7 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
         uint32_t raw[2][32];
         tmem_issue32(s_at, raw[0]);
         tmem_issue32(s_at + 32, raw[1]);
-        int end;
-        const int at = walk.at(j, end);
-        const uint64_t bits = seen(at, end);
+        const uint64_t bits = seen(j * KEYS);
         tmem_arrived32(raw[0]);
         tmem_arrived32(raw[1]);
         if (!__all_sync(0xffffffffu, bits == ~uint64_t(0))) {
@@ -424,21 +469,21 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
       if (ok && steps) {
         tc_fence_after();
         const float inverse = 1.f / total;
-        const bool finite = put_row<DP>(sum_at, inverse, on, w.q.out, row, head, w.q);
-        if (on && w.q.top) w.q.top[(int64_t)head * w.q.n + row] = base, w.q.inverse[(int64_t)head * w.q.n + row] = inverse;
+        const bool finite = put_row<DP>(sum_at, inverse, on, w.q.out, row, mine, w.q);
+        if (on && w.q.top) w.q.top[(int64_t)mine * w.q.n + row] = base, w.q.inverse[(int64_t)mine * w.q.n + row] = inverse;
         __syncwarp();
         for (unsigned bad = __ballot_sync(0xffffffffu, on && !finite); bad; bad &= bad - 1) {
           const int r = __ffs(bad) - 1;
-          again_forward<T>(w, row - lane + r, head, __shfl_sync(0xffffffffu, span.x, r), __shfl_sync(0xffffffffu, span.y, r), lane);
+          again_forward<T>(w, __shfl_sync(0xffffffffu, row, r), __shfl_sync(0xffffffffu, mine, r), __shfl_sync(0xffffffffu, span.x, r), __shfl_sync(0xffffffffu, span.y, r), lane);
         }
       }
     } else if (MODE == ROWS) {
-      const int64_t number = (int64_t)head * w.q.n + row;
+      const int64_t number = (int64_t)mine * w.q.n + row;
       float top = INFINITY, inverse = 0.f, delta = 0.f;
       if (on) {
         top = w.q.top[number];
         inverse = w.q.inverse[number];
-        const int64_t at = ((int64_t)row * w.q.comps * w.q.heads + head) * w.q.size;
+        const int64_t at = ((int64_t)row * w.q.comps * w.q.heads + mine) * w.q.size;
         for (int e = 0; e < values; e += 8) {
           const int comp = e / w.q.size;
           const int64_t place = at + (int64_t)comp * w.q.heads * w.q.size + e - comp * w.q.size;
@@ -450,24 +495,24 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
             delta = fmaf(__uint_as_float(x[i] & 0xffff0000u), __uint_as_float(y[i] & 0xffff0000u), delta);
           }
         }
-        w.q.delta[number] = delta;
+        if (group == 0) w.q.delta[number] = delta;
       }
-      for (int j = 0; j < steps; ++j) {
-        ok = bar_wait(&scores[0], (uint32_t)(j & 1), ab);
+      for (int j = group; j < steps; j += GROUPS) {
+        const int b = j % BUFFERS;
+        ok = bar_wait(&scores[b], (uint32_t)((j / BUFFERS) & 1), ab);
         if (!__all_sync(0xffffffffu, ok)) break;
         tc_fence_after();
-        int end;
-        const int at = walk.at(j, end);
-        const uint64_t bits = seen(at, end);
+        const uint64_t bits = seen(j * KEYS);
         const bool all = __all_sync(0xffffffffu, bits == ~uint64_t(0));
-        uint32_t s[2][32], d[32], high[16], low[16];
-        tmem_issue32(lanes, s[0]);
-        tmem_issue32(lanes + 32, s[1]);
+        uint32_t s[2][32], d[32], large[16], small[16];
+        const uint32_t s_at = lanes + b * F::BUFFER;
+        tmem_issue32(s_at, s[0]);
+        tmem_issue32(s_at + 32, s[1]);
         tmem_arrived32(s[0]);
         tmem_arrived32(s[1]);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          tmem_issue32(lanes + KEYS + 32 * h, d);
+          tmem_issue32(s_at + KEYS + 32 * h, d);
           tmem_arrived32(d);
           const uint32_t word = (uint32_t)(bits >> (32 * h));
 #pragma unroll
@@ -479,42 +524,42 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
               if (!all) x[i] = (word >> (c + i)) & 1 ? x[i] : 0.f;
             }
             const uint32_t two = two_bf16(x[0], x[1]);
-            high[c / 2] = two;
-            low[c / 2] = two_bf16(x[0] - __uint_as_float(two << 16), x[1] - __uint_as_float(two & 0xffff0000u));
+            large[c / 2] = two;
+            small[c / 2] = two_bf16(x[0] - __uint_as_float(two << 16), x[1] - __uint_as_float(two & 0xffff0000u));
           }
-          tmem_put16(lanes + 16 * h, high);
-          tmem_put16(lanes + 32 + 16 * h, low);
+          tmem_put16(s_at + 16 * h, large);
+          tmem_put16(s_at + 32 + 16 * h, small);
         }
         tmem_stored();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) bar_arrive(&weights[0]);
+        if (lane == 0) bar_arrive(&weights[b]);
       }
       ok = __all_sync(0xffffffffu, ok);
       if (ok && steps) ok = __all_sync(0xffffffffu, bar_wait(done, 0, ab));
-      if (ok && steps) {
+      if (ok && steps && group == 0) {
         tc_fence_after();
-        const bool finite = put_row<DP>(sum_at, w.q.scale, on, w.q.dq, row, head, w.q);
+        const bool finite = put_row<DP>(sum_at, w.q.scale, on, w.q.dq, row, mine, w.q);
+
         __syncwarp();
         for (unsigned bad = __ballot_sync(0xffffffffu, on && !finite); bad; bad &= bad - 1) {
           const int r = __ffs(bad) - 1;
-          again_rows<T>(w, row - lane + r, head, __shfl_sync(0xffffffffu, span.x, r), __shfl_sync(0xffffffffu, span.y, r), lane);
+          again_rows<T>(w, __shfl_sync(0xffffffffu, row, r), __shfl_sync(0xffffffffu, mine, r), __shfl_sync(0xffffffffu, span.x, r), __shfl_sync(0xffffffffu, span.y, r), lane);
         }
       }
     } else {
-      const int group = warp >> 2;
+      int at = group % walk.steps * KEYS;
       for (int j = group; j < steps; j += GROUPS) {
         const int b = j % BUFFERS, slot = 2 * j % SLOTS;
         ok = bar_wait(&full[slot], (uint32_t)((2 * j / SLOTS) & 1), ab) && bar_wait(&scores[b], (uint32_t)((j / BUFFERS) & 1), ab);
         if (!__all_sync(0xffffffffu, ok)) break;
         tc_fence_after();
-        int end;
-        const int at = walk.at(j % walk.steps, end);
-        const uint64_t bits = seen(at, end);
+        const uint64_t bits = seen(at);
+        for (at += GROUPS * KEYS; at >= walk.steps * KEYS;) at -= walk.steps * KEYS;
         const bool all = __all_sync(0xffffffffu, bits == ~uint64_t(0));
         const float* num = numbers + slot / 2 * 3 * KEYS;
         const uint32_t s_at = lanes + b * F::BUFFER;
-#pragma unroll
+#pragma unroll 1
         for (int h = 0; h < 2; ++h) {
           uint32_t s[32], d[32], pt[16], dst[16];
           tmem_issue32(s_at + 32 * h, s);
@@ -571,7 +616,12 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
 
   tc_fence_before();
   __syncthreads();
-  if (tid == 0 && *abort_flag) atomicExch(p.status, 2);
+  if (tid == 0 && *abort_flag) {
+    atomicExch(p.status, 2);
+    let_copies_land(full, SLOTS);
+    let_copies_land(own_full, 1);
+  }
+  __syncthreads();
   if (warp == F::SOFT) {
     __syncwarp();
     tc_fence_after();
@@ -595,12 +645,29 @@ __global__ void __launch_bounds__(256) spans_kernel(const int64_t* __restrict__ 
 
 template <int DP, int MODE> int launch(const TcParams& p, cudaStream_t s) {
   using F = Form<DP, MODE>;
-  const int64_t grid = ceil_div(p.w.q.n, TILE_M) * (MODE == COLUMNS ? p.w.kv.heads : p.w.q.heads);
+  const int64_t grid = MODE == COLUMNS ? ceil_div(p.w.q.n, TILE_M) * p.w.kv.heads : ceil_div(p.w.q.n, TILE_M / p.pack) * (p.w.q.heads / p.pack);
   if (grid > INT32_MAX) return fail(EQT_ERR_UNSUPPORTED, "window_attention: %lld tiles are more than one launch takes", (long long)grid);
+  TcParams t = p;
+  const int64_t width = (int64_t)p.w.q.heads * DP, kv_width = (int64_t)p.w.kv.heads * DP;
+  t.tma = p.w.q.comps == 1 && p.w.q.size == DP && p.w.q.q.node >= width && p.w.q.k.node >= kv_width && p.w.q.v.node >= kv_width;
+  if (t.tma) {
+    const AttentionParams& q = p.w.q;
+    auto map = [&](CUtensorMap* m, const Operand& x, int heads, int lines) { return map_bf16(m, x.p, q.n, (int64_t)heads * DP, x.node, x.node, 1, lines); };
+    const int kv_heads = p.w.kv.heads, high = TILE_M / p.pack;
+    int rc;
+    if (MODE == COLUMNS) {
+      (void)((rc = map(&t.own[0], q.k, kv_heads, TILE_M)) || (rc = map(&t.own[1], q.v, kv_heads, TILE_M)) || (rc = map(&t.ring[0], q.q, q.heads, KEYS)) ||
+             (rc = map(&t.ring[1], q.g, q.heads, KEYS)));
+    } else {
+      (void)((rc = map(&t.own[0], q.q, q.heads, high)) || (MODE == ROWS && (rc = map(&t.own[1], q.g, q.heads, high))) ||
+             (rc = map(&t.ring[MODE == ROWS], q.k, kv_heads, KEYS)) || (rc = map(&t.ring[MODE == FORWARD], q.v, kv_heads, KEYS)));
+    }
+    if (rc) return rc;
+  }
   auto kernel = window_tc_kernel<DP, MODE>;
   static std::atomic<uint64_t> allowed{0};
   if (int rc = allow_shared_once(kernel, F::bytes(), allowed)) return rc;
-  kernel<<<(unsigned)grid, F::THREADS, F::bytes(), s>>>(p);
+  kernel<<<(unsigned)grid, F::THREADS, F::bytes(), s>>>(t);
   return check_launch("window_tc");
 }
 
