@@ -14,7 +14,7 @@
 // G of a piece is at most PIECE_BYTES, so scratch does not grow with the table; a piece has a whole number of waves of WEIGHT's tiles.  Sums that
 // would leave SMs idle are cut into parts, float32 partial results that one kernel adds in their order.  Floor: 8 n t c flops for both passes.
 //
-// A CTA per SM; warp 0 copies tiles (TMA), warp 1 issues the MMAs, the other eight are the epilogue.  A k-block is 64
+// A CTA per SM; warp 0 copies tiles (TMA), warp 1 issues the MMAs, the other eight (float32: sixteen) are the epilogue.  A k-block is 64
 // values of k; operands lie along k or along the rows, as they are in memory.  bfloat16: tiles of 128 x 256, four stages of 48 KB, two sums of 256 columns in tensor memory.
 // float32: operands are split once into three bfloat16 parts (24 bits), six products of which leave 2^-26 of a term; a stage has all parts of
 // both operands, 96 KB for 128 x 128 results, and products with small parts have a sum of their own, so that the truncation of the tensor cores' adder counts once every
@@ -33,18 +33,19 @@ namespace {
 using namespace tc;
 
 enum Mode { LOGITS, SCORES, INPUT, WEIGHT };
-constexpr int BK = 64, EPI = 8;                          // k of a block; warps of the epilogue
+constexpr int BK = 64;                                   // k of a block
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int64_t PIECE_BYTES = int64_t(256) << 20, MOST_TERMS = 16384;
 
 template <int PARTS> constexpr int cols() { return PARTS == 1 ? 256 : 128; }             // of a tile
-template <int PARTS> constexpr int share() { return cols<PARTS>() / 2; }                 // of a tile's columns, that a thread of the epilogue has
-constexpr int THREADS = 32 * (2 + EPI);
+template <int PARTS> constexpr int epilogue_warps() { return PARTS == 1 ? 8 : 16; }
+template <int PARTS> constexpr int share() { return 4 * cols<PARTS>() / epilogue_warps<PARTS>(); }     // of a tile's columns, that a thread of the epilogue has
+template <int PARTS> constexpr int threads() { return 32 * (2 + epilogue_warps<PARTS>()); }
 template <int PARTS> constexpr int a_bytes() { return PARTS * TILE_M * BK * 2; }
 template <int PARTS> constexpr int stage_bytes() { return a_bytes<PARTS>() + PARTS * cols<PARTS>() * BK * 2; }
 constexpr int PATCH = 2048;                              // a warp's: 32 rows of 64 bytes
-template <int PARTS> constexpr int stages() { return (232448 - 1024 - EPI * PATCH - 1024) / stage_bytes<PARTS>(); }
-template <int PARTS> constexpr size_t shared_bytes() { return 1024 + (size_t)stages<PARTS>() * stage_bytes<PARTS>() + EPI * PATCH; }
+template <int PARTS> constexpr int stages() { return (232448 - 1024 - epilogue_warps<PARTS>() * PATCH - 1024) / stage_bytes<PARTS>(); }
+template <int PARTS> constexpr size_t shared_bytes() { return 1024 + (size_t)stages<PARTS>() * stage_bytes<PARTS>() + epilogue_warps<PARTS>() * PATCH; }
 
 struct alignas(64) Launch {
   CUtensorMap a, b;
@@ -65,7 +66,7 @@ struct alignas(64) Launch {
   int* status;
 };
 
-__host__ __device__ inline int shares_of(int width, int share) { return width > share ? 2 : 1; }
+__host__ __device__ inline int shares_of(int width, int share) { return (width + share - 1) / share; }
 
 struct Item {
   int64_t row;
@@ -128,7 +129,7 @@ template <typename T> __device__ __forceinline__ void store_block(unsigned char*
   }
 }
 
-template <int PARTS, int MODE> __global__ void __launch_bounds__(THREADS, 1) loss_kernel(const __grid_constant__ Launch p) {
+template <int PARTS, int MODE> __global__ void __launch_bounds__(threads<PARTS>(), 1) loss_kernel(const __grid_constant__ Launch p) {
   constexpr bool F32 = PARTS == 3, A_TURNED = MODE == WEIGHT, B_TURNED = MODE == INPUT || MODE == WEIGHT;
   constexpr int STAGES = stages<PARTS>(), STAGE = stage_bytes<PARTS>(), COLS = cols<PARTS>();
   static_assert(STAGES >= 2, "two stages at least");
@@ -146,7 +147,7 @@ template <int PARTS, int MODE> __global__ void __launch_bounds__(THREADS, 1) los
     }
     for (int a = 0; a < 2; ++a) {
       bar_init(&acc_full[a], 1);
-      bar_init(&acc_empty[a], EPI);
+      bar_init(&acc_empty[a], epilogue_warps<PARTS>());
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -243,12 +244,12 @@ template <int PARTS, int MODE> __global__ void __launch_bounds__(THREADS, 1) los
     }
   } else {
     // ---------------- epilogue ----------------
-    // Warps of the same quarter of the lanes have half of a tile's columns each, 32 at a time.
+    // Warps of the same quarter of the lanes have a share of a tile's columns each, 32 at a time.
     constexpr int SHARE = share<PARTS>();
-    const int e = warp - 2, quarter = warp & 3, half = e >> 2;
+    const int e = warp - 2, quarter = warp & 3, part_of = e >> 2;
     unsigned char* patch = ring + (size_t)STAGES * STAGE + (size_t)e * PATCH;
-    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * SHARE);
-    const int mine = max(0, min(SHARE, p.width - half * SHARE));                         // columns of a narrow tile may be none
+    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(part_of * SHARE);
+    const int mine = max(0, min(SHARE, p.width - part_of * SHARE));                         // columns of a narrow tile may be none
     int piece = 0;
     bool ok = true;
     for (unsigned i = blockIdx.x; i < p.items && ok && !*ab; i += gridDim.x) {
@@ -323,7 +324,7 @@ template <int PARTS, int MODE> __global__ void __launch_bounds__(THREADS, 1) los
         }
       };
       for (int tile = t.tile0; tile < t.tile1 && ok; ++tile) {
-        const int col = tile * p.width + half * SHARE, valid = min(p.columns, (tile + 1) * p.width) - col;
+        const int col = tile * p.width + part_of * SHARE, valid = min(p.columns, (tile + 1) * p.width) - col;
         auto release = [&](int a) {
           tc_fence_before();
           __syncwarp();
@@ -382,7 +383,7 @@ template <int PARTS, int MODE> __global__ void __launch_bounds__(THREADS, 1) los
         }
       }
       if (MODE == LOGITS && ok && there && mine)
-        static_cast<float2*>(p.out)[(int64_t)(t.tile0 / p.run * shares_of(p.width, SHARE) + half) * p.rows + row] = make_float2(top, sum);
+        static_cast<float2*>(p.out)[(int64_t)(t.tile0 / p.run * shares_of(p.width, SHARE) + part_of) * p.rows + row] = make_float2(top, sum);
     }
   }
 
@@ -568,7 +569,7 @@ Plan plan_of(const eqt_type_loss_args& a, bool backward) {
     p.run = (int)std::min<int64_t>(32, std::max<int64_t>(1, row_tiles * col_tiles / (sms * 8)));
     p.runs = (int)ceil_div(col_tiles, p.run);
     p.states = at;
-    p.logit = p.states + up((size_t)p.runs * shares_of(p.width_t, p.cols / 2) * a.n * sizeof(float2));
+    p.logit = p.states + up((size_t)p.runs * shares_of(p.width_t, p.parts == 1 ? share<1>() : share<3>()) * a.n * sizeof(float2));
     p.bytes = p.logit + up((size_t)a.n * 4);
     return p;
   }
@@ -601,7 +602,7 @@ template <int PARTS, int MODE> int launch(const Launch& p, cudaStream_t s) {
   auto kernel = loss_kernel<PARTS, MODE>;
   static std::atomic<uint64_t> allowed{0};
   if (int rc = allow_shared_once(kernel, shared_bytes<PARTS>(), allowed)) return rc;
-  kernel<<<std::min<unsigned>(p.items, (unsigned)sm_count()), THREADS, shared_bytes<PARTS>(), s>>>(p);
+  kernel<<<std::min<unsigned>(p.items, (unsigned)sm_count()), threads<PARTS>(), shared_bytes<PARTS>(), s>>>(p);
   return check_launch("type_loss");
 }
 template <int MODE> int launch(int parts, const Launch& p, cudaStream_t s) { return parts == 1 ? launch<1, MODE>(p, s) : launch<3, MODE>(p, s); }
@@ -676,7 +677,7 @@ extern "C" int eqt_type_loss_forward(const eqt_type_loss_args* args, void* strea
     l.run = p.run, l.kblocks = (int)ceil_div(a.c, BK), l.fold = fold_of(p.parts), l.items = (unsigned)(l.row_tiles * p.runs);
     l.out = base + p.states, l.target = a.target, l.types = a.t, l.target_logit = reinterpret_cast<float*>(base + p.logit), l.status = a.status;
     if (int rc = launch<LOGITS>(p.parts, l, s)) return rc;
-    rows_kernel<<<(unsigned)ceil_div(a.n, 32), 256, 0, s>>>(reinterpret_cast<const float2*>(base + p.states), p.runs * shares_of(p.width_t, p.cols / 2), l.target_logit, a.target, a.n,
+    rows_kernel<<<(unsigned)ceil_div(a.n, 32), 256, 0, s>>>(reinterpret_cast<const float2*>(base + p.states), p.runs * shares_of(p.width_t, p.parts == 1 ? share<1>() : share<3>()), l.target_logit, a.target, a.n,
                                                             a.t, a.lse, a.losses);
     if (int rc = check_launch("type_loss_rows")) return rc;
   }

@@ -14,9 +14,9 @@
 // the sum and the result have the same unit, so that loses nothing.  The scores of the next 64 keys are made while the softmax works on these.
 // dS goes into dq's product in two parts, as within whole graphs: dq has the error of delta, which goes by the rounded result, already.
 //
-// Two CTAs an SM hide each other's chain of copy, product, softmax and product; COLUMNS of more than 64 values, whose two sums take half of the
-// tensor memory, has one CTA of two groups of softmax warps that take turns.  Warps 0 to 3 (7): softmax; then two that issue MMAs and two that copy (16 bytes a
-// thread to the places of the 128-byte swizzle, so that heads of any whole pieces and components of any stride fit one layout).
+// Two CTAs an SM hide each other's chain of copy, product, softmax and product.  By columns two or three groups of softmax warps take turns in one CTA, which
+// has all the tensor memory (64 values a head: 247 -> 217 us for 240 chains of 50 to 500 nodes against two CTAs of one group; by rows, where one thread has
+// half the products to issue, that lost: 189 -> 325).  Warps 0 to 3 (7, 11): softmax; then two that issue MMAs and two that copy.
 //
 // Bound by the special functions at 64 values a head (a score is 4 x 64 flops, 0.16 ps of the tensor cores, and one exponential, 0.22 ps) and by the
 // tensor cores at 128.  Every wait is bounded; on expiry the status flag is raised and the kernel ends.
@@ -37,15 +37,15 @@ constexpr int KEYS = 64, LOADERS = 64;                   // of the other side at
 constexpr float FAR = 8.f;                               // of log2, that a score may be above the unit
 
 template <int DP, int MODE> struct Form {
-  static constexpr int GROUPS = MODE == COLUMNS && DP == 128 ? 2 : 1;               // of softmax warps, each with a buffer of scores
+  static constexpr int GROUPS = MODE == COLUMNS ? (DP == 128 ? 2 : 3) : 1;             // of softmax warps, each with a buffer of scores
   static constexpr int BUFFERS = MODE == FORWARD ? 2 : GROUPS;
-  static constexpr int SOFT = 4 * GROUPS, THREADS = 32 * (SOFT + 2) + LOADERS, CTAS = GROUPS == 2 ? 1 : 2;
+  static constexpr int SOFT = 4 * GROUPS, THREADS = 32 * (SOFT + 2) + LOADERS, CTAS = GROUPS > 1 ? 1 : 2;
   static constexpr int OWN = MODE == FORWARD ? 1 : 2;                                // operands of the tile's rows
   static constexpr int OWN_BYTES = TILE_M * DP * 2, SLOT_BYTES = KEYS * DP * 2;
   static constexpr int SLOTS = MODE == FORWARD && DP == 128 ? 4 : MODE == ROWS && DP == 128 ? 3 : 8;
   static constexpr int NUMBERS = MODE == COLUMNS ? SLOTS / 2 * 3 * KEYS * 4 : 0;     // bytes: a query's greatest score, inverse sum, delta
   static constexpr int BUFFER = MODE == FORWARD ? KEYS : 2 * KEYS;                   // columns of tensor memory: S, or S and dP
-  static constexpr int SUM_AT = BUFFERS * BUFFER, COLS = GROUPS == 2 ? 512 : 256;
+  static constexpr int SUM_AT = BUFFERS * BUFFER, COLS = CTAS == 1 ? 512 : 256;
   static constexpr size_t bytes() { return (size_t)OWN * OWN_BYTES + (size_t)SLOTS * SLOT_BYTES + NUMBERS + 512; }
   static_assert(LOADERS == KEYS, "a number of a query each");
   static_assert(SUM_AT + (MODE == COLUMNS ? 2 : 1) * DP <= COLS, "tensor memory");
@@ -607,8 +607,7 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
         __syncwarp();
         for (unsigned bad = __ballot_sync(0xffffffffu, on && !finite); bad; bad &= bad - 1) {
           const int r = __ffs(bad) - 1;
-          again_columns<T>(w, row - lane + r, kv, __shfl_sync(0xffffffffu, span.x, r), __shfl_sync(0xffffffffu, span.y, r), lane, GROUPS == 1 || group == 0,
-                           GROUPS == 1 || group == 1);
+          again_columns<T>(w, row - lane + r, kv, __shfl_sync(0xffffffffu, span.x, r), __shfl_sync(0xffffffffu, span.y, r), lane, group == 0, group == GROUPS - 1);
         }
       }
     }
