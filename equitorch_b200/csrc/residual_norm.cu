@@ -126,17 +126,32 @@ __global__ void __launch_bounds__(ROW_THREADS < 128 ? 128 : ROW_THREADS) forward
     if (p.w && k < pieces) w[i] = reinterpret_cast<const uint4*>(p.w)[k % (p.channels / V)];
   }
   int turn = 0;
-  for (int64_t row0 = (int64_t)blockIdx.x * ROWS; row0 < p.n; row0 += (int64_t)gridDim.x * ROWS, turn ^= 1) {
-    const int64_t row = row0 + threadIdx.x / ROW_THREADS;
-    const bool there = row < p.n;
-    const int64_t first = row * pieces;
-    uint4 x[PIECES], r[PIECES];
+  constexpr bool AHEAD = PIECES <= 2;                    // the next row is on its way while this one is worked on
+  uint4 x[PIECES], r[PIECES], next_x[PIECES], next_r[PIECES];
+  auto ask = [&](int64_t row, uint4 (&a)[PIECES], uint4 (&b)[PIECES]) {
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
       const int k = at + i * ROW_THREADS;
-      const bool on = there && k < pieces;
-      x[i] = on ? __ldg(reinterpret_cast<const uint4*>(p.x) + first + k) : make_uint4(0, 0, 0, 0);
-      if (RES) r[i] = on ? __ldg(reinterpret_cast<const uint4*>(p.res) + first + k) : make_uint4(0, 0, 0, 0);
+      const bool on = row < p.n && k < pieces;
+      a[i] = on ? __ldg(reinterpret_cast<const uint4*>(p.x) + row * pieces + k) : make_uint4(0, 0, 0, 0);
+      if (RES) b[i] = on ? __ldg(reinterpret_cast<const uint4*>(p.res) + row * pieces + k) : make_uint4(0, 0, 0, 0);
+    }
+  };
+  const int64_t step = (int64_t)gridDim.x * ROWS;
+  if (AHEAD) ask((int64_t)blockIdx.x * ROWS + threadIdx.x / ROW_THREADS, next_x, next_r);
+  for (int64_t row0 = (int64_t)blockIdx.x * ROWS; row0 < p.n; row0 += step, turn ^= 1) {
+    const int64_t row = row0 + threadIdx.x / ROW_THREADS;
+    const bool there = row < p.n;
+    const int64_t first = row * pieces;
+    if constexpr (AHEAD) {
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) {
+        x[i] = next_x[i];
+        if (RES) r[i] = next_r[i];
+      }
+      ask(row + step, next_x, next_r);
+    } else {
+      ask(row, x, r);
     }
     float h[PIECES][V], sum = 0.f;
 #pragma unroll
@@ -264,20 +279,34 @@ __global__ void __launch_bounds__(ROW_THREADS < 128 ? 128 : ROW_THREADS) backwar
     for (int j = 0; j < V; ++j) dw[i][j] = 0.f;
   }
   int turn = 0;
-  for (int64_t row0 = (int64_t)blockIdx.x * ROWS; row0 < p.n; row0 += (int64_t)gridDim.x * ROWS, turn ^= 1) {
-    const int64_t row = row0 + threadIdx.x / ROW_THREADS;
-    const bool there = row < p.n;
-    const int64_t first = row * pieces;
-    uint4 g[PIECES], t[PIECES], s[PIECES];
+  constexpr bool AHEAD = PIECES <= 2;
+  uint4 g[PIECES], t[PIECES], s[PIECES], next_g[PIECES], next_t[PIECES], next_s[PIECES];
+  float inverse, next_inverse = 0.f;
+  auto ask = [&](int64_t row, uint4 (&a)[PIECES], uint4 (&b)[PIECES], uint4 (&c)[PIECES], float& root) {
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
       const int k = at + i * ROW_THREADS;
-      const bool on = there && k < pieces;
-      g[i] = on ? __ldg(reinterpret_cast<const uint4*>(p.g) + first + k) : make_uint4(0, 0, 0, 0);
-      t[i] = on ? __ldg(reinterpret_cast<const uint4*>(p.total) + first + k) : make_uint4(0, 0, 0, 0);
-      s[i] = p.gh && on ? __ldg(reinterpret_cast<const uint4*>(p.gh) + first + k) : make_uint4(0, 0, 0, 0);
+      const bool on = row < p.n && k < pieces;
+      a[i] = on ? __ldg(reinterpret_cast<const uint4*>(p.g) + row * pieces + k) : make_uint4(0, 0, 0, 0);
+      b[i] = on ? __ldg(reinterpret_cast<const uint4*>(p.total) + row * pieces + k) : make_uint4(0, 0, 0, 0);
+      c[i] = p.gh && on ? __ldg(reinterpret_cast<const uint4*>(p.gh) + row * pieces + k) : make_uint4(0, 0, 0, 0);
     }
-    const float inverse = there ? __ldg(p.rstd + row) : 0.f;
+    root = row < p.n ? __ldg(p.rstd + row) : 0.f;
+  };
+  const int64_t step = (int64_t)gridDim.x * ROWS;
+  if (AHEAD) ask((int64_t)blockIdx.x * ROWS + threadIdx.x / ROW_THREADS, next_g, next_t, next_s, next_inverse);
+  for (int64_t row0 = (int64_t)blockIdx.x * ROWS; row0 < p.n; row0 += step, turn ^= 1) {
+    const int64_t row = row0 + threadIdx.x / ROW_THREADS;
+    const bool there = row < p.n;
+    const int64_t first = row * pieces;
+    if constexpr (AHEAD) {
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) g[i] = next_g[i], t[i] = next_t[i], s[i] = next_s[i];
+      inverse = next_inverse;
+      ask(row + step, next_g, next_t, next_s, next_inverse);
+    } else {
+      ask(row, g, t, s, inverse);
+    }
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
@@ -455,16 +484,16 @@ Rows rows_of(int dtype, int64_t length, int64_t channels, uintptr_t bits) {
   const int v = 16 / size_of(dtype);
   if (bits % 16 || length % v || channels % v) return {0, 0};
   const int64_t pieces = length / v;
-  if (pieces <= 128) return {32, pieces <= 32 ? 1 : pieces <= 64 ? 2 : 4};
-  if (pieces <= 512) return {128, pieces <= 256 ? 2 : 4};
+  if (pieces <= 64) return {32, pieces <= 32 ? 1 : 2};
+  if (pieces <= 512) return {128, pieces <= 128 ? 1 : pieces <= 256 ? 2 : 4};
   return pieces <= 2048 ? Rows{512, pieces <= 1024 ? 2 : 4} : Rows{0, 0};
 }
 // A call of `f` with the threads and pieces as constants.
 template <int N> using Constant = std::integral_constant<int, N>;
 template <typename F> void with_rows(Rows r, F f) {
   if (r.threads == 32 && r.pieces == 1) f(Constant<32>(), Constant<1>());
-  else if (r.threads == 32 && r.pieces == 2) f(Constant<32>(), Constant<2>());
-  else if (r.threads == 32) f(Constant<32>(), Constant<4>());
+  else if (r.threads == 32) f(Constant<32>(), Constant<2>());
+  else if (r.threads == 128 && r.pieces == 1) f(Constant<128>(), Constant<1>());
   else if (r.threads == 128 && r.pieces == 2) f(Constant<128>(), Constant<2>());
   else if (r.threads == 128) f(Constant<128>(), Constant<4>());
   else if (r.pieces == 2) f(Constant<512>(), Constant<2>());

@@ -2,11 +2,11 @@
 //
 //     s_j = scale <q, k_j>,   out = sum_j softmax(s)_j v_j,      j in [len - 1 - before, len) or j < sinks,  j < len
 //
-// Bound by HBM: every visible key and value is read once, for all the heads that share it; 2 D values a key against 4 D flops a head.  The
-// visible keys of a chain are one list (sinks, then the window), cut into parts so that the chains' parts fill the SMs; a CTA takes a part of
-// a chain and the heads of one head of keys, up to MOST at a time.  The threads that a key's row takes by pieces of 16 bytes form a team; a team
-// takes key after key with the softmax's maximum and sum, and its sums of the values, in its own registers, so that nothing but the product
-// itself crosses threads on the way.  Teams, and then parts, are joined by their maxima at the end, in one order.
+// Bound by HBM: every visible key and value is read once, for all the heads that share it.  The visible keys of a chain are two stretches (first nodes,
+// window) of steps of 32 keys, cut into parts so that the chains' parts fill the SMs; a CTA takes a part and up to 16 heads of a head of keys, whose queries
+// are the rows of the warp-wide matrix instructions.  Each of its four warps takes every fourth step, with copies of its own three ahead, and has the
+// maxima, sums and weighted values of its keys; warps, and then parts, are joined by their maxima, in one order.
+// 64 chains of up to 8192 nodes, window 4096, 16 heads on 4 of 64 bfloat16 values: JOINED us, WITH us with products by the threads.
 #include <algorithm>
 
 #include "graph_attention.cuh"
@@ -15,292 +15,217 @@ namespace eqt {
 namespace window_step {
 namespace {
 
-constexpr int THREADS = 128, MOST_VALUES = 128, AHEAD = 6;
-using attention::LOG2E;
+using namespace attention;
+constexpr int MOST_VALUES = 128, STAGES = 3, ROWS = 16;
 
 struct StepArgs {
-  const void *q, *k, *v;
+  Operand q, k, v;                                       // of one chain
+  int64_t q_chain, k_chain, v_chain;                     // strides between chains, in values
   void* out;
   float* parts;                                          // [chain][head][part]: maximum, sum, sums of the values
   const int64_t* lengths;
-  int64_t q_chain, q_comp, k_chain, k_node, k_comp, v_chain, v_node, v_comp, capacity, before, sinks;
-  int64_t part_keys;
-  int heads, group, comps, size, values, num_parts;      // group: heads of a head of keys; values: of a head
-  float scale;                                           // times log2 e
+  int64_t capacity, before, sinks, part_steps;
+  int group, num_parts;                                  // group: heads of a head of keys
+  AttentionParams a;                                     // heads, components, channels a head, alignment
 };
 
-using attention::add2;
-using attention::both;
-using attention::exp2_fast;
-using attention::fma2;
-using attention::mul2;
-using attention::pair;
-using attention::parts;
-
-// V values from memory: 16 bytes, or one
-template <int V> __device__ __forceinline__ void unpack(const uint4& u, float (&v)[V]) {
-  if constexpr (V > 1) {
-    const uint32_t r[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (V == 4) v[i] = __uint_as_float(r[i]);
-      else v[2 * i] = __uint_as_float(r[i] << 16), v[2 * i + 1] = __uint_as_float(r[i] & 0xffff0000u);
-    }
-  }
-}
-template <typename T, int V> __device__ __forceinline__ void load(const T* p, float (&v)[V]) {
-  if constexpr (V == 1) v[0] = static_cast<float>(*p);
-  else unpack<V>(__ldg(reinterpret_cast<const uint4*>(p)), v);
+// Keys a step, such that three stages of four warps leave two CTAs an SM.
+template <typename T, int DP> constexpr int step_keys() { return sizeof(T) * DP > 256 ? 8 : sizeof(T) * DP > 128 ? 16 : 32; }
+template <typename T, int DP> constexpr size_t stage_values() { return (size_t)2 * step_keys<T, DP>() * Row<T, DP>::LD; }
+template <typename T, int DP> constexpr size_t shared_bytes() {
+  const size_t tiles = (ROWS * Row<T, DP>::LD + WARPS * STAGES * stage_values<T, DP>()) * sizeof(T), sums = (size_t)WARPS * ROWS * (DP + 2) * 4;
+  return tiles > sums ? tiles : sums;
 }
 
-// What a softmax over some keys leaves.  Without a key the maximum is minus infinity and the sums are zero.
-template <int N> struct State {
-  float top, sum, o[N];
-};
-template <int N> __device__ __forceinline__ void join(State<N>& a, float top, float sum, const float* o) {
-  const float t = top > a.top || top != top ? top : a.top, keep = a.top == -INFINITY ? 0.f : exp2_fast(a.top - t), take = top == -INFINITY ? 0.f : exp2_fast(top - t);
-  a.sum = a.sum * keep + sum * take;
-#pragma unroll
-  for (int i = 0; i < N; ++i) a.o[i] = a.o[i] * keep + o[i] * take;
-  a.top = t;
+template <typename T, int DP, int ROWS_TILE> __device__ __forceinline__ void load_some(T* dst, const Operand& x, int first, int left, int head, const AttentionParams& p, int lane) {
+  const Piece<T, DP, 32> piece(lane, p.comps, p.size);
+  Source<T, DP, 32> from(x, piece, first, head, p);
+  load_rows<T, DP, 32, ROWS_TILE>(dst, from, x, piece, first, left, head, p, lane);
 }
 
-// TEAM threads a key, PIECES pieces of V values each; H heads at a time
-template <typename T, int V, int TEAM, int PIECES, int H> __global__ void __launch_bounds__(THREADS) step_kernel(const StepArgs p) {
-  constexpr int N = V * PIECES, TEAMS = THREADS / TEAM;
-  __shared__ float tops[THREADS / 32][H], sums[THREADS / 32][H], values[THREADS / 32][H][TEAM * N];
-  __shared__ uint4 ring[V > 1 ? AHEAD : 1][2][V > 1 ? THREADS : 1];
-  const int lane = threadIdx.x % TEAM, team = threadIdx.x / TEAM, warp = threadIdx.x >> 5;
-  const int part = blockIdx.x, blocks = (p.group + H - 1) / H, kv = blockIdx.y / blocks, head0 = kv * p.group + blockIdx.y % blocks * H;
-  const int here = min(H, (kv + 1) * p.group - head0);
-  const int64_t chain = blockIdx.z, length = max((int64_t)0, min(p.lengths[chain], p.capacity));
-  const int64_t low = max((int64_t)0, length - 1 - p.before), sinks = min(low, p.sinks), visible = sinks + length - low;
-  const int64_t first = part * p.part_keys, end = min(visible, first + p.part_keys);
-  // this thread's places in a head's row
-  int64_t k_at[PIECES], v_at[PIECES];
-  bool on[PIECES];
-  float q[H][N];
-#pragma unroll
-  for (int i = 0; i < PIECES; ++i) {
-    const int at = (lane + i * TEAM) * V;
-    on[i] = at < p.values;
-    const int comp = on[i] ? at / p.size : 0, channel = on[i] ? at - comp * p.size : 0;
-    k_at[i] = chain * p.k_chain + comp * p.k_comp + (int64_t)kv * p.size + channel;
-    v_at[i] = chain * p.v_chain + comp * p.v_comp + (int64_t)kv * p.size + channel;
-#pragma unroll
-    for (int h = 0; h < H; ++h) {
-      float t[V];
-#pragma unroll
-      for (int j = 0; j < V; ++j) t[j] = 0.f;
-      if (on[i] && h < here) load<T, V>(static_cast<const T*>(p.q) + chain * p.q_chain + comp * p.q_comp + (int64_t)(head0 + h) * p.size + channel, t);
-#pragma unroll
-      for (int j = 0; j < V; ++j) q[h][i * V + j] = t[j] * p.scale;
-    }
+template <typename T, int DP> __global__ void __launch_bounds__(THREADS) step_kernel(const __grid_constant__ StepArgs p) {
+  constexpr int LD = Row<T, DP>::LD, KT = step_keys<T, DP>(), NT = KT / 8;
+  extern __shared__ __align__(16) unsigned char smem[];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3, values = p.a.comps * p.a.size;
+  const int part = blockIdx.x, blocks = (p.group + ROWS - 1) / ROWS, kv = blockIdx.y / blocks, head0 = kv * p.group + blockIdx.y % blocks * ROWS;
+  const int here = min(ROWS, (kv + 1) * p.group - head0);
+  const int64_t chain = blockIdx.z;
+  const int length = (int)max((int64_t)0, min(p.lengths[chain], p.capacity)), low = (int)max((int64_t)0, length - 1 - p.before), sinks = (int)min((int64_t)low, p.sinks);
+  const int steps0 = (sinks + KT - 1) / KT, steps = steps0 + (length - low + KT - 1) / KT;
+  const int first = (int)min((int64_t)steps, part * p.part_steps), end = (int)min((int64_t)steps, first + p.part_steps);
+  T *rows = reinterpret_cast<T*>(smem), *stage = rows + ROWS * LD + warp * STAGES * stage_values<T, DP>();
+  if (values < DP) {                                     // the columns behind a head's values stay zero
+    for (size_t i = tid; i < shared_bytes<T, DP>() / 16; i += THREADS) reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
+    __syncthreads();
   }
-  pair q2[H][N / 2], o2[H][N / 2];
-  float tops_[H], sums_[H];
-#pragma unroll
-  for (int h = 0; h < H; ++h) {
-    tops_[h] = -INFINITY;
-    sums_[h] = 0.f;
-#pragma unroll
-    for (int c = 0; c < N / 2; ++c) {
-      q2[h][c] = both(q[h][2 * c], q[h][2 * c + 1]);
-      o2[h][c] = 0;
-    }
+  auto of = [&](const Operand& x, int64_t stride) { return Operand{static_cast<const T*>(x.p) + chain * stride, x.node, x.comp}; };
+  const Operand q = of(p.q, p.q_chain), k = of(p.k, p.k_chain), v = of(p.v, p.v_chain);
+  for (int i = tid; i < ROWS * values; i += THREADS) {
+    const int h = i / values, e = i - h * values, comp = e / p.a.size;
+    rows[h * LD + e] = h < here ? static_cast<const T*>(q.p)[comp * q.comp + (int64_t)(head0 + h) * p.a.size + e - comp * p.a.size] : static_cast<T>(0.f);
   }
-  auto key_of = [&](int64_t i) { return i < sinks ? i : low + i - sinks; };
-  // Pieces of 16 bytes are on their way AHEAD rounds before they are used, each thread's to a place of its own, so that no thread waits for another.
-  auto ask = [&](int64_t round, int place) {
-    if constexpr (V > 1) {
-      if (round + team < end && on[0]) {
-        const int64_t j = key_of(round + team);
-        attention::copy16(&ring[place][0][threadIdx.x], static_cast<const T*>(p.k) + k_at[0] + j * p.k_node, true);
-        attention::copy16(&ring[place][1][threadIdx.x], static_cast<const T*>(p.v) + v_at[0] + j * p.v_node, true);
-      }
-      attention::copies_commit();
-    }
+  auto key_of = [&](int step, int& stop) {
+    stop = step < steps0 ? sinks : length;
+    return step < steps0 ? step * KT : low + (step - steps0) * KT;
   };
-  if constexpr (V > 1) {
-    if (!on[0])
-      for (int i = 0; i < AHEAD; ++i) ring[i][0][threadIdx.x] = ring[i][1][threadIdx.x] = make_uint4(0, 0, 0, 0);
+  auto ask = [&](int step, int place) {
+    if (step < end) {
+      int stop;
+      const int key = key_of(step, stop);
+      T* to = stage + place * stage_values<T, DP>();
+      load_some<T, DP, KT>(to, k, key, stop - key, kv, p.a, lane);
+      load_some<T, DP, KT>(to + KT * LD, v, key, stop - key, kv, p.a, lane);
+    }
+    copies_commit();
+  };
 #pragma unroll
-    for (int i = 0; i < AHEAD - 1; ++i) ask(first + i * TEAMS, i);
-  }
-  // all threads of a warp take as many rounds, so that the shuffles find them; teams without a key add nothing
+  for (int i = 0; i < STAGES - 1; ++i) ask(first + warp + i * WARPS, i);
+  __syncthreads();
+  const float unit = p.a.scale * LOG2E;
+  float o[DP / 8][4], top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
+#pragma unroll
+  for (int n = 0; n < DP / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
   int place = 0;
-  for (int64_t round = first; round < end; round += TEAMS) {
-    const int64_t i = round + team;
-    const bool there = i < end;
-    float k[N], v[N];
-    if constexpr (V > 1) {
-      ask(round + (AHEAD - 1) * TEAMS, place == 0 ? AHEAD - 1 : place - 1);
-      attention::copies_wait<AHEAD - 1>();
-      unpack<V>(ring[place][0][threadIdx.x], k);
-      unpack<V>(ring[place][1][threadIdx.x], v);
-      if (++place == AHEAD) place = 0;
-    } else {
-      const int64_t j = there ? key_of(i) : 0;
+  for (int step = first + warp; step < end; step += WARPS) {
+    ask(step + (STAGES - 1) * WARPS, place == 0 ? STAGES - 1 : place - 1);
+    copies_wait<STAGES - 1>();
+    __syncwarp();
+    const T *ks = stage + place * stage_values<T, DP>(), *vs = ks + KT * LD;
+    int stop;
+    const int key = key_of(step, stop);
+    float z[NT][4];
+    score_mma<DP, NT>(z, rows, ks, lane);
 #pragma unroll
-      for (int m = 0; m < PIECES; ++m) {
-        k[m] = there && on[m] ? static_cast<float>(static_cast<const T*>(p.k)[k_at[m] + j * p.k_node]) : 0.f;
-        v[m] = there && on[m] ? static_cast<float>(static_cast<const T*>(p.v)[v_at[m] + j * p.v_node]) : 0.f;
-      }
-    }
-    float score[H];
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-    for (int h = 0; h < H; ++h) {
-      pair sum = mul2(q2[h][0], both(k[0], k[1]));
+      for (int i = 0; i < 4; ++i) z[n][i] = key + n * 8 + 2 * t + (i & 1) < stop ? z[n][i] * unit : -INFINITY;
 #pragma unroll
-      for (int c = 1; c < N / 2; ++c) sum = fma2(q2[h][c], both(k[2 * c], k[2 * c + 1]), sum);
-      float x, y;
-      parts(sum, x, y);
-      score[h] = x + y;
-    }
+    for (int r = 0; r < 2; ++r) {
+      float most = top[r];
 #pragma unroll
-    for (int o = TEAM / 2; o > 0; o >>= 1)
+      for (int n = 0; n < NT; ++n) most = fmaxf(most, fmaxf(z[n][2 * r], z[n][2 * r + 1]));
+      most = quad_max(most);
+      const float base = most == -INFINITY ? 0.f : most, keep = exp2_fast(top[r] - base);
+      float add = 0.f;
 #pragma unroll
-      for (int h = 0; h < H; ++h) score[h] += __shfl_xor_sync(0xffffffffu, score[h], o);
-    if (there) {
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int h = 0; h < H; ++h) {
-        if (score[h] > tops_[h] || score[h] != score[h]) {                // a new maximum (or not a number, which stays)
-          const float keep = exp2_fast(tops_[h] - score[h]);
-          sums_[h] *= keep;
-          const pair keeps = both(keep, keep);
-#pragma unroll
-          for (int c = 0; c < N / 2; ++c) o2[h][c] = mul2(o2[h][c], keeps);
-          tops_[h] = score[h];
+        for (int i = 0; i < 2; ++i) {
+          z[n][2 * r + i] = exp2_fast(z[n][2 * r + i] - base);
+          add += z[n][2 * r + i];
         }
-        const float w = score[h] == -INFINITY ? 0.f : exp2_fast(score[h] - tops_[h]);
-        const pair weights = both(w, w);
-        sums_[h] += w;
-        if (w != 0.f) {                                  // of a weight of zero, nothing, whatever the value
+      sum[r] = sum[r] * keep + add;
+      top[r] = most;
 #pragma unroll
-          for (int c = 0; c < N / 2; ++c) o2[h][c] = fma2(weights, both(v[2 * c], v[2 * c + 1]), o2[h][c]);
-        }
-      }
+      for (int n = 0; n < DP / 8; ++n) o[n][2 * r] *= keep, o[n][2 * r + 1] *= keep;
     }
+    out_mma<DP, NT>(o, z, vs, lane);
+    __syncwarp();
+    if (++place == STAGES) place = 0;
   }
-  if constexpr (V > 1) attention::copies_wait<0>();
-  State<N> state[H];
+  copies_wait<0>();
+  __syncthreads();                                       // the tiles' place is the sums' now: [warp][head] maximum, sum, values
+  float* sums = reinterpret_cast<float*>(smem);
 #pragma unroll
-  for (int h = 0; h < H; ++h) {
-    state[h].top = tops_[h];
-    state[h].sum = sums_[h];
+  for (int r = 0; r < 2; ++r) {
+    float* to = sums + (warp * ROWS + g + 8 * r) * (DP + 2);
+    const float all = quad_sum(sum[r]);
+    if (t == 0) to[0] = top[r], to[1] = all;
 #pragma unroll
-    for (int c = 0; c < N / 2; ++c) parts(o2[h][c], state[h].o[2 * c], state[h].o[2 * c + 1]);
-  }
-  // teams of a warp by shuffles, then warps through shared memory
-#pragma unroll
-  for (int o = TEAM; o < 32; o <<= 1)
-#pragma unroll
-    for (int h = 0; h < H; ++h) {
-      float other[N];
-      const float top = __shfl_xor_sync(0xffffffffu, state[h].top, o), sum = __shfl_xor_sync(0xffffffffu, state[h].sum, o);
-#pragma unroll
-      for (int c = 0; c < N; ++c) other[c] = __shfl_xor_sync(0xffffffffu, state[h].o[c], o);
-      join<N>(state[h], top, sum, other);
-    }
-  if ((threadIdx.x & 31) < TEAM) {
-#pragma unroll
-    for (int h = 0; h < H; ++h) {
-      if (lane == 0) tops[warp][h] = state[h].top, sums[warp][h] = state[h].sum;
-#pragma unroll
-      for (int c = 0; c < N; ++c) values[warp][h][lane * N + c] = state[h].o[c];
-    }
+    for (int n = 0; n < DP / 8; ++n) to[2 + n * 8 + 2 * t] = o[n][2 * r], to[2 + n * 8 + 2 * t + 1] = o[n][2 * r + 1];
   }
   __syncthreads();
-  for (int h = warp; h < here; h += THREADS / 32) {
-    if ((threadIdx.x & 31) >= TEAM) continue;
-    State<N> s;
-    s.top = tops[0][h];
-    s.sum = sums[0][h];
+  for (int i = tid; i < here * values; i += THREADS) {
+    const int h = i / values, e = i - h * values;
+    float most = -INFINITY, total = 0.f, value = 0.f;
 #pragma unroll
-    for (int c = 0; c < N; ++c) s.o[c] = values[0][h][lane * N + c];
+    for (int w = 0; w < WARPS; ++w) most = fmaxf(most, sums[(w * ROWS + h) * (DP + 2)]);
+    const float base = most == -INFINITY ? 0.f : most;
 #pragma unroll
-    for (int w = 1; w < THREADS / 32; ++w) join<N>(s, tops[w][h], sums[w][h], &values[w][h][lane * N]);
-    const int head = head0 + h;
+    for (int w = 0; w < WARPS; ++w) {
+      const float* from = sums + (w * ROWS + h) * (DP + 2);
+      const float f = exp2_fast(from[0] - base);
+      total += f * from[1];
+      value += f * from[2 + e];
+    }
+    const int head = head0 + h, comp = e / p.a.size;
     if (p.num_parts > 1) {
-      float* to = p.parts + ((chain * p.heads + head) * p.num_parts + part) * (2 + p.values);
-      if (lane == 0) to[0] = s.top, to[1] = s.sum;
-#pragma unroll
-      for (int m = 0; m < PIECES; ++m)
-#pragma unroll
-        for (int c = 0; c < V; ++c)
-          if (on[m]) to[2 + (lane + m * TEAM) * V + c] = s.o[m * V + c];
+      float* to = p.parts + ((chain * p.a.heads + head) * p.num_parts + part) * (2 + values);
+      if (e == 0) to[0] = most, to[1] = total;
+      to[2 + e] = value;
     } else {
-      const float inverse = visible > 0 ? 1.f / s.sum : 0.f;
-#pragma unroll
-      for (int m = 0; m < PIECES; ++m) {
-        const int at = (lane + m * TEAM) * V, comp = at / p.size, channel = at - comp * p.size;
-#pragma unroll
-        for (int c = 0; c < V; ++c)
-          if (on[m]) st(static_cast<T*>(p.out) + ((chain * p.comps + comp) * p.heads + head) * p.size + channel + c, s.o[m * V + c] * inverse);
-      }
+      st(static_cast<T*>(p.out) + ((chain * p.a.comps + comp) * p.a.heads + head) * p.a.size + e - comp * p.a.size, length > 0 ? value / total : 0.f);
     }
   }
 }
 
-// The parts of a chain and head, one warp: a lane has every 32nd value.
-template <typename T> __global__ void __launch_bounds__(THREADS) step_join_kernel(const StepArgs p, int64_t rows) {
-  const int64_t row = (int64_t)blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5);
+// The parts of a chain and head, one warp: the maxima and sums by the lanes, then a lane has every 32nd value.
+template <typename T> __global__ void __launch_bounds__(THREADS) step_join_kernel(const __grid_constant__ StepArgs p, int64_t rows) {
+  const int64_t row = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5);
   if (row >= rows) return;
-  const int lane = threadIdx.x & 31, head = (int)(row % p.heads);
-  const int64_t chain = row / p.heads;
-  const float* parts = p.parts + row * p.num_parts * (2 + p.values);
-  State<MOST_VALUES / 32> s;
-  s.top = -INFINITY;
-  s.sum = 0.f;
+  const int lane = threadIdx.x & 31, head = (int)(row % p.a.heads), values = p.a.comps * p.a.size;
+  const int64_t chain = row / p.a.heads;
+  const float* parts = p.parts + row * p.num_parts * (2 + values);
+  float most = -INFINITY, total = 0.f;
+  for (int i = lane; i < p.num_parts; i += 32) most = fmaxf(most, parts[i * (2 + values)]);
 #pragma unroll
-  for (int c = 0; c < MOST_VALUES / 32; ++c) s.o[c] = 0.f;
-#pragma unroll 2
-  for (int i = 0; i < p.num_parts; ++i, parts += 2 + p.values) {
-    float o[MOST_VALUES / 32];
+  for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+  const float base = most == -INFINITY ? 0.f : most;
+  for (int i = lane; i < p.num_parts; i += 32) total += exp2_fast(parts[i * (2 + values)] - base) * parts[i * (2 + values) + 1];
 #pragma unroll
-    for (int c = 0; c < MOST_VALUES / 32; ++c) o[c] = lane + 32 * c < p.values ? parts[2 + lane + 32 * c] : 0.f;
-    join<MOST_VALUES / 32>(s, parts[0], parts[1], o);
+  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  float value[MOST_VALUES / 32];
+#pragma unroll
+  for (int c = 0; c < MOST_VALUES / 32; ++c) value[c] = 0.f;
+#pragma unroll 4
+  for (int i = 0; i < p.num_parts; ++i) {
+    const float* from = parts + i * (2 + values);
+    const float f = exp2_fast(from[0] - base);
+#pragma unroll
+    for (int c = 0; c < MOST_VALUES / 32; ++c) value[c] += f * (lane + 32 * c < values ? from[2 + lane + 32 * c] : 0.f);
   }
-  const float inverse = p.lengths[chain] > 0 && p.capacity > 0 ? 1.f / s.sum : 0.f;
+  const bool any = p.lengths[chain] > 0 && p.capacity > 0;
 #pragma unroll
   for (int c = 0; c < MOST_VALUES / 32; ++c) {
-    const int at = lane + 32 * c, comp = at / p.size, channel = at - comp * p.size;
-    if (at < p.values) st(static_cast<T*>(p.out) + ((chain * p.comps + comp) * p.heads + head) * p.size + channel, s.o[c] * inverse);
+    const int at = lane + 32 * c, comp = at / p.a.size, channel = at - comp * p.a.size;
+    if (at < values) st(static_cast<T*>(p.out) + ((chain * p.a.comps + comp) * p.a.heads + head) * p.a.size + channel, any ? value[c] / total : 0.f);
   }
 }
 
-constexpr int64_t LEAST_KEYS = 64;                       // of a part: joining costs as much as some keys
-// Parts of the visible keys: so many that SMs with shorter chains take more of them.
-void cut(StepArgs& p, int64_t chains, int kv_heads) {
-  const int64_t visible = std::max<int64_t>(1, std::min<int64_t>(p.capacity, p.before + 1 + p.sinks));
-  const int64_t others = std::max<int64_t>(1, chains * kv_heads), wanted = ceil_div((int64_t)sm_count() * 16, others);
-  const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(wanted, ceil_div(visible, LEAST_KEYS)), 1024));
-  p.part_keys = ceil_div(ceil_div(visible, parts), 16) * 16;
-  p.num_parts = (int)ceil_div(visible, p.part_keys);
+// ---- host side ----------------------------------------------------------------------------------
+int width_of(int values) { return values <= 16 ? 16 : values <= 32 ? 32 : values <= 64 ? 64 : 128; }
+int keys_of(int dtype, int width) { return (dtype == EQT_F32 ? 4 : 2) * width > 256 ? 8 : (dtype == EQT_F32 ? 4 : 2) * width > 128 ? 16 : 32; }
+
+// Parts of the visible keys: so many that SMs with shorter chains take more of them, and a step for each warp.
+void cut(StepArgs& p, int dtype, int64_t chains, int kv_heads) {
+  const int kt = keys_of(dtype, width_of(p.a.comps * p.a.size));
+  const int64_t window = std::min<int64_t>(p.capacity, p.before + 1), first = std::min<int64_t>(p.capacity, p.sinks);
+  const int64_t steps = std::max<int64_t>(1, ceil_div(window, kt) + ceil_div(first, kt));
+  const int64_t others = std::max<int64_t>(1, chains * kv_heads), wanted = ceil_div((int64_t)sm_count() * 8, others);
+  const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(wanted, ceil_div(steps, WARPS)), 1024));
+  p.part_steps = ceil_div(ceil_div(steps, parts), WARPS) * WARPS;
+  p.num_parts = (int)ceil_div(steps, p.part_steps);
 }
 
-template <typename T, int V, int TEAM, int PIECES, int H> int launch(const StepArgs& p, int64_t chains, int kv_heads, cudaStream_t s) {
-  const dim3 grid((unsigned)p.num_parts, (unsigned)(kv_heads * ceil_div(p.group, H)), (unsigned)chains);
-  step_kernel<T, V, TEAM, PIECES, H><<<grid, THREADS, 0, s>>>(p);
+template <typename T, int DP> int launch(const StepArgs& p, int64_t chains, int kv_heads, cudaStream_t s) {
+  auto kernel = step_kernel<T, DP>;
+  static std::atomic<uint64_t> allowed{0};
+  if (int rc = allow_shared_once(kernel, shared_bytes<T, DP>(), allowed)) return rc;
+  const dim3 grid((unsigned)p.num_parts, (unsigned)(kv_heads * ceil_div(p.group, ROWS)), (unsigned)chains);
+  kernel<<<grid, THREADS, shared_bytes<T, DP>(), s>>>(p);
   if (int rc = check_launch("window_step")) return rc;
   if (p.num_parts == 1) return EQT_OK;
-  const int64_t rows = chains * p.heads;
-  step_join_kernel<T><<<(unsigned)ceil_div(rows, THREADS / 32), THREADS, 0, s>>>(p, rows);
+  const int64_t rows = chains * p.a.heads;
+  step_join_kernel<T><<<(unsigned)ceil_div(rows, WARPS), THREADS, 0, s>>>(p, rows);
   return check_launch("window_step_join");
 }
-template <typename T, int V, int TEAM, int PIECES> int by_group(const StepArgs& p, int64_t chains, int kv_heads, cudaStream_t s) {
-  if (p.group == 1) return launch<T, V, TEAM, PIECES, 1>(p, chains, kv_heads, s);
-  if (p.group == 2) return launch<T, V, TEAM, PIECES, 2>(p, chains, kv_heads, s);
-  return launch<T, V, TEAM, PIECES, 4>(p, chains, kv_heads, s);
-}
-template <typename T> int run(const StepArgs& p, int64_t chains, int kv_heads, bool whole, cudaStream_t s) {
-  constexpr int V = 16 / (int)sizeof(T);
-  if (!whole) return by_group<T, 1, 32, 4>(p, chains, kv_heads, s);
-  const int pieces = (int)ceil_div(p.values, V);
-  if (pieces <= 4) return by_group<T, V, 4, 1>(p, chains, kv_heads, s);
-  if (pieces <= 8) return by_group<T, V, 8, 1>(p, chains, kv_heads, s);
-  if (pieces <= 16) return by_group<T, V, 16, 1>(p, chains, kv_heads, s);
-  return by_group<T, V, 32, 1>(p, chains, kv_heads, s);
+template <typename T> int run(const StepArgs& p, int64_t chains, int kv_heads, cudaStream_t s) {
+  switch (width_of(p.a.comps * p.a.size)) {
+    case 16: return launch<T, 16>(p, chains, kv_heads, s);
+    case 32: return launch<T, 32>(p, chains, kv_heads, s);
+    case 64: return launch<T, 64>(p, chains, kv_heads, s);
+    default: return launch<T, 128>(p, chains, kv_heads, s);
+  }
 }
 
 int fill(StepArgs& p, const eqt_window_step_args* a) {
@@ -312,12 +237,16 @@ int fill(StepArgs& p, const eqt_window_step_args* a) {
   if ((int64_t)a->comps * a->head_channels > MOST_VALUES || a->chains > 65535 || a->heads > 65535 || a->capacity > INT32_MAX || a->before > INT32_MAX ||
       a->sinks > INT32_MAX)
     return fail(EQT_ERR_UNSUPPORTED, "window_step: at most %d values a head, 65535 chains and heads, 2^31 nodes a chain", MOST_VALUES);
-  p.q = a->q, p.k = a->k, p.v = a->v, p.out = a->out, p.parts = a->scratch, p.lengths = a->lengths;
-  p.q_chain = a->q_chain, p.q_comp = a->q_comp, p.k_chain = a->k_chain, p.k_node = a->k_node, p.k_comp = a->k_comp;
-  p.v_chain = a->v_chain, p.v_node = a->v_node, p.v_comp = a->v_comp;
-  p.capacity = a->capacity, p.before = a->before, p.sinks = a->sinks, p.heads = a->heads, p.group = a->heads / a->kv_heads;
-  p.comps = a->comps, p.size = a->head_channels, p.values = a->comps * a->head_channels, p.scale = a->scale * LOG2E;
-  cut(p, a->chains, a->kv_heads);
+  const int v = a->dtype == EQT_F32 ? 4 : 8;
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(a->k) | reinterpret_cast<uintptr_t>(a->v);
+  const int64_t strides = a->k_chain | a->k_node | a->k_comp | a->v_chain | a->v_node | a->v_comp;
+  p.q = {a->q, 0, a->q_comp}, p.k = {a->k, a->k_node, a->k_comp}, p.v = {a->v, a->v_node, a->v_comp};
+  p.q_chain = a->q_chain, p.k_chain = a->k_chain, p.v_chain = a->v_chain;
+  p.out = a->out, p.parts = a->scratch, p.lengths = a->lengths, p.capacity = a->capacity, p.before = a->before, p.sinks = a->sinks;
+  p.group = a->heads / a->kv_heads;
+  p.a.heads = a->heads, p.a.comps = a->comps, p.a.size = a->head_channels, p.a.scale = a->scale;
+  p.a.vec = bits % 16 == 0 && strides % v == 0 && a->head_channels % v == 0;
+  cut(p, a->dtype, a->chains, a->kv_heads);
   return EQT_OK;
 }
 
@@ -331,7 +260,7 @@ using namespace eqt::window_step;
 extern "C" int64_t eqt_window_step_scratch(const eqt_window_step_args* a) {
   StepArgs p{};
   if (fill(p, a) || p.num_parts == 1) return 0;
-  return a->chains * p.heads * p.num_parts * (2 + p.values);
+  return a->chains * p.a.heads * p.num_parts * (2 + p.a.comps * p.a.size);
 }
 
 extern "C" int eqt_window_step(const eqt_window_step_args* a, void* stream) {
@@ -339,13 +268,9 @@ extern "C" int eqt_window_step(const eqt_window_step_args* a, void* stream) {
   if (int rc = fill(p, a)) return rc;
   if (a->chains == 0) return EQT_OK;
   if (!a->q || !a->out || !a->lengths || (a->capacity && (!a->k || !a->v))) return fail(EQT_ERR_BAD_ARGUMENT, "window_step: NULL pointer");
-  const int64_t need = p.num_parts == 1 ? 0 : a->chains * p.heads * p.num_parts * (2 + p.values);
+  const int64_t need = p.num_parts == 1 ? 0 : a->chains * p.a.heads * p.num_parts * (2 + p.a.comps * p.a.size);
   if (need && (!a->scratch || a->scratch_floats < need))
     return fail(EQT_ERR_BAD_ARGUMENT, "window_step: %lld values of scratch given, %lld needed", (long long)a->scratch_floats, (long long)need);
-  const int v = a->dtype == EQT_F32 ? 4 : 8;
-  const uintptr_t bits = reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->k) | reinterpret_cast<uintptr_t>(a->v);
-  const int64_t strides = a->q_chain | a->q_comp | a->k_chain | a->k_node | a->k_comp | a->v_chain | a->v_node | a->v_comp;
-  const bool whole = bits % 16 == 0 && strides % v == 0 && a->head_channels % v == 0;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return a->dtype == EQT_F32 ? run<float>(p, a->chains, a->kv_heads, whole, s) : run<__nv_bfloat16>(p, a->chains, a->kv_heads, whole, s);
+  return a->dtype == EQT_F32 ? run<float>(p, a->chains, a->kv_heads, s) : run<__nv_bfloat16>(p, a->chains, a->kv_heads, s);
 }
