@@ -64,12 +64,12 @@ template <typename T> __device__ __forceinline__ uint4 pack(const float (&v)[VAL
   return make_uint4(r[0], r[1], r[2], r[3]);
 }
 
-template <typename V> __device__ __forceinline__ V larger(V a, V b) { return a > b ? a : b; }
 struct Sum {
   template <typename V> __device__ __forceinline__ V operator()(V a, V b) const { return a + b; }
 };
 struct Max {                                             // drops NaNs
-  template <typename V> __device__ __forceinline__ V operator()(V a, V b) const { return b > a || a != a ? b : a; }
+  __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); }
+  __device__ __forceinline__ double operator()(double a, double b) const { return fmax(a, b); }
 };
 // Over `lanes` neighbouring threads of a warp, a power of two.
 template <typename V, typename F> __device__ __forceinline__ V across_lanes(V v, int lanes, F f) {
@@ -98,7 +98,7 @@ __device__ __forceinline__ float inverse_root(float sum, int length, float eps) 
 // few bits and ties are real) it is formed in float64 and brought to float32 rounding to odd, which keeps on which side of a border it is.
 __device__ __forceinline__ uint8_t to_e4m3(float v) { return (uint8_t)__nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3); }
 __device__ __forceinline__ uint16_t to_e4m3(float v, float w) { return (uint16_t)__nv_cvt_float2_to_fp8x2(make_float2(v, w), __NV_SATFINITE, __NV_E4M3); }
-__device__ __noinline__ uint8_t to_e4m3_exact(double t, double m) {
+__device__ __forceinline__ uint8_t to_e4m3_exact(double t, double m) {
   const double q = t * (double)E4M3_MAX / m;
   float f = __double2float_rz(q);
   if ((double)f != q) f = __uint_as_float(__float_as_uint(f) | 1u);
@@ -111,19 +111,75 @@ __device__ __forceinline__ float scale_of(float most, float inverse) { return (f
 __device__ __forceinline__ double exact_value(float x, float res, float w) { return ((double)x + (double)res) * (double)w; }
 
 // ---- rows in registers --------------------------------------------------------------------------
+// The 8-bit values of a piece, the long way, from memory (`x` NULL: no piece).  The group's greatest |t| comes from the threads whose values are within an error of `m`,
+// the greatest in float32, in float64; the group is `lanes` threads, or (0) known: `known`.  A call and not in line: in line it takes the kernel from 68 to 168
+// registers a thread, and all rows pay for it (32,768 x 2048: 85 | 138 us).
+template <typename T> __device__ __forceinline__ double exact_most(const uint4& x, const uint4& res, const uint4& w, float m) {
+  constexpr int V = VALUES<T>;
+  float a[V], b[V], c[V];
+  unpack<T>(x, a);
+  unpack<T>(res, b);
+  unpack<T>(w, c);
+  double most = 0.0;
+#pragma unroll 1
+  for (int j = 0; j < V; ++j) {
+    float ta = a[0], tb = b[0], tc = c[0];
+#pragma unroll
+    for (int i = 1; i < V; ++i)
+      if (i == j) ta = a[i], tb = b[i], tc = c[i];
+    if (fabsf((ta + tb) * tc) >= m * (1.f - NEAR)) most = fmax(most, fabs(exact_value(ta, tb, tc)));
+  }
+  return most;
+}
+template <typename T> __device__ __forceinline__ void load_piece(const uint4* x, const uint4* res, const uint4* w, uint4& a, uint4& b, uint4& c) {
+  a = b = c = make_uint4(0, 0, 0, 0);
+  if (!x) return;
+  a = __ldg(x);
+  if (res) b = __ldg(res);
+  if (w) c = __ldg(w);
+  else if constexpr (sizeof(T) == 4) c = make_uint4(0x3f800000u, 0x3f800000u, 0x3f800000u, 0x3f800000u);
+  else c = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);
+}
+template <typename T> __device__ __noinline__ double exact_greatest(const uint4* x, const uint4* res, const uint4* w, float m) {
+  uint4 a, b, c;
+  load_piece<T>(x, res, w, a, b, c);
+  return exact_most<T>(a, b, c, m);
+}
+template <typename T> __device__ __noinline__ uint2 exact_piece(const uint4* x, const uint4* res, const uint4* w, float m, int lanes, double known) {
+  constexpr int V = VALUES<T>;
+  uint4 x4, r4, w4;
+  load_piece<T>(x, res, w, x4, r4, w4);
+  const double most = lanes ? across_lanes(exact_most<T>(x4, r4, w4, m), lanes, Max()) : known;
+  float a[V], b[V], c[V];
+  unpack<T>(x4, a);
+  unpack<T>(r4, b);
+  unpack<T>(w4, c);
+  const float to = m > 0.f ? __fdiv_rn(E4M3_MAX, m) : 0.f;
+  uint32_t words[2] = {0, 0};
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    const float t = (a[j] + b[j]) * c[j];
+    uint32_t held = to_e4m3(t * (to * (1.f - NEAR)));
+    if (held != to_e4m3(t * (to * (1.f + NEAR))) || (m < TINY && m > 0.f)) held = to_e4m3_exact(exact_value(a[j], b[j], c[j]), most);
+    words[j / 4] |= held << (8 * (j & 3));
+  }
+  return make_uint2(words[0], words[1]);
+}
+
 // OUT: 0 values of the type, 1 8 bits with a scale a row, 2 with a scale every p.group values (whole pieces, a power of two of at most 32)
 template <typename T, int ROW_THREADS, int PIECES, int OUT, bool RES>
-__global__ void __launch_bounds__(ROW_THREADS < 128 ? 128 : ROW_THREADS) forward_kernel(const NormArgs p) {
+__global__ void __launch_bounds__(ROW_THREADS < 128 ? 128 : ROW_THREADS, OUT != 0 && PIECES <= 2 && ROW_THREADS < 512 ? 6 : 1) forward_kernel(const NormArgs p) {
   constexpr int V = VALUES<T>, ROWS = ROW_THREADS < 128 ? 128 / ROW_THREADS : 1;
   __shared__ float buffer[2][ROW_THREADS / 32], most_of[2][ROW_THREADS / 32];
   __shared__ double exact_of[2][ROW_THREADS / 32];
   const int at = threadIdx.x % ROW_THREADS, pieces = p.length / V;
-  uint4 w[PIECES];
+  float c[PIECES][V];                                    // weights
 #pragma unroll
   for (int i = 0; i < PIECES; ++i) {
     const int k = at + i * ROW_THREADS;
-    w[i] = make_uint4(0, 0, 0, 0);
-    if (p.w && k < pieces) w[i] = reinterpret_cast<const uint4*>(p.w)[k % (p.channels / V)];
+#pragma unroll
+    for (int j = 0; j < V; ++j) c[i][j] = 1.f;
+    if (p.w && k < pieces) unpack<T>(reinterpret_cast<const uint4*>(p.w)[k % (p.channels / V)], c[i]);
   }
   int turn = 0;
   constexpr bool AHEAD = PIECES <= 2;                    // the next row is on its way while this one is worked on
@@ -179,10 +235,9 @@ __global__ void __launch_bounds__(ROW_THREADS < 128 ? 128 : ROW_THREADS) forward
 #pragma unroll
       for (int i = 0; i < PIECES; ++i) {
         const int k = at + i * ROW_THREADS;
-        float y[V], c[V];
-        unpack<T>(w[i], c);
+        float y[V];
 #pragma unroll
-        for (int j = 0; j < V; ++j) y[j] = p.w ? h[i][j] * inverse * c[j] : h[i][j] * inverse;
+        for (int j = 0; j < V; ++j) y[j] = h[i][j] * inverse * c[i][j];
         if (there && k < pieces) reinterpret_cast<uint4*>(p.y)[first + k] = pack<T>(y);
       }
     } else {
@@ -190,12 +245,10 @@ __global__ void __launch_bounds__(ROW_THREADS < 128 ? 128 : ROW_THREADS) forward
       float most[PIECES], all = 0.f;
 #pragma unroll
       for (int i = 0; i < PIECES; ++i) {
-        float c[V];
-        unpack<T>(w[i], c);
         most[i] = 0.f;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          if (p.w) h[i][j] *= c[j];
+          h[i][j] *= c[i][j];
           most[i] = Max()(most[i], fabsf(h[i][j]));
         }
         if (OUT == 2) most[i] = across_lanes(most[i], lanes, Max());
@@ -204,46 +257,41 @@ __global__ void __launch_bounds__(ROW_THREADS < 128 ? 128 : ROW_THREADS) forward
       if (OUT == 1) all = across_row<ROW_THREADS>(all, most_of[turn], Max());
       // both ends of what the quotient may be: one answer, or the long way round
       uint16_t held[PIECES][V / 2];
-      bool unsure = false;
+      unsigned unsure = 0;                               // no branches: any difference leaves a bit
 #pragma unroll
       for (int i = 0; i < PIECES; ++i) {
         if (OUT == 1) most[i] = all;
         const float to = most[i] > 0.f ? __fdiv_rn(E4M3_MAX, most[i]) : 0.f, less = to * (1.f - NEAR), more = to * (1.f + NEAR);
-        unsure = unsure || (most[i] < TINY && most[i] > 0.f);
+        unsure |= (unsigned)(most[i] < TINY) & (unsigned)(most[i] > 0.f);
 #pragma unroll
         for (int j = 0; j < V; j += 2) {
           held[i][j / 2] = to_e4m3(h[i][j] * less, h[i][j + 1] * less);
-          unsure = unsure || held[i][j / 2] != to_e4m3(h[i][j] * more, h[i][j + 1] * more);
+          unsure |= held[i][j / 2] ^ to_e4m3(h[i][j] * more, h[i][j + 1] * more);
         }
       }
-      if (OUT == 1 ? __syncthreads_or(unsure) : __any_sync(0xffffffffu, unsure)) {
-        double exact[PIECES], whole = 0.0;
+      const bool again = OUT == 1 ? __syncthreads_or(unsure != 0) : __any_sync(0xffffffffu, unsure != 0);
+      if (again) {
+        auto of = [&](const void* base, int64_t from, bool on) { return base && on ? reinterpret_cast<const uint4*>(base) + from : nullptr; };
+        double known = 0.0;
+        for (int step = OUT == 1 ? 0 : 1; step < 2; ++step) {             // a row's greatest first
+#pragma unroll 1
+          for (int i = 0; i < PIECES; ++i) {
+            const int k = at + i * ROW_THREADS;
+            const bool on = there && k < pieces;
+            const uint4 *px = of(p.x, first + k, on), *pr = of(p.res, first + k, on), *pw = of(p.w, k % (p.channels / V), on);
+            float m = most[0];
 #pragma unroll
-        for (int i = 0; i < PIECES; ++i) {
-          float c[V], a[V], b[V];
-          unpack<T>(w[i], c);
-          unpack<T>(x[i], a);
-          if (RES) unpack<T>(r[i], b);
-          exact[i] = 0.0;
-#pragma unroll
-          for (int j = 0; j < V; ++j) exact[i] = Max()(exact[i], fabs(exact_value(a[j], RES ? b[j] : 0.f, p.w ? c[j] : 1.f)));
-          if (OUT == 2) exact[i] = across_lanes(exact[i], lanes, Max());
-          else whole = Max()(whole, exact[i]);
-        }
-        if (OUT == 1) whole = across_row<ROW_THREADS>(whole, exact_of[turn], Max());
-#pragma unroll
-        for (int i = 0; i < PIECES; ++i) {
-          const double m = OUT == 1 ? whole : exact[i];
-          const float to = most[i] > 0.f ? __fdiv_rn(E4M3_MAX, most[i]) : 0.f, more = to * (1.f + NEAR);
-          float c[V], a[V], b[V];
-          unpack<T>(w[i], c);
-          unpack<T>(x[i], a);
-          if (RES) unpack<T>(r[i], b);
-#pragma unroll
-          for (int j = 0; j < V; j += 2)
-            if (held[i][j / 2] != to_e4m3(h[i][j] * more, h[i][j + 1] * more) || (most[i] < TINY && most[i] > 0.f))
-              held[i][j / 2] = (uint16_t)(to_e4m3_exact(exact_value(a[j], RES ? b[j] : 0.f, p.w ? c[j] : 1.f), m) |
-                                          to_e4m3_exact(exact_value(a[j + 1], RES ? b[j + 1] : 0.f, p.w ? c[j + 1] : 1.f), m) << 8);
+            for (int q = 1; q < PIECES; ++q) m = q == i ? most[q] : m;
+            if (step == 0) {
+              known = fmax(known, exact_greatest<T>(px, pr, pw, m));
+              continue;
+            }
+            const uint2 words = exact_piece<T>(px, pr, pw, m, OUT == 2 ? lanes : 0, known);
+            if (!on) continue;
+            if constexpr (V == 8) reinterpret_cast<uint2*>(p.values)[first + k] = words;
+            else reinterpret_cast<uint32_t*>(p.values)[first + k] = words.x;
+          }
+          if (OUT == 1 && step == 0) known = across_row<ROW_THREADS>(known, exact_of[turn], Max());
         }
       }
 #pragma unroll
@@ -251,8 +299,10 @@ __global__ void __launch_bounds__(ROW_THREADS < 128 ? 128 : ROW_THREADS) forward
         const int k = at + i * ROW_THREADS;
         if (!there || k >= pieces) continue;
         uint8_t* to_values = p.values + (first + k) * V;
-        if constexpr (V == 8) *reinterpret_cast<uint2*>(to_values) = make_uint2(held[i][0] | (uint32_t)held[i][1] << 16, held[i][2] | (uint32_t)held[i][3] << 16);
-        else *reinterpret_cast<uint32_t*>(to_values) = held[i][0] | (uint32_t)held[i][1] << 16;
+        if (again) {
+        } else if constexpr (V == 8) *reinterpret_cast<uint2*>(to_values) = make_uint2(held[i][0] | (uint32_t)held[i][1] << 16, held[i][2] | (uint32_t)held[i][3] << 16);
+        else
+          *reinterpret_cast<uint32_t*>(to_values) = held[i][0] | (uint32_t)held[i][1] << 16;
         const float scale = scale_of(most[i], inverse);
         if (OUT == 2 && k % lanes == 0) p.scales[(first + k) / lanes] = scale;
         if (OUT == 1 && k == 0) p.scales[row] = scale;
