@@ -34,7 +34,14 @@ using T = __nv_bfloat16;
 
 enum Mode { FORWARD, ROWS, COLUMNS };
 constexpr int KEYS = 64, LOADERS = 64;                   // of the other side at a time; threads that copy
+constexpr int MOST_TILES = 16;                           // of a CTA
 constexpr float FAR = 8.f;                               // of log2, that a score may be above the unit
+
+// What a tile walks over: `ns` first nodes of the chain that its first row is in, from `from0` on, then [from1, to1), as one sequence.
+struct Stretch {
+  int from0, ns, from1, to1, total, steps;
+};
+constexpr int STRETCHES = 8;
 
 template <int DP, int MODE> struct Form {
   static constexpr int GROUPS = MODE == COLUMNS ? (DP == 128 ? 2 : 3) : 1;             // of softmax warps, each with a buffer of scores
@@ -46,76 +53,76 @@ template <int DP, int MODE> struct Form {
   static constexpr int NUMBERS = MODE == COLUMNS ? SLOTS / 2 * 3 * KEYS * 4 : 0;     // bytes: a query's greatest score, inverse sum, delta
   static constexpr int BUFFER = MODE == FORWARD ? KEYS : 2 * KEYS;                   // columns of tensor memory: S, or S and dP
   static constexpr int SUM_AT = BUFFERS * BUFFER, COLS = CTAS == 1 ? 512 : 256;
-  static constexpr size_t bytes() { return (size_t)OWN * OWN_BYTES + (size_t)SLOTS * SLOT_BYTES + NUMBERS + 512; }
+  static constexpr int BARRIERS = 384;                                               // bytes, with the tensor memory's address and the abort flag
+  static constexpr size_t bytes() { return (size_t)OWN * OWN_BYTES + (size_t)SLOTS * SLOT_BYTES + NUMBERS + BARRIERS + STRETCHES * sizeof(Stretch) + SOFT * MOST_TILES * 4; }
+  static_assert((2 * SLOTS + 3 * BUFFERS + 5 + STRETCHES) * 8 + 8 <= BARRIERS, "barriers");
   static_assert(LOADERS == KEYS, "a number of a query each");
   static_assert(SUM_AT + (MODE == COLUMNS ? 2 : 1) * DP <= COLS, "tensor memory");
 };
 
-// What a thread copies of an operand's rows: in each group of 64 values the same 16 bytes of every eighth row, so that where they come from and go
-// (128-byte swizzle, a line of 128 bytes a row) moves on by additions.  Zeros behind the head's values, up to whole sixteens.
+// What a thread copies of an operand's rows: in each group of 64 values the same 16 bytes of every fourth or eighth row (32 or 64 threads), so that where they come
+// from moves on by additions; and goes to, but for the 128-byte swizzle (a line of 128 bytes a row).  Zeros behind the head's values, up to whole
+// sixteens.  Loops are short on purpose: with all copies laid out one after the other the kernel's code is more than the SM's instruction cache
+// holds, and every warp of it waits (by columns, 128 values: 473 -> 604 us).
 template <int DP> struct Copier {
   static constexpr int GROUPS = DP / 64;
   const T* from[GROUPS];
   int64_t node;
-  int row, size;
-  uint32_t to;
+  int row, col, every, size;
   bool on[GROUPS], there[GROUPS];                        // has values; has a place
-  __device__ __forceinline__ Copier(const Operand& x, const AttentionParams& p, int thread) : node(x.node), row(thread >> 3), size(p.size) {
-    const int col = thread & 7, values = p.comps * p.size;
-    to = (uint32_t)(row * 128 + ((col ^ row) << 4));
+  __device__ __forceinline__ Copier(const Operand& x, const AttentionParams& p, int thread, int threads)
+      : node(x.node), row(thread >> 3), col(thread & 7), every(threads >> 3), size(p.size) {
+    const int values = p.comps * p.size;
 #pragma unroll
     for (int g = 0; g < GROUPS; ++g) {
       const int at = (col + 8 * g) * 8;
       on[g] = at < values;
       there[g] = at < (values + 15) / 16 * 16;
       const int comp = on[g] ? at / p.size : 0;
-      from[g] = static_cast<const T*>(x.p) + comp * x.comp + (on[g] ? at - comp * p.size : 0) + row * node;
+      from[g] = static_cast<const T*>(x.p) + comp * x.comp + (on[g] ? at - comp * p.size : 0);
     }
+  }
+  __device__ __forceinline__ uint32_t place(int r) const { return (uint32_t)(r * 128 + ((col ^ (r & 7)) << 4)); }
+  __device__ __forceinline__ void copy(uint32_t d, const T* f, int g, bool in) const {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(in ? f : from[g]), "r"(in ? 16 : 0) : "memory");
   }
   // KEYS rows of a head from `first` on, zeros from the `left`-th on
   __device__ __forceinline__ void next(unsigned char* dst, int first, int left, int head) const {
-    const int64_t move = first * node + (int64_t)head * size, step = 8 * node;
-    const T* f[GROUPS];
+    const int64_t move = (int64_t)(first + row) * node + (int64_t)head * size, step = every * node;
+    const uint32_t d = s32(dst);
 #pragma unroll
-    for (int g = 0; g < GROUPS; ++g) f[g] = from[g] + move;
-    uint32_t d = s32(dst) + to;
+    for (int g = 0; g < GROUPS; ++g) {
+      if (!there[g]) continue;
+      const T* f = from[g] + move;
 #pragma unroll 2
-    for (int r = row; r < KEYS; r += 8, d += 1024) {
-#pragma unroll
-      for (int g = 0; g < GROUPS; ++g, f[g - 1] += step)
-        if (there[g]) copy(d + g * (KEYS * 128), f[g], g, on[g] && r < left);
+      for (int r = row; r < KEYS; r += every, f += step) copy(d + g * (KEYS * 128) + place(r), f, g, on[g] && r < left);
     }
   }
   // the same of a stretch that begins with `ns` rows from `from0` on and goes on at `from1`, from its `at`-th row on
   __device__ __forceinline__ void mixed(unsigned char* dst, int at, int ns, int from0, int from1, int left, int head) const {
+    const uint32_t d = s32(dst);
 #pragma unroll
     for (int g = 0; g < GROUPS; ++g) {
       if (!there[g]) continue;
-      const uint32_t d = s32(dst) + to + g * (KEYS * 128);
-#pragma unroll 1
-      for (int r = 0; r < KEYS; r += 8) {
-        const int v = at + r + row, first = (v < ns ? from0 + v : from1 + v - ns) - row;
-        copy(d + r * 128, from[g] + first * node + (int64_t)head * size, g, on[g] && r + row < left);
+#pragma unroll 2
+      for (int r = row; r < KEYS; r += every) {
+        const int v = at + r;
+        copy(d + g * (KEYS * 128) + place(r), from[g] + (int64_t)(v < ns ? from0 + v : from1 + v - ns) * node + (int64_t)head * size, g, on[g] && r < left);
       }
     }
   }
   // the tile's own: `high` rows of one head after the other
   __device__ __forceinline__ void own(unsigned char* dst, int first, int left, int head, int high) const {
+    const uint32_t d = s32(dst);
 #pragma unroll
     for (int g = 0; g < GROUPS; ++g) {
       if (!there[g]) continue;
-      const uint32_t d = s32(dst) + to + g * (TILE_M * 128);
-      const T* f = from[g] + first * node + (int64_t)head * size;
-      int q = 0;
 #pragma unroll 2
-      for (int r = 0; r < TILE_M; r += 8) {
-        copy(d + r * 128, f + q * node, g, on[g] && q + row < left);
-        if ((q += 8) == high) q = 0, f += size;
+      for (int r = row; r < TILE_M; r += every) {
+        const int h = r / high, q = r - h * high;
+        copy(d + g * (TILE_M * 128) + place(r), from[g] + (int64_t)(first + q) * node + (int64_t)(head + h) * size, g, on[g] && q < left);
       }
     }
-  }
-  __device__ __forceinline__ void copy(uint32_t d, const T* f, int g, bool in) const {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(in ? f : from[g]), "r"(in ? 16 : 0) : "memory");
   }
 };
 
@@ -131,13 +138,7 @@ __device__ __forceinline__ uint64_t bits_of(int lo, int hi) {
   return hi > lo ? (~uint64_t(0) >> (64 - (hi - lo))) << lo : 0;
 }
 
-// What a tile walks over: `ns` first nodes of the chain that its first row is in, from `from0` on, then [from1, to1), as one sequence.
-struct Stretch {
-  int from0, ns, from1, to1, total, steps;
-};
-template <int MODE> __device__ __forceinline__ Stretch stretch_of(const TcParams& p, int first, int last) {       // rows first to last
-  const WindowParams& w = p.w;
-  const int2 a = p.spans[first], b = p.spans[last];
+template <int MODE> __device__ __forceinline__ Stretch stretch_of(const WindowParams& w, int first, int last, int2 a, int2 b) {       // rows first to last, their chains
   Stretch s;
   s.from0 = s.from1 = first;
   s.ns = 0;
@@ -169,8 +170,9 @@ __device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.s
 // A lane's row of results, with `more` where given, `f` times, to (n, components, heads, channels); whether all of it was finite.
 template <int DP> __device__ __forceinline__ bool put_row(uint32_t sum, float f, bool on, void* out, int row, int head, const AttentionParams& p, const float* more = nullptr) {
   bool finite = true;
-  const int values = p.comps * p.size;
+  const int values = p.comps * p.size, jump = (p.heads - 1) * p.size;     // to the head's next component, behind the last one's channels
   T* to = static_cast<T*>(out) + ((int64_t)row * p.comps * p.heads + head) * p.size;
+  int left = p.size;
 #pragma unroll
   for (int h = 0; h < DP; h += 32) {
     if (h >= values) break;
@@ -184,14 +186,14 @@ template <int DP> __device__ __forceinline__ bool put_row(uint32_t sum, float f,
       float v[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        v[j] = __uint_as_float(r[c + j]) + (more ? more[at + j] : 0.f);
+        v[j] = __uint_as_float(r[c + j]);
+        if (more) v[j] += more[at + j];
         finite = finite && is_finite(v[j]);
         v[j] *= f;
       }
-      const int comp = at / p.size;
-      if (on)
-        *reinterpret_cast<uint4*>(to + (int64_t)comp * p.heads * p.size + at - comp * p.size) =
-            make_uint4(two_bf16(v[0], v[1]), two_bf16(v[2], v[3]), two_bf16(v[4], v[5]), two_bf16(v[6], v[7]));
+      if (on) *reinterpret_cast<uint4*>(to) = make_uint4(two_bf16(v[0], v[1]), two_bf16(v[2], v[3]), two_bf16(v[4], v[5]), two_bf16(v[6], v[7]));
+      to += 8;
+      if ((left -= 8) == 0) to += jump, left = p.size;
     }
   }
   return finite;
@@ -204,25 +206,37 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
   unsigned char *own = smem, *ring = own + F::OWN * F::OWN_BYTES;
   float* numbers = reinterpret_cast<float*>(ring + SLOTS * F::SLOT_BYTES);
   uint64_t* bars = reinterpret_cast<uint64_t*>(ring + SLOTS * F::SLOT_BYTES + F::NUMBERS);
-  uint64_t *full = bars, *empty = full + SLOTS, *own_full = empty + SLOTS, *scores = own_full + 1, *weights = scores + BUFFERS, *freed = weights + BUFFERS, *done = freed + BUFFERS, *gathered = done + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gathered + 1);
+  uint64_t *full = bars, *empty = full + SLOTS, *scores = empty + SLOTS, *weights = scores + BUFFERS, *freed = weights + BUFFERS, *own_full = freed + BUFFERS,
+           *own_empty = own_full + 1, *done = own_empty + 1, *sums_free = done + 1, *gathered = sums_free + 1, *known = gathered + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(known + STRETCHES);
   int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
-  static_assert((2 * SLOTS + 3 + 3 * BUFFERS) * 8 + 8 <= 512, "barriers");
+  Stretch* stretches = reinterpret_cast<Stretch*>(reinterpret_cast<unsigned char*>(bars) + F::BARRIERS);
+  unsigned* bad_rows = reinterpret_cast<unsigned*>(stretches + STRETCHES);                                       // [softmax warp][tile of the CTA]
 
   const WindowParams& w = p.w;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   // A tile is `pack` heads that share their keys by `high` nodes: with fewer nodes, the walk over what any of them sees is shorter.
   const int pack = MODE == COLUMNS ? 1 : p.pack, high = TILE_M / pack, heads = (MODE == COLUMNS ? w.kv.heads : w.q.heads) / pack;
-  const int head = (int)(blockIdx.x % (unsigned)heads) * pack, kv = MODE == COLUMNS ? head : head / w.group;
-  const int first = (int)(blockIdx.x / (unsigned)heads) * high, last = min((int)w.q.n, first + high) - 1;
-  const Stretch walk = stretch_of<MODE>(p, first, last);
-  const int steps = walk.steps * (MODE == COLUMNS ? w.group : 1);
   const int values = w.q.comps * w.q.size, wide = (values + 15) / 16 * 16;
+  // A CTA takes every gridDim-th tile.  All roles go through the same tiles and steps and count them, and their barriers' phases, on.  The warps that copy find
+  // a tile's stretch, a tile ahead, and leave it for the others; these are fewer tiles behind than there are places, since scores have at most three buffers (and a barrier
+  // each: a wait by parity must not be two phases behind, as the softmax may be behind the tile's own rows).
+  struct Tile {
+    int head, kv, first, last;
+  };
+  auto tile_of = [&](unsigned i) {
+    Tile t;
+    t.head = (int)(i % (unsigned)heads) * pack;
+    t.kv = MODE == COLUMNS ? t.head : t.head / w.group;
+    t.first = (int)(i / (unsigned)heads) * high;
+    t.last = min((int)w.q.n, t.first + high) - 1;
+    return t;
+  };
 
   if (tid == 0) {
     *abort_flag = (s32(smem) & 1023) != 0;                // the swizzle goes by addresses
     for (int s = 0; s < SLOTS; ++s) {
-      bar_init(&full[s], !p.tma ? LOADERS : MODE == COLUMNS && !(s & 1) ? LOADERS + 1 : 1);
+      bar_init(&full[s], !p.tma ? LOADERS : MODE == COLUMNS && !(s & 1) ? 33 : 1);
       bar_init(&empty[s], 1);
     }
     bar_init(own_full, p.tma ? 1 : LOADERS);
@@ -231,8 +245,11 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
       bar_init(&weights[b], 4);
       bar_init(&freed[b], 1);
     }
-    bar_init(done, 1);                                   // all products
-    bar_init(gathered, LOADERS);                         // a mixed item where others are copied by TMA
+    for (int k = 0; k < STRETCHES; ++k) bar_init(&known[k], 1);
+    bar_init(own_empty, 1);                              // a tile's scores have been made
+    bar_init(done, 1);                                   // and its sums
+    bar_init(sums_free, MODE == COLUMNS && GROUPS > 1 ? 8 : 4);
+    bar_init(gathered, 32);                         // a mixed item where others are copied by TMA
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == F::SOFT) {
@@ -251,54 +268,76 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
     // copied by one thread (TMA); a stretch's first nodes, and all of other heads, by the threads: their copies arrive at the item's barrier when they have landed, and
     // the thread that issues the MMAs, which sees them all there, puts the fence between them and the tensor cores.  Copying by hand takes the warps
     // issue slots that the softmax wants (one chain of 32,781 nodes, 8 heads of 128 values, by hand and by TMA: HAND | TMA us).
-    const int thread = tid - 32 * (F::SOFT + 2);
-    const int left = last + 1 - first;
-    const Copier<DP> even(MODE == FORWARD ? w.q.k : MODE == ROWS ? w.q.v : w.q.q, w.q, thread);
-    const Copier<DP> odd(MODE == FORWARD ? w.q.v : MODE == ROWS ? w.q.k : w.q.g, w.q, thread);
-    if (!p.tma) {
-      Copier<DP>(MODE == COLUMNS ? w.q.k : w.q.q, w.q, thread).own(own, first, left, head, high);
-      if (MODE != FORWARD) Copier<DP>(MODE == COLUMNS ? w.q.v : w.q.g, w.q, thread).own(own + F::OWN_BYTES, first, left, head, high);
-      land_at(own_full);
-    } else if (thread == 0) {
-      bar_expect_tx(own_full, F::OWN * F::OWN_BYTES);
-      for (int x = 0; x < F::OWN; ++x)
-        for (int h = 0; h < pack; ++h)
-          for (int g = 0; g < DP / 64; ++g)
-            tma_load_3d(own + x * F::OWN_BYTES + g * (TILE_M * 128) + h * high * 128, &p.own[x], (head + h) * DP + g * 64, first, 0, own_full);
-    }
-    int at = 0, h = MODE == COLUMNS ? kv * w.group : kv;
-    for (int item = 0; item < 2 * steps; ++item) {
-      const int slot = item % SLOTS;
-      const bool mixed = MODE != COLUMNS && at < walk.ns, numbered = MODE == COLUMNS && !(item & 1);
-      if (!p.tma || mixed || numbered || thread == 0) {  // the others have nothing to do with tiles that are copied whole
-        if (item >= SLOTS && !bar_wait(&empty[slot], (uint32_t)((item / SLOTS - 1) & 1), ab)) break;
+    const int thread = tid - 32 * (F::SOFT + 2), threads = p.tma ? 32 : LOADERS;
+    const Copier<DP> even(MODE == FORWARD ? w.q.k : MODE == ROWS ? w.q.v : w.q.q, w.q, thread, threads);
+    const Copier<DP> odd(MODE == FORWARD ? w.q.v : MODE == ROWS ? w.q.k : w.q.g, w.q, thread, threads);
+    unsigned item = 0, mixed_items = 0, i = blockIdx.x;
+    Tile next = tile_of(i);
+    int2 a = p.spans[next.first], b = p.spans[next.last];
+    auto copy_tile = [&](const Tile& t, const Stretch& walk, int steps, int number) {
+      // All threads wait for every place, also where one copies: who skips waits gets phases ahead, and a wait by parity cannot tell a phase from the one but next.
+      if (number && !bar_wait(own_empty, (uint32_t)((number - 1) & 1), ab)) return false;
+      if (thread == 0) {
+        stretches[number % STRETCHES] = walk;
+        bar_arrive(&known[number % STRETCHES]);
+      }
+      if (!p.tma) {
+        const int left = t.last + 1 - t.first;
+        Copier<DP>(MODE == COLUMNS ? w.q.k : w.q.q, w.q, thread, threads).own(own, t.first, left, t.head, high);
+        if (MODE != FORWARD) Copier<DP>(MODE == COLUMNS ? w.q.v : w.q.g, w.q, thread, threads).own(own + F::OWN_BYTES, t.first, left, t.head, high);
+        land_at(own_full);
+      } else if (thread == 0) {
+        bar_expect_tx(own_full, F::OWN * F::OWN_BYTES);
+        for (int x = 0; x < F::OWN; ++x)
+          for (int h = 0; h < pack; ++h)
+            for (int g = 0; g < DP / 64; ++g)
+              tma_load_3d(own + x * F::OWN_BYTES + g * (TILE_M * 128) + h * high * 128, &p.own[x], (t.head + h) * DP + g * 64, t.first, 0, own_full);
+      }
+      int at = 0, h = MODE == COLUMNS ? t.kv * w.group : t.kv;
+      for (int k = 0; k < 2 * steps; ++k, ++item) {
+        const unsigned slot = item % SLOTS;
+        const bool mixed = MODE != COLUMNS && at < walk.ns, numbered = MODE == COLUMNS && !(k & 1);
+        if (item >= SLOTS && !bar_wait(&empty[slot], (uint32_t)((item / SLOTS - 1) & 1), ab)) return false;
         unsigned char* to = ring + slot * F::SLOT_BYTES;
-        const Copier<DP>& x = item & 1 ? odd : even;
+        const Copier<DP>& x = k & 1 ? odd : even;
         if (mixed) {
           x.mixed(to, at, walk.ns, walk.from0, walk.from1, walk.total - at, h);
           if (p.tma) {                                   // one arrival for all, none of whom is an item ahead
             land_at(gathered);
-            if (!bar_wait(gathered, (uint32_t)(item & 1), ab)) break;
+            if (!bar_wait(gathered, mixed_items++ & 1, ab)) return false;
             if (thread == 0) bar_arrive(&full[slot]);
           }
         } else if (!p.tma) {
           x.next(to, walk.from1 + at - walk.ns, walk.total - at, h);
         } else if (thread == 0) {
           bar_expect_tx(&full[slot], F::SLOT_BYTES);
-          for (int g = 0; g < DP / 64; ++g) tma_load_3d(to + g * (KEYS * 128), &p.ring[item & 1], h * DP + g * 64, walk.from1 + at - walk.ns, 0, &full[slot]);
+          for (int g = 0; g < DP / 64; ++g) tma_load_3d(to + g * (KEYS * 128), &p.ring[k & 1], h * DP + g * 64, walk.from1 + at - walk.ns, 0, &full[slot]);
         }
         if (numbered) {
-          const int i = walk.from1 + at + thread;
-          const bool there = i < walk.to1;
-          const int64_t from = there ? (int64_t)h * w.q.n + i : 0;
-          float* num = numbers + slot / 2 * 3 * KEYS + thread;
-          copy4(num, w.q.top + from, there);
-          copy4(num + KEYS, w.q.inverse + from, there);
-          copy4(num + 2 * KEYS, w.q.delta + from, there);
+          for (int c = thread; c < KEYS; c += threads) {
+            const int query = walk.from1 + at + c;
+            const bool there = query < walk.to1;
+            const int64_t from = there ? (int64_t)h * w.q.n + query : 0;
+            float* num = numbers + slot / 2 * 3 * KEYS + c;
+            copy4(num, w.q.top + from, there);
+            copy4(num + KEYS, w.q.inverse + from, there);
+            copy4(num + 2 * KEYS, w.q.delta + from, there);
+          }
         }
         if (!p.tma || numbered) land_at(&full[slot]);
+        if ((k & 1) && (at += KEYS) >= walk.total) at = 0, ++h;          // COLUMNS: the next head
       }
-      if ((item & 1) && (at += KEYS) >= walk.total) at = 0, ++h;         // COLUMNS: the next head
+      return true;
+    };
+    for (int number = 0; thread < threads; ++number) {
+      const Tile t = next;
+      const Stretch walk = stretch_of<MODE>(w, t.first, t.last, a, b);
+      const bool more = p.tiles - i > gridDim.x;
+      if (more) {
+        next = tile_of(i += gridDim.x);
+        a = p.spans[next.first], b = p.spans[next.last];
+      }
+      if (!copy_tile(t, walk, walk.steps * (MODE == COLUMNS ? w.group : 1), number) || !more) break;
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
   } else if (warp >= F::SOFT) {
@@ -308,12 +347,13 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
       const uint32_t to_scores = idesc_bf16(TILE_M, KEYS), to_sums = idesc_bf16(TILE_M, wide, false, true);
       const uint32_t own_at = s32(own), ring_at = s32(ring), sum = tmem + F::SUM_AT;
       const int ksteps = wide / 16;
-      auto slot_at = [&](int item) { return ring_at + (uint32_t)(item % SLOTS) * F::SLOT_BYTES; };
-      auto arrived = [&](int item) { return bar_wait(&full[item % SLOTS], (uint32_t)((item / SLOTS) & 1), ab); };
+      // of steps counted over all tiles
+      auto slot_at = [&](unsigned item) { return ring_at + item % SLOTS * F::SLOT_BYTES; };
+      auto arrived = [&](unsigned item) { return bar_wait(&full[item % SLOTS], (item / SLOTS) & 1, ab); };
       auto fence = [] { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); };
       // scores of a step are free when the products that read them BUFFERS steps before are done
-      auto free_again = [&](int j) { return j < BUFFERS || bar_wait(&freed[j % BUFFERS], (uint32_t)((j / BUFFERS - 1) & 1), ab); };
-      auto weighted = [&](int j) { return bar_wait(&weights[j % BUFFERS], (uint32_t)((j / BUFFERS) & 1), ab); };
+      auto free_again = [&](unsigned j) { return j < BUFFERS || bar_wait(&freed[j % BUFFERS], (j / BUFFERS - 1) & 1, ab); };
+      auto weighted = [&](unsigned j) { return bar_wait(&weights[j % BUFFERS], (j / BUFFERS) & 1, ab); };
       // d (128 rows x 64) = rows of the tile times rows of the slot
       auto score = [&](uint32_t d, uint32_t a, uint32_t b) {
         const uint32_t a_lo = umma_lo(a), b_lo = umma_lo(b);
@@ -332,7 +372,7 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
       };
       bool ok = true;
       constexpr int S_ITEM = MODE == ROWS ? 1 : 0;
-      auto make_s = [&](int j) {
+      auto make_s = [&](unsigned j) {
         ok = ok && arrived(2 * j + S_ITEM) && free_again(j);
         if (!ok) return;
         fence();
@@ -341,7 +381,7 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
         if (MODE == FORWARD) umma_commit(&empty[2 * j % SLOTS]);
       };
       // By rows, the place of dP is free when the softmax has read it.
-      auto make_dp = [&](int j) {
+      auto make_dp = [&](unsigned j) {
         ok = ok && arrived(2 * j + 1 - S_ITEM) && (MODE == COLUMNS || j < BUFFERS || weighted(j - BUFFERS));
         if (!ok) return;
         fence();
@@ -349,16 +389,24 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
         score(tmem + (j % BUFFERS) * F::BUFFER + KEYS, own_at + F::OWN_BYTES, slot_at(2 * j + 1 - S_ITEM));
         if (MODE == ROWS) umma_commit(&empty[2 * j % SLOTS]);
       };
-      if (warp == F::SOFT) {
-        ok = bar_wait(own_full, 0, ab);
-        for (int j = 0; j < steps && ok; ++j) {
-          if (MODE == ROWS) make_dp(j);
-          make_s(j);
-          if (MODE == COLUMNS) make_dp(j);
-          if (ok) umma_commit(&scores[j % BUFFERS]);
+      unsigned j = 0;
+      int number = 0;
+      for (unsigned i = blockIdx.x; i < p.tiles && ok; i += gridDim.x, ++number) {
+        ok = bar_wait(&known[number % STRETCHES], (uint32_t)(number / STRETCHES & 1), ab) && (warp != F::SOFT || bar_wait(own_full, (uint32_t)(number & 1), ab));
+        if (!ok) break;
+        const unsigned end = j + stretches[number % STRETCHES].steps * (MODE == COLUMNS ? w.group : 1);
+        if (warp == F::SOFT) {
+          for (; j < end && ok; ++j) {
+            if (MODE == ROWS) make_dp(j);
+            make_s(j);
+            if (MODE == COLUMNS) make_dp(j);
+            if (ok) umma_commit(&scores[j % BUFFERS]);
+          }
+          if (ok) umma_commit(own_empty);
+          continue;
         }
-      } else {
-        for (int j = 0; j < steps && ok; ++j) {
+        ok = number == 0 || bar_wait(sums_free, (uint32_t)((number - 1) & 1), ab);
+        for (bool more = false; j < end && ok; ++j, more = true) {
           const uint32_t d = tmem + (j % BUFFERS) * F::BUFFER;
           ok = arrived(2 * j + 1) && (MODE != COLUMNS || arrived(2 * j));
           if (!ok) break;
@@ -366,10 +414,10 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
           ok = weighted(j);
           if (!ok) break;
           tc_fence_after();
-          add(sum, d, slot_at(2 * j + 1), j > 0);
+          add(sum, d, slot_at(2 * j + 1), more);
           if (MODE == ROWS) add(sum, d + 32, slot_at(2 * j + 1), true);
           if (MODE == COLUMNS) {
-            add(sum + DP, d + KEYS, slot_at(2 * j), j > 0);
+            add(sum + DP, d + KEYS, slot_at(2 * j), more);
             umma_commit(&empty[2 * j % SLOTS]);
           }
           umma_commit(&empty[(2 * j + 1) % SLOTS]);
@@ -380,17 +428,34 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
     }
   } else {
     // ---------------- softmax ----------------
-    const int quarter = warp & 3, group = warp >> 2, place = quarter * 32 + lane, row = first + place % high, mine = head + place / high;       // its head
-    const bool there = row <= last;
-    const int2 span = there ? p.spans[row] : make_int2(0, 0);
-    const bool on = span.y > span.x;
+    const int quarter = warp & 3, group = warp >> 2, place = quarter * 32 + lane;
     const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16), sum_at = lanes + F::SUM_AT;
     const float unit = w.q.scale * LOG2E;
+    bool ok = true;
+    unsigned j0 = 0;                                     // steps of the tiles before
+    int tiles_done = 0;
+    // the lane's node, and a tile ahead its chain
+    const int in_tile = place % high, in_pack = place / high;
+    auto span_of = [&](unsigned i) {
+      const int row = (int)(i / (unsigned)heads) * high + in_tile;
+      return i < p.tiles && row < w.q.n ? p.spans[row] : make_int2(0, 0);
+    };
+    int2 next_span = span_of(blockIdx.x);
+    int number = 0;
+    for (unsigned i = blockIdx.x; i < p.tiles; i += gridDim.x, ++number) {
+    const Tile tile = tile_of(i);
+    const int row = tile.first + in_tile, mine = tile.head + in_pack;
+    const int2 span = next_span;
+    next_span = span_of(i + gridDim.x);
+    const bool on = span.y > span.x;
+    ok = __all_sync(0xffffffffu, bar_wait(&known[number % STRETCHES], (uint32_t)(number / STRETCHES & 1), ab));
+    if (!ok) break;
+    const Stretch walk = stretches[number % STRETCHES];
+    const int steps = walk.steps * (MODE == COLUMNS ? w.group : 1);
     // what the row sees: [lo, hi), and the first nodes [span.x, far)
     const int lo = !on ? 0 : max(span.x, row - (MODE == COLUMNS ? w.after : w.before));
     const int hi = !on ? 0 : MODE == COLUMNS ? (!w.split && row < span.x + w.sinks ? span.y : min(span.y, row + w.before + 1)) : min(span.y, row + w.after + 1);
     const int far = on && MODE != COLUMNS ? min(lo, span.x + w.sinks) : 0;
-    bool ok = true;
     // as bits of the 64 from the stretch's `at`-th on; first nodes are before `from1`, or in the stretch behind it, or both
     auto seen = [&](int at) {
       const int shift = walk.from1 - walk.ns + at;
@@ -401,18 +466,34 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
       }
       return bits;
     };
+    // all sums of the tile are there; after reading them they may be written again
+    auto sums_there = [&] {
+      ok = __all_sync(0xffffffffu, ok);
+      if (ok) ok = __all_sync(0xffffffffu, bar_wait(done, (uint32_t)(number & 1), ab));
+      tc_fence_after();
+      return ok;
+    };
+    auto sums_read = [&](bool bad) {
+      tc_fence_before();
+      const unsigned rows = __ballot_sync(0xffffffffu, bad);
+      if (lane == 0) {
+        bar_arrive(sums_free);
+        bad_rows[warp * MOST_TILES + number] = rows;
+      }
+      tiles_done = number + 1;
+    };
     if (MODE == FORWARD) {
       float base = -INFINITY, total = 0.f;
-      for (int j = 0; j < steps; ++j) {
-        const int b = j & 1;
-        ok = bar_wait(&scores[b], (uint32_t)((j >> 1) & 1), ab);
+      for (int k = 0; k < steps; ++k) {
+        const unsigned j = j0 + k, b = j & 1;
+        ok = bar_wait(&scores[b], (j >> 1) & 1, ab);
         if (!__all_sync(0xffffffffu, ok)) break;
         tc_fence_after();
         const uint32_t s_at = lanes + b * F::BUFFER;
         uint32_t raw[2][32];
         tmem_issue32(s_at, raw[0]);
         tmem_issue32(s_at + 32, raw[1]);
-        const uint64_t bits = seen(j * KEYS);
+        const uint64_t bits = seen(k * KEYS);
         tmem_arrived32(raw[0]);
         tmem_arrived32(raw[1]);
         if (!__all_sync(0xffffffffu, bits == ~uint64_t(0))) {
@@ -432,8 +513,8 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
           const float keep = !higher ? 1.f : base == -INFINITY ? 0.f : exp2_fast(base - now);
           total *= keep;
           if (higher) base = now;
-          if (j > 0) {
-            ok = bar_wait(&freed[(j - 1) & 1], (uint32_t)(((j - 1) >> 1) & 1), ab);
+          if (k > 0) {
+            ok = bar_wait(&freed[(j - 1) & 1], ((j - 1) >> 1) & 1, ab);
             if (!__all_sync(0xffffffffu, ok)) break;
             tc_fence_after();
 #pragma unroll
@@ -464,45 +545,23 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
         __syncwarp();
         if (lane == 0) bar_arrive(&weights[b]);
       }
-      ok = __all_sync(0xffffffffu, ok);
-      if (ok && steps) ok = __all_sync(0xffffffffu, bar_wait(done, 0, ab));
-      if (ok && steps) {
-        tc_fence_after();
+      if (sums_there()) {
         const float inverse = 1.f / total;
         const bool finite = put_row<DP>(sum_at, inverse, on, w.q.out, row, mine, w.q);
+        sums_read(on && !finite);
         if (on && w.q.top) w.q.top[(int64_t)mine * w.q.n + row] = base, w.q.inverse[(int64_t)mine * w.q.n + row] = inverse;
-        __syncwarp();
-        for (unsigned bad = __ballot_sync(0xffffffffu, on && !finite); bad; bad &= bad - 1) {
-          const int r = __ffs(bad) - 1;
-          again_forward<T>(w, __shfl_sync(0xffffffffu, row, r), __shfl_sync(0xffffffffu, mine, r), __shfl_sync(0xffffffffu, span.x, r), __shfl_sync(0xffffffffu, span.y, r), lane);
-        }
       }
     } else if (MODE == ROWS) {
-      const int64_t number = (int64_t)mine * w.q.n + row;
+      const int64_t at_row = (int64_t)mine * w.q.n + row;
       float top = INFINITY, inverse = 0.f, delta = 0.f;
-      if (on) {
-        top = w.q.top[number];
-        inverse = w.q.inverse[number];
-        const int64_t at = ((int64_t)row * w.q.comps * w.q.heads + mine) * w.q.size;
-        for (int e = 0; e < values; e += 8) {
-          const int comp = e / w.q.size;
-          const int64_t place = at + (int64_t)comp * w.q.heads * w.q.size + e - comp * w.q.size;
-          const uint4 a = *reinterpret_cast<const uint4*>(static_cast<const T*>(w.q.out) + place), b = *reinterpret_cast<const uint4*>(static_cast<const T*>(w.q.g.p) + place);
-          const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            delta = fmaf(__uint_as_float(x[i] << 16), __uint_as_float(y[i] << 16), delta);
-            delta = fmaf(__uint_as_float(x[i] & 0xffff0000u), __uint_as_float(y[i] & 0xffff0000u), delta);
-          }
-        }
-        if (group == 0) w.q.delta[number] = delta;
-      }
-      for (int j = group; j < steps; j += GROUPS) {
-        const int b = j % BUFFERS;
-        ok = bar_wait(&scores[b], (uint32_t)((j / BUFFERS) & 1), ab);
+      if (on) top = w.q.top[at_row], inverse = w.q.inverse[at_row], delta = w.q.delta[at_row];
+      static_assert(MODE != ROWS || GROUPS == 1, "one group by rows");
+      for (int k = 0; k < steps; ++k) {
+        const unsigned j = j0 + k, b = j % BUFFERS;
+        ok = bar_wait(&scores[b], (j / BUFFERS) & 1, ab);
         if (!__all_sync(0xffffffffu, ok)) break;
         tc_fence_after();
-        const uint64_t bits = seen(j * KEYS);
+        const uint64_t bits = seen(k * KEYS);
         const bool all = __all_sync(0xffffffffu, bits == ~uint64_t(0));
         uint32_t s[2][32], d[32], large[16], small[16];
         const uint32_t s_at = lanes + b * F::BUFFER;
@@ -535,23 +594,16 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
         __syncwarp();
         if (lane == 0) bar_arrive(&weights[b]);
       }
-      ok = __all_sync(0xffffffffu, ok);
-      if (ok && steps) ok = __all_sync(0xffffffffu, bar_wait(done, 0, ab));
-      if (ok && steps && group == 0) {
-        tc_fence_after();
+      if (sums_there()) {
         const bool finite = put_row<DP>(sum_at, w.q.scale, on, w.q.dq, row, mine, w.q);
-
-        __syncwarp();
-        for (unsigned bad = __ballot_sync(0xffffffffu, on && !finite); bad; bad &= bad - 1) {
-          const int r = __ffs(bad) - 1;
-          again_rows<T>(w, __shfl_sync(0xffffffffu, row, r), __shfl_sync(0xffffffffu, mine, r), __shfl_sync(0xffffffffu, span.x, r), __shfl_sync(0xffffffffu, span.y, r), lane);
-        }
+        sums_read(on && !finite);
       }
     } else {
-      int at = group % walk.steps * KEYS;
-      for (int j = group; j < steps; j += GROUPS) {
-        const int b = j % BUFFERS, slot = 2 * j % SLOTS;
-        ok = bar_wait(&full[slot], (uint32_t)((2 * j / SLOTS) & 1), ab) && bar_wait(&scores[b], (uint32_t)((j / BUFFERS) & 1), ab);
+      const int skip = (int)((group + GROUPS - j0 % GROUPS) % GROUPS);      // the groups take turns over all tiles' steps
+      int at = skip % walk.steps * KEYS;
+      for (int k = skip; k < steps; k += GROUPS) {
+        const unsigned j = j0 + k, b = j % BUFFERS, slot = 2 * j % SLOTS;
+        ok = bar_wait(&full[slot], (2 * j / SLOTS) & 1, ab) && bar_wait(&scores[b], (j / BUFFERS) & 1, ab);
         if (!__all_sync(0xffffffffu, ok)) break;
         tc_fence_after();
         const uint64_t bits = seen(at);
@@ -596,19 +648,29 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
         __syncwarp();
         if (lane == 0) bar_arrive(&weights[b]);
       }
+      // one group stores each sum, the others go on
       ok = __all_sync(0xffffffffu, ok);
-      if (ok && steps) ok = __all_sync(0xffffffffu, bar_wait(done, 0, ab));
-      if (ok && steps) {                                  // of two groups, one stores each sum
-        tc_fence_after();
+      if ((group == 0 || group == GROUPS - 1) && sums_there()) {
         bool finite = true;
-        const float* more = on ? far_of(w, row, kv, span.x, span.y) : nullptr;
-        if (group == 0) finite = put_row<DP>(sum_at, 1.f, on, w.kv.dv, row, kv, w.kv, more ? more + FAR_ROWS * values : nullptr);
-        if (group == GROUPS - 1) finite = put_row<DP>(sum_at + DP, w.q.scale, on, w.kv.dk, row, kv, w.kv, more) && finite;
-        __syncwarp();
-        for (unsigned bad = __ballot_sync(0xffffffffu, on && !finite); bad; bad &= bad - 1) {
-          const int r = __ffs(bad) - 1;
-          again_columns<T>(w, row - lane + r, kv, __shfl_sync(0xffffffffu, span.x, r), __shfl_sync(0xffffffffu, span.y, r), lane, group == 0, group == GROUPS - 1);
-        }
+        const float* more = on ? far_of(w, row, tile.kv, span.x, span.y) : nullptr;
+        if (group == 0) finite = put_row<DP>(sum_at, 1.f, on, w.kv.dv, row, tile.kv, w.kv, more ? more + FAR_ROWS * values : nullptr);
+        if (group == GROUPS - 1) finite = put_row<DP>(sum_at + DP, w.q.scale, on, w.kv.dk, row, tile.kv, w.kv, more) && finite;
+        sums_read(on && !finite);
+      }
+    }
+    j0 += steps;
+    if (!__all_sync(0xffffffffu, ok)) break;
+    }
+    // Rows that are not finite, when no role waits for this one any more: a row takes long.
+    __syncwarp();
+    for (int number = 0; number < tiles_done; ++number) {
+      const Tile tile = tile_of(blockIdx.x + number * gridDim.x);
+      for (unsigned bad = bad_rows[warp * MOST_TILES + number]; bad; bad &= bad - 1) {
+        const int at = quarter * 32 + __ffs(bad) - 1, row = tile.first + at % high, mine = tile.head + at / high;
+        const int2 span = p.spans[row];
+        if (MODE == FORWARD) again_forward<T>(w, row, mine, span.x, span.y, lane);
+        if (MODE == ROWS) again_rows<T>(w, row, mine, span.x, span.y, lane);
+        if (MODE == COLUMNS) again_columns<T>(w, row, tile.kv, span.x, span.y, lane, group == 0, group == GROUPS - 1);
       }
     }
   }
@@ -628,6 +690,31 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
   }
 }
 
+// delta = <g, out> of every node and head: `lanes` threads a head (a power of two), 16 bytes each, neighbouring heads side by side.  Apart from the rows' pass, whose
+// threads have a row each and would read both with a line for every 16 bytes.
+__global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ WindowParams p, int lanes) {
+  const int values = p.q.comps * p.q.size, lane = threadIdx.x & (lanes - 1);
+  const int64_t count = p.q.n * p.q.heads, step = (int64_t)gridDim.x * 256 / lanes, rounds = ceil_div(count, step);
+  int64_t at = (blockIdx.x * (int64_t)256 + threadIdx.x) / lanes;
+  for (int64_t k = 0; k < rounds; ++k, at += step) {     // as many for all: the shuffles want whole warps
+    const int64_t node = count <= UINT32_MAX ? (unsigned)at / (unsigned)p.q.heads : at / p.q.heads;
+    const int head = (int)(at - node * p.q.heads), e = lane * 8, comp = e / p.q.size;
+    float sum = 0.f;
+    if (at < count && e < values) {
+      const int64_t place = ((node * p.q.comps + comp) * p.q.heads + head) * p.q.size + e - comp * p.q.size;
+      const uint4 a = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.q.out) + place)), b = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.q.g.p) + place));
+      const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        sum = fmaf(__uint_as_float(x[i] << 16), __uint_as_float(y[i] << 16), sum);
+        sum = fmaf(__uint_as_float(x[i] & 0xffff0000u), __uint_as_float(y[i] & 0xffff0000u), sum);
+      }
+    }
+    for (int o = lanes >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (at < count && lane == 0) p.q.delta[(int64_t)head * p.q.n + node] = sum;
+  }
+}
+
 // The chain of every node, [0, 0) of none.
 __global__ void __launch_bounds__(256) spans_kernel(const int64_t* __restrict__ ptr, int64_t chains, int2* __restrict__ spans, int64_t n) {
   const int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x;
@@ -644,9 +731,11 @@ __global__ void __launch_bounds__(256) spans_kernel(const int64_t* __restrict__ 
 
 template <int DP, int MODE> int launch(const TcParams& p, cudaStream_t s) {
   using F = Form<DP, MODE>;
-  const int64_t grid = MODE == COLUMNS ? ceil_div(p.w.q.n, TILE_M) * p.w.kv.heads : ceil_div(p.w.q.n, TILE_M / p.pack) * (p.w.q.heads / p.pack);
-  if (grid > INT32_MAX) return fail(EQT_ERR_UNSUPPORTED, "window_attention: %lld tiles are more than one launch takes", (long long)grid);
+  const int64_t tiles = MODE == COLUMNS ? ceil_div(p.w.q.n, TILE_M) * p.w.kv.heads : ceil_div(p.w.q.n, TILE_M / p.pack) * (p.w.q.heads / p.pack);
+  if (tiles > INT32_MAX) return fail(EQT_ERR_UNSUPPORTED, "window_attention: %lld tiles are more than one launch takes", (long long)tiles);
+  const int64_t grid = std::min<int64_t>(tiles, std::max<int64_t>((int64_t)sm_count() * F::CTAS, ceil_div(tiles, MOST_TILES)));
   TcParams t = p;
+  t.tiles = (unsigned)tiles;
   const int64_t width = (int64_t)p.w.q.heads * DP, kv_width = (int64_t)p.w.kv.heads * DP;
   t.tma = p.w.q.comps == 1 && p.w.q.size == DP && p.w.q.q.node >= width && p.w.q.k.node >= kv_width && p.w.q.v.node >= kv_width;
   if (t.tma) {
@@ -683,6 +772,10 @@ int eqt::window::tc_forward(const TcParams& p, cudaStream_t s) {
 }
 int eqt::window::tc_backward(const TcParams& p, cudaStream_t s) {
   const bool narrow = p.w.q.comps * p.w.q.size <= 64;
+  int lanes = 1;
+  while (lanes * 8 < p.w.q.comps * p.w.q.size) lanes *= 2;
+  delta_kernel<<<flat_grid(ceil_div(p.w.q.n * p.w.q.heads * lanes, 2), 256), 256, 0, s>>>(p.w, lanes);
+  if (int rc = check_launch("window_delta")) return rc;
   if (int rc = narrow ? launch<64, ROWS>(p, s) : launch<128, ROWS>(p, s)) return rc;
   if (p.w.split)
     if (int rc = far_bf16(p.w, s)) return rc;

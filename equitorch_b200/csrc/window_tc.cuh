@@ -11,6 +11,7 @@ struct alignas(64) TcParams {
   CUtensorMap own[2], ring[2];   // where `tma`: of the tile's operands, and of the others in the order of their use
   WindowParams w;
   const int2* spans;         // [node]: its chain
+  unsigned tiles;
   int* status;
   int pack;                  // heads of a tile, by rows: a power of two of at most eight that divides the heads that share keys
   int tma;                   // a head's rows are one or two whole lines of 64 values: tiles are copied by the tensor memory accelerator

@@ -125,6 +125,23 @@ def test_many_tiles_at_once(size):
         assert all(torch.equal(a, b) for a, b in zip(first, run(qkv, g, graphs, 8, 64, 64, 4, kv_heads=2)))
 
 
+@pytest.mark.parametrize("size", [64, 128, 32])
+@pytest.mark.parametrize("window", [(3, 3, 0), (0, 0, 1), (40, 0, 2), (700, 0, 4), (64, 64, 300)])
+def test_many_tiles_of_few_and_many_steps(window, size):
+    """Thousands of tiles, of one step and of dozens, one after the other on an SM: the same bits each time, and those of the chains one by one."""
+    sizes = [3 + (i * 37) % 60 for i in range(300)] + [1500, 2, 900] + [20] * 200
+    qkv, g, graphs = make(sizes, 1, 8, 2, size, torch.bfloat16)
+    first = run(qkv, g, graphs, 8, *window, kv_heads=2)
+    for _ in range(5):
+        assert all(torch.equal(a, b) for a, b in zip(first, run(qkv, g, graphs, 8, *window, kv_heads=2)))
+    ends = torch.tensor([0] + sizes).cumsum(0).tolist()
+    for c in (0, 17, 299, 300, 301, 302, 400):
+        lo, hi = ends[c], ends[c + 1]
+        part = [t.detach()[lo:hi].clone().requires_grad_(True) for t in qkv]
+        want, bound = reference(*part, g[lo:hi], seen((hi - lo,), hi - lo, *window), 8, 2, None)
+        compare([t[lo:hi] for t in first], want, bound)
+
+
 def test_no_nodes():
     qkv, g, graphs = make((), 1, 2, 2, 16, torch.float32)
     assert [t.shape[0] for t in run(qkv, g, graphs, 2, 3)] == [0] * 4
