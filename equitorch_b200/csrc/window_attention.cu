@@ -38,9 +38,9 @@ WindowParams params(const eqt_window_attention_args& a) {
   q.vec = bits % 16 == 0 && strides % v == 0 && a.head_channels % v == 0;
   p.kv = q;
   p.kv.heads = a.kv_heads;
-  // A tile of keys that holds a chain's first nodes would walk to the chain's end, alone, while the others are done: one chain of 32,781 nodes, 8 heads of 128
-  // values, window of 1024, backward by columns 876 us, with these queries apart 390 in all.  Two launches more, so not for what is walked in a few steps; and not for so
-  // many first nodes that tiles are full of them.
+  // A tile of keys that holds a chain's first nodes would walk to the chain's end, alone, while the others are done (one chain of 32,781 nodes, 8 heads of 128
+  // values, window of 1024: by columns 876 us; with these queries apart 473 and 62 for them).  Two launches more, so not for what is walked in a few steps (240
+  // chains of 50 to 500 nodes, window of 64 on both sides: 217 us walked, 164 and 61 apart); and not for so many first nodes that tiles are full of them.
   p.ptr = a.ptr, p.chains = a.num_graphs;
   p.split = p.sinks > 0 && p.sinks <= MOST_SPLIT_SINKS && a.longest - p.before > 2 * FAR_BLOCK;
   return p;

@@ -448,7 +448,7 @@ __global__ void __launch_bounds__(256) window_far_join_kernel(const __grid_const
 
 // ---- host side ----------------------------------------------------------------------------------
 template <typename T, int DP> int launch_far(const WindowParams& p, cudaStream_t s) {
-  constexpr int KT = DP > 64 ? 16 : 32;
+  constexpr int KT = DP > 32 ? 16 : 32;
   using S = attention::Shape<T, DP, 1, KT>;
   const int64_t pairs = ceil_div(p.q.n, FAR_BLOCK) + p.chains;
   if (pairs > INT32_MAX || p.kv.heads > 65535) return fail(EQT_ERR_UNSUPPORTED, "window_attention: %lld chains are more than one launch takes", (long long)p.chains);
