@@ -11,10 +11,13 @@ from .graph_layers import SO3LinearGraph
 from .linears import IrrepsLinear, IrrepWiseLinear, SO2Linear, SO3Linear
 from .norm import MeanSquaredNorm, Norm, SquaredNorm
 from .normalization import BatchRMSNorm, LayerRMSNorm
+from .residual_norm import AddRMSNorm
 from .sphericals import SphericalHarmonics
 from .tensor_products import TensorDot, TensorProduct
+from .type_loss import TypeCrossEntropy
 from .wigner_d import DenseWignerRotation, SparseWignerRotation, WignerD
+from .window import WindowAttention
 
 __all__ = ["Gate", "MeanSquaredNorm", "Norm", "SquaredNorm", "BatchRMSNorm", "LayerRMSNorm", "SinCos", "IrrepsLinear", "IrrepWiseLinear", "SO2Linear", "SO3Linear", "SO3LinearGraph", "SphericalHarmonics",
-           "TypeEmbedding", "GraphAttention", "GatedLinear",
+           "TypeEmbedding", "GraphAttention", "GatedLinear", "AddRMSNorm", "WindowAttention", "TypeCrossEntropy",
            "TensorDot", "TensorProduct", "DenseWignerRotation", "SparseWignerRotation", "WignerD", "functional"]
