@@ -112,7 +112,7 @@ class WindowAttentionArgs(C.Structure):
     _fields_ = ([(f, C.c_int32) for f in ("dtype", "comps", "heads", "kv_heads", "head_channels", "tile_rows")] + [("scale", C.c_float)]
                 + [(f, C.c_int64) for f in ("n", "num_graphs", "longest", "num_tiles", "before", "after", "sinks", "q_node", "q_comp", "k_node", "k_comp",
                                             "v_node", "v_comp", "scratch_bytes")]
-                + [(f, C.c_void_p) for f in ("ptr", "tiles", "q", "k", "v", "grad", "out", "dq", "dk", "dv", "stats", "scratch", "status")])
+                + [(f, C.c_void_p) for f in ("ptr", "tiles", "q", "k", "v", "grad", "out", "rest", "dq", "dk", "dv", "stats", "scratch", "status")])
 
 
 class TypeLossArgs(C.Structure):
@@ -232,7 +232,7 @@ SIGNATURES = {
     "eqt_add_rms_norm_forward": (C.c_int, [C.c_int32] + [C.c_void_p] * 6 + [C.c_int64] * 3 + [C.c_double, C.c_void_p]),
     "eqt_add_rms_norm_e4m3": (C.c_int, [C.c_int32] + [C.c_void_p] * 6 + [C.c_int64] * 4 + [C.c_double, C.c_void_p]),
     "eqt_add_rms_norm_scratch": (C.c_int64, [C.c_int32] + [C.c_int64] * 3),
-    "eqt_add_rms_norm_backward": (C.c_int, [C.c_int32] + [C.c_void_p] * 8 + [C.c_int64] * 4 + [C.c_void_p]),
+    "eqt_add_rms_norm_backward": (C.c_int, [C.c_int32] + [C.c_void_p] * 9 + [C.c_int64] * 4 + [C.c_void_p]),
     "eqt_rotary": (C.c_int, [C.POINTER(RotaryArgs), C.c_void_p]),
     "eqt_window_step_scratch": (C.c_int64, [C.POINTER(WindowStepArgs)]),
     "eqt_window_step": (C.c_int, [C.POINTER(WindowStepArgs), C.c_void_p]),

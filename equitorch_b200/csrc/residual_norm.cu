@@ -7,8 +7,9 @@
 //         dx = dres = gh + r (gw - u mean(gw u))        dw[channel] = sum over nodes and components of g u
 //     8 bits: of every group of values, t = h w, m = max |t|:   value = e4m3(448 t / m), scale = m r / 448
 //
-// All of it is bound by HBM: 16 bytes a bfloat16 value and its residual forward and backward.  A row stays in the registers of 32, 128 or 512
-// threads, one, two or four pieces of 16 bytes each: one reads x and the residual, adds, reduces by shuffles and writes.  A CTA
+// All of it is bound by HBM: 16 bytes a bfloat16 value and its residual forward and backward.  Of bfloat16 the backward pass reads x and the residual and not the
+// sum as it was returned, whose rounding would go into dw beside dw's own (2-norm of the error 2.5e-3 | 1.7e-3; backward pass
+// 137 | WITH us).  A row stays in the registers of 32, 128 or 512 threads, one, two or four pieces of 16 bytes each: one reads x and the residual, adds, reduces by shuffles and writes.  A CTA
 // strides over the rows, so the weight is read once and the backward pass has the weight's gradient in registers, summed over the CTA's rows; the
 // CTAs' sums are added in their order by a second kernel (no atomics).  Rows that are no whole pieces of 16 bytes, or longer than 2048
 // pieces, are read twice by loops.
@@ -49,6 +50,12 @@ template <typename T> __device__ __forceinline__ void unpack(const uint4& u, flo
       v[2 * i + 1] = __uint_as_float(r[i] & 0xffff0000u);
     }
   }
+}
+template <typename T> __device__ __forceinline__ void add_to(const uint4& u, float (&v)[VALUES<T>]) {
+  float a[VALUES<T>];
+  unpack<T>(u, a);
+#pragma unroll
+  for (int j = 0; j < VALUES<T>; ++j) v[j] += a[j];
 }
 template <typename T> __device__ __forceinline__ uint4 pack(const float (&v)[VALUES<T>]) {
   uint32_t r[4];
@@ -312,7 +319,7 @@ __global__ void __launch_bounds__(ROW_THREADS < 128 ? 128 : ROW_THREADS, OUT != 
 }
 
 // parts [CTA][values of a row]: the CTA's sums of g u
-template <typename T, int ROW_THREADS, int PIECES>
+template <typename T, int ROW_THREADS, int PIECES, bool RES>
 __global__ void __launch_bounds__(ROW_THREADS < 128 ? 128 : ROW_THREADS) backward_kernel(const NormArgs p) {
   constexpr int V = VALUES<T>, ROWS = ROW_THREADS < 128 ? 128 / ROW_THREADS : 1;
   __shared__ float buffer[2][ROW_THREADS / 32];
@@ -330,32 +337,36 @@ __global__ void __launch_bounds__(ROW_THREADS < 128 ? 128 : ROW_THREADS) backwar
   }
   int turn = 0;
   constexpr bool AHEAD = PIECES <= 2;
-  uint4 g[PIECES], t[PIECES], s[PIECES], next_g[PIECES], next_t[PIECES], next_s[PIECES];
+  uint4 g[PIECES], t[PIECES], e[PIECES], s[PIECES], next_g[PIECES], next_t[PIECES], next_e[PIECES], next_s[PIECES];
   float inverse, next_inverse = 0.f;
-  auto ask = [&](int64_t row, uint4 (&a)[PIECES], uint4 (&b)[PIECES], uint4 (&c)[PIECES], float& root) {
+  auto ask = [&](int64_t row, uint4 (&a)[PIECES], uint4 (&b)[PIECES], uint4 (&d)[PIECES], uint4 (&c)[PIECES], float& root) {
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
       const int k = at + i * ROW_THREADS;
       const bool on = row < p.n && k < pieces;
       a[i] = on ? __ldg(reinterpret_cast<const uint4*>(p.g) + row * pieces + k) : make_uint4(0, 0, 0, 0);
       b[i] = on ? __ldg(reinterpret_cast<const uint4*>(p.total) + row * pieces + k) : make_uint4(0, 0, 0, 0);
+      if (RES) d[i] = on ? __ldg(reinterpret_cast<const uint4*>(p.res) + row * pieces + k) : make_uint4(0, 0, 0, 0);
       c[i] = p.gh && on ? __ldg(reinterpret_cast<const uint4*>(p.gh) + row * pieces + k) : make_uint4(0, 0, 0, 0);
     }
     root = row < p.n ? __ldg(p.rstd + row) : 0.f;
   };
   const int64_t step = (int64_t)gridDim.x * ROWS;
-  if (AHEAD) ask((int64_t)blockIdx.x * ROWS + threadIdx.x / ROW_THREADS, next_g, next_t, next_s, next_inverse);
+  if (AHEAD) ask((int64_t)blockIdx.x * ROWS + threadIdx.x / ROW_THREADS, next_g, next_t, next_e, next_s, next_inverse);
   for (int64_t row0 = (int64_t)blockIdx.x * ROWS; row0 < p.n; row0 += step, turn ^= 1) {
     const int64_t row = row0 + threadIdx.x / ROW_THREADS;
     const bool there = row < p.n;
     const int64_t first = row * pieces;
     if constexpr (AHEAD) {
 #pragma unroll
-      for (int i = 0; i < PIECES; ++i) g[i] = next_g[i], t[i] = next_t[i], s[i] = next_s[i];
+      for (int i = 0; i < PIECES; ++i) {
+        g[i] = next_g[i], t[i] = next_t[i], s[i] = next_s[i];
+        if (RES) e[i] = next_e[i];
+      }
       inverse = next_inverse;
-      ask(row + step, next_g, next_t, next_s, next_inverse);
+      ask(row + step, next_g, next_t, next_e, next_s, next_inverse);
     } else {
-      ask(row, g, t, s, inverse);
+      ask(row, g, t, e, s, inverse);
     }
     float sum = 0.f;
 #pragma unroll
@@ -364,6 +375,7 @@ __global__ void __launch_bounds__(ROW_THREADS < 128 ? 128 : ROW_THREADS) backwar
       unpack<T>(g[i], a);
       unpack<T>(w[i], c);
       unpack<T>(t[i], h);
+      if (RES) add_to<T>(e[i], h);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         const float u = h[j] * inverse;
@@ -375,13 +387,14 @@ __global__ void __launch_bounds__(ROW_THREADS < 128 ? 128 : ROW_THREADS) backwar
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
       const int k = at + i * ROW_THREADS;
-      float a[V], c[V], h[V], e[V], out[V];
+      float a[V], c[V], h[V], more[V], out[V];
       unpack<T>(g[i], a);
       unpack<T>(w[i], c);
       unpack<T>(t[i], h);
-      unpack<T>(s[i], e);
+      if (RES) add_to<T>(e[i], h);
+      unpack<T>(s[i], more);
 #pragma unroll
-      for (int j = 0; j < V; ++j) out[j] = fmaf(inverse, fmaf(-(h[j] * inverse), mean, p.w ? a[j] * c[j] : a[j]), e[j]);
+      for (int j = 0; j < V; ++j) out[j] = fmaf(inverse, fmaf(-(h[j] * inverse), mean, p.w ? a[j] * c[j] : a[j]), more[j]);
       if (there && k < pieces) reinterpret_cast<uint4*>(p.dx)[first + k] = pack<T>(out);
     }
   }
@@ -477,28 +490,32 @@ template <typename T, bool EIGHT> __global__ void __launch_bounds__(LONG_THREADS
 
 template <typename T> __global__ void __launch_bounds__(LONG_THREADS) backward_long_kernel(const NormArgs p) {
   __shared__ float buffer[2][LONG_THREADS / 32];
-  const T *g = static_cast<const T*>(p.g), *gh = static_cast<const T*>(p.gh), *total = static_cast<const T*>(p.total), *w = static_cast<const T*>(p.w);
+  const T *g = static_cast<const T*>(p.g), *gh = static_cast<const T*>(p.gh), *total = static_cast<const T*>(p.total), *res = static_cast<const T*>(p.res), *w = static_cast<const T*>(p.w);
   int turn = 0;
   for (int64_t row = blockIdx.x; row < p.n; row += gridDim.x, turn ^= 1) {
     const int64_t first = row * p.length;
     const float inverse = p.rstd[row];
     auto weighted = [&](int k) { return w ? ld(g + first + k) * ld(w + k % p.channels) : ld(g + first + k); };
+    auto unit = [&](int k) { return (ld(total + first + k) + (res ? ld(res + first + k) : 0.f)) * inverse; };
     float sum = 0.f;
-    for (int k = threadIdx.x; k < p.length; k += LONG_THREADS) sum = fmaf(weighted(k), ld(total + first + k) * inverse, sum);
+    for (int k = threadIdx.x; k < p.length; k += LONG_THREADS) sum = fmaf(weighted(k), unit(k), sum);
     const float mean = across_row<LONG_THREADS>(sum, buffer[turn], Sum()) / (float)p.length;
     for (int k = threadIdx.x; k < p.length; k += LONG_THREADS)
-      st(static_cast<T*>(p.dx) + first + k, fmaf(inverse, fmaf(-(ld(total + first + k) * inverse), mean, weighted(k)), gh ? ld(gh + first + k) : 0.f));
+      st(static_cast<T*>(p.dx) + first + k, fmaf(inverse, fmaf(-unit(k), mean, weighted(k)), gh ? ld(gh + first + k) : 0.f));
   }
 }
 // The weight's gradient of such rows: a thread has a place of the row, a CTA a part of the rows.
 template <typename T> __global__ void __launch_bounds__(LONG_THREADS) weight_long_kernel(const NormArgs p, int64_t part_rows) {
-  const T *g = static_cast<const T*>(p.g), *total = static_cast<const T*>(p.total);
+  const T *g = static_cast<const T*>(p.g), *total = static_cast<const T*>(p.total), *res = static_cast<const T*>(p.res);
   const int k = blockIdx.y * LONG_THREADS + threadIdx.x;
   if (k >= p.length) return;
   const int64_t end = min(p.n, (int64_t)(blockIdx.x + 1) * part_rows);
   float sum = 0.f;
 #pragma unroll 4
-  for (int64_t row = blockIdx.x * part_rows; row < end; ++row) sum = fmaf(ld(g + row * p.length + k), ld(total + row * p.length + k) * __ldg(p.rstd + row), sum);
+  for (int64_t row = blockIdx.x * part_rows; row < end; ++row) {
+    const int64_t at = row * p.length + k;
+    sum = fmaf(ld(g + at), (ld(total + at) + (res ? ld(res + at) : 0.f)) * __ldg(p.rstd + row), sum);
+  }
   p.parts[(int64_t)blockIdx.x * p.length + k] = sum;
 }
 
@@ -584,7 +601,8 @@ template <typename T> int launch_backward(const NormArgs& p, Rows r, cudaStream_
     parts = (int)part_ctas(r.threads, p.n);
     with_rows(r, [&](auto threads, auto pieces) {
       constexpr int N = decltype(threads)::value, K = decltype(pieces)::value;
-      backward_kernel<T, N, K><<<parts, N < 128 ? 128 : N, 0, s>>>(p);
+      if (p.res) backward_kernel<T, N, K, true><<<parts, N < 128 ? 128 : N, 0, s>>>(p);
+      else backward_kernel<T, N, K, false><<<parts, N < 128 ? 128 : N, 0, s>>>(p);
     });
     if (int rc = check_launch("add_rms_norm_backward")) return rc;
   } else {
@@ -650,8 +668,8 @@ extern "C" int64_t eqt_add_rms_norm_scratch(int32_t dtype, int64_t n, int64_t co
   return std::max<int64_t>(rows.threads ? part_ctas(rows.threads, n) : 0, long_parts(n)) * comps * channels;
 }
 
-extern "C" int eqt_add_rms_norm_backward(int32_t dtype, const void* grad, const void* grad_total, const void* total, const void* weight, const float* rstd,
-                                         void* dx, void* dweight, float* scratch, int64_t scratch_floats, int64_t n, int64_t comps, int64_t channels,
+extern "C" int eqt_add_rms_norm_backward(int32_t dtype, const void* grad, const void* grad_total, const void* total, const void* residual, const void* weight,
+                                         const float* rstd, void* dx, void* dweight, float* scratch, int64_t scratch_floats, int64_t n, int64_t comps, int64_t channels,
                                          void* stream) {
   if (int rc = check(dtype, n, comps, channels)) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -664,8 +682,8 @@ extern "C" int eqt_add_rms_norm_backward(int32_t dtype, const void* grad, const 
     return fail(EQT_ERR_BAD_ARGUMENT, "add_rms_norm backward: %lld values of scratch given, %lld needed", (long long)scratch_floats,
                 (long long)eqt_add_rms_norm_scratch(dtype, n, comps, channels));
   NormArgs p{};
-  p.g = grad, p.gh = grad_total, p.total = const_cast<void*>(total), p.w = weight, p.rstd = const_cast<float*>(rstd), p.dx = dx, p.dw = dweight;
+  p.g = grad, p.gh = grad_total, p.total = const_cast<void*>(total), p.res = residual, p.w = weight, p.rstd = const_cast<float*>(rstd), p.dx = dx, p.dw = dweight;
   p.parts = dweight ? scratch : nullptr, p.n = n, p.length = (int)(comps * channels), p.channels = (int)channels;
-  const Rows rows = rows_of(dtype, p.length, channels, bits_of({grad, grad_total, total, weight, dx}));
+  const Rows rows = rows_of(dtype, p.length, channels, bits_of({grad, grad_total, total, residual, weight, dx}));
   return dtype == EQT_F32 ? launch_backward<float>(p, rows, s) : launch_backward<__nv_bfloat16>(p, rows, s);
 }

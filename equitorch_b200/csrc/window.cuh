@@ -8,6 +8,10 @@
 //
 // over the heads that share k and v, for dk and dv.
 //
+// Where a weight is almost one, dP - delta is what two such numbers leave, and delta has to be that of the very weights: sum_j P_ij dP_ij.  bfloat16 weights are
+// rounded for their product with v, so the forward pass divides by the sum of the rounded ones and keeps what the rounding of its result left; the rows' pass takes
+// the same rounded weights, whose delta is <g, out + rest>.  On its way it sums P, and P dP, of the weights before rounding, by which the columns go.
+//
 // A tile's products run over nodes that some of its rows do not see, with weights of zero, and zero times infinity or a NaN is a NaN.  So a row whose
 // result is not finite is done again, one visible node at a time (`again_*`): a NaN that is not seen does not reach it, and one that is seen does.
 #pragma once
@@ -26,6 +30,8 @@ struct WindowParams {
   int before, after, sinks, group;
   // Gradients of the first nodes of chains from queries behind their windows, made apart (SPLIT) because a chain may have any number of those: sums of dS q and of P g
   // by blocks of FAR_BLOCK nodes of the batch, [pair of a block and a chain][head of keys][16 first nodes][dk, dv][node][value], then joined in the chain's first place.
+  void* rest;                // what the rounding of the results left (bfloat16, for the backward pass)
+  float* inverse;            // [head][node]: one over the sum of weights as the columns have them, not rounded
   const int64_t* ptr;
   int64_t chains;
   float* far;
@@ -97,11 +103,18 @@ template <typename T> __device__ __noinline__ void again_forward(const WindowPar
     top = now;
   }
   lane_put<T>(p.q.out, o, 1.f / sum, i, head, p.q, lane);
+  if (!p.rest) return;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const float x = o[c] / sum;
+    o[c] = x - static_cast<float>(static_cast<T>(x));
+  }
+  lane_put<T>(p.rest, o, 1.f, i, head, p.q, lane);
 }
 template <typename T> __device__ __noinline__ void again_rows(const WindowParams& p, int i, int head, int lo, int hi, int lane) {
   const int kv = head / p.group;
   const int64_t at = (int64_t)head * p.q.n + i;
-  const float top = p.q.top[at], inverse = p.q.inverse[at], delta = p.q.delta[at];
+  const float top = p.q.top[at], inverse = p.inverse[at], delta = p.q.delta[at];
   float q[4], k[4], v[4], g[4], dq[4] = {0.f, 0.f, 0.f, 0.f};
   lane_row<T>(q, p.q.q, i, head, p.q, lane);
   lane_row<T>(g, p.q.g, i, head, p.q, lane);
@@ -126,7 +139,7 @@ template <typename T> __device__ __noinline__ void again_columns(const WindowPar
       const int64_t at = (int64_t)head * p.q.n + i;
       lane_row<T>(q, p.q.q, i, head, p.q, lane);
       lane_row<T>(g, p.q.g, i, head, p.q, lane);
-      const float w = exp2_fast(lanes_dot(q, k) * (p.q.scale * LOG2E) - p.q.top[at]) * p.q.inverse[at], ds = w * (lanes_dot(g, v) - p.q.delta[at]);
+      const float w = exp2_fast(lanes_dot(q, k) * (p.q.scale * LOG2E) - p.q.top[at]) * p.inverse[at], ds = w * (lanes_dot(g, v) - p.q.delta[at]);
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         dv[c] = fmaf(w, g[c], dv[c]);

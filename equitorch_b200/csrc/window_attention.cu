@@ -34,14 +34,14 @@ WindowParams params(const eqt_window_attention_args& a) {
   const int v = a.dtype == EQT_F32 ? 4 : 8;
   const int64_t strides = a.q_node | a.q_comp | a.k_node | a.k_comp | a.v_node | a.v_comp;
   uintptr_t bits = 0;
-  for (const void* x : {a.q, a.k, a.v, a.grad, (const void*)a.out, (const void*)a.dq, (const void*)a.dk, (const void*)a.dv}) bits |= reinterpret_cast<uintptr_t>(x);
+  for (const void* x : {a.q, a.k, a.v, a.grad, (const void*)a.out, (const void*)a.rest, (const void*)a.dq, (const void*)a.dk, (const void*)a.dv}) bits |= reinterpret_cast<uintptr_t>(x);
   q.vec = bits % 16 == 0 && strides % v == 0 && a.head_channels % v == 0;
   p.kv = q;
   p.kv.heads = a.kv_heads;
   // A tile of keys that holds a chain's first nodes would walk to the chain's end, alone, while the others are done (one chain of 32,781 nodes, 8 heads of 128
   // values, window of 1024: by columns 876 us; with these queries apart 473 and 62 for them).  Two launches more, so not for what is walked in a few steps (240
   // chains of 50 to 500 nodes, window of 64 on both sides: 217 us walked, 164 and 61 apart); and not for so many first nodes that tiles are full of them.
-  p.ptr = a.ptr, p.chains = a.num_graphs;
+  p.ptr = a.ptr, p.chains = a.num_graphs, p.rest = a.dtype == EQT_BF16 ? a.rest : nullptr;
   p.split = p.sinks > 0 && p.sinks <= MOST_SPLIT_SINKS && a.longest - p.before > 2 * FAR_BLOCK;
   return p;
 }
@@ -51,19 +51,19 @@ WindowParams params(const eqt_window_attention_args& a) {
 bool on_tensor_cores(const eqt_window_attention_args& a) {
   if (a.dtype != EQT_BF16 || !(a.scale > 0.f)) return false;
   const int64_t strides = a.q_node | a.q_comp | a.k_node | a.k_comp | a.v_node | a.v_comp;
-  const uintptr_t bits = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) | reinterpret_cast<uintptr_t>(a.out) |
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) | reinterpret_cast<uintptr_t>(a.out) | reinterpret_cast<uintptr_t>(a.rest) |
                          reinterpret_cast<uintptr_t>(a.grad) | reinterpret_cast<uintptr_t>(a.dq) | reinterpret_cast<uintptr_t>(a.dk) | reinterpret_cast<uintptr_t>(a.dv);
   return bits % 16 == 0 && strides % 8 == 0 && a.head_channels % 8 == 0;
 }
 
-// Scratch: the nodes' chains, and for the backward pass the deltas and what far queries give first nodes.
+// Scratch: the nodes' chains, and for the backward pass the deltas, the inverse sums and what far queries give first nodes.
 int64_t spans_bytes(const eqt_window_attention_args& a) { return a.dtype == EQT_BF16 ? (int64_t)up((size_t)a.n * sizeof(int2)) : 0; }
 int64_t delta_bytes(const eqt_window_attention_args& a) { return (int64_t)up((size_t)a.heads * a.n * 4); }
 int64_t scratch_bytes(const eqt_window_attention_args& a, bool backward) {
   if (!backward) return spans_bytes(a);
   const WindowParams p = params(a);
   const int64_t pairs = ceil_div(a.n, FAR_BLOCK) + a.num_graphs;
-  return spans_bytes(a) + delta_bytes(a) + (p.split ? pairs * a.kv_heads * far_groups(p) * 2 * FAR_ROWS * a.comps * a.head_channels * 4 : 0);
+  return spans_bytes(a) + 2 * delta_bytes(a) + (p.split ? pairs * a.kv_heads * far_groups(p) * 2 * FAR_ROWS * a.comps * a.head_channels * 4 : 0);
 }
 int check_scratch(const eqt_window_attention_args& a, bool backward) {
   const int64_t need = scratch_bytes(a, backward);
@@ -101,7 +101,7 @@ extern "C" int eqt_window_attention_forward(const eqt_window_attention_args* arg
   if (int rc = check(args)) return rc;
   const eqt_window_attention_args& a = *args;
   if (a.n == 0 || a.num_tiles == 0) return EQT_OK;
-  if (!a.q || !a.k || !a.v || !a.out || !a.tiles) return fail(EQT_ERR_BAD_ARGUMENT, "window_attention: NULL pointer");
+  if (!a.q || !a.k || !a.v || !a.out || !a.tiles || (a.dtype == EQT_BF16 && a.stats && !a.rest)) return fail(EQT_ERR_BAD_ARGUMENT, "window_attention: NULL pointer");
   if (int rc = check_scratch(a, false)) return rc;
   const WindowParams p = params(a);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -117,13 +117,14 @@ extern "C" int eqt_window_attention_backward(const eqt_window_attention_args* ar
   if (int rc = check(args)) return rc;
   const eqt_window_attention_args& a = *args;
   if (a.n == 0 || a.num_tiles == 0) return EQT_OK;
-  if (!a.q || !a.k || !a.v || !a.grad || !a.out || !a.stats || !a.dq || !a.dk || !a.dv || !a.tiles) return fail(EQT_ERR_BAD_ARGUMENT, "window_attention backward: NULL pointer");
+  if (!a.q || !a.k || !a.v || !a.grad || !a.out || (a.dtype == EQT_BF16 && !a.rest) || !a.stats || !a.dq || !a.dk || !a.dv || !a.tiles) return fail(EQT_ERR_BAD_ARGUMENT, "window_attention backward: NULL pointer");
   if (int rc = check_scratch(a, true)) return rc;
   WindowParams p = params(a);
   if (p.split && !a.ptr) return fail(EQT_ERR_BAD_ARGUMENT, "window_attention backward: NULL pointer");
   unsigned char* base = static_cast<unsigned char*>(a.scratch) + spans_bytes(a);
   p.q.delta = p.kv.delta = reinterpret_cast<float*>(base);
-  p.far = reinterpret_cast<float*>(base + delta_bytes(a));
+  p.inverse = reinterpret_cast<float*>(base + delta_bytes(a));
+  p.far = reinterpret_cast<float*>(base + 2 * delta_bytes(a));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (on_tensor_cores(a)) {
     TcParams t;

@@ -12,7 +12,8 @@
 //
 // The forward pass keeps its unit of the exponentials until a row's greatest score is over 2^8 of it, and only then rescales the sums in tensor memory;
 // the sum and the result have the same unit, so that loses nothing.  The scores of the next 64 keys are made while the softmax works on these.
-// dS goes into dq's product in two parts, as within whole graphs: dq has the error of delta, which goes by the rounded result, already.
+// dS goes into dq's product in two parts, as within whole graphs: dq has the error of rounded weights already.  2-norm of the errors 2.3e-3 to 2.4e-3, a rounding of the result
+// alone 1.7e-3; with a delta of rounded results and weights not rounded, dq's was 3.4e-3 where windows are of few nodes, and dk's 2.7e-3.
 //
 // Two CTAs an SM hide each other's chain of copy, product, softmax and product.  By columns two or three groups of softmax warps take turns in one CTA, which
 // has all the tensor memory (64 values a head: 247 -> 217 us for 240 chains of 50 to 500 nodes against two CTAs of one group; by rows, where one thread has
@@ -168,10 +169,12 @@ __device__ __forceinline__ void tmem_put16(uint32_t at, const uint32_t* r) {
 __device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // A lane's row of results, with `more` where given, `f` times, to (n, components, heads, channels); whether all of it was finite.
-template <int DP> __device__ __forceinline__ bool put_row(uint32_t sum, float f, bool on, void* out, int row, int head, const AttentionParams& p, const float* more = nullptr) {
+template <int DP> __device__ __forceinline__ bool put_row(uint32_t sum, float f, bool on, void* out, int row, int head, const AttentionParams& p, const float* more = nullptr,
+                                                          void* rest = nullptr) {
   bool finite = true;
   const int values = p.comps * p.size, jump = (p.heads - 1) * p.size;     // to the head's next component, behind the last one's channels
-  T* to = static_cast<T*>(out) + ((int64_t)row * p.comps * p.heads + head) * p.size;
+  const int64_t place = ((int64_t)row * p.comps * p.heads + head) * p.size;
+  T *to = static_cast<T*>(out) + place, *to_rest = static_cast<T*>(rest) + place;
   int left = p.size;
 #pragma unroll
   for (int h = 0; h < DP; h += 32) {
@@ -191,9 +194,17 @@ template <int DP> __device__ __forceinline__ bool put_row(uint32_t sum, float f,
         finite = finite && is_finite(v[j]);
         v[j] *= f;
       }
-      if (on) *reinterpret_cast<uint4*>(to) = make_uint4(two_bf16(v[0], v[1]), two_bf16(v[2], v[3]), two_bf16(v[4], v[5]), two_bf16(v[6], v[7]));
-      to += 8;
-      if ((left -= 8) == 0) to += jump, left = p.size;
+      uint32_t u[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) u[j] = two_bf16(v[2 * j], v[2 * j + 1]);
+      if (on) *reinterpret_cast<uint4*>(to) = make_uint4(u[0], u[1], u[2], u[3]);
+      if (on && rest) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) u[j] = two_bf16(v[2 * j] - __uint_as_float(u[j] << 16), v[2 * j + 1] - __uint_as_float(u[j] & 0xffff0000u));
+        *reinterpret_cast<uint4*>(to_rest) = make_uint4(u[0], u[1], u[2], u[3]);
+      }
+      to += 8, to_rest += 8;
+      if ((left -= 8) == 0) to += jump, to_rest += jump, left = p.size;
     }
   }
   return finite;
@@ -320,7 +331,7 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
             const int64_t from = there ? (int64_t)h * w.q.n + query : 0;
             float* num = numbers + slot / 2 * 3 * KEYS + c;
             copy4(num, w.q.top + from, there);
-            copy4(num + KEYS, w.q.inverse + from, there);
+            copy4(num + KEYS, w.inverse + from, there);
             copy4(num + 2 * KEYS, w.q.delta + from, there);
           }
         }
@@ -534,8 +545,8 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
 #pragma unroll
         for (int c = 0; c < 64; c += 2) {
           const float x = exp2_fast(fmaf(__uint_as_float(raw[c >> 5][c & 31]), unit, minus)), y = exp2_fast(fmaf(__uint_as_float(raw[c >> 5][(c & 31) + 1]), unit, minus));
-          add[(c >> 1) & 3] += x + y;
-          out[c >> 1] = two_bf16(x, y);
+          out[c >> 1] = two_bf16(x, y);                  // and the sum is that of the rounded weights
+          add[(c >> 1) & 3] += __uint_as_float(out[c >> 1] << 16) + __uint_as_float(out[c >> 1] & 0xffff0000u);
         }
         total += (add[0] + add[1]) + (add[2] + add[3]);
         tmem_put16(s_at, out);
@@ -547,7 +558,7 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
       }
       if (sums_there()) {
         const float inverse = 1.f / total;
-        const bool finite = put_row<DP>(sum_at, inverse, on, w.q.out, row, mine, w.q);
+        const bool finite = put_row<DP>(sum_at, inverse, on, w.q.out, row, mine, w.q, nullptr, w.rest);
         sums_read(on && !finite);
         if (on && w.q.top) w.q.top[(int64_t)mine * w.q.n + row] = base, w.q.inverse[(int64_t)mine * w.q.n + row] = inverse;
       }
@@ -555,6 +566,7 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
       const int64_t at_row = (int64_t)mine * w.q.n + row;
       float top = INFINITY, inverse = 0.f, delta = 0.f;
       if (on) top = w.q.top[at_row], inverse = w.q.inverse[at_row], delta = w.q.delta[at_row];
+      float sums[2] = {0.f, 0.f}, exact[2] = {0.f, 0.f}; // of weights before rounding, and of these times dP: for the columns
       static_assert(MODE != ROWS || GROUPS == 1, "one group by rows");
       for (int k = 0; k < steps; ++k) {
         const unsigned j = j0 + k, b = j % BUFFERS;
@@ -576,11 +588,21 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
           const uint32_t word = (uint32_t)(bits >> (32 * h));
 #pragma unroll
           for (int c = 0; c < 32; c += 2) {
-            float x[2];
+            float x[2], e[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-              x[i] = exp2_fast(fmaf(__uint_as_float(s[h][c + i]), unit, -top)) * inverse * (__uint_as_float(d[c + i]) - delta);
-              if (!all) x[i] = (word >> (c + i)) & 1 ? x[i] : 0.f;
+              e[i] = exp2_fast(fmaf(__uint_as_float(s[h][c + i]), unit, -top));
+              if (!all) e[i] = (word >> (c + i)) & 1 ? e[i] : 0.f;
+            }
+            const uint32_t weights_ = two_bf16(e[0], e[1]);
+            const float rounded[2] = {__uint_as_float(weights_ << 16), __uint_as_float(weights_ & 0xffff0000u)};
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              float dp = __uint_as_float(d[c + i]);
+              if (!all) dp = (word >> (c + i)) & 1 ? dp : 0.f;            // zero times what is not seen
+              x[i] = rounded[i] * inverse * (dp - delta);
+              sums[i] += e[i];
+              exact[i] = fmaf(e[i], dp, exact[i]);
             }
             const uint32_t two = two_bf16(x[0], x[1]);
             large[c / 2] = two;
@@ -597,6 +619,11 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
       if (sums_there()) {
         const bool finite = put_row<DP>(sum_at, w.q.scale, on, w.q.dq, row, mine, w.q);
         sums_read(on && !finite);
+        if (on) {
+          const float sum = 1.f / (sums[0] + sums[1]);
+          w.q.delta[at_row] = (exact[0] + exact[1]) * sum;
+          w.inverse[at_row] = sum;
+        }
       }
     } else {
       const int skip = (int)((group + GROUPS - j0 % GROUPS) % GROUPS);      // the groups take turns over all tiles' steps
@@ -690,7 +717,7 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
   }
 }
 
-// delta = <g, out> of every node and head: `lanes` threads a head (a power of two), 16 bytes each, neighbouring heads side by side.  Apart from the rows' pass, whose
+// delta = <g, out + rest> of every node and head: `lanes` threads a head (a power of two), 16 bytes each, neighbouring heads side by side.  Apart from the rows' pass, whose
 // threads have a row each and would read both with a line for every 16 bytes.
 __global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ WindowParams p, int lanes) {
   const int values = p.q.comps * p.q.size, lane = threadIdx.x & (lanes - 1);
@@ -702,12 +729,13 @@ __global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ Wind
     float sum = 0.f;
     if (at < count && e < values) {
       const int64_t place = ((node * p.q.comps + comp) * p.q.heads + head) * p.q.size + e - comp * p.q.size;
-      const uint4 a = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.q.out) + place)), b = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.q.g.p) + place));
-      const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+      auto words = [&](const void* base) { return __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(base) + place)); };
+      const uint4 a = words(p.q.out), b = words(p.q.g.p), c = words(p.rest);
+      const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w}, z[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        sum = fmaf(__uint_as_float(x[i] << 16), __uint_as_float(y[i] << 16), sum);
-        sum = fmaf(__uint_as_float(x[i] & 0xffff0000u), __uint_as_float(y[i] & 0xffff0000u), sum);
+        sum = fmaf(__uint_as_float(x[i] << 16) + __uint_as_float(z[i] << 16), __uint_as_float(y[i] << 16), sum);
+        sum = fmaf(__uint_as_float(x[i] & 0xffff0000u) + __uint_as_float(z[i] & 0xffff0000u), __uint_as_float(y[i] & 0xffff0000u), sum);
       }
     }
     for (int o = lanes >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);

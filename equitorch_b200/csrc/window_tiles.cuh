@@ -65,6 +65,8 @@ template <typename F> __device__ __forceinline__ void each_bad_row(bool bad0, bo
     if ((((r < 8 ? b0 : b1) >> (4 * (r & 7))) & 15) && row + r < end) again(row + r);
 }
 
+template <typename T> __device__ __forceinline__ float rounded(float x) { return sizeof(T) == 4 ? x : __bfloat162float(__float2bfloat16_rn(x)); }
+
 template <typename T, int DP, int WR, int KT>
 __global__ void __launch_bounds__(THREADS, DP <= 64 ? 4 : 3) window_forward_kernel(const __grid_constant__ WindowParams p) {
   using S = attention::Shape<T, DP, WR, KT>;
@@ -135,7 +137,7 @@ __global__ void __launch_bounds__(THREADS, DP <= 64 ? 4 : 3) window_forward_kern
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            z[n][2 * r + i] = exp2_fast(z[n][2 * r + i] - base);
+            z[n][2 * r + i] = rounded<T>(exp2_fast(z[n][2 * r + i] - base));
             add += z[n][2 * r + i];
           }
         sum[r] = sum[r] * keep + add;
@@ -158,6 +160,16 @@ __global__ void __launch_bounds__(THREADS, DP <= 64 ? 4 : 3) window_forward_kern
   }
   const bool ok0 = finite_rows(o, 0), ok1 = finite_rows(o, 1);
   store_rows<T, DP>(const_cast<T*>(mine), p.q.out, o, f[0], f[1], row, hi, head, p.q, lane);
+  if (p.rest) {
+#pragma unroll
+    for (int n = 0; n < DP / 8; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float x = o[n][i] * f[i >> 1];
+        o[n][i] = x - rounded<T>(x);
+      }
+    store_rows<T, DP>(const_cast<T*>(mine), p.rest, o, 1.f, 1.f, row, hi, head, p.q, lane);
+  }
   each_bad_row(!ok0, !ok1, row, hi, [&](int i) { again_forward<T>(p, i, head, lo, hi, lane); });
 }
 
@@ -198,15 +210,24 @@ __global__ void __launch_bounds__(THREADS, DP <= 32 ? 4 : DP <= 96 ? 3 : 2) wind
   const T *mq = rows + (warp % WR) * 16 * LD, *mg = grads + (warp % WR) * 16 * LD;
   const float unit = p.q.scale * LOG2E;
   float delta[2] = {0.f, 0.f}, top[2] = {INFINITY, INFINITY}, inverse[2] = {0.f, 0.f};
-  if (work) row_delta<T, DP>(mg, row, hi, head, p.q, lane, delta);
+  if (work) {
+    row_delta<T, DP>(mg, row, hi, head, p.q, lane, delta);
+    if (p.rest) {
+      AttentionParams rest = p.q;
+      rest.out = p.rest;
+      float more[2];
+      row_delta<T, DP>(mg, row, hi, head, rest, lane, more);
+      delta[0] += more[0], delta[1] += more[1];
+    }
+  }
   const int64_t at = (int64_t)head * p.q.n + row + g;
 #pragma unroll
   for (int r = 0; r < 2; ++r)
     if (work && row + g + 8 * r < hi) {
       top[r] = p.q.top[at + 8 * r];
       inverse[r] = p.q.inverse[at + 8 * r];
-      if (t == 0) p.q.delta[at + 8 * r] = delta[r];
     }
+  float sums[2] = {0.f, 0.f}, exact[2] = {0.f, 0.f};     // of weights before rounding, and of these times dP: for the columns
   float dq[DP / 8][4];
 #pragma unroll
   for (int n = 0; n < DP / 8; ++n) dq[n][0] = dq[n][1] = dq[n][2] = dq[n][3] = 0.f;
@@ -231,13 +252,22 @@ __global__ void __launch_bounds__(THREADS, DP <= 32 ? 4 : DP <= 96 ? 3 : 2) wind
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int r = i >> 1, j = key + n * 8 + 2 * t + (i & 1);
-          z[n][i] = all || (j < end && sees(p, row + g + 8 * r, j, lo)) ? exp2_fast(z[n][i] * unit - top[r]) * inverse[r] * (dp[n][i] - delta[r]) : 0.f;
+          const bool on = all || (j < end && sees(p, row + g + 8 * r, j, lo));
+          const float weight = exp2_fast(z[n][i] * unit - top[r]);
+          z[n][i] = on ? rounded<T>(weight) * inverse[r] * (dp[n][i] - delta[r]) : 0.f;
+          sums[r] += on ? weight : 0.f;
+          exact[r] += on ? weight * dp[n][i] : 0.f;
         }
       out_mma<DP, NT, true>(dq, z, ks, lane);
     }
     __syncthreads();
   }
   if (!work) return;
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const float all = quad_sum(exact[r]), sum = 1.f / quad_sum(sums[r]);
+    if (t == 0 && row + g + 8 * r < hi) p.q.delta[at + 8 * r] = all * sum, p.inverse[at + 8 * r] = sum;
+  }
   const bool ok0 = finite_rows(dq, 0), ok1 = finite_rows(dq, 1);
   store_rows<T, DP>(const_cast<T*>(mq), p.q.dq, dq, p.q.scale, p.q.scale, row, hi, head, p.q, lane);
   each_bad_row(!ok0, !ok1, row, hi, [&](int i) { again_rows<T>(p, i, head, lo, hi, lane); });
@@ -270,7 +300,7 @@ __global__ void __launch_bounds__(THREADS, DP <= 64 ? 3 : 2) window_columns_kern
     load_tile<T, DP, S::TH, KT>(stage + s * S::STAGE + KT * LD, p.q.g, i, here ? end - i : 0, head, p.q, ht);
     for (int c = ht; c < 3 * KT; c += S::TH) {
       const int r = c % KT;
-      const float* from = c < KT ? p.q.top : c < 2 * KT ? p.q.inverse : p.q.delta;
+      const float* from = c < KT ? p.q.top : c < 2 * KT ? p.inverse : p.q.delta;
       const bool there = here && i + r < end;
       copy4(numbers + s * 3 * KT + c, from + (there ? (int64_t)head * p.q.n + i + r : 0), there);
     }
@@ -371,7 +401,7 @@ template <typename T, int DP, int KT> __global__ void __launch_bounds__(THREADS)
     load_tile<T, DP, 32, KT>(stage + s * S::STAGE + KT * LD, p.q.g, i, to - i, head, p.q, lane);
     for (int c = lane; c < 3 * KT; c += 32) {
       const int r = c % KT;
-      const float* x = c < KT ? p.q.top : c < 2 * KT ? p.q.inverse : p.q.delta;
+      const float* x = c < KT ? p.q.top : c < 2 * KT ? p.inverse : p.q.delta;
       const bool there = i + r < to;
       copy4(numbers + s * 3 * KT + c, x + (there ? (int64_t)head * p.q.n + i + r : 0), there);
     }

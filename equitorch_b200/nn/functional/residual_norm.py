@@ -15,19 +15,20 @@ class _AddRMSNorm(Function):
     @staticmethod
     def forward(ctx, x, residual, weight, eps):
         out, total, rstd = _ops.norm_forward(x, residual, weight, eps, any(ctx.needs_input_grad))
-        ctx.save_for_backward(x if residual is None else total, weight, rstd)
+        apart = residual is not None and x.dtype == torch.bfloat16
+        ctx.save_for_backward(x if residual is None or apart else total, residual if apart else None, weight, rstd)
         ctx.set_materialize_grads(False)
         return out, total
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad, grad_total):
-        total, weight, rstd = ctx.saved_tensors
+        total, residual, weight, rstd = ctx.saved_tensors
         need_x, need_residual, need_weight, _ = ctx.needs_input_grad
         if grad is None:                                 # only the sum was used
             dx, dweight = grad_total, torch.zeros_like(weight) if need_weight else None
         else:
-            dx, dweight = _ops.norm_backward(grad, grad_total, total, weight, rstd, need_weight)
+            dx, dweight = _ops.norm_backward(grad, grad_total, total, residual, weight, rstd, need_weight)
         return dx if need_x else None, dx if need_residual else None, dweight, None
 
 
@@ -39,8 +40,8 @@ def add_rms_norm(x: Tensor, residual: Optional[Tensor] = None, weight: Optional[
 
     ``x`` and ``residual`` (or ``None``: the sum is ``x`` itself) are ``(N, channels)`` or ``(N, components, channels)``; the mean is over all
     of a node's components and channels and ``weight`` (channels,) has no components, so equivariant features stay so.  float32 or bfloat16, all of one
-    type; sums in float32.  ``out`` is computed from the sum before its rounding, the backward pass from the sum as it was returned
-    (of bfloat16: within 2^-9 of each value), which is all that is kept beside one number a node.
+    type; sums in float32.  ``out`` is computed from the sum before its rounding.  Kept for the backward pass are one number a node and the sum, or, of
+    bfloat16, ``x`` and ``residual``, since the sum's rounding would go into the gradients beside their own.
 
     Differentiable once, in ``x``, ``residual`` and ``weight``; the weight's gradient uses no atomics and is the same bits at every call."""
     _ops.check(x, residual, weight, eps)

@@ -15,16 +15,16 @@ from ...ops import window_op as _ops
 class _WindowAttention(Function):
     @staticmethod
     def forward(ctx, q, k, v, graphs, heads, kv_heads, window, scale):
-        out, stats = _ops.window_forward(q, k, v, graphs, heads, kv_heads, window, scale, any(ctx.needs_input_grad))
-        ctx.save_for_backward(q, k, v, out, stats)
+        out, rest, stats = _ops.window_forward(q, k, v, graphs, heads, kv_heads, window, scale, any(ctx.needs_input_grad))
+        ctx.save_for_backward(q, k, v, out, rest, stats)
         ctx.args = graphs, heads, kv_heads, window, scale
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        q, k, v, out, stats = ctx.saved_tensors
-        grads = _ops.window_backward(grad, q, k, v, *ctx.args, out, stats)
+        q, k, v, out, rest, stats = ctx.saved_tensors
+        grads = _ops.window_backward(grad, q, k, v, *ctx.args, out, rest, stats)
         return (*(g if need else None for g, need in zip(grads, ctx.needs_input_grad)), *[None] * 5)
 
 
@@ -45,7 +45,8 @@ def window_attention(q: Tensor, k: Tensor, v: Tensor, graphs: PackedGraphs, num_
     touch each other.
 
     Differentiable once in ``q``, ``k`` and ``v``.  Sums in float32, one order of sums, no atomics; of bfloat16 features, weights and score
-    gradients are rounded to bfloat16 for the products."""
+    gradients are rounded to bfloat16 for the products.  Beside its inputs and result the backward pass keeps two numbers a node and head and, of
+    bfloat16, what the result's rounding left: where a node's weight is almost one, its gradient is what two such numbers leave."""
     kv_heads = num_heads if kv_heads is None else kv_heads
     _ops.check(q, k, v, graphs, num_heads, kv_heads, (before, after, sinks), scale)
     if scale is None:

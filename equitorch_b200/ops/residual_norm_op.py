@@ -66,11 +66,11 @@ def norm_e4m3(x: Tensor, residual: Optional[Tensor], weight: Optional[Tensor], e
     return values, scales, total
 
 
-def norm_backward(grad: Tensor, grad_total: Optional[Tensor], total: Tensor, weight: Optional[Tensor], rstd: Tensor, want_weight: bool
-                  ) -> Tuple[Tensor, Optional[Tensor]]:
-    """The gradient of the features, which is the residual's too, and that of the weight."""
+def norm_backward(grad: Tensor, grad_total: Optional[Tensor], total: Tensor, residual: Optional[Tensor], weight: Optional[Tensor], rstd: Tensor,
+                  want_weight: bool) -> Tuple[Tensor, Optional[Tensor]]:
+    """The gradient of the features, which is the residual's too, and that of the weight; the sum is ``total``, or that of both."""
     dev = total.device
-    grad, grad_total, total, weight = _whole(grad), _whole(grad_total), _whole(total), _whole(weight)
+    grad, grad_total, total, residual, weight = _whole(grad), _whole(grad_total), _whole(total), _whole(residual), _whole(weight)
     n, comps, channels = _sizes(total)
     dx = torch.empty_like(total)
     dweight = torch.empty_like(weight) if want_weight else None
@@ -78,7 +78,7 @@ def norm_backward(grad: Tensor, grad_total: Optional[Tensor], total: Tensor, wei
     with _lib.on_device(dev):
         size = lib.eqt_add_rms_norm_scratch(code, n, comps, channels) if want_weight else 0
         scratch = torch.empty(size, dtype=torch.float32, device=dev) if size else None
-        _lib.check(lib.eqt_add_rms_norm_backward(code, grad.data_ptr(), _lib.ptr(grad_total), total.data_ptr(), _lib.ptr(weight), rstd.data_ptr(),
-                                                 dx.data_ptr(), _lib.ptr(dweight), _lib.ptr(scratch), size, n, comps, channels, _lib.stream_ptr(dev)),
+        _lib.check(lib.eqt_add_rms_norm_backward(code, grad.data_ptr(), _lib.ptr(grad_total), total.data_ptr(), _lib.ptr(residual), _lib.ptr(weight),
+                                                 rstd.data_ptr(), dx.data_ptr(), _lib.ptr(dweight), _lib.ptr(scratch), size, n, comps, channels, _lib.stream_ptr(dev)),
                    "eqt_add_rms_norm_backward")
     return dx, dweight

@@ -58,14 +58,14 @@ def _rows(x: Tensor) -> Tensor:
     return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
 
 
-def _args(q, k, v, graphs, heads, kv_heads, window, scale, out, stats) -> _lib.WindowAttentionArgs:
+def _args(q, k, v, graphs, heads, kv_heads, window, scale, out, rest, stats) -> _lib.WindowAttentionArgs:
     n, comps, channels = q.shape
     return _lib.WindowAttentionArgs(
         dtype=_lib.DTYPE_CODE[q.dtype], comps=comps, heads=heads, kv_heads=kv_heads, head_channels=channels // heads, tile_rows=graphs.tile_rows,
         scale=scale, n=n, num_graphs=graphs.num_graphs, longest=graphs.longest, num_tiles=graphs.tiles.shape[0], before=window[0], after=window[1],
         sinks=window[2], q_node=q.stride(0), q_comp=q.stride(1), k_node=k.stride(0), k_comp=k.stride(1), v_node=v.stride(0), v_comp=v.stride(1),
         ptr=graphs.ptr.data_ptr(), tiles=graphs.tiles.data_ptr(), q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), out=out.data_ptr(),
-        stats=_lib.ptr(stats), status=status_flag(q.device).data_ptr())
+        rest=_lib.ptr(rest), stats=_lib.ptr(stats), status=status_flag(q.device).data_ptr())
 
 
 def _new(like: Tensor, graphs: PackedGraphs) -> Tensor:
@@ -81,24 +81,26 @@ def _scratch(args: _lib.WindowAttentionArgs, backward: bool, dev: torch.device) 
 
 
 def window_forward(q: Tensor, k: Tensor, v: Tensor, graphs: PackedGraphs, heads: int, kv_heads: int, window: Tuple[int, int, int], scale: float,
-                   want_stats: bool) -> Tuple[Tensor, Optional[Tensor]]:
+                   want_stats: bool) -> Tuple[Tensor, Optional[Tensor], Optional[Tensor]]:
+    """The result and, for the backward pass, what its rounding left (of bfloat16) and the rows' statistics."""
     dev = q.device
     q, k, v = _rows(q), _rows(k), _rows(v)
     out = _new(q, graphs)
+    rest = _new(q, graphs) if want_stats and q.dtype == torch.bfloat16 else None
     stats = torch.empty(2, heads, q.shape[0], dtype=torch.float32, device=dev) if want_stats else None
-    args = _args(q, k, v, graphs, heads, kv_heads, window, scale, out, stats)
+    args = _args(q, k, v, graphs, heads, kv_heads, window, scale, out, rest, stats)
     with _lib.on_device(dev):
         scratch = _scratch(args, False, dev)  # noqa: F841 - kept alive for the call
         _lib.check(_lib.lib().eqt_window_attention_forward(C.byref(args), _lib.stream_ptr(dev)), "eqt_window_attention_forward")
-    return out, stats
+    return out, rest, stats
 
 
 def window_backward(grad: Tensor, q: Tensor, k: Tensor, v: Tensor, graphs: PackedGraphs, heads: int, kv_heads: int, window: Tuple[int, int, int],
-                    scale: float, out: Tensor, stats: Tensor) -> Tuple[Tensor, Tensor, Tensor]:
+                    scale: float, out: Tensor, rest: Optional[Tensor], stats: Tensor) -> Tuple[Tensor, Tensor, Tensor]:
     dev = q.device
     q, k, v, grad = _rows(q), _rows(k), _rows(v), grad.contiguous()
     dq, dk, dv = _new(q, graphs), _new(k, graphs), _new(k, graphs)
-    args = _args(q, k, v, graphs, heads, kv_heads, window, scale, out, stats)
+    args = _args(q, k, v, graphs, heads, kv_heads, window, scale, out, rest, stats)
     args.grad, args.dq, args.dk, args.dv = grad.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
     with _lib.on_device(dev):
         scratch = _scratch(args, True, dev)  # noqa: F841 - kept alive for the call

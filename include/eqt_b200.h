@@ -718,15 +718,16 @@ int eqt_gated_backward(int32_t dtype, const void* x, const void* w, const void* 
  * inverse roots, for the backward pass) may be NULL.  All (n, comps, channels), contiguous, float32 or bfloat16; weight (channels).
  * The e4m3 form has 8-bit values and a float scale for every `group` values (a divisor of comps * channels); value = the nearest to 448 t / max |t| of
  * t = h weight, ties to even, not a rounded quotient's.
- * Backward: dx (also the residual's gradient) from grad and grad_total (dL/dh; may be NULL), and dweight (may be NULL); no atomics.
+ * Backward: dx (also the residual's gradient) from grad and grad_total (dL/dh; may be NULL), and dweight (may be NULL); no atomics.  h is total, or, with
+ * a residual, the sum of both (x and the residual: without total's rounding).
  * scratch: eqt_add_rms_norm_scratch floats, needed for dweight. */
 int eqt_add_rms_norm_forward(int32_t dtype, const void* x, const void* residual, const void* weight, void* out, void* total, float* rstd, int64_t n,
                              int64_t comps, int64_t channels, double eps, void* stream);
 int eqt_add_rms_norm_e4m3(int32_t dtype, const void* x, const void* residual, const void* weight, void* values, float* scales, void* total, int64_t n,
                           int64_t comps, int64_t channels, int64_t group, double eps, void* stream);
 int64_t eqt_add_rms_norm_scratch(int32_t dtype, int64_t n, int64_t comps, int64_t channels);
-int eqt_add_rms_norm_backward(int32_t dtype, const void* grad, const void* grad_total, const void* total, const void* weight, const float* rstd, void* dx,
-                              void* dweight, float* scratch, int64_t scratch_floats, int64_t n, int64_t comps, int64_t channels, void* stream);
+int eqt_add_rms_norm_backward(int32_t dtype, const void* grad, const void* grad_total, const void* total, const void* residual, const void* weight,
+                              const float* rstd, void* dx, void* dweight, float* scratch, int64_t scratch_floats, int64_t n, int64_t comps, int64_t channels, void* stream);
 
 /* Rotary positions of q and, where given, k: (n, comps, heads * size), channels next to each other, any strides (in values) of nodes and
  * components; results contiguous.  The first 2 * half channels of a head turn by positions[node] * frequencies[pair] (backward: by minus that)
@@ -763,6 +764,7 @@ int eqt_window_step(const eqt_window_step_args* args, void* stream);
  * comps, kv_heads * head_channels); inputs with channels next to each other and any strides (in values), the others contiguous; float32 or
  * bfloat16; at most 128 values (comps * head_channels) a head.  Head h has the keys of head h / (heads / kv_heads).
  *   s_ij = scale <q_i, k_j>,   out_i = sum_j softmax_j(s_ij) v_j;   rows of nodes that belong to no chain are zero, their gradients too
+ * rest (as out; may be NULL with stats NULL, and for float32): what the rounding of out left, for the backward pass, whose sum_j P_ij dP_ij is <grad_i, out_i + rest_i>.
  * stats (2, heads, n): a row's greatest score in units of log2 and one over its sum of weights from there, needed for the backward pass.  tiles: as for eqt_attention_forward.  scratch:
  * eqt_window_attention_scratch bytes, 16-byte aligned; status as for eqt_gated_forward.  Backward: grad contiguous; all three gradients are written; no atomics. */
 typedef struct {
@@ -772,7 +774,7 @@ typedef struct {
   const int64_t* ptr;
   const int32_t* tiles;
   const void *q, *k, *v, *grad;
-  void *out, *dq, *dk, *dv;
+  void *out, *rest, *dq, *dk, *dv;
   float* stats;
   void* scratch;
   int32_t* status;

@@ -42,7 +42,7 @@ def test_against_float64(shape, residual, weight, dtype):
     wide = d(w) if weight else torch.ones(shape[-1], dtype=torch.float64, device=DEV)
     r = (h.square().mean((1, 2), keepdim=True) + 1e-3).rsqrt()
     u, gw, count = h * r, d(g) * wide, shape[1] * shape[2]
-    un, sums = U[dtype], U[dtype] if residual else 0.0       # the backward pass has the sum as it was rounded
+    un, sums = U[dtype], 0.0                                # the backward pass has the sum as it was before its rounding
     within(out, u * wide, (u * wide).abs() * (un + C), "out")
     within(total, h, h.abs() * un + d(x).abs() * 2.0 ** -23, "sum")
     mean, size = (gw * u).sum((1, 2), keepdim=True) / count, (gw * u).abs().sum((1, 2), keepdim=True) / count

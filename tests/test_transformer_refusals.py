@@ -128,7 +128,7 @@ def test_library_checks_its_arguments():
     assert lib.eqt_add_rms_norm_forward(0, 16, 16, 16, 16, 16, 16, -1, 1, 8, 1e-6, None) == 1
     assert lib.eqt_add_rms_norm_forward(0, 16, 16, 16, 16, 16, 16, 1, 2 ** 20, 2 ** 20, 1e-6, None) == 2
     assert lib.eqt_add_rms_norm_e4m3(0, 16, 16, 16, 16, 16, 16, 1, 1, 8, 3, 1e-6, None) == 1
-    assert lib.eqt_add_rms_norm_backward(0, 16, 16, 16, 16, 16, 16, 16, None, 0, 1, 1, 8, None) == 1
+    assert lib.eqt_add_rms_norm_backward(0, 16, 16, 16, 16, 16, 16, 16, 16, None, 0, 1, 1, 8, None) == 1
     assert lib.eqt_rotary(None, None) == 1 and lib.eqt_window_step(None, None) == 1
     rotary = dict(dtype=0, comps=1, heads=1, kv_heads=1, size=8, half=4, n=1, q=16, q_out=16, positions=16, frequencies=16)
     for bad, code in ((dict(dtype=9), 1), (dict(half=5), 1), (dict(size=0), 1), (dict(n=-1), 1), (dict(positions=None), 1), (dict(k=16), 1), (dict(half=600, size=1200), 2)):
@@ -136,7 +136,7 @@ def test_library_checks_its_arguments():
     step = dict(dtype=0, comps=1, heads=2, kv_heads=1, head_channels=8, scale=1.0, chains=1, capacity=4, before=1, sinks=0, q=16, k=16, v=16, out=16, lengths=16)
     for bad, code in ((dict(heads=3, kv_heads=2), 1), (dict(before=-1), 1), (dict(lengths=None), 1), (dict(head_channels=129), 2), (dict(chains=70_000), 2)):
         assert lib.eqt_window_step(C.byref(_lib.WindowStepArgs(**{**step, **bad})), None) == code
-    window = dict(dtype=0, comps=1, heads=2, kv_heads=1, head_channels=8, tile_rows=16, scale=1.0, n=4, num_graphs=1, longest=4, num_tiles=1, q=16, k=16, v=16, out=16, tiles=16, ptr=16)
+    window = dict(dtype=0, comps=1, heads=2, kv_heads=1, head_channels=8, tile_rows=16, scale=1.0, n=4, num_graphs=1, longest=4, num_tiles=1, q=16, k=16, v=16, out=16, rest=16, tiles=16, ptr=16)
     for bad, code in ((dict(dtype=1), 1), (dict(tile_rows=8), 1), (dict(sinks=-1), 1), (dict(q=None), 1), (dict(n=2 ** 30), 2), (dict(head_channels=130), 2)):
         assert lib.eqt_window_attention_forward(C.byref(_lib.WindowAttentionArgs(**{**window, **bad})), None) == code
         assert bad.get("q", 1) is None or lib.eqt_window_attention_form(C.byref(_lib.WindowAttentionArgs(**{**window, **bad}))) == -1
