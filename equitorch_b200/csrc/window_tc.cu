@@ -168,6 +168,31 @@ __device__ __forceinline__ void tmem_put16(uint32_t at, const uint32_t* r) {
 }
 __device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// Two float32 values in a pair of registers: packed instructions take half the issue slots, which bound the softmax beside the exponentials.
+struct Two {
+  uint64_t v;
+  __device__ __forceinline__ Two() = default;
+  __device__ __forceinline__ Two(float x, float y) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y)); }
+  __device__ __forceinline__ void apart(float& x, float& y) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+};
+__device__ __forceinline__ Two two_of(const uint32_t* r) { return Two(__uint_as_float(r[0]), __uint_as_float(r[1])); }
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+  Two d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return d;
+}
+__device__ __forceinline__ Two mul2(Two a, Two b) {
+  Two d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+  return d;
+}
+__device__ __forceinline__ Two add2(Two a, Two b) {
+  Two d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+  return d;
+}
+__device__ __forceinline__ Two bf16_values(uint32_t u) { return Two(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u)); }
+
 // A lane's row of results, with `more` where given, `f` times, to (n, components, heads, channels); whether all of it was finite.
 template <int DP> __device__ __forceinline__ bool put_row(uint32_t sum, float f, bool on, void* out, int row, int head, const AttentionParams& p, const float* more = nullptr,
                                                           void* rest = nullptr) {
@@ -540,15 +565,19 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
           }
         }
         const float minus = base == -INFINITY ? 0.f : -base;
-        float add[4] = {0.f, 0.f, 0.f, 0.f};
+        const Two units(unit, unit), minuses(minus, minus);
+        Two add[2] = {Two(0.f, 0.f), Two(0.f, 0.f)};
         uint32_t out[32];
 #pragma unroll
         for (int c = 0; c < 64; c += 2) {
-          const float x = exp2_fast(fmaf(__uint_as_float(raw[c >> 5][c & 31]), unit, minus)), y = exp2_fast(fmaf(__uint_as_float(raw[c >> 5][(c & 31) + 1]), unit, minus));
-          out[c >> 1] = two_bf16(x, y);                  // and the sum is that of the rounded weights
-          add[(c >> 1) & 3] += __uint_as_float(out[c >> 1] << 16) + __uint_as_float(out[c >> 1] & 0xffff0000u);
+          float x, y;
+          fma2(two_of(&raw[c >> 5][c & 31]), units, minuses).apart(x, y);
+          out[c >> 1] = two_bf16(exp2_fast(x), exp2_fast(y));
+          add[(c >> 1) & 1] = add2(add[(c >> 1) & 1], bf16_values(out[c >> 1]));       // the sum is that of the rounded weights
         }
-        total += (add[0] + add[1]) + (add[2] + add[3]);
+        float even, odd;
+        add2(add[0], add[1]).apart(even, odd);
+        total += even + odd;
         tmem_put16(s_at, out);
         tmem_put16(s_at + 16, out + 16);
         tmem_stored();
@@ -566,7 +595,8 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
       const int64_t at_row = (int64_t)mine * w.q.n + row;
       float top = INFINITY, inverse = 0.f, delta = 0.f;
       if (on) top = w.q.top[at_row], inverse = w.q.inverse[at_row], delta = w.q.delta[at_row];
-      float sums[2] = {0.f, 0.f}, exact[2] = {0.f, 0.f}; // of weights before rounding, and of these times dP: for the columns
+      Two sums(0.f, 0.f), exact(0.f, 0.f);               // of weights before rounding, and of these times dP: for the columns
+      const Two units(unit, unit), minuses(-top, -top), inverses(inverse, inverse), deltas(-delta * inverse, -delta * inverse), less(-1.f, -1.f);
       static_assert(MODE != ROWS || GROUPS == 1, "one group by rows");
       for (int k = 0; k < steps; ++k) {
         const unsigned j = j0 + k, b = j % BUFFERS;
@@ -588,25 +618,23 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
           const uint32_t word = (uint32_t)(bits >> (32 * h));
 #pragma unroll
           for (int c = 0; c < 32; c += 2) {
-            float x[2], e[2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              e[i] = exp2_fast(fmaf(__uint_as_float(s[h][c + i]), unit, -top));
-              if (!all) e[i] = (word >> (c + i)) & 1 ? e[i] : 0.f;
+            float e[2], x[2];
+            fma2(two_of(&s[h][c]), units, minuses).apart(e[0], e[1]);
+            Two dp = two_of(&d[c]);
+            e[0] = exp2_fast(e[0]), e[1] = exp2_fast(e[1]);
+            if (!all) {                                  // zero times zero for what is not seen
+              const bool see[2] = {(bool)((word >> c) & 1), (bool)((word >> (c + 1)) & 1)};
+              e[0] = see[0] ? e[0] : 0.f, e[1] = see[1] ? e[1] : 0.f;
+              dp = Two(see[0] ? __uint_as_float(d[c]) : 0.f, see[1] ? __uint_as_float(d[c + 1]) : 0.f);
             }
-            const uint32_t weights_ = two_bf16(e[0], e[1]);
-            const float rounded[2] = {__uint_as_float(weights_ << 16), __uint_as_float(weights_ & 0xffff0000u)};
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              float dp = __uint_as_float(d[c + i]);
-              if (!all) dp = (word >> (c + i)) & 1 ? dp : 0.f;            // zero times what is not seen
-              x[i] = rounded[i] * inverse * (dp - delta);
-              sums[i] += e[i];
-              exact[i] = fmaf(e[i], dp, exact[i]);
-            }
-            const uint32_t two = two_bf16(x[0], x[1]);
-            large[c / 2] = two;
-            small[c / 2] = two_bf16(x[0] - __uint_as_float(two << 16), x[1] - __uint_as_float(two & 0xffff0000u));
+            const Two before(e[0], e[1]);
+            sums = add2(sums, before);
+            exact = fma2(before, dp, exact);
+            const Two ds = mul2(bf16_values(two_bf16(e[0], e[1])), fma2(dp, inverses, deltas));
+            ds.apart(x[0], x[1]);
+            large[c / 2] = two_bf16(x[0], x[1]);
+            fma2(bf16_values(large[c / 2]), less, ds).apart(x[0], x[1]);
+            small[c / 2] = two_bf16(x[0], x[1]);
           }
           tmem_put16(s_at + 16 * h, large);
           tmem_put16(s_at + 32 + 16 * h, small);
@@ -620,14 +648,17 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
         const bool finite = put_row<DP>(sum_at, w.q.scale, on, w.q.dq, row, mine, w.q);
         sums_read(on && !finite);
         if (on) {
-          const float sum = 1.f / (sums[0] + sums[1]);
-          w.q.delta[at_row] = (exact[0] + exact[1]) * sum;
+          float s[2], x[2];
+          sums.apart(s[0], s[1]), exact.apart(x[0], x[1]);
+          const float sum = 1.f / (s[0] + s[1]);
+          w.q.delta[at_row] = (x[0] + x[1]) * sum;
           w.inverse[at_row] = sum;
         }
       }
     } else {
       const int skip = (int)((group + GROUPS - j0 % GROUPS) % GROUPS);      // the groups take turns over all tiles' steps
       int at = skip % walk.steps * KEYS;
+      const Two minus_units(-unit, -unit), less(-1.f, -1.f);
       for (int k = skip; k < steps; k += GROUPS) {
         const unsigned j = j0 + k, b = j % BUFFERS, slot = 2 * j % SLOTS;
         ok = bar_wait(&full[slot], (2 * j / SLOTS) & 1, ab) && bar_wait(&scores[b], (j / BUFFERS) & 1, ab);
@@ -650,13 +681,19 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
           for (int c = 0; c < 32; c += 4) {
             const float4 top = *reinterpret_cast<const float4*>(num + 32 * h + c), inverse = *reinterpret_cast<const float4*>(num + KEYS + 32 * h + c),
                          delta = *reinterpret_cast<const float4*>(num + 2 * KEYS + 32 * h + c);
-            const float tops[4] = {top.x, top.y, top.z, top.w}, inverses[4] = {inverse.x, inverse.y, inverse.z, inverse.w}, deltas[4] = {delta.x, delta.y, delta.z, delta.w};
+            const Two tops[2] = {Two(top.x, top.y), Two(top.z, top.w)}, inverses[2] = {Two(inverse.x, inverse.y), Two(inverse.z, inverse.w)},
+                      deltas[2] = {Two(delta.x, delta.y), Two(delta.z, delta.w)};
             float x[4], y[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              x[i] = exp2_fast(fmaf(__uint_as_float(s[c + i]), unit, -tops[i])) * inverses[i];
-              y[i] = x[i] * (__uint_as_float(d[c + i]) - deltas[i]);
-              if (!all) {
+            for (int i = 0; i < 4; i += 2) {
+              fma2(two_of(&s[c + i]), minus_units, tops[i / 2]).apart(x[i], x[i + 1]);
+              const Two weight = mul2(Two(exp2_fast(-x[i]), exp2_fast(-x[i + 1])), inverses[i / 2]);
+              weight.apart(x[i], x[i + 1]);
+              mul2(weight, fma2(deltas[i / 2], less, two_of(&d[c + i]))).apart(y[i], y[i + 1]);
+            }
+            if (!all) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
                 const bool see = (word >> (c + i)) & 1;
                 x[i] = see ? x[i] : 0.f;
                 y[i] = see ? y[i] : 0.f;
