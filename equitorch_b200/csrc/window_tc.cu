@@ -34,30 +34,35 @@ using attention::copy4;
 using T = __nv_bfloat16;
 
 enum Mode { FORWARD, ROWS, COLUMNS };
-constexpr int KEYS = 64, LOADERS = 64;                   // of the other side at a time; threads that copy
+constexpr int LOADERS = 64;                              // threads that copy
 constexpr int MOST_TILES = 16;                           // of a CTA
 constexpr float FAR = 8.f;                               // of log2, that a score may be above the unit
 
-// What a tile walks over: `ns` first nodes of the chain that its first row is in, from `from0` on, then [from1, to1), as one sequence.
+// What a tile walks over: `ns` first nodes of the chain that its first row is in, from `from0` on, to `wide` places (whole eights, what the 128-byte swizzle repeats
+// by), then [from1, to1), as one sequence.
 struct Stretch {
-  int from0, ns, from1, to1, total, steps;
+  int from0, ns, wide, from1, to1, total, steps;
 };
 constexpr int STRETCHES = 8;
 
 template <int DP, int MODE> struct Form {
   static constexpr int GROUPS = MODE == COLUMNS ? (DP == 128 ? 2 : 3) : 1;             // of softmax warps, each with a buffer of scores
-  static constexpr int BUFFERS = MODE == FORWARD ? 2 : GROUPS;
-  static constexpr int SOFT = 4 * GROUPS, THREADS = 32 * (SOFT + 2) + LOADERS, CTAS = GROUPS > 1 ? 1 : 2;
+  static constexpr int KEYS = MODE == FORWARD && DP == 128 ? 128 : 64;                 // of the other side at a time
+  static constexpr int BUFFERS = MODE == FORWARD ? 128 / KEYS : GROUPS;
+  static constexpr int HALVES = MODE == COLUMNS ? 1 : 2;                               // warps that share a row's others
+  static constexpr int SOFT = 4 * HALVES * GROUPS, THREADS = 32 * (SOFT + 2) + LOADERS, CTAS = GROUPS > 1 ? 1 : 2;
   static constexpr int OWN = MODE == FORWARD ? 1 : 2;                                // operands of the tile's rows
   static constexpr int OWN_BYTES = TILE_M * DP * 2, SLOT_BYTES = KEYS * DP * 2;
-  static constexpr int SLOTS = MODE == FORWARD && DP == 128 ? 4 : MODE == ROWS && DP == 128 ? 3 : 8;
+  static constexpr int SLOTS = MODE == FORWARD && DP == 128 ? 2 : MODE == ROWS && DP == 128 ? 3 : 8;
   static constexpr int NUMBERS = MODE == COLUMNS ? SLOTS / 2 * 3 * KEYS * 4 : 0;     // bytes: a query's greatest score, inverse sum, delta
   static constexpr int BUFFER = MODE == FORWARD ? KEYS : 2 * KEYS;                   // columns of tensor memory: S, or S and dP
   static constexpr int SUM_AT = BUFFERS * BUFFER, COLS = CTAS == 1 ? 512 : 256;
   static constexpr int BARRIERS = 384;                                               // bytes, with the tensor memory's address and the abort flag
-  static constexpr size_t bytes() { return (size_t)OWN * OWN_BYTES + (size_t)SLOTS * SLOT_BYTES + NUMBERS + BARRIERS + STRETCHES * sizeof(Stretch) + SOFT * MOST_TILES * 4; }
-  static_assert((2 * SLOTS + 3 * BUFFERS + 5 + STRETCHES) * 8 + 8 <= BARRIERS, "barriers");
-  static_assert(LOADERS == KEYS, "a number of a query each");
+  static constexpr int ROW_NUMBERS = MODE == FORWARD ? 6 * TILE_M * 4 : 0;           // bytes: halves' maxima, and sums of two tiles
+  static constexpr size_t bytes() {
+    return (size_t)OWN * OWN_BYTES + (size_t)SLOTS * SLOT_BYTES + NUMBERS + BARRIERS + STRETCHES * sizeof(Stretch) + 4 * GROUPS * MOST_TILES * 4 + ROW_NUMBERS;
+  }
+  static_assert((2 * SLOTS + 3 * BUFFERS + 4 + STRETCHES) * 8 + 8 <= BARRIERS, "barriers");
   static_assert(SUM_AT + (MODE == COLUMNS ? 2 : 1) * DP <= COLS, "tensor memory");
 };
 
@@ -65,7 +70,7 @@ template <int DP, int MODE> struct Form {
 // from moves on by additions; and goes to, but for the 128-byte swizzle (a line of 128 bytes a row).  Zeros behind the head's values, up to whole
 // sixteens.  Loops are short on purpose: with all copies laid out one after the other the kernel's code is more than the SM's instruction cache
 // holds, and every warp of it waits (by columns, 128 values: 473 -> 604 us).
-template <int DP> struct Copier {
+template <int DP, int KEYS> struct Copier {
   static constexpr int GROUPS = DP / 64;
   const T* from[GROUPS];
   int64_t node;
@@ -99,8 +104,8 @@ template <int DP> struct Copier {
       for (int r = row; r < KEYS; r += every, f += step) copy(d + g * (KEYS * 128) + place(r), f, g, on[g] && r < left);
     }
   }
-  // the same of a stretch that begins with `ns` rows from `from0` on and goes on at `from1`, from its `at`-th row on
-  __device__ __forceinline__ void mixed(unsigned char* dst, int at, int ns, int from0, int from1, int left, int head) const {
+  // the same of a stretch from its `at`-th row on
+  __device__ __forceinline__ void mixed(unsigned char* dst, int at, const Stretch& s, int left, int head) const {
     const uint32_t d = s32(dst);
 #pragma unroll
     for (int g = 0; g < GROUPS; ++g) {
@@ -108,7 +113,7 @@ template <int DP> struct Copier {
 #pragma unroll 2
       for (int r = row; r < KEYS; r += every) {
         const int v = at + r;
-        copy(d + g * (KEYS * 128) + place(r), from[g] + (int64_t)(v < ns ? from0 + v : from1 + v - ns) * node + (int64_t)head * size, g, on[g] && r < left);
+        copy(d + g * (KEYS * 128) + place(r), from[g] + (int64_t)(v < s.ns ? s.from0 + v : s.from1 + v - s.wide) * node + (int64_t)head * size, g, on[g] && r < left && (v < s.ns || v >= s.wide));
       }
     }
   }
@@ -132,14 +137,14 @@ __device__ __forceinline__ void land_at(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(s32(bar)) : "memory");
 }
 
-// The bits of [lo, hi) within 64
-__device__ __forceinline__ uint64_t bits_of(int lo, int hi) {
+// The bits of [lo, hi) within 32
+__device__ __forceinline__ uint32_t bits_of(int lo, int hi) {
   lo = max(lo, 0);
-  hi = min(hi, 64);
-  return hi > lo ? (~uint64_t(0) >> (64 - (hi - lo))) << lo : 0;
+  hi = min(hi, 32);
+  return hi > lo ? (~0u >> (32 - (hi - lo))) << lo : 0;
 }
 
-template <int MODE> __device__ __forceinline__ Stretch stretch_of(const WindowParams& w, int first, int last, int2 a, int2 b) {       // rows first to last, their chains
+template <int MODE, int KEYS> __device__ __forceinline__ Stretch stretch_of(const WindowParams& w, int first, int last, int2 a, int2 b) {       // rows first to last, their chains
   Stretch s;
   s.from0 = s.from1 = first;
   s.ns = 0;
@@ -155,7 +160,8 @@ template <int MODE> __device__ __forceinline__ Stretch stretch_of(const WindowPa
     }
     if (b.y > b.x) s.to1 = min(b.y, last + w.after + 1);
   }
-  s.total = s.ns + s.to1 - s.from1;
+  s.wide = (s.ns + 7) & ~7;
+  s.total = s.wide + s.to1 - s.from1;
   s.steps = (s.total + KEYS - 1) / KEYS;
   return s;
 }
@@ -193,43 +199,61 @@ __device__ __forceinline__ Two add2(Two a, Two b) {
 }
 __device__ __forceinline__ Two bf16_values(uint32_t u) { return Two(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u)); }
 
-// A lane's row of results, with `more` where given, `f` times, to (n, components, heads, channels); whether all of it was finite.
-template <int DP> __device__ __forceinline__ bool put_row(uint32_t sum, float f, bool on, void* out, int row, int head, const AttentionParams& p, const float* more = nullptr,
-                                                          void* rest = nullptr) {
-  bool finite = true;
-  const int values = p.comps * p.size, jump = (p.heads - 1) * p.size;     // to the head's next component, behind the last one's channels
-  const int64_t place = ((int64_t)row * p.comps * p.heads + head) * p.size;
-  T *to = static_cast<T*>(out) + place, *to_rest = static_cast<T*>(rest) + place;
-  int left = p.size;
+// Rows of 64 bytes, a lane each, to lines that four lanes write: piece lane & 3 of the rows of lanes lane, lane ^ 1, lane ^ 2 and lane ^ 3.
+__device__ __forceinline__ void across_lanes(uint32_t (&u)[16], int lane) {
+  const bool b0 = lane & 1, b1 = lane & 2;
 #pragma unroll
-  for (int h = 0; h < DP; h += 32) {
-    if (h >= values) break;
+  for (int k = 0; k < 8; ++k) {                          // halves of the rows
+    const uint32_t keep = b1 ? u[8 + k] : u[k], send = b1 ? u[k] : u[8 + k];
+    u[k] = keep;
+    u[8 + k] = __shfl_xor_sync(0xffffffffu, send, 2);
+  }
+#pragma unroll
+  for (int h = 0; h < 16; h += 8)                        // and of the halves
+#pragma unroll
+    for (int k = h; k < h + 4; ++k) {
+      const uint32_t keep = b0 ? u[4 + k] : u[k], send = b0 ? u[k] : u[4 + k];
+      u[k] = keep;
+      u[4 + k] = __shfl_xor_sync(0xffffffffu, send, 1);
+    }
+}
+
+// Of the lanes' rows of results the WIDE values from the `first` on, with `more` where given, `f` times, to (n, components, heads, channels), and what the rounding
+// left to `rest`; whether they were finite.  Loops are not unrolled: code that runs once a tile comes from beyond the instruction cache.
+template <int WIDE> __device__ __forceinline__ bool put_row(uint32_t sum, int first, float f, bool on, void* out, int row, int head, const AttentionParams& p, int lane,
+                                                            const float* more = nullptr, void* rest = nullptr) {
+  bool finite = true;
+  const int values = p.comps * p.size;
+  const int64_t place = on ? ((int64_t)row * p.comps * p.heads + head) * p.size : -1;
+#pragma unroll 1
+  for (int h = first; h < min(first + WIDE, values); h += 32) {
     uint32_t r[32];
     tmem_issue32(sum + h, r);
     tmem_arrived32(r);
+    if (more) {
 #pragma unroll
-    for (int c = 0; c < 32; c += 8) {
-      const int at = h + c;
-      if (at >= values) break;
-      float v[8];
+      for (int c = 0; c < 32; ++c) r[c] = __float_as_uint(__uint_as_float(r[c]) + (h + c < values ? more[h + c] : 0.f));
+    }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        v[j] = __uint_as_float(r[c + j]);
-        if (more) v[j] += more[at + j];
-        finite = finite && is_finite(v[j]);
-        v[j] *= f;
+    for (int c = 0; c < 32; ++c) finite = finite && (h + c >= values || is_finite(__uint_as_float(r[c])));
+    const int at = h + 8 * (lane & 3), comp = at / p.size;
+    const int64_t offset = (int64_t)comp * (p.heads - 1) * p.size + at;
+    void* base = out;
+#pragma unroll 1
+    for (int t = 0; t < 2 && base; ++t, base = rest) {
+      uint32_t u[16];
+#pragma unroll
+      for (int c = 0; c < 32; c += 2) {
+        const float x = __uint_as_float(r[c]) * f, y = __uint_as_float(r[c + 1]) * f;
+        u[c / 2] = two_bf16(x, y);
+        if (t) u[c / 2] = two_bf16(x - __uint_as_float(u[c / 2] << 16), y - __uint_as_float(u[c / 2] & 0xffff0000u));
       }
-      uint32_t u[4];
+      across_lanes(u, lane);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) u[j] = two_bf16(v[2 * j], v[2 * j + 1]);
-      if (on) *reinterpret_cast<uint4*>(to) = make_uint4(u[0], u[1], u[2], u[3]);
-      if (on && rest) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) u[j] = two_bf16(v[2 * j] - __uint_as_float(u[j] << 16), v[2 * j + 1] - __uint_as_float(u[j] & 0xffff0000u));
-        *reinterpret_cast<uint4*>(to_rest) = make_uint4(u[0], u[1], u[2], u[3]);
+      for (int e = 0; e < 4; ++e) {
+        const int64_t to = __shfl_xor_sync(0xffffffffu, place, e);
+        if (to >= 0 && at < values) *reinterpret_cast<uint4*>(static_cast<T*>(base) + to + offset) = make_uint4(u[4 * e], u[4 * e + 1], u[4 * e + 2], u[4 * e + 3]);
       }
-      to += 8, to_rest += 8;
-      if ((left -= 8) == 0) to += jump, to_rest += jump, left = p.size;
     }
   }
   return finite;
@@ -237,17 +261,18 @@ template <int DP> __device__ __forceinline__ bool put_row(uint32_t sum, float f,
 
 template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::THREADS, Form<DP, MODE>::CTAS) window_tc_kernel(const __grid_constant__ TcParams p) {
   using F = Form<DP, MODE>;
-  constexpr int SLOTS = F::SLOTS, GROUPS = F::GROUPS, BUFFERS = F::BUFFERS;
+  constexpr int KEYS = F::KEYS, SLOTS = F::SLOTS, GROUPS = F::GROUPS, BUFFERS = F::BUFFERS;
   extern __shared__ __align__(1024) unsigned char smem[];
   unsigned char *own = smem, *ring = own + F::OWN * F::OWN_BYTES;
   float* numbers = reinterpret_cast<float*>(ring + SLOTS * F::SLOT_BYTES);
   uint64_t* bars = reinterpret_cast<uint64_t*>(ring + SLOTS * F::SLOT_BYTES + F::NUMBERS);
   uint64_t *full = bars, *empty = full + SLOTS, *scores = empty + SLOTS, *weights = scores + BUFFERS, *freed = weights + BUFFERS, *own_full = freed + BUFFERS,
-           *own_empty = own_full + 1, *done = own_empty + 1, *sums_free = done + 1, *gathered = sums_free + 1, *known = gathered + 1;
+           *own_empty = own_full + 1, *done = own_empty + 1, *sums_free = done + 1, *known = sums_free + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(known + STRETCHES);
   int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
   Stretch* stretches = reinterpret_cast<Stretch*>(reinterpret_cast<unsigned char*>(bars) + F::BARRIERS);
-  unsigned* bad_rows = reinterpret_cast<unsigned*>(stretches + STRETCHES);                                       // [softmax warp][tile of the CTA]
+  unsigned* bad_rows = reinterpret_cast<unsigned*>(stretches + STRETCHES);                                       // [group's quarter][tile of the CTA]
+  float* row_numbers = reinterpret_cast<float*>(bad_rows + 4 * GROUPS * MOST_TILES);
 
   const WindowParams& w = p.w;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -278,16 +303,16 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
     bar_init(own_full, p.tma ? 1 : LOADERS);
     for (int b = 0; b < BUFFERS; ++b) {
       bar_init(&scores[b], 1);
-      bar_init(&weights[b], 4);
+      bar_init(&weights[b], 4 * F::HALVES);
       bar_init(&freed[b], 1);
     }
     for (int k = 0; k < STRETCHES; ++k) bar_init(&known[k], 1);
     bar_init(own_empty, 1);                              // a tile's scores have been made
     bar_init(done, 1);                                   // and its sums
-    bar_init(sums_free, MODE == COLUMNS && GROUPS > 1 ? 8 : 4);
-    bar_init(gathered, 32);                         // a mixed item where others are copied by TMA
+    bar_init(sums_free, (GROUPS > 1 ? 8 : 4) * F::HALVES);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  for (int b = tid; b < 4 * GROUPS * MOST_TILES; b += F::THREADS) bad_rows[b] = 0;
   if (warp == F::SOFT) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s32(tmem_slot)), "r"(F::COLS) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -305,22 +330,22 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
     // the thread that issues the MMAs, which sees them all there, puts the fence between them and the tensor cores.  Copying by hand takes the warps
     // issue slots that the softmax wants (one chain of 32,781 nodes, 8 heads of 128 values, by hand and by TMA: HAND | TMA us).
     const int thread = tid - 32 * (F::SOFT + 2), threads = p.tma ? 32 : LOADERS;
-    const Copier<DP> even(MODE == FORWARD ? w.q.k : MODE == ROWS ? w.q.v : w.q.q, w.q, thread, threads);
-    const Copier<DP> odd(MODE == FORWARD ? w.q.v : MODE == ROWS ? w.q.k : w.q.g, w.q, thread, threads);
-    unsigned item = 0, mixed_items = 0, i = blockIdx.x;
+    const Copier<DP, KEYS> even(MODE == FORWARD ? w.q.k : MODE == ROWS ? w.q.v : w.q.q, w.q, thread, threads);
+    const Copier<DP, KEYS> odd(MODE == FORWARD ? w.q.v : MODE == ROWS ? w.q.k : w.q.g, w.q, thread, threads);
+    unsigned item = 0, i = blockIdx.x;
     Tile next = tile_of(i);
     int2 a = p.spans[next.first], b = p.spans[next.last];
     auto copy_tile = [&](const Tile& t, const Stretch& walk, int steps, int number) {
       // All threads wait for every place, also where one copies: who skips waits gets phases ahead, and a wait by parity cannot tell a phase from the one but next.
-      if (number && !bar_wait(own_empty, (uint32_t)((number - 1) & 1), ab)) return false;
+      if (!__all_sync(0xffffffffu, number == 0 || bar_wait(own_empty, (uint32_t)((number - 1) & 1), ab))) return false;
       if (thread == 0) {
         stretches[number % STRETCHES] = walk;
         bar_arrive(&known[number % STRETCHES]);
       }
       if (!p.tma) {
         const int left = t.last + 1 - t.first;
-        Copier<DP>(MODE == COLUMNS ? w.q.k : w.q.q, w.q, thread, threads).own(own, t.first, left, t.head, high);
-        if (MODE != FORWARD) Copier<DP>(MODE == COLUMNS ? w.q.v : w.q.g, w.q, thread, threads).own(own + F::OWN_BYTES, t.first, left, t.head, high);
+        Copier<DP, KEYS>(MODE == COLUMNS ? w.q.k : w.q.q, w.q, thread, threads).own(own, t.first, left, t.head, high);
+        if (MODE != FORWARD) Copier<DP, KEYS>(MODE == COLUMNS ? w.q.v : w.q.g, w.q, thread, threads).own(own + F::OWN_BYTES, t.first, left, t.head, high);
         land_at(own_full);
       } else if (thread == 0) {
         bar_expect_tx(own_full, F::OWN * F::OWN_BYTES);
@@ -332,22 +357,24 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
       int at = 0, h = MODE == COLUMNS ? t.kv * w.group : t.kv;
       for (int k = 0; k < 2 * steps; ++k, ++item) {
         const unsigned slot = item % SLOTS;
-        const bool mixed = MODE != COLUMNS && at < walk.ns, numbered = MODE == COLUMNS && !(k & 1);
-        if (item >= SLOTS && !bar_wait(&empty[slot], (uint32_t)((item / SLOTS - 1) & 1), ab)) return false;
+        const bool mixed = MODE != COLUMNS && at < walk.wide, numbered = MODE == COLUMNS && !(k & 1);
+        if (!__all_sync(0xffffffffu, item < SLOTS || bar_wait(&empty[slot], (uint32_t)((item / SLOTS - 1) & 1), ab))) return false;
         unsigned char* to = ring + slot * F::SLOT_BYTES;
-        const Copier<DP>& x = k & 1 ? odd : even;
-        if (mixed) {
-          x.mixed(to, at, walk.ns, walk.from0, walk.from1, walk.total - at, h);
-          if (p.tma) {                                   // one arrival for all, none of whom is an item ahead
-            land_at(gathered);
-            if (!bar_wait(gathered, mixed_items++ & 1, ab)) return false;
-            if (thread == 0) bar_arrive(&full[slot]);
-          }
+        const Copier<DP, KEYS>& x = k & 1 ? odd : even;
+        if (mixed && p.tma) {                            // eight rows a copy, each lane its own: all of them by hand took longer than a step
+          if (thread == 0) bar_expect_tx(&full[slot], F::SLOT_BYTES);
+          __syncwarp();
+          const int v = at + 8 * thread;
+          if (8 * thread < KEYS)
+            for (int g = 0; g < DP / 64; ++g)
+              tma_load_3d(to + g * (KEYS * 128) + thread * 1024, &p.eight[k & 1], h * DP + g * 64, v < walk.wide ? walk.from0 + v : walk.from1 + v - walk.wide, 0, &full[slot]);
+        } else if (mixed) {
+          x.mixed(to, at, walk, walk.total - at, h);
         } else if (!p.tma) {
-          x.next(to, walk.from1 + at - walk.ns, walk.total - at, h);
+          x.next(to, walk.from1 + at - walk.wide, walk.total - at, h);
         } else if (thread == 0) {
           bar_expect_tx(&full[slot], F::SLOT_BYTES);
-          for (int g = 0; g < DP / 64; ++g) tma_load_3d(to + g * (KEYS * 128), &p.ring[k & 1], h * DP + g * 64, walk.from1 + at - walk.ns, 0, &full[slot]);
+          for (int g = 0; g < DP / 64; ++g) tma_load_3d(to + g * (KEYS * 128), &p.ring[k & 1], h * DP + g * 64, walk.from1 + at - walk.wide, 0, &full[slot]);
         }
         if (numbered) {
           for (int c = thread; c < KEYS; c += threads) {
@@ -367,7 +394,7 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
     };
     for (int number = 0; thread < threads; ++number) {
       const Tile t = next;
-      const Stretch walk = stretch_of<MODE>(w, t.first, t.last, a, b);
+      const Stretch walk = stretch_of<MODE, KEYS>(w, t.first, t.last, a, b);
       const bool more = p.tiles - i > gridDim.x;
       if (more) {
         next = tile_of(i += gridDim.x);
@@ -398,13 +425,13 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
         for (int k = 1; k < DP / 16; ++k)
           if (k < ksteps) umma_bf16<true>(d, a_lo + (k >> 2) * (TILE_M * 128 / 16) + (k & 3) * K_STEP, b_lo + (k >> 2) * (KEYS * 128 / 16) + (k & 3) * K_STEP, to_scores);
       };
-      // d (128 rows x values) += weights in tensor memory times the slot
+      // d (128 rows x values) += weights in tensor memory, 32 at the front of every 32 columns, times the slot
       auto add = [&](uint32_t d, uint32_t a, uint32_t b, bool more) {
         const uint32_t b_lo = umma_lo_rows(b, KEYS * 128);
         if (more) umma_bf16_ta<true>(d, a, b_lo, to_sums);
         else umma_bf16_ta<false>(d, a, b_lo, to_sums);
 #pragma unroll
-        for (int k = 1; k < KEYS / 16; ++k) umma_bf16_ta<true>(d, a + k * 8, b_lo + k * ROWS_STEP, to_sums);
+        for (int k = 1; k < KEYS / 16; ++k) umma_bf16_ta<true>(d, a + (k >> 1) * 32 + (k & 1) * 8, b_lo + k * ROWS_STEP, to_sums);
       };
       bool ok = true;
       constexpr int S_ITEM = MODE == ROWS ? 1 : 0;
@@ -451,7 +478,7 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
           if (!ok) break;
           tc_fence_after();
           add(sum, d, slot_at(2 * j + 1), more);
-          if (MODE == ROWS) add(sum, d + 32, slot_at(2 * j + 1), true);
+          if (MODE == ROWS) add(sum, d + 16, slot_at(2 * j + 1), true);
           if (MODE == COLUMNS) {
             add(sum + DP, d + KEYS, slot_at(2 * j), more);
             umma_commit(&empty[2 * j % SLOTS]);
@@ -464,8 +491,17 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
     }
   } else {
     // ---------------- softmax ----------------
-    const int quarter = warp & 3, group = warp >> 2, place = quarter * 32 + lane;
+    constexpr int HALVES = F::HALVES, WIDE = DP / HALVES, MINE = KEYS / HALVES, CHUNKS = MINE / 32;         // of the others and the results a thread has a half
+    const int quarter = warp & 3, half = (warp >> 2) % HALVES, group = warp / (4 * HALVES), place = quarter * 32 + lane, first_value = half * WIDE;
     const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16), sum_at = lanes + F::SUM_AT;
+    // whether all threads of a row's two warps have it so; they meet here
+    auto both = [&](bool x) {
+      if (HALVES == 1) return __all_sync(0xffffffffu, x) != 0;
+      int r;
+      asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.s32 p, %1, 0;\n\tbarrier.cta.red.and.pred q, %2, 64, p;\n\tselp.s32 %0, 1, 0, q;\n\t}"
+                   : "=r"(r) : "r"((int)x), "r"(1 + group * 4 + quarter) : "memory");
+      return r != 0;
+    };
     const float unit = w.q.scale * LOG2E;
     bool ok = true;
     unsigned j0 = 0;                                     // steps of the tiles before
@@ -484,7 +520,7 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
     const int2 span = next_span;
     next_span = span_of(i + gridDim.x);
     const bool on = span.y > span.x;
-    ok = __all_sync(0xffffffffu, bar_wait(&known[number % STRETCHES], (uint32_t)(number / STRETCHES & 1), ab));
+    ok = both(bar_wait(&known[number % STRETCHES], (uint32_t)(number / STRETCHES & 1), ab));       // both warps go on or neither
     if (!ok) break;
     const Stretch walk = stretches[number % STRETCHES];
     const int steps = walk.steps * (MODE == COLUMNS ? w.group : 1);
@@ -492,10 +528,10 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
     const int lo = !on ? 0 : max(span.x, row - (MODE == COLUMNS ? w.after : w.before));
     const int hi = !on ? 0 : MODE == COLUMNS ? (!w.split && row < span.x + w.sinks ? span.y : min(span.y, row + w.before + 1)) : min(span.y, row + w.after + 1);
     const int far = on && MODE != COLUMNS ? min(lo, span.x + w.sinks) : 0;
-    // as bits of the 64 from the stretch's `at`-th on; first nodes are before `from1`, or in the stretch behind it, or both
+    // as bits of the 32 from the stretch's `at`-th on; first nodes are before `from1`, or in the stretch behind it, or both
     auto seen = [&](int at) {
-      const int shift = walk.from1 - walk.ns + at;
-      uint64_t bits = bits_of(lo - shift, hi - shift);
+      const int shift = walk.from1 - walk.wide + at;
+      uint32_t bits = bits_of(lo - shift, hi - shift);
       if (MODE != COLUMNS) {
         bits |= bits_of(max(span.x, walk.from1) - shift, far - shift);
         if (at < walk.ns && span.x < walk.from1) bits |= bits_of(span.x - walk.from0 - at, min(far - walk.from0, walk.ns) - at);
@@ -504,8 +540,8 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
     };
     // all sums of the tile are there; after reading them they may be written again
     auto sums_there = [&] {
-      ok = __all_sync(0xffffffffu, ok);
-      if (ok) ok = __all_sync(0xffffffffu, bar_wait(done, (uint32_t)(number & 1), ab));
+      ok = both(ok);
+      if (ok) ok = both(bar_wait(done, (uint32_t)(number & 1), ab));
       tc_fence_after();
       return ok;
     };
@@ -514,82 +550,91 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
       const unsigned rows = __ballot_sync(0xffffffffu, bad);
       if (lane == 0) {
         bar_arrive(sums_free);
-        bad_rows[warp * MOST_TILES + number] = rows;
+        if (rows) atomicOr(&bad_rows[(group * 4 + quarter) * MOST_TILES + number], rows);
       }
       tiles_done = number + 1;
     };
     if (MODE == FORWARD) {
       float base = -INFINITY, total = 0.f;
+      float* maxima = row_numbers + place;                                         // of the halves
+      float* totals = row_numbers + (2 + 2 * (number & 1)) * TILE_M + place;       // what a tile leaves is read before the next but one writes
       for (int k = 0; k < steps; ++k) {
-        const unsigned j = j0 + k, b = j & 1;
-        ok = bar_wait(&scores[b], (j >> 1) & 1, ab);
-        if (!__all_sync(0xffffffffu, ok)) break;
+        const unsigned j = j0 + k, b = j % BUFFERS;
+        ok = __all_sync(0xffffffffu, bar_wait(&scores[b], (j / BUFFERS) & 1, ab));
         tc_fence_after();
-        const uint32_t s_at = lanes + b * F::BUFFER;
-        uint32_t raw[2][32];
-        tmem_issue32(s_at, raw[0]);
-        tmem_issue32(s_at + 32, raw[1]);
-        const uint64_t bits = seen(k * KEYS);
-        tmem_arrived32(raw[0]);
-        tmem_arrived32(raw[1]);
-        if (!__all_sync(0xffffffffu, bits == ~uint64_t(0))) {
+        const uint32_t s_at = lanes + b * F::BUFFER + MINE * half;
+        // Scores are read once for the greatest and once more for the weights: 64 of them in registers want more than there are
+        uint32_t raw[32];
+        auto read = [&](int c0) {
+          tmem_issue32(s_at + c0, raw);
+          const uint32_t bits = seen(k * KEYS + MINE * half + c0);
+          tmem_arrived32(raw);
+          if (__all_sync(0xffffffffu, bits == ~0u)) return;
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint32_t word = (uint32_t)(bits >> (32 * h));
-#pragma unroll
-            for (int c = 0; c < 32; ++c) raw[h][c] = (word >> c) & 1 ? raw[h][c] : 0xff800000u;
-          }
-        }
+          for (int c = 0; c < 32; ++c) raw[c] = (bits >> c) & 1 ? raw[c] : 0xff800000u;
+        };
         float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int c = 0; c < 64; ++c) most[c & 3] = fmaxf(most[c & 3], __uint_as_float(raw[c >> 5][c & 31]));
-        const float now = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * unit;
-        const bool higher = now > base + FAR || (base == -INFINITY && now > base);
-        if (__any_sync(0xffffffffu, higher)) {           // another unit: what there is so far goes by it
+        for (int h = 0; h < CHUNKS; ++h) {
+          read(32 * h);
+#pragma unroll
+          for (int c = 0; c < 32; ++c) most[c & 3] = fmaxf(most[c & 3], __uint_as_float(raw[c]));
+        }
+        float now = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * unit;
+        if (!both(ok && !(now > base + FAR || (base == -INFINITY && now > base)))) {          // another unit: what there is so far goes by it
+          maxima[half * TILE_M] = now;
+          ok = both(ok);
+          if (!ok) break;
+          now = fmaxf(now, maxima[(half ^ 1) * TILE_M]);
+          const bool higher = now > base + FAR || (base == -INFINITY && now > base);
           const float keep = !higher ? 1.f : base == -INFINITY ? 0.f : exp2_fast(base - now);
           total *= keep;
           if (higher) base = now;
           if (k > 0) {
-            ok = bar_wait(&freed[(j - 1) & 1], ((j - 1) >> 1) & 1, ab);
-            if (!__all_sync(0xffffffffu, ok)) break;
+            ok = both(bar_wait(&freed[(j - 1) % BUFFERS], ((j - 1) / BUFFERS) & 1, ab));
+            if (!ok) break;
             tc_fence_after();
 #pragma unroll
-            for (int h = 0; h < DP; h += 32) {
-              if (h >= wide) break;
+            for (int h = 0; h < WIDE; h += 32) {
+              if (first_value + h >= wide) break;
               float v[32];
-              tmem_ld32(sum_at + h, v);
+              tmem_ld32(sum_at + first_value + h, v);
 #pragma unroll
               for (int c = 0; c < 32; ++c) v[c] *= keep;
-              tmem_st32(sum_at + h, v);
+              tmem_st32(sum_at + first_value + h, v);
             }
           }
         }
         const float minus = base == -INFINITY ? 0.f : -base;
         const Two units(unit, unit), minuses(minus, minus);
         Two add[2] = {Two(0.f, 0.f), Two(0.f, 0.f)};
-        uint32_t out[32];
 #pragma unroll
-        for (int c = 0; c < 64; c += 2) {
-          float x, y;
-          fma2(two_of(&raw[c >> 5][c & 31]), units, minuses).apart(x, y);
-          out[c >> 1] = two_bf16(exp2_fast(x), exp2_fast(y));
-          add[(c >> 1) & 1] = add2(add[(c >> 1) & 1], bf16_values(out[c >> 1]));       // the sum is that of the rounded weights
+        for (int h = CHUNKS - 1; h >= 0; --h) {          // the last is there already
+          if (h < CHUNKS - 1) read(32 * h);
+          uint32_t out[16];
+#pragma unroll
+          for (int c = 0; c < 32; c += 2) {
+            float x, y;
+            fma2(two_of(&raw[c]), units, minuses).apart(x, y);
+            out[c >> 1] = two_bf16(exp2_fast(x), exp2_fast(y));
+            add[(c >> 1) & 1] = add2(add[(c >> 1) & 1], bf16_values(out[c >> 1]));     // the sum is that of the rounded weights
+          }
+          tmem_put16(s_at + 32 * h, out);
         }
         float even, odd;
         add2(add[0], add[1]).apart(even, odd);
         total += even + odd;
-        tmem_put16(s_at, out);
-        tmem_put16(s_at + 16, out + 16);
         tmem_stored();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) bar_arrive(&weights[b]);
       }
+      totals[half * TILE_M] = total;
       if (sums_there()) {
-        const float inverse = 1.f / total;
-        const bool finite = put_row<DP>(sum_at, inverse, on, w.q.out, row, mine, w.q, nullptr, w.rest);
+        const float inverse = 1.f / (totals[0] + totals[TILE_M]);
+        const bool finite = put_row<WIDE>(sum_at, first_value, inverse, on, w.q.out, row, mine, w.q, lane, nullptr, w.rest);
         sums_read(on && !finite);
-        if (on && w.q.top) w.q.top[(int64_t)mine * w.q.n + row] = base, w.q.inverse[(int64_t)mine * w.q.n + row] = inverse;
+        if (on && w.q.top && half == 0) w.q.top[(int64_t)mine * w.q.n + row] = base, w.q.inverse[(int64_t)mine * w.q.n + row] = inverse;
       }
     } else if (MODE == ROWS) {
       const int64_t at_row = (int64_t)mine * w.q.n + row;
@@ -603,56 +648,54 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
         ok = bar_wait(&scores[b], (j / BUFFERS) & 1, ab);
         if (!__all_sync(0xffffffffu, ok)) break;
         tc_fence_after();
-        const uint64_t bits = seen(k * KEYS);
-        const bool all = __all_sync(0xffffffffu, bits == ~uint64_t(0));
-        uint32_t s[2][32], d[32], large[16], small[16];
-        const uint32_t s_at = lanes + b * F::BUFFER;
-        tmem_issue32(s_at, s[0]);
-        tmem_issue32(s_at + 32, s[1]);
-        tmem_arrived32(s[0]);
-        tmem_arrived32(s[1]);
+        const uint32_t word = seen(k * KEYS + 32 * half);
+        const bool all = __all_sync(0xffffffffu, word == ~0u);
+        uint32_t s[32], d[32], large[16], small[16];
+        const uint32_t s_at = lanes + b * F::BUFFER + 32 * half;
+        tmem_issue32(s_at, s);
+        tmem_issue32(s_at + KEYS, d);
+        tmem_arrived32(s);
+        tmem_arrived32(d);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          tmem_issue32(s_at + KEYS + 32 * h, d);
-          tmem_arrived32(d);
-          const uint32_t word = (uint32_t)(bits >> (32 * h));
-#pragma unroll
-          for (int c = 0; c < 32; c += 2) {
-            float e[2], x[2];
-            fma2(two_of(&s[h][c]), units, minuses).apart(e[0], e[1]);
-            Two dp = two_of(&d[c]);
-            e[0] = exp2_fast(e[0]), e[1] = exp2_fast(e[1]);
-            if (!all) {                                  // zero times zero for what is not seen
-              const bool see[2] = {(bool)((word >> c) & 1), (bool)((word >> (c + 1)) & 1)};
-              e[0] = see[0] ? e[0] : 0.f, e[1] = see[1] ? e[1] : 0.f;
-              dp = Two(see[0] ? __uint_as_float(d[c]) : 0.f, see[1] ? __uint_as_float(d[c + 1]) : 0.f);
-            }
-            const Two before(e[0], e[1]);
-            sums = add2(sums, before);
-            exact = fma2(before, dp, exact);
-            const Two ds = mul2(bf16_values(two_bf16(e[0], e[1])), fma2(dp, inverses, deltas));
-            ds.apart(x[0], x[1]);
-            large[c / 2] = two_bf16(x[0], x[1]);
-            fma2(bf16_values(large[c / 2]), less, ds).apart(x[0], x[1]);
-            small[c / 2] = two_bf16(x[0], x[1]);
+        for (int c = 0; c < 32; c += 2) {
+          float e[2], x[2];
+          fma2(two_of(&s[c]), units, minuses).apart(e[0], e[1]);
+          Two dp = two_of(&d[c]);
+          e[0] = exp2_fast(e[0]), e[1] = exp2_fast(e[1]);
+          if (!all) {                                  // zero times zero for what is not seen
+            const bool see[2] = {(bool)((word >> c) & 1), (bool)((word >> (c + 1)) & 1)};
+            e[0] = see[0] ? e[0] : 0.f, e[1] = see[1] ? e[1] : 0.f;
+            dp = Two(see[0] ? __uint_as_float(d[c]) : 0.f, see[1] ? __uint_as_float(d[c + 1]) : 0.f);
           }
-          tmem_put16(s_at + 16 * h, large);
-          tmem_put16(s_at + 32 + 16 * h, small);
+          const Two before(e[0], e[1]);
+          sums = add2(sums, before);
+          exact = fma2(before, dp, exact);
+          const Two ds = mul2(bf16_values(two_bf16(e[0], e[1])), fma2(dp, inverses, deltas));
+          ds.apart(x[0], x[1]);
+          large[c / 2] = two_bf16(x[0], x[1]);
+          fma2(bf16_values(large[c / 2]), less, ds).apart(x[0], x[1]);
+          small[c / 2] = two_bf16(x[0], x[1]);
         }
+        tmem_put16(s_at, large);
+        tmem_put16(s_at + 16, small);
         tmem_stored();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) bar_arrive(&weights[b]);
       }
       if (sums_there()) {
-        const bool finite = put_row<DP>(sum_at, w.q.scale, on, w.q.dq, row, mine, w.q);
+        const bool finite = put_row<WIDE>(sum_at, first_value, w.q.scale, on, w.q.dq, row, mine, w.q, lane);
         sums_read(on && !finite);
-        if (on) {
-          float s[2], x[2];
-          sums.apart(s[0], s[1]), exact.apart(x[0], x[1]);
-          const float sum = 1.f / (s[0] + s[1]);
-          w.q.delta[at_row] = (x[0] + x[1]) * sum;
-          w.inverse[at_row] = sum;
+        // One half leaves its sums where the other's go, whose threads have had delta and wait for it (there is no more shared memory at 128 values).
+        float s[2], x[2];
+        sums.apart(s[0], s[1]), exact.apart(x[0], x[1]);
+        float weight = s[0] + s[1], weighted = x[0] + x[1];
+        if (half && on) w.inverse[at_row] = weight, w.q.delta[at_row] = weighted;
+        both(true);
+        if (!half && on) {
+          weight = 1.f / (weight + w.inverse[at_row]);
+          w.q.delta[at_row] = (weighted + w.q.delta[at_row]) * weight;
+          w.inverse[at_row] = weight;
         }
       }
     } else {
@@ -664,19 +707,19 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
         ok = bar_wait(&full[slot], (2 * j / SLOTS) & 1, ab) && bar_wait(&scores[b], (j / BUFFERS) & 1, ab);
         if (!__all_sync(0xffffffffu, ok)) break;
         tc_fence_after();
-        const uint64_t bits = seen(at);
+        const int from = at;
         for (at += GROUPS * KEYS; at >= walk.steps * KEYS;) at -= walk.steps * KEYS;
-        const bool all = __all_sync(0xffffffffu, bits == ~uint64_t(0));
         const float* num = numbers + slot / 2 * 3 * KEYS;
         const uint32_t s_at = lanes + b * F::BUFFER;
 #pragma unroll 1
-        for (int h = 0; h < 2; ++h) {
+        for (int h = half * CHUNKS; h < (half + 1) * CHUNKS; ++h) {
+          const uint32_t word = seen(from + 32 * h);
+          const bool all = __all_sync(0xffffffffu, word == ~0u);
           uint32_t s[32], d[32], pt[16], dst[16];
           tmem_issue32(s_at + 32 * h, s);
           tmem_issue32(s_at + KEYS + 32 * h, d);
           tmem_arrived32(s);
           tmem_arrived32(d);
-          const uint32_t word = (uint32_t)(bits >> (32 * h));
 #pragma unroll
           for (int c = 0; c < 32; c += 4) {
             const float4 top = *reinterpret_cast<const float4*>(num + 32 * h + c), inverse = *reinterpret_cast<const float4*>(num + KEYS + 32 * h + c),
@@ -704,8 +747,8 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
             dst[c / 2] = two_bf16(y[0], y[1]);
             dst[c / 2 + 1] = two_bf16(y[2], y[3]);
           }
-          tmem_put16(s_at + 16 * h, pt);
-          tmem_put16(s_at + KEYS + 16 * h, dst);
+          tmem_put16(s_at + 32 * h, pt);
+          tmem_put16(s_at + KEYS + 32 * h, dst);
         }
         tmem_stored();
         tc_fence_before();
@@ -713,23 +756,23 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
         if (lane == 0) bar_arrive(&weights[b]);
       }
       // one group stores each sum, the others go on
-      ok = __all_sync(0xffffffffu, ok);
+      ok = both(ok);
       if ((group == 0 || group == GROUPS - 1) && sums_there()) {
         bool finite = true;
         const float* more = on ? far_of(w, row, tile.kv, span.x, span.y) : nullptr;
-        if (group == 0) finite = put_row<DP>(sum_at, 1.f, on, w.kv.dv, row, tile.kv, w.kv, more ? more + FAR_ROWS * values : nullptr);
-        if (group == GROUPS - 1) finite = put_row<DP>(sum_at + DP, w.q.scale, on, w.kv.dk, row, tile.kv, w.kv, more) && finite;
+        if (group == 0) finite = put_row<WIDE>(sum_at, first_value, 1.f, on, w.kv.dv, row, tile.kv, w.kv, lane, more ? more + FAR_ROWS * values : nullptr);
+        if (group == GROUPS - 1) finite = put_row<WIDE>(sum_at + DP, first_value, w.q.scale, on, w.kv.dk, row, tile.kv, w.kv, lane, more) && finite;
         sums_read(on && !finite);
       }
     }
     j0 += steps;
     if (!__all_sync(0xffffffffu, ok)) break;
     }
-    // Rows that are not finite, when no role waits for this one any more: a row takes long.
-    __syncwarp();
-    for (int number = 0; number < tiles_done; ++number) {
+    // Rows that are not finite, when no role waits for this one any more and both halves have theirs: a row takes long.
+    asm volatile("barrier.cta.sync 15, %0;" ::"n"(32 * F::SOFT) : "memory");
+    for (int number = half; number < tiles_done; number += HALVES) {
       const Tile tile = tile_of(blockIdx.x + number * gridDim.x);
-      for (unsigned bad = bad_rows[warp * MOST_TILES + number]; bad; bad &= bad - 1) {
+      for (unsigned bad = bad_rows[(group * 4 + quarter) * MOST_TILES + number]; bad; bad &= bad - 1) {
         const int at = quarter * 32 + __ffs(bad) - 1, row = tile.first + at % high, mine = tile.head + at / high;
         const int2 span = p.spans[row];
         if (MODE == FORWARD) again_forward<T>(w, row, mine, span.x, span.y, lane);
@@ -811,11 +854,12 @@ template <int DP, int MODE> int launch(const TcParams& p, cudaStream_t s) {
     const int kv_heads = p.w.kv.heads, high = TILE_M / p.pack;
     int rc;
     if (MODE == COLUMNS) {
-      (void)((rc = map(&t.own[0], q.k, kv_heads, TILE_M)) || (rc = map(&t.own[1], q.v, kv_heads, TILE_M)) || (rc = map(&t.ring[0], q.q, q.heads, KEYS)) ||
-             (rc = map(&t.ring[1], q.g, q.heads, KEYS)));
+      (void)((rc = map(&t.own[0], q.k, kv_heads, TILE_M)) || (rc = map(&t.own[1], q.v, kv_heads, TILE_M)) || (rc = map(&t.ring[0], q.q, q.heads, F::KEYS)) ||
+             (rc = map(&t.ring[1], q.g, q.heads, F::KEYS)));
     } else {
       (void)((rc = map(&t.own[0], q.q, q.heads, high)) || (MODE == ROWS && (rc = map(&t.own[1], q.g, q.heads, high))) ||
-             (rc = map(&t.ring[MODE == ROWS], q.k, kv_heads, KEYS)) || (rc = map(&t.ring[MODE == FORWARD], q.v, kv_heads, KEYS)));
+             (rc = map(&t.ring[MODE == ROWS], q.k, kv_heads, F::KEYS)) || (rc = map(&t.ring[MODE == FORWARD], q.v, kv_heads, F::KEYS)) ||
+             (rc = map(&t.eight[MODE == ROWS], q.k, kv_heads, 8)) || (rc = map(&t.eight[MODE == FORWARD], q.v, kv_heads, 8)));
     }
     if (rc) return rc;
   }

@@ -8,7 +8,7 @@ namespace eqt {
 namespace window {
 
 struct alignas(64) TcParams {
-  CUtensorMap own[2], ring[2];   // where `tma`: of the tile's operands, and of the others in the order of their use
+  CUtensorMap own[2], ring[2], eight[2];   // where `tma`: of the tile's operands, of the others in the order of their use, and of eight rows of these
   WindowParams w;
   const int2* spans;         // [node]: its chain
   unsigned tiles;
