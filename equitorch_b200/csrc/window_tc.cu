@@ -34,7 +34,7 @@ using attention::copy4;
 using T = __nv_bfloat16;
 
 enum Mode { FORWARD, ROWS, COLUMNS };
-constexpr int LOADERS = 64;                              // threads that copy
+constexpr int KEYS = 64, LOADERS = 64;                   // of the other side at a time; threads that copy
 constexpr int MOST_TILES = 16;                           // of a CTA
 constexpr float FAR = 8.f;                               // of log2, that a score may be above the unit
 
@@ -47,20 +47,18 @@ constexpr int STRETCHES = 8;
 
 template <int DP, int MODE> struct Form {
   static constexpr int GROUPS = MODE == COLUMNS ? (DP == 128 ? 2 : 3) : 1;             // of softmax warps, each with a buffer of scores
-  static constexpr int KEYS = MODE == FORWARD && DP == 128 ? 128 : 64;                 // of the other side at a time
-  static constexpr int BUFFERS = MODE == FORWARD ? 128 / KEYS : GROUPS;
-  static constexpr int HALVES = MODE == COLUMNS ? 1 : 2;                               // warps that share a row's others
+  static constexpr int BUFFERS = MODE == FORWARD ? 2 : GROUPS;
+  static constexpr int HALVES = MODE == ROWS ? 2 : 1;                               // warps that share a row's others
   static constexpr int SOFT = 4 * HALVES * GROUPS, THREADS = 32 * (SOFT + 2) + LOADERS, CTAS = GROUPS > 1 ? 1 : 2;
   static constexpr int OWN = MODE == FORWARD ? 1 : 2;                                // operands of the tile's rows
   static constexpr int OWN_BYTES = TILE_M * DP * 2, SLOT_BYTES = KEYS * DP * 2;
-  static constexpr int SLOTS = MODE == FORWARD && DP == 128 ? 2 : MODE == ROWS && DP == 128 ? 3 : 8;
+  static constexpr int SLOTS = MODE == FORWARD && DP == 128 ? 4 : MODE == ROWS && DP == 128 ? 3 : 8;
   static constexpr int NUMBERS = MODE == COLUMNS ? SLOTS / 2 * 3 * KEYS * 4 : 0;     // bytes: a query's greatest score, inverse sum, delta
   static constexpr int BUFFER = MODE == FORWARD ? KEYS : 2 * KEYS;                   // columns of tensor memory: S, or S and dP
   static constexpr int SUM_AT = BUFFERS * BUFFER, COLS = CTAS == 1 ? 512 : 256;
   static constexpr int BARRIERS = 384;                                               // bytes, with the tensor memory's address and the abort flag
-  static constexpr int ROW_NUMBERS = MODE == FORWARD ? 6 * TILE_M * 4 : 0;           // bytes: halves' maxima, and sums of two tiles
   static constexpr size_t bytes() {
-    return (size_t)OWN * OWN_BYTES + (size_t)SLOTS * SLOT_BYTES + NUMBERS + BARRIERS + STRETCHES * sizeof(Stretch) + 4 * GROUPS * MOST_TILES * 4 + ROW_NUMBERS;
+    return (size_t)OWN * OWN_BYTES + (size_t)SLOTS * SLOT_BYTES + NUMBERS + BARRIERS + STRETCHES * sizeof(Stretch) + 4 * GROUPS * MOST_TILES * 4;
   }
   static_assert((2 * SLOTS + 3 * BUFFERS + 4 + STRETCHES) * 8 + 8 <= BARRIERS, "barriers");
   static_assert(SUM_AT + (MODE == COLUMNS ? 2 : 1) * DP <= COLS, "tensor memory");
@@ -70,7 +68,7 @@ template <int DP, int MODE> struct Form {
 // from moves on by additions; and goes to, but for the 128-byte swizzle (a line of 128 bytes a row).  Zeros behind the head's values, up to whole
 // sixteens.  Loops are short on purpose: with all copies laid out one after the other the kernel's code is more than the SM's instruction cache
 // holds, and every warp of it waits (by columns, 128 values: 473 -> 604 us).
-template <int DP, int KEYS> struct Copier {
+template <int DP> struct Copier {
   static constexpr int GROUPS = DP / 64;
   const T* from[GROUPS];
   int64_t node;
@@ -144,7 +142,7 @@ __device__ __forceinline__ uint32_t bits_of(int lo, int hi) {
   return hi > lo ? (~0u >> (32 - (hi - lo))) << lo : 0;
 }
 
-template <int MODE, int KEYS> __device__ __forceinline__ Stretch stretch_of(const WindowParams& w, int first, int last, int2 a, int2 b) {       // rows first to last, their chains
+template <int MODE> __device__ __forceinline__ Stretch stretch_of(const WindowParams& w, int first, int last, int2 a, int2 b) {       // rows first to last, their chains
   Stretch s;
   s.from0 = s.from1 = first;
   s.ns = 0;
@@ -222,20 +220,28 @@ __device__ __forceinline__ void across_lanes(uint32_t (&u)[16], int lane) {
 // left to `rest`; whether they were finite.  Loops are not unrolled: code that runs once a tile comes from beyond the instruction cache.
 template <int WIDE> __device__ __forceinline__ bool put_row(uint32_t sum, int first, float f, bool on, void* out, int row, int head, const AttentionParams& p, int lane,
                                                             const float* more = nullptr, void* rest = nullptr) {
-  bool finite = true;
   const int values = p.comps * p.size;
   const int64_t place = on ? ((int64_t)row * p.comps * p.heads + head) * p.size : -1;
+  int64_t to[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) to[e] = __shfl_xor_sync(0xffffffffu, place, e);
+  const Two times(f, f), zero(0.f, 0.f), less(-1.f, -1.f);
+  Two nought = zero;                                     // or NaN, once a sum is not finite
 #pragma unroll 1
   for (int h = first; h < min(first + WIDE, values); h += 32) {
     uint32_t r[32];
     tmem_issue32(sum + h, r);
     tmem_arrived32(r);
-    if (more) {
 #pragma unroll
-      for (int c = 0; c < 32; ++c) r[c] = __float_as_uint(__uint_as_float(r[c]) + (h + c < values ? more[h + c] : 0.f));
+    for (int c = 0; c < 32; c += 8) {
+      if (h + c >= values) break;
+      if (more) {
+#pragma unroll
+        for (int j = c; j < c + 8; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) + more[h + j]);
+      }
+#pragma unroll
+      for (int j = c; j < c + 8; j += 2) nought = fma2(two_of(&r[j]), zero, nought);
     }
-#pragma unroll
-    for (int c = 0; c < 32; ++c) finite = finite && (h + c >= values || is_finite(__uint_as_float(r[c])));
     const int at = h + 8 * (lane & 3), comp = at / p.size;
     const int64_t offset = (int64_t)comp * (p.heads - 1) * p.size + at;
     void* base = out;
@@ -244,24 +250,29 @@ template <int WIDE> __device__ __forceinline__ bool put_row(uint32_t sum, int fi
       uint32_t u[16];
 #pragma unroll
       for (int c = 0; c < 32; c += 2) {
-        const float x = __uint_as_float(r[c]) * f, y = __uint_as_float(r[c + 1]) * f;
+        const Two v = mul2(two_of(&r[c]), times);
+        float x, y;
+        v.apart(x, y);
         u[c / 2] = two_bf16(x, y);
-        if (t) u[c / 2] = two_bf16(x - __uint_as_float(u[c / 2] << 16), y - __uint_as_float(u[c / 2] & 0xffff0000u));
+        if (t) {
+          fma2(bf16_values(u[c / 2]), less, v).apart(x, y);
+          u[c / 2] = two_bf16(x, y);
+        }
       }
       across_lanes(u, lane);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int64_t to = __shfl_xor_sync(0xffffffffu, place, e);
-        if (to >= 0 && at < values) *reinterpret_cast<uint4*>(static_cast<T*>(base) + to + offset) = make_uint4(u[4 * e], u[4 * e + 1], u[4 * e + 2], u[4 * e + 3]);
-      }
+      for (int e = 0; e < 4; ++e)
+        if (to[e] >= 0 && at < values) *reinterpret_cast<uint4*>(static_cast<T*>(base) + to[e] + offset) = make_uint4(u[4 * e], u[4 * e + 1], u[4 * e + 2], u[4 * e + 3]);
     }
   }
-  return finite;
+  float x, y;
+  nought.apart(x, y);
+  return x + y == 0.f;
 }
 
 template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::THREADS, Form<DP, MODE>::CTAS) window_tc_kernel(const __grid_constant__ TcParams p) {
   using F = Form<DP, MODE>;
-  constexpr int KEYS = F::KEYS, SLOTS = F::SLOTS, GROUPS = F::GROUPS, BUFFERS = F::BUFFERS;
+  constexpr int SLOTS = F::SLOTS, GROUPS = F::GROUPS, BUFFERS = F::BUFFERS;
   extern __shared__ __align__(1024) unsigned char smem[];
   unsigned char *own = smem, *ring = own + F::OWN * F::OWN_BYTES;
   float* numbers = reinterpret_cast<float*>(ring + SLOTS * F::SLOT_BYTES);
@@ -272,7 +283,6 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
   int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
   Stretch* stretches = reinterpret_cast<Stretch*>(reinterpret_cast<unsigned char*>(bars) + F::BARRIERS);
   unsigned* bad_rows = reinterpret_cast<unsigned*>(stretches + STRETCHES);                                       // [group's quarter][tile of the CTA]
-  float* row_numbers = reinterpret_cast<float*>(bad_rows + 4 * GROUPS * MOST_TILES);
 
   const WindowParams& w = p.w;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -330,8 +340,8 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
     // the thread that issues the MMAs, which sees them all there, puts the fence between them and the tensor cores.  Copying by hand takes the warps
     // issue slots that the softmax wants (one chain of 32,781 nodes, 8 heads of 128 values, by hand and by TMA: HAND | TMA us).
     const int thread = tid - 32 * (F::SOFT + 2), threads = p.tma ? 32 : LOADERS;
-    const Copier<DP, KEYS> even(MODE == FORWARD ? w.q.k : MODE == ROWS ? w.q.v : w.q.q, w.q, thread, threads);
-    const Copier<DP, KEYS> odd(MODE == FORWARD ? w.q.v : MODE == ROWS ? w.q.k : w.q.g, w.q, thread, threads);
+    const Copier<DP> even(MODE == FORWARD ? w.q.k : MODE == ROWS ? w.q.v : w.q.q, w.q, thread, threads);
+    const Copier<DP> odd(MODE == FORWARD ? w.q.v : MODE == ROWS ? w.q.k : w.q.g, w.q, thread, threads);
     unsigned item = 0, i = blockIdx.x;
     Tile next = tile_of(i);
     int2 a = p.spans[next.first], b = p.spans[next.last];
@@ -344,8 +354,8 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
       }
       if (!p.tma) {
         const int left = t.last + 1 - t.first;
-        Copier<DP, KEYS>(MODE == COLUMNS ? w.q.k : w.q.q, w.q, thread, threads).own(own, t.first, left, t.head, high);
-        if (MODE != FORWARD) Copier<DP, KEYS>(MODE == COLUMNS ? w.q.v : w.q.g, w.q, thread, threads).own(own + F::OWN_BYTES, t.first, left, t.head, high);
+        Copier<DP>(MODE == COLUMNS ? w.q.k : w.q.q, w.q, thread, threads).own(own, t.first, left, t.head, high);
+        if (MODE != FORWARD) Copier<DP>(MODE == COLUMNS ? w.q.v : w.q.g, w.q, thread, threads).own(own + F::OWN_BYTES, t.first, left, t.head, high);
         land_at(own_full);
       } else if (thread == 0) {
         bar_expect_tx(own_full, F::OWN * F::OWN_BYTES);
@@ -360,7 +370,7 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
         const bool mixed = MODE != COLUMNS && at < walk.wide, numbered = MODE == COLUMNS && !(k & 1);
         if (!__all_sync(0xffffffffu, item < SLOTS || bar_wait(&empty[slot], (uint32_t)((item / SLOTS - 1) & 1), ab))) return false;
         unsigned char* to = ring + slot * F::SLOT_BYTES;
-        const Copier<DP, KEYS>& x = k & 1 ? odd : even;
+        const Copier<DP>& x = k & 1 ? odd : even;
         if (mixed && p.tma) {                            // eight rows a copy, each lane its own: all of them by hand took longer than a step
           if (thread == 0) bar_expect_tx(&full[slot], F::SLOT_BYTES);
           __syncwarp();
@@ -394,7 +404,7 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
     };
     for (int number = 0; thread < threads; ++number) {
       const Tile t = next;
-      const Stretch walk = stretch_of<MODE, KEYS>(w, t.first, t.last, a, b);
+      const Stretch walk = stretch_of<MODE>(w, t.first, t.last, a, b);
       const bool more = p.tiles - i > gridDim.x;
       if (more) {
         next = tile_of(i += gridDim.x);
@@ -491,7 +501,7 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
     }
   } else {
     // ---------------- softmax ----------------
-    constexpr int HALVES = F::HALVES, WIDE = DP / HALVES, MINE = KEYS / HALVES, CHUNKS = MINE / 32;         // of the others and the results a thread has a half
+    constexpr int HALVES = F::HALVES, WIDE = DP / HALVES, CHUNKS = KEYS / HALVES / 32;         // a thread's part of the results and of 64 others
     const int quarter = warp & 3, half = (warp >> 2) % HALVES, group = warp / (4 * HALVES), place = quarter * 32 + lane, first_value = half * WIDE;
     const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16), sum_at = lanes + F::SUM_AT;
     // whether all threads of a row's two warps have it so; they meet here
@@ -556,52 +566,45 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
     };
     if (MODE == FORWARD) {
       float base = -INFINITY, total = 0.f;
-      float* maxima = row_numbers + place;                                         // of the halves
-      float* totals = row_numbers + (2 + 2 * (number & 1)) * TILE_M + place;       // what a tile leaves is read before the next but one writes
       for (int k = 0; k < steps; ++k) {
         const unsigned j = j0 + k, b = j % BUFFERS;
         ok = __all_sync(0xffffffffu, bar_wait(&scores[b], (j / BUFFERS) & 1, ab));
+        if (!ok) break;
         tc_fence_after();
-        const uint32_t s_at = lanes + b * F::BUFFER + MINE * half;
-        // Scores are read once for the greatest and once more for the weights: 64 of them in registers want more than there are
-        uint32_t raw[32];
-        auto read = [&](int c0) {
-          tmem_issue32(s_at + c0, raw);
-          const uint32_t bits = seen(k * KEYS + MINE * half + c0);
-          tmem_arrived32(raw);
-          if (__all_sync(0xffffffffu, bits == ~0u)) return;
+        const uint32_t s_at = lanes + b * F::BUFFER;
+        uint32_t raw[CHUNKS][32];
 #pragma unroll
-          for (int c = 0; c < 32; ++c) raw[c] = (bits >> c) & 1 ? raw[c] : 0xff800000u;
-        };
+        for (int h = 0; h < CHUNKS; ++h) tmem_issue32(s_at + 32 * h, raw[h]);
         float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int h = 0; h < CHUNKS; ++h) {
-          read(32 * h);
+          tmem_arrived32(raw[h]);
+          const uint32_t bits = seen(k * KEYS + 32 * h);
+          if (!__all_sync(0xffffffffu, bits == ~0u)) {
 #pragma unroll
-          for (int c = 0; c < 32; ++c) most[c & 3] = fmaxf(most[c & 3], __uint_as_float(raw[c]));
+            for (int c = 0; c < 32; ++c) raw[h][c] = (bits >> c) & 1 ? raw[h][c] : 0xff800000u;
+          }
+#pragma unroll
+          for (int c = 0; c < 32; ++c) most[c & 3] = fmaxf(most[c & 3], __uint_as_float(raw[h][c]));
         }
-        float now = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * unit;
-        if (!both(ok && !(now > base + FAR || (base == -INFINITY && now > base)))) {          // another unit: what there is so far goes by it
-          maxima[half * TILE_M] = now;
-          ok = both(ok);
-          if (!ok) break;
-          now = fmaxf(now, maxima[(half ^ 1) * TILE_M]);
-          const bool higher = now > base + FAR || (base == -INFINITY && now > base);
+        const float now = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * unit;
+        const bool higher = now > base + FAR || (base == -INFINITY && now > base);
+        if (__any_sync(0xffffffffu, higher)) {           // another unit: what there is so far goes by it
           const float keep = !higher ? 1.f : base == -INFINITY ? 0.f : exp2_fast(base - now);
           total *= keep;
           if (higher) base = now;
           if (k > 0) {
-            ok = both(bar_wait(&freed[(j - 1) % BUFFERS], ((j - 1) / BUFFERS) & 1, ab));
+            ok = __all_sync(0xffffffffu, bar_wait(&freed[(j - 1) % BUFFERS], ((j - 1) / BUFFERS) & 1, ab));
             if (!ok) break;
             tc_fence_after();
 #pragma unroll
-            for (int h = 0; h < WIDE; h += 32) {
-              if (first_value + h >= wide) break;
+            for (int h = 0; h < DP; h += 32) {
+              if (h >= wide) break;
               float v[32];
-              tmem_ld32(sum_at + first_value + h, v);
+              tmem_ld32(sum_at + h, v);
 #pragma unroll
               for (int c = 0; c < 32; ++c) v[c] *= keep;
-              tmem_st32(sum_at + first_value + h, v);
+              tmem_st32(sum_at + h, v);
             }
           }
         }
@@ -609,13 +612,12 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
         const Two units(unit, unit), minuses(minus, minus);
         Two add[2] = {Two(0.f, 0.f), Two(0.f, 0.f)};
 #pragma unroll
-        for (int h = CHUNKS - 1; h >= 0; --h) {          // the last is there already
-          if (h < CHUNKS - 1) read(32 * h);
+        for (int h = 0; h < CHUNKS; ++h) {
           uint32_t out[16];
 #pragma unroll
           for (int c = 0; c < 32; c += 2) {
             float x, y;
-            fma2(two_of(&raw[c]), units, minuses).apart(x, y);
+            fma2(two_of(&raw[h][c]), units, minuses).apart(x, y);
             out[c >> 1] = two_bf16(exp2_fast(x), exp2_fast(y));
             add[(c >> 1) & 1] = add2(add[(c >> 1) & 1], bf16_values(out[c >> 1]));     // the sum is that of the rounded weights
           }
@@ -629,12 +631,11 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
         __syncwarp();
         if (lane == 0) bar_arrive(&weights[b]);
       }
-      totals[half * TILE_M] = total;
       if (sums_there()) {
-        const float inverse = 1.f / (totals[0] + totals[TILE_M]);
+        const float inverse = 1.f / total;
         const bool finite = put_row<WIDE>(sum_at, first_value, inverse, on, w.q.out, row, mine, w.q, lane, nullptr, w.rest);
         sums_read(on && !finite);
-        if (on && w.q.top && half == 0) w.q.top[(int64_t)mine * w.q.n + row] = base, w.q.inverse[(int64_t)mine * w.q.n + row] = inverse;
+        if (on && w.q.top) w.q.top[(int64_t)mine * w.q.n + row] = base, w.q.inverse[(int64_t)mine * w.q.n + row] = inverse;
       }
     } else if (MODE == ROWS) {
       const int64_t at_row = (int64_t)mine * w.q.n + row;
@@ -854,11 +855,11 @@ template <int DP, int MODE> int launch(const TcParams& p, cudaStream_t s) {
     const int kv_heads = p.w.kv.heads, high = TILE_M / p.pack;
     int rc;
     if (MODE == COLUMNS) {
-      (void)((rc = map(&t.own[0], q.k, kv_heads, TILE_M)) || (rc = map(&t.own[1], q.v, kv_heads, TILE_M)) || (rc = map(&t.ring[0], q.q, q.heads, F::KEYS)) ||
-             (rc = map(&t.ring[1], q.g, q.heads, F::KEYS)));
+      (void)((rc = map(&t.own[0], q.k, kv_heads, TILE_M)) || (rc = map(&t.own[1], q.v, kv_heads, TILE_M)) || (rc = map(&t.ring[0], q.q, q.heads, KEYS)) ||
+             (rc = map(&t.ring[1], q.g, q.heads, KEYS)));
     } else {
       (void)((rc = map(&t.own[0], q.q, q.heads, high)) || (MODE == ROWS && (rc = map(&t.own[1], q.g, q.heads, high))) ||
-             (rc = map(&t.ring[MODE == ROWS], q.k, kv_heads, F::KEYS)) || (rc = map(&t.ring[MODE == FORWARD], q.v, kv_heads, F::KEYS)) ||
+             (rc = map(&t.ring[MODE == ROWS], q.k, kv_heads, KEYS)) || (rc = map(&t.ring[MODE == FORWARD], q.v, kv_heads, KEYS)) ||
              (rc = map(&t.eight[MODE == ROWS], q.k, kv_heads, 8)) || (rc = map(&t.eight[MODE == FORWARD], q.v, kv_heads, 8)));
     }
     if (rc) return rc;
