@@ -3,7 +3,7 @@
 // Node i of a chain [lo, hi) sees the nodes j of it with  j <= i + after  and  (j >= i - before  or  j < lo + sinks):
 //
 //     s_ij = scale <q_i, k_j>      P_ij = exp(s_ij) / sum_j exp(s_ij)      out_i = sum_j P_ij v_j
-//     dP_ij = <g_i, v_j>           delta_i = <g_i, out_i>                  dS_ij = P_ij (dP_ij - delta_i)
+//     dP_ij = <g_i, v_j>           delta_i = sum_j P_ij dP_ij              dS_ij = P_ij (dP_ij - delta_i)
 //     dv_j = sum_i P_ij g_i        dq_i = scale sum_j dS_ij k_j            dk_j = scale sum_i dS_ij q_i
 //
 // over the heads that share k and v, for dk and dv.

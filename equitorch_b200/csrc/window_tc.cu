@@ -17,10 +17,15 @@
 //
 // Two CTAs an SM hide each other's chain of copy, product, softmax and product.  By columns two or three groups of softmax warps take turns in one CTA, which
 // has all the tensor memory (64 values a head: 247 -> 217 us for 240 chains of 50 to 500 nodes against two CTAs of one group; by rows, where one thread has
-// half the products to issue, that lost: 189 -> 325).  Warps 0 to 3 (7, 11): softmax; then two that issue MMAs and two that copy.
+// half the products to issue, that lost: 189 -> 325).  By rows, with one buffer of scores, two warps share a row's 64 others (64 values 196 -> 172 us, 128 values
+// 430 -> 406); forward and by columns that lost (128 values 240 -> 266 us, 408 -> 441), for want of registers and of room for the instructions.
+// The first 4 (8, 12) warps: softmax; then two that issue MMAs and two that copy.
 //
-// Bound by the special functions at 64 values a head (a score is 4 x 64 flops, 0.16 ps of the tensor cores, and one exponential, 0.22 ps) and by the
-// tensor cores at 128.  Every wait is bounded; on expiry the status flag is raised and the kernel ends.
+// Two bounds: the special functions (a score is one exponential, 0.22 ps of the GPU; of 4 x 64 flops, 0.16 ps of the tensor cores), and the tensor cores, whose MMA
+// of 128 x 64 takes as long as one of 128 x 128: S and dP run at half the rate.  128 keys at a time have the full rate, and lost forward (240 -> 267 us), where tensor
+// memory then has one buffer of scores.  One chain of 32,781 nodes, 8 heads of 128, window of 1024 and 4 first nodes: forward 240 us, by rows 395, by columns
+// 393, tensor pipe 33 to 37 % busy; a step of 64 takes a CTA 2200 cycles, 1400 of them softmax, the rest the way to the MMAs and back.
+// Every wait is bounded; on expiry the status flag is raised and the kernel ends.
 #include <algorithm>
 
 #include "tc_bf16.cuh"
@@ -336,9 +341,9 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
   if (warp >= F::SOFT + 2) {
     // ---------------- copies ----------------
     // Items in the order of their use: FORWARD k, v; ROWS v, k; COLUMNS q with its numbers, g.  Heads of 64 or 128 values in one component are
-    // copied by one thread (TMA); a stretch's first nodes, and all of other heads, by the threads: their copies arrive at the item's barrier when they have landed, and
+    // copied by TMA, eight rows a lane where a stretch's first nodes are among them; other heads by the threads: their copies arrive at the item's barrier when they have landed, and
     // the thread that issues the MMAs, which sees them all there, puts the fence between them and the tensor cores.  Copying by hand takes the warps
-    // issue slots that the softmax wants (one chain of 32,781 nodes, 8 heads of 128 values, by hand and by TMA: HAND | TMA us).
+    // issue slots that the softmax wants (one chain of 32,781 nodes, 8 heads of 128 values, by hand and by TMA: 1270 | 1197 us of kernels).
     const int thread = tid - 32 * (F::SOFT + 2), threads = p.tma ? 32 : LOADERS;
     const Copier<DP> even(MODE == FORWARD ? w.q.k : MODE == ROWS ? w.q.v : w.q.q, w.q, thread, threads);
     const Copier<DP> odd(MODE == FORWARD ? w.q.v : MODE == ROWS ? w.q.k : w.q.g, w.q, thread, threads);

@@ -34,7 +34,7 @@ def type_cross_entropy(x: Tensor, weight: Tensor, target: Tensor, reduction: str
     no gradient, and what their features hold reaches nothing.  A target that the table does not have gives NaN.  ``reduction``: ``mean`` over the rows
     that count (zero if none does), ``sum`` or ``none``; the loss is float32.
 
-    float32 or bfloat16 features and table of one type.  The logits are formed in tiles and never kept, once forward and once backward, where
+    float32 or bfloat16 features and table of one type, at most 16384 channels.  The logits are formed in tiles and never kept, once forward and once backward, where
     their gradients are in scratch for at most 256 MB of types at a time.  Sums in float32, no atomics; of bfloat16 the logits' gradients are rounded
     to bfloat16 for their products.  Differentiable once, in ``x`` and ``weight``."""
     _ops.check(x, weight, target, reduction)

@@ -286,3 +286,16 @@ def test_step_in_a_graph_while_lengths_grow():
         graph.replay()
         assert torch.equal(held, F.window_attention_step(q, keys, values, lengths, 2, 300, 2))
         lengths += 1
+
+
+@pytest.mark.parametrize("size", [32, 64, 128])
+@pytest.mark.parametrize("window", [(1, 0, 0), (2, 1, 1), (30, 30, 4)])
+def test_errors_of_few_and_many_nodes_as_a_whole(window, size):
+    """bfloat16.  Rounding a result leaves 1.66e-3 of its 2-norm, rounding the weights (or score gradients) of a product as much of its result, so two of
+    these are the most: a delta of other weights than the rows' own would be a third where few nodes are seen, and cancel."""
+    sizes = (150, 3, 90, 257)
+    qkv, g, graphs = make(sizes, 1, 4, 2, size, torch.bfloat16, seed=size)
+    want, _ = reference(*qkv, g, seen(sizes, sum(sizes), *window), 4, 2, None)
+    for what, a, b in zip(("out", "dq", "dk", "dv"), run(qkv, g, graphs, 4, *window, kv_heads=2), want):
+        error = ((a.double() - b).norm() / b.norm()).item()
+        assert error < 2 * 1.66e-3, f"{what}: {error:.2e}"

@@ -145,3 +145,12 @@ def test_library_checks_its_arguments():
     for bad, code in ((dict(dtype=1), 1), (dict(reduction=3), 1), (dict(c=0), 1), (dict(t=0), 1), (dict(x=None), 1), (dict(c=20_000), 2), (dict(scratch=16), 1)):
         assert lib.eqt_type_loss_forward(C.byref(_lib.TypeLossArgs(**{**loss, **bad})), None) == code
     assert lib.eqt_type_loss_backward(C.byref(_lib.TypeLossArgs(**loss)), None) == 1
+
+
+def test_bfloat16_windows_keep_what_rounding_left():
+    """Where the backward pass is to follow: its deltas go by it."""
+    lib = _lib.lib()
+    window = dict(dtype=_lib.DTYPE_CODE[torch.bfloat16], comps=1, heads=2, kv_heads=1, head_channels=8, tile_rows=16, scale=1.0, n=4, num_graphs=1, longest=4, num_tiles=1,
+                  q=16, k=16, v=16, out=16, stats=16, tiles=16, ptr=16, grad=16, dq=16, dk=16, dv=16)
+    assert lib.eqt_window_attention_forward(C.byref(_lib.WindowAttentionArgs(**window)), None) == 1
+    assert lib.eqt_window_attention_backward(C.byref(_lib.WindowAttentionArgs(**window)), None) == 1
