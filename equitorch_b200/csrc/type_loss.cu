@@ -4,11 +4,14 @@
 //     backward, with r_i the row's share of the result (zero where the target is negative):
 //         G_it = r_i (exp(z_it - lse_i) - [t = target_i])        dx = G w        dw = G^T x
 //
+// A share that all rows have (a sum's, a mean's) is left out of G and multiplied to the sums: early in training G is -r_i at the target and little elsewhere, and
+// the rounding of one r would be every row's (1000 rows, 2-norm of dx's error 3.3e-3 | 2.3e-3, of a result's rounding 1.7e-3).
+//
 // One kernel of warp roles on the 5th-generation tensor cores makes all four products:
 //
 //   LOGITS   z, tile by tile; a thread of the epilogue has a row's 64 logits of a tile in registers and carries their maximum and sum of
 //            exponentials over a run of tiles, which is all that leaves the SM (8 bytes for 64 to 2048 logits)
-//   SCORES   z again for a piece of the types, and from it G, rounded to bfloat16 (float32: to three parts of it), to scratch
+//   SCORES   z again for a piece of the types, and from it G, rounded to bfloat16 (of few types to two, float32 to three parts of it), to scratch
 //   INPUT    dx += G w of the piece         WEIGHT   dw = G^T x of the piece
 //
 // G of a piece is at most PIECE_BYTES, so scratch does not grow with the table; a piece has a whole number of waves of WEIGHT's tiles.  Sums that
@@ -54,6 +57,7 @@ struct alignas(64) Launch {
   CUtensorMap a, b;
   int64_t rows;                                          // of the results
   int columns, width;                                    // of the results, of a tile
+  int planes, plane_blocks;                              // of G, bfloat16: what rounding its first leaves is in the second; k-blocks of each
   int row_tiles, col_tiles, run, kblocks, part_blocks, fold;       // run: LOGITS, column tiles of an item
   unsigned items;
   int a_first, b_first;                                  // SCORES: the piece's first type; INPUT: of w's rows
@@ -132,7 +136,8 @@ template <typename T> __device__ __forceinline__ void store_block(unsigned char*
   }
 }
 
-template <int PARTS, int MODE> __global__ void __launch_bounds__(threads<PARTS>(), 1) loss_kernel(const __grid_constant__ Launch p) {
+// PLANES: parts of G that SCORES makes of bfloat16
+template <int PARTS, int MODE, int PLANES> __global__ void __launch_bounds__(threads<PARTS>(), 1) loss_kernel(const __grid_constant__ Launch p) {
   constexpr bool F32 = PARTS == 3, A_TURNED = MODE == WEIGHT, B_TURNED = MODE == INPUT || MODE == WEIGHT;
   constexpr int STAGES = stages<PARTS>(), STAGE = stage_bytes<PARTS>(), COLS = cols<PARTS>();
   static_assert(STAGES >= 2, "two stages at least");
@@ -177,21 +182,22 @@ template <int PARTS, int MODE> __global__ void __launch_bounds__(threads<PARTS>(
           const int col = tile * p.width;
           for (int kb = t.kb0; kb < t.kb1; ++kb) {
             if (!bar_wait(&empty[s], ph, ab)) { ok = false; break; }
+            const int plane = (MODE == INPUT || MODE == WEIGHT) && kb >= p.plane_blocks, k = (kb - plane * p.plane_blocks) * BK;
             unsigned char* at = ring + (size_t)s * STAGE;
             bar_expect_tx(&full[s], bytes);
 #pragma unroll
             for (int q = 0; q < PARTS; ++q) {
               unsigned char *sa = at + q * TILE_M * BK * 2, *sb = at + a_bytes<PARTS>() + q * COLS * BK * 2;
               if (A_TURNED) {
-                tma_load_3d(sa, &p.a, (int)t.row, kb * BK, q, &full[s]);
-                tma_load_3d(sa + 8192, &p.a, (int)t.row + 64, kb * BK, q, &full[s]);
+                tma_load_3d(sa, &p.a, (int)t.row, k, q + plane, &full[s]);
+                tma_load_3d(sa + 8192, &p.a, (int)t.row + 64, k, q + plane, &full[s]);
               } else {
-                tma_load_3d(sa, &p.a, kb * BK, (int)t.row, q, &full[s]);
+                tma_load_3d(sa, &p.a, k, (int)t.row, q + plane, &full[s]);
               }
               if (B_TURNED) {
-                for (int c = 0; c < p.width / 64; ++c) tma_load_3d(sb + c * 8192, &p.b, col + c * 64, p.b_first + kb * BK, q, &full[s]);
+                for (int c = 0; c < p.width / 64; ++c) tma_load_3d(sb + c * 8192, &p.b, col + c * 64, p.b_first + k, q, &full[s]);
               } else {
-                tma_load_3d(sb, &p.b, kb * BK, p.b_first + col, q, &full[s]);
+                tma_load_3d(sb, &p.b, k, p.b_first + col, q, &full[s]);
               }
             }
             if (++s == STAGES) s = 0, ph ^= 1;
@@ -265,9 +271,11 @@ template <int PARTS, int MODE> __global__ void __launch_bounds__(threads<PARTS>(
       if (MODE != WEIGHT && there) target = p.target[row];
       if (MODE == SCORES && target >= 0) {
         lse = p.lse[row];
-        part = p.reduction == 0 ? p.grad[row] : p.reduction == 1 ? p.grad[0] : p.grad[0] / p.count[0];
+        part = p.reduction == 0 ? p.grad[row] : 1.f;
         if (target >= p.types) part = NAN;
       }
+      float factor = 1.f;
+      if (MODE == INPUT || MODE == WEIGHT) factor = p.reduction == 0 ? 1.f : p.reduction == 1 ? p.grad[0] : p.count[0] > 0.f ? p.grad[0] / p.count[0] : 0.f;
       // 32 columns from `col` on, of which `valid` exist
       auto block = [&](float* v, int col, int valid) {
         if constexpr (MODE == LOGITS) {
@@ -305,14 +313,16 @@ template <int PARTS, int MODE> __global__ void __launch_bounds__(threads<PARTS>(
           }
           __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.out) + row0 * p.out_pitch + col;
 #pragma unroll
-          for (int q = 0; q < PARTS; ++q) {
+          for (int q = 0; q < PARTS * PLANES; ++q) {
             store_block<__nv_bfloat16>(patch, v, out + q * p.out_part, p.out_pitch, lines, valid, true, lane);
-            if constexpr (F32) {
+            if constexpr (PARTS * PLANES > 1) {
 #pragma unroll
               for (int c = 0; c < 32; ++c) v[c] -= __bfloat162float(__float2bfloat16_rn(v[c]));
             }
           }
         } else {
+#pragma unroll
+          for (int c = 0; c < 32; ++c) v[c] *= factor;
           if (MODE == INPUT && p.typed && target < 0) {
 #pragma unroll
             for (int c = 0; c < 32; ++c) v[c] = 0.f;
@@ -542,7 +552,7 @@ struct Plan {
   int parts, pitch, cols;                                // of the operands: bfloat16 parts, values a row; columns a tile
   int64_t piece, pieces, g_pitch;
   int width_t, width_c, run, runs;
-  int input_parts, input_blocks, weight_parts, weight_blocks;
+  int planes, input_parts, input_blocks, weight_parts, weight_blocks;
   size_t x, w, states, logit, g, dx, dw, bytes;          // places in the scratch
 };
 int width_of(int64_t columns, int most) {
@@ -555,6 +565,9 @@ void cut(int64_t blocks, int64_t tiles, int& parts, int& part_blocks) {
   part_blocks = (int)std::min<int64_t>(MOST_TERMS / BK, std::max<int64_t>(std::min<int64_t>(blocks, 8), ceil_div(blocks, wanted)));
   parts = (int)ceil_div(blocks, part_blocks);
 }
+// bfloat16 G of few types goes into its products in two parts: a row's few numbers are often of one size, whose rounding does not average out (1000 rows, 2 to
+// 10 types: 2-norm of dx's error 2.15e-3 in one part, 1.65e-3 in two, that of a result's rounding); up to 64 types are one k-block, so it costs a few microseconds.
+int planes_of(const eqt_type_loss_args& a) { return a.dtype == EQT_BF16 && a.t <= BK ? 2 : 1; }
 Plan plan_of(const eqt_type_loss_args& a, bool backward) {
   Plan p{};
   const int64_t sms = sm_count(), row_tiles = ceil_div(a.n, TILE_M);
@@ -578,14 +591,15 @@ Plan plan_of(const eqt_type_loss_args& a, bool backward) {
   }
   // a piece: whole waves of WEIGHT's tiles, as many as the scratch for G takes
   const int64_t col_tiles = ceil_div(a.c, p.width_c), wave = std::max<int64_t>(1, sms / col_tiles) * TILE_M;
+  p.planes = planes_of(a);
   const int64_t most = std::max<int64_t>(TILE_M, PIECE_BYTES / (2 * p.parts) / up_to(a.n, TILE_M) / TILE_M * TILE_M);
   p.piece = std::min<int64_t>(up_to(a.t, TILE_M), most >= wave ? most / wave * wave : most);
   p.pieces = ceil_div(a.t, p.piece);
   p.g_pitch = p.piece;
-  cut(ceil_div(p.piece, BK), row_tiles * col_tiles, p.input_parts, p.input_blocks);
-  cut(ceil_div(a.n, BK), ceil_div(p.piece, TILE_M) * col_tiles, p.weight_parts, p.weight_blocks);
+  cut(p.planes * ceil_div(p.piece, BK), row_tiles * col_tiles, p.input_parts, p.input_blocks);
+  cut(p.planes * ceil_div(a.n, BK), ceil_div(p.piece, TILE_M) * col_tiles, p.weight_parts, p.weight_blocks);
   p.g = at;
-  p.dx = p.g + up((size_t)a.n * p.g_pitch * 2 * p.parts);
+  p.dx = p.g + up((size_t)a.n * p.g_pitch * 2 * p.parts * p.planes);
   p.dw = p.dx + (p.input_parts * p.pieces > 1 ? up((size_t)p.input_parts * p.pieces * a.n * p.pitch * 4) : 0);
   p.bytes = p.dw + (p.weight_parts > 1 ? up((size_t)p.weight_parts * p.piece * p.pitch * 4) : 0);
   return p;
@@ -601,14 +615,18 @@ int check(const eqt_type_loss_args* a) {
   return EQT_OK;
 }
 
-template <int PARTS, int MODE> int launch(const Launch& p, cudaStream_t s) {
-  auto kernel = loss_kernel<PARTS, MODE>;
+template <int PARTS, int MODE, int PLANES = 1> int launch(const Launch& p, cudaStream_t s) {
+  auto kernel = loss_kernel<PARTS, MODE, PLANES>;
   static std::atomic<uint64_t> allowed{0};
   if (int rc = allow_shared_once(kernel, shared_bytes<PARTS>(), allowed)) return rc;
   kernel<<<std::min<unsigned>(p.items, (unsigned)sm_count()), threads<PARTS>(), shared_bytes<PARTS>(), s>>>(p);
   return check_launch("type_loss");
 }
-template <int MODE> int launch(int parts, const Launch& p, cudaStream_t s) { return parts == 1 ? launch<1, MODE>(p, s) : launch<3, MODE>(p, s); }
+template <int MODE> int launch(int parts, const Launch& p, cudaStream_t s) {
+  if constexpr (MODE == SCORES)
+    if (parts == 1 && p.planes == 2) return launch<1, MODE, 2>(p, s);
+  return parts == 1 ? launch<1, MODE>(p, s) : launch<3, MODE>(p, s);
+}
 
 int sum_parts(int dtype, const float* parts, void* out, int64_t rows, int cols, int pitch, int slots, const int64_t* target, cudaStream_t s) {
   const unsigned grid = flat_grid(rows * (pitch / 8), 256);
@@ -712,27 +730,29 @@ extern "C" int eqt_type_loss_backward(const eqt_type_loss_args* args, void* stre
     if (int rc = tc::map_bf16(&l.b, w, a.t, p.pitch, p.pitch, a.t * p.pitch, p.parts, p.width_t)) return rc;
     l.rows = a.n, l.columns = (int)here, l.width = p.width_t, l.row_tiles = (int)ceil_div(a.n, tc::TILE_M), l.col_tiles = (int)ceil_div(here, p.width_t);
     l.run = 1, l.kblocks = (int)ceil_div(a.c, BK), l.fold = fold_of(p.parts), l.items = (unsigned)(l.row_tiles * l.col_tiles);
-    l.a_first = l.b_first = (int)t0, l.out = base + p.g, l.out_pitch = p.g_pitch, l.out_part = a.n * p.g_pitch;
+    l.planes = p.planes, l.a_first = l.b_first = (int)t0, l.out = base + p.g, l.out_pitch = p.g_pitch, l.out_part = a.n * p.g_pitch;
     l.target = a.target, l.types = a.t, l.lse = a.lse, l.grad = a.grad, l.count = a.count, l.reduction = a.reduction, l.status = a.status;
     if (int rc = launch<SCORES>(p.parts, l, s)) return rc;
     if (a.dx) {
       Launch d{};
-      if (int rc = tc::map_bf16(&d.a, base + p.g, a.n, here, p.g_pitch, a.n * p.g_pitch, p.parts, tc::TILE_M)) return rc;
+      if (int rc = tc::map_bf16(&d.a, base + p.g, a.n, here, p.g_pitch, a.n * p.g_pitch, p.parts * p.planes, tc::TILE_M)) return rc;
       if (int rc = tc::map_bf16(&d.b, w, a.t, p.pitch, p.pitch, a.t * p.pitch, p.parts, BK)) return rc;
       d.rows = a.n, d.columns = (int)a.c, d.width = p.width_c, d.row_tiles = l.row_tiles, d.col_tiles = (int)ceil_div(a.c, p.width_c);
-      d.kblocks = (int)ceil_div(p.piece, BK), d.part_blocks = p.input_blocks, d.fold = l.fold, d.items = (unsigned)(d.row_tiles * d.col_tiles * p.input_parts);
+      d.plane_blocks = (int)ceil_div(p.piece, BK), d.kblocks = p.planes * d.plane_blocks, d.part_blocks = p.input_blocks, d.fold = l.fold, d.items = (unsigned)(d.row_tiles * d.col_tiles * p.input_parts);
       d.b_first = (int)t0, d.typed = dx_slots == 1, d.target = a.target, d.types = a.t, d.status = a.status;
+      d.grad = a.grad, d.count = a.count, d.reduction = a.reduction;
       d.out = d.typed ? a.dx : dx_parts, d.out_pitch = d.typed ? a.c : p.pitch, d.out_part = a.n * p.pitch, d.slot = (int)(i * p.input_parts);
       d.whole = !d.typed || a.c * size % 16 == 0;
       if (int rc = launch<INPUT>(p.parts, d, s)) return rc;
     }
     if (a.dw) {
       Launch d{};
-      if (int rc = tc::map_bf16(&d.a, base + p.g, a.n, here, p.g_pitch, a.n * p.g_pitch, p.parts, BK)) return rc;
+      if (int rc = tc::map_bf16(&d.a, base + p.g, a.n, here, p.g_pitch, a.n * p.g_pitch, p.parts * p.planes, BK)) return rc;
       if (int rc = tc::map_bf16(&d.b, x, a.n, p.pitch, p.pitch, a.n * p.pitch, p.parts, BK)) return rc;
       d.rows = here, d.columns = (int)a.c, d.width = p.width_c, d.row_tiles = (int)ceil_div(here, tc::TILE_M), d.col_tiles = (int)ceil_div(a.c, p.width_c);
-      d.kblocks = (int)ceil_div(a.n, BK), d.part_blocks = p.weight_blocks, d.fold = l.fold, d.items = (unsigned)(d.row_tiles * d.col_tiles * p.weight_parts);
+      d.plane_blocks = (int)ceil_div(a.n, BK), d.kblocks = p.planes * d.plane_blocks, d.part_blocks = p.weight_blocks, d.fold = l.fold, d.items = (unsigned)(d.row_tiles * d.col_tiles * p.weight_parts);
       d.typed = p.weight_parts == 1, d.status = a.status;
+      d.grad = a.grad, d.count = a.count, d.reduction = a.reduction;
       void* to = static_cast<unsigned char*>(a.dw) + (size_t)t0 * a.c * size;
       d.out = d.typed ? to : dw_parts, d.out_pitch = d.typed ? a.c : p.pitch, d.out_part = here * p.pitch;
       d.whole = !d.typed || a.c * size % 16 == 0;
