@@ -13,7 +13,7 @@
 // The forward pass keeps its unit of the exponentials until a row's greatest score is over 2^8 of it, and only then rescales the sums in tensor memory;
 // the sum and the result have the same unit, so that loses nothing.  The scores of the next 64 keys are made while the softmax works on these.
 // dS goes into dq's product in two parts, as within whole graphs: dq has the error of rounded weights already.  2-norm of the errors 2.3e-3 to 2.4e-3, a rounding of the result
-// alone 1.7e-3; with a delta of rounded results and weights not rounded, dq's was 3.4e-3 where windows are of few nodes, and dk's 2.7e-3.
+// alone 1.7e-3 (dk and dv have that where there are few tiles, see `launch`); with a delta of rounded results and weights not rounded, dq's was 3.4e-3 where windows are of few nodes, and dk's 2.7e-3.
 //
 // Two CTAs an SM hide each other's chain of copy, product, softmax and product.  By columns two or three groups of softmax warps take turns in one CTA, which
 // has all the tensor memory (64 values a head: 247 -> 217 us for 240 chains of 50 to 500 nodes against two CTAs of one group; by rows, where one thread has
@@ -275,7 +275,8 @@ template <int WIDE> __device__ __forceinline__ bool put_row(uint32_t sum, int fi
   return x + y == 0.f;
 }
 
-template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::THREADS, Form<DP, MODE>::CTAS) window_tc_kernel(const __grid_constant__ TcParams p) {
+// FINE, by columns: weights and score gradients go into their products in two parts
+template <int DP, int MODE, bool FINE> __global__ void __launch_bounds__(Form<DP, MODE>::THREADS, Form<DP, MODE>::CTAS) window_tc_kernel(const __grid_constant__ TcParams p) {
   using F = Form<DP, MODE>;
   constexpr int SLOTS = F::SLOTS, GROUPS = F::GROUPS, BUFFERS = F::BUFFERS;
   extern __shared__ __align__(1024) unsigned char smem[];
@@ -493,9 +494,10 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
           if (!ok) break;
           tc_fence_after();
           add(sum, d, slot_at(2 * j + 1), more);
-          if (MODE == ROWS) add(sum, d + 16, slot_at(2 * j + 1), true);
+          if (MODE == ROWS || FINE) add(sum, d + 16, slot_at(2 * j + 1), true);
           if (MODE == COLUMNS) {
             add(sum + DP, d + KEYS, slot_at(2 * j), more);
+            if (FINE) add(sum + DP, d + KEYS + 16, slot_at(2 * j), true);
             umma_commit(&empty[2 * j % SLOTS]);
           }
           umma_commit(&empty[(2 * j + 1) % SLOTS]);
@@ -721,7 +723,7 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
         for (int h = half * CHUNKS; h < (half + 1) * CHUNKS; ++h) {
           const uint32_t word = seen(from + 32 * h);
           const bool all = __all_sync(0xffffffffu, word == ~0u);
-          uint32_t s[32], d[32], pt[16], dst[16];
+          uint32_t s[32], d[32], pt[2][16], dst[2][16];  // large and small parts
           tmem_issue32(s_at + 32 * h, s);
           tmem_issue32(s_at + KEYS + 32 * h, d);
           tmem_arrived32(s);
@@ -748,13 +750,25 @@ template <int DP, int MODE> __global__ void __launch_bounds__(Form<DP, MODE>::TH
                 y[i] = see ? y[i] : 0.f;
               }
             }
-            pt[c / 2] = two_bf16(x[0], x[1]);
-            pt[c / 2 + 1] = two_bf16(x[2], x[3]);
-            dst[c / 2] = two_bf16(y[0], y[1]);
-            dst[c / 2 + 1] = two_bf16(y[2], y[3]);
+            auto parts = [&](uint32_t(&to)[2][16], int at, float a, float b) {
+              to[0][at] = two_bf16(a, b);
+              if (FINE) {
+                float a1, b1;
+                fma2(bf16_values(to[0][at]), less, Two(a, b)).apart(a1, b1);
+                to[1][at] = two_bf16(a1, b1);
+              }
+            };
+#pragma unroll
+            for (int i = 0; i < 4; i += 2) {
+              parts(pt, (c + i) / 2, x[i], x[i + 1]);
+              parts(dst, (c + i) / 2, y[i], y[i + 1]);
+            }
           }
-          tmem_put16(s_at + 32 * h, pt);
-          tmem_put16(s_at + KEYS + 32 * h, dst);
+#pragma unroll
+          for (int part = 0; part < (FINE ? 2 : 1); ++part) {
+            tmem_put16(s_at + 32 * h + 16 * part, pt[part]);
+            tmem_put16(s_at + KEYS + 32 * h + 16 * part, dst[part]);
+          }
         }
         tmem_stored();
         tc_fence_before();
@@ -869,9 +883,15 @@ template <int DP, int MODE> int launch(const TcParams& p, cudaStream_t s) {
     }
     if (rc) return rc;
   }
-  auto kernel = window_tc_kernel<DP, MODE>;
-  static std::atomic<uint64_t> allowed{0};
-  if (int rc = allow_shared_once(kernel, F::bytes(), allowed)) return rc;
+  // In two parts, dk and dv have no rounding but their own, and a step by columns a fifth more to do.  Where there are no more tiles than SMs, what a call takes is
+  // latency, and where few nodes share a chain their roundings do not average out (2-norm of the errors up to 2.6e-3 | 1.7e-3; one chain of 2000 nodes, 8
+  // heads of 64: 84 | 89 us of kernels; one chain of 32,781, 128 values, dS alone in two: 1131 | 1180).
+  const bool fine = MODE == COLUMNS && tiles <= sm_count();
+  auto kernel = window_tc_kernel<DP, MODE, false>;
+  if constexpr (MODE == COLUMNS)
+    if (fine) kernel = window_tc_kernel<DP, MODE, true>;
+  static std::atomic<uint64_t> allowed[2]{};
+  if (int rc = allow_shared_once(kernel, F::bytes(), allowed[fine])) return rc;
   kernel<<<(unsigned)grid, F::THREADS, F::bytes(), s>>>(t);
   return check_launch("window_tc");
 }

@@ -45,7 +45,7 @@ def window_attention(q: Tensor, k: Tensor, v: Tensor, graphs: PackedGraphs, num_
     touch each other.
 
     Differentiable once in ``q``, ``k`` and ``v``.  Sums in float32, one order of sums, no atomics; of bfloat16 features, weights and score
-    gradients are rounded to bfloat16 for the products.  Beside its inputs and result the backward pass keeps two numbers a node and head and, of
+    gradients are rounded to bfloat16 for the products (of small batches, to two parts for the gradients of keys and values).  Beside its inputs and result the backward pass keeps two numbers a node and head and, of
     bfloat16, what the result's rounding left: where a node's weight is almost one, its gradient is what two such numbers leave."""
     kv_heads = num_heads if kv_heads is None else kv_heads
     _ops.check(q, k, v, graphs, num_heads, kv_heads, (before, after, sinks), scale)
