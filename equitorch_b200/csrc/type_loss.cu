@@ -9,7 +9,7 @@
 //
 // One kernel of warp roles on the 5th-generation tensor cores makes all four products:
 //
-//   LOGITS   z, tile by tile; a thread of the epilogue has a row's 64 logits of a tile in registers and carries their maximum and sum of
+//   LOGITS   z, tile by tile; a thread of the epilogue has a row's 64 logits of a tile in registers and carries their maximum, in units of log2, and sum of
 //            exponentials over a run of tiles, which is all that leaves the SM (8 bytes for 64 to 2048 logits)
 //   SCORES   z again for a piece of the types, and from it G, rounded to bfloat16 (of few types to two, float32 to three parts of it), to scratch
 //   INPUT    dx += G w of the piece         WEIGHT   dw = G^T x of the piece
@@ -290,18 +290,19 @@ template <int PARTS, int MODE, int PLANES> __global__ void __launch_bounds__(thr
             for (int c = 0; c < 32; ++c) z = c == (int)at ? v[c] : z;
             p.target_logit[row] = z;
           }
-          float most[4] = {top, -INFINITY, -INFINITY, -INFINITY}, add[4] = {0.f, 0.f, 0.f, 0.f};
+          float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, add[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int c = 0; c < 32; ++c) most[c & 3] = fmaxf(most[c & 3], v[c]);
-          const float now = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])), base = now == -INFINITY ? 0.f : now * LOG2E;
+          // The unit of the sum is the rounded product, so a sum whose unit stays is multiplied by one: with the greatest logit as the unit it was by what the
+          // product's rounding left, every 32 columns in the same direction (greatest logit 100 of 32,768: the loss 2.7e-4 off).
+          const float now = fmaxf(top, fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * LOG2E), base = now == -INFINITY ? 0.f : now;
 #pragma unroll
           for (int c = 0; c < 32; ++c) add[c & 3] += exp2_fast(fmaf(v[c], LOG2E, -base));
-          sum = sum * exp2_fast(fmaf(top, LOG2E, -base)) + ((add[0] + add[1]) + (add[2] + add[3]));
+          sum = sum * exp2_fast(top - base) + ((add[0] + add[1]) + (add[2] + add[3]));
           top = now;
         } else if constexpr (MODE == SCORES) {
-          const float base = lse * LOG2E;
 #pragma unroll
-          for (int c = 0; c < 32; ++c) v[c] = part * (F32 ? exp2_fast((v[c] - lse) * LOG2E) : exp2_fast(fmaf(v[c], LOG2E, -base)));
+          for (int c = 0; c < 32; ++c) v[c] = part * exp2_fast(fmaf(v[c], LOG2E, -lse));
           if (__any_sync(0xffffffffu, target < 0)) {     // set, whatever the product
 #pragma unroll
             for (int c = 0; c < 32; ++c) v[c] = target < 0 ? 0.f : v[c];
@@ -462,7 +463,8 @@ template <typename T> __global__ void __launch_bounds__(256) prepare_kernel(cons
   }
 }
 
-// The rows' log sums and losses from the states of their runs: eight threads a row.
+// The rows' log sums, in units of log2, and losses from the states of their runs: eight threads a row.  The logits of all of them were multiplied by the float32
+// LOG2E, so the target's is as well, and the difference is formed where it is exact.
 __global__ void __launch_bounds__(256) rows_kernel(const float2* __restrict__ states, int count, const float* __restrict__ target_logit,
                                                    const int64_t* __restrict__ target, int64_t n, int64_t types, float* __restrict__ lse, float* __restrict__ losses) {
   __shared__ float2 shared[8][33];
@@ -471,7 +473,7 @@ __global__ void __launch_bounds__(256) rows_kernel(const float2* __restrict__ st
   float top = -INFINITY, sum = 0.f;
   auto join = [&](float2 s) {
     const float now = fmaxf(top, s.x), base = now == -INFINITY ? 0.f : now;
-    sum = sum * exp2_fast((top - base) * LOG2E) + s.y * exp2_fast((s.x - base) * LOG2E);
+    sum = sum * exp2_fast(top - base) + s.y * exp2_fast(s.x - base);
     top = now;
   };
   if (row < n)
@@ -481,10 +483,10 @@ __global__ void __launch_bounds__(256) rows_kernel(const float2* __restrict__ st
   if (warp || row >= n) return;
 #pragma unroll
   for (int w = 1; w < 8; ++w) join(shared[w][lane]);
-  const float more = logf(sum);
-  lse[row] = top + more;
+  const double more = log2((double)sum);
+  lse[row] = (float)((double)top + more);
   const int64_t t = target[row];
-  losses[row] = t < 0 ? 0.f : t >= types ? NAN : (top - target_logit[row]) + more;
+  losses[row] = t < 0 ? 0.f : t >= types ? NAN : (float)((((double)top - (double)target_logit[row] * (double)LOG2E) + more) * 0.693147180559945309);
 }
 __global__ void __launch_bounds__(1024) reduce_kernel(const float* __restrict__ losses, const int64_t* __restrict__ target, int64_t n, int mean, float* result,
                                                       float* count) {

@@ -47,7 +47,7 @@ def _scratch(args: _lib.TypeLossArgs, backward: bool, dev: torch.device) -> Opti
 
 
 def loss_forward(x: Tensor, weight: Tensor, target: Tensor, reduction: str) -> Tuple[Tensor, Tensor, Tensor]:
-    """The loss (of every row, or one number), the rows' log sums and how many rows count; all float32."""
+    """The loss (of every row, or one number), the rows' log sums (in units of log2) and how many rows count; all float32."""
     dev = x.device
     x, weight, target = _aligned(x), _aligned(weight), target.contiguous()
     losses = torch.empty(target.shape, dtype=torch.float32, device=dev)
