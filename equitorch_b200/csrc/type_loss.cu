@@ -14,8 +14,9 @@
 //   SCORES   z again for a piece of the types, and from it G, rounded to bfloat16 (of few types to two, float32 to three parts of it), to scratch
 //   INPUT    dx += G w of the piece         WEIGHT   dw = G^T x of the piece
 //
-// G of a piece is at most PIECE_BYTES, so scratch does not grow with the table; a piece has a whole number of waves of WEIGHT's tiles.  Sums that
-// would leave SMs idle are cut into parts, float32 partial results that one kernel adds in their order.  Floor: 8 n t c flops for both passes.
+// G of a piece is at most PIECE_BYTES (or, of over a million rows, of 128 types), and pieces add to one float32 dx, which the last one rounds, so scratch does not grow with the
+// table; a piece that has a wave of WEIGHT's tiles has whole ones.  Sums that would leave SMs idle are cut into parts, float32 partial results that one kernel adds
+// in their order.  Floor: 8 n t c flops for both passes.
 // At most MOST_TERMS channels.  Bound by the tensor cores: 16,384 rows, 32,768 types, 512 bfloat16 channels 565 us of LOGITS (0.97 PFLOP/s, the exponentials
 // at the same time), four pieces of 132, 123 and 119 (1.04 to 1.15 PFLOP/s); pairs of CTAs for a tile of 256 x 256 took 532, 151, 114 and 122 (2100 | 2130 us in
 // all).  float32 5003 x 14,161 x 128: LOGITS 96, then 86, 71 and 56 twice, bound by the shared memory that six products of split operands read.
@@ -64,7 +65,9 @@ struct alignas(64) Launch {
   // LOGITS: states [run and share][row]; SCORES: g (parts, rows, pitch); INPUT, WEIGHT: results, or partial ones [slot][row][pitch]
   void* out;
   int64_t out_pitch, out_part;
-  int slot, whole, typed;                                // typed: results of the tensors' type, else float32 partial ones
+  int whole, typed;                                      // typed: results of the tensors' type, else float32 partial ones
+  const float* before;                                   // INPUT: the sums of the pieces before this one, NULL for the first
+  int64_t before_pitch, before_part;
   const int64_t* target;
   int64_t types;
   float* target_logit;
@@ -324,12 +327,21 @@ template <int PARTS, int MODE, int PLANES> __global__ void __launch_bounds__(thr
         } else {
 #pragma unroll
           for (int c = 0; c < 32; ++c) v[c] *= factor;
+          if (MODE == INPUT && p.before && there) {      // the place may be the one that is written: store_block has a warp's barrier before it
+            const float* from = p.before + t.part * p.before_part + row * p.before_pitch + col;
+#pragma unroll
+            for (int c = 0; c < 32; c += 4)
+              if (col + c < p.before_pitch) {
+                const float4 a = *reinterpret_cast<const float4*>(from + c);
+                v[c] += a.x, v[c + 1] += a.y, v[c + 2] += a.z, v[c + 3] += a.w;
+              }
+          }
           if (MODE == INPUT && p.typed && target < 0) {
 #pragma unroll
             for (int c = 0; c < 32; ++c) v[c] = 0.f;
           }
           if (F32 || !p.typed) {
-            float* out = static_cast<float*>(p.out) + (p.typed ? 0 : (p.slot + t.part) * p.out_part) + row0 * p.out_pitch + col;
+            float* out = static_cast<float*>(p.out) + (p.typed ? 0 : t.part * p.out_part) + row0 * p.out_pitch + col;
             store_block<float>(patch, v, out, p.out_pitch, lines, valid, p.whole, lane);
             store_block<float>(patch, v + 16, out + 16, p.out_pitch, lines, valid - 16, p.whole, lane);
           } else {
@@ -568,7 +580,7 @@ void cut(int64_t blocks, int64_t tiles, int& parts, int& part_blocks) {
   parts = (int)ceil_div(blocks, part_blocks);
 }
 // bfloat16 G of few types goes into its products in two parts: a row's few numbers are often of one size, whose rounding does not average out (1000 rows, 2 to
-// 10 types: 2-norm of dx's error 2.15e-3 in one part, 1.65e-3 in two, that of a result's rounding); up to 64 types are one k-block, so it costs a few microseconds.
+// 10 types: 2-norm of dx's error 2.15e-3 in one part, 1.65e-3 in two, that of a result's rounding); up to 64 types are one k-block a part, so it costs a few microseconds.
 int planes_of(const eqt_type_loss_args& a) { return a.dtype == EQT_BF16 && a.t <= BK ? 2 : 1; }
 Plan plan_of(const eqt_type_loss_args& a, bool backward) {
   Plan p{};
@@ -598,12 +610,12 @@ Plan plan_of(const eqt_type_loss_args& a, bool backward) {
   p.piece = std::min<int64_t>(up_to(a.t, TILE_M), most >= wave ? most / wave * wave : most);
   p.pieces = ceil_div(a.t, p.piece);
   p.g_pitch = p.piece;
-  cut(p.planes * ceil_div(p.piece, BK), row_tiles * col_tiles, p.input_parts, p.input_blocks);
+  cut(p.planes * ceil_div(std::min<int64_t>(p.piece, a.t), BK), row_tiles * col_tiles, p.input_parts, p.input_blocks);
   cut(p.planes * ceil_div(a.n, BK), ceil_div(p.piece, TILE_M) * col_tiles, p.weight_parts, p.weight_blocks);
   p.g = at;
   p.dx = p.g + up((size_t)a.n * p.g_pitch * 2 * p.parts * p.planes);
-  p.dw = p.dx + (p.input_parts * p.pieces > 1 ? up((size_t)p.input_parts * p.pieces * a.n * p.pitch * 4) : 0);
-  p.bytes = p.dw + (p.weight_parts > 1 ? up((size_t)p.weight_parts * p.piece * p.pitch * 4) : 0);
+  p.dw = p.dx + (a.dx && (p.input_parts > 1 || p.pieces > 1) ? up((size_t)p.input_parts * a.n * p.pitch * 4) : 0);
+  p.bytes = p.dw + (a.dw && p.weight_parts > 1 ? up((size_t)p.weight_parts * p.piece * p.pitch * 4) : 0);
   return p;
 }
 
@@ -724,7 +736,7 @@ extern "C" int eqt_type_loss_backward(const eqt_type_loss_args* args, void* stre
   if (int rc = operands(a, p, true, x, w, s)) return rc;
   unsigned char* base = static_cast<unsigned char*>(a.scratch);
   float *dx_parts = reinterpret_cast<float*>(base + p.dx), *dw_parts = reinterpret_cast<float*>(base + p.dw);
-  const int dx_slots = (int)(p.input_parts * p.pieces), size = size_of(a.dtype);
+  const int size = size_of(a.dtype);
   for (int64_t i = 0; i < p.pieces; ++i) {
     const int64_t t0 = i * p.piece, here = std::min<int64_t>(p.piece, a.t - t0);
     Launch l{};
@@ -740,10 +752,12 @@ extern "C" int eqt_type_loss_backward(const eqt_type_loss_args* args, void* stre
       if (int rc = tc::map_bf16(&d.a, base + p.g, a.n, here, p.g_pitch, a.n * p.g_pitch, p.parts * p.planes, tc::TILE_M)) return rc;
       if (int rc = tc::map_bf16(&d.b, w, a.t, p.pitch, p.pitch, a.t * p.pitch, p.parts, BK)) return rc;
       d.rows = a.n, d.columns = (int)a.c, d.width = p.width_c, d.row_tiles = l.row_tiles, d.col_tiles = (int)ceil_div(a.c, p.width_c);
-      d.plane_blocks = (int)ceil_div(p.piece, BK), d.kblocks = p.planes * d.plane_blocks, d.part_blocks = p.input_blocks, d.fold = l.fold, d.items = (unsigned)(d.row_tiles * d.col_tiles * p.input_parts);
-      d.b_first = (int)t0, d.typed = dx_slots == 1, d.target = a.target, d.types = a.t, d.status = a.status;
+      d.plane_blocks = (int)ceil_div(here, BK), d.kblocks = p.planes * d.plane_blocks, d.part_blocks = p.input_blocks, d.fold = l.fold;
+      d.items = (unsigned)(d.row_tiles * d.col_tiles * ceil_div(d.kblocks, d.part_blocks));                 // a short last piece adds to the first parts only
+      d.b_first = (int)t0, d.typed = p.input_parts == 1 && i == p.pieces - 1, d.target = a.target, d.types = a.t, d.status = a.status;
       d.grad = a.grad, d.count = a.count, d.reduction = a.reduction;
-      d.out = d.typed ? a.dx : dx_parts, d.out_pitch = d.typed ? a.c : p.pitch, d.out_part = a.n * p.pitch, d.slot = (int)(i * p.input_parts);
+      d.out = d.typed ? a.dx : dx_parts, d.out_pitch = d.typed ? a.c : p.pitch, d.out_part = a.n * p.pitch;
+      d.before = i ? dx_parts : nullptr, d.before_pitch = p.pitch, d.before_part = a.n * p.pitch;
       d.whole = !d.typed || a.c * size % 16 == 0;
       if (int rc = launch<INPUT>(p.parts, d, s)) return rc;
     }
@@ -763,6 +777,6 @@ extern "C" int eqt_type_loss_backward(const eqt_type_loss_args* args, void* stre
         if (int rc = sum_parts(a.dtype, dw_parts, to, here, (int)a.c, p.pitch, p.weight_parts, nullptr, s)) return rc;
     }
   }
-  if (a.dx && dx_slots > 1) return sum_parts(a.dtype, dx_parts, a.dx, a.n, (int)a.c, p.pitch, dx_slots, a.target, s);
+  if (a.dx && p.input_parts > 1) return sum_parts(a.dtype, dx_parts, a.dx, a.n, (int)a.c, p.pitch, p.input_parts, a.target, s);
   return EQT_OK;
 }

@@ -35,7 +35,8 @@ def type_cross_entropy(x: Tensor, weight: Tensor, target: Tensor, reduction: str
     that count (zero if none does), ``sum`` or ``none``; the loss is float32.
 
     float32 or bfloat16 features and table of one type, at most 16384 channels.  The logits are formed in tiles and never kept, once forward and once backward, where
-    their gradients are in scratch for at most 256 MB of types at a time.  Sums in float32, no atomics; of bfloat16 the logits' gradients are rounded
+    their gradients are in scratch for some types at a time (256 MB, or 128 types of over a million rows), beside a float32 sum of the size of ``x``
+    and operands that are laid out anew (``x``; of float32 both, in three parts).  Sums in float32, no atomics; of bfloat16 the logits' gradients are rounded
     to bfloat16 for their products.  Differentiable once, in ``x`` and ``weight``."""
     _ops.check(x, weight, target, reduction)
     return _TypeCrossEntropy.apply(x, weight, target, reduction)

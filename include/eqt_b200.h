@@ -789,7 +789,7 @@ int eqt_window_attention_backward(const eqt_window_attention_args* args, void* s
  * Rows of a negative target do not count: their loss is zero and they have no gradient.  A target from t on gives NaN.  reduction: 0 none,
  * 1 sum, 2 mean over the rows that count (zero if none does), to result[0]; count[0]: how many count.  lse (n): the rows' log sums in units of log2, for the backward pass.
  * Backward: grad (n floats for reduction 0, else 1) and what the forward pass left; dx (n, c), dw (t, c), either may be NULL.  float32 (as six
- * bfloat16 products of three parts each) or bfloat16, all contiguous; sums in float32, no atomics.  scratch: eqt_type_loss_scratch bytes, 16-byte aligned. */
+ * bfloat16 products of three parts each) or bfloat16, all contiguous; sums in float32, no atomics.  scratch: eqt_type_loss_scratch bytes, 16-byte aligned; backward it goes by which of dx and dw are given. */
 typedef struct {
   int32_t dtype, reduction;
   int64_t n, c, t, scratch_bytes;

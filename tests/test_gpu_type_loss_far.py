@@ -60,3 +60,46 @@ def test_gradients_of_large_and_far_logits(scale, dtype):
     _, _, *grads = reference(x, w, target, torch.full((100,), 1.0, dtype=torch.float64, device=DEV) / count)
     within(dx, *grads[:2], "dx")
     within(dw, *grads[2:], "dw")
+
+
+def check_against_reference(x, w, target):
+    loss = F.type_cross_entropy(x, w, target)
+    dx, dw = torch.autograd.grad(loss, [x, w])
+    peak = torch.cuda.max_memory_allocated()
+    want, eloss, *grads = reference(x, w, target, torch.full((x.shape[0],), 1.0, dtype=torch.float64, device=DEV) / (target >= 0).sum())
+    within(loss, want.sum() / (target >= 0).sum(), eloss.sum() / (target >= 0).sum() + 2.0 ** -22 * want.mean(), "loss")
+    within(dx, *grads[:2], "dx")
+    within(dw, *grads[2:], "dw")
+    assert not dx[target < 0].any()
+    return peak
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_many_pieces_of_types_with_many_channels(dtype):
+    """The features' gradient is one float32 sum that the pieces are added to, in scratch of the features' size and not of the table's.  A piece rounds it once, 2^-24."""
+    n, t, c = (12_000, 60_000, 512) if dtype == torch.bfloat16 else (9_000, 30_000, 512)
+    x, w, target = make(n, t, c, dtype)
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    torch.cuda.reset_peak_memory_stats()
+    start, size = torch.cuda.memory_allocated(), x.element_size()
+    peak = check_against_reference(x, w, target) - start
+    operands = n * c * 2 if dtype == torch.bfloat16 else (n + t) * c * 6
+    assert peak < 256 * 2 ** 20 + operands + n * c * 4 + (n + t) * c * size + 16 * 2 ** 20
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("more", [-1, 0, 1, 63, 64, 65, 130])
+def test_short_last_pieces(more, dtype):
+    """Tables that end a little before or behind a piece's end."""
+    n = 20_000
+    piece = (256 * 2 ** 20 // (2 if dtype == torch.bfloat16 else 6) // 20_096) // 128 * 128
+    for c in (16, 20):
+        check_against_reference(*make(n, piece + more, c, dtype))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_pieces_of_few_rows_of_results(dtype):
+    """Few tiles of results, so that sums over the types are cut into parts, and several pieces."""
+    n, t, c = 900, (160_000 if dtype == torch.bfloat16 else 60_000), 40
+    check_against_reference(*make(n, t, c, dtype))
