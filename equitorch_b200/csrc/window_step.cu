@@ -108,12 +108,15 @@ template <typename T, int DP> __global__ void __launch_bounds__(THREADS) step_ke
       const float base = most == -INFINITY ? 0.f : most, keep = exp2_fast(top[r] - base);
       float add = 0.f;
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          z[n][2 * r + i] = exp2_fast(z[n][2 * r + i] - base);
-          add += z[n][2 * r + i];
+      for (int n = 0; n < NT; ++n) {
+        float &x = z[n][2 * r], &y = z[n][2 * r + 1];
+        x = exp2_fast(x - base), y = exp2_fast(y - base);
+        if constexpr (sizeof(T) == 2) {                  // the sum is that of the weights in the product
+          const uint32_t two = pack_bf16(x, y);
+          x = __uint_as_float(two << 16), y = __uint_as_float(two & 0xffff0000u);
         }
+        add += x + y;
+      }
       sum[r] = sum[r] * keep + add;
       top[r] = most;
 #pragma unroll
