@@ -199,14 +199,15 @@ template <typename T> __global__ void __launch_bounds__(THREADS) step_join_kerne
 int width_of(int values) { return values <= 16 ? 16 : values <= 32 ? 32 : values <= 64 ? 64 : 128; }
 int keys_of(int dtype, int width) { return (dtype == EQT_F32 ? 4 : 2) * width > 256 ? 8 : (dtype == EQT_F32 ? 4 : 2) * width > 128 ? 16 : 32; }
 
-// Parts of the visible keys: so many that SMs with shorter chains take more of them, and a step for each warp.
+// Parts of the visible keys: so many that SMs with shorter chains take more of them, a step for each warp, and of a warp no more than what bfloat16 products may add up in
+// the matrix instructions, whose adder truncates (1,048,576 keys in one part: 1e-3 of a sum of one sign).
 void cut(StepArgs& p, int dtype, int64_t chains, int kv_heads) {
   const int kt = keys_of(dtype, width_of(p.a.comps * p.a.size));
   const int64_t window = std::min<int64_t>(p.capacity, p.before + 1), first = std::min<int64_t>(p.capacity, p.sinks);
   const int64_t steps = std::max<int64_t>(1, ceil_div(window, kt) + ceil_div(first, kt));
   const int64_t others = std::max<int64_t>(1, chains * kv_heads), wanted = ceil_div((int64_t)sm_count() * 8, others);
   const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(wanted, ceil_div(steps, WARPS)), 1024));
-  p.part_steps = ceil_div(ceil_div(steps, parts), WARPS) * WARPS;
+  p.part_steps = std::min<int64_t>(ceil_div(ceil_div(steps, parts), WARPS), FOLD / kt) * WARPS;
   p.num_parts = (int)ceil_div(steps, p.part_steps);
 }
 
