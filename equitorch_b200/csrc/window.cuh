@@ -36,6 +36,7 @@ struct WindowParams {
   int64_t chains;
   float* far;
   int split;
+  int folds_rows, folds_columns;   // bfloat16: sums of results and dq, and of dk and dv, of more than FOLD terms
 };
 constexpr int FAR_BLOCK = 512, FAR_ROWS = 16, MOST_SPLIT_SINKS = 64;
 __host__ __device__ inline int far_groups(const WindowParams& p) { return (p.sinks + FAR_ROWS - 1) / FAR_ROWS; }

@@ -43,6 +43,11 @@ WindowParams params(const eqt_window_attention_args& a) {
   // chains of 50 to 500 nodes, window of 64 on both sides: 217 us walked, 164 and 61 apart); and not for so many first nodes that tiles are full of them.
   p.ptr = a.ptr, p.chains = a.num_graphs, p.rest = a.dtype == EQT_BF16 ? a.rest : nullptr;
   p.split = p.sinks > 0 && p.sinks <= MOST_SPLIT_SINKS && a.longest - p.before > 2 * FAR_BLOCK;
+  if (a.dtype == EQT_BF16) {
+    const int64_t window = std::min<int64_t>((int64_t)p.before + p.after + 1, reach);
+    p.folds_rows = std::min<int64_t>(window + p.sinks, reach) > attention::FOLD;
+    p.folds_columns = p.group * (p.sinks && !p.split ? reach : window) > attention::FOLD;
+  }
   return p;
 }
 
@@ -70,6 +75,11 @@ int check_scratch(const eqt_window_attention_args& a, bool backward) {
   if (need && (!a.scratch || a.scratch_bytes < need))
     return fail(EQT_ERR_BAD_ARGUMENT, "window_attention: %lld bytes of scratch given, %lld needed", (long long)a.scratch_bytes, (long long)need);
   return reinterpret_cast<uintptr_t>(a.scratch) % 16 ? fail(EQT_ERR_BAD_ARGUMENT, "window_attention: scratch must start on a 16-byte boundary") : EQT_OK;
+}
+int check_tiles(const eqt_window_attention_args& a, const WindowParams& p) {
+  if (p.folds_rows && a.tile_rows != 64)
+    return fail(EQT_ERR_UNSUPPORTED, "window_attention: bfloat16 windows of more than %d nodes need tiles of 64 rows, got %d", attention::FOLD, a.tile_rows);
+  return EQT_OK;
 }
 int tensor_params(TcParams& t, const eqt_window_attention_args& a, const WindowParams& p, cudaStream_t s) {
   if (!a.ptr || !a.status) return fail(EQT_ERR_BAD_ARGUMENT, "window_attention: NULL pointer");
@@ -110,6 +120,7 @@ extern "C" int eqt_window_attention_forward(const eqt_window_attention_args* arg
     if (int rc = tensor_params(t, a, p, s)) return rc;
     return tc_forward(t, s);
   }
+  if (int rc = check_tiles(a, p)) return rc;
   return a.dtype == EQT_F32 ? tiles_forward_f32(p, a.tile_rows, a.num_tiles, s) : tiles_forward_bf16(p, a.tile_rows, a.num_tiles, s);
 }
 
@@ -131,5 +142,6 @@ extern "C" int eqt_window_attention_backward(const eqt_window_attention_args* ar
     if (int rc = tensor_params(t, a, p, s)) return rc;
     return tc_backward(t, s);
   }
+  if (int rc = check_tiles(a, p)) return rc;
   return a.dtype == EQT_F32 ? tiles_backward_f32(p, a.tile_rows, a.num_tiles, s) : tiles_backward_bf16(p, a.tile_rows, a.num_tiles, s);
 }

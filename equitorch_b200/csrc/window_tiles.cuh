@@ -66,9 +66,12 @@ template <typename F> __device__ __forceinline__ void each_bad_row(bool bad0, bo
     if ((((r < 8 ? b0 : b1) >> (4 * (r & 7))) & 15) && row + r < end) again(row + r);
 }
 
+// Whether the sums of bfloat16 products are taken out of the matrix instructions before a step, so that they are of at most FOLD terms.
+template <int KT> __device__ __forceinline__ bool fold_now(int step) { return step > 0 && step % (FOLD / KT) == 0; }
+
 template <typename T> __device__ __forceinline__ float rounded(float x) { return sizeof(T) == 4 ? x : __bfloat162float(__float2bfloat16_rn(x)); }
 
-template <typename T, int DP, int WR, int KT>
+template <typename T, int DP, int WR, int KT, bool FOLDS>
 __global__ void __launch_bounds__(THREADS, DP <= 64 ? 4 : 3) window_forward_kernel(const __grid_constant__ WindowParams p) {
   using S = attention::Shape<T, DP, WR, KT>;
   constexpr int LD = S::LD, NT = KT / 8;
@@ -100,10 +103,17 @@ __global__ void __launch_bounds__(THREADS, DP <= 64 ? 4 : 3) window_forward_kern
   const bool work = here && row < hi;
   const T* mine = rows + (warp % WR) * 16 * LD;
   const float unit = p.q.scale * LOG2E;
-  float o[DP / 8][4], top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
+  float o[DP / 8][4], top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f}, kept[2] = {1.f, 1.f};
+  Far<FOLDS ? DP : 2> waiting;                           // FOLDS: the sums of the steps before, in a unit that was `kept` times as great
 #pragma unroll
   for (int n = 0; n < DP / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
   for (int step = 0, s = 0; step < walk.steps; ++step, s ^= 1) {
+    if constexpr (FOLDS) {
+      if (fold_now<KT>(step) && work) {
+        fold<DP>(waiting.at(), o, step == FOLD / KT, kept[0], kept[1]);
+        kept[0] = kept[1] = 1.f;
+      }
+    }
     if (step + 1 < walk.steps) {
       fetch(step + 1, s ^ 1);
       copies_wait<1>();
@@ -142,6 +152,7 @@ __global__ void __launch_bounds__(THREADS, DP <= 64 ? 4 : 3) window_forward_kern
             add += z[n][2 * r + i];
           }
         sum[r] = sum[r] * keep + add;
+        if (FOLDS) kept[r] *= keep;
         top[r] = most;
 #pragma unroll
         for (int n = 0; n < DP / 8; ++n) o[n][2 * r] *= keep, o[n][2 * r + 1] *= keep;
@@ -151,6 +162,8 @@ __global__ void __launch_bounds__(THREADS, DP <= 64 ? 4 : 3) window_forward_kern
     __syncthreads();
   }
   if (!work) return;
+  if constexpr (FOLDS)
+    if (walk.steps > FOLD / KT) unfold<DP>(waiting.at(), o, kept[0], kept[1]);
   float f[2];
 #pragma unroll
   for (int r = 0; r < 2; ++r) f[r] = 1.f / quad_sum(sum[r]);
@@ -174,7 +187,7 @@ __global__ void __launch_bounds__(THREADS, DP <= 64 ? 4 : 3) window_forward_kern
   each_bad_row(!ok0, !ok1, row, hi, [&](int i) { again_forward<T>(p, i, head, lo, hi, lane); });
 }
 
-template <typename T, int DP, int WR, int KT>
+template <typename T, int DP, int WR, int KT, bool FOLDS>
 __global__ void __launch_bounds__(THREADS, DP <= 32 ? 4 : DP <= 96 ? 3 : 2) window_rows_kernel(const __grid_constant__ WindowParams p) {
   using S = attention::Shape<T, DP, WR, KT>;
   constexpr int LD = S::LD, NT = KT / 8;
@@ -232,7 +245,10 @@ __global__ void __launch_bounds__(THREADS, DP <= 32 ? 4 : DP <= 96 ? 3 : 2) wind
   float dq[DP / 8][4];
 #pragma unroll
   for (int n = 0; n < DP / 8; ++n) dq[n][0] = dq[n][1] = dq[n][2] = dq[n][3] = 0.f;
+  Far<FOLDS ? DP : 2> waiting;
   for (int step = 0, s = 0; step < walk.steps; ++step, s ^= 1) {
+    if constexpr (FOLDS)
+      if (fold_now<KT>(step) && work) fold<DP>(waiting.at(), dq, step == FOLD / KT);
     if (step + 1 < walk.steps) {
       fetch(step + 1, s ^ 1);
       copies_wait<1>();
@@ -264,6 +280,8 @@ __global__ void __launch_bounds__(THREADS, DP <= 32 ? 4 : DP <= 96 ? 3 : 2) wind
     __syncthreads();
   }
   if (!work) return;
+  if constexpr (FOLDS)
+    if (walk.steps > FOLD / KT) unfold<DP>(waiting.at(), dq);
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
     const float all = quad_sum(exact[r]), sum = 1.f / quad_sum(sums[r]);
@@ -274,7 +292,7 @@ __global__ void __launch_bounds__(THREADS, DP <= 32 ? 4 : DP <= 96 ? 3 : 2) wind
   each_bad_row(!ok0, !ok1, row, hi, [&](int i) { again_rows<T>(p, i, head, lo, hi, lane); });
 }
 
-template <typename T, int DP, int WR, int KT>
+template <typename T, int DP, int WR, int KT, bool FOLDS>
 __global__ void __launch_bounds__(THREADS, DP <= 64 ? 3 : 2) window_columns_kernel(const __grid_constant__ WindowParams p) {
   using S = attention::Shape<T, DP, WR, KT>;
   constexpr int LD = S::LD, NT = KT / 8;
@@ -319,7 +337,13 @@ __global__ void __launch_bounds__(THREADS, DP <= 64 ? 3 : 2) window_columns_kern
   for (int n = 0; n < DP / 8; ++n)
 #pragma unroll
     for (int i = 0; i < 4; ++i) dk[n][i] = dv[n][i] = 0.f;
+  Far<FOLDS ? DP : 2> waiting_k, waiting_v;
   for (int step = 0, s = 0; step < steps; ++step, s ^= 1) {
+    if constexpr (FOLDS)
+      if (fold_now<KT>(step) && work) {
+        fold<DP>(waiting_k.at(), dk, step == FOLD / KT);
+        fold<DP>(waiting_v.at(), dv, step == FOLD / KT);
+      }
     if (step + 1 < steps) {
       fetch(step + 1, s ^ 1);
       copies_wait<1>();
@@ -351,6 +375,11 @@ __global__ void __launch_bounds__(THREADS, DP <= 64 ? 3 : 2) window_columns_kern
     __syncthreads();
   }
   if (!work) return;
+  if constexpr (FOLDS)
+    if (steps > FOLD / KT) {
+      unfold<DP>(waiting_k.at(), dk);
+      unfold<DP>(waiting_v.at(), dv);
+    }
   if (p.split && row < lo + p.sinks) {
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
@@ -376,7 +405,7 @@ __global__ void __launch_bounds__(THREADS, DP <= 64 ? 3 : 2) window_columns_kern
 
 // 16 first nodes of a chain and the queries behind their windows in one block of the batch: a CTA, whose warps take the steps of all heads in turn and
 // add their sums up in order.
-template <typename T, int DP, int KT> __global__ void __launch_bounds__(THREADS) window_far_kernel(const __grid_constant__ WindowParams p) {
+template <typename T, int DP, int KT, bool FOLDS> __global__ void __launch_bounds__(THREADS) window_far_kernel(const __grid_constant__ WindowParams p) {
   using S = attention::Shape<T, DP, 1, KT>;
   constexpr int LD = S::LD, NT = KT / 8;
   extern __shared__ __align__(16) unsigned char smem[];
@@ -417,7 +446,13 @@ template <typename T, int DP, int KT> __global__ void __launch_bounds__(THREADS)
   for (int n = 0; n < DP / 8; ++n)
 #pragma unroll
     for (int i = 0; i < 4; ++i) dk[n][i] = dv[n][i] = 0.f;
+  Far<FOLDS ? DP : 2> waiting_k, waiting_v;
   for (int step = warp, s = 0; step < steps; step += WARPS, s ^= 1) {
+    if constexpr (FOLDS)
+      if (fold_now<KT>(step / WARPS)) {
+        fold<DP>(waiting_k.at(), dk, step / WARPS == FOLD / KT);
+        fold<DP>(waiting_v.at(), dv, step / WARPS == FOLD / KT);
+      }
     if (step + WARPS < steps) {
       fetch(step + WARPS, s ^ 1);
       copies_wait<1>();
@@ -445,6 +480,11 @@ template <typename T, int DP, int KT> __global__ void __launch_bounds__(THREADS)
     __syncwarp();
   }
   copies_wait<0>();
+  if constexpr (FOLDS)
+    if ((steps - warp + WARPS - 1) / WARPS > FOLD / KT) {
+      unfold<DP>(waiting_k.at(), dk);
+      unfold<DP>(waiting_v.at(), dv);
+    }
   float* sums = reinterpret_cast<float*>(smem);          // [dk, dv][node][value], where the tiles were
   for (int w = 0; w < WARPS; ++w) {
     __syncthreads();
@@ -484,9 +524,14 @@ template <typename T, int DP> int launch_far(const WindowParams& p, cudaStream_t
   const int64_t pairs = ceil_div(p.q.n, FAR_BLOCK) + p.chains;
   if (pairs > INT32_MAX || p.kv.heads > 65535) return fail(EQT_ERR_UNSUPPORTED, "window_attention: %lld chains are more than one launch takes", (long long)p.chains);
   const size_t shared = S::bytes(2, WARPS * 6 * KT * 4);
-  auto kernel = window_far_kernel<T, DP, KT>;
-  static std::atomic<uint64_t> allowed{0};
-  if (int rc = allow_shared_once(kernel, shared, allowed)) return rc;
+  auto kernel = window_far_kernel<T, DP, KT, false>;
+  bool folds = false;                                    // a warp has a quarter of a block's queries of all heads
+  if constexpr (sizeof(T) == 2) {
+    folds = p.group > FOLD / (FAR_BLOCK / WARPS);
+    if (folds) kernel = window_far_kernel<T, DP, KT, true>;
+  }
+  static std::atomic<uint64_t> allowed[2]{};
+  if (int rc = allow_shared_once(kernel, shared, allowed[folds])) return rc;
   kernel<<<dim3((unsigned)pairs, (unsigned)p.kv.heads, (unsigned)far_groups(p)), THREADS, shared, s>>>(p);
   if (int rc = check_launch("window_far")) return rc;
   const int groups = far_groups(p), chunks = (int)ceil_div(2 * FAR_ROWS * p.q.comps * p.q.size, 256);
@@ -499,13 +544,13 @@ template <typename T> int far(const WindowParams& p, cudaStream_t s) {
 }
 
 enum Pass { FORWARD, ROWS, COLUMNS };
-template <typename T, int DP, int WR, int KT, int PASS> int launch(const WindowParams& p, int64_t num_tiles, cudaStream_t s) {
+template <typename T, int DP, int WR, int KT, int PASS, bool FOLDS = false> int launch(const WindowParams& p, int64_t num_tiles, cudaStream_t s) {
   using S = attention::Shape<T, DP, WR, KT>;
   const int heads = PASS == COLUMNS ? p.kv.heads : p.q.heads;
   const int64_t grid = num_tiles * ceil_div(heads, S::HEADS);
   if (grid > INT32_MAX) return fail(EQT_ERR_UNSUPPORTED, "window_attention: %lld tiles are more than one launch takes", (long long)grid);
   const size_t shared = S::bytes(PASS == FORWARD ? 1 : 2, PASS == COLUMNS ? S::HEADS * 6 * KT * 4 : 0);
-  auto kernel = PASS == FORWARD ? window_forward_kernel<T, DP, WR, KT> : PASS == ROWS ? window_rows_kernel<T, DP, WR, KT> : window_columns_kernel<T, DP, WR, KT>;
+  auto kernel = PASS == FORWARD ? window_forward_kernel<T, DP, WR, KT, FOLDS> : PASS == ROWS ? window_rows_kernel<T, DP, WR, KT, FOLDS> : window_columns_kernel<T, DP, WR, KT, FOLDS>;
   static std::atomic<uint64_t> allowed{0};
   if (int rc = allow_shared_once(kernel, shared, allowed)) return rc;
   kernel<<<(unsigned)grid, THREADS, shared, s>>>(p);
@@ -514,6 +559,16 @@ template <typename T, int DP, int WR, int KT, int PASS> int launch(const WindowP
 // Keys a step: 32, of wide float32 rows 16, whose two stages would not fit three CTAs an SM.
 template <typename T, int DP, int PASS> int by_rows(const WindowParams& p, int tile_rows, int64_t num_tiles, cudaStream_t s) {
   constexpr int KT = sizeof(T) == 4 && DP > 64 ? 16 : 32;
+  // Long sums, in kernels of their own, whose registers the others need not pay for: by columns of chains of any length, since heads add up; of rows where chains are so long
+  // that tiles have 64 rows.
+  if constexpr (sizeof(T) == 2) {
+    if constexpr (PASS == COLUMNS)
+      if (p.folds_columns)
+        return tile_rows == 16 ? launch<T, DP, 1, KT, COLUMNS, true>(p, num_tiles, s) : tile_rows == 32 ? launch<T, DP, 2, KT, COLUMNS, true>(p, num_tiles, s)
+                                                                                                         : launch<T, DP, 4, KT, COLUMNS, true>(p, num_tiles, s);
+    if constexpr (PASS != COLUMNS)
+      if (p.folds_rows) return launch<T, DP, 4, KT, PASS, true>(p, num_tiles, s);
+  }
   switch (tile_rows) {
     case 16: return launch<T, DP, 1, KT, PASS>(p, num_tiles, s);
     case 32: return launch<T, DP, 2, KT, PASS>(p, num_tiles, s);

@@ -1,0 +1,23 @@
+"""What the windows' entry points refuse besides, without a GPU."""
+import ctypes as C
+
+import torch
+
+from equitorch_b200 import _lib
+
+
+def window(**more):
+    args = dict(dtype=_lib.DTYPE_CODE[torch.bfloat16], comps=1, heads=2, kv_heads=1, head_channels=8, tile_rows=64, scale=-1.0, n=40_000, num_graphs=1, longest=40_000, num_tiles=625,
+                before=30_000, after=0, sinks=0, q_node=16, k_node=8, v_node=8, q=16, k=16, v=16, out=16, rest=16, stats=16, tiles=16, ptr=16, status=16, grad=16, dq=16, dk=16, dv=16)
+    args = _lib.WindowAttentionArgs(**{**args, **more})
+    for backward in (0, 1):
+        args.scratch, args.scratch_bytes = 16, max(args.scratch_bytes, _lib.lib().eqt_window_attention_scratch(C.byref(args), backward))
+    return args
+
+
+def test_long_windows_of_bfloat16_need_the_highest_tiles_of_one_chain():
+    """Whose kernels alone take long sums apart; a packed batch with a chain of more than 8192 nodes has these."""
+    lib = _lib.lib()
+    for rows in (16, 32):
+        assert lib.eqt_window_attention_forward(C.byref(window(tile_rows=rows)), None) == 2
+        assert lib.eqt_window_attention_backward(C.byref(window(tile_rows=rows)), None) == 2
