@@ -25,6 +25,8 @@
 // of 128 x 64 takes as long as one of 128 x 128: S and dP run at half the rate.  128 keys at a time have the full rate, and lost forward (240 -> 267 us), where tensor
 // memory then has one buffer of scores.  One chain of 32,781 nodes, 8 heads of 128, window of 1024 and 4 first nodes: forward 240 us, by rows 395, by columns
 // 393, tensor pipe 33 to 37 % busy; a step of 64 takes a CTA 2200 cycles, 1400 of them softmax, the rest the way to the MMAs and back.
+// The tensor cores' adder truncates, 1.2e-7 of a sum of one sign at every 16 terms, so sums that may be of more than 8192 terms are taken out every 126 steps, in kernels of
+// their own (one chain of 32,781 nodes, window of 16,384, 8 heads of 128: 9.0 -> 9.8 ms; of 64, two heads of keys: 7.5 -> 7.8).
 // Every wait is bounded; on expiry the status flag is raised and the kernel ends.
 #include <algorithm>
 
@@ -221,10 +223,35 @@ __device__ __forceinline__ void across_lanes(uint32_t (&u)[16], int lane) {
     }
 }
 
-// Of the lanes' rows of results the WIDE values from the `first` on, with `more` where given, `f` times, to (n, components, heads, channels), and what the rounding
+// FOLDS: a lane's WIDE sums out of tensor memory, onto those that wait in local memory (in a unit that was `kept` times as great), so that the tensor cores' adder, which
+// truncates, adds up at most 128 steps (8192 terms).  Before a tile's step of the group's first turn and FOLD_STEPS, and every FOLD_STEPS from there.
+constexpr int FOLD_STEPS = 126;                          // a multiple of the groups, which are one, two or three
+template <int WIDE> __device__ __noinline__ void take_out(float* beside, uint32_t sum, int wide, bool first, float kept) {
+#pragma unroll 1
+  for (int h = 0; h < WIDE; h += 32) {
+    if (h >= wide) break;
+    uint32_t r[32];
+    tmem_issue32(sum + h, r);
+    tmem_arrived32(r);
+    float4* to = reinterpret_cast<float4*>(beside + h);
+    float4 v[8];                                         // all of them on their way at once: memory is far
+    if (!first) {
+#pragma unroll
+      for (int c = 0; c < 8; ++c) v[c] = to[c];
+    } else {
+#pragma unroll
+      for (int c = 0; c < 8; ++c) v[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+      to[c] = make_float4(fmaf(v[c].x, kept, __uint_as_float(r[4 * c])), fmaf(v[c].y, kept, __uint_as_float(r[4 * c + 1])), fmaf(v[c].z, kept, __uint_as_float(r[4 * c + 2])),
+                          fmaf(v[c].w, kept, __uint_as_float(r[4 * c + 3])));
+  }
+}
+// Of the lanes' rows of results the WIDE values from the `first` on, with `more` and those `beside` where given, `f` times, to (n, components, heads, channels), and what the rounding
 // left to `rest`; whether they were finite.  Loops are not unrolled: code that runs once a tile comes from beyond the instruction cache.
 template <int WIDE> __device__ __forceinline__ bool put_row(uint32_t sum, int first, float f, bool on, void* out, int row, int head, const AttentionParams& p, int lane,
-                                                            const float* more = nullptr, void* rest = nullptr) {
+                                                            const float* more = nullptr, void* rest = nullptr, const float* beside = nullptr, float kept = 1.f) {
   const int values = p.comps * p.size;
   const int64_t place = on ? ((int64_t)row * p.comps * p.heads + head) * p.size : -1;
   int64_t to[4];
@@ -240,6 +267,10 @@ template <int WIDE> __device__ __forceinline__ bool put_row(uint32_t sum, int fi
 #pragma unroll
     for (int c = 0; c < 32; c += 8) {
       if (h + c >= values) break;
+      if (beside) {
+#pragma unroll
+        for (int j = c; j < c + 8; ++j) r[j] = __float_as_uint(fmaf(beside[h - first + j], kept, __uint_as_float(r[j])));
+      }
       if (more) {
 #pragma unroll
         for (int j = c; j < c + 8; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) + more[h + j]);
@@ -275,8 +306,8 @@ template <int WIDE> __device__ __forceinline__ bool put_row(uint32_t sum, int fi
   return x + y == 0.f;
 }
 
-// FINE, by columns: weights and score gradients go into their products in two parts
-template <int DP, int MODE, bool FINE> __global__ void __launch_bounds__(Form<DP, MODE>::THREADS, Form<DP, MODE>::CTAS) window_tc_kernel(const __grid_constant__ TcParams p) {
+// FINE, by columns: weights and score gradients go into their products in two parts.  FOLDS: sums may be of more than 8192 terms.
+template <int DP, int MODE, bool FINE, bool FOLDS> __global__ void __launch_bounds__(Form<DP, MODE>::THREADS, Form<DP, MODE>::CTAS) window_tc_kernel(const __grid_constant__ TcParams p) {
   using F = Form<DP, MODE>;
   constexpr int SLOTS = F::SLOTS, GROUPS = F::GROUPS, BUFFERS = F::BUFFERS;
   extern __shared__ __align__(1024) unsigned char smem[];
@@ -485,7 +516,15 @@ template <int DP, int MODE, bool FINE> __global__ void __launch_bounds__(Form<DP
           continue;
         }
         ok = number == 0 || bar_wait(sums_free, (uint32_t)((number - 1) & 1), ab);
-        for (bool more = false; j < end && ok; ++j, more = true) {
+        const unsigned start = j;
+        // a sum starts anew where a group takes out what there is: that of dk the last group, others the first
+        unsigned anew = start + (GROUPS - start % GROUPS) % GROUPS + FOLD_STEPS, anew_k = start + (GROUPS - 1 + GROUPS - start % GROUPS) % GROUPS + FOLD_STEPS;
+        auto goes_on = [&](unsigned& next) {
+          if (!FOLDS || j != next) return j != start;
+          next += FOLD_STEPS;
+          return false;
+        };
+        for (; j < end && ok; ++j) {
           const uint32_t d = tmem + (j % BUFFERS) * F::BUFFER;
           ok = arrived(2 * j + 1) && (MODE != COLUMNS || arrived(2 * j));
           if (!ok) break;
@@ -493,10 +532,10 @@ template <int DP, int MODE, bool FINE> __global__ void __launch_bounds__(Form<DP
           ok = weighted(j);
           if (!ok) break;
           tc_fence_after();
-          add(sum, d, slot_at(2 * j + 1), more);
+          add(sum, d, slot_at(2 * j + 1), goes_on(anew));
           if (MODE == ROWS || FINE) add(sum, d + 16, slot_at(2 * j + 1), true);
           if (MODE == COLUMNS) {
-            add(sum + DP, d + KEYS, slot_at(2 * j), more);
+            add(sum + DP, d + KEYS, slot_at(2 * j), goes_on(anew_k));
             if (FINE) add(sum + DP, d + KEYS + 16, slot_at(2 * j), true);
             umma_commit(&empty[2 * j % SLOTS]);
           }
@@ -531,8 +570,22 @@ template <int DP, int MODE, bool FINE> __global__ void __launch_bounds__(Form<DP
     };
     int2 next_span = span_of(blockIdx.x);
     int number = 0;
+    alignas(16) attention::Far<FOLDS ? 2 * WIDE : 2> waiting;
+    float* const beside = FOLDS ? waiting.at() : nullptr;
     for (unsigned i = blockIdx.x; i < p.tiles; i += gridDim.x, ++number) {
     const Tile tile = tile_of(i);
+    bool taken = false;                                  // some of the tile's sums are beside
+    int take_next = FOLD_STEPS;
+    // before the tile's k-th step, once all products of those before it are there
+    auto take_out_sums = [&](unsigned j, uint32_t sum, float kept) {
+      take_next += FOLD_STEPS;
+      ok = __all_sync(0xffffffffu, bar_wait(&freed[(j - 1) % BUFFERS], ((j - 1) / BUFFERS) & 1, ab));
+      if (!ok) return false;
+      tc_fence_after();
+      take_out<WIDE>(beside, sum, values - first_value, !taken, kept);
+      taken = true;
+      return true;
+    };
     const int row = tile.first + in_tile, mine = tile.head + in_pack;
     const int2 span = next_span;
     next_span = span_of(i + gridDim.x);
@@ -572,7 +625,7 @@ template <int DP, int MODE, bool FINE> __global__ void __launch_bounds__(Form<DP
       tiles_done = number + 1;
     };
     if (MODE == FORWARD) {
-      float base = -INFINITY, total = 0.f;
+      float base = -INFINITY, total = 0.f, kept = 1.f;
       for (int k = 0; k < steps; ++k) {
         const unsigned j = j0 + k, b = j % BUFFERS;
         ok = __all_sync(0xffffffffu, bar_wait(&scores[b], (j / BUFFERS) & 1, ab));
@@ -594,11 +647,16 @@ template <int DP, int MODE, bool FINE> __global__ void __launch_bounds__(Form<DP
 #pragma unroll
           for (int c = 0; c < 32; ++c) most[c & 3] = fmaxf(most[c & 3], __uint_as_float(raw[h][c]));
         }
+        if (FOLDS && k == take_next) {
+          if (!take_out_sums(j, sum_at, kept)) break;
+          kept = 1.f;
+        }
         const float now = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * unit;
         const bool higher = now > base + FAR || (base == -INFINITY && now > base);
         if (__any_sync(0xffffffffu, higher)) {           // another unit: what there is so far goes by it
           const float keep = !higher ? 1.f : base == -INFINITY ? 0.f : exp2_fast(base - now);
           total *= keep;
+          if (FOLDS) kept *= keep;
           if (higher) base = now;
           if (k > 0) {
             ok = __all_sync(0xffffffffu, bar_wait(&freed[(j - 1) % BUFFERS], ((j - 1) / BUFFERS) & 1, ab));
@@ -640,7 +698,7 @@ template <int DP, int MODE, bool FINE> __global__ void __launch_bounds__(Form<DP
       }
       if (sums_there()) {
         const float inverse = 1.f / total;
-        const bool finite = put_row<WIDE>(sum_at, first_value, inverse, on, w.q.out, row, mine, w.q, lane, nullptr, w.rest);
+        const bool finite = put_row<WIDE>(sum_at, first_value, inverse, on, w.q.out, row, mine, w.q, lane, nullptr, w.rest, taken ? beside : nullptr, kept);
         sums_read(on && !finite);
         if (on && w.q.top) w.q.top[(int64_t)mine * w.q.n + row] = base, w.q.inverse[(int64_t)mine * w.q.n + row] = inverse;
       }
@@ -656,6 +714,7 @@ template <int DP, int MODE, bool FINE> __global__ void __launch_bounds__(Form<DP
         ok = bar_wait(&scores[b], (j / BUFFERS) & 1, ab);
         if (!__all_sync(0xffffffffu, ok)) break;
         tc_fence_after();
+        if (FOLDS && k == take_next && !take_out_sums(j, sum_at + first_value, 1.f)) break;
         const uint32_t word = seen(k * KEYS + 32 * half);
         const bool all = __all_sync(0xffffffffu, word == ~0u);
         uint32_t s[32], d[32], large[16], small[16];
@@ -692,7 +751,7 @@ template <int DP, int MODE, bool FINE> __global__ void __launch_bounds__(Form<DP
         if (lane == 0) bar_arrive(&weights[b]);
       }
       if (sums_there()) {
-        const bool finite = put_row<WIDE>(sum_at, first_value, w.q.scale, on, w.q.dq, row, mine, w.q, lane);
+        const bool finite = put_row<WIDE>(sum_at, first_value, w.q.scale, on, w.q.dq, row, mine, w.q, lane, nullptr, nullptr, taken ? beside : nullptr);
         sums_read(on && !finite);
         // One half leaves its sums where the other's go, whose threads have had delta and wait for it (there is no more shared memory at 128 values).
         float s[2], x[2];
@@ -709,12 +768,14 @@ template <int DP, int MODE, bool FINE> __global__ void __launch_bounds__(Form<DP
     } else {
       const int skip = (int)((group + GROUPS - j0 % GROUPS) % GROUPS);      // the groups take turns over all tiles' steps
       int at = skip % walk.steps * KEYS;
+      take_next += skip;
       const Two minus_units(-unit, -unit), less(-1.f, -1.f);
       for (int k = skip; k < steps; k += GROUPS) {
         const unsigned j = j0 + k, b = j % BUFFERS, slot = 2 * j % SLOTS;
         ok = bar_wait(&full[slot], (2 * j / SLOTS) & 1, ab) && bar_wait(&scores[b], (j / BUFFERS) & 1, ab);
         if (!__all_sync(0xffffffffu, ok)) break;
         tc_fence_after();
+        if (FOLDS && (group == 0 || group == GROUPS - 1) && k == take_next && !take_out_sums(j, group == 0 ? sum_at : sum_at + DP, 1.f)) break;
         const int from = at;
         for (at += GROUPS * KEYS; at >= walk.steps * KEYS;) at -= walk.steps * KEYS;
         const float* num = numbers + slot / 2 * 3 * KEYS;
@@ -780,8 +841,8 @@ template <int DP, int MODE, bool FINE> __global__ void __launch_bounds__(Form<DP
       if ((group == 0 || group == GROUPS - 1) && sums_there()) {
         bool finite = true;
         const float* more = on ? far_of(w, row, tile.kv, span.x, span.y) : nullptr;
-        if (group == 0) finite = put_row<WIDE>(sum_at, first_value, 1.f, on, w.kv.dv, row, tile.kv, w.kv, lane, more ? more + FAR_ROWS * values : nullptr);
-        if (group == GROUPS - 1) finite = put_row<WIDE>(sum_at + DP, first_value, w.q.scale, on, w.kv.dk, row, tile.kv, w.kv, lane, more) && finite;
+        if (group == 0) finite = put_row<WIDE>(sum_at, first_value, 1.f, on, w.kv.dv, row, tile.kv, w.kv, lane, more ? more + FAR_ROWS * values : nullptr, nullptr, taken ? beside : nullptr);
+        if (group == GROUPS - 1) finite = put_row<WIDE>(sum_at + DP, first_value, w.q.scale, on, w.kv.dk, row, tile.kv, w.kv, lane, more, nullptr, taken ? beside : nullptr) && finite;
         sums_read(on && !finite);
       }
     }
@@ -886,12 +947,12 @@ template <int DP, int MODE> int launch(const TcParams& p, cudaStream_t s) {
   // In two parts, dk and dv have no rounding but their own, and a step by columns a fifth more to do.  Where there are no more tiles than SMs, what a call takes is
   // latency, and where few nodes share a chain their roundings do not average out (2-norm of the errors up to 2.6e-3 | 1.7e-3; one chain of 2000 nodes, 8
   // heads of 64: 84 | 89 us of kernels; one chain of 32,781, 128 values, dS alone in two: 1131 | 1180).
-  const bool fine = MODE == COLUMNS && tiles <= sm_count();
-  auto kernel = window_tc_kernel<DP, MODE, false>;
+  const bool fine = MODE == COLUMNS && tiles <= sm_count(), folds = MODE == COLUMNS ? p.w.folds_columns : p.w.folds_rows;
+  auto kernel = folds ? window_tc_kernel<DP, MODE, false, true> : window_tc_kernel<DP, MODE, false, false>;
   if constexpr (MODE == COLUMNS)
-    if (fine) kernel = window_tc_kernel<DP, MODE, true>;
-  static std::atomic<uint64_t> allowed[2]{};
-  if (int rc = allow_shared_once(kernel, F::bytes(), allowed[fine])) return rc;
+    if (fine) kernel = folds ? window_tc_kernel<DP, MODE, true, true> : window_tc_kernel<DP, MODE, true, false>;
+  static std::atomic<uint64_t> allowed[4]{};
+  if (int rc = allow_shared_once(kernel, F::bytes(), allowed[2 * folds + fine])) return rc;
   kernel<<<(unsigned)grid, F::THREADS, F::bytes(), s>>>(t);
   return check_launch("window_tc");
 }

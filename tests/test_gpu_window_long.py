@@ -12,9 +12,12 @@ from equitorch_b200.graph import PackedGraphs
 from equitorch_b200.nn import functional as F
 from equitorch_b200.ops.fused_tp_op import check_status
 
+from .test_gpu_window import compare, make
+from .window_reference import reference, seen
+
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
-SCALES = [-0.125]                                          # tiles of one chain
+SCALES = [0.125, -0.125]                                   # tiles of 128 nodes, and of one chain
 STEP, MARGIN = 2.0 ** -7, 2.0 ** -12
 LOW = 199 / 256                                             # exp(-1/4) in bfloat16
 THIRD = 3 * torch.tensor(1 / 3).bfloat16().item()           # what a third's rounding makes of a sum
@@ -126,3 +129,34 @@ def test_gradients_of_first_nodes_that_many_heads_share(scale):
     nought, one = torch.zeros(n, heads, size, device=DEV), torch.zeros(n, 1, size, device=DEV)
     dv = run(nought, one, one, g, graphs, heads, before, 0, sinks, kv_heads=1, scale=scale)[3]
     assert (dv[0] == 8 * heads * (levels(size).double() + STEP)).all()
+
+
+@pytest.mark.parametrize("scale", SCALES)
+@pytest.mark.parametrize("size,spread", [(64, 1.0), (64, 20.0), (128, 3.0), (24, 1.0)])
+def test_against_float64(size, spread, scale):
+    """Chains of which one is longer than a piece, in windows that are and in windows that are not, with scores that rise behind the first piece."""
+    sizes, heads = (9000, 40, 700, 1), 2
+    n = sum(sizes)
+    qkv, g, graphs = make(sizes, 1, heads, 1, size, torch.bfloat16, seed=size, spread=spread)
+    for window in ((8500, 20, 2), (5000, 4000, 70)):
+        want, bound = reference(*qkv, g, seen(sizes, n, *window), heads, 1, scale)
+        out = F.window_attention(*qkv, graphs, heads, *window, kv_heads=1, scale=scale)
+        compare([out.detach(), *torch.autograd.grad(out, qkv, g)], want, bound)
+
+
+@pytest.mark.parametrize("scale", SCALES)
+@pytest.mark.parametrize("size", [32, 64, 128])
+def test_many_tiles_of_keys_that_many_heads_share(size, scale):
+    """Gradients of keys in pieces of several heads each, in tiles of few and many steps one after the other: the same bits each time."""
+    sizes, heads, window = [3 + (i * 37) % 60 for i in range(30)] + [1500, 2, 400], 64, (150, 30, 3)
+    n = sum(sizes)
+    qkv, g, graphs = make(sizes, 1, heads, 2, size, torch.bfloat16, seed=size)
+
+    def run_it():
+        out = F.window_attention(*qkv, graphs, heads, *window, kv_heads=2, scale=scale)
+        return [out.detach(), *torch.autograd.grad(out, qkv, g)]
+    first = run_it()
+    for _ in range(5):
+        assert all(torch.equal(a, b) for a, b in zip(first, run_it()))
+    want, bound = reference(*qkv, g, seen(sizes, n, *window), heads, 2, scale)
+    compare(first, want, bound)
