@@ -28,19 +28,24 @@ using attention::LOG2E;
 struct WindowParams {
   AttentionParams q, kv;     // of the heads of queries; of the heads of keys (dk and dv)
   int before, after, sinks, group;
-  // Gradients of the first nodes of chains from queries behind their windows, made apart (SPLIT) because a chain may have any number of those: sums of dS q and of P g
+  // Gradients of the first nodes of long chains from queries behind their windows, made apart (SPLIT) because a chain may have any number of those: sums of dS q and of P g
   // by blocks of FAR_BLOCK nodes of the batch, [pair of a block and a chain][head of keys][16 first nodes][dk, dv][node][value], then joined in the chain's first place.
   void* rest;                // what the rounding of the results left (bfloat16, for the backward pass)
   float* inverse;            // [head][node]: one over the sum of weights as the columns have them, not rounded
   const int64_t* ptr;
   int64_t chains;
   float* far;
-  int split;
+  int split, apart;          // apart: nodes of a chain from which it is such a long one, none where not SPLIT
   int folds_rows, folds_columns;   // bfloat16: sums of results and dq, and of dk and dv, of more than FOLD terms
 };
 constexpr int FAR_BLOCK = 512, FAR_ROWS = 16, MOST_SPLIT_SINKS = 64;
 __host__ __device__ inline int far_groups(const WindowParams& p) { return (p.sinks + FAR_ROWS - 1) / FAR_ROWS; }
-// A block b and a chain g that has nodes in it are pair b + g, which no other two are: going on, either the block or the chain moves by one.
+// Chains of at least that many nodes start so far from one another that no two have the same slot, start / far_length, so places go by the nodes and not by the chains, of which
+// a batch may have any number; a block b and a chain of slot g that has nodes in it are pair b + g, which no other two are: going on, the block or the slot moves on.
+__host__ __device__ inline int far_length(const WindowParams& p) { return p.before + 1 + FAR_BLOCK; }
+__host__ __device__ inline int64_t far_slots(const WindowParams& p) { return p.q.n / far_length(p) + 1; }
+__host__ __device__ inline int64_t far_pairs(const WindowParams& p) { return (p.q.n + FAR_BLOCK - 1) / FAR_BLOCK + far_slots(p); }
+__device__ __forceinline__ bool apart(const WindowParams& p, int lo, int hi) { return hi - lo >= p.apart; }
 __device__ __forceinline__ int64_t far_place(const WindowParams& p, int64_t pair, int kv, int group) {
   return ((pair * p.kv.heads + kv) * far_groups(p) + group) * (2 * FAR_ROWS * (int64_t)(p.q.comps * p.q.size));
 }
@@ -56,10 +61,9 @@ template <typename F> __device__ __forceinline__ int64_t last_chain(int64_t chai
 }
 // What queries behind its window give a first node j of the chain [lo, hi): dk, with dv FAR_ROWS rows on; none: NULL.
 __device__ __forceinline__ const float* far_of(const WindowParams& p, int j, int kv, int lo, int hi) {
-  if (!p.split || j >= lo + p.sinks || j + p.before + 1 >= hi) return nullptr;
-  const int64_t g = last_chain(p.chains, j, [&](int64_t c) { return p.ptr[c]; });
+  if (!apart(p, lo, hi) || j >= lo + p.sinks || j + p.before + 1 >= hi) return nullptr;
   const int group = (j - lo) / FAR_ROWS, first = lo + group * FAR_ROWS;
-  return p.far + far_place(p, (first + p.before + 1) / FAR_BLOCK + g, kv, group) + (int64_t)(j - first) * (p.q.comps * p.q.size);
+  return p.far + far_place(p, (first + p.before + 1) / FAR_BLOCK + lo / far_length(p), kv, group) + (int64_t)(j - first) * (p.q.comps * p.q.size);
 }
 
 __device__ __forceinline__ bool sees(const WindowParams& p, int i, int j, int lo) { return j <= i + p.after && (j >= i - p.before || j < lo + p.sinks); }

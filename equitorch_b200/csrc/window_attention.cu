@@ -39,10 +39,12 @@ WindowParams params(const eqt_window_attention_args& a) {
   p.kv = q;
   p.kv.heads = a.kv_heads;
   // A tile of keys that holds a chain's first nodes would walk to the chain's end, alone, while the others are done (one chain of 32,781 nodes, 8 heads of 128
-  // values, window of 1024: by columns 876 us; with these queries apart 473 and 62 for them).  Two launches more, so not for what is walked in a few steps (240
-  // chains of 50 to 500 nodes, window of 64 on both sides: 217 us walked, 164 and 61 apart); and not for so many first nodes that tiles are full of them.
+  // values, window of 1024: by columns 876 us; with these queries apart 473 and 62 for them).  Two launches more, so not for batches whose chains are all walked in a few steps (240
+  // chains of 50 to 500 nodes, window of 64 on both sides: 217 us walked, 164 and 61 apart), nor for such chains beside a longer one (`apart`), which would take scratch each;
+  // and not for so many first nodes that tiles are full of them.
   p.ptr = a.ptr, p.chains = a.num_graphs, p.rest = a.dtype == EQT_BF16 ? a.rest : nullptr;
   p.split = p.sinks > 0 && p.sinks <= MOST_SPLIT_SINKS && a.longest - p.before > 2 * FAR_BLOCK;
+  p.apart = p.split ? far_length(p) : INT32_MAX;
   if (a.dtype == EQT_BF16) {
     const int64_t window = std::min<int64_t>((int64_t)p.before + p.after + 1, reach);
     p.folds_rows = std::min<int64_t>(window + p.sinks, reach) > attention::FOLD;
@@ -67,8 +69,7 @@ int64_t delta_bytes(const eqt_window_attention_args& a) { return (int64_t)up((si
 int64_t scratch_bytes(const eqt_window_attention_args& a, bool backward) {
   if (!backward) return spans_bytes(a);
   const WindowParams p = params(a);
-  const int64_t pairs = ceil_div(a.n, FAR_BLOCK) + a.num_graphs;
-  return spans_bytes(a) + 2 * delta_bytes(a) + (p.split ? pairs * a.kv_heads * far_groups(p) * 2 * FAR_ROWS * a.comps * a.head_channels * 4 : 0);
+  return spans_bytes(a) + 2 * delta_bytes(a) + (p.split ? far_pairs(p) * a.kv_heads * far_groups(p) * 2 * FAR_ROWS * a.comps * a.head_channels * 4 : 0);
 }
 int check_scratch(const eqt_window_attention_args& a, bool backward) {
   const int64_t need = scratch_bytes(a, backward);

@@ -156,7 +156,7 @@ template <int MODE> __device__ __forceinline__ Stretch stretch_of(const WindowPa
   s.to1 = last + 1;
   if (MODE == COLUMNS) {
     if (a.y > a.x) s.from1 = max(a.x, first - w.after);
-    if (b.y > b.x) s.to1 = !w.split && max(b.x, first) < b.x + w.sinks ? b.y : min(b.y, last + w.before + 1);
+    if (b.y > b.x) s.to1 = !apart(w, b.x, b.y) && max(b.x, first) < b.x + w.sinks ? b.y : min(b.y, last + w.before + 1);
   } else {
     if (a.y > a.x) {
       s.from1 = max(a.x, first - w.before);
@@ -596,7 +596,7 @@ template <int DP, int MODE, bool FINE, bool FOLDS> __global__ void __launch_boun
     const int steps = walk.steps * (MODE == COLUMNS ? w.group : 1);
     // what the row sees: [lo, hi), and the first nodes [span.x, far)
     const int lo = !on ? 0 : max(span.x, row - (MODE == COLUMNS ? w.after : w.before));
-    const int hi = !on ? 0 : MODE == COLUMNS ? (!w.split && row < span.x + w.sinks ? span.y : min(span.y, row + w.before + 1)) : min(span.y, row + w.after + 1);
+    const int hi = !on ? 0 : MODE == COLUMNS ? (!apart(w, span.x, span.y) && row < span.x + w.sinks ? span.y : min(span.y, row + w.before + 1)) : min(span.y, row + w.after + 1);
     const int far = on && MODE != COLUMNS ? min(lo, span.x + w.sinks) : 0;
     // as bits of the 32 from the stretch's `at`-th on; first nodes are before `from1`, or in the stretch behind it, or both
     auto seen = [&](int at) {
@@ -922,8 +922,10 @@ template <int DP, int MODE> int launch(const TcParams& p, cudaStream_t s) {
   using F = Form<DP, MODE>;
   const int64_t tiles = MODE == COLUMNS ? ceil_div(p.w.q.n, TILE_M) * p.w.kv.heads : ceil_div(p.w.q.n, TILE_M / p.pack) * (p.w.q.heads / p.pack);
   if (tiles > INT32_MAX) return fail(EQT_ERR_UNSUPPORTED, "window_attention: %lld tiles are more than one launch takes", (long long)tiles);
-  // Tiles of a CTA are settled beforehand, which is for even ones: by columns, those with first nodes walk further (217 us with a CTA each, 234 so; of even ones 470 and 416).
-  const bool even = MODE != COLUMNS || p.w.sinks == 0 || p.w.split;
+  // Tiles of a CTA are settled beforehand, which is for even ones: by columns, those with first nodes walk further (217 us with a CTA each, 234 so; of even ones 470
+  // and 416; one chain of 32,781 and 400 of 300: 447 and 561), unless chains are on average so short that it is not far (100,000 chains of 20: 7970 and 5620 us) or so long
+  // that they are taken apart.
+  const bool even = MODE != COLUMNS || p.w.sinks == 0 || p.w.q.n / TILE_M <= p.w.chains || (p.w.split && p.w.q.n / p.w.apart >= p.w.chains);
   const int64_t grid = even ? std::min<int64_t>(tiles, std::max<int64_t>((int64_t)sm_count() * F::CTAS, ceil_div(tiles, MOST_TILES))) : tiles;
   TcParams t = p;
   t.tiles = (unsigned)tiles;

@@ -41,7 +41,7 @@ __device__ __forceinline__ Walk queries_of(const WindowParams& p, int first, int
   Walk w;
   w.from0 = w.to0 = lo;
   w.from1 = max(lo, first - p.after);
-  w.to1 = first < lo + p.sinks && !p.split ? hi : min(hi, last + p.before);
+  w.to1 = first < lo + p.sinks && !apart(p, lo, hi) ? hi : min(hi, last + p.before);
   return w;
 }
 
@@ -312,6 +312,7 @@ __global__ void __launch_bounds__(THREADS, DP <= 64 ? 3 : 2) window_columns_kern
   Walk walk = queries_of(p, first, last, lo, hi);
   walk.set<KT>();
   const int steps = walk.steps * p.group;                // the heads one after the other
+  const bool far_apart = apart(p, lo, hi);
   auto fetch = [&](int step, int s) {
     int end;
     const int i = walk.at<KT>(step % walk.steps, end), head = here ? kv * p.group + step / walk.steps : 0;
@@ -365,7 +366,7 @@ __global__ void __launch_bounds__(THREADS, DP <= 64 ? 3 : 2) window_columns_kern
         for (int i = 0; i < 4; ++i) {
           const int c = n * 8 + 2 * t + (i & 1), q = query + c;
           const int j = row + g + 8 * (i >> 1);
-          const bool on = q < end && sees(p, q, j, lo) && (!p.split || q <= j + p.before);
+          const bool on = q < end && sees(p, q, j, lo) && (!far_apart || q <= j + p.before);
           z[n][i] = on ? exp2_fast(z[n][i] * unit - num[c]) * num[KT + c] : 0.f;
           dp[n][i] = on ? z[n][i] * (dp[n][i] - num[2 * KT + c]) : 0.f;
         }
@@ -380,7 +381,7 @@ __global__ void __launch_bounds__(THREADS, DP <= 64 ? 3 : 2) window_columns_kern
       unfold<DP>(waiting_k.at(), dk);
       unfold<DP>(waiting_v.at(), dv);
     }
-  if (p.split && row < lo + p.sinks) {
+  if (far_apart && row < lo + p.sinks) {
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const int j = row + g + 8 * r, values = p.q.comps * p.q.size;
@@ -411,15 +412,16 @@ template <typename T, int DP, int KT, bool FOLDS> __global__ void __launch_bound
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ int64_t chain;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3, kv = blockIdx.y, values = p.q.comps * p.q.size;
-  if (tid == 0) chain = last_chain(p.chains, blockIdx.x, [&](int64_t c) { return p.ptr[c] / FAR_BLOCK + c; });
+  // The only chain that may be that pair's: what comes behind a long chain has a greater number than its last pair.
+  if (tid == 0) chain = last_chain(p.chains, blockIdx.x, [&](int64_t c) { return p.ptr[c] / FAR_BLOCK + p.ptr[c] / far_length(p); });
   if (values < DP)
     for (size_t i = tid; i < S::bytes(2, 0) / 16; i += THREADS) reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
   __syncthreads();
   if (chain < 0) return;
   const int lo = (int)p.ptr[chain], hi = (int)p.ptr[chain + 1];
-  const int64_t block = blockIdx.x - chain;
+  const int64_t block = blockIdx.x - lo / far_length(p);
   const int first = lo + (int)blockIdx.z * FAR_ROWS, last = min(min(lo + p.sinks, hi), first + FAR_ROWS);
-  if (hi <= lo || block > (hi - 1) / FAR_BLOCK || first >= last) return;
+  if (!apart(p, lo, hi) || block > (hi - 1) / FAR_BLOCK || first >= last) return;
   const int from = max((int)(block * FAR_BLOCK), first + p.before + 1), to = (int)min((block + 1) * FAR_BLOCK, (int64_t)hi);
   if (from >= to) return;
   T *keys = reinterpret_cast<T*>(smem) + warp * S::head_elements(2), *vals = keys + 16 * LD, *stage = vals + 16 * LD;
@@ -502,15 +504,19 @@ template <typename T, int DP, int KT, bool FOLDS> __global__ void __launch_bound
   float* out = p.far + far_place(p, blockIdx.x, kv, blockIdx.z);
   for (int i = tid; i < 2 * FAR_ROWS * values; i += THREADS) out[i] = sums[i / values * DP + i % values];
 }
-// The blocks of a chain, in their order, into its first one: a thread has one number.
+// The blocks of a slot's chain, in their order, into its first one: a thread has one number.
 __global__ void __launch_bounds__(256) window_far_join_kernel(const __grid_constant__ WindowParams p, int groups) {
-  const int64_t chain = blockIdx.x;
+  __shared__ int64_t found;
+  if (threadIdx.x == 0) found = last_chain(p.chains, blockIdx.x, [&](int64_t c) { return p.ptr[c] / far_length(p); });
+  __syncthreads();
+  const int64_t chain = found;
+  if (chain < 0) return;
   const int group = blockIdx.z % groups, at = blockIdx.z / groups * 256 + threadIdx.x;
   const int lo = (int)p.ptr[chain], hi = (int)p.ptr[chain + 1], first = lo + group * FAR_ROWS;
-  if (hi <= lo || first >= lo + p.sinks || first + p.before + 1 >= hi || at >= 2 * FAR_ROWS * p.q.comps * p.q.size) return;
+  if (!apart(p, lo, hi) || lo / far_length(p) != blockIdx.x || first >= lo + p.sinks || first + p.before + 1 >= hi || at >= 2 * FAR_ROWS * p.q.comps * p.q.size) return;
   const int64_t begin = (first + p.before + 1) / FAR_BLOCK, end = (hi - 1) / FAR_BLOCK;
   const int64_t step = far_place(p, 1, 0, 0);
-  float* to = p.far + far_place(p, begin + chain, blockIdx.y, group) + at;
+  float* to = p.far + far_place(p, begin + blockIdx.x, blockIdx.y, group) + at;
   float sum = 0.f;
 #pragma unroll 16
   for (int64_t b = 0; b <= end - begin; ++b) sum += to[b * step];
@@ -521,8 +527,7 @@ __global__ void __launch_bounds__(256) window_far_join_kernel(const __grid_const
 template <typename T, int DP> int launch_far(const WindowParams& p, cudaStream_t s) {
   constexpr int KT = DP > 32 ? 16 : 32;
   using S = attention::Shape<T, DP, 1, KT>;
-  const int64_t pairs = ceil_div(p.q.n, FAR_BLOCK) + p.chains;
-  if (pairs > INT32_MAX || p.kv.heads > 65535) return fail(EQT_ERR_UNSUPPORTED, "window_attention: %lld chains are more than one launch takes", (long long)p.chains);
+  const int64_t pairs = far_pairs(p);                    // fewer than 2^22
   const size_t shared = S::bytes(2, WARPS * 6 * KT * 4);
   auto kernel = window_far_kernel<T, DP, KT, false>;
   bool folds = false;                                    // a warp has a quarter of a block's queries of all heads
@@ -535,7 +540,7 @@ template <typename T, int DP> int launch_far(const WindowParams& p, cudaStream_t
   kernel<<<dim3((unsigned)pairs, (unsigned)p.kv.heads, (unsigned)far_groups(p)), THREADS, shared, s>>>(p);
   if (int rc = check_launch("window_far")) return rc;
   const int groups = far_groups(p), chunks = (int)ceil_div(2 * FAR_ROWS * p.q.comps * p.q.size, 256);
-  window_far_join_kernel<<<dim3((unsigned)p.chains, (unsigned)p.kv.heads, (unsigned)(groups * chunks)), 256, 0, s>>>(p, groups);
+  window_far_join_kernel<<<dim3((unsigned)far_slots(p), (unsigned)p.kv.heads, (unsigned)(groups * chunks)), 256, 0, s>>>(p, groups);
   return check_launch("window_far_join");
 }
 template <typename T> int far(const WindowParams& p, cudaStream_t s) {

@@ -21,3 +21,14 @@ def test_long_windows_of_bfloat16_need_the_highest_tiles_of_one_chain():
     for rows in (16, 32):
         assert lib.eqt_window_attention_forward(C.byref(window(tile_rows=rows)), None) == 2
         assert lib.eqt_window_attention_backward(C.byref(window(tile_rows=rows)), None) == 2
+
+
+def test_scratch_goes_by_the_nodes_and_not_by_the_chains():
+    """Of first nodes' gradients: one long chain among many."""
+    chains = 100_000
+    n = 4000 + 20 * chains
+    for sinks, groups in ((4, 1), (64, 4)):
+        for dtype in (torch.float32, torch.bfloat16):
+            args = window(dtype=_lib.DTYPE_CODE[dtype], n=n, num_graphs=chains + 1, longest=4000, heads=8, kv_heads=8, head_channels=64, before=30, sinks=sinks)
+            size = _lib.lib().eqt_window_attention_scratch(C.byref(args), 1)
+            assert size <= n * (8 + 2 * 8 * 4 + 0.55 * groups * 8 * 64) + 2 ** 20
