@@ -10,7 +10,8 @@
 //
 // Where a weight is almost one, dP - delta is what two such numbers leave, and delta has to be that of the very weights: sum_j P_ij dP_ij.  bfloat16 weights are
 // rounded for their product with v, so the forward pass divides by the sum of the rounded ones and keeps what the rounding of its result left; the rows' pass takes
-// the same rounded weights, whose delta is <g, out + rest>.  On its way it sums P, and P dP, of the weights before rounding, by which the columns go.
+// the same rounded weights, whose delta is <g, out + rest>.  The forward pass rounds a weight in the unit that its row has at that moment,
+// so a row's units differ by whole powers of two.  On its way it sums P, and P dP, of the weights before rounding, by which the columns go.
 //
 // A tile's products run over nodes that some of its rows do not see, with weights of zero, and zero times infinity or a NaN is a NaN.  So a row whose
 // result is not finite is done again, one visible node at a time (`again_*`): a NaN that is not seen does not reach it, and one that is seen does.

@@ -654,10 +654,11 @@ template <int DP, int MODE, bool FINE, bool FOLDS> __global__ void __launch_boun
         const float now = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * unit;
         const bool higher = now > base + FAR || (base == -INFINITY && now > base);
         if (__any_sync(0xffffffffu, higher)) {           // another unit: what there is so far goes by it
-          const float keep = !higher ? 1.f : base == -INFINITY ? 0.f : exp2_fast(base - now);
+          const float unit_now = base == -INFINITY ? now : base + ceilf(now - base);         // by whole steps: the rounding of a weight is the same in any unit of a row
+          const float keep = !higher ? 1.f : base == -INFINITY ? 0.f : exp2_fast(base - unit_now);
           total *= keep;
           if (FOLDS) kept *= keep;
-          if (higher) base = now;
+          if (higher) base = unit_now;
           if (k > 0) {
             ok = __all_sync(0xffffffffu, bar_wait(&freed[(j - 1) % BUFFERS], ((j - 1) / BUFFERS) & 1, ab));
             if (!ok) break;

@@ -142,6 +142,7 @@ __global__ void __launch_bounds__(THREADS, DP <= 64 ? 4 : 3) window_forward_kern
 #pragma unroll
         for (int n = 0; n < NT; ++n) most = fmaxf(most, fmaxf(z[n][2 * r], z[n][2 * r + 1]));
         most = quad_max(most);
+        if (sizeof(T) == 2 && most > top[r] && top[r] > -INFINITY) most = top[r] + ceilf(most - top[r]);         // whole steps: a weight's rounding is the same in any unit
         const float base = most == -INFINITY ? 0.f : most, keep = exp2_fast(top[r] - base);
         float add = 0.f;
 #pragma unroll

@@ -765,7 +765,7 @@ int eqt_window_step(const eqt_window_step_args* args, void* stream);
  * bfloat16; at most 128 values (comps * head_channels) a head.  Head h has the keys of head h / (heads / kv_heads).
  *   s_ij = scale <q_i, k_j>,   out_i = sum_j softmax_j(s_ij) v_j;   rows of nodes that belong to no chain are zero, their gradients too
  * rest (as out; may be NULL with stats NULL, and for float32): what the rounding of out left, for the backward pass, whose sum_j P_ij dP_ij is <grad_i, out_i + rest_i>.
- * stats (2, heads, n): a row's greatest score in units of log2 and one over its sum of weights from there, needed for the backward pass.  tiles: as for eqt_attention_forward.  scratch:
+ * stats (2, heads, n): what is taken off a row's scores, in units of log2, and one over its sum of weights from there, needed for the backward pass.  tiles: as for eqt_attention_forward.  scratch:
  * eqt_window_attention_scratch bytes, 16-byte aligned; status as for eqt_gated_forward.  Backward: grad contiguous; all three gradients are written; no atomics. */
 typedef struct {
   int32_t dtype, comps, heads, kv_heads, head_channels, tile_rows;
