@@ -189,6 +189,14 @@ __global__ void __launch_bounds__(ROW_THREADS < 128 ? 128 : ROW_THREADS, OUT != 
     for (int j = 0; j < V; ++j) c[i][j] = 1.f;
     if (p.w && k < pieces) unpack<T>(reinterpret_cast<const uint4*>(p.w)[k % (p.channels / V)], c[i]);
   }
+  bool bad_weight = false;                               // one that is not finite: no scale is a number then
+  if constexpr (OUT != 0) {
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) bad_weight = bad_weight || !(fabsf(c[i][j]) < INFINITY);
+    bad_weight = __syncthreads_or(bad_weight);
+  }
   int turn = 0;
   constexpr bool AHEAD = PIECES <= 2;                    // the next row is on its way while this one is worked on
   uint4 x[PIECES], r[PIECES], next_x[PIECES], next_r[PIECES];
@@ -230,7 +238,8 @@ __global__ void __launch_bounds__(ROW_THREADS < 128 ? 128 : ROW_THREADS, OUT != 
 #pragma unroll
       for (int j = 0; j < V; ++j) sum = fmaf(h[i][j], h[i][j], sum);
     }
-    const float inverse = inverse_root(across_row<ROW_THREADS>(sum, buffer[turn], Sum()), p.length, p.eps);
+    sum = across_row<ROW_THREADS>(sum, buffer[turn], Sum());
+    const float inverse = inverse_root(sum, p.length, p.eps);
     if (p.rstd && at == 0 && there) p.rstd[row] = inverse;
     if (RES && p.total) {
 #pragma unroll
@@ -311,7 +320,7 @@ __global__ void __launch_bounds__(ROW_THREADS < 128 ? 128 : ROW_THREADS, OUT != 
         } else if constexpr (V == 8) *reinterpret_cast<uint2*>(to_values) = make_uint2(held[i][0] | (uint32_t)held[i][1] << 16, held[i][2] | (uint32_t)held[i][3] << 16);
         else
           *reinterpret_cast<uint32_t*>(to_values) = held[i][0] | (uint32_t)held[i][1] << 16;
-        const float scale = scale_of(most[i], inverse);
+        const float scale = bad_weight || !(sum < INFINITY) ? NAN : scale_of(most[i], inverse);
         if (OUT == 2 && k % lanes == 0) p.scales[(first + k) / lanes] = scale;
         if (OUT == 1 && k == 0) p.scales[row] = scale;
       }
@@ -432,6 +441,12 @@ template <typename T, bool EIGHT> __global__ void __launch_bounds__(LONG_THREADS
   __shared__ float buffer[2][LONG_THREADS / 32], most_of[2][LONG_THREADS / 32];
   __shared__ double exact_of[2][LONG_THREADS / 32];
   const T *x = static_cast<const T*>(p.x), *res = static_cast<const T*>(p.res), *w = static_cast<const T*>(p.w);
+  bool bad_weight = false;
+  if constexpr (EIGHT) {
+    if (w)
+      for (int k = threadIdx.x; k < p.channels; k += LONG_THREADS) bad_weight = bad_weight || !(fabsf(ld(w + k)) < INFINITY);
+    bad_weight = __syncthreads_or(bad_weight);
+  }
   int turn = 0;
   for (int64_t row = blockIdx.x; row < p.n; row += gridDim.x, turn ^= 1) {
     const int64_t first = row * p.length;
@@ -443,7 +458,8 @@ template <typename T, bool EIGHT> __global__ void __launch_bounds__(LONG_THREADS
       const float h = value(k);
       sum = fmaf(h, h, sum);
     }
-    const float inverse = inverse_root(across_row<LONG_THREADS>(sum, buffer[turn], Sum()), p.length, p.eps);
+    sum = across_row<LONG_THREADS>(sum, buffer[turn], Sum());
+    const float inverse = inverse_root(sum, p.length, p.eps);
     if (p.rstd && threadIdx.x == 0) p.rstd[row] = inverse;
     if constexpr (!EIGHT) {
       for (int k = threadIdx.x; k < p.length; k += LONG_THREADS) {
@@ -483,7 +499,7 @@ template <typename T, bool EIGHT> __global__ void __launch_bounds__(LONG_THREADS
           p.values[first + k] = held;
           if (res && p.total) st(static_cast<T*>(p.total) + first + k, h);
         }
-        if (whole ? threadIdx.x == 0 : lane == 0) p.scales[row * (p.length / p.group) + start / p.group] = scale_of(most, inverse);
+        if (whole ? threadIdx.x == 0 : lane == 0) p.scales[row * (p.length / p.group) + start / p.group] = bad_weight || !(sum < INFINITY) ? NAN : scale_of(most, inverse);
       }
     }
   }

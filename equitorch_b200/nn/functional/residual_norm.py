@@ -55,8 +55,8 @@ def add_rms_norm_e4m3(x: Tensor, residual: Optional[Tensor] = None, weight: Opti
     """:func:`add_rms_norm` for a product in 8 bits at inference: ``values`` (float8_e4m3fn, of the shape of ``x``), ``scales`` (float32,
     ``(N, groups)``) and the sum.  Every ``group`` values of a node (a divisor of components times channels; all of them where not given) share a
     scale, which brings the greatest of them to 448, the greatest number of the type; ``out = values * scale``.  The values are the nearest
-    to the exact quotients, ties to even.  A group of zeros has the scale zero.  Values or weights that are not finite make the node's scales
-    NaN.  No gradients: inputs that need one are refused while gradients are recorded."""
+    to the exact quotients, ties to even.  A group of zeros has the scale zero.  Values that are not finite, or whose squares' sum is not in
+    float32, make all of the node's scales NaN, weights that are not finite all nodes'.  No gradients: inputs that need one are refused while gradients are recorded."""
     _ops.check(x, residual, weight, eps)
     values = x.shape[-1] * (x.shape[1] if x.ndim == 3 else 1)
     if group is not None and (group < 1 or values % group):
