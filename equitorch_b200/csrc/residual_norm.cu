@@ -591,6 +591,9 @@ unsigned part_ctas(int threads, int64_t n) {
 // Parts of the rows where they are read by loops.
 int64_t long_parts(int64_t n) { return std::min<int64_t>(ceil_div(n, 16), 128); }
 
+int check_eps(double eps) {
+  return (float)eps > 0.f && (float)eps < INFINITY ? EQT_OK : fail(EQT_ERR_BAD_ARGUMENT, "add_rms_norm: eps of %g is no positive float32", eps);
+}
 int check(int dtype, int64_t n, int64_t comps, int64_t channels) {
   if (dtype != EQT_F32 && dtype != EQT_BF16) return fail(EQT_ERR_BAD_ARGUMENT, "add_rms_norm: unknown dtype %d", dtype);
   if (n < 0 || comps < 0 || channels < 0) return fail(EQT_ERR_BAD_ARGUMENT, "add_rms_norm: negative size");
@@ -651,6 +654,7 @@ using namespace eqt::residual_norm;
 extern "C" int eqt_add_rms_norm_forward(int32_t dtype, const void* x, const void* residual, const void* weight, void* out, void* total, float* rstd,
                                         int64_t n, int64_t comps, int64_t channels, double eps, void* stream) {
   if (int rc = check(dtype, n, comps, channels)) return rc;
+  if (int rc = check_eps(eps)) return rc;
   if (n == 0 || comps * channels == 0) return EQT_OK;
   if (!x || !out) return fail(EQT_ERR_BAD_ARGUMENT, "add_rms_norm: NULL pointer");
   NormArgs p{};
@@ -664,6 +668,7 @@ extern "C" int eqt_add_rms_norm_forward(int32_t dtype, const void* x, const void
 extern "C" int eqt_add_rms_norm_e4m3(int32_t dtype, const void* x, const void* residual, const void* weight, void* values, float* scales, void* total,
                                      int64_t n, int64_t comps, int64_t channels, int64_t group, double eps, void* stream) {
   if (int rc = check(dtype, n, comps, channels)) return rc;
+  if (int rc = check_eps(eps)) return rc;
   if (n == 0 || comps * channels == 0) return EQT_OK;
   if (!x || !values || !scales) return fail(EQT_ERR_BAD_ARGUMENT, "add_rms_norm: NULL pointer");
   if (group < 1 || (comps * channels) % group) return fail(EQT_ERR_BAD_ARGUMENT, "add_rms_norm: rows of %lld values are no groups of %lld", (long long)(comps * channels), (long long)group);

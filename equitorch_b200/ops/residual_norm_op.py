@@ -1,7 +1,6 @@
 """Root-mean-square norm with the residual's addition (operator layer over ``eqt_add_rms_norm_forward`` / ``_e4m3`` / ``_backward``)."""
 from __future__ import annotations
 
-import math
 from typing import Optional, Tuple
 
 import torch
@@ -22,8 +21,8 @@ def check(x: Tensor, residual: Optional[Tensor], weight: Optional[Tensor], eps: 
     for what, t in (("residual", residual), ("weight", weight)):
         if t is not None and t.dtype != x.dtype:
             raise TypeError(f"{what} of type {t.dtype} for features of type {x.dtype}")
-    if not (0 < eps and math.isfinite(eps)):
-        raise ValueError(f"eps must be positive, got {eps}")
+    if not 1e-45 <= eps <= 3.4e38:                        # what float32 has
+        raise ValueError(f"eps must be a positive float32, got {eps}")
     _lib.require_cuda(x, residual, weight)
 
 

@@ -33,3 +33,11 @@ def test_a_weight(value, shape, group, dtype):
     w[5] = value
     _, scales, _ = F.add_rms_norm_e4m3(x, None, w, group=group)
     assert torch.isnan(scales).all()
+
+
+def test_the_least_eps():
+    """Of what float32 has below its normal numbers."""
+    x = torch.zeros(3, 1, 64, device=DEV)
+    out, _ = F.add_rms_norm(x, None, None, 1.5e-45)
+    values, scales, _ = F.add_rms_norm_e4m3(x, None, None, 1.5e-45)
+    assert not out.any() and not values.float().any() and not scales.any()
