@@ -524,16 +524,16 @@ template <typename T> __global__ void __launch_bounds__(LONG_THREADS) backward_l
 // The weight's gradient of such rows: a thread has a place of the row, a CTA a part of the rows.
 template <typename T> __global__ void __launch_bounds__(LONG_THREADS) weight_long_kernel(const NormArgs p, int64_t part_rows) {
   const T *g = static_cast<const T*>(p.g), *total = static_cast<const T*>(p.total), *res = static_cast<const T*>(p.res);
-  const int k = blockIdx.y * LONG_THREADS + threadIdx.x;
+  const int k = blockIdx.x * LONG_THREADS + threadIdx.x;          // a row may have more pieces than a grid's y
   if (k >= p.length) return;
-  const int64_t end = min(p.n, (int64_t)(blockIdx.x + 1) * part_rows);
+  const int64_t end = min(p.n, (int64_t)(blockIdx.y + 1) * part_rows);
   float sum = 0.f;
 #pragma unroll 4
-  for (int64_t row = blockIdx.x * part_rows; row < end; ++row) {
+  for (int64_t row = blockIdx.y * part_rows; row < end; ++row) {
     const int64_t at = row * p.length + k;
     sum = fmaf(ld(g + at), (ld(total + at) + (res ? ld(res + at) : 0.f)) * __ldg(p.rstd + row), sum);
   }
-  p.parts[(int64_t)blockIdx.x * p.length + k] = sum;
+  p.parts[(int64_t)blockIdx.y * p.length + k] = sum;
 }
 
 // dw[c] = the parts' sums over the components: a CTA has eight channels, 64 slices of the parts each
@@ -630,7 +630,7 @@ template <typename T> int launch_backward(const NormArgs& p, Rows r, cudaStream_
     if (int rc = check_launch("add_rms_norm_backward")) return rc;
     if (!p.parts) return EQT_OK;
     parts = (int)long_parts(p.n);
-    weight_long_kernel<T><<<dim3((unsigned)parts, (unsigned)ceil_div(p.length, LONG_THREADS)), LONG_THREADS, 0, s>>>(p, ceil_div(p.n, parts));
+    weight_long_kernel<T><<<dim3((unsigned)ceil_div(p.length, LONG_THREADS), (unsigned)parts), LONG_THREADS, 0, s>>>(p, ceil_div(p.n, parts));
     if (int rc = check_launch("add_rms_norm_weight")) return rc;
   }
   if (!p.parts) return EQT_OK;
