@@ -238,7 +238,7 @@ int fill(StepArgs& p, const eqt_window_step_args* a) {
   if (a->chains < 0 || a->capacity < 0 || a->before < 0 || a->sinks < 0 || a->heads < 1 || a->kv_heads < 1 || a->comps < 1 || a->head_channels < 1 ||
       a->heads % a->kv_heads)
     return fail(EQT_ERR_BAD_ARGUMENT, "window_step: sizes");
-  if ((int64_t)a->comps * a->head_channels > MOST_VALUES || a->chains > 65535 || a->heads > 65535 || a->capacity > INT32_MAX || a->before > INT32_MAX ||
+  if ((int64_t)a->comps * a->head_channels > MOST_VALUES || a->chains > 65535 || a->heads > 65535 || a->capacity > INT32_MAX - 64 || a->before > INT32_MAX ||
       a->sinks > INT32_MAX)
     return fail(EQT_ERR_UNSUPPORTED, "window_step: at most %d values a head, 65535 chains and heads, 2^31 nodes a chain", MOST_VALUES);
   const int v = a->dtype == EQT_F32 ? 4 : 8;

@@ -32,3 +32,10 @@ def test_scratch_goes_by_the_nodes_and_not_by_the_chains():
             args = window(dtype=_lib.DTYPE_CODE[dtype], n=n, num_graphs=chains + 1, longest=4000, heads=8, kv_heads=8, head_channels=64, before=30, sinks=sinks)
             size = _lib.lib().eqt_window_attention_scratch(C.byref(args), 1)
             assert size <= n * (8 + 2 * 8 * 4 + 0.55 * groups * 8 * 64) + 2 ** 20
+
+
+def test_a_cache_whose_places_do_not_fit_32_bits():
+    """Numbers of keys go a step beyond the capacity."""
+    step = dict(dtype=0, comps=1, heads=1, kv_heads=1, head_channels=1, scale=1.0, chains=1, capacity=2 ** 31 - 1, before=2 ** 31 - 1, sinks=0, q=16, k=16, v=16, out=16, lengths=16,
+                scratch=16, scratch_floats=2 ** 40)
+    assert _lib.lib().eqt_window_step(C.byref(_lib.WindowStepArgs(**step)), None) == 2
