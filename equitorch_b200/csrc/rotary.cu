@@ -6,10 +6,10 @@
 // node's features turn alike, so that rotations of space and these commute.  The gradient is the same with -t.
 //
 // Bound by HBM: every value is read and written once.  A CTA's angles go to shared memory as (cos, sin), each computed once for all heads and
-// components of q and k, in float64 up to what is left of whole turns (the product of a position of a million and a frequency has no
-// place in float32: half an ulp of it is 0.03 of a radian).  A thread has the same piece of a head of four nodes in registers, on their way while the angles
+// components of q and k, in pairs of float64 up to what is left of whole turns, for any position (the product of a position of a million and a frequency has no
+// place in float32: half an ulp of it is 0.03 of a radian; one of 2^40 loses 2e-4 in float64).  A thread has the same piece of a head of four nodes in registers, on their way while the angles
 // are made: two times 16 bytes of both halves, or 16 bytes of neighbouring pairs; single values where these do not lie on 16-byte boundaries.
-// 65,536 nodes, 8 and 2 heads of 64 bfloat16 values: 33 us (5.1 TB/s) each way.
+// 65,536 nodes, 8 and 2 heads of 64 bfloat16 values: 34 us (4.9 TB/s) each way, 33.5 with angles in single float64 numbers.
 #include <algorithm>
 
 #include "common.cuh"
@@ -33,8 +33,21 @@ struct RotaryArgs {
   int64_t n;
   int comps, size, half, sides, units;                   // units: pieces of a head
   float magnitude;
-  double turns;                                          // one over a whole turn, negative for the gradient
+  float sign;                                            // negative for the gradient
 };
+
+// What a position's angle is of a turn, within half of one.  Position, their product and one over a whole turn are sums of two float64 numbers each, and what the
+// first parts' product is of whole turns goes before anything is added to it.
+__device__ __forceinline__ float part_of_turn(int64_t position, double frequency) {
+  constexpr double TURN = 0.15915494309189533577, TURN_REST = -9.839338337591243e-18;          // 1 / 2 pi
+  const double at = (double)position;
+  const uint64_t whole = at == 9223372036854775808.0 ? uint64_t(1) << 63 : (uint64_t)(int64_t)at;
+  const double rest = (double)(int64_t)((uint64_t)position - whole);
+  const double angle = at * frequency, angle_rest = fma(at, frequency, -angle) + rest * frequency;
+  const double turns = angle * TURN, turns_rest = fma(angle, TURN, -turns) + (angle * TURN_REST + angle_rest * TURN);
+  const double left = turns - rint(turns) + turns_rest;
+  return (float)(left - rint(left));
+}
 
 // A piece as it lies in memory: 16 bytes, or one value, of each of the two places that turn together (interleaved: of the one place).
 template <typename T, int V> struct Raw { using type = uint4; };
@@ -133,10 +146,8 @@ template <typename T, int V, bool INTERLEAVED> __global__ void __launch_bounds__
         __syncthreads();
         for (int i = threadIdx.x; i < here * p.half; i += THREADS) {
           const int node = i / p.half, pair = i - node * p.half;
-          double t = (double)p.positions[first + node] * (p.frequencies[pair] * p.turns);
-          t -= rint(t);
           float s, c;
-          sincospif(2.f * (float)t, &s, &c);
+          sincospif(2.f * p.sign * part_of_turn(p.positions[first + node], p.frequencies[pair]), &s, &c);
           angles[i] = make_float2(c * p.magnitude, s * p.magnitude);
         }
         __syncthreads();
@@ -222,7 +233,7 @@ extern "C" int eqt_rotary(const eqt_rotary_args* a, void* stream) {
   p.sides = pair ? 2 : 1;
   p.positions = a->positions, p.frequencies = a->frequencies, p.n = a->n, p.comps = a->comps, p.size = a->size, p.half = a->half;
   p.magnitude = a->magnitude;
-  p.turns = (a->backward ? -1.0 : 1.0) * 0.15915494309189533577;
+  p.sign = a->backward ? -1.f : 1.f;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return a->dtype == EQT_F32 ? run<float>(p, a->interleaved != 0, s) : run<__nv_bfloat16>(p, a->interleaved != 0, s);
 }

@@ -66,7 +66,7 @@ def rotary(q: Tensor, k: Optional[Tensor], positions: Tensor, frequencies: Tenso
     ``q`` is ``(N, components, channels)`` of ``num_heads`` heads, ``k`` (or ``None``: then ``q`` alone is returned) of ``kv_heads`` (as many where not given), float32
     or bfloat16, of any strides; ``positions`` (N,), int64, any values; ``frequencies`` (pairs,), float64, see :func:`rotary_frequencies`.  The
     pairs are channels ``(j, j + pairs)`` of a head, ``interleaved`` ``(2 j, 2 j + 1)``; a head's channels behind ``2 * pairs`` stay as they are.  Turned
-    channels are multiplied by ``magnitude``.  Angles are formed in float64 and reduced to one turn there, so far positions are as exact as near ones.
+    channels are multiplied by ``magnitude``.  Angles are formed from the exact product and reduced to one turn before float32, so far positions are as exact as near ones.
 
     Differentiable any number of times in ``q`` and ``k``."""
     kv_heads = num_heads if kv_heads is None else kv_heads
