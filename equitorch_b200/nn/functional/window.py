@@ -42,7 +42,7 @@ def window_attention(q: Tensor, k: Tensor, v: Tensor, graphs: PackedGraphs, num_
     the keys of head ``h // (num_heads // kv_heads)``); float32 or bfloat16, of any strides, at most 128 values (components times channels a head) a
     head.  Inner products run over all components, as in :func:`graph_attention`, so equivariant features stay so.  ``scale``: one over the root
     of a head's values where not given.  Nodes of no graph get zeros.  What a node does not see does not reach it, not even a NaN, and chains do not
-    touch each other.
+    touch each other; next to values that are not finite a row's sums may be of another order, and its weights not rounded.
 
     Differentiable once in ``q``, ``k`` and ``v``.  Sums in float32, one order of sums, no atomics; of bfloat16 features, weights and score
     gradients are rounded to bfloat16 for the products (of small batches, to two parts for the gradients of keys and values).  Beside its inputs and result the backward pass keeps two numbers a node and head and, of
