@@ -6,7 +6,7 @@
 // window) of steps of 32 keys, cut into parts so that the chains' parts fill the SMs; a CTA takes a part and up to 16 heads of a head of keys, whose queries
 // are the rows of the warp-wide matrix instructions.  Each of its four warps takes every fourth step, with copies of its own three ahead, and has the
 // maxima, sums and weighted values of its keys; warps, and then parts, are joined by their maxima, in one order.
-// 64 chains of up to 8192 nodes, window 4096, 16 heads on 4 of 64 bfloat16 values: 52 us (4.0 TB/s) and 6 for the join; with products by the threads 87.
+// 64 chains of up to 8192 nodes, window 4096, 16 heads on 4 of 64 bfloat16 values: 56 us (3.7 TB/s) and 6 for the join; with products by the threads 87.
 #include <algorithm>
 
 #include "graph_attention.cuh"
@@ -111,10 +111,6 @@ template <typename T, int DP> __global__ void __launch_bounds__(THREADS) step_ke
       for (int n = 0; n < NT; ++n) {
         float &x = z[n][2 * r], &y = z[n][2 * r + 1];
         x = exp2_fast(x - base), y = exp2_fast(y - base);
-        if constexpr (sizeof(T) == 2) {                  // the sum is that of the weights in the product
-          const uint32_t two = pack_bf16(x, y);
-          x = __uint_as_float(two << 16), y = __uint_as_float(two & 0xffff0000u);
-        }
         add += x + y;
       }
       sum[r] = sum[r] * keep + add;
@@ -122,7 +118,7 @@ template <typename T, int DP> __global__ void __launch_bounds__(THREADS) step_ke
 #pragma unroll
       for (int n = 0; n < DP / 8; ++n) o[n][2 * r] *= keep, o[n][2 * r + 1] *= keep;
     }
-    out_mma<DP, NT>(o, z, vs, lane);
+    out_mma<DP, NT, true>(o, z, vs, lane);              // in two parts: a result has no rounding but its own (2-norm of its error 1.85e-3 | 1.64e-3; 53.2 | 55.9 us)
     __syncwarp();
     if (++place == STAGES) place = 0;
   }

@@ -1,8 +1,8 @@
 """Attention within windows whose sums are long: bfloat16 products add up in an adder that truncates, so a sum may not stay in it from end to end.
 
 Values lie between two neighbours of bfloat16, so many of any 64 in a row the upper one that the weighted mean over whole sixty-fours is at least 2^-12 above the middle and
-has to round up.  Weights have eight bits, so that products have sixteen and every addition to a long sum loses some.  Pieces of 8192 terms lose at most 512 times 2^-23
-of sums below two, 2^-13; a sum of 100,000 terms that stays in the adder loses some 2^-10."""
+has to round up.  Weights have eight bits, so that products have sixteen and every addition to a long sum loses some.  Pieces of 8192 terms are 512 additions, or 1024
+of weights in two parts, that lose at most 2^-23 of a sum that grows to two, 2^-13 together; a sum of 100,000 terms that stays in the adder loses some 2^-10."""
 import math
 
 import pytest

@@ -26,7 +26,8 @@ def test_a_long_cache():
     """bfloat16 products add up in an adder that truncates: a sum of a million keys may not stay in it.
 
     Of any 64 keys one has the weight one and the others exp(-1/4), 199 / 256 in bfloat16; values lie between two neighbours of bfloat16, so many of the 64 the upper one that
-    the mean is at least 2^-12 above the middle and has to round up.  A warp's 8192 terms lose at most 512 times 2^-23 of a sum below two, 2^-13."""
+    the mean is at least 2^-12 above the middle and has to round up.  A warp's 8192 keys, in two parts of their weights, are 1024 additions that
+    lose at most 2^-23 of a sum that grows to two, 2^-13 together."""
     chains, length, size, low, step = 1200, 2 ** 20, 8, 199 / 256, 2.0 ** -7       # more chains than the GPU has places, so that none is cut for their sake
     base = 1 + step * (torch.arange(size, device=DEV) * 11 % 127)
     count = ((step / 2 + 2.0 ** -12) / (step * low / (63 * low + 1)) + 0.0 * base).ceil()
@@ -40,3 +41,21 @@ def test_a_long_cache():
     q[:, 0, 0] = 1.0
     out = F.window_attention_step(q, spread(keys), spread(values), torch.full((chains,), length, device=DEV), 1, length, scale=0.125)
     assert (out[:, 0].double() == base.double() + step).all()
+
+
+@pytest.mark.parametrize("size", [8, 32, 64, 128])
+def test_errors_as_a_whole(size):
+    """bfloat16.  Weights go into their product in two parts, which leave 2^-17 of them, so the rounding of the result is all that is to be seen: both errors are within 2^-15
+    of the result's 2-norm of each other, where weights of one part leave half as much again."""
+    chains, length, heads = 20, 3000, 4
+    gen = torch.Generator(device=DEV).manual_seed(size)
+    q, keys, values = (torch.randn(*s, device=DEV, generator=gen).bfloat16() for s in ((chains, 1, heads * size), (chains, length, 1, 2 * size), (chains, length, 1, 2 * size)))
+    lengths = torch.randint(1, length + 1, (chains,), device=DEV, generator=gen)
+    got = F.window_attention_step(q, keys, values, lengths, heads, 400, 3, kv_heads=2).double().view(chains, heads, size)
+    for i, n in enumerate(lengths.tolist()):
+        seen = torch.arange(n, device=DEV)
+        seen = seen[(seen >= n - 401) | (seen < 3)]
+        k, v = (t[i, seen, 0].double().view(-1, 2, 1, size).expand(-1, -1, 2, -1).reshape(-1, heads, size) for t in (keys, values))
+        p = (torch.einsum("hc,jhc->hj", q[i, 0].double().view(heads, size), k) * size ** -0.5).softmax(1)
+        want = torch.einsum("hj,jhc->hc", p, v)
+        assert (got[i] - want).norm() <= (want.bfloat16().double() - want).norm() + 2.0 ** -15 * want.norm()
