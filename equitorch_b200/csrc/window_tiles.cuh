@@ -3,7 +3,7 @@
 // columns (dk, dv, over the heads that share them); every result is written by one warp and sums have one order.
 //
 // A tile walks two stretches of keys, the chain's first ones and those of its rows' windows, so its work goes by the window, not by the chain.  What a
-// tile of 64 rows sees of 64 + before + after keys it uses in full but for the two triangles at its ends.  32 chains of 30 float32 nodes: 41 us for three kernels and
+// tile of 64 rows sees of 64 + before + after keys it uses in full but for the two triangles at its ends.  32 chains of 30 float32 nodes: 48 us for three kernels and
 // the call bound by the host; bfloat16 that the 5th-generation tensor cores take (window_tc.cu) come here only unaligned, or with a scale that is not positive.
 #pragma once
 
@@ -314,6 +314,7 @@ __global__ void __launch_bounds__(THREADS, DP <= 64 ? 3 : 2) window_columns_kern
   walk.set<KT>();
   const int steps = walk.steps * p.group;                // the heads one after the other
   const bool far_apart = apart(p, lo, hi);
+  const int first_end = far_apart ? lo : lo + p.sinks;   // nodes before it are seen from behind their windows here
   auto fetch = [&](int step, int s) {
     int end;
     const int i = walk.at<KT>(step % walk.steps, end), head = here ? kv * p.group + step / walk.steps : 0;
@@ -355,7 +356,7 @@ __global__ void __launch_bounds__(THREADS, DP <= 64 ? 3 : 2) window_columns_kern
     __syncthreads();
     int end;
     const int query = walk.at<KT>(step % walk.steps, end);
-    if (work && row <= query + KT - 1 + p.after && (row + 15 >= query - p.before || row < lo + p.sinks)) {
+    if (work && row <= query + KT - 1 + p.after && (row + 15 >= query - p.before || row < first_end)) {
       const T *qs = stage + s * S::STAGE, *gs = qs + KT * LD;
       const float* num = numbers + s * 3 * KT;
       float z[NT][4], dp[NT][4];
@@ -367,7 +368,7 @@ __global__ void __launch_bounds__(THREADS, DP <= 64 ? 3 : 2) window_columns_kern
         for (int i = 0; i < 4; ++i) {
           const int c = n * 8 + 2 * t + (i & 1), q = query + c;
           const int j = row + g + 8 * (i >> 1);
-          const bool on = q < end && sees(p, q, j, lo) && (!far_apart || q <= j + p.before);
+          const bool on = q < end && j <= q + p.after && (j >= q - p.before || j < first_end);
           z[n][i] = on ? exp2_fast(z[n][i] * unit - num[c]) * num[KT + c] : 0.f;
           dp[n][i] = on ? z[n][i] * (dp[n][i] - num[2 * KT + c]) : 0.f;
         }
