@@ -17,9 +17,9 @@
 // G of a piece is at most PIECE_BYTES (or, of over a million rows, of 128 types), and pieces add to one float32 dx, which the last one rounds, so scratch does not grow with the
 // table; a piece that has a wave of WEIGHT's tiles has whole ones.  Sums that would leave SMs idle are cut into parts, float32 partial results that one kernel adds
 // in their order.  Floor: 8 n t c flops for both passes.
-// At most MOST_TERMS channels.  Bound by the tensor cores: 16,384 rows, 32,768 types, 512 bfloat16 channels 565 us of LOGITS (0.97 PFLOP/s, the exponentials
-// at the same time), four pieces of 132, 123 and 119 (1.04 to 1.15 PFLOP/s); pairs of CTAs for a tile of 256 x 256 took 532, 151, 114 and 122 (2100 | 2130 us in
-// all).  float32 5003 x 14,161 x 128: LOGITS 96, then 86, 71 and 56 twice, bound by the shared memory that six products of split operands read.
+// At most MOST_TERMS channels.  Bound by the tensor cores: 16,384 rows, 32,768 types, 512 bfloat16 channels 573 us of LOGITS (0.96 PFLOP/s, the exponentials
+// at the same time), four pieces of 124, 130 and 120 (1.06 to 1.15 PFLOP/s); pairs of CTAs for a tile of 256 x 256 took 532, 151, 114 and 122 (2100 | 2130 us in
+// all).  float32 5003 x 14,161 x 128: LOGITS 102, then 81, 74 and 57 twice, bound by the shared memory that six products of split operands read.
 //
 // A CTA per SM; warp 0 copies tiles (TMA), warp 1 issues the MMAs, the other eight (float32: sixteen) are the epilogue.  A k-block is 64
 // values of k; operands lie along k or along the rows, as they are in memory.  bfloat16: tiles of 128 x 256, four stages of 48 KB, two sums of 256 columns in tensor memory.
