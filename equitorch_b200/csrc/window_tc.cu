@@ -654,7 +654,8 @@ template <int DP, int MODE, bool FINE, bool FOLDS> __global__ void __launch_boun
         const float now = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * unit;
         const bool higher = now > base + FAR || (base == -INFINITY && now > base);
         if (__any_sync(0xffffffffu, higher)) {           // another unit: what there is so far goes by it
-          const float unit_now = base == -INFINITY ? now : base + ceilf(now - base);         // by whole steps: the rounding of a weight is the same in any unit of a row
+          // by whole steps, if float32 has the step: the rounding of a weight is the same in any unit of a row
+          const float rise = now - base, unit_now = rise < INFINITY ? base + ceilf(rise) : now;
           const float keep = !higher ? 1.f : base == -INFINITY ? 0.f : exp2_fast(base - unit_now);
           total *= keep;
           if (FOLDS) kept *= keep;

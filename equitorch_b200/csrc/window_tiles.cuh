@@ -142,7 +142,10 @@ __global__ void __launch_bounds__(THREADS, DP <= 64 ? 4 : 3) window_forward_kern
 #pragma unroll
         for (int n = 0; n < NT; ++n) most = fmaxf(most, fmaxf(z[n][2 * r], z[n][2 * r + 1]));
         most = quad_max(most);
-        if (sizeof(T) == 2 && most > top[r] && top[r] > -INFINITY) most = top[r] + ceilf(most - top[r]);         // whole steps: a weight's rounding is the same in any unit
+        if constexpr (sizeof(T) == 2) {                  // by whole steps, if float32 has the step: a weight's rounding is the same in any unit
+          const float rise = most - top[r];
+          if (rise > 0.f && rise < INFINITY) most = top[r] + ceilf(rise);
+        }
         const float base = most == -INFINITY ? 0.f : most, keep = exp2_fast(top[r] - base);
         float add = 0.f;
 #pragma unroll

@@ -33,3 +33,18 @@ def test_score_gradients_of_a_row_cancel(rise, size, sign):
     (dq,) = torch.autograd.grad(out, q, g)
     assert dq[:, :, 1].abs().max() <= math.log(2) * 2.0 ** -15
     check_status()
+
+
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("size", [16, 64, 128])
+def test_scores_far_apart(size, sign):
+    """From -2e6 to 2e6 in units of log2: the row goes by the greatest, and by those before where these are all there is."""
+    n, high = 192, 1024.0
+    q, k, v = (torch.zeros(n, 1, size, device=DEV, dtype=torch.bfloat16) for _ in range(3))
+    q[:, :, 0] = sign * high
+    k[:, 0, 0] = torch.tensor([-high, high, -high], device=DEV).repeat_interleave(64)
+    v[:, 0, 0] = torch.tensor([1.0, 2.0, 4.0], device=DEV).repeat_interleave(64)
+    graphs = PackedGraphs(torch.tensor([0, n], device=DEV), n)
+    out = F.window_attention(q, k, v, graphs, 1, n, 0, scale=sign * 1.4)
+    assert (out[:64, 0, 0] == 1).all() and (out[64:, 0, 0] == 2).all()
+    check_status()
