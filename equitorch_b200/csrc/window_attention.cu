@@ -48,7 +48,9 @@ WindowParams params(const eqt_window_attention_args& a) {
   if (a.dtype == EQT_BF16) {
     const int64_t window = std::min<int64_t>((int64_t)p.before + p.after + 1, reach);
     p.folds_rows = std::min<int64_t>(window + p.sinks, reach) > attention::FOLD;
-    p.folds_columns = p.group * (p.sinks && !p.split ? reach : window) > attention::FOLD;
+    // a first node is seen to its chain's end, or apart to the length from which chains are
+    const int64_t far = !p.sinks ? 0 : p.split ? std::min<int64_t>(p.apart, reach) : reach;
+    p.folds_columns = p.group * std::max(window, far) > attention::FOLD;
   }
   return p;
 }
